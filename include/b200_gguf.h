@@ -387,6 +387,94 @@ int b2_attention_decode_static(int device, const float* dev_q, const uint16_t* d
                                const int32_t* dev_pos, int n_head, int n_kv, int head_dim, int block_tokens,
                                int n_splits, float* dev_out, void* stream);
 
+/* ---- operators over a caller's device memory: a paged cache that the caller owns is filled, read and its logits are
+ *      scored without an engine (no counterpart in the reference, whose library owns its cache). llama_cpp/device_ops.py
+ *      calls them on tensors.
+ *
+ * All pointers inside the structs and argument lists are DEVICE pointers; the structs themselves are host memory, read
+ * during the call. Every call only enqueues work on `stream` (a cudaStream_t, NULL = default stream): nothing is
+ * allocated, nothing waits, nothing is remembered, so calls may be captured into graphs and may run at once on several
+ * streams as long as they share no memory that one of them writes (a workspace among it). The caller's current CUDA
+ * device is left as it was. Arguments are checked before anything is enqueued; what lies in device memory (page ids,
+ * lengths) is held inside the given sizes by the kernels. Tensors' last dimension is contiguous, other strides are
+ * free (in elements). */
+
+/* Rows of a ragged batch and the pages of its sequences. Rows row_start[s] .. row_start[s + 1] - 1 belong to sequence s
+ * (row_start [n_seqs + 1], ascending, row_start[0] = 0) and are the newest of its lengths[s] own tokens, the earliest of them first: row i
+ * of n is own token lengths[s] - n + i. Own token j lies in page pages[s][j / block_tokens] at offset j % block_tokens.
+ * Rows from row_start[n_seqs] on belong to nobody and are left alone. */
+typedef struct b2_ragged_pages {
+    const int32_t* row_start;
+    const int32_t* lengths;   /* [n_seqs] own tokens of each sequence, its rows among them */
+    const int32_t* pages;     /* [n_seqs][table_stride], max_pages entries of each row are used */
+    int64_t table_stride;
+    int64_t n_pages;          /* pages of the pools */
+    int32_t max_pages, n_seqs /* <= 65535 */, n_rows;
+    int32_t block_tokens;     /* tokens of a page, a multiple of 16 */
+} b2_ragged_pages;
+
+/* Append the rows' keys and values to the cache, the keys rotated by their positions; rotate the rows' queries beside
+ * them (q may be NULL). Row i's position is first_pos + its own token number. The rotation turns the entries (2i, 2i + 1)
+ * (B2_ROTATE_PAIRS) or (i, i + rot_dims / 2) (B2_ROTATE_HALVES) of the first rot_dims entries of a head by
+ * position * freqs[i], computed in 64 bits, and multiplies them by amplitude; the others stay as they are. One rounding
+ * to the cache's type. Pools [n_pages][n_kv][block_tokens][head_dim]. A row whose place is not in its table, or whose
+ * page id is outside the pool, is not stored (its query is still rotated). q_out has the cache's type; it may be q
+ * itself if q has that type. The places of a call must be different ones (no two tables may name one page that the call
+ * writes to). head_dim even, <= 1024; rot_dims even, <= 512. */
+#define B2_ROTATE_PAIRS 0
+#define B2_ROTATE_HALVES 1
+typedef struct b2_kv_append_args {
+    const void *k, *v, *q;    /* [n_rows][heads][head_dim] of in_type */
+    void *k_pool, *v_pool, *q_out;
+    const float* freqs;       /* [rot_dims / 2] */
+    int64_t k_row, k_head, v_row, v_head, q_row, q_head, q_out_row, q_out_head;    /* strides */
+    int64_t first_pos;
+    int32_t in_type;          /* B2_TYPE_F32, _F16 or _BF16 */
+    int32_t cache_type;       /* B2_TYPE_F16 or _BF16 */
+    int32_t n_head, n_kv, head_dim, rot_dims, layout;
+    float amplitude;
+} b2_kv_append_args;
+int b2_kv_append(int device, const b2_ragged_pages* where, const b2_kv_append_args* args, void* stream);
+
+/* Attention of a ragged batch whose sequences share their first n_prefix tokens: row i sees the prefix (pages
+ * prefix_pages[0 .. (n_prefix - 1) / block_tokens], the last one perhaps in part) and its sequence's own tokens up to itself.
+ * out = softmax(scale * q.k) v over them, 0 where there are none. The prefix is read once for all rows; its partial
+ * results (32 bits) go through the workspace. Queries, cache and output are all f16 or all bf16; scores, maxima and
+ * sums are 32-bit, probabilities are rounded to the cache's type for the weighted sum. max_rows: most rows any sequence
+ * has (rows past it are not computed); 1 for single tokens. Page ids are held inside the pool. head_dim 64 or 128,
+ * n_head a multiple of n_kv, at most 64 times it; pools and workspace 16-byte aligned. Lengths may be smaller than a
+ * sequence's rows (the rows ahead see the prefix alone). */
+typedef struct b2_shared_prefix_args {
+    const void* q;            /* [n_rows][n_head][head_dim] */
+    const void *k_pool, *v_pool;      /* [n_pages][n_kv][block_tokens][head_dim] */
+    const int32_t* prefix_pages;
+    void* out;                /* like q */
+    void* workspace;          /* b2_attention_shared_prefix_workspace bytes; may be NULL when n_prefix is 0 */
+    int64_t workspace_bytes;
+    int64_t q_row, q_head, out_row, out_head;
+    int32_t n_prefix, max_rows, n_head, n_kv, head_dim;
+    int32_t type;             /* B2_TYPE_F16 or _BF16 */
+    float scale;              /* > 0, usually 1 / sqrt(head_dim) */
+} b2_shared_prefix_args;
+int b2_attention_shared_prefix(int device, const b2_ragged_pages* where, const b2_shared_prefix_args* args, void* stream);
+/* bytes that a call with so many rows needs, whatever the lengths are */
+int b2_attention_shared_prefix_workspace(int n_rows, int n_head, int n_kv, int head_dim, int64_t* bytes);
+
+/* Log softmax of logits [n_rows][n_vocab] (rows row_stride elements apart; B2_TYPE_F32, _F16 or _BF16): the log
+ * probability of tokens[r] -> logprob[r], the entropy (nats) -> entropy[r] (either may be NULL), and the n_top (0..64)
+ * most likely ids with their log probabilities -> top_id, top_logprob [n_rows][n_top], most likely first, equal ones by
+ * id; -1 and -infinity past the vocabulary's end. Arithmetic in 32 bits. A token outside the vocabulary has log
+ * probability -infinity. Masked entries (-infinity) have probability 0; a row of nothing else has log probabilities
+ * -infinity and entropy 0. A row that holds a NaN or +infinity has NaN for entropy and log probabilities; NaNs are the
+ * last of the alternatives. */
+int b2_token_logprobs(int device, const void* logits, int type, int64_t row_stride, int n_rows, int n_vocab,
+                      const int32_t* tokens, float* logprob, float* entropy, int n_top, float* top_logprob,
+                      int32_t* top_id, void* stream);
+
+/* Kernels of these operators bound every wait; the code of the first wait that ran out on the device (0: none; results
+ * since then are not to be used). Waits for the device. */
+int b2_device_op_error(int device, uint32_t* code);
+
 #ifdef __cplusplus
 }
 #endif

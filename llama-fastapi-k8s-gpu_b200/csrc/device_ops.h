@@ -1,0 +1,85 @@
+// Launch interfaces of the operators over a caller's device memory (device_ops.cu checks their arguments and exports them).
+#pragma once
+#include "kernels.h"
+
+namespace b2 {
+
+enum ElemType { ELEM_F32 = 0, ELEM_F16 = 1, ELEM_BF16 = 2 };
+
+// Which rows belong to which sequence, and where a sequence's own cached tokens lie. Row r belongs to sequence s when row_start[s] <= r < row_start[s + 1]; the
+// rows of a sequence are the newest of its lengths[s] own tokens. All arrays are device memory.
+struct RaggedPages {
+    const int *row_start, *lengths;
+    const int* pages;            // [n_seqs][table_stride], the first max_pages entries of each are read
+    long table_stride;
+    int max_pages, n_seqs, n_rows;
+    int block_tokens;
+    long n_pages;                // pages of the pools: ids outside are not followed
+};
+
+// ---------------------------------------------------------------- kv_append.cu
+struct KvAppendArgs {
+    RaggedPages r;
+    const void *k, *v, *q;       // rows x heads x head_dim, last dimension contiguous; q may be null
+    long k_row, k_head, v_row, v_head, q_row, q_head, qo_row, qo_head;      // strides in elements
+    void *k_pool, *v_pool;       // [n_pages][n_kv][block_tokens][head_dim]
+    void* q_out;                 // cache type
+    const float* freqs;          // [rot_dims / 2]
+    long first_pos;
+    int n_head, n_kv, head_dim, rot_dims, halves;
+    float amplitude;
+    int in_type, cache_type;
+};
+cudaError_t kv_append_launch(const KvAppendArgs& a, cudaStream_t s);
+
+// ---------------------------------------------------------------- logprobs.cu
+constexpr int LOGPROB_MAX_TOP = 64;
+struct LogprobArgs {
+    const void* logits;          // [n_rows][n_vocab], rows row_stride elements apart
+    long row_stride;
+    const int* tokens;           // [n_rows] or null
+    float *logprob, *entropy;    // [n_rows], either may be null
+    float* top_logprob;          // [n_rows][n_top]
+    int* top_id;
+    int n_rows, n_vocab, n_top, type;
+};
+cudaError_t logprobs_launch(const LogprobArgs& a, cudaStream_t s);
+
+// ---------------------------------------------------------------- shared_prefix.cu, shared_prefix_tc.cu
+struct SharedPrefixArgs {
+    RaggedPages r;
+    const void* q;               // [n_rows][n_head][head_dim] of the cache's type (q_f32: 32-bit, rounded to it)
+    long q_row, q_head;
+    int q_f32;
+    const void *k_pool, *v_pool;
+    const int* prefix_pages;
+    int n_prefix;
+    void* out;                   // like q, cache's type
+    long out_row, out_head;
+    float* work;                 // partial results of the prefix
+    int max_rows;                // most rows of a sequence
+    int n_head, n_kv, head_dim, type;
+    float scale_log2;
+    // batched steps of the engine: the slots' own page tables and positions instead of r's arrays, one row each; out in operand order
+    const SlotDev* tab;
+    BatchIdx slots;
+    __half* out_h;
+    int out_T_pad;
+};
+size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim);
+cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s);
+
+// Prefix pass on tensor memory: the key blocks of every (KV head, 256 query rows) laid end to end and cut into equal runs, one run a CTA. A unit's
+// partial results are numbered by the CTAs that its blocks fall to.
+struct PrefixCut {
+    int units, pairs, blocks, run, ctas;      // units = n_kv * pairs; blocks of 128 keys a unit; blocks a CTA
+    __host__ __device__ int first_cta(int unit) const { return (int)((long)unit * blocks / run); }
+    __host__ __device__ int slots(int unit) const { return (int)(((long)(unit + 1) * blocks - 1) / run) - first_cta(unit) + 1; }
+};
+PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix);
+cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, cudaStream_t s);
+
+// the first wait of the device-memory operators that ran out, if any (0: none); set by the kernels, read by b2_device_op_error
+unsigned int* device_op_error(int device);
+
+}  // namespace b2

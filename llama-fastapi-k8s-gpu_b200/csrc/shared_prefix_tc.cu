@@ -1,0 +1,308 @@
+// The prefix pass of shared_prefix.cu on the 5th-generation tensor cores: many query rows of a KV head over the keys that all sequences share.
+//
+// Rows are (row of the batch, head of the KV head's group); a unit is 256 of them, two tiles of 128. A CTA takes a run of key blocks of 128 (PrefixCut), which
+// may end one unit and start the next. Keys and values come by tensor copies from their pages (64 columns a part in 128-byte-swizzled rows, two stages
+// each) and serve both tiles. Tensor memory: two score tiles (2 x 128 columns, probabilities are written over them as the A operand of the second product)
+// and two outputs. While one tile's softmax runs, the other's products do. Warps 0-3 and 4-7: softmax of a tile, a thread a row; 8: copies; 9: matrix
+// instructions.
+// The output is rescaled only where a row's maximum has grown by more than 2^8 (probabilities are then up to 2^8, sums stay 32-bit).
+#include "device_ops.h"
+#include "ptx.cuh"
+#include "tc05.cuh"
+#include "tensor_map.h"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace b2 {
+
+namespace {
+constexpr int ST_ROWS = 128, ST_K = 128, ST_PART = 128 * 128;    // rows of a tile, keys of a block; bytes of a part (128 rows x 64 columns)
+constexpr int ST_THREADS = 320;
+
+__device__ unsigned int st_error[5];                             // see mbar_give_up
+
+__device__ __forceinline__ float st_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+template <bool F16>
+__device__ __forceinline__ uint32_t st_pack(float a, float b) {
+    if constexpr (F16) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+    else { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+}
+}  // namespace
+
+unsigned int* device_op_error(int device) {
+    (void)device;                                                // (the current device's copy)
+    void* p = nullptr;
+    return cudaGetSymbolAddress(&p, st_error) == cudaSuccess ? (unsigned int*)p : nullptr;
+}
+
+template <int HD, bool F16>
+__global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                         const SharedPrefixArgs a, const PrefixCut cut, const int box_rows, const size_t ml_at) {
+    constexpr int PARTS = HD / 64;
+    extern __shared__ uint8_t st_smem[];
+    __shared__ uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+    __shared__ uint32_t tmem_at;
+    unsigned int* err = st_error;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    uint8_t* qs = reinterpret_cast<uint8_t*>(((uintptr_t)st_smem + 1023) & ~(uintptr_t)1023);      // [tile][part]
+    uint8_t* ks = qs + 2 * PARTS * ST_PART;                      // [stage][part]
+    uint8_t* vs = ks + 2 * PARTS * ST_PART;
+    if (warp == 9) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; i++) {
+                mbar_init(&q_full[i], 128); mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+                mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1);
+            }
+            fence_mbar_init();
+        }
+        __syncwarp();
+        tc_alloc(&tmem_at, 512);
+    }
+    tc_before_sync();
+    __syncthreads();
+    tc_after_sync();
+    griddep_wait();
+    griddep_launch();
+    const uint32_t s_at = tmem_at, o_at = tmem_at + 256;
+    const int G = a.n_head / a.n_kv, M = a.r.n_rows * G, n_prefix = a.n_prefix;
+    const long total = (long)cut.units * cut.blocks;
+    const long x0 = (long)blockIdx.x * cut.run, x1 = min(total, x0 + cut.run);
+
+    // runs of blocks of one unit: every role walks them the same way
+    struct Segment { int kvh, row0, b0, n; bool two; };
+    auto segment = [&](long x) {
+        Segment g;
+        const int u = (int)(x / cut.blocks);
+        g.b0 = (int)(x - (long)u * cut.blocks);
+        g.n = (int)min((long)(cut.blocks - g.b0), x1 - x);
+        g.kvh = u / cut.pairs;
+        g.row0 = u % cut.pairs * 2 * ST_ROWS;
+        g.two = M - g.row0 > ST_ROWS;
+        return g;
+    };
+
+    if (warp == 8) {
+        // ================= copies: a lane has a box of keys (one page, or a part of one)
+        const int bt = a.r.block_tokens, boxes = ST_K / box_rows;
+        int it = 0;
+        for (long x = x0; x < x1;) {
+            const Segment g = segment(x);
+            x += g.n;
+            for (int i = 0; i < g.n; i++, it++) {
+                const int j0 = (g.b0 + i) * ST_K, n_box = min(boxes, (n_prefix - j0 + box_rows - 1) / box_rows), st = it & 1;
+                int row = 0;
+                if (lane < n_box) {
+                    const int j = j0 + lane * box_rows;
+                    const int page = min(max(a.prefix_pages[j / bt], 0), (int)a.r.n_pages - 1);
+                    row = (int)(((long)page * a.n_kv + g.kvh) * bt + j % bt);
+                }
+                for (int kv = 0; kv < 2; kv++) {
+                    uint64_t *full = kv ? &v_full[st] : &k_full[st], *empty = kv ? &v_empty[st] : &k_empty[st];
+                    uint8_t* dst = (kv ? vs : ks) + st * PARTS * ST_PART + lane * box_rows * 128;
+                    if (it >= 2) mbar_wait_warp(empty, ((it >> 1) - 1) & 1, err, 0x90001u, (unsigned)it);
+                    if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)(n_box * box_rows * 128 * PARTS));
+                    __syncwarp();
+                    if (lane < n_box)
+                        for (int c = 0; c < PARTS; c++) tma_load_3d(dst + c * ST_PART, kv ? &map_v : &map_k, c * 64, row, 0, full);
+                    __syncwarp();
+                }
+            }
+        }
+    } else if (warp == 9) {
+        // ================= matrix instructions (all lanes run the loop, one issues)
+        const bool one = elect_one();
+        const uint32_t f16 = F16 ? ~((1u << 7) | (1u << 10)) : ~0u;      // (tc_idesc_bf16 without the bits that say bf16)
+        const uint32_t id_s = tc_idesc_bf16(ST_ROWS, ST_K) & f16, id_o = tc_idesc_bf16(ST_ROWS, HD, true) & f16;
+        const uint32_t qa = smem_u32(qs), ka = smem_u32(ks), va = smem_u32(vs);
+        int it = 0, segs[2] = {0, 0}, done[2] = {0, 0};          // blocks of the CTA, segments and blocks of each tile so far
+        for (long x = x0; x < x1;) {
+            const Segment g = segment(x);
+            x += g.n;
+            const int tiles = g.two ? 2 : 1;
+            auto scores = [&](int t, int at) {
+                if (!one) return;
+                const uint64_t dq = tc_desc(qa + t * PARTS * ST_PART), dk = tc_desc(ka + (at & 1) * PARTS * ST_PART);
+#pragma unroll
+                for (int c = 0; c < PARTS; c++)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) tc_mma(s_at + t * ST_K, dq + c * (ST_PART >> 4) + 2 * k, dk + c * (ST_PART >> 4) + 2 * k, id_s, (c | k) ? 1u : 0u);
+                tc_commit(&s_full[t]);
+            };
+            mbar_wait_warp(&k_full[it & 1], (it >> 1) & 1, err, 0x90002u, (unsigned)it);
+            for (int t = 0; t < tiles; t++) {
+                mbar_wait_warp(&q_full[t], segs[t]++ & 1, err, 0x90003u, (unsigned)it);
+                tc_after_sync();
+                scores(t, it);
+            }
+            if (one) tc_commit(&k_empty[it & 1]);
+            for (int i = 0; i < g.n; i++) {
+                const int at = it + i;
+                mbar_wait_warp(&v_full[at & 1], (at >> 1) & 1, err, 0x90004u, (unsigned)at);
+                const int valid = min(ST_K, n_prefix - (g.b0 + i) * ST_K), steps = (valid + 15) / 16;
+                if (valid & 15) {
+                    // keys past the prefix up to the next 16: whatever the page holds must not meet the zero weights as values
+                    const int n_bad = 16 - (valid & 15);
+                    for (int e = lane; e < PARTS * n_bad * 8; e += 32)
+                        *reinterpret_cast<uint4*>(vs + ((at & 1) * PARTS + e / (n_bad * 8)) * ST_PART + (valid + e / 8 % n_bad) * 128 + (e & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();
+                    __syncwarp();
+                }
+                const uint64_t dv = tc_desc(va + (at & 1) * PARTS * ST_PART, ST_PART);
+                for (int t = 0; t < tiles; t++) {
+                    mbar_wait_warp(&p_full[t], done[t] & 1, err, 0x90005u, (unsigned)at);
+                    done[t]++;
+                    tc_after_sync();
+                    if (one) {
+                        for (int k = 0; k < steps; k++) tc_mma_ts(o_at + t * HD, s_at + t * ST_K + k * 8, dv + k * (2048 >> 4), id_o, (i | k) ? 1u : 0u);
+                        tc_commit(&pv_done[t]);
+                        if (t == tiles - 1) tc_commit(&v_empty[at & 1]);
+                    }
+                    if (i + 1 < g.n) {
+                        // the next scores replace the probabilities that this product reads
+                        mbar_wait_warp(&pv_done[t], (done[t] - 1) & 1, err, 0x90009u, (unsigned)at);
+                        if (t == 0) { mbar_wait_warp(&k_full[(at + 1) & 1], ((at + 1) >> 1) & 1, err, 0x90002u, (unsigned)at); }
+                        tc_after_sync();
+                        scores(t, at + 1);
+                        if (one && t == tiles - 1) tc_commit(&k_empty[(at + 1) & 1]);
+                    }
+                }
+            }
+            it += g.n;
+        }
+    } else {
+        // ================= softmax: a thread a row of its tile
+        const int t = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_mine = s_at + t * ST_K + lanes, o_mine = o_at + t * HD + lanes;
+        uint32_t done = 0;                                       // blocks of this tile so far
+        for (long x = x0; x < x1;) {
+            const Segment g = segment(x);
+            const int unit = (int)(x / cut.blocks);
+            x += g.n;
+            if (t == 1 && !g.two) continue;
+            // ---- this row's query, into 128-byte-swizzled rows (rows past the end: zeros)
+            const int f = g.row0 + t * ST_ROWS + row;
+            const bool in = f < M;
+            const int r = in ? f / G : 0, head = g.kvh * G + (in ? f % G : 0);
+            const size_t q_at = (size_t)r * a.q_row + (size_t)head * a.q_head;
+#pragma unroll
+            for (int c8 = 0; c8 < HD / 8; c8++) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (in) {
+                    if (a.q_f32) {
+                        const float* q = (const float*)a.q + q_at + c8 * 8;
+                        v = make_uint4(st_pack<F16>(q[0], q[1]), st_pack<F16>(q[2], q[3]), st_pack<F16>(q[4], q[5]), st_pack<F16>(q[6], q[7]));
+                    } else {
+                        const uint16_t* q = (const uint16_t*)a.q + q_at + c8 * 8;
+                        if (((uintptr_t)q & 15) == 0) v = *reinterpret_cast<const uint4*>(q);
+                        else v = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+                    }
+                }
+                *reinterpret_cast<uint4*>(qs + (t * PARTS + (c8 >> 3)) * ST_PART + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) = v;
+            }
+            fence_proxy_async();
+            mbar_arrive(&q_full[t]);
+            float m_ref = -INFINITY;
+            uint64_t l2 = f2_pack(0.f, 0.f), l3 = l2;            // sums of even and odd entries, twice
+            const uint64_t scale2 = f2_pack(a.scale_log2, a.scale_log2);
+            for (int i = 0; i < g.n; i++, done++) {
+                mbar_wait(&s_full[t], done & 1, err, 0x90006u, done);
+                tc_after_sync();
+                __syncwarp();
+                uint32_t raw[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tc_ld32(s_mine + c * 32, raw[c]);
+                tc_wait_ld();
+                const int valid = n_prefix - (g.b0 + i) * ST_K;
+                if (valid < ST_K) {
+#pragma unroll
+                    for (int j = 0; j < ST_K; j++) if (j >= valid) raw[j >> 5][j & 31] = 0xff800000u;
+                }
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int j = 0; j < ST_K; j++) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(raw[j >> 5][j & 31]));
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
+                const bool grow = mx > m_ref + 8.f || (m_ref == -INFINITY && mx > -INFINITY);
+                float fall = 1.f;
+                if (grow) {
+                    fall = st_exp2(m_ref - mx);                  // (0 the first time)
+                    m_ref = mx;
+                    const uint64_t fall2 = f2_pack(fall, fall);
+                    l2 = f2_mul(l2, fall2); l3 = f2_mul(l3, fall2);
+                }
+                const float ref = m_ref > -INFINITY ? -m_ref : 0.f;
+                const uint64_t ref2 = f2_pack(ref, ref);
+                uint32_t p[2][32];
+#pragma unroll
+                for (int j = 0; j < ST_K; j += 2) {
+                    const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[j >> 5][j & 31]), __uint_as_float(raw[j >> 5][(j & 31) + 1])), scale2, ref2));
+                    const float e0 = st_exp2(d.x), e1 = st_exp2(d.y);
+                    if (j & 2) l3 = f2_add(l3, f2_pack(e0, e1)); else l2 = f2_add(l2, f2_pack(e0, e1));
+                    p[j >> 6][(j & 63) >> 1] = st_pack<F16>(e0, e1);
+                }
+                if (i > 0 && __any_sync(0xffffffffu, grow)) {    // the products so far must be in before they are rescaled
+                    mbar_wait(&pv_done[t], (done - 1) & 1, err, 0x90007u, done);
+                    tc_after_sync();
+                    __syncwarp();
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t o[32];
+                        tc_ld32(o_mine + c, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fall);
+                        tc_st32(o_mine + c, o);
+                    }
+                }
+                __syncwarp();
+                tc_st32(s_mine, p[0]);
+                tc_st32(s_mine + 32, p[1]);
+                tc_wait_st();
+                tc_before_sync();
+                mbar_arrive(&p_full[t]);
+            }
+            // ---- this segment's results of the row
+            mbar_wait(&pv_done[t], (done - 1) & 1, err, 0x90008u, done);
+            tc_after_sync();
+            __syncwarp();
+            const int slot = blockIdx.x - cut.first_cta(unit);
+            const size_t at = ((size_t)slot * a.r.n_rows + r) * a.n_head + head;
+#pragma unroll
+            for (int c = 0; c < HD; c += 32) {
+                uint32_t o[32];
+                __syncwarp();
+                tc_ld32(o_mine + c, o);
+                tc_wait_ld();
+                if (!in) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(a.work + at * HD + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+            const float2 la = f2_unpack(l2), lb = f2_unpack(l3);
+            if (in) *reinterpret_cast<float2*>(a.work + ml_at + at * 2) = make_float2(m_ref, (la.x + la.y) + (lb.x + lb.y));
+            tc_before_sync();
+        }
+    }
+    __syncthreads();
+    if (warp == 9) tc_dealloc(tmem_at, 512);
+}
+
+// ---------------------------------------------------------------- host side
+template <int HD, bool F16>
+static cudaError_t st_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, cudaStream_t s) {
+    constexpr int parts = HD / 64, smem = 6 * parts * ST_PART + 1024;
+    if (!allow_smem<shared_prefix_tc_kernel<HD, F16>>(smem)) return cudaErrorInvalidValue;
+    int box = ST_K;
+    while (a.r.block_tokens % box) box /= 2;
+    const long rows = a.r.n_pages * a.n_kv * a.r.block_tokens;
+    CUtensorMap mk, mv;                                          // (copies move 16-bit entries whatever their format)
+    if (!bf16_rows_map(&mk, a.k_pool, HD, rows, HD, 1, 0, box) || !bf16_rows_map(&mv, a.v_pool, HD, rows, HD, 1, 0, box)) return cudaErrorInvalidValue;
+    return launch_chain(shared_prefix_tc_kernel<HD, F16>, dim3(cut.ctas), dim3(ST_THREADS), smem, s, mk, mv, a, cut, box, ml_at);
+}
+
+cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, cudaStream_t s) {
+    const size_t ml_at = shared_prefix_work_floats(a.r.n_rows, a.n_head, a.n_kv, a.head_dim) / (a.head_dim + 2) * a.head_dim;
+    if (a.r.block_tokens % 16 || cut.ctas < 1) return cudaErrorInvalidValue;
+    if (a.head_dim == 64) return a.type == ELEM_F16 ? st_launch<64, true>(a, cut, ml_at, s) : st_launch<64, false>(a, cut, ml_at, s);
+    if (a.head_dim == 128) return a.type == ELEM_F16 ? st_launch<128, true>(a, cut, ml_at, s) : st_launch<128, false>(a, cut, ml_at, s);
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace b2

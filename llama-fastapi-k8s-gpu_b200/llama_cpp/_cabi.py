@@ -26,6 +26,7 @@ B2_ATTN_CONV, B2_ATTN_FULL_NORM, B2_ATTN_UNIT_SINK, B2_ATTN_OUT_BIAS = 128, 256,
 B2_ROUTE_SOFTMAX_ALL, B2_ROUTE_TOPK_SOFTMAX, B2_ROUTE_SIGMOID, B2_ROUTE_TABLE = 0, 1, 2, 3
 B2_BLOCK_POSTSUM_LN, B2_BLOCK_PRENORM_RMS, B2_BLOCK_OUTNORM_RMS, B2_BLOCK_HYPER_RMS, B2_BLOCK_PARALLEL_LN, B2_BLOCK_PARALLEL_ONE_LN = 0, 1, 2, 3, 4, 5
 B2_STEP_MAX_ENTRIES = 64
+B2_ROTATE_PAIRS, B2_ROTATE_HALVES = 0, 1
 
 
 class B2Config(ctypes.Structure):
@@ -62,6 +63,24 @@ class B2Sampling(ctypes.Structure):
     _fields_ = [("temperature", c_float), ("top_p", c_float), ("min_p", c_float), ("repeat_penalty", c_float),
                 ("frequency_penalty", c_float), ("presence_penalty", c_float), ("top_k", c_int32),
                 ("penalty_last_n", c_int32)]
+
+
+class B2RaggedPages(ctypes.Structure):
+    """b2_ragged_pages: rows of a ragged batch and the pages of its sequences."""
+    _fields_ = [(n, c_void_p) for n in ("row_start", "lengths", "pages")] + [(n, c_int64) for n in ("table_stride", "n_pages")] + [
+        (n, c_int32) for n in ("max_pages", "n_seqs", "n_rows", "block_tokens")]
+
+
+class B2KvAppend(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("k", "v", "q", "k_pool", "v_pool", "q_out", "freqs")] + [
+        (n, c_int64) for n in ("k_row", "k_head", "v_row", "v_head", "q_row", "q_head", "q_out_row", "q_out_head", "first_pos")] + [
+        (n, c_int32) for n in ("in_type", "cache_type", "n_head", "n_kv", "head_dim", "rot_dims", "layout")] + [("amplitude", c_float)]
+
+
+class B2SharedPrefix(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "k_pool", "v_pool", "prefix_pages", "out", "workspace")] + [
+        (n, c_int64) for n in ("workspace_bytes", "q_row", "q_head", "out_row", "out_head")] + [
+        (n, c_int32) for n in ("n_prefix", "max_rows", "n_head", "n_kv", "head_dim", "type")] + [("scale", c_float)]
 
 
 # name -> (restype, argtypes); every symbol include/b200_gguf.h declares
@@ -111,6 +130,11 @@ SIGNATURES = {
     "b2_op_attention_decode": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p]),
     "b2_attention_decode_static": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_int, c_int, c_int,
                                            c_int, c_int, c_void_p, c_void_p]),
+    "b2_kv_append": (c_int, [c_int, c_void_p, c_void_p, c_void_p]),          # b2_ragged_pages, b2_kv_append_args: structures or their bytes
+    "b2_attention_shared_prefix": (c_int, [c_int, c_void_p, c_void_p, c_void_p]),
+    "b2_attention_shared_prefix_workspace": (c_int, [c_int] * 4 + [POINTER(c_int64)]),
+    "b2_token_logprobs": (c_int, [c_int, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "b2_device_op_error": (c_int, [c_int, POINTER(ctypes.c_uint32)]),
     "b2_op_sample": (c_int, [c_int, c_void_p, c_int, POINTER(B2Sampling), c_void_p, c_int, c_double, POINTER(c_int32)]),
 }
 
