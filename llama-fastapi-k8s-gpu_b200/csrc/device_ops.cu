@@ -140,7 +140,5 @@ extern "C" int b2_device_op_error(int device, uint32_t* code) {
     if (!code) return bad("b2_device_op_error", "null result");
     OnDevice on(device);
     if (on.status != cudaSuccess) return done("b2_device_op_error", on.status);
-    unsigned int* word = device_op_error(device);
-    if (!word) return b2_fail(B2_ERR_CUDA, "b2_device_op_error: no such device variable");
-    return done("b2_device_op_error", cudaMemcpy(code, word, 4, cudaMemcpyDeviceToHost));
+    return done("b2_device_op_error", shared_prefix_error(code));
 }

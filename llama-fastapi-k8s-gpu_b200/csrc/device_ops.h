@@ -73,13 +73,15 @@ cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s);
 // partial results are numbered by the CTAs that its blocks fall to.
 struct PrefixCut {
     int units, pairs, blocks, run, ctas;      // units = n_kv * pairs; blocks of 128 keys a unit; blocks a CTA
-    __host__ __device__ int first_cta(int unit) const { return (int)((long)unit * blocks / run); }
-    __host__ __device__ int slots(int unit) const { return (int)(((long)(unit + 1) * blocks - 1) / run) - first_cta(unit) + 1; }
+    // (units * blocks fits 31 bits: shared_prefix_launch refuses more)
+    __host__ __device__ int first_cta(int unit) const { return (int)((unsigned)(unit * blocks) / (unsigned)run); }
+    __host__ __device__ int slots(int unit) const { return (int)((unsigned)((unit + 1) * blocks - 1) / (unsigned)run) - first_cta(unit) + 1; }
 };
 PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix);
 cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, cudaStream_t s);
 
-// the first wait of the device-memory operators that ran out, if any (0: none); set by the kernels, read by b2_device_op_error
-unsigned int* device_op_error(int device);
+// code of the first wait of these kernels that ran out on the current device (0: none); waits for the device
+cudaError_t shared_prefix_error(unsigned int* code);
+cudaError_t shared_prefix_tc_error(unsigned int* code);
 
 }  // namespace b2

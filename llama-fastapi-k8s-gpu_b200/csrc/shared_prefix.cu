@@ -4,23 +4,27 @@
 // The prefix is read once for all rows: its pass leaves (m, sum, weighted sum) of every row in 32 bits, the pass over the sequences' own tokens joins them.
 //
 // The prefix pass is shared_prefix_tc.cu (tensor memory) or, where the rows of a KV head fill no more than one tile of 64, the kernel here over the same
-// rows; the own pass is the kernel here. Here: mma.sync m16n8k16, tiles of 64 keys by cp.async in rows padded by 16 bytes, three buffers. A row of the
+// rows; the own pass is the kernel here. Here: mma.sync m16n8k16, tiles of 64 keys by tensor copies (a warp of its own) in 128-byte-swizzled rows. A row of the
 // tile is (token, head of the KV head's group). MT 16: a CTA's four warps take 16 keys of a tile each and are merged at the end, which is the form for single
 // tokens, bound by the cache's bytes; MT 64: a warp has 16 rows and all keys. The keys of a tile of rows are split over a cluster of up to eight CTAs, which
 // join through each other's shared memory.
 // Probabilities are rounded to the cache's type for the weighted sum (the other operand is the cache as it is); scores, maxima, sums, joins stay 32-bit.
 #include "device_ops.h"
 #include "ptx.cuh"
+#include "tensor_map.h"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <limits.h>
 #include <math.h>
 
 namespace b2 {
 
 namespace {
-constexpr int SP_THREADS = 128;
+constexpr int SP_WARPS = 4, SP_THREADS = 32 * (SP_WARPS + 1);
 constexpr int SP_TT = 64;            // keys of a tile
-constexpr int SP_STAGES = 3;
+constexpr int sp_stages(int hd) { return hd == 64 ? 4 : 2; }             // tiles under way: 64 KB, three CTAs an SM
+
+__device__ unsigned int sp_error[5];                             // see mbar_give_up
 
 __device__ __forceinline__ float sp_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
@@ -49,11 +53,6 @@ __device__ __forceinline__ void sp_ldmatrix_x4(uint32_t (&r)[4], const void* p) 
 __device__ __forceinline__ void sp_ldmatrix_x4_trans(uint32_t (&r)[4], const void* p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem_u32(p)));
 }
-__device__ __forceinline__ void sp_cp16(void* dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void sp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void sp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ uint32_t sp_cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ float sp_cluster_load(uint32_t address) {
     float v;
@@ -62,323 +61,604 @@ __device__ __forceinline__ float sp_cluster_load(uint32_t address) {
 }
 }  // namespace
 
-enum SpRole { SP_PREFIX = 0, SP_OWN = 1, SP_JOINED = 2 };      // the prefix for all rows; own tokens of a sequence; both, one after the other
 struct SpPlan {
-    int role, splits;            // CTAs that share the keys of a tile (a cluster, except for SP_PREFIX)
-    int fixed_slots;             // SP_OWN: partial results of the prefix per row (0: none; < 0: as `cut` says)
+    int prefix;                  // 1: the prefix for all rows, partial results; 0: a sequence's own tokens, behind the prefix's results
+    int splits;                  // CTAs that share the keys of a tile of rows (a cluster, except for the prefix)
+    int steal;                   // single-token form without splits: a CTA goes on with the work of CTAs that have not started
+    int fixed_slots;             // partial results of the prefix per row (0: none; < 0: as `cut` says)
+    int box_rows;                // keys of a copy: a page, or a power of two that divides it
     PrefixCut cut;
+    size_t ml_at;                // where the (maximum, sum) of the partial results lie in the workspace
 };
 
 // partial results of the prefix: [slot][row][head][head_dim] weighted sums, then [slot][row][head][2] (maximum in log2, sum)
 __device__ __forceinline__ size_t sp_part(const SharedPrefixArgs& a, int slot, int row, int head) { return ((size_t)slot * a.r.n_rows + row) * a.n_head + head; }
 
-// grid: (tile * splits + split, KV head, sequence)
-template <typename E, int HD, int MT>
-__global__ void __launch_bounds__(SP_THREADS) shared_prefix_rows_kernel(const SharedPrefixArgs a, const SpPlan p, const size_t ml_at) {
-    constexpr int LD = HD + 8;                                   // padded row (entries)
-    constexpr int KS = MT == 16 ? 1 : 4;                         // 16-key steps of a tile that a warp takes
-    using T = SpType<E>;
-    extern __shared__ __align__(16) uint8_t sp_smem[];
-    uint16_t* ks = reinterpret_cast<uint16_t*>(sp_smem);         // [SP_STAGES][SP_TT][LD]
-    uint16_t* vs = ks + SP_STAGES * SP_TT * LD;
-    __shared__ float row_m[MT], row_l[MT];
-    // behind another kernel of the engine's chain: what it wrote (q, this step's keys). Behind the prefix pass that is long done, and only the joining waits.
-    if (p.role != SP_OWN || p.fixed_slots == 0) griddep_wait();
-    griddep_launch();
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, tq = lane & 3;
-    const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, kvh = blockIdx.y, z = blockIdx.z;
-    const int G = a.n_head / a.n_kv, bt = a.r.block_tokens;
-
-    // ---- the rows and keys of this tile
-    int r0 = 0, n_tok = a.r.n_rows, own = 0;
-    const int* table = nullptr;
-    const int lead = p.role == SP_OWN ? 0 : a.n_prefix;
-    if (p.role != SP_PREFIX) {
-        if (a.tab) {
-            const SlotDev sd = a.tab[a.slots.slot[z]];
-            r0 = z; n_tok = 1; own = sd.ints[1] + 1 - a.n_prefix; table = sd.block_table + a.n_prefix / bt;
-        } else {
-            const int b = a.r.row_start[z], e = a.r.row_start[z + 1];
-            r0 = max(0, b); n_tok = min(e, a.r.n_rows) - r0;
-            own = a.r.lengths[z]; table = a.r.pages + z * a.r.table_stride;
-        }
-    }
-    const int f0 = tile * MT, n_f = min(MT, n_tok * G - f0);     // rows (token, head) of the tile, numbered within the sequence
-    if (n_f <= 0) { griddep_wait(); return; }                    // (all CTAs of the cluster)
-    const int cap = a.r.max_pages * bt;
+// the rows and keys that a CTA works on
+struct SpWork {
+    int r0, n_tok, own;          // first row of the sequence, its rows, its own tokens (prefix pass: 0, all rows, the prefix's tokens)
+    const int* table;
+    int f0, n_f;                 // rows (token, head) of the tile, numbered within the sequence
+    int G, lim_lo, lim_hi, q0, q1, n_tiles;      // keys that the tile's first and last rows see; this CTA's share of them; its tiles of keys
+    bool own_pass;
     // keys that token i of the sequence sees
-    auto limit = [&](int i) { return p.role == SP_PREFIX ? lead : lead + max(0, min(own - n_tok + i + 1, cap)); };
-    const int lim_lo = limit(f0 / G), lim_hi = limit((f0 + n_f - 1) / G);
-    const int chunk = ((lim_hi + p.splits - 1) / p.splits + 15) & ~15;
-    const int q0 = min(lim_hi, split * chunk), q1 = min(lim_hi, q0 + chunk);
-    const int n_tiles = (q1 - q0 + SP_TT - 1) / SP_TT;
+    __device__ int limit(int i) const { return own_pass ? max(0, own - n_tok + i + 1) : own; }
+    __device__ SpWork() {}
+    __device__ SpWork(const SharedPrefixArgs& a, const SpPlan& p, int mt, int tile, int split, int z) {
+        const int bt = a.r.block_tokens;
+        G = a.n_head / a.n_kv; own_pass = !p.prefix;
+        r0 = 0; n_tok = a.r.n_rows; own = a.n_prefix; table = a.prefix_pages;
+        if (own_pass) {
+            if (a.tab) {
+                const SlotDev sd = a.tab[a.slots.slot[z]];
+                r0 = z; n_tok = 1; own = sd.ints[1] + 1 - a.n_prefix; table = sd.block_table + a.n_prefix / bt;
+            } else {
+                const int b = a.r.row_start[z], e = a.r.row_start[z + 1];
+                own = a.r.lengths[z];
+                r0 = max(0, b); n_tok = min(e, a.r.n_rows) - r0; table = a.r.pages + z * a.r.table_stride;
+            }
+            own = min(own, a.r.max_pages * bt);
+        }
+        f0 = tile * mt; n_f = min(mt, n_tok * G - f0);
+        lim_lo = limit(f0 / G); lim_hi = limit((f0 + max(n_f, 1) - 1) / G);
+        const int chunk = ((lim_hi + p.splits - 1) / p.splits + SP_TT - 1) / SP_TT * SP_TT;
+        q0 = min(lim_hi, split * chunk); q1 = min(lim_hi, q0 + chunk);
+        n_tiles = (q1 - q0 + SP_TT - 1) / SP_TT;
+    }
+};
 
-    // ---- q fragments: rows g and g + 8 of this warp's 16
-    const int w_row = MT == 16 ? 0 : 16 * warp;
-    uint32_t qa[HD / 16][4];
-    int lim[2];
+// The copying warp: the tiles of keys and values of one KV head, numbers it .. it + n_tiles - 1 of the CTA. A lane has a box of keys; page ids of 32 boxes are
+// read at once.
+template <int HD, int STAGES>
+__device__ __forceinline__ void sp_copy(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, const CUtensorMap* map_k, const CUtensorMap* map_v, int kvh, int it,
+                                        uint8_t* tiles_at, uint64_t* full, uint64_t* empty, int lane) {
+    constexpr int PARTS = HD / 64, PART = SP_TT * 128;
+    const int boxes = SP_TT / p.box_rows, ahead = 32 / boxes, bt = a.r.block_tokens;
+    int ids = 0;
+    for (int ti = 0; ti < w.n_tiles; ti++, it++) {
+        const int st = it % STAGES, t0 = w.q0 + ti * SP_TT, n_box = min(boxes, (w.q1 - t0 + p.box_rows - 1) / p.box_rows), j = t0 + lane * p.box_rows;
+        if (ti % ahead == 0) ids = j < w.q1 ? w.table[j / bt] : 0;
+        const int id = __shfl_sync(0xffffffffu, ids, ti % ahead * boxes + lane % boxes);
+        const int row = (int)(((long)min(max(id, 0), (int)a.r.n_pages - 1) * a.n_kv + kvh) * bt + j % bt);
+        if (it >= STAGES) mbar_wait_warp(&empty[st], (it / STAGES - 1) & 1, sp_error, 0xa0001u, (unsigned)it);
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(n_box * p.box_rows * 128 * PARTS * 2));
+        __syncwarp();
+        if (lane < n_box)
+            for (int c = 0; c < PARTS; c++) {
+                uint8_t* dst = tiles_at + (st * 2 * PARTS + c) * PART + lane * p.box_rows * 128;
+                tma_load_3d(dst, map_k, c * 64, row, 0, &full[st]);
+                tma_load_3d(dst + PARTS * PART, map_v, c * 64, row, 0, &full[st]);
+            }
+        __syncwarp();
+    }
+}
+
+// Take over the work of a CTA of this grid that has not started: asked for by one thread, the answer (16 bytes) arrives on a barrier. After a refusal nothing more may be
+// asked.
+__device__ __forceinline__ void sp_ask_work(void* answer, uint64_t* bar) {
+    mbar_arrive_expect_tx(bar, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(smem_u32(answer)), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool sp_answered_work(const uint64_t* answer, int& x, int& y, int& z) {
+    uint32_t got, i, j, k;
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tmov.b128 r, {%4, %5};\n\tclusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\t"
+                 "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, r;\n\t}"
+                 : "=&r"(got), "=&r"(i), "=&r"(j), "=&r"(k) : "l"(answer[0]), "l"(answer[1]) : "memory");
+    x = (int)i; y = (int)j; z = (int)k;
+    return got != 0;
+}
+
+// q fragments of rows f and f + 8 (numbered within the sequence; `in`: they belong to the tile)
+template <typename E, int HD>
+__device__ __forceinline__ void sp_load_q(const SharedPrefixArgs& a, const SpWork& w, int kvh, int row, int tq, uint32_t (&qa)[HD / 16][4]) {
+    using T = SpType<E>;
+    const bool words = !a.q_f32 && (((uintptr_t)a.q | (a.q_row * 2) | (a.q_head * 2)) & 3) == 0;
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-        const int f = f0 + w_row + g + 8 * h;
-        const bool in = w_row + g + 8 * h < n_f;
-        const int i = in ? f / G : 0, head = kvh * G + (in ? f % G : 0);
-        lim[h] = in ? limit(i) : lim_hi;
-        const size_t at = (size_t)(r0 + i) * a.q_row + (size_t)head * a.q_head;
+        const bool in = row + 8 * h < w.n_f;
+        const int f = w.f0 + row + 8 * h, i = in ? f / w.G : 0, head = kvh * w.G + (in ? f - i * w.G : 0);
+        const size_t at = (size_t)(w.r0 + i) * a.q_row + (size_t)head * a.q_head + 2 * tq;
 #pragma unroll
         for (int kk = 0; kk < HD / 16; kk++)
 #pragma unroll
             for (int part = 0; part < 2; part++) {
                 uint32_t v = 0;
-                const size_t d = at + kk * 16 + part * 8 + 2 * tq;
+                const size_t d = at + kk * 16 + part * 8;
                 if (in) {
-                    if (a.q_f32) { const float* q = (const float*)a.q + d; v = T::pack(__ldcg(q), __ldcg(q + 1)); }
+                    if (words) v = __ldcg(reinterpret_cast<const uint32_t*>((const uint16_t*)a.q + d));
+                    else if (a.q_f32) { const float* q = (const float*)a.q + d; v = T::pack(__ldcg(q), __ldcg(q + 1)); }
                     else { const uint16_t* q = (const uint16_t*)a.q + d; v = (uint32_t)__ldcg(q) | (uint32_t)__ldcg(q + 1) << 16; }
                 }
                 qa[kk][2 * part + h] = v;
             }
     }
-    float o[HD / 8][4];
-#pragma unroll
-    for (int i = 0; i < HD / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};          // (l: this thread's columns)
+}
 
-    // all threads: tile ti -> buffer ti % SP_STAGES. A thread copies one 16-byte piece of every eighth (sixteenth) row.
-    constexpr int CPR = HD / 8, RPP = SP_THREADS / CPR;
-    const int c8 = tid % CPR * 8;
-    auto issue = [&](int ti) {
-        const int st = ti % SP_STAGES, t0 = q0 + ti * SP_TT;
-        uint16_t *kd = ks + st * SP_TT * LD + c8, *vd = vs + st * SP_TT * LD + c8;
-        if (ti < n_tiles) {
-            int page[SP_TT / RPP], off[SP_TT / RPP];
+// The prefix's partial results of a row, joined: maximum, sum, and the columns col, col + 1, col + 8, ... of the weighted sum
+template <int HD, int N>
+__device__ __forceinline__ void sp_take_prefix(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, int kvh, int row, int col, float& m, float& l, float (&o)[N][4], int h) {
+    const int f = w.f0 + row, i = f / w.G;
+    const int slots = p.fixed_slots < 0 ? p.cut.slots(kvh * p.cut.pairs + (w.r0 * w.G + f) / 256) : p.fixed_slots;
+    const size_t at = sp_part(a, 0, w.r0 + i, kvh * w.G + f - i * w.G), step = (size_t)a.r.n_rows * a.n_head;
+    const float* ml = a.work + p.ml_at + at * 2;
+    const float* from = a.work + at * HD + col;
+    constexpr int B = N > 8 ? 1 : 4;                             // results under way
+    for (int j0 = 0; j0 < slots; j0 += B) {
+        float2 one[B], v[B][N];
+        float m2 = m;
 #pragma unroll
-            for (int m = 0; m < SP_TT / RPP; m++) {
-                int j = min(t0 + tid / CPR + m * RPP, q1 - 1);
-                const int* from = j < lead ? a.prefix_pages : table;
-                if (j >= lead) j -= lead;
-                off[m] = j % bt;
-                page[m] = min(max(from[j / bt], 0), (int)a.r.n_pages - 1);
-            }
+        for (int j = 0; j < B; j++) {
+            one[j] = make_float2(-INFINITY, 0.f);
+            if (j0 + j < slots) {
+                one[j] = __ldcg(reinterpret_cast<const float2*>(ml + (j0 + j) * step * 2));
 #pragma unroll
-            for (int m = 0; m < SP_TT / RPP; m++) {
-                const int j = tid / CPR + m * RPP;
-                if (t0 + j < q1) {
-                    const size_t at = (((size_t)page[m] * a.n_kv + kvh) * bt + off[m]) * HD + c8;
-                    sp_cp16(kd + j * LD, (const uint16_t*)a.k_pool + at);
-                    sp_cp16(vd + j * LD, (const uint16_t*)a.v_pool + at);
-                } else {                                         // 0 * garbage must stay 0 in the weighted sum
-                    *reinterpret_cast<uint4*>(kd + j * LD) = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(vd + j * LD) = make_uint4(0, 0, 0, 0);
-                }
+                for (int nt = 0; nt < N; nt++) v[j][nt] = __ldcg(reinterpret_cast<const float2*>(from + (j0 + j) * step * HD + nt * 8));
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < N; nt++) v[j][nt] = make_float2(0.f, 0.f);
             }
         }
-        sp_commit();
-    };
-    for (int i = 0; i < SP_STAGES - 1; i++) issue(i);
-    for (int ti = 0; ti < n_tiles; ti++) {
-        sp_wait<SP_STAGES - 2>();
-        __syncthreads();                                         // tile ti is here for every warp, and every warp is done with the one before
-        issue(ti + SP_STAGES - 1);
-        const int st = ti % SP_STAGES, t0 = q0 + ti * SP_TT, k0 = MT == 16 ? 16 * warp : 0;      // this warp's first key of the tile
-        if (t0 + k0 >= q1) continue;
-        float sc[2 * KS][4];
 #pragma unroll
-        for (int nt = 0; nt < 2 * KS; nt++) {
-            sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-            const uint16_t* kr = ks + (st * SP_TT + k0 + nt * 8 + (lane & 7)) * LD + (lane >> 3) * 8;
+        for (int j = 0; j < B; j++) m2 = fmaxf(m2, one[j].x);
+        const float ref = m2 == -INFINITY ? 0.f : m2, fall = sp_exp2(m - ref);
+        m = m2; l *= fall;
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; kk += 2) {
-                uint32_t b4[4];                                  // dims kk * 16 .. + 31 of eight keys
-                sp_ldmatrix_x4(b4, kr + kk * 16);
-                T::mma(sc[nt], qa[kk], b4[0], b4[1]);
-                T::mma(sc[nt], qa[kk + 1], b4[2], b4[3]);
-            }
-        }
-        // ---- scale, mask, running maxima of rows g and g + 8; this thread's columns are 2 tq, 2 tq + 1 of every eight keys
-        float mx[2] = {m_run[0], m_run[1]};
+        for (int nt = 0; nt < N; nt++) { o[nt][2 * h] *= fall; o[nt][2 * h + 1] *= fall; }
 #pragma unroll
-        for (int nt = 0; nt < 2 * KS; nt++)
+        for (int j = 0; j < B; j++) {
+            const float c = sp_exp2(one[j].x - ref);
+            l = fmaf(c, one[j].y, l);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int key = t0 + k0 + nt * 8 + 2 * tq + (e & 1);
-                sc[nt][e] = key < min(lim[e >> 1], q1) ? sc[nt][e] * a.scale_log2 : -INFINITY;
-                mx[e >> 1] = fmaxf(mx[e >> 1], sc[nt][e]);
-            }
-        float ref[2], fall[2];
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            ref[h] = mx[h] == -INFINITY ? 0.f : mx[h];           // nothing seen yet: every weight is 0
-            fall[h] = sp_exp2(m_run[h] - ref[h]);
-            m_run[h] = mx[h];
-            l_run[h] *= fall[h];
-        }
-#pragma unroll
-        for (int nt = 0; nt < 2 * KS; nt++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) { sc[nt][e] = sp_exp2(sc[nt][e] - ref[e >> 1]); l_run[e >> 1] += sc[nt][e]; }
-#pragma unroll
-        for (int nt = 0; nt < HD / 8; nt++) { o[nt][0] *= fall[0]; o[nt][1] *= fall[0]; o[nt][2] *= fall[1]; o[nt][3] *= fall[1]; }
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const uint32_t pa[4] = {T::pack(sc[2 * s][0], sc[2 * s][1]), T::pack(sc[2 * s][2], sc[2 * s][3]),
-                                    T::pack(sc[2 * s + 1][0], sc[2 * s + 1][1]), T::pack(sc[2 * s + 1][2], sc[2 * s + 1][3])};
-            const uint16_t* vb = vs + (st * SP_TT + k0 + 16 * s) * LD;
-            // keys that only later rows of the tile see: a value there that is no number must not reach the earlier rows through a weight of 0
-            if (t0 + k0 + 16 * s + 16 > lim_lo && lim_lo < lim_hi) {
-                uint32_t bad = 0;
-                for (int e = lane; e < 16 * (HD / 2); e += 32) {
-                    const uint32_t v = *reinterpret_cast<const uint32_t*>(vb + e / (HD / 2) * LD + e % (HD / 2) * 2);
-                    bad |= (v & T::EXP) == T::EXP || (v >> 16 & T::EXP) == T::EXP;
-                }
-                if (__any_sync(0xffffffffu, bad)) {
-                    for (int k = 0; k < 16; k++) {
-                        const int from = (lane & ~3) | (k & 7) >> 1;
-                        float w[2];
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            float mine = 0.f;
-#pragma unroll
-                            for (int e = 0; e < 4; e++) if (e == (k >> 3) * 2 + (k & 1)) mine = sc[2 * s + (e >> 1)][2 * h + (e & 1)];
-                            w[h] = __shfl_sync(0xffffffffu, mine, from);
-                        }
-#pragma unroll
-                        for (int nt = 0; nt < HD / 8; nt++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++)
-                                if (w[e >> 1] != 0.f) o[nt][e] = fmaf(w[e >> 1], T::value(vb[k * LD + nt * 8 + 2 * tq + (e & 1)]), o[nt][e]);
-                    }
-                    continue;
-                }
-            }
-#pragma unroll
-            for (int nt = 0; nt < HD / 8; nt += 2) {
-                uint32_t b4[4];                                  // 16 keys x 16 dims, transposed on load
-                sp_ldmatrix_x4_trans(b4, vb + (lane & 15) * LD + nt * 8 + (lane >> 4) * 8);
-                T::mma(o[nt], pa, b4[0], b4[1]);
-                T::mma(o[nt + 1], pa, b4[2], b4[3]);
-            }
+            for (int nt = 0; nt < N; nt++) { o[nt][2 * h] = fmaf(c, v[j][nt].x, o[nt][2 * h]); o[nt][2 * h + 1] = fmaf(c, v[j][nt].y, o[nt][2 * h + 1]); }
         }
     }
-    sp_wait<0>();
-    __syncthreads();                                             // everyone is done with the buffers
+}
 
-    // ---- this CTA's (maximum, sum, weighted sum) of every row: merged over the warps (MT 16) or as they are (MT 64)
-    float* acc = reinterpret_cast<float*>(sp_smem);              // [MT][HD]
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
-        l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
+// two neighbouring columns of a row's output
+template <typename E, int HD>
+__device__ __forceinline__ void sp_store_out(const SharedPrefixArgs& a, int t, int head, int d, float x, float y) {
+    const uint32_t v = SpType<E>::pack(x, y);
+    if (a.out_h) {
+        const int col = head * HD + d;
+        *reinterpret_cast<uint32_t*>(a.out_h + ((size_t)(col >> 3) * a.out_T_pad + t) * 8 + (col & 7)) = v;
+    } else {
+        uint16_t* dst = (uint16_t*)a.out + (size_t)t * a.out_row + (size_t)head * a.out_head + d;
+        if (((uintptr_t)dst & 3) == 0) *reinterpret_cast<uint32_t*>(dst) = v;
+        else { dst[0] = (uint16_t)v; dst[1] = (uint16_t)(v >> 16); }
     }
-    if (MT == 16) {
-        float* wo = acc + MT * HD;                               // [4][16][HD]
-        float* wm = wo + 4 * MT * HD;                            // [4][16]
-        float* wl = wm + 4 * MT;
+}
+
+// What a thread's columns of a row (numbers col, col + 1, col + 8, ...) come to: partial results (prefix pass), this CTA's share of a cluster's, or output
+template <typename E, int HD, int N>
+__device__ __forceinline__ void sp_finish(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, int kvh, int split, int row, int col, float m, float l, const float (&o)[N][4], int h,
+                                          float* acc, float* row_m, float* row_l) {
+    const int f = w.f0 + row, i = f / w.G, head = kvh * w.G + f - i * w.G;
+    if (!w.own_pass) {
+        const size_t at = sp_part(a, split, w.r0 + i, head);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+        for (int nt = 0; nt < N; nt++) *reinterpret_cast<float2*>(a.work + at * HD + col + nt * 8) = make_float2(o[nt][2 * h], o[nt][2 * h + 1]);
+        if (col == 0) *reinterpret_cast<float2*>(a.work + p.ml_at + at * 2) = make_float2(m, l);
+    } else if (p.splits > 1) {
 #pragma unroll
-            for (int nt = 0; nt < HD / 8; nt++)
-                *reinterpret_cast<float2*>(wo + (warp * MT + g + 8 * h) * HD + nt * 8 + 2 * tq) = make_float2(o[nt][2 * h], o[nt][2 * h + 1]);
-            if (tq == 0) { wm[warp * MT + g + 8 * h] = m_run[h]; wl[warp * MT + g + 8 * h] = l_run[h]; }
+        for (int nt = 0; nt < N; nt++) *reinterpret_cast<float2*>(acc + row * HD + col + nt * 8) = make_float2(o[nt][2 * h], o[nt][2 * h + 1]);
+        if (col == 0) { row_m[row] = m; row_l[row] = l; }
+    } else {
+        const float inv = l == 0.f ? 0.f : 1.f / l;              // (0: no keys. A NaN stays one.)
+#pragma unroll
+        for (int nt = 0; nt < N; nt++) sp_store_out<E, HD>(a, w.r0 + i, head, col + nt * 8, o[nt][2 * h] * inv, o[nt][2 * h + 1] * inv);
+    }
+}
+
+// the cluster's CTAs joined; every CTA writes its share of the tile
+template <typename E, int HD>
+__device__ __forceinline__ void sp_join_cluster(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, int kvh, const float* acc, const float* row_m, const float* row_l) {
+    cluster_sync();
+    for (int e = sp_cluster_rank() * SP_THREADS + threadIdx.x; e < w.n_f * (HD / 4); e += p.splits * SP_THREADS) {
+        const int row = e / (HD / 4), d = e % (HD / 4) * 4, f = w.f0 + row, i = f / w.G, head = kvh * w.G + f - i * w.G;
+        float m = -INFINITY, l = 0.f;
+        for (int c = 0; c < p.splits; c++) m = fmaxf(m, sp_cluster_load(cluster_address(smem_u32(row_m + row), c)));
+        const float ref = m == -INFINITY ? 0.f : m;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < p.splits; c++) {
+            const float c1 = sp_exp2(sp_cluster_load(cluster_address(smem_u32(row_m + row), c)) - ref);
+            const float4 v = cluster_load4(cluster_address(smem_u32(acc + row * HD + d), c));
+            l = fmaf(c1, sp_cluster_load(cluster_address(smem_u32(row_l + row), c)), l);
+            sum.x = fmaf(c1, v.x, sum.x); sum.y = fmaf(c1, v.y, sum.y); sum.z = fmaf(c1, v.z, sum.z); sum.w = fmaf(c1, v.w, sum.w);
         }
-        __syncthreads();
-        for (int e = tid; e < n_f * (HD / 4); e += SP_THREADS) {
-            const int row = e / (HD / 4), d = e % (HD / 4) * 4;
-            float m = -INFINITY, l = 0.f;
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        sp_store_out<E, HD>(a, w.r0 + i, head, d, sum.x * inv, sum.y * inv);
+        sp_store_out<E, HD>(a, w.r0 + i, head, d + 2, sum.z * inv, sum.w * inv);
+    }
+    cluster_sync();                                              // (the others may still read this one's results)
+}
+
+// 16 bytes at (key, eight dims) of a tile's keys or values in 128-byte-swizzled rows
+__device__ __forceinline__ uint8_t* sp_piece(uint8_t* base, int key, int c8) { return base + (c8 >> 3) * (SP_TT * 128) + key * 128 + (((c8 ^ key) & 7) << 4); }
+
+// Does a value of 16 keys from `ks` on, dims 8 c0 .. 8 (c0 + n) - 1, have all exponent bits set (infinity or NaN)?
+template <typename E>
+__device__ __forceinline__ bool sp_any_bad(uint8_t* vb, int ks, int c0, int n, int lane) {
+    uint32_t bad = 0;
+    for (int e = lane; e < 16 * n; e += 32) {
+        const uint4 v4 = *reinterpret_cast<const uint4*>(sp_piece(vb, ks + e / n, c0 + e % n));
+        const uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
 #pragma unroll
-            for (int w = 0; w < 4; w++) m = fmaxf(m, wm[w * MT + row]);
-            const float ref = m == -INFINITY ? 0.f : m;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float f = sp_exp2(wm[w * MT + row] - ref);
-                const float4 v = *reinterpret_cast<const float4*>(wo + (w * MT + row) * HD + d);
-                sum.x += f * v.x; sum.y += f * v.y; sum.z += f * v.z; sum.w += f * v.w;
-                l += f * wl[w * MT + row];
+        for (int w = 0; w < 4; w++) bad |= (v[w] & SpType<E>::EXP) == SpType<E>::EXP || (v[w] >> 16 & SpType<E>::EXP) == SpType<E>::EXP;
+    }
+    return __any_sync(0xffffffffu, bad);
+}
+
+// Single tokens: a tile of up to 16 rows (the group's heads, a few tokens), the four computing warps share a tile of keys. Scores: a warp has 16 keys; maxima and
+// probabilities go through shared memory; weighted sums: a warp has a quarter of the dims and all 64 keys, so that nothing has to be merged at the end.
+// What a CTA waits for before its first keys are here takes as long as the keys of some 100 tokens (3 us): CTAs that run go on with the work of those that have not
+// started (p.steal), and their copies run ahead into it.
+// grid: (tile * splits + split, KV head, sequence)
+template <typename E, int HD>
+__global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedPrefixArgs a,
+                                                                           const SpPlan p) {
+    constexpr int PARTS = HD / 64, PART = SP_TT * 128, STAGES = sp_stages(HD), NT = HD / 32;
+    using T = SpType<E>;
+    extern __shared__ uint8_t sp_raw[];
+    __shared__ uint64_t full[STAGES], empty[STAGES], next_full[2], next_empty[2], answered;
+    __shared__ alignas(16) uint64_t answer[2];
+    __shared__ SpWork next[2];                                   // the work after the first, n_f < 0: no more
+    __shared__ int next_kvh[2];
+    __shared__ float wmax[2][SP_WARPS][16], wsum[2][SP_WARPS][16], row_m[16], row_l[16];
+    __shared__ alignas(16) uint16_t prob[2][16][SP_TT + 8];
+    uint8_t* tiles_at = reinterpret_cast<uint8_t*>(((uintptr_t)sp_raw + 1023) & ~(uintptr_t)1023);      // [stage][keys, values][part]
+    float* acc = reinterpret_cast<float*>(tiles_at);             // [16][HD], behind the last tile of a CTA that shares its keys
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, tq = lane & 3;
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], SP_WARPS); }
+        for (int i = 0; i < 2; i++) { mbar_init(&next_full[i], 1); mbar_init(&next_empty[i], SP_WARPS); }
+        mbar_init(&answered, 1);
+        fence_mbar_init();
+    }
+    // behind another kernel of the engine's chain: what it wrote (q, this step's keys). Behind the prefix pass that is long done.
+    if (p.prefix || p.fixed_slots == 0) griddep_wait();
+    griddep_launch();
+    const int split = blockIdx.x % p.splits;
+    int kvh = blockIdx.y;
+    SpWork w(a, p, 16, blockIdx.x / p.splits, split, blockIdx.z);
+    if (w.n_f <= 0) { griddep_wait(); return; }                  // (all CTAs of the cluster, none of which ends before the prefix pass)
+    __syncthreads();
+
+    if (warp == SP_WARPS) {
+        SpWork v = w;
+        int v_kvh = kvh;
+        for (int it = 0, n = 0, asked = 0;;) {
+            if (p.steal && lane == 0) sp_ask_work(answer, &answered);
+            sp_copy<HD, STAGES>(a, p, v, &map_k, &map_v, v_kvh, it, tiles_at, full, empty, lane);
+            it += v.n_tiles;
+            bool more = false;
+            while (p.steal) {                                    // (work without rows is passed over)
+                int x, y, z;
+                mbar_wait_warp(&answered, asked++ & 1, sp_error, 0xa0004u, (unsigned)n);
+                more = sp_answered_work(answer, x, y, z) && x == 0 && y < (int)gridDim.y && z < (int)gridDim.z;      // (a wait that ran out leaves anything)
+                if (!more) break;
+                v = SpWork(a, p, 16, x, 0, z);
+                v_kvh = y;
+                if (v.n_f > 0) break;
+                __syncwarp();
+                if (lane == 0) { fence_proxy_async(); sp_ask_work(answer, &answered); }
             }
-            *reinterpret_cast<float4*>(acc + row * HD + d) = sum;
-            if (d == 0) { row_m[row] = m; row_l[row] = l; }
+            if (n >= 2) mbar_wait_warp(&next_empty[n & 1], ((n >> 1) - 1) & 1, sp_error, 0xa0005u, (unsigned)n);
+            __syncwarp();
+            if (lane == 0) {
+                if (!more) v.n_f = -1;
+                next[n & 1] = v; next_kvh[n & 1] = v_kvh;
+                mbar_arrive(&next_full[n & 1]);
+                fence_proxy_async();                             // (the answer has been read, the next may replace it)
+            }
+            n++;
+            if (!more) break;
         }
     } else {
+        const int k0 = 16 * warp, c0 = warp * (HD / 32), col = warp * (HD / 4) + 2 * tq;
+        for (int hh = 0, it = 0;; hh++) {
+            if (hh > 0) {
+                const int i = (hh - 1) & 1;
+                mbar_wait(&next_full[i], ((hh - 1) >> 1) & 1, sp_error, 0xa0006u, (unsigned)hh);
+                if (next[i].n_f < 0) break;
+                w = next[i]; kvh = next_kvh[i];
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&next_empty[i]);
+            }
+            int lim[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) lim[h] = g + 8 * h < w.n_f ? min(w.q1, w.limit((w.f0 + g + 8 * h) / w.G)) : w.q1;
+            uint32_t qa[HD / 16][4];
+            sp_load_q<E, HD>(a, w, kvh, g, tq, qa);
+            float o[NT][4], m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};      // (l: this thread's columns of scores)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
+            if (w.own_pass && p.fixed_slots != 0) {
+                if (hh == 0) griddep_wait();
+                if (split == 0) {                                // (the first CTA of a cluster takes the prefix's results)
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (g + 8 * h < w.n_f) {
+                            sp_take_prefix<HD, NT>(a, p, w, kvh, g + 8 * h, col, m_run[h], l_run[h], o, h);
+                            if (warp || tq) l_run[h] = 0.f;      // (counted once)
+                        }
+                }
+            }
+            for (int ti = 0; ti < w.n_tiles; ti++, it++) {
+                const int st = it % STAGES, buf = it & 1, t0 = w.q0 + ti * SP_TT, valid = min(SP_TT, w.q1 - t0);
+                uint8_t *kb = tiles_at + st * 2 * PARTS * PART, *vb = kb + PARTS * PART;
+                mbar_wait(&full[st], (it / STAGES) & 1, sp_error, 0xa0002u, (unsigned)it);
+                __syncwarp();
+                // ---- scores of this warp's keys, scaled, masked, and their maxima in rows g and g + 8; this thread's columns are 2 tq, 2 tq + 1 of every eight keys
+                float sc[2][4], mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int nt = 0; nt < 2; nt++) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+                if (k0 < valid) {
+#pragma unroll
+                    for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+                        for (int kk = 0; kk < HD / 16; kk += 2) {
+                            uint32_t b4[4];                      // dims kk * 16 .. + 31 of eight keys
+                            sp_ldmatrix_x4(b4, sp_piece(kb, k0 + nt * 8 + (lane & 7), kk * 2 + (lane >> 3)));
+                            T::mma(sc[nt], qa[kk], b4[0], b4[1]);
+                            T::mma(sc[nt], qa[kk + 1], b4[2], b4[3]);
+                        }
+                }
+#pragma unroll
+                for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int key = t0 + k0 + nt * 8 + 2 * tq + (e & 1);
+                        sc[nt][e] = key < lim[e >> 1] ? sc[nt][e] * a.scale_log2 : -INFINITY;
+                        mx[e >> 1] = fmaxf(mx[e >> 1], sc[nt][e]);
+                    }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                    if (tq == 0) wmax[buf][warp][g + 8 * h] = mx[h];
+                }
+                named_bar_sync(1, SP_WARPS * 32);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float m = m_run[h];
+#pragma unroll
+                    for (int i = 0; i < SP_WARPS; i++) m = fmaxf(m, wmax[buf][i][g + 8 * h]);
+                    const float ref = m == -INFINITY ? 0.f : m, fall = sp_exp2(m_run[h] - ref);      // (nothing seen yet: every weight is 0)
+                    m_run[h] = m;
+                    l_run[h] *= fall;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) { o[nt][2 * h] *= fall; o[nt][2 * h + 1] *= fall; }
+#pragma unroll
+                    for (int nt = 0; nt < 2; nt++) {
+                        const float e0 = sp_exp2(sc[nt][2 * h] - ref), e1 = sp_exp2(sc[nt][2 * h + 1] - ref);
+                        l_run[h] += e0 + e1;
+                        *reinterpret_cast<uint32_t*>(&prob[buf][g + 8 * h][k0 + nt * 8 + 2 * tq]) = T::pack(e0, e1);
+                    }
+                }
+                if (valid & 15) {
+                    // values past the last key up to the next 16: 0 * garbage must stay 0 in the weighted sum (every warp clears its dims)
+                    const int n_bad = 16 - (valid & 15);
+                    for (int e = lane; e < n_bad * NT; e += 32) *reinterpret_cast<uint4*>(sp_piece(vb, valid + e / NT, c0 + e % NT)) = make_uint4(0, 0, 0, 0);
+                    fence_proxy_async();                         // (later copies may replace them)
+                    __syncwarp();
+                }
+                named_bar_sync(1, SP_WARPS * 32);
+#pragma unroll
+                for (int s = 0; s < SP_TT / 16; s++) {
+                    if (16 * s >= valid) break;
+                    // keys that only later rows of the tile see: a value there that is no number must not reach the earlier rows through a weight of 0
+                    if (w.lim_lo < w.lim_hi && t0 + 16 * s + 16 > w.lim_lo && sp_any_bad<E>(vb, 16 * s, c0, NT, lane)) {
+#pragma unroll 1
+                        for (int k = 16 * s; k < 16 * s + 16; k++)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                const uint32_t v = *reinterpret_cast<const uint32_t*>(sp_piece(vb, k, c0 + nt) + 4 * tq);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const float weight = T::value(prob[buf][g + 8 * (e >> 1)][k]);
+                                    if (weight != 0.f) o[nt][e] = fmaf(weight, T::value((uint16_t)(e & 1 ? v >> 16 : v)), o[nt][e]);
+                                }
+                            }
+                        continue;
+                    }
+                    uint32_t pa[4];
+                    sp_ldmatrix_x4(pa, &prob[buf][lane & 15][16 * s + (lane >> 4) * 8]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt += 2) {
+                        uint32_t b4[4];                          // 16 keys x 16 dims, transposed on load
+                        sp_ldmatrix_x4_trans(b4, sp_piece(vb, 16 * s + (lane & 15), c0 + nt + (lane >> 4)));
+                        T::mma(o[nt], pa, b4[0], b4[1]);
+                        T::mma(o[nt + 1], pa, b4[2], b4[3]);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[st]);
+            }
+            // ---- sums over the warps' keys
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
+                l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
+                if (tq == 0) wsum[hh & 1][warp][g + 8 * h] = l_run[h];
+            }
+            named_bar_sync(1, SP_WARPS * 32);                    // (and everyone is done with the tiles of this head)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int row = g + 8 * h;
+                if (row >= w.n_f) continue;
+                const float l = (wsum[hh & 1][0][row] + wsum[hh & 1][1][row]) + (wsum[hh & 1][2][row] + wsum[hh & 1][3][row]);
+                sp_finish<E, HD, NT>(a, p, w, kvh, split, row, col, m_run[h], l, o, h, acc, row_m, row_l);
+            }
+        }
+    }
+    if (w.own_pass && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
+}
+
+// Several tokens of a sequence, or the prefix pass of up to 64 rows: a tile of 64 rows, a warp has 16 of them and all keys.
+// grid: (tile * splits + split, KV head, sequence)
+template <typename E, int HD>
+__global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedPrefixArgs a,
+                                                                           const SpPlan p) {
+    constexpr int PARTS = HD / 64, PART = SP_TT * 128, STAGES = sp_stages(HD), MT = 64, KS = SP_TT / 16, NT = HD / 8;
+    using T = SpType<E>;
+    extern __shared__ uint8_t sp_raw[];
+    __shared__ uint64_t full[STAGES], empty[STAGES];
+    __shared__ float row_m[MT], row_l[MT];
+    uint8_t* tiles_at = reinterpret_cast<uint8_t*>(((uintptr_t)sp_raw + 1023) & ~(uintptr_t)1023);      // [stage][keys, values][part]
+    float* acc = reinterpret_cast<float*>(tiles_at);             // [MT][HD], behind the last tile of a CTA that shares its keys
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, tq = lane & 3;
+    if (tid == 0) {
+        for (int i = 0; i < STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], SP_WARPS); }
+        fence_mbar_init();
+    }
+    if (p.prefix || p.fixed_slots == 0) griddep_wait();
+    griddep_launch();
+    const int split = blockIdx.x % p.splits, kvh = blockIdx.y;
+    const SpWork w(a, p, MT, blockIdx.x / p.splits, split, blockIdx.z);
+    if (w.n_f <= 0) { griddep_wait(); return; }
+    __syncthreads();
+
+    if (warp == SP_WARPS) {
+        sp_copy<HD, STAGES>(a, p, w, &map_k, &map_v, kvh, 0, tiles_at, full, empty, lane);
+    } else {
+        const int row0 = 16 * warp + g;
+        const bool idle = 16 * warp >= w.n_f;                    // this warp has no rows
+        uint32_t qa[HD / 16][4];
+        sp_load_q<E, HD>(a, w, kvh, row0, tq, qa);
+        float o[NT][4], m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};          // (l: this thread's columns of scores)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
+        int lim[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int row = w_row + g + 8 * h;
+            const bool in = row0 + 8 * h < w.n_f;
+            lim[h] = in ? min(w.q1, w.limit((w.f0 + row0 + 8 * h) / w.G)) : w.q1;
+        }
+        if (w.own_pass && p.fixed_slots != 0) {
+            griddep_wait();
+            if (split == 0) {
 #pragma unroll
-            for (int nt = 0; nt < HD / 8; nt++) *reinterpret_cast<float2*>(acc + row * HD + nt * 8 + 2 * tq) = make_float2(o[nt][2 * h], o[nt][2 * h + 1]);
-            if (tq == 0) { row_m[row] = m_run[h]; row_l[row] = l_run[h]; }
+                for (int h = 0; h < 2; h++)
+                    if (row0 + 8 * h < w.n_f) {
+                        sp_take_prefix<HD, NT>(a, p, w, kvh, row0 + 8 * h, 2 * tq, m_run[h], l_run[h], o, h);
+                        if (tq) l_run[h] = 0.f;                  // (counted once)
+                    }
+            }
+        }
+        for (int ti = 0; ti < w.n_tiles; ti++) {
+            const int st = ti % STAGES, t0 = w.q0 + ti * SP_TT, valid = min(SP_TT, w.q1 - t0);
+            uint8_t *kb = tiles_at + st * 2 * PARTS * PART, *vb = kb + PARTS * PART;
+            mbar_wait(&full[st], (ti / STAGES) & 1, sp_error, 0xa0003u, (unsigned)ti);
+            __syncwarp();
+            if (!idle) {
+                if (valid & 15) {                                // (every warp clears what it reads)
+                    const int n_bad = 16 - (valid & 15);
+                    for (int e = lane; e < n_bad * (HD / 8); e += 32) *reinterpret_cast<uint4*>(sp_piece(vb, valid + e / (HD / 8), e % (HD / 8))) = make_uint4(0, 0, 0, 0);
+                    __syncwarp();
+                }
+                float sc[2 * KS][4], mx[2] = {m_run[0], m_run[1]}, ref[2];
+#pragma unroll
+                for (int nt = 0; nt < 2 * KS; nt++) {
+                    sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; kk += 2) {
+                        uint32_t b4[4];
+                        sp_ldmatrix_x4(b4, sp_piece(kb, nt * 8 + (lane & 7), kk * 2 + (lane >> 3)));
+                        T::mma(sc[nt], qa[kk], b4[0], b4[1]);
+                        T::mma(sc[nt], qa[kk + 1], b4[2], b4[3]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < 2 * KS; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int key = t0 + nt * 8 + 2 * tq + (e & 1);
+                        sc[nt][e] = key < lim[e >> 1] ? sc[nt][e] * a.scale_log2 : -INFINITY;
+                        mx[e >> 1] = fmaxf(mx[e >> 1], sc[nt][e]);
+                    }
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                    mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                    ref[h] = mx[h] == -INFINITY ? 0.f : mx[h];
+                    const float fall = sp_exp2(m_run[h] - ref[h]);
+                    m_run[h] = mx[h];
+                    l_run[h] *= fall;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) { o[nt][2 * h] *= fall; o[nt][2 * h + 1] *= fall; }
+                }
+#pragma unroll
+                for (int nt = 0; nt < 2 * KS; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) { sc[nt][e] = sp_exp2(sc[nt][e] - ref[e >> 1]); l_run[e >> 1] += sc[nt][e]; }
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    if (16 * s >= valid) break;
+                    if (w.lim_lo < w.lim_hi && t0 + 16 * s + 16 > w.lim_lo && sp_any_bad<E>(vb, 16 * s, 0, HD / 8, lane)) {
+#pragma unroll 1
+                        for (int k = 0; k < 16; k++) {
+                            const int from = (lane & ~3) | (k & 7) >> 1;
+                            float weight[2];
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                float mine = 0.f;
+#pragma unroll
+                                for (int e = 0; e < 4; e++) if (e == (k >> 3) * 2 + (k & 1)) mine = sc[2 * s + (e >> 1)][2 * h + (e & 1)];
+                                weight[h] = __shfl_sync(0xffffffffu, mine, from);
+                            }
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                const uint32_t v = *reinterpret_cast<const uint32_t*>(sp_piece(vb, 16 * s + k, nt) + 4 * tq);
+#pragma unroll
+                                for (int e = 0; e < 4; e++)
+                                    if (weight[e >> 1] != 0.f) o[nt][e] = fmaf(weight[e >> 1], T::value((uint16_t)(e & 1 ? v >> 16 : v)), o[nt][e]);
+                            }
+                        }
+                        continue;
+                    }
+                    const uint32_t pa[4] = {T::pack(sc[2 * s][0], sc[2 * s][1]), T::pack(sc[2 * s][2], sc[2 * s][3]),
+                                            T::pack(sc[2 * s + 1][0], sc[2 * s + 1][1]), T::pack(sc[2 * s + 1][2], sc[2 * s + 1][3])};
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt += 2) {
+                        uint32_t b4[4];
+                        sp_ldmatrix_x4_trans(b4, sp_piece(vb, 16 * s + (lane & 15), nt + (lane >> 4)));
+                        T::mma(o[nt], pa, b4[0], b4[1]);
+                        T::mma(o[nt + 1], pa, b4[2], b4[3]);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
+        }
+        named_bar_sync(1, SP_WARPS * 32);                        // everyone is done with the tiles
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
+            l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
+            if (row0 + 8 * h < w.n_f) sp_finish<E, HD, NT>(a, p, w, kvh, split, row0 + 8 * h, 2 * tq, m_run[h], l_run[h], o, h, acc, row_m, row_l);
         }
     }
-    __syncthreads();
-    float* ml = a.work + ml_at;
-    if (p.role == SP_PREFIX) {
-        for (int e = tid; e < n_f * (HD / 4); e += SP_THREADS) {
-            const int f = f0 + e / (HD / 4), d = e % (HD / 4) * 4;
-            const size_t at = sp_part(a, split, f / G, kvh * G + f % G);
-            *reinterpret_cast<float4*>(a.work + at * HD + d) = *reinterpret_cast<const float4*>(acc + (f - f0) * HD + d);
-            if (d == 0) *reinterpret_cast<float2*>(ml + at * 2) = make_float2(row_m[f - f0], row_l[f - f0]);
-        }
-        return;
-    }
-    // ---- join the cluster's CTAs and the prefix; this CTA writes its share of the tile
-    if (p.splits > 1) cluster_sync();
-    griddep_wait();                                              // the prefix's partial results are there
-    const uint32_t rank = p.splits > 1 ? sp_cluster_rank() : 0;
-    const int n_pieces = n_f * (HD / 4);
-    for (int e = rank * SP_THREADS + tid; e < n_pieces; e += p.splits * SP_THREADS) {
-        const int row = e / (HD / 4), d = e % (HD / 4) * 4, f = f0 + row, t = r0 + f / G, head = kvh * G + f % G;
-        int slots = p.fixed_slots;
-        if (slots < 0) slots = p.cut.slots(kvh * p.cut.pairs + (t * G + f % G) / 256);
-        float m = -INFINITY, l = 0.f;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        auto add = [&](float m1, float l1, const float4& v) {
-            const float m2 = fmaxf(m, m1), ref = m2 == -INFINITY ? 0.f : m2, c0 = sp_exp2(m - ref), c1 = sp_exp2(m1 - ref);
-            l = c0 * l + c1 * l1;
-            sum.x = c0 * sum.x + c1 * v.x; sum.y = c0 * sum.y + c1 * v.y; sum.z = c0 * sum.z + c1 * v.z; sum.w = c0 * sum.w + c1 * v.w;
-            m = m2;
-        };
-#pragma unroll 4
-        for (int i = 0; i < slots; i++) {
-            const size_t at = sp_part(a, i, t, head);
-            const float2 one = __ldcg(reinterpret_cast<const float2*>(ml + at * 2));
-            add(one.x, one.y, __ldcg(reinterpret_cast<const float4*>(a.work + at * HD + d)));
-        }
-        if (p.splits > 1) {
-#pragma unroll 2
-            for (int c = 0; c < p.splits; c++)
-                add(sp_cluster_load(cluster_address(smem_u32(row_m + row), c)), sp_cluster_load(cluster_address(smem_u32(row_l + row), c)),
-                    cluster_load4(cluster_address(smem_u32(acc + row * HD + d), c)));
-        } else {
-            add(row_m[row], row_l[row], *reinterpret_cast<const float4*>(acc + row * HD + d));
-        }
-        const float inv = l == 0.f ? 0.f : 1.f / l;              // (0: no keys. A NaN stays one.)
-        sum.x *= inv; sum.y *= inv; sum.z *= inv; sum.w *= inv;
-        const uint32_t lo = T::pack(sum.x, sum.y), hi = T::pack(sum.z, sum.w);
-        if (a.out_h) {
-            const int col = head * HD + d;
-            *reinterpret_cast<uint2*>(a.out_h + ((size_t)(col >> 3) * a.out_T_pad + t) * 8 + (col & 7)) = make_uint2(lo, hi);
-        } else {
-            uint16_t* dst = (uint16_t*)a.out + (size_t)t * a.out_row + (size_t)head * a.out_head + d;
-            if (((uintptr_t)dst & 7) == 0) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-            else { dst[0] = (uint16_t)lo; dst[1] = (uint16_t)(lo >> 16); dst[2] = (uint16_t)hi; dst[3] = (uint16_t)(hi >> 16); }
-        }
-    }
-    if (p.splits > 1) cluster_sync();                            // (the others may still read this one's results)
+    if (w.own_pass && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
 }
 
 // ---------------------------------------------------------------- host side
 namespace {
 constexpr int SP_SMS = 148;
-constexpr size_t sp_smem(int hd) { return (size_t)SP_STAGES * 2 * SP_TT * (hd + 8) * 2; }
+constexpr size_t sp_smem(int hd) { return (size_t)sp_stages(hd) * 2 * SP_TT * hd * 2 + 1024; }
 
-template <typename E, int HD, int MT>
-cudaError_t sp_rows(const SharedPrefixArgs& a, const SpPlan& p, size_t ml_at, dim3 grid, cudaStream_t s, bool pdl) {
-    const auto kernel = shared_prefix_rows_kernel<E, HD, MT>;
-    if (!allow_smem<shared_prefix_rows_kernel<E, HD, MT>>((int)sp_smem(HD))) return cudaErrorInvalidValue;
+template <typename E, int HD>
+cudaError_t sp_rows(const SharedPrefixArgs& a, SpPlan p, bool single, dim3 grid, cudaStream_t s, bool pdl) {
+    if (!(single ? allow_smem<shared_prefix_step_kernel<E, HD>>((int)sp_smem(HD)) : allow_smem<shared_prefix_rows_kernel<E, HD>>((int)sp_smem(HD)))) return cudaErrorInvalidValue;
+    p.box_rows = SP_TT;
+    while (a.r.block_tokens % p.box_rows) p.box_rows /= 2;
+    const long rows = a.r.n_pages * a.n_kv * a.r.block_tokens;
+    CUtensorMap mk, mv;                                          // (copies move 16-bit entries whatever their format)
+    if (!bf16_rows_map(&mk, a.k_pool, HD, rows, HD, 1, 0, p.box_rows) || !bf16_rows_map(&mv, a.v_pool, HD, rows, HD, 1, 0, p.box_rows)) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid; cfg.blockDim = dim3(SP_THREADS); cfg.dynamicSmemBytes = sp_smem(HD); cfg.stream = s;
     cudaLaunchAttribute at[2];
     int n = 0;
-    if (p.role != SP_PREFIX && p.splits > 1) {
+    if (!p.prefix && p.splits > 1) {
         at[n].id = cudaLaunchAttributeClusterDimension;
         at[n].val.clusterDim.x = p.splits; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
         n++;
@@ -389,13 +669,13 @@ cudaError_t sp_rows(const SharedPrefixArgs& a, const SpPlan& p, size_t ml_at, di
         n++;
     }
     cfg.attrs = at; cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, kernel, a, p, ml_at);
+    return single ? cudaLaunchKernelEx(&cfg, shared_prefix_step_kernel<E, HD>, mk, mv, a, p) : cudaLaunchKernelEx(&cfg, shared_prefix_rows_kernel<E, HD>, mk, mv, a, p);
 }
-template <int MT>
-cudaError_t sp_rows_of(const SharedPrefixArgs& a, const SpPlan& p, size_t ml_at, dim3 grid, cudaStream_t s, bool pdl) {
+// at most 16 rows a KV head of a sequence (prefix pass: of the batch): the single-token form
+cudaError_t sp_rows_of(const SharedPrefixArgs& a, const SpPlan& p, bool single, dim3 grid, cudaStream_t s, bool pdl) {
     const bool h = a.type == ELEM_F16;
-    if (a.head_dim == 64) return h ? sp_rows<__half, 64, MT>(a, p, ml_at, grid, s, pdl) : sp_rows<__nv_bfloat16, 64, MT>(a, p, ml_at, grid, s, pdl);
-    return h ? sp_rows<__half, 128, MT>(a, p, ml_at, grid, s, pdl) : sp_rows<__nv_bfloat16, 128, MT>(a, p, ml_at, grid, s, pdl);
+    if (a.head_dim == 64) return h ? sp_rows<__half, 64>(a, p, single, grid, s, pdl) : sp_rows<__nv_bfloat16, 64>(a, p, single, grid, s, pdl);
+    return h ? sp_rows<__half, 128>(a, p, single, grid, s, pdl) : sp_rows<__nv_bfloat16, 128>(a, p, single, grid, s, pdl);
 }
 // CTAs that share a tile's keys: about two CTAs an SM in all, no fewer keys than a tile each, at most a portable cluster
 int sp_splits(long tiles, long keys, int most) {
@@ -428,39 +708,39 @@ size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim
     return (size_t)sp_most_slots(n_rows, n_head, n_kv) * n_rows * n_head * (head_dim + 2);
 }
 
+cudaError_t shared_prefix_error(unsigned int* code) {
+    const cudaError_t e = cudaMemcpyFromSymbol(code, sp_error, sizeof(*code));
+    return e == cudaSuccess && *code == 0 ? shared_prefix_tc_error(code) : e;
+}
+
 cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s) {
     const int R = a.r.n_rows, G = a.n_head / a.n_kv, S = a.r.n_seqs;
     if (R == 0 || S == 0) return cudaSuccess;
+    if ((long)prefix_cut(R, a.n_head, a.n_kv, 1).units * ((a.n_prefix + 127) / 128) > INT_MAX / 2) return cudaErrorInvalidValue;
     cudaError_t e;
     SpPlan own = {};
-    own.role = SP_OWN;
-    size_t ml_at = 0;
     bool behind = false;
     if (a.n_prefix > 0) {
-        int slots;
         if ((long)R * G <= SP_PREFIX_ROWS) {
             SpPlan p = {};
-            p.role = SP_PREFIX;
-            const int mt = R * G <= 16 ? 16 : 64;
-            p.splits = sp_splits((long)a.n_kv, a.n_prefix, SP_PREFIX_SPLITS);
-            slots = own.fixed_slots = p.splits;
-            ml_at = (size_t)slots * R * a.n_head * a.head_dim;
-            const dim3 grid(p.splits, a.n_kv, 1);
-            e = mt == 16 ? sp_rows_of<16>(a, p, ml_at, grid, s, g_chain_pdl) : sp_rows_of<64>(a, p, ml_at, grid, s, g_chain_pdl);
+            p.prefix = 1;
+            p.splits = own.fixed_slots = sp_splits((long)a.n_kv, a.n_prefix, SP_PREFIX_SPLITS);
+            p.ml_at = own.ml_at = (size_t)p.splits * R * a.n_head * a.head_dim;
+            e = sp_rows_of(a, p, R * G <= 16, dim3(p.splits, a.n_kv, 1), s, g_chain_pdl);
         } else {
             own.cut = prefix_cut(R, a.n_head, a.n_kv, a.n_prefix);
             own.fixed_slots = -1;
-            slots = (int)sp_most_slots(R, a.n_head, a.n_kv);
-            ml_at = (size_t)slots * R * a.n_head * a.head_dim;
+            own.ml_at = (size_t)sp_most_slots(R, a.n_head, a.n_kv) * R * a.n_head * a.head_dim;
             e = shared_prefix_tc_launch(a, own.cut, s);
         }
         if (e != cudaSuccess) return e;
         behind = true;
     }
-    const int mt = a.max_rows * G <= 16 ? 16 : 64, tiles = (a.max_rows * G + mt - 1) / mt;
+    const bool single = a.max_rows * G <= 16;
+    const int mt = single ? 16 : 64, tiles = (a.max_rows * G + mt - 1) / mt;
     own.splits = sp_splits((long)tiles * a.n_kv * S, (long)a.r.max_pages * a.r.block_tokens, 8);
-    const dim3 grid(tiles * own.splits, a.n_kv, S);
-    return mt == 16 ? sp_rows_of<16>(a, own, ml_at, grid, s, behind || g_chain_pdl) : sp_rows_of<64>(a, own, ml_at, grid, s, behind || g_chain_pdl);
+    own.steal = single && own.splits == 1;
+    return sp_rows_of(a, own, single, dim3(tiles * own.splits, a.n_kv, S), s, behind || g_chain_pdl);
 }
 
 }  // namespace b2

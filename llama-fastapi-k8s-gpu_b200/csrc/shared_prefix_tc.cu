@@ -29,11 +29,7 @@ __device__ __forceinline__ uint32_t st_pack(float a, float b) {
 }
 }  // namespace
 
-unsigned int* device_op_error(int device) {
-    (void)device;                                                // (the current device's copy)
-    void* p = nullptr;
-    return cudaGetSymbolAddress(&p, st_error) == cudaSuccess ? (unsigned int*)p : nullptr;
-}
+cudaError_t shared_prefix_tc_error(unsigned int* code) { return cudaMemcpyFromSymbol(code, st_error, sizeof(*code)); }
 
 template <int HD, bool F16>
 __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -65,16 +61,15 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
     griddep_launch();
     const uint32_t s_at = tmem_at, o_at = tmem_at + 256;
     const int G = a.n_head / a.n_kv, M = a.r.n_rows * G, n_prefix = a.n_prefix;
-    const long total = (long)cut.units * cut.blocks;
-    const long x0 = (long)blockIdx.x * cut.run, x1 = min(total, x0 + cut.run);
+    const int x0 = blockIdx.x * cut.run, x1 = min(cut.units * cut.blocks, x0 + cut.run);
 
     // runs of blocks of one unit: every role walks them the same way
     struct Segment { int kvh, row0, b0, n; bool two; };
-    auto segment = [&](long x) {
+    auto segment = [&](int x) {
         Segment g;
-        const int u = (int)(x / cut.blocks);
-        g.b0 = (int)(x - (long)u * cut.blocks);
-        g.n = (int)min((long)(cut.blocks - g.b0), x1 - x);
+        const int u = x / cut.blocks;
+        g.b0 = x - u * cut.blocks;
+        g.n = min(cut.blocks - g.b0, x1 - x);
         g.kvh = u / cut.pairs;
         g.row0 = u % cut.pairs * 2 * ST_ROWS;
         g.two = M - g.row0 > ST_ROWS;
@@ -85,7 +80,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
         // ================= copies: a lane has a box of keys (one page, or a part of one)
         const int bt = a.r.block_tokens, boxes = ST_K / box_rows;
         int it = 0;
-        for (long x = x0; x < x1;) {
+        for (int x = x0; x < x1;) {
             const Segment g = segment(x);
             x += g.n;
             for (int i = 0; i < g.n; i++, it++) {
@@ -115,7 +110,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
         const uint32_t id_s = tc_idesc_bf16(ST_ROWS, ST_K) & f16, id_o = tc_idesc_bf16(ST_ROWS, HD, true) & f16;
         const uint32_t qa = smem_u32(qs), ka = smem_u32(ks), va = smem_u32(vs);
         int it = 0, segs[2] = {0, 0}, done[2] = {0, 0};          // blocks of the CTA, segments and blocks of each tile so far
-        for (long x = x0; x < x1;) {
+        for (int x = x0; x < x1;) {
             const Segment g = segment(x);
             x += g.n;
             const int tiles = g.two ? 2 : 1;
@@ -171,33 +166,45 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
         }
     } else {
         // ================= softmax: a thread a row of its tile
-        const int t = warp >> 2, row = threadIdx.x & 127;
+        const int t = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_mine = s_at + t * ST_K + lanes, o_mine = o_at + t * HD + lanes;
         uint32_t done = 0;                                       // blocks of this tile so far
-        for (long x = x0; x < x1;) {
+        for (int x = x0; x < x1;) {
             const Segment g = segment(x);
-            const int unit = (int)(x / cut.blocks);
+            const int unit = x / cut.blocks;
             x += g.n;
             if (t == 1 && !g.two) continue;
-            // ---- this row's query, into 128-byte-swizzled rows (rows past the end: zeros)
-            const int f = g.row0 + t * ST_ROWS + row;
+            // ---- the warp's 32 queries, into 128-byte-swizzled rows (rows past the end: zeros): neighbouring lanes have neighbouring pieces of a row
+            const int f0 = g.row0 + t * ST_ROWS + (warp & 3) * 32, f = f0 + lane;
             const bool in = f < M;
-            const int r = in ? f / G : 0, head = g.kvh * G + (in ? f % G : 0);
-            const size_t q_at = (size_t)r * a.q_row + (size_t)head * a.q_head;
+            const int r = in ? f / G : 0, head = g.kvh * G + (in ? f - r * G : 0);
+            const size_t q_mine = (size_t)r * a.q_row + (size_t)head * a.q_head;
+            constexpr int LANES = HD / 8, ROWS = 32 / LANES;     // lanes a row, rows at once
+            // (all of a batch's loads ahead of its stores: one after the other, they took 6 us)
+            constexpr int BATCH = 8;
 #pragma unroll
-            for (int c8 = 0; c8 < HD / 8; c8++) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (in) {
+            for (int i0 = 0; i0 < 32; i0 += BATCH * ROWS) {
+                uint4 v[BATCH];
+#pragma unroll
+                for (int b = 0; b < BATCH; b++) {
+                    const int from = i0 + b * ROWS + lane / LANES;
+                    const size_t at = __shfl_sync(0xffffffffu, q_mine, from) + lane % LANES * 8;
+                    v[b] = make_uint4(0, 0, 0, 0);
+                    if (f0 + from >= M) continue;
                     if (a.q_f32) {
-                        const float* q = (const float*)a.q + q_at + c8 * 8;
-                        v = make_uint4(st_pack<F16>(q[0], q[1]), st_pack<F16>(q[2], q[3]), st_pack<F16>(q[4], q[5]), st_pack<F16>(q[6], q[7]));
+                        const float* q = (const float*)a.q + at;
+                        v[b] = make_uint4(st_pack<F16>(q[0], q[1]), st_pack<F16>(q[2], q[3]), st_pack<F16>(q[4], q[5]), st_pack<F16>(q[6], q[7]));
                     } else {
-                        const uint16_t* q = (const uint16_t*)a.q + q_at + c8 * 8;
-                        if (((uintptr_t)q & 15) == 0) v = *reinterpret_cast<const uint4*>(q);
-                        else v = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+                        const uint16_t* q = (const uint16_t*)a.q + at;
+                        if (((uintptr_t)q & 15) == 0) v[b] = *reinterpret_cast<const uint4*>(q);
+                        else v[b] = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
                     }
                 }
-                *reinterpret_cast<uint4*>(qs + (t * PARTS + (c8 >> 3)) * ST_PART + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) = v;
+#pragma unroll
+                for (int b = 0; b < BATCH; b++) {
+                    const int c8 = lane % LANES, row = (warp & 3) * 32 + i0 + b * ROWS + lane / LANES;
+                    *reinterpret_cast<uint4*>(qs + (t * PARTS + (c8 >> 3)) * ST_PART + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) = v[b];
+                }
             }
             fence_proxy_async();
             mbar_arrive(&q_full[t]);
@@ -265,15 +272,27 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
             __syncwarp();
             const int slot = blockIdx.x - cut.first_cta(unit);
             const size_t at = ((size_t)slot * a.r.n_rows + r) * a.n_head + head;
+            // 32 columns at a time through the part of shared memory that held the warp's queries (nothing reads them any more), so that a row's
+            // columns leave side by side: straight from the registers, every lane's 16 bytes went to a row of their own and a run of 4 blocks took 20 us
+            // longer than its blocks
+            uint8_t* mine = qs + t * PARTS * ST_PART + (warp & 3) * 32 * 128;
+            size_t to[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) to[i] = __shfl_sync(0xffffffffu, at, i * 4 + (lane >> 3)) * HD + (lane & 7) * 4;
 #pragma unroll
             for (int c = 0; c < HD; c += 32) {
                 uint32_t o[32];
                 __syncwarp();
                 tc_ld32(o_mine + c, o);
                 tc_wait_ld();
-                if (!in) continue;
 #pragma unroll
-                for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(a.work + at * HD + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                for (int e = 0; e < 32; e += 4) *reinterpret_cast<uint4*>(mine + lane * 128 + (((e >> 2) ^ (lane & 7)) << 4)) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                __syncwarp();
+                uint4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = *reinterpret_cast<const uint4*>(mine + (i * 4 + (lane >> 3)) * 128 + (((lane & 7) ^ ((i * 4 + (lane >> 3)) & 7)) << 4));
+#pragma unroll
+                for (int i = 0; i < 8; i++) if (f0 + i * 4 + (lane >> 3) < M) *reinterpret_cast<uint4*>(a.work + to[i] + c) = v[i];
             }
             const float2 la = f2_unpack(l2), lb = f2_unpack(l3);
             if (in) *reinterpret_cast<float2*>(a.work + ml_at + at * 2) = make_float2(m_ref, (la.x + la.y) + (lb.x + lb.y));
