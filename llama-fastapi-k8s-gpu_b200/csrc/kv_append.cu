@@ -30,19 +30,6 @@ template <> __device__ __forceinline__ __nv_bfloat16 ka_round(float v) { return 
 template <typename T, int VEC>
 struct alignas(VEC == 8 ? 16 : sizeof(T)) Piece { T v[VEC]; };
 
-// the sequence of row `row`: how many of row_start[1..n_seqs] are <= row, by the whole warp, 32 probes a round
-__device__ __forceinline__ int seq_of_row(const int* row_start, int n_seqs, int row, int lane) {
-    int lo = 0, n = n_seqs;                                      // the count lies in [lo, lo + n]
-    while (n > 0) {
-        const int step = (n + 31) / 32, at = lo + (lane + 1) * step - 1;        // probes entries lo + step - 1, lo + 2 step - 1, ...
-        const bool below = at < lo + n && row_start[1 + at] <= row;
-        const int passed = __popc(__ballot_sync(0xffffffffu, below));
-        const int skip = min(passed * step, n);
-        lo += skip;
-        n = min(n - skip, step - 1);
-    }
-    return lo;
-}
 }  // namespace
 
 template <typename In, typename Out, int VEC, int ROWS>

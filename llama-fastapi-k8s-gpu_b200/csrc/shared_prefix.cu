@@ -65,7 +65,9 @@ struct SpPlan {
     int prefix;                  // 1: the prefix for all rows, partial results; 0: a sequence's own tokens, behind the prefix's results
     int splits;                  // CTAs that share the keys of a tile of rows (a cluster, except for the prefix)
     int steal;                   // single-token form without splits: a CTA goes on with the work of CTAs that have not started
-    int fixed_slots;             // partial results of the prefix per row (0: none; < 0: as `cut` says)
+    int fixed_slots;             // partial results of the prefix per row that this pass joins (0: none; < 0: as `cut` says)
+    int own_slot;                // >= 0: beside the prefix pass on tensor memory: its results are partial ones too, in this slot, and a third kernel joins
+    int mrows;                   // rows of a tile that q is staged for (single-token form)
     int box_rows;                // keys of a copy: a page, or a power of two that divides it
     PrefixCut cut;
     size_t ml_at;                // where the (maximum, sum) of the partial results lie in the workspace
@@ -99,7 +101,7 @@ struct SpWork {
             }
             own = min(own, a.r.max_pages * bt);
         }
-        f0 = tile * mt; n_f = min(mt, n_tok * G - f0);
+        f0 = tile * mt; n_f = min(mt, (own_pass ? min(n_tok, a.max_rows) : n_tok) * G - f0);
         lim_lo = limit(f0 / G); lim_hi = limit((f0 + max(n_f, 1) - 1) / G);
         const int chunk = ((lim_hi + p.splits - 1) / p.splits + SP_TT - 1) / SP_TT * SP_TT;
         q0 = min(lim_hi, split * chunk); q1 = min(lim_hi, q0 + chunk);
@@ -146,6 +148,25 @@ __device__ __forceinline__ bool sp_answered_work(const uint64_t* answer, int& x,
                  : "=&r"(got), "=&r"(i), "=&r"(j), "=&r"(k) : "l"(answer[0]), "l"(answer[1]) : "memory");
     x = (int)i; y = (int)j; z = (int)k;
     return got != 0;
+}
+
+// The tile's queries into shared memory, rows padded by 16 bytes, by `n` threads
+template <typename E, int HD>
+__device__ __forceinline__ void sp_stage_q(const SharedPrefixArgs& a, const SpWork& w, int kvh, uint16_t* q_s, int thread, int n) {
+    for (int e = thread; e < w.n_f * (HD / 8); e += n) {
+        const int row = e / (HD / 8), c8 = e % (HD / 8), f = w.f0 + row, i = f / w.G;
+        const size_t at = (size_t)(w.r0 + i) * a.q_row + (size_t)(kvh * w.G + f - i * w.G) * a.q_head + c8 * 8;
+        uint4 v;
+        if (a.q_f32) {
+            const float* q = (const float*)a.q + at;
+            v = make_uint4(SpType<E>::pack(q[0], q[1]), SpType<E>::pack(q[2], q[3]), SpType<E>::pack(q[4], q[5]), SpType<E>::pack(q[6], q[7]));
+        } else {
+            const uint16_t* q = (const uint16_t*)a.q + at;
+            if (((uintptr_t)q & 15) == 0) v = *reinterpret_cast<const uint4*>(q);
+            else v = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+        }
+        *reinterpret_cast<uint4*>(q_s + row * (HD + 8) + c8 * 8) = v;
+    }
 }
 
 // q fragments of rows f and f + 8 (numbered within the sequence; `in`: they belong to the tile)
@@ -233,8 +254,8 @@ template <typename E, int HD, int N>
 __device__ __forceinline__ void sp_finish(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, int kvh, int split, int row, int col, float m, float l, const float (&o)[N][4], int h,
                                           float* acc, float* row_m, float* row_l) {
     const int f = w.f0 + row, i = f / w.G, head = kvh * w.G + f - i * w.G;
-    if (!w.own_pass) {
-        const size_t at = sp_part(a, split, w.r0 + i, head);
+    if (!w.own_pass || p.own_slot >= 0) {
+        const size_t at = sp_part(a, w.own_pass ? p.own_slot : split, w.r0 + i, head);
 #pragma unroll
         for (int nt = 0; nt < N; nt++) *reinterpret_cast<float2*>(a.work + at * HD + col + nt * 8) = make_float2(o[nt][2 * h], o[nt][2 * h + 1]);
         if (col == 0) *reinterpret_cast<float2*>(a.work + p.ml_at + at * 2) = make_float2(m, l);
@@ -292,6 +313,7 @@ __device__ __forceinline__ bool sp_any_bad(uint8_t* vb, int ks, int c0, int n, i
 // probabilities go through shared memory; weighted sums: a warp has a quarter of the dims and all 64 keys, so that nothing has to be merged at the end.
 // What a CTA waits for before its first keys are here takes as long as the keys of some 100 tokens (3 us): CTAs that run go on with the work of those that have not
 // started (p.steal), and their copies run ahead into it.
+// Beside the prefix pass on tensor memory (p.own_slot >= 0) nothing waits for that pass before the end.
 // grid: (tile * splits + split, KV head, sequence)
 template <typename E, int HD>
 __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedPrefixArgs a,
@@ -307,6 +329,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
     __shared__ alignas(16) uint16_t prob[2][16][SP_TT + 8];
     uint8_t* tiles_at = reinterpret_cast<uint8_t*>(((uintptr_t)sp_raw + 1023) & ~(uintptr_t)1023);      // [stage][keys, values][part]
     float* acc = reinterpret_cast<float*>(tiles_at);             // [16][HD], behind the last tile of a CTA that shares its keys
+    uint16_t* q_s = reinterpret_cast<uint16_t*>(tiles_at + STAGES * 2 * PARTS * PART);      // [2][mrows][HD + 8], by turns
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, tq = lane & 3;
     if (tid == 0) {
         for (int i = 0; i < STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], SP_WARPS); }
@@ -315,12 +338,13 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
         fence_mbar_init();
     }
     // behind another kernel of the engine's chain: what it wrote (q, this step's keys). Behind the prefix pass that is long done.
-    if (p.prefix || p.fixed_slots == 0) griddep_wait();
-    griddep_launch();
+    if (p.prefix || (p.fixed_slots == 0 && p.own_slot < 0)) griddep_wait();
+    if (p.own_slot < 0) griddep_launch();
     const int split = blockIdx.x % p.splits;
     int kvh = blockIdx.y;
     SpWork w(a, p, 16, blockIdx.x / p.splits, split, blockIdx.z);
-    if (w.n_f <= 0) { griddep_wait(); return; }                  // (all CTAs of the cluster, none of which ends before the prefix pass)
+    if (w.n_f <= 0 && !p.steal) { griddep_wait(); return; }      // (all CTAs of the cluster, none of which ends before the prefix pass)
+    if (w.n_f <= 0) w.n_tiles = 0;
     __syncthreads();
 
     if (warp == SP_WARPS) {
@@ -342,7 +366,9 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
                 __syncwarp();
                 if (lane == 0) { fence_proxy_async(); sp_ask_work(answer, &answered); }
             }
-            if (n >= 2) mbar_wait_warp(&next_empty[n & 1], ((n >> 1) - 1) & 1, sp_error, 0xa0005u, (unsigned)n);
+            // (work n + 1's place, and the queries of work n - 1, are free again)
+            if (n >= 1) mbar_wait_warp(&next_empty[n & 1], ((n - 1) >> 1) & 1, sp_error, 0xa0005u, (unsigned)n);
+            if (more) sp_stage_q<E, HD>(a, v, v_kvh, q_s + ((n + 1) & 1) * p.mrows * (HD + 8), lane, 32);
             __syncwarp();
             if (lane == 0) {
                 if (!more) v.n_f = -1;
@@ -361,14 +387,23 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
                 mbar_wait(&next_full[i], ((hh - 1) >> 1) & 1, sp_error, 0xa0006u, (unsigned)hh);
                 if (next[i].n_f < 0) break;
                 w = next[i]; kvh = next_kvh[i];
+            } else {
+                sp_stage_q<E, HD>(a, w, kvh, q_s, tid, SP_WARPS * 32);
+                named_bar_sync(1, SP_WARPS * 32);
+            }
+            if (w.n_f <= 0) {                                    // (only the first work may have no rows)
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&next_empty[i]);
+                if (lane == 0) mbar_arrive(&next_empty[1]);
+                continue;
             }
             int lim[2];
 #pragma unroll
             for (int h = 0; h < 2; h++) lim[h] = g + 8 * h < w.n_f ? min(w.q1, w.limit((w.f0 + g + 8 * h) / w.G)) : w.q1;
-            uint32_t qa[HD / 16][4];
-            sp_load_q<E, HD>(a, w, kvh, g, tq, qa);
+            uint32_t qa[HD / 16][4];                             // (rows past the staged ones repeat the last: nothing of them is kept)
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; kk++) sp_ldmatrix_x4(qa[kk], q_s + (hh & 1) * p.mrows * (HD + 8) + min(lane & 15, p.mrows - 1) * (HD + 8) + kk * 16 + (lane >> 4) * 8);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&next_empty[(hh + 1) & 1]);
             float o[NT][4], m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};      // (l: this thread's columns of scores)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
@@ -389,10 +424,12 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
                 mbar_wait(&full[st], (it / STAGES) & 1, sp_error, 0xa0002u, (unsigned)it);
                 __syncwarp();
                 // ---- scores of this warp's keys, scaled, masked, and their maxima in rows g and g + 8; this thread's columns are 2 tq, 2 tq + 1 of every eight keys
-                float sc[2][4], mx[2] = {-INFINITY, -INFINITY};
+                float sc[2][4], sd[2][4], mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                for (int nt = 0; nt < 2; nt++) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-                if (k0 < valid) {
+                for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) sc[nt][e] = sd[nt][e] = 0.f;
+                if (k0 < valid) {                                // (two sums, added up: shorter chains of dependent products)
 #pragma unroll
                     for (int nt = 0; nt < 2; nt++)
 #pragma unroll
@@ -400,7 +437,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
                             uint32_t b4[4];                      // dims kk * 16 .. + 31 of eight keys
                             sp_ldmatrix_x4(b4, sp_piece(kb, k0 + nt * 8 + (lane & 7), kk * 2 + (lane >> 3)));
                             T::mma(sc[nt], qa[kk], b4[0], b4[1]);
-                            T::mma(sc[nt], qa[kk + 1], b4[2], b4[3]);
+                            T::mma(sd[nt], qa[kk + 1], b4[2], b4[3]);
                         }
                 }
 #pragma unroll
@@ -408,7 +445,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         const int key = t0 + k0 + nt * 8 + 2 * tq + (e & 1);
-                        sc[nt][e] = key < lim[e >> 1] ? sc[nt][e] * a.scale_log2 : -INFINITY;
+                        sc[nt][e] = key < lim[e >> 1] ? (sc[nt][e] + sd[nt][e]) * a.scale_log2 : -INFINITY;
                         mx[e >> 1] = fmaxf(mx[e >> 1], sc[nt][e]);
                     }
 #pragma unroll
@@ -492,6 +529,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
         }
     }
     if (w.own_pass && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
+    if (p.own_slot >= 0) { griddep_launch(); griddep_wait(); }   // (a kernel behind this one is behind the prefix pass too)
 }
 
 // Several tokens of a sequence, or the prefix pass of up to 64 rows: a tile of 64 rows, a warp has 16 of them and all keys.
@@ -641,21 +679,77 @@ __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const
     if (w.own_pass && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
 }
 
+// The partial results of the prefix pass on tensor memory and of the pass over the own tokens, joined: a CTA a row of the batch, a thread four dims of a head.
+constexpr int SP_JOIN = 256;
+template <typename E, int HD>
+__global__ void __launch_bounds__(SP_JOIN) shared_prefix_join_kernel(const SharedPrefixArgs a, const SpPlan p) {
+    __shared__ int live;
+    const int t = blockIdx.x, G = a.n_head / a.n_kv;
+    griddep_wait();
+    griddep_launch();
+    // rows that no sequence has, or that are past a sequence's max_rows, have no result
+    if (!a.tab) {
+        if (threadIdx.x < 32) {
+            const int s = seq_of_row(a.r.row_start, a.r.n_seqs, t, threadIdx.x);
+            if (threadIdx.x == 0) live = s < a.r.n_seqs && t >= a.r.row_start[0] && t - max(0, a.r.row_start[s]) < a.max_rows;
+        }
+        __syncthreads();
+        if (!live) return;
+    }
+    const size_t step = (size_t)a.r.n_rows * a.n_head;
+    for (int e = threadIdx.x; e < a.n_head * (HD / 4); e += SP_JOIN) {
+        const int head = e / (HD / 4), d = e % (HD / 4) * 4, kvh = head / G;
+        const int slots = p.cut.slots(kvh * p.cut.pairs + (t * G + head - kvh * G) / 256);
+        const size_t at = sp_part(a, 0, t, head);
+        const float* ml = a.work + p.ml_at + at * 2;
+        const float* from = a.work + at * HD + d;
+        float m = -INFINITY, l = 0.f;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int B = 4;                                     // results under way
+        for (int j0 = 0; j0 <= slots; j0 += B) {                 // (number `slots`: the own tokens')
+            float2 one[B];
+            float4 v[B];
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                one[j] = make_float2(-INFINITY, 0.f); v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (j0 + j > slots) continue;
+                const size_t off = (j0 + j < slots ? j0 + j : p.own_slot) * step;
+                one[j] = __ldcg(reinterpret_cast<const float2*>(ml + off * 2));
+                v[j] = __ldcg(reinterpret_cast<const float4*>(from + off * HD));
+            }
+            float m2 = m;
+#pragma unroll
+            for (int j = 0; j < B; j++) m2 = fmaxf(m2, one[j].x);
+            const float ref = m2 == -INFINITY ? 0.f : m2, fall = sp_exp2(m - ref);
+            m = m2; l *= fall; sum.x *= fall; sum.y *= fall; sum.z *= fall; sum.w *= fall;
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                const float c = sp_exp2(one[j].x - ref);
+                l = fmaf(c, one[j].y, l);
+                sum.x = fmaf(c, v[j].x, sum.x); sum.y = fmaf(c, v[j].y, sum.y); sum.z = fmaf(c, v[j].z, sum.z); sum.w = fmaf(c, v[j].w, sum.w);
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;              // (0: no keys. A NaN stays one.)
+        sp_store_out<E, HD>(a, t, head, d, sum.x * inv, sum.y * inv);
+        sp_store_out<E, HD>(a, t, head, d + 2, sum.z * inv, sum.w * inv);
+    }
+}
+
 // ---------------------------------------------------------------- host side
 namespace {
 constexpr int SP_SMS = 148;
-constexpr size_t sp_smem(int hd) { return (size_t)sp_stages(hd) * 2 * SP_TT * hd * 2 + 1024; }
+constexpr size_t sp_smem(int hd, int mrows) { return (size_t)sp_stages(hd) * 2 * SP_TT * hd * 2 + 2 * mrows * (hd + 8) * 2 + 1024; }
 
 template <typename E, int HD>
 cudaError_t sp_rows(const SharedPrefixArgs& a, SpPlan p, bool single, dim3 grid, cudaStream_t s, bool pdl) {
-    if (!(single ? allow_smem<shared_prefix_step_kernel<E, HD>>((int)sp_smem(HD)) : allow_smem<shared_prefix_rows_kernel<E, HD>>((int)sp_smem(HD)))) return cudaErrorInvalidValue;
+    if (!(single ? allow_smem<shared_prefix_step_kernel<E, HD>>((int)sp_smem(HD, 16)) : allow_smem<shared_prefix_rows_kernel<E, HD>>((int)sp_smem(HD, 0)))) return cudaErrorInvalidValue;
     p.box_rows = SP_TT;
     while (a.r.block_tokens % p.box_rows) p.box_rows /= 2;
     const long rows = a.r.n_pages * a.n_kv * a.r.block_tokens;
     CUtensorMap mk, mv;                                          // (copies move 16-bit entries whatever their format)
     if (!bf16_rows_map(&mk, a.k_pool, HD, rows, HD, 1, 0, p.box_rows) || !bf16_rows_map(&mv, a.v_pool, HD, rows, HD, 1, 0, p.box_rows)) return cudaErrorInvalidValue;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid; cfg.blockDim = dim3(SP_THREADS); cfg.dynamicSmemBytes = sp_smem(HD); cfg.stream = s;
+    cfg.gridDim = grid; cfg.blockDim = dim3(SP_THREADS); cfg.dynamicSmemBytes = sp_smem(HD, single ? p.mrows : 0); cfg.stream = s;
     cudaLaunchAttribute at[2];
     int n = 0;
     if (!p.prefix && p.splits > 1) {
@@ -670,6 +764,16 @@ cudaError_t sp_rows(const SharedPrefixArgs& a, SpPlan p, bool single, dim3 grid,
     }
     cfg.attrs = at; cfg.numAttrs = n;
     return single ? cudaLaunchKernelEx(&cfg, shared_prefix_step_kernel<E, HD>, mk, mv, a, p) : cudaLaunchKernelEx(&cfg, shared_prefix_rows_kernel<E, HD>, mk, mv, a, p);
+}
+template <typename E, int HD>
+cudaError_t sp_join(const SharedPrefixArgs& a, const SpPlan& p, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(a.r.n_rows); cfg.blockDim = dim3(SP_JOIN); cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, shared_prefix_join_kernel<E, HD>, a, p);
 }
 // at most 16 rows a KV head of a sequence (prefix pass: of the batch): the single-token form
 cudaError_t sp_rows_of(const SharedPrefixArgs& a, const SpPlan& p, bool single, dim3 grid, cudaStream_t s, bool pdl) {
@@ -702,7 +806,7 @@ PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix) {
 static long sp_most_slots(long n_rows, int n_head, int n_kv) {
     if (n_rows * (n_head / n_kv) <= SP_PREFIX_ROWS) return SP_PREFIX_SPLITS;
     const PrefixCut c = prefix_cut(n_rows, n_head, n_kv, 1);
-    return (SP_SMS + c.units - 1) / c.units + 1;
+    return (SP_SMS + c.units - 1) / c.units + 2;                  // (and the own tokens')
 }
 size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim) {
     return (size_t)sp_most_slots(n_rows, n_head, n_kv) * n_rows * n_head * (head_dim + 2);
@@ -724,6 +828,7 @@ cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s) {
         if ((long)R * G <= SP_PREFIX_ROWS) {
             SpPlan p = {};
             p.prefix = 1;
+            p.mrows = R * G; p.own_slot = -1;
             p.splits = own.fixed_slots = sp_splits((long)a.n_kv, a.n_prefix, SP_PREFIX_SPLITS);
             p.ml_at = own.ml_at = (size_t)p.splits * R * a.n_head * a.head_dim;
             e = sp_rows_of(a, p, R * G <= 16, dim3(p.splits, a.n_kv, 1), s, g_chain_pdl);
@@ -740,7 +845,16 @@ cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s) {
     const int mt = single ? 16 : 64, tiles = (a.max_rows * G + mt - 1) / mt;
     own.splits = sp_splits((long)tiles * a.n_kv * S, (long)a.r.max_pages * a.r.block_tokens, 8);
     own.steal = single && own.splits == 1;
-    return sp_rows_of(a, own, single, dim3(tiles * own.splits, a.n_kv, S), s, behind || g_chain_pdl);
+    own.mrows = single ? a.max_rows * G : 0;
+    own.own_slot = -1;
+    // single tokens run beside the pass on tensor memory, whose CTAs leave them room, and are joined with it afterwards
+    const bool beside = own.fixed_slots < 0 && own.steal;
+    if (beside) { own.own_slot = (int)sp_most_slots(R, a.n_head, a.n_kv) - 1; own.fixed_slots = 0; }
+    const cudaError_t e2 = sp_rows_of(a, own, single, dim3(tiles * own.splits, a.n_kv, S), s, behind || g_chain_pdl);
+    if (e2 != cudaSuccess || !beside) return e2;
+    const bool h = a.type == ELEM_F16;
+    if (a.head_dim == 64) return h ? sp_join<__half, 64>(a, own, s) : sp_join<__nv_bfloat16, 64>(a, own, s);
+    return h ? sp_join<__half, 128>(a, own, s) : sp_join<__nv_bfloat16, 128>(a, own, s);
 }
 
 }  // namespace b2

@@ -1,10 +1,10 @@
 // The prefix pass of shared_prefix.cu on the 5th-generation tensor cores: many query rows of a KV head over the keys that all sequences share.
 //
 // Rows are (row of the batch, head of the KV head's group); a unit is 256 of them, two tiles of 128. A CTA takes a run of key blocks of 128 (PrefixCut), which
-// may end one unit and start the next. Keys and values come by tensor copies from their pages (64 columns a part in 128-byte-swizzled rows, two stages
-// each) and serve both tiles. Tensor memory: two score tiles (2 x 128 columns, probabilities are written over them as the A operand of the second product)
-// and two outputs. While one tile's softmax runs, the other's products do. Warps 0-3 and 4-7: softmax of a tile, a thread a row; 8: copies; 9: matrix
-// instructions.
+// may end one unit and start the next. Keys and values come by tensor copies from their pages (64 columns a part in 128-byte-swizzled rows, two blocks under
+// way) and serve both tiles. Tensor memory: two score tiles (2 x 128 columns, probabilities are written over them as the A operand of the second product) and
+// two outputs. While one tile's softmax runs, the other's products do; the second product starts with the first half of the probabilities. Warps 0-3 and 4-7:
+// softmax of a tile, a thread a row, scores read from tensor memory twice (maximum, then exponentials); 8: copies; 9: matrix instructions.
 // The output is rescaled only where a row's maximum has grown by more than 2^8 (probabilities are then up to 2^8, sums stay 32-bit).
 #include "device_ops.h"
 #include "ptx.cuh"
@@ -36,7 +36,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
                                                                          const SharedPrefixArgs a, const PrefixCut cut, const int box_rows, const size_t ml_at) {
     constexpr int PARTS = HD / 64;
     extern __shared__ uint8_t st_smem[];
-    __shared__ uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+    __shared__ uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2];
     __shared__ uint32_t tmem_at;
     unsigned int* err = st_error;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
         if (lane == 0) {
             for (int i = 0; i < 2; i++) {
                 mbar_init(&q_full[i], 128); mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
-                mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1);
+                mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 128); mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1);
             }
             fence_mbar_init();
         }
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
     tc_after_sync();
     griddep_wait();
     griddep_launch();
-    const uint32_t s_at = tmem_at, o_at = tmem_at + 256;
+    const uint32_t s_at = __shfl_sync(0xffffffffu, tmem_at, 0), o_at = s_at + 256;      // (known to be uniform)
     const int G = a.n_head / a.n_kv, M = a.r.n_rows * G, n_prefix = a.n_prefix;
     const int x0 = blockIdx.x * cut.run, x1 = min(cut.units * cut.blocks, x0 + cut.run);
 
@@ -105,7 +105,6 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
         }
     } else if (warp == 9) {
         // ================= matrix instructions (all lanes run the loop, one issues)
-        const bool one = elect_one();
         const uint32_t f16 = F16 ? ~((1u << 7) | (1u << 10)) : ~0u;      // (tc_idesc_bf16 without the bits that say bf16)
         const uint32_t id_s = tc_idesc_bf16(ST_ROWS, ST_K) & f16, id_o = tc_idesc_bf16(ST_ROWS, HD, true) & f16;
         const uint32_t qa = smem_u32(qs), ka = smem_u32(ks), va = smem_u32(vs);
@@ -115,13 +114,10 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
             x += g.n;
             const int tiles = g.two ? 2 : 1;
             auto scores = [&](int t, int at) {
-                if (!one) return;
                 const uint64_t dq = tc_desc(qa + t * PARTS * ST_PART), dk = tc_desc(ka + (at & 1) * PARTS * ST_PART);
 #pragma unroll
-                for (int c = 0; c < PARTS; c++)
-#pragma unroll
-                    for (int k = 0; k < 4; k++) tc_mma(s_at + t * ST_K, dq + c * (ST_PART >> 4) + 2 * k, dk + c * (ST_PART >> 4) + 2 * k, id_s, (c | k) ? 1u : 0u);
-                tc_commit(&s_full[t]);
+                for (int c = 0; c < PARTS; c++) tc_mma4_one<2, 2>(s_at + t * ST_K, dq + c * (ST_PART >> 4), dk + c * (ST_PART >> 4), id_s, c ? 1u : 0u);
+                tc_commit_one(&s_full[t]);
             };
             mbar_wait_warp(&k_full[it & 1], (it >> 1) & 1, err, 0x90002u, (unsigned)it);
             for (int t = 0; t < tiles; t++) {
@@ -129,7 +125,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
                 tc_after_sync();
                 scores(t, it);
             }
-            if (one) tc_commit(&k_empty[it & 1]);
+            tc_commit_one(&k_empty[it & 1]);
             for (int i = 0; i < g.n; i++) {
                 const int at = it + i;
                 mbar_wait_warp(&v_full[at & 1], (at >> 1) & 1, err, 0x90004u, (unsigned)at);
@@ -144,21 +140,26 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
                 }
                 const uint64_t dv = tc_desc(va + (at & 1) * PARTS * ST_PART, ST_PART);
                 for (int t = 0; t < tiles; t++) {
-                    mbar_wait_warp(&p_full[t], done[t] & 1, err, 0x90005u, (unsigned)at);
+                    auto sums = [&](int k0, int k1) {            // 16-key steps k0 .. k1 - 1 of the block
+                        if (k1 - k0 == 4) tc_mma4_ts_one<8, 128>(o_at + t * HD, s_at + t * ST_K + k0 * 8, dv + k0 * 128, id_o, (i | k0) ? 1u : 0u);
+                        else for (int k = k0; k < k1; k++) tc_mma_ts_one(o_at + t * HD, s_at + t * ST_K + k * 8, dv + k * 128, id_o, (i | k) ? 1u : 0u);
+                    };
+                    mbar_wait_warp(&p_half[t], done[t] & 1, err, 0x90005u, (unsigned)at);
+                    tc_after_sync();
+                    sums(0, min(steps, 4));
+                    mbar_wait_warp(&p_full[t], done[t] & 1, err, 0x9000au, (unsigned)at);
                     done[t]++;
                     tc_after_sync();
-                    if (one) {
-                        for (int k = 0; k < steps; k++) tc_mma_ts(o_at + t * HD, s_at + t * ST_K + k * 8, dv + k * (2048 >> 4), id_o, (i | k) ? 1u : 0u);
-                        tc_commit(&pv_done[t]);
-                        if (t == tiles - 1) tc_commit(&v_empty[at & 1]);
-                    }
+                    sums(4, max(steps, 4));
+                    tc_commit_one(&pv_done[t]);
+                    if (t == tiles - 1) tc_commit_one(&v_empty[at & 1]);
                     if (i + 1 < g.n) {
                         // the next scores replace the probabilities that this product reads
                         mbar_wait_warp(&pv_done[t], (done[t] - 1) & 1, err, 0x90009u, (unsigned)at);
                         if (t == 0) { mbar_wait_warp(&k_full[(at + 1) & 1], ((at + 1) >> 1) & 1, err, 0x90002u, (unsigned)at); }
                         tc_after_sync();
                         scores(t, at + 1);
-                        if (one && t == tiles - 1) tc_commit(&k_empty[(at + 1) & 1]);
+                        if (t == tiles - 1) tc_commit_one(&k_empty[(at + 1) & 1]);
                     }
                 }
             }
@@ -215,18 +216,26 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
                 mbar_wait(&s_full[t], done & 1, err, 0x90006u, done);
                 tc_after_sync();
                 __syncwarp();
-                uint32_t raw[4][32];
-#pragma unroll
-                for (int c = 0; c < 4; c++) tc_ld32(s_mine + c * 32, raw[c]);
-                tc_wait_ld();
                 const int valid = n_prefix - (g.b0 + i) * ST_K;
-                if (valid < ST_K) {
+                // 32 scores at a time, the next ones on their way: the maximum, then the exponentials
+                uint32_t raw[2][32];
+                auto load = [&](int c) { tc_ld32(s_mine + c * 32, raw[c & 1]); };
+                auto mask = [&](int c) {
+                    if (valid < ST_K) {
 #pragma unroll
-                    for (int j = 0; j < ST_K; j++) if (j >= valid) raw[j >> 5][j & 31] = 0xff800000u;
-                }
+                        for (int j = 0; j < 32; j++) if (c * 32 + j >= valid) raw[c & 1][j] = 0xff800000u;
+                    }
+                };
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                load(0);
 #pragma unroll
-                for (int j = 0; j < ST_K; j++) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(raw[j >> 5][j & 31]));
+                for (int c = 0; c < 4; c++) {
+                    tc_wait_ld(raw[c & 1]);
+                    load((c + 1) & 3);                           // (the last of these: the first scores again)
+                    mask(c);
+#pragma unroll
+                    for (int j = 0; j < 32; j++) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(raw[c & 1][j]));
+                }
                 const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
                 const bool grow = mx > m_ref + 8.f || (m_ref == -INFINITY && mx > -INFINITY);
                 float fall = 1.f;
@@ -238,33 +247,39 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
                 }
                 const float ref = m_ref > -INFINITY ? -m_ref : 0.f;
                 const uint64_t ref2 = f2_pack(ref, ref);
-                uint32_t p[2][32];
-#pragma unroll
-                for (int j = 0; j < ST_K; j += 2) {
-                    const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[j >> 5][j & 31]), __uint_as_float(raw[j >> 5][(j & 31) + 1])), scale2, ref2));
-                    const float e0 = st_exp2(d.x), e1 = st_exp2(d.y);
-                    if (j & 2) l3 = f2_add(l3, f2_pack(e0, e1)); else l2 = f2_add(l2, f2_pack(e0, e1));
-                    p[j >> 6][(j & 63) >> 1] = st_pack<F16>(e0, e1);
-                }
                 if (i > 0 && __any_sync(0xffffffffu, grow)) {    // the products so far must be in before they are rescaled
+                    tc_wait_ld(raw[0]);
                     mbar_wait(&pv_done[t], (done - 1) & 1, err, 0x90007u, done);
                     tc_after_sync();
                     __syncwarp();
-                    for (int c = 0; c < HD; c += 32) {
-                        uint32_t o[32];
-                        tc_ld32(o_mine + c, o);
-                        tc_wait_ld();
+                    for (int c = 0; c < HD; c += 16) {
+                        float o[16];
+                        tc_ld16(o_mine + c, o);
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * fall);
-                        tc_st32(o_mine + c, o);
+                        for (int e = 0; e < 16; e++) o[e] *= fall;
+                        tc_st16(o_mine + c, o);
                     }
                 }
-                __syncwarp();
-                tc_st32(s_mine, p[0]);
-                tc_st32(s_mine + 32, p[1]);
-                tc_wait_st();
-                tc_before_sync();
-                mbar_arrive(&p_full[t]);
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    tc_wait_ld(raw[c & 1]);
+                    if (c < 3) load(c + 1);
+                    mask(c);
+                    uint32_t p[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(raw[c & 1][j]), __uint_as_float(raw[c & 1][j + 1])), scale2, ref2));
+                        const float e0 = st_exp2(d.x), e1 = st_exp2(d.y);
+                        if (j & 2) l3 = f2_add(l3, f2_pack(e0, e1)); else l2 = f2_add(l2, f2_pack(e0, e1));
+                        p[j >> 1] = st_pack<F16>(e0, e1);
+                    }
+                    tc_st16(s_mine + c * 16, p);                 // over scores that have been read
+                    if (c == 1 || c == 3) {
+                        tc_wait_st();
+                        tc_before_sync();
+                        mbar_arrive(c == 1 ? &p_half[t] : &p_full[t]);
+                    }
+                }
             }
             // ---- this segment's results of the row
             mbar_wait(&pv_done[t], (done - 1) & 1, err, 0x90008u, done);
