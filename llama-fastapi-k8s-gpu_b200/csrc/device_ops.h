@@ -85,13 +85,23 @@ struct SharedPrefixArgs {
 size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim);
 cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s);
 
-// Prefix pass on tensor memory: the key blocks of every (KV head, 256 query rows) laid end to end and cut into equal runs, one run a CTA. A unit's
-// partial results are numbered by the CTAs that its blocks fall to.
+// Prefix pass on tensor memory: the key blocks of every (KV head, 256 query rows) cut into equal runs, one run a CTA. A unit's partial results are numbered by
+// the CTAs that its blocks fall to.
 struct PrefixCut {
     int units, pairs, blocks, run, ctas;      // units = n_kv * pairs; blocks of 128 keys a unit; blocks a CTA
+    int per_unit;                             // != 0: every unit is cut by itself, else all of them laid end to end
+    __host__ __device__ int runs() const { return (blocks + run - 1) / run; }      // (of a unit that is cut by itself)
     // (units * blocks fits 31 bits: shared_prefix_launch refuses more)
-    __host__ __device__ int first_cta(int unit) const { return (int)((unsigned)(unit * blocks) / (unsigned)run); }
-    __host__ __device__ int slots(int unit) const { return (int)((unsigned)((unit + 1) * blocks - 1) / (unsigned)run) - first_cta(unit) + 1; }
+    __host__ __device__ int first_cta(int unit) const { return per_unit ? unit * runs() : (int)((unsigned)(unit * blocks) / (unsigned)run); }
+    __host__ __device__ int slots(int unit) const {
+        return per_unit ? runs() : (int)((unsigned)((unit + 1) * blocks - 1) / (unsigned)run) - first_cta(unit) + 1;
+    }
+    // the blocks [begin, end) of all units laid end to end that a CTA has
+    __host__ __device__ int begin(int cta) const { return per_unit ? cta / runs() * blocks + cta % runs() * run : cta * run; }
+    __host__ __device__ int end(int cta) const {
+        const int e = begin(cta) + run, most = per_unit ? (cta / runs() + 1) * blocks : units * blocks;
+        return e < most ? e : most;
+    }
 };
 PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix);
 cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, cudaStream_t s);

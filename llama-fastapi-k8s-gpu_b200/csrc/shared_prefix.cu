@@ -86,20 +86,22 @@ struct SpWork {
     // keys that token i of the sequence sees
     __device__ int limit(int i) const { return own_pass ? max(0, own - n_tok + i + 1) : own; }
     __device__ SpWork() {}
-    __device__ SpWork(const SharedPrefixArgs& a, const SpPlan& p, int mt, int tile, int split, int z) {
-        const int bt = a.r.block_tokens;
+    // what a sequence's work is known from: its first row, the row behind it, its own tokens
+    struct Read { int b, e, held; };
+    static __device__ __forceinline__ Read read(const SharedPrefixArgs& a, int z) {
+        if (a.tab) return {z, z + 1, a.tab[a.slots.slot[z]].ints[1] + 1 - a.n_prefix};
+        return {a.r.row_start[z], a.r.row_start[z + 1], a.r.lengths[z]};
+    }
+    static __device__ __forceinline__ const int* table_of(const SharedPrefixArgs& a, int z) {
+        return a.tab ? a.tab[a.slots.slot[z]].block_table + a.n_prefix / a.r.block_tokens : a.r.pages + z * a.r.table_stride;
+    }
+    __device__ SpWork(const SharedPrefixArgs& a, const SpPlan& p, int mt, int tile, int split, int z) : SpWork(a, p, mt, tile, split, z, p.prefix ? Read{0, 0, 0} : read(a, z)) {}
+    __device__ SpWork(const SharedPrefixArgs& a, const SpPlan& p, int mt, int tile, int split, int z, const Read& r) {
         G = a.n_head / a.n_kv; own_pass = !p.prefix;
         r0 = 0; n_tok = a.r.n_rows; own = a.n_prefix; table = a.prefix_pages;
         if (own_pass) {
-            if (a.tab) {
-                const SlotDev sd = a.tab[a.slots.slot[z]];
-                r0 = z; n_tok = 1; own = sd.ints[1] + 1 - a.n_prefix; table = sd.block_table + a.n_prefix / bt;
-            } else {
-                const int b = a.r.row_start[z], e = a.r.row_start[z + 1];
-                own = a.r.lengths[z];
-                r0 = max(0, b); n_tok = min(e, a.r.n_rows) - r0; table = a.r.pages + z * a.r.table_stride;
-            }
-            own = min(own, a.r.max_pages * bt);
+            r0 = max(0, r.b); n_tok = min(r.e, a.r.n_rows) - r0; table = table_of(a, z);
+            own = min(r.held, a.r.max_pages * a.r.block_tokens);
         }
         f0 = tile * mt; n_f = min(mt, (own_pass ? min(n_tok, a.max_rows) : n_tok) * G - f0);
         lim_lo = limit(f0 / G); lim_hi = limit((f0 + max(n_f, 1) - 1) / G);
@@ -109,17 +111,16 @@ struct SpWork {
     }
 };
 
-// The copying warp: the tiles of keys and values of one KV head, numbers it .. it + n_tiles - 1 of the CTA. A lane has a box of keys; page ids of 32 boxes are
-// read at once.
+// The copying warp: tiles ti .. to - 1 of one KV head's keys and values; `it` counts the CTA's tiles. A lane has a box of keys; page ids of 32 boxes are read at once
+// (`ids`: those of the first, read by sp_first_ids).
 template <int HD, int STAGES>
-__device__ __forceinline__ void sp_copy(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, const CUtensorMap* map_k, const CUtensorMap* map_v, int kvh, int it,
-                                        uint8_t* tiles_at, uint64_t* full, uint64_t* empty, int lane) {
+__device__ __forceinline__ void sp_copy(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, const CUtensorMap* map_k, const CUtensorMap* map_v, int kvh, int ti, int to, int& it,
+                                        int& ids, uint8_t* tiles_at, uint64_t* full, uint64_t* empty, int lane) {
     constexpr int PARTS = HD / 64, PART = SP_TT * 128;
     const int boxes = SP_TT / p.box_rows, ahead = 32 / boxes, bt = a.r.block_tokens;
-    int ids = 0;
-    for (int ti = 0; ti < w.n_tiles; ti++, it++) {
+    for (; ti < to; ti++, it++) {
         const int st = it % STAGES, t0 = w.q0 + ti * SP_TT, n_box = min(boxes, (w.q1 - t0 + p.box_rows - 1) / p.box_rows), j = t0 + lane * p.box_rows;
-        if (ti % ahead == 0) ids = j < w.q1 ? w.table[j / bt] : 0;
+        if (ti && ti % ahead == 0) ids = j < w.q1 ? w.table[j / bt] : 0;
         const int id = __shfl_sync(0xffffffffu, ids, ti % ahead * boxes + lane % boxes);
         const int row = (int)(((long)min(max(id, 0), (int)a.r.n_pages - 1) * a.n_kv + kvh) * bt + j % bt);
         if (it >= STAGES) mbar_wait_warp(&empty[st], (it / STAGES - 1) & 1, sp_error, 0xa0001u, (unsigned)it);
@@ -133,6 +134,11 @@ __device__ __forceinline__ void sp_copy(const SharedPrefixArgs& a, const SpPlan&
             }
         __syncwarp();
     }
+}
+// this lane's page of the first 32 boxes from key q0 on (whatever the table holds behind the last token: it is not followed)
+__device__ __forceinline__ int sp_first_ids(const SharedPrefixArgs& a, const SpPlan& p, const int* table, int q0, int most, int lane) {
+    const long j = q0 + (long)lane * p.box_rows;
+    return j < most ? table[j / a.r.block_tokens] : 0;
 }
 
 // Take over the work of a CTA of this grid that has not started: asked for by one thread, the answer (16 bytes) arrives on a barrier. After a refusal nothing more may be
@@ -349,23 +355,31 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
 
     if (warp == SP_WARPS) {
         SpWork v = w;
-        int v_kvh = kvh;
-        for (int it = 0, n = 0, asked = 0;;) {
+        int v_kvh = kvh, ids = sp_first_ids(a, p, v.table, v.q0, v.q1, lane);
+        for (int it = 0, n = 0, asked = 0;; n++) {
             if (p.steal && lane == 0) sp_ask_work(answer, &answered);
-            sp_copy<HD, STAGES>(a, p, v, &map_k, &map_v, v_kvh, it, tiles_at, full, empty, lane);
-            it += v.n_tiles;
-            bool more = false;
-            while (p.steal) {                                    // (work without rows is passed over)
-                int x, y, z;
+            // ahead of the last tile: which work is next, and what it is known from is asked for, to be here when the tile is on its way
+            const int first = max(v.n_tiles - 1, min(1, v.n_tiles));
+            sp_copy<HD, STAGES>(a, p, v, &map_k, &map_v, v_kvh, 0, first, it, ids, tiles_at, full, empty, lane);
+            int x = 0, y = 0, z = 0, next_ids = 0;
+            SpWork::Read read = {0, 0, 0};
+            auto take = [&]() {
                 mbar_wait_warp(&answered, asked++ & 1, sp_error, 0xa0004u, (unsigned)n);
-                more = sp_answered_work(answer, x, y, z) && x == 0 && y < (int)gridDim.y && z < (int)gridDim.z;      // (a wait that ran out leaves anything)
-                if (!more) break;
-                v = SpWork(a, p, 16, x, 0, z);
-                v_kvh = y;
+                if (!sp_answered_work(answer, x, y, z) || x || y >= (int)gridDim.y || z >= (int)gridDim.z) return false;      // (a wait that ran out leaves anything)
+                read = SpWork::read(a, z);
+                next_ids = sp_first_ids(a, p, SpWork::table_of(a, z), 0, a.r.max_pages * a.r.block_tokens, lane);
+                return true;
+            };
+            bool more = p.steal && take();
+            sp_copy<HD, STAGES>(a, p, v, &map_k, &map_v, v_kvh, first, v.n_tiles, it, ids, tiles_at, full, empty, lane);
+            while (more) {                                       // (work without rows is passed over)
+                v = SpWork(a, p, 16, 0, 0, z, read);
                 if (v.n_f > 0) break;
                 __syncwarp();
                 if (lane == 0) { fence_proxy_async(); sp_ask_work(answer, &answered); }
+                more = take();
             }
+            v_kvh = y; ids = next_ids;
             // (work n + 1's place, and the queries of work n - 1, are free again)
             if (n >= 1) mbar_wait_warp(&next_empty[n & 1], ((n - 1) >> 1) & 1, sp_error, 0xa0005u, (unsigned)n);
             if (more) sp_stage_q<E, HD>(a, v, v_kvh, q_s + ((n + 1) & 1) * p.mrows * (HD + 8), lane, 32);
@@ -376,7 +390,6 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
                 mbar_arrive(&next_full[n & 1]);
                 fence_proxy_async();                             // (the answer has been read, the next may replace it)
             }
-            n++;
             if (!more) break;
         }
     } else {
@@ -557,7 +570,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const
     __syncthreads();
 
     if (warp == SP_WARPS) {
-        sp_copy<HD, STAGES>(a, p, w, &map_k, &map_v, kvh, 0, tiles_at, full, empty, lane);
+        int it = 0, ids = sp_first_ids(a, p, w.table, w.q0, w.q1, lane);
+        sp_copy<HD, STAGES>(a, p, w, &map_k, &map_v, kvh, 0, w.n_tiles, it, ids, tiles_at, full, empty, lane);
     } else {
         const int row0 = 16 * warp + g;
         const bool idle = 16 * warp >= w.n_f;                    // this warp has no rows
@@ -679,60 +693,57 @@ __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const
     if (w.own_pass && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
 }
 
-// The partial results of the prefix pass on tensor memory and of the pass over the own tokens, joined: a CTA a row of the batch, a thread four dims of a head.
-constexpr int SP_JOIN = 256;
+// The partial results of the prefix pass on tensor memory and of the pass over the own tokens, joined: a thread four dims of a row and head, all of whose reads
+// are under way at once (up to eight results; four CTAs' worth of one row in one CTA, three results at a time, took 12 us).
+constexpr int SP_JOIN = 128;
 template <typename E, int HD>
 __global__ void __launch_bounds__(SP_JOIN) shared_prefix_join_kernel(const SharedPrefixArgs a, const SpPlan p) {
     __shared__ int live;
-    const int t = blockIdx.x, G = a.n_head / a.n_kv;
+    constexpr int B = 8;
+    const int per_row = (a.n_head * (HD / 4) + SP_JOIN - 1) / SP_JOIN, t = blockIdx.x / per_row, e = blockIdx.x % per_row * SP_JOIN + threadIdx.x;
+    const int G = a.n_head / a.n_kv, head = e / (HD / 4), d = e % (HD / 4) * 4, kvh = head / G;
+    const bool in = head < a.n_head;
+    const int slots = in ? p.cut.slots(kvh * p.cut.pairs + (t * G + head - kvh * G) / 256) : 0;
+    const size_t at = sp_part(a, 0, t, head), step = (size_t)a.r.n_rows * a.n_head;
+    const float* ml = a.work + p.ml_at + at * 2;
+    const float* from = a.work + at * HD + d;
+    // rows that no sequence has, or that are past a sequence's max_rows, have no result
+    if (!a.tab && threadIdx.x < 32) {
+        const int s = seq_of_row(a.r.row_start, a.r.n_seqs, t, threadIdx.x);
+        if (threadIdx.x == 0) live = s < a.r.n_seqs && t >= a.r.row_start[0] && t - max(0, a.r.row_start[s]) < a.max_rows;
+    }
     griddep_wait();
     griddep_launch();
-    // rows that no sequence has, or that are past a sequence's max_rows, have no result
-    if (!a.tab) {
-        if (threadIdx.x < 32) {
-            const int s = seq_of_row(a.r.row_start, a.r.n_seqs, t, threadIdx.x);
-            if (threadIdx.x == 0) live = s < a.r.n_seqs && t >= a.r.row_start[0] && t - max(0, a.r.row_start[s]) < a.max_rows;
+    float m = -INFINITY, l = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = 0; j0 <= slots; j0 += B) {                     // (number `slots`: the own tokens')
+        float2 one[B];
+        float4 v[B];
+#pragma unroll
+        for (int j = 0; j < B; j++) {
+            one[j] = make_float2(-INFINITY, 0.f); v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (j0 + j > slots || !in) continue;
+            const size_t off = (j0 + j < slots ? j0 + j : p.own_slot) * step;
+            one[j] = __ldcg(reinterpret_cast<const float2*>(ml + off * 2));
+            v[j] = __ldcg(reinterpret_cast<const float4*>(from + off * HD));
         }
-        __syncthreads();
-        if (!live) return;
-    }
-    const size_t step = (size_t)a.r.n_rows * a.n_head;
-    for (int e = threadIdx.x; e < a.n_head * (HD / 4); e += SP_JOIN) {
-        const int head = e / (HD / 4), d = e % (HD / 4) * 4, kvh = head / G;
-        const int slots = p.cut.slots(kvh * p.cut.pairs + (t * G + head - kvh * G) / 256);
-        const size_t at = sp_part(a, 0, t, head);
-        const float* ml = a.work + p.ml_at + at * 2;
-        const float* from = a.work + at * HD + d;
-        float m = -INFINITY, l = 0.f;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        constexpr int B = 4;                                     // results under way
-        for (int j0 = 0; j0 <= slots; j0 += B) {                 // (number `slots`: the own tokens')
-            float2 one[B];
-            float4 v[B];
+        float m2 = m;
 #pragma unroll
-            for (int j = 0; j < B; j++) {
-                one[j] = make_float2(-INFINITY, 0.f); v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (j0 + j > slots) continue;
-                const size_t off = (j0 + j < slots ? j0 + j : p.own_slot) * step;
-                one[j] = __ldcg(reinterpret_cast<const float2*>(ml + off * 2));
-                v[j] = __ldcg(reinterpret_cast<const float4*>(from + off * HD));
-            }
-            float m2 = m;
+        for (int j = 0; j < B; j++) m2 = fmaxf(m2, one[j].x);
+        const float ref = m2 == -INFINITY ? 0.f : m2, fall = sp_exp2(m - ref);
+        m = m2; l *= fall; sum.x *= fall; sum.y *= fall; sum.z *= fall; sum.w *= fall;
 #pragma unroll
-            for (int j = 0; j < B; j++) m2 = fmaxf(m2, one[j].x);
-            const float ref = m2 == -INFINITY ? 0.f : m2, fall = sp_exp2(m - ref);
-            m = m2; l *= fall; sum.x *= fall; sum.y *= fall; sum.z *= fall; sum.w *= fall;
-#pragma unroll
-            for (int j = 0; j < B; j++) {
-                const float c = sp_exp2(one[j].x - ref);
-                l = fmaf(c, one[j].y, l);
-                sum.x = fmaf(c, v[j].x, sum.x); sum.y = fmaf(c, v[j].y, sum.y); sum.z = fmaf(c, v[j].z, sum.z); sum.w = fmaf(c, v[j].w, sum.w);
-            }
+        for (int j = 0; j < B; j++) {
+            const float c = sp_exp2(one[j].x - ref);
+            l = fmaf(c, one[j].y, l);
+            sum.x = fmaf(c, v[j].x, sum.x); sum.y = fmaf(c, v[j].y, sum.y); sum.z = fmaf(c, v[j].z, sum.z); sum.w = fmaf(c, v[j].w, sum.w);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;              // (0: no keys. A NaN stays one.)
-        sp_store_out<E, HD>(a, t, head, d, sum.x * inv, sum.y * inv);
-        sp_store_out<E, HD>(a, t, head, d + 2, sum.z * inv, sum.w * inv);
     }
+    __syncthreads();
+    if (!in || (!a.tab && !live)) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;                  // (0: no keys. A NaN stays one.)
+    sp_store_out<E, HD>(a, t, head, d, sum.x * inv, sum.y * inv);
+    sp_store_out<E, HD>(a, t, head, d + 2, sum.z * inv, sum.w * inv);
 }
 
 // ---------------------------------------------------------------- host side
@@ -768,7 +779,7 @@ cudaError_t sp_rows(const SharedPrefixArgs& a, SpPlan p, bool single, dim3 grid,
 template <typename E, int HD>
 cudaError_t sp_join(const SharedPrefixArgs& a, const SpPlan& p, cudaStream_t s) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(a.r.n_rows); cfg.blockDim = dim3(SP_JOIN); cfg.stream = s;
+    cfg.gridDim = dim3((unsigned)((a.n_head * (HD / 4) + SP_JOIN - 1) / SP_JOIN * a.r.n_rows)); cfg.blockDim = dim3(SP_JOIN); cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -791,6 +802,8 @@ constexpr int SP_PREFIX_ROWS = 64;          // up to so many rows a KV head the 
 constexpr int SP_PREFIX_SPLITS = 32;
 }  // namespace
 
+// Runs of equal length over all units laid end to end, or over every unit by itself where that makes them no more than three blocks longer: a run that goes on
+// into another unit loads queries, starts and ends its pipeline and writes its results twice, which takes as long as three blocks (6 us).
 PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix) {
     PrefixCut c = {};
     c.pairs = (int)((n_rows * (n_head / n_kv) + 255) / 256);
@@ -798,7 +811,10 @@ PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix) {
     c.blocks = (n_prefix + 127) / 128;
     const long total = (long)c.units * c.blocks;
     c.run = (int)((total + SP_SMS - 1) / SP_SMS);
-    c.ctas = c.run ? (int)((total + c.run - 1) / c.run) : 0;
+    const int parts = c.units <= SP_SMS ? SP_SMS / c.units : 1, each = (c.blocks + parts - 1) / parts;
+    c.per_unit = c.run && c.units <= SP_SMS && each <= c.run + 3;
+    if (c.per_unit) c.run = each;
+    c.ctas = c.run == 0 ? 0 : c.per_unit ? c.units * ((c.blocks + each - 1) / each) : (int)((total + c.run - 1) / c.run);
     return c;
 }
 

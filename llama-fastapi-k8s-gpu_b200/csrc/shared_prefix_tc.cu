@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
     griddep_launch();
     const uint32_t s_at = __shfl_sync(0xffffffffu, tmem_at, 0), o_at = s_at + 256;      // (known to be uniform)
     const int G = a.n_head / a.n_kv, M = a.r.n_rows * G, n_prefix = a.n_prefix;
-    const int x0 = blockIdx.x * cut.run, x1 = min(cut.units * cut.blocks, x0 + cut.run);
+    const int x0 = cut.begin(blockIdx.x), x1 = cut.end(blockIdx.x);
 
     // runs of blocks of one unit: every role walks them the same way
     struct Segment { int kvh, row0, b0, n; bool two; };
