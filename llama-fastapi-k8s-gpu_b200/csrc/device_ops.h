@@ -104,7 +104,7 @@ struct PrefixCut {
     }
 };
 PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix);
-cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, cudaStream_t s);
+cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, cudaStream_t s);      // ml_at: see SpPlan
 
 // code of the first wait of these kernels that ran out on the current device (0: none); waits for the device
 cudaError_t shared_prefix_error(unsigned int* code);

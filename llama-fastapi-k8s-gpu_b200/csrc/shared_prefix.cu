@@ -14,6 +14,7 @@
 #include "tensor_map.h"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <algorithm>
 #include <limits.h>
 #include <math.h>
 
@@ -62,23 +63,25 @@ __device__ __forceinline__ float sp_cluster_load(uint32_t address) {
 }  // namespace
 
 struct SpPlan {
-    int prefix;                  // 1: the prefix for all rows, partial results; 0: a sequence's own tokens, behind the prefix's results
-    int splits;                  // CTAs that share the keys of a tile of rows (a cluster, except for the prefix)
-    int steal;                   // single-token form without splits: a CTA goes on with the work of CTAs that have not started
-    int fixed_slots;             // partial results of the prefix per row that this pass joins (0: none; < 0: as `cut` says)
-    int own_slot;                // >= 0: beside the prefix pass on tensor memory: its results are partial ones too, in this slot, and a third kernel joins
+    int prefix_z;                // blockIdx.z that is the prefix for all rows (-1: none); the others are sequences
+    int prefix_splits, splits;   // CTAs that share the keys of a tile of rows, of the prefix and of a sequence's own tokens
+    int own_slot;                // >= 0: there is a prefix, and the own tokens' results are partial ones too, in slots from here on; -1: they are the output, and
+                                 //   the CTAs that share a tile are a cluster
+    int behind;                  // launched behind the prefix pass, which it runs beside
+    int steal;                   // a CTA goes on with the work of CTAs that have not started (single-token form without clusters)
     int mrows;                   // rows of a tile that q is staged for (single-token form)
     int box_rows;                // keys of a copy: a page, or a power of two that divides it
+    int slots;                   // joining: partial results of the prefix per row (< 0: as `cut` says)
     PrefixCut cut;
     size_t ml_at;                // where the (maximum, sum) of the partial results lie in the workspace
 };
 
-// partial results of the prefix: [slot][row][head][head_dim] weighted sums, then [slot][row][head][2] (maximum in log2, sum)
+// partial results: [slot][row][head][head_dim] weighted sums, then [slot][row][head][2] (maximum in log2, sum)
 __device__ __forceinline__ size_t sp_part(const SharedPrefixArgs& a, int slot, int row, int head) { return ((size_t)slot * a.r.n_rows + row) * a.n_head + head; }
 
 // the rows and keys that a CTA works on
 struct SpWork {
-    int r0, n_tok, own;          // first row of the sequence, its rows, its own tokens (prefix pass: 0, all rows, the prefix's tokens)
+    int split, r0, n_tok, own;   // its number among the CTAs that share the tile's keys; first row of the sequence, its rows, its own tokens (prefix pass: 0, all rows, the prefix's tokens)
     const int* table;
     int f0, n_f;                 // rows (token, head) of the tile, numbered within the sequence
     int G, lim_lo, lim_hi, q0, q1, n_tiles;      // keys that the tile's first and last rows see; this CTA's share of them; its tiles of keys
@@ -95,9 +98,11 @@ struct SpWork {
     static __device__ __forceinline__ const int* table_of(const SharedPrefixArgs& a, int z) {
         return a.tab ? a.tab[a.slots.slot[z]].block_table + a.n_prefix / a.r.block_tokens : a.r.pages + z * a.r.table_stride;
     }
-    __device__ SpWork(const SharedPrefixArgs& a, const SpPlan& p, int mt, int tile, int split, int z) : SpWork(a, p, mt, tile, split, z, p.prefix ? Read{0, 0, 0} : read(a, z)) {}
-    __device__ SpWork(const SharedPrefixArgs& a, const SpPlan& p, int mt, int tile, int split, int z, const Read& r) {
-        G = a.n_head / a.n_kv; own_pass = !p.prefix;
+    __device__ SpWork(const SharedPrefixArgs& a, const SpPlan& p, int mt, int x, int z) : SpWork(a, p, mt, x, z, z == p.prefix_z ? Read{0, 0, 0} : read(a, z)) {}
+    __device__ SpWork(const SharedPrefixArgs& a, const SpPlan& p, int mt, int x, int z, const Read& r) {
+        G = a.n_head / a.n_kv; own_pass = z != p.prefix_z;
+        const int splits = own_pass ? p.splits : p.prefix_splits, tile = x / splits;
+        split = x % splits;
         r0 = 0; n_tok = a.r.n_rows; own = a.n_prefix; table = a.prefix_pages;
         if (own_pass) {
             r0 = max(0, r.b); n_tok = min(r.e, a.r.n_rows) - r0; table = table_of(a, z);
@@ -105,7 +110,7 @@ struct SpWork {
         }
         f0 = tile * mt; n_f = min(mt, (own_pass ? min(n_tok, a.max_rows) : n_tok) * G - f0);
         lim_lo = limit(f0 / G); lim_hi = limit((f0 + max(n_f, 1) - 1) / G);
-        const int chunk = ((lim_hi + p.splits - 1) / p.splits + SP_TT - 1) / SP_TT * SP_TT;
+        const int chunk = ((lim_hi + splits - 1) / splits + SP_TT - 1) / SP_TT * SP_TT;
         q0 = min(lim_hi, split * chunk); q1 = min(lim_hi, q0 + chunk);
         n_tiles = (q1 - q0 + SP_TT - 1) / SP_TT;
     }
@@ -201,46 +206,6 @@ __device__ __forceinline__ void sp_load_q(const SharedPrefixArgs& a, const SpWor
     }
 }
 
-// The prefix's partial results of a row, joined: maximum, sum, and the columns col, col + 1, col + 8, ... of the weighted sum
-template <int HD, int N>
-__device__ __forceinline__ void sp_take_prefix(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, int kvh, int row, int col, float& m, float& l, float (&o)[N][4], int h) {
-    const int f = w.f0 + row, i = f / w.G;
-    const int slots = p.fixed_slots < 0 ? p.cut.slots(kvh * p.cut.pairs + (w.r0 * w.G + f) / 256) : p.fixed_slots;
-    const size_t at = sp_part(a, 0, w.r0 + i, kvh * w.G + f - i * w.G), step = (size_t)a.r.n_rows * a.n_head;
-    const float* ml = a.work + p.ml_at + at * 2;
-    const float* from = a.work + at * HD + col;
-    constexpr int B = N > 8 ? 1 : 4;                             // results under way
-    for (int j0 = 0; j0 < slots; j0 += B) {
-        float2 one[B], v[B][N];
-        float m2 = m;
-#pragma unroll
-        for (int j = 0; j < B; j++) {
-            one[j] = make_float2(-INFINITY, 0.f);
-            if (j0 + j < slots) {
-                one[j] = __ldcg(reinterpret_cast<const float2*>(ml + (j0 + j) * step * 2));
-#pragma unroll
-                for (int nt = 0; nt < N; nt++) v[j][nt] = __ldcg(reinterpret_cast<const float2*>(from + (j0 + j) * step * HD + nt * 8));
-            } else {
-#pragma unroll
-                for (int nt = 0; nt < N; nt++) v[j][nt] = make_float2(0.f, 0.f);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < B; j++) m2 = fmaxf(m2, one[j].x);
-        const float ref = m2 == -INFINITY ? 0.f : m2, fall = sp_exp2(m - ref);
-        m = m2; l *= fall;
-#pragma unroll
-        for (int nt = 0; nt < N; nt++) { o[nt][2 * h] *= fall; o[nt][2 * h + 1] *= fall; }
-#pragma unroll
-        for (int j = 0; j < B; j++) {
-            const float c = sp_exp2(one[j].x - ref);
-            l = fmaf(c, one[j].y, l);
-#pragma unroll
-            for (int nt = 0; nt < N; nt++) { o[nt][2 * h] = fmaf(c, v[j][nt].x, o[nt][2 * h]); o[nt][2 * h + 1] = fmaf(c, v[j][nt].y, o[nt][2 * h + 1]); }
-        }
-    }
-}
-
 // two neighbouring columns of a row's output
 template <typename E, int HD>
 __device__ __forceinline__ void sp_store_out(const SharedPrefixArgs& a, int t, int head, int d, float x, float y) {
@@ -255,13 +220,13 @@ __device__ __forceinline__ void sp_store_out(const SharedPrefixArgs& a, int t, i
     }
 }
 
-// What a thread's columns of a row (numbers col, col + 1, col + 8, ...) come to: partial results (prefix pass), this CTA's share of a cluster's, or output
+// What a thread's columns of a row (numbers col, col + 1, col + 8, ...) come to: partial results, this CTA's share of a cluster's, or output
 template <typename E, int HD, int N>
-__device__ __forceinline__ void sp_finish(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, int kvh, int split, int row, int col, float m, float l, const float (&o)[N][4], int h,
-                                          float* acc, float* row_m, float* row_l) {
+__device__ __forceinline__ void sp_finish(const SharedPrefixArgs& a, const SpPlan& p, const SpWork& w, int kvh, int row, int col, float m, float l, const float (&o)[N][4], int h, float* acc,
+                                          float* row_m, float* row_l) {
     const int f = w.f0 + row, i = f / w.G, head = kvh * w.G + f - i * w.G;
-    if (!w.own_pass || p.own_slot >= 0) {
-        const size_t at = sp_part(a, w.own_pass ? p.own_slot : split, w.r0 + i, head);
+    if (p.own_slot >= 0) {
+        const size_t at = sp_part(a, w.own_pass ? p.own_slot + w.split : w.split, w.r0 + i, head);
 #pragma unroll
         for (int nt = 0; nt < N; nt++) *reinterpret_cast<float2*>(a.work + at * HD + col + nt * 8) = make_float2(o[nt][2 * h], o[nt][2 * h + 1]);
         if (col == 0) *reinterpret_cast<float2*>(a.work + p.ml_at + at * 2) = make_float2(m, l);
@@ -315,12 +280,17 @@ __device__ __forceinline__ bool sp_any_bad(uint8_t* vb, int ks, int c0, int n, i
     return __any_sync(0xffffffffu, bad);
 }
 
+// A pass that is the operator's first kernel waits for what the kernels before it wrote (q, this step's keys); one behind the prefix pass starts beside it, since that
+// has waited, and does not end before it, so that what is behind this pass is behind both. The next kernel may start early, but not to sit on SMs beside
+// a pass that is to run beside the prefix's.
+__device__ __forceinline__ void sp_begin(const SpPlan& p) { if (!p.behind) { griddep_wait(); griddep_launch(); } }
+__device__ __forceinline__ void sp_end(const SpPlan& p) { if (p.behind) { griddep_launch(); griddep_wait(); } }
+
 // Single tokens: a tile of up to 16 rows (the group's heads, a few tokens), the four computing warps share a tile of keys. Scores: a warp has 16 keys; maxima and
 // probabilities go through shared memory; weighted sums: a warp has a quarter of the dims and all 64 keys, so that nothing has to be merged at the end.
 // What a CTA waits for before its first keys are here takes as long as the keys of some 100 tokens (3 us): CTAs that run go on with the work of those that have not
 // started (p.steal), and their copies run ahead into it.
-// Beside the prefix pass on tensor memory (p.own_slot >= 0) nothing waits for that pass before the end.
-// grid: (tile * splits + split, KV head, sequence)
+// grid: (tile * splits + split, KV head, sequence), the prefix's CTAs among them (p.prefix_z) where its rows are as few
 template <typename E, int HD>
 __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedPrefixArgs a,
                                                                            const SpPlan p) {
@@ -343,13 +313,10 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
         mbar_init(&answered, 1);
         fence_mbar_init();
     }
-    // behind another kernel of the engine's chain: what it wrote (q, this step's keys). Behind the prefix pass that is long done.
-    if (p.prefix || (p.fixed_slots == 0 && p.own_slot < 0)) griddep_wait();
-    if (p.own_slot < 0) griddep_launch();
-    const int split = blockIdx.x % p.splits;
+    sp_begin(p);
     int kvh = blockIdx.y;
-    SpWork w(a, p, 16, blockIdx.x / p.splits, split, blockIdx.z);
-    if (w.n_f <= 0 && !p.steal) { griddep_wait(); return; }      // (all CTAs of the cluster, none of which ends before the prefix pass)
+    SpWork w(a, p, 16, blockIdx.x, blockIdx.z);
+    if (w.n_f <= 0 && !p.steal) { sp_end(p); return; }           // (all CTAs of the cluster)
     if (w.n_f <= 0) w.n_tiles = 0;
     __syncthreads();
 
@@ -365,21 +332,23 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
             SpWork::Read read = {0, 0, 0};
             auto take = [&]() {
                 mbar_wait_warp(&answered, asked++ & 1, sp_error, 0xa0004u, (unsigned)n);
-                if (!sp_answered_work(answer, x, y, z) || x || y >= (int)gridDim.y || z >= (int)gridDim.z) return false;      // (a wait that ran out leaves anything)
+                if (!sp_answered_work(answer, x, y, z) || x >= (int)gridDim.x || y >= (int)gridDim.y || z >= (int)gridDim.z) return false;      // (a wait that ran out leaves anything)
+                if (z == p.prefix_z) return true;
                 read = SpWork::read(a, z);
-                next_ids = sp_first_ids(a, p, SpWork::table_of(a, z), 0, a.r.max_pages * a.r.block_tokens, lane);
+                if (p.splits == 1) next_ids = sp_first_ids(a, p, SpWork::table_of(a, z), 0, a.r.max_pages * a.r.block_tokens, lane);
                 return true;
             };
             bool more = p.steal && take();
             sp_copy<HD, STAGES>(a, p, v, &map_k, &map_v, v_kvh, first, v.n_tiles, it, ids, tiles_at, full, empty, lane);
             while (more) {                                       // (work without rows is passed over)
-                v = SpWork(a, p, 16, 0, 0, z, read);
+                v = SpWork(a, p, 16, x, z, read);
                 if (v.n_f > 0) break;
                 __syncwarp();
                 if (lane == 0) { fence_proxy_async(); sp_ask_work(answer, &answered); }
                 more = take();
             }
-            v_kvh = y; ids = next_ids;
+            v_kvh = y;
+            ids = !more || (p.splits == 1 && v.own_pass) ? next_ids : sp_first_ids(a, p, v.table, v.q0, v.q1, lane);
             // (work n + 1's place, and the queries of work n - 1, are free again)
             if (n >= 1) mbar_wait_warp(&next_empty[n & 1], ((n - 1) >> 1) & 1, sp_error, 0xa0005u, (unsigned)n);
             if (more) sp_stage_q<E, HD>(a, v, v_kvh, q_s + ((n + 1) & 1) * p.mrows * (HD + 8), lane, 32);
@@ -420,17 +389,6 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
             float o[NT][4], m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};      // (l: this thread's columns of scores)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) o[nt][0] = o[nt][1] = o[nt][2] = o[nt][3] = 0.f;
-            if (w.own_pass && p.fixed_slots != 0) {
-                if (hh == 0) griddep_wait();
-                if (split == 0) {                                // (the first CTA of a cluster takes the prefix's results)
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        if (g + 8 * h < w.n_f) {
-                            sp_take_prefix<HD, NT>(a, p, w, kvh, g + 8 * h, col, m_run[h], l_run[h], o, h);
-                            if (warp || tq) l_run[h] = 0.f;      // (counted once)
-                        }
-                }
-            }
             for (int ti = 0; ti < w.n_tiles; ti++, it++) {
                 const int st = it % STAGES, buf = it & 1, t0 = w.q0 + ti * SP_TT, valid = min(SP_TT, w.q1 - t0);
                 uint8_t *kb = tiles_at + st * 2 * PARTS * PART, *vb = kb + PARTS * PART;
@@ -537,16 +495,16 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
                 const int row = g + 8 * h;
                 if (row >= w.n_f) continue;
                 const float l = (wsum[hh & 1][0][row] + wsum[hh & 1][1][row]) + (wsum[hh & 1][2][row] + wsum[hh & 1][3][row]);
-                sp_finish<E, HD, NT>(a, p, w, kvh, split, row, col, m_run[h], l, o, h, acc, row_m, row_l);
+                sp_finish<E, HD, NT>(a, p, w, kvh, row, col, m_run[h], l, o, h, acc, row_m, row_l);
             }
         }
     }
-    if (w.own_pass && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
-    if (p.own_slot >= 0) { griddep_launch(); griddep_wait(); }   // (a kernel behind this one is behind the prefix pass too)
+    if (p.own_slot < 0 && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
+    sp_end(p);
 }
 
 // Several tokens of a sequence, or the prefix pass of up to 64 rows: a tile of 64 rows, a warp has 16 of them and all keys.
-// grid: (tile * splits + split, KV head, sequence)
+// grid: (tile * splits + split, KV head, sequence, or prefix)
 template <typename E, int HD>
 __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedPrefixArgs a,
                                                                            const SpPlan p) {
@@ -562,11 +520,10 @@ __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const
         for (int i = 0; i < STAGES; i++) { mbar_init(&full[i], 1); mbar_init(&empty[i], SP_WARPS); }
         fence_mbar_init();
     }
-    if (p.prefix || p.fixed_slots == 0) griddep_wait();
-    griddep_launch();
-    const int split = blockIdx.x % p.splits, kvh = blockIdx.y;
-    const SpWork w(a, p, MT, blockIdx.x / p.splits, split, blockIdx.z);
-    if (w.n_f <= 0) { griddep_wait(); return; }
+    sp_begin(p);
+    const int kvh = blockIdx.y;
+    const SpWork w(a, p, MT, blockIdx.x, blockIdx.z);
+    if (w.n_f <= 0) { sp_end(p); return; }
     __syncthreads();
 
     if (warp == SP_WARPS) {
@@ -585,17 +542,6 @@ __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const
         for (int h = 0; h < 2; h++) {
             const bool in = row0 + 8 * h < w.n_f;
             lim[h] = in ? min(w.q1, w.limit((w.f0 + row0 + 8 * h) / w.G)) : w.q1;
-        }
-        if (w.own_pass && p.fixed_slots != 0) {
-            griddep_wait();
-            if (split == 0) {
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-                    if (row0 + 8 * h < w.n_f) {
-                        sp_take_prefix<HD, NT>(a, p, w, kvh, row0 + 8 * h, 2 * tq, m_run[h], l_run[h], o, h);
-                        if (tq) l_run[h] = 0.f;                  // (counted once)
-                    }
-            }
         }
         for (int ti = 0; ti < w.n_tiles; ti++) {
             const int st = ti % STAGES, t0 = w.q0 + ti * SP_TT, valid = min(SP_TT, w.q1 - t0);
@@ -687,13 +633,14 @@ __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const
         for (int h = 0; h < 2; h++) {
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 1);
             l_run[h] += __shfl_xor_sync(0xffffffffu, l_run[h], 2);
-            if (row0 + 8 * h < w.n_f) sp_finish<E, HD, NT>(a, p, w, kvh, split, row0 + 8 * h, 2 * tq, m_run[h], l_run[h], o, h, acc, row_m, row_l);
+            if (row0 + 8 * h < w.n_f) sp_finish<E, HD, NT>(a, p, w, kvh, row0 + 8 * h, 2 * tq, m_run[h], l_run[h], o, h, acc, row_m, row_l);
         }
     }
-    if (w.own_pass && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
+    if (p.own_slot < 0 && p.splits > 1) sp_join_cluster<E, HD>(a, p, w, kvh, acc, row_m, row_l);
+    sp_end(p);
 }
 
-// The partial results of the prefix pass on tensor memory and of the pass over the own tokens, joined: a thread four dims of a row and head, all of whose reads
+// The partial results of the prefix and of the own tokens, joined: a thread four dims of a row and head, all of whose reads
 // are under way at once (up to eight results; four CTAs' worth of one row in one CTA, three results at a time, took 12 us).
 constexpr int SP_JOIN = 128;
 template <typename E, int HD>
@@ -703,7 +650,7 @@ __global__ void __launch_bounds__(SP_JOIN) shared_prefix_join_kernel(const Share
     const int per_row = (a.n_head * (HD / 4) + SP_JOIN - 1) / SP_JOIN, t = blockIdx.x / per_row, e = blockIdx.x % per_row * SP_JOIN + threadIdx.x;
     const int G = a.n_head / a.n_kv, head = e / (HD / 4), d = e % (HD / 4) * 4, kvh = head / G;
     const bool in = head < a.n_head;
-    const int slots = in ? p.cut.slots(kvh * p.cut.pairs + (t * G + head - kvh * G) / 256) : 0;
+    const int slots = !in ? 0 : p.slots >= 0 ? p.slots : p.cut.slots(kvh * p.cut.pairs + (t * G + head - kvh * G) / 256), all = slots + p.splits;
     const size_t at = sp_part(a, 0, t, head), step = (size_t)a.r.n_rows * a.n_head;
     const float* ml = a.work + p.ml_at + at * 2;
     const float* from = a.work + at * HD + d;
@@ -716,14 +663,14 @@ __global__ void __launch_bounds__(SP_JOIN) shared_prefix_join_kernel(const Share
     griddep_launch();
     float m = -INFINITY, l = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = 0; j0 <= slots; j0 += B) {                     // (number `slots`: the own tokens')
+    for (int j0 = 0; j0 < all; j0 += B) {                        // (behind the prefix's: the own tokens')
         float2 one[B];
         float4 v[B];
 #pragma unroll
         for (int j = 0; j < B; j++) {
             one[j] = make_float2(-INFINITY, 0.f); v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (j0 + j > slots || !in) continue;
-            const size_t off = (j0 + j < slots ? j0 + j : p.own_slot) * step;
+            if (j0 + j >= all || !in) continue;
+            const size_t off = (j0 + j < slots ? j0 + j : p.own_slot + j0 + j - slots) * step;
             one[j] = __ldcg(reinterpret_cast<const float2*>(ml + off * 2));
             v[j] = __ldcg(reinterpret_cast<const float4*>(from + off * HD));
         }
@@ -763,7 +710,7 @@ cudaError_t sp_rows(const SharedPrefixArgs& a, SpPlan p, bool single, dim3 grid,
     cfg.gridDim = grid; cfg.blockDim = dim3(SP_THREADS); cfg.dynamicSmemBytes = sp_smem(HD, single ? p.mrows : 0); cfg.stream = s;
     cudaLaunchAttribute at[2];
     int n = 0;
-    if (!p.prefix && p.splits > 1) {
+    if (p.own_slot < 0 && p.splits > 1) {
         at[n].id = cudaLaunchAttributeClusterDimension;
         at[n].val.clusterDim.x = p.splits; at[n].val.clusterDim.y = 1; at[n].val.clusterDim.z = 1;
         n++;
@@ -798,8 +745,8 @@ int sp_splits(long tiles, long keys, int most) {
     while (2 * n <= most && tiles * n * 2 <= 2 * SP_SMS && keys / (2 * n) >= SP_TT) n *= 2;
     return n;
 }
-constexpr int SP_PREFIX_ROWS = 64;          // up to so many rows a KV head the prefix pass is the kernel above
-constexpr int SP_PREFIX_SPLITS = 32;
+constexpr int SP_PREFIX_ROWS = 64;          // up to so many rows a KV head the prefix is read by the kernels above
+constexpr int SP_PREFIX_SPLITS = 32, SP_OWN_SPLITS = 8;
 }  // namespace
 
 // Runs of equal length over all units laid end to end, or over every unit by itself where that makes them no more than three blocks longer: a run that goes on
@@ -818,14 +765,18 @@ PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix) {
     return c;
 }
 
-// most partial results a row can have: a unit of b blocks in runs of ceil(u b / 148) lies in at most ceil(148 / u) + 1 of them
-static long sp_most_slots(long n_rows, int n_head, int n_kv) {
+// most partial results that a row's prefix can have: a unit of b blocks in runs of ceil(u b / 148) lies in at most ceil(148 / u) + 1 of them
+static long sp_prefix_slots(long n_rows, int n_head, int n_kv) {
     if (n_rows * (n_head / n_kv) <= SP_PREFIX_ROWS) return SP_PREFIX_SPLITS;
     const PrefixCut c = prefix_cut(n_rows, n_head, n_kv, 1);
-    return (SP_SMS + c.units - 1) / c.units + 2;                  // (and the own tokens')
+    return (SP_SMS + c.units - 1) / c.units + 1;
+}
+// and its own tokens: the splits of the fewest CTAs that so many rows can be
+static long sp_own_slots(long n_rows, int n_head, int n_kv) {
+    return sp_splits((n_rows * (n_head / n_kv) + 63) / 64 * n_kv, LONG_MAX, SP_OWN_SPLITS);
 }
 size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim) {
-    return (size_t)sp_most_slots(n_rows, n_head, n_kv) * n_rows * n_head * (head_dim + 2);
+    return (size_t)(sp_prefix_slots(n_rows, n_head, n_kv) + sp_own_slots(n_rows, n_head, n_kv)) * n_rows * n_head * (head_dim + 2);
 }
 
 cudaError_t shared_prefix_error(unsigned int* code) {
@@ -838,37 +789,44 @@ cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s) {
     if (R == 0 || S == 0) return cudaSuccess;
     if ((long)prefix_cut(R, a.n_head, a.n_kv, 1).units * ((a.n_prefix + 127) / 128) > INT_MAX / 2) return cudaErrorInvalidValue;
     cudaError_t e;
+    const bool few = (long)R * G <= SP_PREFIX_ROWS, single = a.max_rows * G <= 16, h = a.type == ELEM_F16;
+    const int mt = single ? 16 : 64, tiles = (a.max_rows * G + mt - 1) / mt;
     SpPlan own = {};
-    bool behind = false;
-    if (a.n_prefix > 0) {
-        if ((long)R * G <= SP_PREFIX_ROWS) {
-            SpPlan p = {};
-            p.prefix = 1;
-            p.mrows = R * G; p.own_slot = -1;
-            p.splits = own.fixed_slots = sp_splits((long)a.n_kv, a.n_prefix, SP_PREFIX_SPLITS);
-            p.ml_at = own.ml_at = (size_t)p.splits * R * a.n_head * a.head_dim;
-            e = sp_rows_of(a, p, R * G <= 16, dim3(p.splits, a.n_kv, 1), s, g_chain_pdl);
+    own.prefix_z = own.own_slot = -1;
+    own.splits = sp_splits((long)tiles * a.n_kv * S, (long)a.r.max_pages * a.r.block_tokens, SP_OWN_SPLITS);
+    own.mrows = single ? a.max_rows * G : 0;
+    if (a.n_prefix == 0) {
+        own.steal = single && own.splits == 1;
+        return sp_rows_of(a, own, single, dim3(tiles * own.splits, a.n_kv, S), s, g_chain_pdl);
+    }
+    const long slots = sp_prefix_slots(R, a.n_head, a.n_kv);
+    own.own_slot = (int)slots;
+    own.ml_at = (size_t)(slots + sp_own_slots(R, a.n_head, a.n_kv)) * R * a.n_head * a.head_dim;
+    own.splits = std::min(own.splits, (int)sp_own_slots(R, a.n_head, a.n_kv));      // (fewer sequences than their rows need: max_rows was too small)
+    own.steal = single;
+    if (few) own.slots = own.prefix_splits = sp_splits((long)a.n_kv, a.n_prefix, SP_PREFIX_SPLITS);
+    if (few && single && R * G <= 16) {
+        // the prefix and the own tokens in one launch
+        own.prefix_z = S;
+        own.mrows = R * G;
+        own.steal = 0;
+        e = sp_rows_of(a, own, true, dim3(std::max(own.prefix_splits, own.splits), a.n_kv, S + 1), s, g_chain_pdl);
+    } else {
+        if (few) {
+            SpPlan p = own;
+            p.prefix_z = 0;
+            p.steal = 0;
+            e = sp_rows_of(a, p, false, dim3(p.prefix_splits, a.n_kv, 1), s, g_chain_pdl);
         } else {
             own.cut = prefix_cut(R, a.n_head, a.n_kv, a.n_prefix);
-            own.fixed_slots = -1;
-            own.ml_at = (size_t)sp_most_slots(R, a.n_head, a.n_kv) * R * a.n_head * a.head_dim;
-            e = shared_prefix_tc_launch(a, own.cut, s);
+            own.slots = -1;
+            e = shared_prefix_tc_launch(a, own.cut, own.ml_at, s);
         }
         if (e != cudaSuccess) return e;
-        behind = true;
+        own.behind = 1;
+        e = sp_rows_of(a, own, single, dim3(tiles * own.splits, a.n_kv, S), s, true);
     }
-    const bool single = a.max_rows * G <= 16;
-    const int mt = single ? 16 : 64, tiles = (a.max_rows * G + mt - 1) / mt;
-    own.splits = sp_splits((long)tiles * a.n_kv * S, (long)a.r.max_pages * a.r.block_tokens, 8);
-    own.steal = single && own.splits == 1;
-    own.mrows = single ? a.max_rows * G : 0;
-    own.own_slot = -1;
-    // single tokens run beside the pass on tensor memory, whose CTAs leave them room, and are joined with it afterwards
-    const bool beside = own.fixed_slots < 0 && own.steal;
-    if (beside) { own.own_slot = (int)sp_most_slots(R, a.n_head, a.n_kv) - 1; own.fixed_slots = 0; }
-    const cudaError_t e2 = sp_rows_of(a, own, single, dim3(tiles * own.splits, a.n_kv, S), s, behind || g_chain_pdl);
-    if (e2 != cudaSuccess || !beside) return e2;
-    const bool h = a.type == ELEM_F16;
+    if (e != cudaSuccess) return e;
     if (a.head_dim == 64) return h ? sp_join<__half, 64>(a, own, s) : sp_join<__nv_bfloat16, 64>(a, own, s);
     return h ? sp_join<__half, 128>(a, own, s) : sp_join<__nv_bfloat16, 128>(a, own, s);
 }

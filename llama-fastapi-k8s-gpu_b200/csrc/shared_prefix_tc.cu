@@ -331,8 +331,7 @@ static cudaError_t st_launch(const SharedPrefixArgs& a, const PrefixCut& cut, si
     return launch_chain(shared_prefix_tc_kernel<HD, F16>, dim3(cut.ctas), dim3(ST_THREADS), smem, s, mk, mv, a, cut, box, ml_at);
 }
 
-cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, cudaStream_t s) {
-    const size_t ml_at = shared_prefix_work_floats(a.r.n_rows, a.n_head, a.n_kv, a.head_dim) / (a.head_dim + 2) * a.head_dim;
+cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, cudaStream_t s) {
     if (a.r.block_tokens % 16 || cut.ctas < 1) return cudaErrorInvalidValue;
     if (a.head_dim == 64) return a.type == ELEM_F16 ? st_launch<64, true>(a, cut, ml_at, s) : st_launch<64, false>(a, cut, ml_at, s);
     if (a.head_dim == 128) return a.type == ELEM_F16 ? st_launch<128, true>(a, cut, ml_at, s) : st_launch<128, false>(a, cut, ml_at, s);
