@@ -5,9 +5,9 @@
 // the cluster. A masked entry (-infinity) adds nothing; a row of nothing else gets log probabilities of -infinity and entropy 0; a NaN makes the row's
 // numbers NaN.
 //
-// The most likely tokens come from the same pass: a thread's running maximum bounds its entries. Entries above the n-th largest of the threads' maxima can
-// only lie with the threads whose maximum reaches it, n of them unless some are equal; their entries are read once more (from L2) and the few that reach the
-// bound are ranked by (value, lower id). Rows that would give too many of those (hundreds of equal entries) are searched n times instead.
+// The most likely tokens come from the same pass: a thread's running maximum bounds its entries. Of the maxima of 32 or 64 groups of threads the n-th largest is
+// reached by n entries at least, so that the n most likely are among the entries that reach it, which lie with the few threads whose maximum does; their entries
+// are read once more (from L2) and ranked by (value, lower id). Rows that would give too many of those (hundreds of equal entries) are searched n times instead.
 //
 // Bound by memory for many rows (each logit read once), by the latency of the phases behind the pass for few.
 #include "device_ops.h"
@@ -19,7 +19,7 @@ namespace b2 {
 
 namespace {
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_UNROLL = 4;              // 16-byte pieces a thread has under way
+constexpr int LP_UNROLL = 2;              // 16-byte pieces a thread has under way (four, and five CTAs an SM: 1024 rows of 128256 110 instead of 92 us)
 constexpr int LP_CAND = 1024;             // entries that may be ranked
 constexpr int LP_SEL = 128;               // threads whose entries are read again
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
@@ -64,29 +64,30 @@ struct Pieces {
     }
     __device__ int first(int p) const { return base + p * VEC; }
     // entries outside come out as -infinity (they add nothing and are never ranked: see id_ok)
-    __device__ void load(int p, float (&x)[VEC]) const {
+    __device__ uint4 load(int p) const {
         const int i0 = first(p);
-        if (p < n && i0 >= begin && i0 + VEC <= end) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4*>(row + i0));
-            const T* v = reinterpret_cast<const T*>(&raw);
+        if (p < n && i0 >= begin && i0 + VEC <= end) return __ldg(reinterpret_cast<const uint4*>(row + i0));
+        uint4 raw;
+        T* v = reinterpret_cast<T*>(&raw);
 #pragma unroll
-            for (int e = 0; e < VEC; e++) x[e] = lp_float(v[e]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < VEC; e++) x[e] = p < n && i0 + e >= begin && i0 + e < end ? lp_float(row[i0 + e]) : -INFINITY;
-        }
+        for (int e = 0; e < VEC; e++) v[e] = p < n && i0 + e >= begin && i0 + e < end ? row[i0 + e] : (T)(-INFINITY);
+        return raw;
     }
+    static __device__ __forceinline__ float at(const uint4& raw, int e) { return lp_float(reinterpret_cast<const T*>(&raw)[e]); }
     __device__ bool id_ok(int id) const { return id >= begin && id < end; }
 };
 
 struct LpShared {
     Sums sums[LP_WARPS], cta;
-    unsigned tmax[LP_THREADS];
-    unsigned bound;
+    unsigned group[64], bound;
     int n_sel, n_cand, n_own, sel[LP_SEL];
     unsigned long long cand[LP_CAND], own[LOGPROB_MAX_TOP], wbest[LP_WARPS];
 };
 
+__device__ __forceinline__ float lp_value(unsigned long long key) {      // of the entry that a rank key was made of (-0 comes back as 0)
+    const unsigned k = (unsigned)(key >> 32);
+    return k == 0 ? __int_as_float(0x7fffffff) : __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
 __device__ __forceinline__ unsigned long long lp_rank_key(float x, int id) { return ((unsigned long long)lp_key(x) << 32) | (unsigned)~id; }
 
 // ranks n keys (all different) in `keys`, the first `want` go to `put(rank, key)`
@@ -109,7 +110,7 @@ __device__ __forceinline__ uint32_t lp_cluster_rank() { uint32_t r; asm("mov.u32
 
 // cluster of `parts` CTAs a row (1: none)
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs a, int parts) {
+__global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobArgs a, int parts) {
     constexpr int VEC = 16 / sizeof(T);
     __shared__ LpShared sh;
     __shared__ unsigned long long all[8 * LOGPROB_MAX_TOP];
@@ -121,17 +122,22 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
     const int top = min(a.n_top, pc.end - pc.begin);              // of this CTA's entries
     if (tid == 0) { sh.n_sel = sh.n_cand = sh.n_own = 0; }
 
+    // (the asked token's logit, read ahead by the thread that will want it)
+    const int token = part == 0 && tid == 0 && a.logprob ? a.tokens[r] : -1;
+    const bool has_token = token >= 0 && token < a.n_vocab;
+    const float token_logit = has_token ? lp_float(row[token]) : 0.f;
+
     // ---- the pass
     Sums v = {-INFINITY, 0.f, 0.f};
     for (int p0 = tid; p0 < pc.n; p0 += LP_UNROLL * LP_THREADS) {
-        float x[LP_UNROLL][VEC];
+        uint4 x[LP_UNROLL];
 #pragma unroll
-        for (int u = 0; u < LP_UNROLL; u++) pc.load(p0 + u * LP_THREADS, x[u]);
+        for (int u = 0; u < LP_UNROLL; u++) x[u] = pc.load(p0 + u * LP_THREADS);
         float m = v.m;
 #pragma unroll
         for (int u = 0; u < LP_UNROLL; u++)
 #pragma unroll
-            for (int e = 0; e < VEC; e++) m = fmaxf(m, x[u][e]);
+            for (int e = 0; e < VEC; e++) m = fmaxf(m, pc.at(x[u], e));
         const float ref = m == -INFINITY ? 0.f : m;
         const float dm = fmaxf((v.m - ref) * LP_LOG2E, LP_FLOOR), c = lp_exp2(dm);
         float s = c * v.s, t = c * (v.t + dm * v.s);
@@ -139,13 +145,20 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
         for (int u = 0; u < LP_UNROLL; u++)
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                const float d = (x[u][e] - ref) * LP_LOG2E, w = lp_exp2(d);
+                const float d = (pc.at(x[u], e) - ref) * LP_LOG2E, w = lp_exp2(d);
                 s += w;
                 t = fmaf(fmaxf(d, LP_FLOOR), w, t);
             }
         v = {m, s, t};
     }
-    sh.tmax[tid] = pc.n > tid ? lp_key(v.m) : 0u;
+    const unsigned mine = pc.n > tid ? lp_key(v.m) : 0u;
+    if (a.n_top > 0) {                                            // maxima of groups of four (eight) threads
+        unsigned g = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+        g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+        if (a.n_top <= 32) g = max(g, __shfl_xor_sync(0xffffffffu, g, 4));
+        const int size = a.n_top <= 32 ? 8 : 4;
+        if (tid % size == 0) sh.group[tid / size] = g;
+    }
     const Sums w = lp_join_warp(v);
     if (lane == 0) sh.sums[warp] = w;
     __syncthreads();
@@ -155,25 +168,22 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
         if (lane == 0) sh.cta = j;
     }
     if (a.n_top > 0 && top > 0) {
-        // ---- the top-th largest of the threads' maxima: the largest bound that `top` of them reach (0 if fewer threads have entries at all)
+        // ---- the top-th largest of the groups' maxima (of 32 or 64, equal ones in any order; 0 where fewer groups have entries)
         if (warp == 0) {
-            unsigned mine[LP_THREADS / 32], bound = 0;
-#pragma unroll
-            for (int i = 0; i < LP_THREADS / 32; i++) mine[i] = sh.tmax[lane + 32 * i];
-            for (int bit = 31; bit >= 0; bit--) {
-                const unsigned trial = bound | 1u << bit;
-                unsigned n = 0;
-#pragma unroll
-                for (int i = 0; i < LP_THREADS / 32; i++) n += mine[i] >= trial;
-                n = __reduce_add_sync(0xffffffffu, n);
-                if ((int)n >= top) bound = trial;
-                if ((int)n == top) break;                          // (any bound that exactly `top` reach will do)
+            const unsigned g0 = sh.group[lane], g1 = a.n_top <= 32 ? 0u : sh.group[lane + 32];
+            int above0 = 0, above1 = 0;
+#pragma unroll 8
+            for (int i = 0; i < 32; i++) {
+                const unsigned o0 = __shfl_sync(0xffffffffu, g0, i), o1 = __shfl_sync(0xffffffffu, g1, i);
+                above0 += (o0 > g0 || (o0 == g0 && i < lane)) + (o1 > g0);
+                above1 += (o0 > g1 || o0 == g1) + (o1 > g1 || (o1 == g1 && i < lane));
             }
-            if (lane == 0) sh.bound = bound;
+            if (above0 == top - 1) sh.bound = g0;
+            else if (above1 == top - 1) sh.bound = g1;
         }
         __syncthreads();
         const unsigned bound = sh.bound;
-        if (sh.tmax[tid] >= bound && pc.n > tid) {
+        if (mine >= bound && pc.n > tid) {
             const int i = atomicAdd(&sh.n_sel, 1);
             if (i < LP_SEL) sh.sel[i] = tid;
         }
@@ -182,14 +192,13 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
         if (n_sel <= LP_SEL) {
             for (int i = tid; i < n_sel * rounds; i += LP_THREADS) {
                 const int p = sh.sel[i % n_sel] + i / n_sel * LP_THREADS;
-                float x[VEC];
-                pc.load(p, x);
+                const uint4 x = pc.load(p);
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
                     const int id = pc.first(p) + e;
-                    if (lp_key(x[e]) >= bound && pc.id_ok(id)) {
+                    if (lp_key(pc.at(x, e)) >= bound && pc.id_ok(id)) {
                         const int at = atomicAdd(&sh.n_cand, 1);
-                        if (at < LP_CAND) sh.cand[at] = lp_rank_key(x[e], id);
+                        if (at < LP_CAND) sh.cand[at] = lp_rank_key(pc.at(x, e), id);
                     }
                 }
             }
@@ -203,12 +212,11 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
             for (int place = 0; place < top; place++) {
                 unsigned long long best = 0;
                 for (int p = tid; p < pc.n; p += LP_THREADS) {
-                    float x[VEC];
-                    pc.load(p, x);
+                    const uint4 x = pc.load(p);
 #pragma unroll
                     for (int e = 0; e < VEC; e++) {
                         const int id = pc.first(p) + e;
-                        const unsigned long long k = lp_rank_key(x[e], id);
+                        const unsigned long long k = lp_rank_key(pc.at(x, e), id);
                         if (pc.id_ok(id) && k < below && k > best) best = k;
                     }
                 }
@@ -233,13 +241,13 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
     if (parts > 1) {
         cluster_sync();
         if (part != 0) { cluster_sync(); return; }                // (its shared memory is read until then)
-        total = Sums{-INFINITY, 0.f, 0.f};
-        for (int i = 0; i < parts; i++) {
-            const uint32_t at = cluster_address(smem_u32(&sh.cta), i);
+        if (warp == 0) {                                          // (a lane a part)
+            const uint32_t at = cluster_address(smem_u32(&sh.cta), min(lane, parts - 1));
             float f[3];
 #pragma unroll
             for (int e = 0; e < 3; e++) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f[e]) : "r"(at + 4 * e) : "memory");
-            total = lp_join(total, Sums{f[0], f[1], f[2]});
+            const Sums j = lp_join_warp(lane < parts ? Sums{f[0], f[1], f[2]} : Sums{-INFINITY, 0.f, 0.f});
+            if (lane == 0) sh.sums[0] = j;
         }
         if (a.n_top > 0) {
             // part i has min(n_top, its entries) keys
@@ -253,6 +261,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
             keys = all;
         }
         __syncthreads();
+        total = sh.sums[0];
         cluster_sync();
     }
     const float log2_s = log2f(total.s), ref = total.m == -INFINITY ? 0.f : total.m;
@@ -264,7 +273,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
         auto put = [&](int rank, unsigned long long k) {
             const int id = (int)~(unsigned)k;
             ids[rank] = id;
-            lp[rank] = none ? -INFINITY : logprob(lp_float(row[id]));
+            lp[rank] = none ? -INFINITY : logprob(lp_value(k));
         };
         if (parts > 1) lp_rank(keys, n_keys, a.n_top, put);
         else for (int i = tid; i < n_keys; i += LP_THREADS) put(i, keys[i]);
@@ -272,10 +281,7 @@ __global__ void __launch_bounds__(LP_THREADS) logprobs_kernel(const LogprobArgs 
     }
     if (tid == 0) {
         if (a.entropy) a.entropy[r] = none ? 0.f : (log2_s - total.t / total.s) * LP_LN2;
-        if (a.logprob) {
-            const int t = a.tokens[r];
-            a.logprob[r] = t < 0 || t >= a.n_vocab || none ? -INFINITY : logprob(lp_float(row[t]));
-        }
+        if (a.logprob) a.logprob[r] = !has_token || none ? -INFINITY : logprob(token_logit);
     }
 }
 
@@ -283,7 +289,7 @@ template <typename T>
 static cudaError_t logprobs_typed(const LogprobArgs& a, cudaStream_t s) {
     // few rows: up to eight CTAs a row, as long as they fit the SMs at once and a thread still has entries
     int parts = 1;
-    while (parts < 8 && (long)a.n_rows * parts * 2 <= 2 * 148 && a.n_vocab / (parts * 2) >= 2 * LP_THREADS) parts *= 2;
+    while (parts < 8 && (long)a.n_rows * parts * 2 <= 4 * 148 && a.n_vocab / (parts * 2) >= 2 * LP_THREADS) parts *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(a.n_rows * parts)); cfg.blockDim = dim3(LP_THREADS); cfg.stream = s;
     cudaLaunchAttribute at[1];

@@ -7,6 +7,8 @@ There is no CPU fallback: if the library is missing or fails to load this raises
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import sysconfig
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
@@ -179,6 +181,24 @@ def load_lists() -> ctypes.PyDLL | None:
             lib.b2_py_step.argtypes = [c_void_p, c_void_p, ctypes.py_object, ctypes.py_object, ctypes.py_object, c_int, c_int, c_void_p, c_int]
         _lists = lib
     return _lists
+
+
+_calls = False
+
+
+def load_calls():
+    """The module inside libb200_pylists that makes device_ops' calls in native code, or None (as for load_lists)."""
+    global _calls
+    if _calls is False:
+        path = os.path.join(os.path.dirname(LIB_PATH), "libb200_pylists" + sysconfig.get_config_var("EXT_SUFFIX"))
+        try:
+            loader = importlib.machinery.ExtensionFileLoader("libb200_pylists", path)
+            module = importlib.util.module_from_spec(importlib.util.spec_from_file_location("libb200_pylists", path, loader=loader))
+            loader.exec_module(module)
+        except ImportError:
+            module = None
+        _calls = module
+    return _calls
 
 
 class B2Error(RuntimeError):

@@ -9,8 +9,9 @@ package does not import torch itself); results go into tensors of the caller's, 
 handle, or None for the default stream; the call only enqueues work there, so tensors that other streams use must be ordered by the caller. Wrong
 shapes, types or devices raise ValueError before anything is enqueued.
 
-The checks are written for few attribute reads (each is 0.05 to 0.1 us on a tensor, and a single token's call is a few microseconds of device time): one
-condition a tensor, and what was wrong with it is only looked for once it fails.
+A call is made by native code where that has been built (csrc/py_tensors.cpp: a single token's call is a few microseconds of device time, and reading a dozen
+tensors in Python takes more). What it does not take comes back here, where the same checks say what is wrong: one condition a tensor, and what was
+wrong with it is only looked for once it fails.
 """
 from __future__ import annotations
 
@@ -28,11 +29,23 @@ _ROWS, _CACHE = (_F32, _F16, _BF16), (_F16, _BF16)
 _LAYOUTS = {"pairs": _cabi.B2_ROTATE_PAIRS, "halves": _cabi.B2_ROTATE_HALVES}
 
 
+def _entry(name):
+    """The native call and the address of the C entry point that it is to call, or two None."""
+    calls = _cabi.load_calls()
+    return (None, None) if calls is None else (getattr(calls, name), ctypes.cast(getattr(_cabi.load_library(), "b2_" + name), ctypes.c_void_p).value)
+
+
+_entries = {}        # name -> _entry(name), once it has been called
+
+
 class _Codes(dict):
     """dtype object -> type id (-1: none of ours); filled as dtypes are met."""
 
     def __missing__(self, dtype):
         code = self[dtype] = _TYPES.get(str(dtype).rpartition(".")[2], -1)
+        calls = _cabi.load_calls()
+        if calls is not None and code >= 0:
+            calls.add_type(dtype, code)
         return code
 
 
@@ -106,6 +119,14 @@ def kv_append(k, v, k_pool, v_pool, pages, row_start, lengths, *, freqs=None, la
     row_start [sequences + 1], lengths [sequences] int32: rows row_start[s] .. row_start[s + 1] - 1 are the newest of sequence s's lengths[s] tokens.
     `freqs` (float32 [rotated entries / 2], None: no rotation) are radians per position, `first_pos` the position of a sequence's first own token.
     `q` [rows, heads, dim] of k's type is rotated into `q_out` of the cache's type."""
+    stream = getattr(stream, "cuda_stream", stream)
+    call, entry = _entries.get("kv_append") or _entries.setdefault("kv_append", _entry("kv_append"))
+    if call is not None and layout in _LAYOUTS:
+        code = call(entry, k, v, k_pool, v_pool, pages, row_start, lengths, freqs, q, q_out, _LAYOUTS[layout], first_pos, amplitude, stream)
+        if code is not None:
+            if code:
+                check(code, "b2_kv_append")
+            return
     device, shape, rows = _begin("k", k, 3, _ROWS)
     n, n_kv, dim = shape
     kp, vp, pool, cache, where = _where(n, k_pool, v_pool, pages, row_start, lengths, device)
@@ -131,7 +152,7 @@ def kv_append(k, v, k_pool, v_pool, pages, row_start, lengths, *, freqs=None, la
         pf, rot = _dense("freqs", freqs, freqs.shape if len(freqs.shape) == 1 else (None,), (_F32,), device), 2 * freqs.shape[0]
     args = _kv_append(pk, pv, pq, kp, vp, po, pf, sk[0], sk[1], sv[0], sv[1], sq[0], sq[1], so[0], so[1], first_pos, rows, cache, heads, n_kv, dim, rot,
                       _LAYOUTS[layout], amplitude)
-    check(_cabi.load_library().b2_kv_append(device, where, args, getattr(stream, "cuda_stream", stream)), "b2_kv_append")
+    check(_cabi.load_library().b2_kv_append(device, where, args, stream), "b2_kv_append")
 
 
 def attention_shared_prefix_workspace(rows, n_head, n_kv, head_dim) -> int:
@@ -148,6 +169,14 @@ def attention_shared_prefix(q, k_pool, v_pool, prefix_pages, n_prefix, pages, ro
     row_start, lengths int32 as for kv_append: lengths count a sequence's own tokens, those behind the prefix. `workspace`: a contiguous tensor of at
     least attention_shared_prefix_workspace bytes, which no other call on another stream uses meanwhile (None when n_prefix is 0). `max_rows`: most
     rows of a sequence (None: all rows may be one sequence's; 1 for a batched step of single tokens is much faster than leaving it open)."""
+    stream = getattr(stream, "cuda_stream", stream)
+    call, entry = _entries.get("attention_shared_prefix") or _entries.setdefault("attention_shared_prefix", _entry("attention_shared_prefix"))
+    if call is not None:
+        code = call(entry, q, k_pool, v_pool, pages, row_start, lengths, prefix_pages, n_prefix, out, workspace, max_rows, scale, stream)
+        if code is not None:
+            if code:
+                check(code, "b2_attention_shared_prefix")
+            return
     device, shape, kind = _begin("q", q, 3, _CACHE)
     n, heads, dim = shape
     kp, vp, pool, cache, where = _where(n, k_pool, v_pool, pages, row_start, lengths, device)
@@ -168,7 +197,7 @@ def attention_shared_prefix(q, k_pool, v_pool, prefix_pages, n_prefix, pages, ro
         pw, size = workspace.data_ptr(), workspace.nbytes
     args = _shared_prefix(pq, kp, vp, pp, po, pw, size, sq[0], sq[1], so[0], so[1], n_prefix, max(1, n) if max_rows is None else max_rows, heads, pool[1], dim,
                           kind, 1.0 / math.sqrt(dim) if scale is None else scale)
-    check(_cabi.load_library().b2_attention_shared_prefix(device, where, args, getattr(stream, "cuda_stream", stream)), "b2_attention_shared_prefix")
+    check(_cabi.load_library().b2_attention_shared_prefix(device, where, args, stream), "b2_attention_shared_prefix")
 
 
 def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_logprob=None, top_id=None, *, stream=None):
@@ -176,6 +205,14 @@ def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_logprob=
 
     logits float32, float16 or bfloat16; logprob, entropy float32 [rows]; top_logprob float32 and top_id int32 [rows, n], n <= 64. A result whose tensor is None is
     left out."""
+    stream = getattr(stream, "cuda_stream", stream)
+    call, entry = _entries.get("token_logprobs") or _entries.setdefault("token_logprobs", _entry("token_logprobs"))
+    if call is not None:
+        code = call(entry, logits, tokens, logprob, entropy, top_logprob, top_id, stream)
+        if code is not None:
+            if code:
+                check(code, "b2_token_logprobs")
+            return
     device, shape, kind = _begin("logits", logits, 2, _ROWS)
     n, vocab = shape
     p, stride = _rows("logits", logits, shape, (kind,), device)
@@ -195,4 +232,4 @@ def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_logprob=
         n_top = top_id.shape[1]
         pti, ptl = _dense("top_id", top_id, (n, n_top), (_I32,), device), _dense("top_logprob", top_logprob, (n, n_top), (_F32,), device)
     check(_cabi.load_library().b2_token_logprobs(device, p, kind, stride[0] if n > 1 else vocab, n, vocab, pt, pl, pe, n_top, ptl, pti,
-                                                 getattr(stream, "cuda_stream", stream)), "b2_token_logprobs")
+                                                 stream), "b2_token_logprobs")

@@ -170,3 +170,74 @@ def test_python_refusals_of_logprobs(native_lib):
             token_logprobs(**{**good, **over})
     with pytest.raises(RuntimeError, match="n_top"):
         token_logprobs(**{**good, "top_logprob": f(5, 65, dtype=torch.float32), "top_id": i(5, 65)})
+
+
+# ------------------------------------------------------------------------------------------------------ the native calls
+def native_calls():
+    from llama_cpp import _cabi
+    calls = _cabi.load_calls()
+    if calls is None:
+        pytest.skip("the native calls are not built for this interpreter")
+    return calls
+
+
+def test_native_calls_pass_what_the_python_ones_pass(native_lib, monkeypatch):
+    """every argument reaches the entry point alike, whether the call is made in native code or in Python"""
+    import struct
+    from llama_cpp import _cabi, device_ops as ops
+    calls = native_calls()
+    seen = []
+    where, append, shared = (struct.Struct("@" + "".join({ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}[t] for _, t in s._fields_))
+                             for s in (_cabi.B2RaggedPages, _cabi.B2KvAppend, _cabi.B2SharedPrefix))
+
+    def entry(kind):
+        def f(device, w, args, stream):
+            seen.append((device, where.unpack(ctypes.string_at(w, where.size)), kind.unpack(ctypes.string_at(args, kind.size)), stream))
+            return 0
+        return ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p)(f)
+
+    def flat(*a):
+        seen.append(a)
+        return 0
+
+    class Lib:
+        b2_kv_append, b2_attention_shared_prefix = entry(append), entry(shared)
+        b2_token_logprobs = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p,
+                                             ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p)(flat)
+
+    f, i = tensors()
+    wide = OnGpu(torch.zeros(5, 9, 64).half(), 3)
+    part = lambda a, b: OnGpu(wide.t[:, a:b], 3)
+    g = lambda *s, dtype=torch.float16: f(*s, dtype=dtype, device=3)
+    j = lambda *s: g(*s, dtype=torch.int32)
+    pools = dict(k_pool=g(9, 2, 16, 64), v_pool=g(9, 2, 16, 64), pages=j(3, 4), row_start=j(4), lengths=j(3))
+    jobs = [lambda: ops.kv_append(part(0, 2), part(2, 4), **pools, freqs=g(20, dtype=torch.float32), layout="halves", first_pos=77, amplitude=1.5, q=part(4, 9), q_out=g(5, 5, 64), stream=1234),
+            lambda: ops.kv_append(part(0, 2), part(2, 4), **{**pools, "pages": OnGpu(pools["pages"].t[:, :2], 3)}),
+            lambda: ops.attention_shared_prefix(part(0, 4), pools["k_pool"], pools["v_pool"], j(2), 30, pools["pages"], pools["row_start"], pools["lengths"], g(5, 4, 64), g(1000), max_rows=2, stream=5),
+            lambda: ops.attention_shared_prefix(part(0, 4), pools["k_pool"], pools["v_pool"], None, 0, pools["pages"], pools["row_start"], pools["lengths"], g(5, 4, 64), None, scale=0.3),
+            lambda: ops.token_logprobs(OnGpu(torch.zeros(5, 20)[:, :18], 3), j(5), g(5, dtype=torch.float32), g(5, dtype=torch.float32), g(5, 3, dtype=torch.float32), j(5, 3), stream=9),
+            lambda: ops.token_logprobs(g(1, 20), entropy=g(1, dtype=torch.float32))]
+    held = []
+    real = torch.zeros
+    monkeypatch.setattr(torch, "zeros", lambda *a, **k: held.append(real(*a, **k)) or held[-1])      # (addresses stay taken, so that they can be compared)
+    monkeypatch.setattr(_cabi, "load_library", lambda path=None: Lib)
+    for job in jobs:
+        monkeypatch.setattr(ops, "_entries", {})
+        job()                                                           # (dtypes are met)
+        for native in (True, False):
+            monkeypatch.setattr(ops, "_entries", {} if native else {n: (None, None) for n in ("kv_append", "attention_shared_prefix", "token_logprobs")})
+            seen.clear()
+            made = []
+            if native:
+                for name in ("kv_append", "attention_shared_prefix", "token_logprobs"):
+                    fn = getattr(calls, name)
+                    ops._entries[name] = ((lambda fn: lambda *a: made.append(fn(*a)) or made[-1])(fn), ctypes.cast(getattr(Lib, "b2_" + name), ctypes.c_void_p).value)
+            start = len(held)
+            job()
+            new = {t.data_ptr(): n for n, t in enumerate(held[start:])}     # a call's own tensors by their order
+            call = [tuple(tuple(new.get(v, v) for v in part) if isinstance(part, tuple) else new.get(part, part) for part in one) for one in seen]
+            assert len(call) == 1 and (not native or made == [0])
+            if native:
+                want = call
+            else:
+                assert call == want
