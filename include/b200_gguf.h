@@ -98,6 +98,9 @@ int b2_engine_device_bytes(b2_engine* e, int64_t* weight_bytes, int64_t* kv_byte
 /* ---- sequences (paged KV): replaces llama_kv_cache_* bookkeeping (llama.cpp llama_kv_cache).
  *      The page allocator lives in the host (llama_cpp/kv_pages.py); the engine only holds
  *      each slot's page table. -------------------------------------------------------------- */
+/* Tables may begin with the same pages: batched steps (b2_decode) of slots that share at least 128 tokens' whole pages
+ * read those once for all of them. No slot may write to a page that another one reads: the token at position n_past has
+ * to lie behind the shared pages. */
 int b2_seq_set_blocks(b2_engine* e, int slot, const int32_t* host_blocks, int n_blocks);
 /* Start (or restart) a slot: n_past tokens are already in its KV pages; `host_history` are the
  * last <= 64 tokens of the sequence so far (for the penalties); `host_uniforms` are n_uniform
@@ -131,6 +134,12 @@ int b2_seq_set_token(b2_engine* e, int slot, int32_t token);
 int b2_forward_pending(b2_engine* e, int slot);
 /* Copy the slot's current logits [n_vocab] to the host (llama_get_logits). */
 int b2_get_logits(b2_engine* e, int slot, float* host_out);
+/* Log probabilities of sampled tokens: while n_top is 0..64 (-1, the start: off), b2_sample, b2_decode and b2_step also
+ * work out, from the logits as the model gave them (before the penalties), the log probability of every token that they
+ * sample, the entropy and the n_top most likely tokens (see b2_token_logprobs); b2_decode_n is refused. b2_get_logprobs
+ * reads those of the slot's latest sampled token (any pointer may be NULL; top_logprob, top_id [n_top]). */
+int b2_set_logprobs(b2_engine* e, int n_top);
+int b2_get_logprobs(b2_engine* e, int slot, float* host_logprob, float* host_entropy, float* host_top_logprob, int32_t* host_top_id);
 int b2_synchronize(b2_engine* e);
 
 /* ---- layer-list models: decoders given as a list of layers over dense bf16 / f32 tensors (no counterpart in the
@@ -279,6 +288,12 @@ int b2_engine_create_layered(const b2_layered_config* cfg, const b2_layer_desc* 
 #define B2_STEP_MAX_ENTRIES 64
 int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const int32_t* n_tokens, const int32_t* host_tokens,
             const int32_t* want_rows, int n_want, float* host_logits, const int32_t* sample, int32_t* host_sampled);
+/* The same without sampling, for scoring: instead of the wanted rows' logits their log probabilities of want_tokens
+ * [n_want], entropies and n_top (0..64) most likely tokens come to the host (as b2_token_logprobs gives them; logprob, entropy [n_want] may be
+ * NULL, top_logprob, top_id [n_want][n_top]). A row's logits stay on the device. */
+int b2_step_scores(b2_engine* e, int n_entries, const int32_t* slots, const int32_t* n_tokens, const int32_t* host_tokens,
+                   const int32_t* want_rows, const int32_t* want_tokens, int n_want, int n_top, float* host_logprob,
+                   float* host_entropy, float* host_top_logprob, int32_t* host_top_id);
 /* Debugging / parity: keep the residual stream after every layer of the next steps (on != 0), and read it back:
  * host_out [n_layer][T][n_embd] for the T tokens of the last step. */
 int b2_step_trace(b2_engine* e, int on);

@@ -50,6 +50,7 @@ cudaError_t kv_append_launch(const KvAppendArgs& a, cudaStream_t s);
 
 // ---------------------------------------------------------------- logprobs.cu
 constexpr int LOGPROB_MAX_TOP = 64;
+struct RowMap { int n; int token[BATCH_MAX], out[BATCH_MAX]; };      // row r's token is tokens[token[r]], its results go to row out[r] (n 0: to r, tokens[r])
 struct LogprobArgs {
     const void* logits;          // [n_rows][n_vocab], rows row_stride elements apart
     long row_stride;
@@ -59,7 +60,7 @@ struct LogprobArgs {
     int* top_id;
     int n_rows, n_vocab, n_top, type;
 };
-cudaError_t logprobs_launch(const LogprobArgs& a, cudaStream_t s);
+cudaError_t logprobs_launch(const LogprobArgs& a, cudaStream_t s, const RowMap* map = nullptr);
 
 // ---------------------------------------------------------------- shared_prefix.cu, shared_prefix_tc.cu
 struct SharedPrefixArgs {
@@ -81,6 +82,7 @@ struct SharedPrefixArgs {
     BatchIdx slots;
     __half* out_h;
     int out_T_pad;
+    unsigned int* err;           // where a wait that runs out is recorded (null: see shared_prefix_error)
 };
 size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim);
 cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s);

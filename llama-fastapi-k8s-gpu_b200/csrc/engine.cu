@@ -4,6 +4,7 @@
 // Stands in for libllama's llama_model + llama_context behind llama-cpp-python's Llama object
 // (api.py:24-28,55-63).
 #include "engine_state.h"
+#include "device_ops.h"
 #include "layered.h"
 #include "ptx.cuh"
 #include "quant_blocks.cuh"
@@ -212,6 +213,8 @@ extern "C" int b2_engine_destroy(b2_engine* e) {
     if (e->pinned) cudaFreeHost(e->pinned);
     if (e->slot_token) cudaFreeHost(e->slot_token);
     if (e->logits_stage) cudaFreeHost(e->logits_stage);
+    cudaFree(e->lp.raw); cudaFree(e->sp_work);
+    for (void* p : {(void*)e->lp.logprob, (void*)e->lp.entropy, (void*)e->lp.top_logprob, (void*)e->lp.top_id}) if (p) cudaFreeHost(p);
     if (e->ev0) cudaEventDestroy(e->ev0);
     if (e->ev1) cudaEventDestroy(e->ev1);
     if (e->stream) cudaStreamDestroy(e->stream);
@@ -637,6 +640,7 @@ extern "C" int b2_seq_set_blocks(b2_engine* e, int slot, const int32_t* blocks, 
     for (int i = 0; i < n; i++)
         if (blocks[i] < 0 || blocks[i] >= e->cfg.kv_num_blocks) return fail(B2_ERR_ARG, "KV page id out of range");
     CK(cudaSetDevice(e->cfg.device));
+    e->slots[slot].blocks.assign(blocks, blocks + n);
     if (n) CK(cudaMemcpyAsync(e->slots[slot].block_table, blocks, sizeof(int) * n, cudaMemcpyHostToDevice, e->stream));
     CK(cudaStreamSynchronize(e->stream));   // `blocks` is caller memory
     return B2_OK;
@@ -713,6 +717,7 @@ extern "C" int b2_seq_begin(b2_engine* e, int slot, int n_past, const int32_t* h
     s.n_past = n_past;
     s.last_token = -1;
     s.n_sampled = 0;
+    s.lp_kept = false;
     return B2_OK;
 }
 
@@ -851,15 +856,31 @@ extern "C" int b2_prefill(b2_engine* e, int slot, const int32_t* tokens, int n) 
 }
 
 
+// enqueue: log probabilities of the tokens that n rows of logits (as they were before the penalties) were sampled to; row r is slot slots[r]'s
+static int sampled_logprobs(b2_engine* e, const float* raw, int n, const int32_t* tokens, const int* slots) {
+    SampledLogprobs& lp = e->lp;
+    RowMap map = {};
+    map.n = n;
+    for (int r = 0; r < n; r++) { map.token[r] = r; map.out[r] = slots[r]; e->slots[slots[r]].lp_kept = true; }
+    LogprobArgs a = {};
+    a.logits = raw; a.type = ELEM_F32; a.n_rows = n; a.n_vocab = e->cfg.n_vocab; a.row_stride = a.n_vocab; a.tokens = tokens;
+    a.logprob = lp.logprob; a.entropy = lp.entropy; a.n_top = lp.n_top; a.top_logprob = lp.top_logprob; a.top_id = lp.top_id;
+    CK(logprobs_launch(a, e->stream, &map));
+    e->launches++;
+    return B2_OK;
+}
+
 // enqueue: sample from the slot's logit buffer (the token at position n_past - 1 was the last one evaluated); the token
 // is in e->slot_token once the stream has been synchronised
 static int sample_enqueue(b2_engine* e, Slot& s) {
+    const int at = (int)(&s - e->slots.data());
+    if (e->lp.n_top >= 0) CK(cudaMemcpyAsync(e->lp.raw, s.logits, sizeof(float) * e->cfg.n_vocab, cudaMemcpyDeviceToDevice, e->stream));
     // (the sampler moves the position on from the last evaluated token)
     CK(sample_launch(s.logits, e->cfg.n_vocab, s.sp, s.sst, s.uniforms, s.ints + 3, s.ints + 2, s.ints + 0,
-                     s.ints + 1, s.ring, e->cfg.n_ctx + 1, e->stream, false, e->slot_token + (&s - e->slots.data()), s.n_past - 1));
+                     s.ints + 1, s.ring, e->cfg.n_ctx + 1, e->stream, false, e->slot_token + at, s.n_past - 1));
     e->launches++;
     s.n_sampled += 1;
-    return B2_OK;
+    return e->lp.n_top >= 0 ? sampled_logprobs(e, e->lp.raw, 1, e->slot_token + at, &at) : B2_OK;
 }
 
 extern "C" int b2_sample(b2_engine* e, int slot, int32_t* out) {
@@ -887,6 +908,23 @@ static int ensure_batch_workspace(b2_engine* e) {
     return B2_OK;
 }
 
+// Tokens at the start that all sequences of a batched step have in the same pages (whole pages; the token that the step writes lies behind them). 0: fewer than
+// are worth the attention that reads them once.
+constexpr int SHARED_MIN_TOKENS = 128;
+static int shared_prefix_tokens(const b2_engine* e, const BatchIdx& b) {
+    const Slot& first = e->slots[b.slot[0]];
+    size_t pages = first.blocks.size();
+    for (int i = 0; i < b.n && pages; i++) {
+        const Slot& s = e->slots[b.slot[i]];
+        pages = std::min({pages, s.blocks.size(), (size_t)(s.n_past / e->cfg.kv_block_tokens)});
+        size_t same = 0;
+        while (same < pages && s.blocks[same] == first.blocks[same]) same++;
+        pages = same;
+    }
+    const int tokens = (int)pages * e->cfg.kv_block_tokens;
+    return e->attn_mma != 0 && tokens >= SHARED_MIN_TOKENS ? tokens : 0;
+}
+
 // One decode step for b.n sequences at once: the weights are read (and dequantised) once for all of them by the
 // tensor-core GEMM; attention and sampling run one CTA group per sequence from the per-slot device tables.
 // Enqueued kernel by kernel. Captured per list of slots, 8 steps of 32 sequences (4 layers of 4096) took 6580 us instead of 6750; but the list
@@ -898,6 +936,16 @@ static int batch_step(b2_engine* e, const BatchIdx& b, const BatchTokens& set, i
     const int T = b.n, T_pad = (T + 15) / 16 * 16, E = c.n_embd, F = c.n_ff, hd = c.head_dim, qd = c.n_head * hd;
     int rc, np = 0;
     long ps = 0;
+    const int shared = shared_prefix_tokens(e, b);
+    if (shared > 0) {
+        const size_t need = shared_prefix_work_floats(T, c.n_head, c.n_head_kv, hd);
+        if (need > e->sp_work_floats) {          // (frees only behind what runs: cudaFree waits)
+            cudaFree(e->sp_work);
+            e->sp_work = nullptr; e->sp_work_floats = 0;
+            CK(cudaMalloc(&e->sp_work, need * 4));
+            e->sp_work_floats = need;
+        }
+    }
     CK(embed_batch_launch(e->tok_embd.type, e->tok_embd.ptr, E, e->slot_tab, b, set, e->pf_x, st));
     for (int i = 0; i < T; i++) e->slots[b.slot[i]].set_token = -1;
     e->launches++;
@@ -918,7 +966,16 @@ static int batch_step(b2_engine* e, const BatchIdx& b, const BatchTokens& set, i
         while (ns > 1 && (long)ns * c.n_head_kv * T > 2L * e->n_sms) ns >>= 1;
         if (e->batch_attn_splits > 0 && e->batch_attn_splits <= e->n_splits) ns = e->batch_attn_splits;
         a.n_splits = ns; a.scale = 1.0f / sqrtf((float)hd); a.err = kernel_error_word(); a.max_pages = e->max_blocks;
-        if (e->attn_mma != 0) {      // the tensor-core kernel writes f16 in the o-projection GEMM's operand order itself
+        if (shared > 0) {
+            SharedPrefixArgs x = {};
+            x.r.n_seqs = x.r.n_rows = T; x.r.max_pages = e->max_blocks - shared / c.kv_block_tokens; x.r.block_tokens = c.kv_block_tokens; x.r.n_pages = c.kv_num_blocks;
+            x.q = e->bd_q; x.q_row = qd; x.q_head = hd; x.q_f32 = 1; x.k_pool = kc; x.v_pool = vc;
+            x.prefix_pages = e->slots[b.slot[0]].block_table; x.n_prefix = shared; x.work = e->sp_work; x.max_rows = 1;
+            x.n_head = c.n_head; x.n_kv = c.n_head_kv; x.head_dim = hd; x.type = ELEM_F16; x.scale_log2 = a.scale * 1.4426950408889634f;
+            x.tab = e->slot_tab; x.slots = b; x.out_h = e->pf_att; x.out_T_pad = T_pad; x.err = a.err;
+            CK(shared_prefix_launch(x, st));
+            e->launches += 2;
+        } else if (e->attn_mma != 0) {      // the tensor-core kernel writes f16 in the o-projection GEMM's operand order itself
             a.out_h = e->pf_att; a.out_T_pad = T_pad;
             CK(attn_decode_mma_launch(a, e->slot_tab, &b, st, false));
         } else {
@@ -949,9 +1006,11 @@ static int batch_step(b2_engine* e, const BatchIdx& b, const BatchTokens& set, i
         }
         CK(gemm_launch(it->second, st));
     }
+    float* raw = e->lp.raw;
+    if (e->lp.n_top >= 0) CK(cudaMemcpyAsync(raw, e->pf_part, sizeof(float) * T * c.n_vocab, cudaMemcpyDeviceToDevice, st));
     CK(sample_batch_launch(e->pf_part, c.n_vocab, c.n_vocab, e->slot_tab, b, c.n_ctx + 1, tokens_out, st));
     e->launches += 3;
-    return B2_OK;
+    return e->lp.n_top >= 0 ? sampled_logprobs(e, raw, T, tokens_out, b.slot) : B2_OK;
 }
 
 extern "C" int b2_decode(b2_engine* e, const int32_t* slots, int n, int32_t* out) {
@@ -988,10 +1047,11 @@ extern "C" int b2_decode(b2_engine* e, const int32_t* slots, int n, int32_t* out
         for (int i = 0; i < n; i++) {
             Slot& s = e->slots[slots[i]];
             int rc = enter_set_token(e, s);
-            if (!rc) rc = run_step(e, s, GK_DECODE);
+            if (!rc) rc = run_step(e, s, e->lp.n_top >= 0 ? GK_FWD : GK_DECODE);
             if (rc) return rc;
             s.n_past += 1;
-            s.n_sampled += 1;
+            if (e->lp.n_top >= 0) { if ((rc = sample_enqueue(e, s))) return rc; }      // (the captured step samples without keeping the logits)
+            else s.n_sampled += 1;
         }
     }
     CK(cudaStreamSynchronize(e->stream));
@@ -1006,6 +1066,7 @@ extern "C" int b2_decode_n(b2_engine* e, int slot, int n, int32_t* out) {
     std::lock_guard<std::mutex> lk(e->mu);
     Slot& s = e->slots[slot];
     if (n <= 0) return fail(B2_ERR_ARG, "n must be positive");
+    if (e->lp.n_top >= 0) return fail(B2_ERR_STATE, "log probabilities are kept step by step: use b2_decode");
     if (s.n_past + n > e->cfg.n_ctx) return fail(B2_ERR_ARG, "context window full");
     CK(cudaSetDevice(e->cfg.device));
     if ((rc = enter_set_token(e, s))) return rc;
@@ -1115,6 +1176,46 @@ extern "C" int b2_get_logits(b2_engine* e, int slot, float* out) {
     CK(cudaMemcpyAsync(e->logits_stage, s.logits_view ? s.logits_view : s.logits, bytes, cudaMemcpyDeviceToHost, e->stream));
     CK(cudaStreamSynchronize(e->stream));
     memcpy(out, e->logits_stage, bytes);
+    return B2_OK;
+}
+
+int b2_logprob_buffers(b2_engine* e) {
+    SampledLogprobs& lp = e->lp;
+    if (lp.top_id) return B2_OK;
+    const size_t kept = e->layered ? 1 : std::min<size_t>(e->slots.size(), BATCH_MAX);      // (a ragged step keeps its logits itself)
+    const size_t rows = e->slots.size() + (e->layered ? LOGIT_ROWS : 0);
+    if (!lp.raw) CK(cudaMalloc(&lp.raw, sizeof(float) * kept * e->cfg.n_vocab));
+    if (!lp.logprob) CK(cudaMallocHost(&lp.logprob, sizeof(float) * rows));
+    if (!lp.entropy) CK(cudaMallocHost(&lp.entropy, sizeof(float) * rows));
+    if (!lp.top_logprob) CK(cudaMallocHost(&lp.top_logprob, sizeof(float) * rows * LOGPROB_MAX_TOP));
+    CK(cudaMallocHost(&lp.top_id, sizeof(int32_t) * rows * LOGPROB_MAX_TOP));
+    return B2_OK;
+}
+
+extern "C" int b2_set_logprobs(b2_engine* e, int n_top) {
+    if (!e) return fail(B2_ERR_ARG, "null engine");
+    if (!e->finalized) return fail(B2_ERR_STATE, "engine not finalized");
+    if (n_top < -1 || n_top > LOGPROB_MAX_TOP) return fail(B2_ERR_ARG, "n_top must be in -1..64");
+    std::lock_guard<std::mutex> lk(e->mu);
+    SampledLogprobs& lp = e->lp;
+    CK(cudaSetDevice(e->cfg.device));
+    if (n_top >= 0) if (int rc = b2_logprob_buffers(e)) return rc;
+    if (n_top != lp.n_top) for (auto& s : e->slots) s.lp_kept = false;
+    lp.n_top = n_top;
+    return B2_OK;
+}
+
+extern "C" int b2_get_logprobs(b2_engine* e, int slot, float* logprob, float* entropy, float* top_logprob, int32_t* top_id) {
+    int rc = check_slot(e, slot); if (rc) return rc;
+    std::lock_guard<std::mutex> lk(e->mu);
+    const SampledLogprobs& lp = e->lp;
+    if (lp.n_top < 0 || !e->slots[slot].lp_kept) return fail(B2_ERR_STATE, "no log probabilities of this slot's latest token have been kept");
+    CK(cudaSetDevice(e->cfg.device));
+    CK(cudaStreamSynchronize(e->stream));
+    if (logprob) *logprob = lp.logprob[slot];
+    if (entropy) *entropy = lp.entropy[slot];
+    if (top_logprob) memcpy(top_logprob, lp.top_logprob + (size_t)slot * lp.n_top, sizeof(float) * lp.n_top);
+    if (top_id) memcpy(top_id, lp.top_id + (size_t)slot * lp.n_top, sizeof(int32_t) * lp.n_top);
     return B2_OK;
 }
 

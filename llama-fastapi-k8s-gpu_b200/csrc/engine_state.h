@@ -54,7 +54,24 @@ struct Slot {
     int set_token = -1;            // set by the caller and not yet in ints[0] (-1: none)
     int last_token = -1;           // layer-list models: the token at position n_past - 1 (-1: none yet)
     int n_sampled = 0;             // host mirror of ints[3]
+    std::vector<int32_t> blocks;   // host mirror of block_table
+    bool lp_kept = false;          // the engine holds log probabilities of this slot's latest sampled token
 };
+
+constexpr int LOGIT_ROWS = 256;      // rows of logits that a step of a layer-list engine works out at once
+
+// log probabilities of sampled tokens (b2_set_logprobs): logits as the model gave them, kept while the sampler applies its penalties in place, and results in
+// host memory that the kernel writes, slot by slot; behind the slots, in layer-list engines, a chunk of rows that are scored
+struct SampledLogprobs {
+    int n_top = -1;                // -1: off
+    float* raw = nullptr;          // device [rows of a step][n_vocab]
+    float *logprob = nullptr, *entropy = nullptr, *top_logprob = nullptr;      // pinned [slots + chunk], top_logprob and top_id [..][64] with n_top of a row in use, side by side
+    int32_t* top_id = nullptr;
+};
+
+struct b2_engine;
+// the buffers of b2_engine::lp; made by the first call that wants them and kept (captured steps hold their addresses)
+int b2_logprob_buffers(b2_engine* e);
 
 // recurrent state that starts from zero with every sequence: `floats` of them per slot
 struct ResetRegion { float* base; size_t floats; };
@@ -112,6 +129,9 @@ struct b2_engine {
     std::unordered_map<uint64_t, GemmParams> gemm_plans;
     // layer-list models (b2_engine_create_layered): graph, dense weights, KV pools and recurrent state live here
     LayeredModel* layered = nullptr;
+    SampledLogprobs lp;
+    float* sp_work = nullptr;      // partial results of batched attention behind a prefix that the sequences' tables share
+    size_t sp_work_floats = 0;
     std::mutex mu;
 };
 

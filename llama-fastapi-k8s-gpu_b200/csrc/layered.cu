@@ -12,6 +12,7 @@
 // llama graph (engine.cu): tensors, sequence slots and their page tables, sampler state, stream, error reporting. Owns: fused
 // projection matrices, per-layer cache pages, per-slot recurrent state, the step workspace.
 #include "engine_state.h"
+#include "device_ops.h"
 #include "layered.h"
 #include "ptx.cuh"
 #include "quant_blocks.cuh"
@@ -135,7 +136,6 @@ struct LayeredModel {
     int prof_n[8] = {};
 };
 
-constexpr int LOGIT_ROWS = 256;
 
 __global__ void to_f32_kernel(int type, const void* src, long n, float* dst) {
     const long i = blockIdx.x * (long)blockDim.x + threadIdx.x;
@@ -1735,12 +1735,15 @@ struct StepChainPdl {
     ~StepChainPdl() { g_chain_pdl = prev; }
 };
 
-extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const int32_t* n_tokens, const int32_t* tokens,
-                       const int32_t* want_rows, int n_want, float* host_logits, const int32_t* sample, int32_t* host_sampled) {
+// log probabilities of given tokens in place of the wanted rows' logits
+struct StepScores { const int32_t* tokens; int n_top; float *logprob, *entropy, *top_logprob; int32_t* top_id; };
+
+static int step_impl(b2_engine* e, int n_entries, const int32_t* slots, const int32_t* n_tokens, const int32_t* tokens, const int32_t* want_rows, int n_want, float* host_logits,
+                     const int32_t* sample, int32_t* host_sampled, const StepScores* scores) {
     if (!e || !e->layered) return b2_fail(B2_ERR_UNSUPPORTED, "b2_step needs an engine made by b2_engine_create_layered");
     if (!e->finalized) return b2_fail(B2_ERR_STATE, "engine not finalized");
     if (n_entries <= 0 || n_entries > B2_STEP_MAX_ENTRIES || !slots || !n_tokens || !tokens) return b2_fail(B2_ERR_ARG, "bad arguments");
-    if (n_want < 0 || (n_want > 0 && (!want_rows || !host_logits))) return b2_fail(B2_ERR_ARG, "bad wanted rows");
+    if (n_want < 0 || (n_want > 0 && (!want_rows || (!host_logits && !scores)))) return b2_fail(B2_ERR_ARG, "bad wanted rows");
     std::lock_guard<std::mutex> lk(e->mu);
     LayeredModel* m = e->layered;
     const b2_layered_config& c = m->c;
@@ -1758,7 +1761,7 @@ extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const 
     int n_tiles = 0;
     for (int i = 0; i < n_entries; i++) n_tiles += (n_tokens[i] + 63) / 64;
     // (rows may be asked for more than once: as often as the description of the step has room for)
-    if ((size_t)4 * T + 5 * n_entries + 2 * n_tiles + n_want > m->meta_ints) return b2_fail(B2_ERR_ARG, "more wanted rows than a step of this engine holds");
+    if ((size_t)4 * T + 5 * n_entries + 2 * n_tiles + (scores ? 2 : 1) * n_want > m->meta_ints) return b2_fail(B2_ERR_ARG, "more wanted rows than a step of this engine holds");
     CK(cudaSetDevice(c.device));
     cudaStream_t st = e->stream;
     StepChainPdl chain(e->chain_pdl);
@@ -1798,7 +1801,11 @@ extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const 
     std::vector<int> samp_row(n, -1);
     for (int i = 0; i < n; i++)
         if (sample && sample[i]) { samp_row[i] = n_rows; h_rows[n_rows++] = h_start[i] + h_len[i] - 1; }
-    const size_t n_meta = (size_t)4 * T + 4 * n + 2 * n_tiles + n_rows;
+    if (scores) for (int i = 0; i < n_want; i++) h_rows[n_rows + i] = scores->tokens[i];      // (nothing is sampled beside them)
+    const size_t n_meta = (size_t)4 * T + 4 * n + 2 * n_tiles + n_rows + (scores ? n_want : 0);
+    SampledLogprobs& lp = e->lp;
+    if (scores) if (int rc0 = b2_logprob_buffers(e)) return rc0;
+    const size_t scored = e->slots.size();                       // (scores go behind the slots' log probabilities)
     RaggedDev r = {};
     r.tok_id = m->meta; r.tok_seg = m->meta + T; r.tok_pos = m->meta + 2 * T; r.tok_prev = m->meta + 3 * T; r.seg_slot = m->meta + 4 * T;
     r.seg_start = r.seg_slot + n; r.seg_len = r.seg_start + n; r.seg_pos0 = r.seg_len + n; r.T = T; r.n_seg = n;
@@ -1828,6 +1835,15 @@ extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const 
         hs.scale = c.logit_scale != 0.f ? c.logit_scale : 1.f;
         int rc2 = dense(e, m, m->head, m->rows, W, m->logits, V, nr, nullptr, EPI_NONE, 6, &hs);
         if (rc2) return rc2;
+        LogprobArgs la = {};
+        la.type = ELEM_F32; la.n_vocab = V; la.row_stride = V; la.logprob = lp.logprob; la.entropy = lp.entropy; la.top_logprob = lp.top_logprob; la.top_id = lp.top_id;
+        if (scores) {
+            la.logits = m->logits; la.n_rows = nr; la.n_top = scores->n_top; la.tokens = d_rows + n_rows + r0;
+            la.logprob += scored; la.entropy += scored; la.top_logprob += scored * LOGPROB_MAX_TOP; la.top_id += scored * LOGPROB_MAX_TOP;
+            CK(logprobs_launch(la, st));
+            e->launches++;
+            return B2_OK;
+        }
         const int n_w = std::max(0, std::min(n_want - r0, nr));
         if (n_w > 0) {
             CK(cudaMemcpyAsync(m->logits_host, m->logits, (size_t)n_w * V * 4, cudaMemcpyDeviceToHost, st));
@@ -1839,6 +1855,14 @@ extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const 
         if (sr.n > 0) {
             CK(sample_rows_launch(m->logits, V, m->slot_tab, m->slot_logits, sr, r.seg_slot, r.seg_pos0, r.seg_len, c.n_ctx + 1, e->pinned, st));
             e->launches++;
+            if (lp.n_top >= 0) {                                 // (the sampled rows are neighbours; their tokens arrive entry by entry)
+                RowMap map = {};
+                map.n = sr.n;
+                for (int i = 0; i < sr.n; i++) { map.token[i] = sr.entry[i]; map.out[i] = slots[sr.entry[i]]; }
+                la.logits = m->logits + (size_t)sr.row[0] * V; la.n_rows = sr.n; la.n_top = lp.n_top; la.tokens = e->pinned;
+                CK(logprobs_launch(la, st, &map));
+                e->launches++;
+            }
         }
         return B2_OK;
     };
@@ -1854,11 +1878,11 @@ extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const 
     // (The description goes ahead of the graph: as its first node, the copy kept the kernels behind it waiting for a while.)
     CK(cudaMemcpyAsync(m->meta, h, n_meta * 4, cudaMemcpyHostToDevice, st));
     bool done = false;
-    if (m->graphs_on && !m->trace && !m->profile && T <= 64 && n_rows <= LOGIT_ROWS) {
+    if (m->graphs_on && !m->trace && !m->profile && !scores && T <= 64 && n_rows <= LOGIT_ROWS) {
         std::string key;
         key.reserve(16 + 12 * n);
         auto put = [&](int v) { key.append(reinterpret_cast<const char*>(&v), sizeof(v)); };
-        put(n); put(n_want);
+        put(n); put(n_want); put(lp.n_top);
         for (int i = 0; i < n; i++) { put(slots[i]); put(n_tokens[i]); put(samp_row[i]); }
         auto it = m->graphs.find(key);
         if (it == m->graphs.end()) {
@@ -1897,7 +1921,24 @@ extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const 
     }
     m->last_T = T;
     for (int i = 0; i < n; i++) if (samp_row[i] >= 0) e->slots[slots[i]].logits_view = e->slots[slots[i]].logits;
-    if (n_rows <= LOGIT_ROWS) {
+    auto hand_out = [&](int r0, int nr) -> int {                 // scores of a chunk of rows
+        CK(cudaStreamSynchronize(st));
+        if (scores->logprob) memcpy(scores->logprob + r0, lp.logprob + scored, sizeof(float) * nr);
+        if (scores->entropy) memcpy(scores->entropy + r0, lp.entropy + scored, sizeof(float) * nr);
+        if (scores->n_top) {
+            memcpy(scores->top_logprob + (size_t)r0 * scores->n_top, lp.top_logprob + scored * LOGPROB_MAX_TOP, sizeof(float) * nr * scores->n_top);
+            memcpy(scores->top_id + (size_t)r0 * scores->n_top, lp.top_id + scored * LOGPROB_MAX_TOP, sizeof(int32_t) * nr * scores->n_top);
+        }
+        return B2_OK;
+    };
+    if (scores) {
+        if (n_rows <= LOGIT_ROWS) { if ((rc = hand_out(0, n_rows))) return rc; }
+        else
+            for (int r0 = 0; r0 < n_rows; r0 += LOGIT_ROWS) {
+                const int nr = std::min(LOGIT_ROWS, n_rows - r0);
+                if ((rc = head_chunk(r0, nr)) || (rc = hand_out(r0, nr))) return rc;
+            }
+    } else if (n_rows <= LOGIT_ROWS) {
         if (n_want > 0) {
             // (to the caller while the sampler runs, unless a graph has hidden where the copy ends)
             CK(done ? cudaStreamSynchronize(st) : cudaEventSynchronize(m->logits_here));
@@ -1921,6 +1962,7 @@ extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const 
     CK(cudaStreamSynchronize(st));
     if ((rc = b2_check_kernel_error())) return rc;
     for (int i = 0; i < n; i++) {
+        if (samp_row[i] >= 0) e->slots[slots[i]].lp_kept = lp.n_top >= 0;
         if (host_sampled) host_sampled[i] = samp_row[i] >= 0 ? e->pinned[i] : -1;
         if (samp_row[i] >= 0) e->slots[slots[i]].n_sampled += 1;
     }
@@ -1933,6 +1975,19 @@ extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const 
         }
     }
     return B2_OK;
+}
+
+extern "C" int b2_step(b2_engine* e, int n_entries, const int32_t* slots, const int32_t* n_tokens, const int32_t* tokens,
+                       const int32_t* want_rows, int n_want, float* host_logits, const int32_t* sample, int32_t* host_sampled) {
+    return step_impl(e, n_entries, slots, n_tokens, tokens, want_rows, n_want, host_logits, sample, host_sampled, nullptr);
+}
+
+extern "C" int b2_step_scores(b2_engine* e, int n_entries, const int32_t* slots, const int32_t* n_tokens, const int32_t* tokens, const int32_t* want_rows, const int32_t* want_tokens,
+                              int n_want, int n_top, float* logprob, float* entropy, float* top_logprob, int32_t* top_id) {
+    if (n_want <= 0 || !want_rows || !want_tokens) return b2_fail(B2_ERR_ARG, "bad wanted rows");
+    if (n_top < 0 || n_top > LOGPROB_MAX_TOP || (n_top && (!top_logprob || !top_id))) return b2_fail(B2_ERR_ARG, "n_top must be in 0..64, with room for the alternatives");
+    const StepScores sc = {want_tokens, n_top, logprob, entropy, top_logprob, top_id};
+    return step_impl(e, n_entries, slots, n_tokens, tokens, want_rows, n_want, nullptr, nullptr, nullptr, &sc);
 }
 
 extern "C" int b2_step_trace(b2_engine* e, int on) {

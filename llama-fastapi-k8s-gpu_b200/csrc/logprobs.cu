@@ -110,12 +110,14 @@ __device__ __forceinline__ uint32_t lp_cluster_rank() { uint32_t r; asm("mov.u32
 
 // cluster of `parts` CTAs a row (1: none)
 template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobArgs a, int parts) {
+__global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobArgs a, const RowMap map, int parts) {
     constexpr int VEC = 16 / sizeof(T);
     __shared__ LpShared sh;
     __shared__ unsigned long long all[8 * LOGPROB_MAX_TOP];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    griddep_wait();                                               // (in the engines' chains: the logits, the sampled tokens)
     const int part = parts > 1 ? (int)lp_cluster_rank() : 0, r = blockIdx.x / parts;
+    const int to = map.n ? map.out[r] : r;
     const T* row = (const T*)a.logits + (long)r * a.row_stride;
     const int chunk = ((a.n_vocab + parts - 1) / parts + VEC - 1) / VEC * VEC;
     const Pieces<T, VEC> pc(row, min(a.n_vocab, part * chunk), min(a.n_vocab, (part + 1) * chunk));
@@ -123,7 +125,7 @@ __global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobAr
     if (tid == 0) { sh.n_sel = sh.n_cand = sh.n_own = 0; }
 
     // (the asked token's logit, read ahead by the thread that will want it)
-    const int token = part == 0 && tid == 0 && a.logprob ? a.tokens[r] : -1;
+    const int token = part == 0 && tid == 0 && a.logprob ? a.tokens[map.n ? map.token[r] : r] : -1;
     const bool has_token = token >= 0 && token < a.n_vocab;
     const float token_logit = has_token ? lp_float(row[token]) : 0.f;
 
@@ -268,8 +270,8 @@ __global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobAr
     auto logprob = [&](float x) { return ((x - ref) * LP_LOG2E - log2_s) * LP_LN2; };
     const bool none = total.s == 0.f;                              // every entry masked
     if (a.n_top > 0) {
-        float* lp = a.top_logprob + (long)r * a.n_top;
-        int* ids = a.top_id + (long)r * a.n_top;
+        float* lp = a.top_logprob + (long)to * a.n_top;
+        int* ids = a.top_id + (long)to * a.n_top;
         auto put = [&](int rank, unsigned long long k) {
             const int id = (int)~(unsigned)k;
             ids[rank] = id;
@@ -280,13 +282,13 @@ __global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobAr
         for (int i = min(a.n_top, a.n_vocab) + tid; i < a.n_top; i += LP_THREADS) { ids[i] = -1; lp[i] = -INFINITY; }
     }
     if (tid == 0) {
-        if (a.entropy) a.entropy[r] = none ? 0.f : (log2_s - total.t / total.s) * LP_LN2;
-        if (a.logprob) a.logprob[r] = !has_token || none ? -INFINITY : logprob(token_logit);
+        if (a.entropy) a.entropy[to] = none ? 0.f : (log2_s - total.t / total.s) * LP_LN2;
+        if (a.logprob) a.logprob[to] = !has_token || none ? -INFINITY : logprob(token_logit);
     }
 }
 
 template <typename T>
-static cudaError_t logprobs_typed(const LogprobArgs& a, cudaStream_t s) {
+static cudaError_t logprobs_typed(const LogprobArgs& a, const RowMap& map, cudaStream_t s) {
     // few rows: up to eight CTAs a row, as long as they fit the SMs at once and a thread still has entries
     int parts = 1;
     while (parts < 8 && (long)a.n_rows * parts * 2 <= 4 * 148 && a.n_vocab / (parts * 2) >= 2 * LP_THREADS) parts *= 2;
@@ -296,15 +298,16 @@ static cudaError_t logprobs_typed(const LogprobArgs& a, cudaStream_t s) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = parts; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a, parts);
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a, map, parts);
 }
 
-cudaError_t logprobs_launch(const LogprobArgs& a, cudaStream_t s) {
+cudaError_t logprobs_launch(const LogprobArgs& a, cudaStream_t s, const RowMap* map) {
     if (a.n_rows == 0) return cudaSuccess;
+    const RowMap none = {};
     switch (a.type) {
-        case ELEM_F32: return logprobs_typed<float>(a, s);
-        case ELEM_F16: return logprobs_typed<__half>(a, s);
-        default: return logprobs_typed<__nv_bfloat16>(a, s);
+        case ELEM_F32: return logprobs_typed<float>(a, map ? *map : none, s);
+        case ELEM_F16: return logprobs_typed<__half>(a, map ? *map : none, s);
+        default: return logprobs_typed<__nv_bfloat16>(a, map ? *map : none, s);
     }
 }
 

@@ -26,6 +26,7 @@ constexpr int SP_TT = 64;            // keys of a tile
 constexpr int sp_stages(int hd) { return hd == 64 ? 4 : 2; }             // tiles under way: 64 KB, three CTAs an SM
 
 __device__ unsigned int sp_error[5];                             // see mbar_give_up
+__device__ __forceinline__ unsigned int* sp_err(const SharedPrefixArgs& a) { return a.err ? a.err : sp_error; }
 
 __device__ __forceinline__ float sp_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
 
@@ -128,7 +129,7 @@ __device__ __forceinline__ void sp_copy(const SharedPrefixArgs& a, const SpPlan&
         if (ti && ti % ahead == 0) ids = j < w.q1 ? w.table[j / bt] : 0;
         const int id = __shfl_sync(0xffffffffu, ids, ti % ahead * boxes + lane % boxes);
         const int row = (int)(((long)min(max(id, 0), (int)a.r.n_pages - 1) * a.n_kv + kvh) * bt + j % bt);
-        if (it >= STAGES) mbar_wait_warp(&empty[st], (it / STAGES - 1) & 1, sp_error, 0xa0001u, (unsigned)it);
+        if (it >= STAGES) mbar_wait_warp(&empty[st], (it / STAGES - 1) & 1, sp_err(a), 0xa0001u, (unsigned)it);
         if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(n_box * p.box_rows * 128 * PARTS * 2));
         __syncwarp();
         if (lane < n_box)
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
             int x = 0, y = 0, z = 0, next_ids = 0;
             SpWork::Read read = {0, 0, 0};
             auto take = [&]() {
-                mbar_wait_warp(&answered, asked++ & 1, sp_error, 0xa0004u, (unsigned)n);
+                mbar_wait_warp(&answered, asked++ & 1, sp_err(a), 0xa0004u, (unsigned)n);
                 if (!sp_answered_work(answer, x, y, z) || x >= (int)gridDim.x || y >= (int)gridDim.y || z >= (int)gridDim.z) return false;      // (a wait that ran out leaves anything)
                 if (z == p.prefix_z) return true;
                 read = SpWork::read(a, z);
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
             v_kvh = y;
             ids = !more || (p.splits == 1 && v.own_pass) ? next_ids : sp_first_ids(a, p, v.table, v.q0, v.q1, lane);
             // (work n + 1's place, and the queries of work n - 1, are free again)
-            if (n >= 1) mbar_wait_warp(&next_empty[n & 1], ((n - 1) >> 1) & 1, sp_error, 0xa0005u, (unsigned)n);
+            if (n >= 1) mbar_wait_warp(&next_empty[n & 1], ((n - 1) >> 1) & 1, sp_err(a), 0xa0005u, (unsigned)n);
             if (more) sp_stage_q<E, HD>(a, v, v_kvh, q_s + ((n + 1) & 1) * p.mrows * (HD + 8), lane, 32);
             __syncwarp();
             if (lane == 0) {
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
         for (int hh = 0, it = 0;; hh++) {
             if (hh > 0) {
                 const int i = (hh - 1) & 1;
-                mbar_wait(&next_full[i], ((hh - 1) >> 1) & 1, sp_error, 0xa0006u, (unsigned)hh);
+                mbar_wait(&next_full[i], ((hh - 1) >> 1) & 1, sp_err(a), 0xa0006u, (unsigned)hh);
                 if (next[i].n_f < 0) break;
                 w = next[i]; kvh = next_kvh[i];
             } else {
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
             for (int ti = 0; ti < w.n_tiles; ti++, it++) {
                 const int st = it % STAGES, buf = it & 1, t0 = w.q0 + ti * SP_TT, valid = min(SP_TT, w.q1 - t0);
                 uint8_t *kb = tiles_at + st * 2 * PARTS * PART, *vb = kb + PARTS * PART;
-                mbar_wait(&full[st], (it / STAGES) & 1, sp_error, 0xa0002u, (unsigned)it);
+                mbar_wait(&full[st], (it / STAGES) & 1, sp_err(a), 0xa0002u, (unsigned)it);
                 __syncwarp();
                 // ---- scores of this warp's keys, scaled, masked, and their maxima in rows g and g + 8; this thread's columns are 2 tq, 2 tq + 1 of every eight keys
                 float sc[2][4], sd[2][4], mx[2] = {-INFINITY, -INFINITY};
@@ -546,7 +547,7 @@ __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const
         for (int ti = 0; ti < w.n_tiles; ti++) {
             const int st = ti % STAGES, t0 = w.q0 + ti * SP_TT, valid = min(SP_TT, w.q1 - t0);
             uint8_t *kb = tiles_at + st * 2 * PARTS * PART, *vb = kb + PARTS * PART;
-            mbar_wait(&full[st], (ti / STAGES) & 1, sp_error, 0xa0003u, (unsigned)ti);
+            mbar_wait(&full[st], (ti / STAGES) & 1, sp_err(a), 0xa0003u, (unsigned)ti);
             __syncwarp();
             if (!idle) {
                 if (valid & 15) {                                // (every warp clears what it reads)

@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
     extern __shared__ uint8_t st_smem[];
     __shared__ uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2];
     __shared__ uint32_t tmem_at;
-    unsigned int* err = st_error;
+    unsigned int* err = a.err ? a.err : st_error;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     uint8_t* qs = reinterpret_cast<uint8_t*>(((uintptr_t)st_smem + 1023) & ~(uintptr_t)1023);      // [tile][part]
     uint8_t* ks = qs + 2 * PARTS * ST_PART;                      // [stage][part]

@@ -107,6 +107,9 @@ SIGNATURES = {
     "b2_seq_set_token": (c_int, [c_void_p, c_int, c_int32]),
     "b2_forward_pending": (c_int, [c_void_p, c_int]),
     "b2_get_logits": (c_int, [c_void_p, c_int, c_void_p]),
+    "b2_set_logprobs": (c_int, [c_void_p, c_int]),
+    "b2_get_logprobs": (c_int, [c_void_p, c_int] + [c_void_p] * 4),
+    "b2_step_scores": (c_int, [c_void_p, c_int] + [POINTER(c_int32)] * 5 + [c_int, c_int] + [c_void_p] * 4),
     "b2_synchronize": (c_int, [c_void_p]),
     "b2_engine_create_layered": (c_int, [POINTER(B2LayeredConfig), POINTER(B2LayerDesc), POINTER(c_void_p)]),
     "b2_step": (c_int, [c_void_p, c_int, POINTER(c_int32), POINTER(c_int32), POINTER(c_int32), POINTER(c_int32), c_int, c_void_p,

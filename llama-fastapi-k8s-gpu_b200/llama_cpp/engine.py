@@ -12,7 +12,7 @@ import ctypes
 import os
 import threading
 from dataclasses import dataclass
-from typing import List, Optional, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import numpy as np
 
@@ -69,6 +69,14 @@ class SamplingSettings:
                           self.frequency_penalty, self.presence_penalty, self.top_k, self.penalty_last_n)
 
 
+@dataclass
+class TokenLogprobs:
+    """A sampled token's log probability, the entropy of its distribution (nats) and the most likely tokens, (id, log probability) each."""
+    logprob: float
+    entropy: float
+    top: List[Tuple[int, float]]
+
+
 def read_dims(g: GGUFFile) -> ModelDims:
     md = g.metadata
     arch = md.get("general.architecture", "llama")
@@ -94,6 +102,7 @@ def read_dims(g: GGUFFile) -> ModelDims:
 class EngineBase:
     """What every native engine handle shares: lifecycle, sequence slots with their page tables, the device sampler,
     logits read-back and the measurement hooks. `Engine` adds the llama graph's calls, `LayeredEngine` the ragged step."""
+    _n_top: Optional[int] = None
     ragged = False      # True: the scheduler drives `step()` (prompt portions and decoded tokens in one batch)
 
     # ---------------------------------------------------------------- lifecycle
@@ -123,12 +132,34 @@ class EngineBase:
     def ensure_pages(self, slot: int, n_tokens: int):
         """Make sure the slot's page table covers n_tokens positions (uploads it if it grew)."""
         if self.pages.ensure(slot, n_tokens):
-            tbl = self.pages.table(slot)
-            arr = int32s(tbl)
-            check(self.lib.b2_seq_set_blocks(self._h, slot, arr, len(tbl)), "b2_seq_set_blocks")
+            self._set_table(slot)
 
     def release(self, slot: int):
         self.pages.release(slot)
+
+    def share_pages(self, slot: int, other: int, n_tokens: int) -> int:
+        """Let the slot begin with the whole pages of another one's first n_tokens instead of what it holds (GGUF models: no recurrent state). Returns the
+        tokens they cover; batched steps read shared pages once for all slots."""
+        if self.ragged:
+            raise ValueError("layer-list models start every sequence at position 0: pages cannot be shared")
+        if slot == other:
+            raise ValueError("a slot cannot share its own pages")
+        self.pages.release(slot)
+        n = self.pages.share(slot, other, n_tokens)
+        self._set_table(slot)
+        return n
+
+    def own_pages(self, slot: int, n_tokens: int) -> int:
+        """Before the slot is written from its token n_tokens on: see PageAllocator.own_from."""
+        held = len(self.pages.table(slot))
+        kept = self.pages.own_from(slot, n_tokens)
+        if len(self.pages.table(slot)) != held:
+            self._set_table(slot)
+        return kept
+
+    def _set_table(self, slot: int):
+        tbl = self.pages.table(slot)
+        check(self.lib.b2_seq_set_blocks(self._h, slot, int32s(tbl), len(tbl)), "b2_seq_set_blocks")
 
     def sample(self, slot: int) -> int:
         out = ctypes.c_int32()
@@ -139,6 +170,20 @@ class EngineBase:
         out = np.empty(self.dims.n_vocab, dtype=np.float32)
         check(self.lib.b2_get_logits(self._h, slot, out.ctypes.data_as(ctypes.c_void_p)), "b2_get_logits")
         return out
+
+    # ---------------------------------------------------------------- log probabilities of sampled tokens
+    def set_logprobs(self, n_top: Optional[int]):
+        """From now on work out the log probability of every sampled token, its step's entropy and the n_top (0..64) most likely tokens, from the logits
+        ahead of the penalties; None: stop. `decode_n` cannot."""
+        check(self.lib.b2_set_logprobs(self._h, -1 if n_top is None else int(n_top)), "b2_set_logprobs")
+        self._n_top = n_top
+
+    def logprobs(self, slot: int) -> TokenLogprobs:
+        """Of the slot's latest sampled token."""
+        n = self._n_top or 0
+        lp, h, tl, ti = ctypes.c_float(), ctypes.c_float(), (ctypes.c_float * max(n, 1))(), (ctypes.c_int32 * max(n, 1))()
+        check(self.lib.b2_get_logprobs(self._h, slot, ctypes.byref(lp), ctypes.byref(h), tl, ti), "b2_get_logprobs")
+        return TokenLogprobs(lp.value, h.value, [(ti[i], tl[i]) for i in range(n) if ti[i] >= 0])
 
     # ---------------------------------------------------------------- measurement
     def timer_start(self):
@@ -412,6 +457,26 @@ class LayeredEngine(EngineBase):
                 if flags[b]:
                     sampled[i] = int(out_tok[b])
         return logits, sampled
+
+    def score(self, entries, want, tokens, n_top: int = 0):
+        """One ragged step that scores: log probabilities of given tokens instead of logits. entries as for `step`; want: per entry, indices into its tokens;
+        tokens: per entry, for each of those, the token whose log probability is asked for (the one that follows, say). Returns (logprob, entropy, top_logprob,
+        top_id) with a row per wanted token, in entry order. The entries must fit one native step."""
+        flat, rows, asked, lens = [], [], [], []
+        for (_, toks), w, t in zip(entries, want, tokens):
+            if len(w) != len(t) or not all(0 <= i < len(toks) for i in w):
+                raise ValueError("every wanted row needs one token, and must be a row of its entry")
+            rows.extend(len(flat) + i for i in w)
+            asked.extend(t)
+            flat.extend(toks)
+            lens.append(len(toks))
+        n = len(rows)
+        lp, h = np.empty(n, dtype=np.float32), np.empty(n, dtype=np.float32)
+        tl, ti = np.empty((n, n_top), dtype=np.float32), np.empty((n, n_top), dtype=np.int32)
+        ptr = lambda a: a.ctypes.data_as(ctypes.c_void_p)
+        check(self.lib.b2_step_scores(self._h, len(entries), int32s([slot for slot, _ in entries]), int32s(lens), int32s(flat), int32s(rows), int32s(asked), n, n_top, ptr(lp), ptr(h),
+                                      ptr(tl) if n_top else None, ptr(ti) if n_top else None), "b2_step_scores")
+        return lp, h, tl, ti
 
     def trace_layers(self, on: bool = True):
         check(self.lib.b2_step_trace(self._h, 1 if on else 0), "b2_step_trace")

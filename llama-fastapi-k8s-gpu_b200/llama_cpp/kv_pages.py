@@ -6,8 +6,11 @@ This engine pages it: the device holds one pool of fixed-size pages shared by al
 and each sequence owns a page table. This class hands out page ids; the engine only ever sees
 `b2_seq_set_blocks(slot, pages)`.
 
-Invariants (property-tested in tests/test_kv_pages.py): a page is owned by at most one sequence,
-pages are never leaked, `free + owned == num_blocks`.
+Invariants (property-tested in tests/test_kv_pages.py): a page is owned by at most one sequence unless `share` gave it to another one too,
+pages are never leaked, `free + pages in some table == num_blocks`.
+
+Sharing: sequences that begin with the same tokens may begin with the same pages (`share`); such a page is free again when the last table drops it.
+Nobody may write to a shared page, so a sequence that is to write from a token on first gets pages of its own there (`own_from`).
 """
 from __future__ import annotations
 
@@ -27,6 +30,7 @@ class PageAllocator:
         self.block_tokens = block_tokens
         self._free: List[int] = list(range(num_blocks - 1, -1, -1))   # pop() hands out low ids first
         self._owned: Dict[int, List[int]] = {}
+        self._more: Dict[int, int] = {}      # page -> how many tables hold it beyond the first
         self._lock = threading.Lock()
 
     def pages_for(self, n_tokens: int) -> int:
@@ -52,10 +56,42 @@ class PageAllocator:
                 pages.append(self._free.pop())
             return True
 
+    def _drop(self, page: int) -> None:
+        more = self._more.get(page, 0)
+        if more == 0:
+            self._free.append(page)
+        elif more == 1:
+            del self._more[page]
+        else:
+            self._more[page] = more - 1
+
     def release(self, seq_id: int) -> None:
         with self._lock:
-            pages = self._owned.pop(seq_id, [])
-            self._free.extend(reversed(pages))
+            for page in reversed(self._owned.pop(seq_id, [])):
+                self._drop(page)
+
+    def share(self, seq_id: int, other: int, n_tokens: int) -> int:
+        """Give seq_id, which must hold nothing, the whole pages of `other`'s first n_tokens. Returns the tokens they cover."""
+        with self._lock:
+            if self._owned.get(seq_id):
+                raise ValueError(f"sequence {seq_id} holds pages already")
+            pages = self._owned.get(other, [])[:n_tokens // self.block_tokens]
+            for page in pages:
+                self._more[page] = self._more.get(page, 0) + 1
+            self._owned[seq_id] = list(pages)
+            return len(pages) * self.block_tokens
+
+    def own_from(self, seq_id: int, n_tokens: int) -> int:
+        """Before seq_id writes from its token n_tokens on: the pages from there on that others hold too are dropped from its table. Returns how many of
+        its tokens are still cached: n_tokens, or fewer where the page of that token was shared (it is to be written anew)."""
+        with self._lock:
+            pages = self._owned.get(seq_id, [])
+            first = next((i for i in range(n_tokens // self.block_tokens, len(pages)) if pages[i] in self._more), None)
+            if first is None:
+                return n_tokens
+            while len(pages) > first:
+                self._drop(pages.pop())
+            return min(n_tokens, first * self.block_tokens)
 
     def truncate(self, seq_id: int, n_tokens: int) -> None:
         """Keep only the pages covering the first n_tokens (prefix reuse)."""
@@ -63,7 +99,7 @@ class PageAllocator:
             pages = self._owned.get(seq_id, [])
             keep = self.pages_for(n_tokens)
             while len(pages) > keep:
-                self._free.append(pages.pop())
+                self._drop(pages.pop())
 
 
 class SequenceSlots:

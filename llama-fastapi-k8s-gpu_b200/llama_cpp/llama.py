@@ -37,7 +37,9 @@ class Llama:
         means "all layers on the GPU"; 0 asks for upstream's CPU path, which this engine does not
         have. n_ctx=0 takes the model's training context. Extra upstream keywords (n_threads,
         use_mmap, rope_*, flash_attn, ...) are accepted and ignored. `n_seq_max` (or env
-        B200_MAX_SEQS) is how many callers can be batched concurrently (default 1, like the reference).
+        B200_MAX_SEQS) is how many callers can be batched concurrently (default 1, like the reference). `share_prefix` (or env
+        B200_SHARE_PREFIX=1; GGUF models): prompts that begin alike, with the same system prompt say, share the cache's whole pages of it while they run
+        side by side: it is evaluated once, and batched steps read it once.
         `tp` = (rank, world, nccl_id) makes this object one rank of a tensor-parallel group (70B-class models; one process
         per GPU, every rank makes the same calls in the same order)."""
         if not os.path.exists(model_path):
@@ -68,7 +70,7 @@ class Llama:
         self._ragged = bool(getattr(self._engine, "ragged", False))
         self._vocab = Vocab(self._md, self._engine.dims.n_vocab)
         self._last_logits = None
-        self._scheduler = Scheduler(self._engine, self._vocab)
+        self._scheduler = Scheduler(self._engine, self._vocab, share_prefix=bool(kwargs.get("share_prefix", os.environ.get("B200_SHARE_PREFIX") == "1")))
         self._stream = UniformStream(seed)
         self._stream_lock = threading.Lock()
         # chat format selection (upstream Llama.__init__)
@@ -147,6 +149,8 @@ class Llama:
             self._scheduler.drop_cache()
             if self._ragged and not self._direct_open:
                 eng.release(0)
+            if self._scheduler.share_prefix and not self._direct_open:
+                eng.own_pages(0, 0)
             eng.ensure_pages(0, len(self._input_ids) + len(toks))
             if self._ragged:
                 if not self._direct_open:
@@ -195,7 +199,7 @@ class Llama:
                                 penalty_last_n=self.last_n_tokens_size)
 
     def _make_request(self, prompt_tokens: List[int], max_tokens: Optional[int], sampling: SamplingSettings,
-                      stop: List[bytes], seed: Optional[int], on_token=None, cancel_event=None) -> Request:
+                      stop: List[bytes], seed: Optional[int], on_token=None, cancel_event=None, logprobs: Optional[int] = None) -> Request:
         if len(prompt_tokens) == 0:
             prompt_tokens = [self._vocab.bos_id if self._vocab.bos_id >= 0 else 0]
         if len(prompt_tokens) >= self._n_ctx:
@@ -214,11 +218,11 @@ class Llama:
         self._direct_open = False
         self._input_ids = []
         return Request(prompt=list(prompt_tokens), max_tokens=int(max_tokens), sampling=sampling, stop=stop,
-                       uniforms=uniforms, on_token=on_token, cancel_event=cancel_event)
+                       uniforms=uniforms, on_token=on_token, cancel_event=cancel_event, logprobs=logprobs)
 
     def _run(self, prompt_tokens: List[int], max_tokens: Optional[int], sampling: SamplingSettings,
-             stop: List[bytes], seed: Optional[int], on_token=None, cancel_event=None) -> Request:
-        req = self._make_request(prompt_tokens, max_tokens, sampling, stop, seed, on_token, cancel_event)
+             stop: List[bytes], seed: Optional[int], on_token=None, cancel_event=None, logprobs: Optional[int] = None) -> Request:
+        req = self._make_request(prompt_tokens, max_tokens, sampling, stop, seed, on_token, cancel_event, logprobs)
         self._scheduler.submit(req).wait()
         n = len(req.completion_tokens)
         self.last_timings = dict(
@@ -238,9 +242,14 @@ class Llama:
                           logit_bias: Optional[Dict[str, float]] = None, _add_bos: bool = True,
                           _special: bool = False, cancel_event: Optional[threading.Event] = None, **kwargs: Any):
         """`cancel_event` (not in upstream): set it from another thread to abandon the generation; the call then returns
-        what was produced so far with finish_reason "cancelled" and the sequence slot is free again."""
+        what was produced so far with finish_reason "cancelled" and the sequence slot is free again. `logprobs` = n: the choice's "logprobs" holds every token's
+        log probability and its n (at most 64) most likely alternatives, from the logits ahead of the penalties, as upstream; unlike there, no
+        `logits_all` is needed."""
         if logprobs is not None:
-            raise NotImplementedError("logprobs are not implemented")
+            if stream or not hasattr(self._engine, "set_logprobs"):
+                raise NotImplementedError("logprobs are not implemented for streamed completions" if stream else "this engine has no log probabilities")
+            if not 0 <= logprobs <= 64:
+                raise ValueError("logprobs must be in 0..64")
         if stopping_criteria is not None:
             raise NotImplementedError("stopping_criteria is not implemented")
         if isinstance(prompt, str):
@@ -259,16 +268,34 @@ class Llama:
         model_name = model if model is not None else self.model_path
         if stream:
             return self._stream_completion(tokens, max_tokens, sampling, stop_b, seed, cid, created, model_name, cancel_event)
-        req = self._run(tokens, max_tokens, sampling, stop_b, seed, cancel_event=cancel_event)
+        req = self._run(tokens, max_tokens, sampling, stop_b, seed, cancel_event=cancel_event, logprobs=logprobs)
         text = req.text.decode("utf-8", errors="ignore")
-        if echo and prompt_text is not None:
-            text = prompt_text + text
+        before = prompt_text if echo and prompt_text is not None else ""
+        text = before + text
         return {
             "id": cid, "object": "text_completion", "created": created, "model": model_name,
-            "choices": [{"text": text, "index": 0, "logprobs": None, "finish_reason": req.finish_reason}],
+            "choices": [{"text": text, "index": 0, "logprobs": None if logprobs is None else self._logprobs_of(req, len(before)), "finish_reason": req.finish_reason}],
             "usage": {"prompt_tokens": len(req.prompt), "completion_tokens": len(req.completion_tokens),
                       "total_tokens": len(req.prompt) + len(req.completion_tokens)},
         }
+
+    def _logprobs_of(self, req: Request, offset: int) -> Dict[str, list]:
+        """The "logprobs" of a choice, shaped as upstream: tokens (those whose text the choice holds), where each begins in it, log probabilities, and per token a
+        dict of the alternatives' texts, the token itself among them."""
+        out: Dict[str, list] = {"tokens": [], "text_offset": [], "token_logprobs": [], "top_logprobs": []}
+        piece = lambda t: self._vocab.detokenize([t])
+        text = lambda b: b.decode("utf-8", errors="ignore")
+        at = 0                              # bytes of the text so far
+        cut = len(req.text) < len(self._vocab.detokenize(req.completion_tokens))       # by a stop string
+        for tok, lp in zip(req.completion_tokens, req.token_logprobs):
+            if cut and at >= len(req.text):
+                break
+            out["tokens"].append(text(piece(tok)))
+            out["text_offset"].append(offset + len(text(req.text[:at])))
+            out["token_logprobs"].append(lp.logprob)
+            out["top_logprobs"].append({**{text(piece(t)): v for t, v in reversed(lp.top)}, text(piece(tok)): lp.logprob})      # (of equal texts the likelier token's)
+            at += len(piece(tok))
+        return out
 
     def _stream_completion(self, tokens, max_tokens, sampling, stop_b, seed, cid, created, model_name,
                            cancel_event=None) -> Iterator[dict]:
@@ -353,13 +380,14 @@ class Llama:
                                      repeat_penalty=repeat_penalty, tfs_z=tfs_z, mirostat_mode=mirostat_mode,
                                      mirostat_tau=mirostat_tau, mirostat_eta=mirostat_eta, model=model,
                                      logits_processor=logits_processor, grammar=grammar, logit_bias=logit_bias,
-                                     cancel_event=cancel_event)
+                                     cancel_event=cancel_event,
+                                     logprobs=(top_logprobs or 0) if logprobs and not stream and hasattr(self._engine, "set_logprobs") else None)
         if stream:
             return self._chat_chunks(out)
         return {
             "id": "chat" + out["id"], "object": "chat.completion", "created": out["created"], "model": out["model"],
             "choices": [{"index": 0, "message": {"role": "assistant", "content": out["choices"][0]["text"]},
-                         "logprobs": None, "finish_reason": out["choices"][0]["finish_reason"]}],
+                         "logprobs": out["choices"][0]["logprobs"], "finish_reason": out["choices"][0]["finish_reason"]}],
             "usage": out["usage"],
         }
 

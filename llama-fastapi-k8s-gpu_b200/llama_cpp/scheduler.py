@@ -23,7 +23,7 @@ from typing import Callable, Deque, List, Optional
 
 import numpy as np
 
-from .engine import Engine, SamplingSettings
+from .engine import Engine, SamplingSettings, TokenLogprobs
 from .tokenizer import Vocab
 
 
@@ -36,6 +36,7 @@ class Request:
     uniforms: Optional[np.ndarray] = None
     on_token: Optional[Callable[[int], None]] = None     # streaming hook (scheduler thread)
     cancel_event: Optional[threading.Event] = None       # set by the caller to abandon the request (e.g. after a 408)
+    logprobs: Optional[int] = None                       # keep every token's log probability and so many alternatives
     # results
     completion_tokens: List[int] = field(default_factory=list)
     raw: bytearray = field(default_factory=bytearray)     # bytes of the completion so far (stop-string search window)
@@ -46,6 +47,7 @@ class Request:
     t_first: float = 0.0
     t_done: float = 0.0
     n_reused: int = 0
+    token_logprobs: List[TokenLogprobs] = field(default_factory=list)      # one per completion token, if asked for
     done: threading.Event = field(default_factory=threading.Event)
 
     def cancelled(self) -> bool:
@@ -102,8 +104,11 @@ class Scheduler:
     ADMIT_PER_STEP = 2     # while sequences are decoding, at most this many new prompts are processed between two decode steps
     PROMPT_PORTION = 512   # ragged engines: most prompt tokens one sequence brings into a step (decoding sequences ride along)
 
-    def __init__(self, engine: Engine, vocab: Vocab):
+    def __init__(self, engine: Engine, vocab: Vocab, share_prefix: bool = False):
+        """`share_prefix`: a prompt that begins like one whose tokens are cached in another slot shares that slot's whole pages (GGUF models)."""
         self.engine = engine
+        self.share_prefix = share_prefix and not getattr(engine, "ragged", False)
+        self._n_top: Optional[int] = None     # what the engine keeps of sampled tokens (None: nothing)
         self.vocab = vocab
         self.slots = [_Slot(i) for i in range(engine.max_seqs)]
         self.queue: Deque[Request] = deque()
@@ -204,6 +209,24 @@ class Scheduler:
         self.stats["cancelled"] += 1
         req.done.set()
 
+    def _keep_logprobs(self, reqs):
+        """Have the engine keep as many alternatives as the most demanding of the requests whose tokens are sampled next."""
+        n = max((r.logprobs for r in reqs if r.logprobs is not None), default=None)
+        if n != self._n_top:
+            self.engine.set_logprobs(n)
+            self._n_top = n
+
+    def _token(self, slot: _Slot, tok: int) -> bool:
+        """Account for a token sampled in the slot; True when its request is finished."""
+        req = slot.req
+        got = self.engine.logprobs(slot.idx) if req.logprobs is not None else None
+        n = len(req.completion_tokens)
+        done = check_token(req, self.vocab, tok)
+        if got is not None and len(req.completion_tokens) > n:
+            got.top = got.top[:req.logprobs]
+            req.token_logprobs.append(got)
+        return done
+
     def _finish(self, slot: _Slot):
         req = slot.req
         slot.req = None
@@ -225,11 +248,23 @@ class Scheduler:
                 n += 1
             return n
 
-        slot = max(free, key=lambda s: lcp(s.cached, req.prompt))
-        slot.req = req
+        same = lambda s: min(lcp(s.cached, req.prompt), len(req.prompt) - 1)
+        slot = max(free, key=same)
+        n_keep, other = same(slot), None
         eng = self.engine
+        if self.share_prefix:
+            # a running sequence has a page or more of the prompt that no free slot has: begin with its pages, in the free slot with the least to lose
+            best = max(self.slots, key=same)
+            whole = same(best) // eng.block_tokens * eng.block_tokens
+            if whole >= n_keep + eng.block_tokens:
+                slot, n_keep, other = min(free, key=lambda s: len(s.cached)), whole, best
+        slot.req = req
         try:
-            n_keep = min(lcp(slot.cached, req.prompt), len(req.prompt) - 1)
+            if other is not None:
+                slot.cached = []
+                n_keep = eng.share_pages(slot.idx, other.idx, n_keep)
+            elif self.share_prefix:
+                n_keep = eng.own_pages(slot.idx, n_keep)
             req.n_reused = n_keep
             eng.ensure_pages(slot.idx, min(eng.n_ctx, len(req.prompt) + req.max_tokens + 1))
             eng.seq_begin(slot.idx, n_keep, req.prompt[:n_keep], req.sampling, req.uniforms)
@@ -237,10 +272,11 @@ class Scheduler:
             slot.cached = list(req.prompt)
             self.stats["prefill_tokens"] += len(req.prompt) - n_keep
             self.stats["reused_tokens"] += n_keep
+            self._keep_logprobs([req])
             tok = eng.sample(slot.idx)
             req.t_first = time.perf_counter()
             slot.pending = tok
-            if check_token(req, self.vocab, tok):
+            if self._token(slot, tok):
                 self._finish(slot)
         except BaseException as exc:  # noqa: BLE001 - forwarded to the caller
             self._fail(slot, exc)
@@ -252,7 +288,8 @@ class Scheduler:
         eng = self.engine
         self.stats["max_batch"] = max(self.stats["max_batch"], len(live))
         try:
-            if len(live) == 1 and waiting == 0:
+            self._keep_logprobs([s.req for s in live])
+            if len(live) == 1 and waiting == 0 and self._n_top is None:
                 s = live[0]
                 req = s.req
                 room = eng.n_ctx - len(s.cached)
@@ -283,7 +320,7 @@ class Scheduler:
                     s.cached.append(s.pending)
                     s.pending = t
                     self.stats["tokens"] += 1
-                    if check_token(s.req, self.vocab, t):
+                    if self._token(s, t):
                         self._finish(s)
         except BaseException as exc:  # noqa: BLE001
             for s in live:
@@ -324,6 +361,7 @@ class Scheduler:
                 batch.append((s, s.req.prompt[s.fed:s.fed + take], take == left))
                 room -= take
         try:
+            self._keep_logprobs([s.req for s, _, last in batch if last])
             td = time.perf_counter()
             _, toks = eng.step([(s.idx, t) for s, t, _ in batch], sample=[last for _, _, last in batch])
             self.stats["t_decode"] += time.perf_counter() - td
@@ -339,7 +377,7 @@ class Scheduler:
                     self.stats["tokens"] += 1
                 s.cached.extend(t)
                 s.pending = tok
-                if check_token(s.req, self.vocab, tok):
+                if self._token(s, tok):
                     self._finish(s)
         except BaseException as exc:  # noqa: BLE001
             for s in live:

@@ -39,3 +39,43 @@ def test_no_page_is_leaked_or_shared(ops):
         assert all(0 <= p < 12 for p in owned)
         for s in range(6):
             pass
+
+
+@settings(max_examples=300, deadline=None)
+@given(st.lists(st.tuples(st.sampled_from(["ensure", "release", "truncate", "share", "own"]), st.integers(0, 5), st.integers(0, 5), st.integers(0, 300)), max_size=60))
+def test_shared_pages_are_counted_and_never_written(ops):
+    """A page is free exactly when no table holds it; pages that two tables hold are their leading ones, at the same places; after own_from nobody else holds
+    what is written from there on."""
+    from llama_cpp.kv_pages import OutOfPages, PageAllocator
+    a = PageAllocator(12, 32)
+    for op, seq, other, n in ops:
+        before = a.table(seq)
+        try:
+            if op == "ensure":
+                a.ensure(seq, n)
+                assert a.table(seq)[:len(before)] == before
+            elif op == "release":
+                a.release(seq)
+            elif op == "truncate":
+                a.truncate(seq, n)
+            elif op == "share" and seq != other:
+                if before:
+                    with pytest.raises(ValueError):
+                        a.share(seq, other, n)
+                else:
+                    kept = a.share(seq, other, n)
+                    assert kept % 32 == 0 and kept <= n and a.table(seq) == a.table(other)[:kept // 32]
+            elif op == "own":
+                kept = a.own_from(seq, n)
+                assert kept == n or (kept < n and kept % 32 == 0 and len(a.table(seq)) == kept // 32)
+                mine = a.table(seq)[n // 32:]
+                assert not any(p in a.table(s) for p in mine for s in range(6) if s != seq)
+                assert before[:len(a.table(seq))] == a.table(seq)
+        except OutOfPages:
+            pass
+        tables = [a.table(s) for s in range(6)]
+        held = {p for t in tables for p in t}
+        assert all(len(t) == len(set(t)) for t in tables) and len(held) + a.free_pages == 12
+        assert held.isdisjoint(a._free) and len(set(a._free)) == len(a._free)
+        for p in held:
+            assert len({t.index(p) for t in tables if p in t}) == 1
