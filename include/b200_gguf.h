@@ -98,8 +98,8 @@ int b2_engine_device_bytes(b2_engine* e, int64_t* weight_bytes, int64_t* kv_byte
 /* ---- sequences (paged KV): replaces llama_kv_cache_* bookkeeping (llama.cpp llama_kv_cache).
  *      The page allocator lives in the host (llama_cpp/kv_pages.py); the engine only holds
  *      each slot's page table. -------------------------------------------------------------- */
-/* Tables may begin with the same pages: batched steps (b2_decode) of slots that share at least 128 tokens' whole pages
- * read those once for all of them. No slot may write to a page that another one reads: the token at position n_past has
+/* Tables may begin with the same pages: a batched step (b2_decode) whose slots all share whole pages reads those once for
+ * all of them, if that is faster (16384 tokens or more over the slots, or few heads and slots). No slot may write to a page that another one reads: the token at position n_past has
  * to lie behind the shared pages. */
 int b2_seq_set_blocks(b2_engine* e, int slot, const int32_t* host_blocks, int n_blocks);
 /* Start (or restart) a slot: n_past tokens are already in its KV pages; `host_history` are the

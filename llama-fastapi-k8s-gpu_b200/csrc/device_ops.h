@@ -86,6 +86,7 @@ struct SharedPrefixArgs {
 };
 size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim);
 cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s);
+int shared_prefix_launches(const SharedPrefixArgs& a);
 
 // Prefix pass on tensor memory: the key blocks of every (KV head, 256 query rows) cut into equal runs, one run a CTA. A unit's partial results are numbered by
 // the CTAs that its blocks fall to.

@@ -908,9 +908,10 @@ static int ensure_batch_workspace(b2_engine* e) {
     return B2_OK;
 }
 
-// Tokens at the start that all sequences of a batched step have in the same pages (whole pages; the token that the step writes lies behind them). 0: fewer than
-// are worth the attention that reads them once.
-constexpr int SHARED_MIN_TOKENS = 128;
+// Tokens at the start that all sequences of a batched step have in the same pages (whole pages; the token that the step writes lies behind them). 0: reading
+// them once is not worth the launches. Measured per layer (32 heads over 8 KV heads of 128; saved, us): three launches instead of one cost about 9 us, won back
+// from about 16384 tokens in all: 8 sequences behind 1024 tokens 0.4, 4096: 20; 16 behind 512 -2, 1024: 4, 4096: 41; 32 behind 256 -5, 512: 2, 4096: 83;
+// 64 behind 128 -5, 256: 1, 512: 15, 4096: 180. Where prefix and own tokens are one launch (16 rows a KV head): 4 behind 128 0.6, 4096: 8.
 static int shared_prefix_tokens(const b2_engine* e, const BatchIdx& b) {
     const Slot& first = e->slots[b.slot[0]];
     size_t pages = first.blocks.size();
@@ -922,7 +923,8 @@ static int shared_prefix_tokens(const b2_engine* e, const BatchIdx& b) {
         pages = same;
     }
     const int tokens = (int)pages * e->cfg.kv_block_tokens;
-    return e->attn_mma != 0 && tokens >= SHARED_MIN_TOKENS ? tokens : 0;
+    const bool worth = b.n * (e->cfg.n_head / e->cfg.n_head_kv) <= 16 ? tokens >= 128 : (long)tokens * b.n >= 16384;
+    return e->attn_mma != 0 && worth ? tokens : 0;
 }
 
 // One decode step for b.n sequences at once: the weights are read (and dequantised) once for all of them by the
@@ -974,7 +976,7 @@ static int batch_step(b2_engine* e, const BatchIdx& b, const BatchTokens& set, i
             x.n_head = c.n_head; x.n_kv = c.n_head_kv; x.head_dim = hd; x.type = ELEM_F16; x.scale_log2 = a.scale * 1.4426950408889634f;
             x.tab = e->slot_tab; x.slots = b; x.out_h = e->pf_att; x.out_T_pad = T_pad; x.err = a.err;
             CK(shared_prefix_launch(x, st));
-            e->launches += 2;
+            e->launches += shared_prefix_launches(x) - 1;
         } else if (e->attn_mma != 0) {      // the tensor-core kernel writes f16 in the o-projection GEMM's operand order itself
             a.out_h = e->pf_att; a.out_T_pad = T_pad;
             CK(attn_decode_mma_launch(a, e->slot_tab, &b, st, false));

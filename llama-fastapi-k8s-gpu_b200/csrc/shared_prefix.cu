@@ -1,13 +1,19 @@
 // Attention of a batch over a paged cache whose first n_prefix tokens are the same pages for every sequence.
 //   keys of row i of a sequence with n rows and c own tokens: the prefix, and own tokens 0 .. c - n + i;   out = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m),
 //   s_j = scale log2(e) q.k_j. No key: 0.
-// The prefix is read once for all rows: its pass leaves (m, sum, weighted sum) of every row in 32 bits, the pass over the sequences' own tokens joins them.
-//
-// The prefix pass is shared_prefix_tc.cu (tensor memory) or, where the rows of a KV head fill no more than one tile of 64, the kernel here over the same
-// rows; the own pass is the kernel here. Here: mma.sync m16n8k16, tiles of 64 keys by tensor copies (a warp of its own) in 128-byte-swizzled rows. A row of the
-// tile is (token, head of the KV head's group). MT 16: a CTA's four warps take 16 keys of a tile each and are merged at the end, which is the form for single
-// tokens, bound by the cache's bytes; MT 64: a warp has 16 rows and all keys. The keys of a tile of rows are split over a cluster of up to eight CTAs, which
+// Bound by the bytes of the cache: the prefix is read once for all rows, each sequence's own tokens once for its rows. With a prefix every pass leaves partial
+// results (maximum, sum, weighted sum) of its keys in 32 bits, and a small kernel joins them; without one, the CTAs that share a tile's keys are a cluster and
 // join through each other's shared memory.
+//
+// Three forms of a pass. A row of a tile is (token, head of the KV head's group).
+//   up to 16 rows (single tokens): shared_prefix_step_kernel; the four computing warps share each tile of 64 keys. A CTA whose keys are done takes over the work
+//     of one that has not started, so that copies of the next sequence are under way while this one ends.
+//   up to 64 rows: shared_prefix_rows_kernel; a warp has 16 rows and all keys.
+//   more rows (the prefix of a batch): shared_prefix_tc.cu, on tensor memory.
+// Both kernels here: mma.sync m16n8k16, keys and values by tensor copies (a warp of its own) in 128-byte-swizzled rows. They are bound by the copies, not by
+// the products: 32 rows of 64 keys want 1 % of the tensor cores.
+// The pass over own tokens runs beside the prefix pass (which leaves SMs or memory idle). Up to 16 rows of a KV head in the whole batch: one launch for both.
+//
 // Probabilities are rounded to the cache's type for the weighted sum (the other operand is the cache as it is); scores, maxima, sums, joins stay 32-bit.
 #include "device_ops.h"
 #include "ptx.cuh"
@@ -780,6 +786,13 @@ size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim
     return (size_t)(sp_prefix_slots(n_rows, n_head, n_kv) + sp_own_slots(n_rows, n_head, n_kv)) * n_rows * n_head * (head_dim + 2);
 }
 
+// the prefix and the own tokens in one launch (grid.z: the sequences and the prefix)
+static bool sp_one_launch(const SharedPrefixArgs& a) {
+    const int G = a.n_head / a.n_kv;
+    return (long)a.r.n_rows * G <= 16 && a.max_rows * G <= 16 && a.r.n_seqs < 65535;
+}
+int shared_prefix_launches(const SharedPrefixArgs& a) { return a.n_prefix == 0 ? 1 : sp_one_launch(a) ? 2 : 3; }
+
 cudaError_t shared_prefix_error(unsigned int* code) {
     const cudaError_t e = cudaMemcpyFromSymbol(code, sp_error, sizeof(*code));
     return e == cudaSuccess && *code == 0 ? shared_prefix_tc_error(code) : e;
@@ -806,8 +819,7 @@ cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s) {
     own.splits = std::min(own.splits, (int)sp_own_slots(R, a.n_head, a.n_kv));      // (fewer sequences than their rows need: max_rows was too small)
     own.steal = single;
     if (few) own.slots = own.prefix_splits = sp_splits((long)a.n_kv, a.n_prefix, SP_PREFIX_SPLITS);
-    if (few && single && R * G <= 16) {
-        // the prefix and the own tokens in one launch
+    if (sp_one_launch(a)) {
         own.prefix_z = S;
         own.mrows = R * G;
         own.steal = 0;

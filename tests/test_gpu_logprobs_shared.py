@@ -138,7 +138,7 @@ def test_batched(native_lib, tmp_models, monkeypatch, slots):
 
 
 SHARED = [("tiny", "Q4_K_M", 1, 16, 140, 3), ("tiny128", "Q8_0", 6, 16, 128, 5), ("tiny128", "Q8_0", 6, 64, 200, 8), ("tiny", "Q4_K_M", 1, 16, 520, 17),
-          ("tiny128", "Q8_0", 6, 32, 900, 33), ("tiny", "Q4_K_M", 1, 64, 300, 66)]
+          ("tiny", "Q4_K_M", 1, 16, 980, 17), ("tiny128", "Q8_0", 6, 32, 900, 33), ("tiny", "Q4_K_M", 1, 64, 300, 66)]
 
 
 @pytest.mark.parametrize("arch,ftype,seed,bt,common,n", SHARED)
@@ -156,7 +156,7 @@ def test_batched_decoding_over_shared_pages(native_lib, tmp_models, monkeypatch,
     rest = [prompt_of(1 + (5 * i) % 23, 100 + i) for i in range(n)]
     forced = [prompt_of(4, 500 + i) for i in range(n)]
     whole = common // bt * bt
-    out = {}
+    out, launches = {}, {}
     for share in (False, True):
         eng = _engine(path, max_seqs=n, n_ctx=1024, bt=bt)
         for s in range(n):
@@ -173,10 +173,15 @@ def test_batched_decoding_over_shared_pages(native_lib, tmp_models, monkeypatch,
         for i in range(4):
             for s in range(n):
                 eng.set_token(s, forced[s][i])
+            before = eng.launch_count()
             eng.decode(list(range(n)))
+            launches[share] = eng.launch_count() - before
             got.append(np.stack([eng.logits(s).copy() for s in range(max(0, n - 64) if n > 64 else 0, n)]))      # (of more than 64 the last step's rows)
         out[share] = got
         eng.close()
+    group = {"tiny": 4, "tiny128": 2}[arch]
+    more = [0 if k * group > 16 and k * whole < 16384 else 1 if k * group <= 16 else 2 for k in ([n] if n <= 64 else [64, n - 64])]      # kernels a layer
+    assert launches[True] - launches[False] == 2 * sum(more)
     worst = max(np.abs(a - b).max() for a, b in zip(out[False], out[True]))
     assert worst <= LOGIT_TOL, worst
     ref = RefModel(path)
