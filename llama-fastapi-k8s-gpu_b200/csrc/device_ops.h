@@ -106,8 +106,13 @@ struct PrefixCut {
         return e < most ? e : most;
     }
 };
-PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix);
-cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, cudaStream_t s);      // ml_at: see SpPlan
+constexpr int PREFIX_SMS = 148;
+PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix, int sms);
+// What the prefix pass leaves to a pass of single own tokens, which runs beside it and is bound by other things: which of the cuts it takes goes by the mean of
+// the sequences' own tokens, 16 << level or fewer (the last: any). It writes {run, per_unit} into the workspace at cut_at.
+constexpr int SHARE_LEVELS = 8;
+struct PrefixShare { int adapt; size_t cut_at; int run[SHARE_LEVELS]; short ctas[SHARE_LEVELS], per_unit[SHARE_LEVELS]; };      // adapt 0: all SMs
+cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, const PrefixShare& share, cudaStream_t s);      // ml_at: see SpPlan
 
 // code of the first wait of these kernels that ran out on the current device (0: none); waits for the device
 cudaError_t shared_prefix_error(unsigned int* code);

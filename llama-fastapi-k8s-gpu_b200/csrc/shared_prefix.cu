@@ -81,6 +81,7 @@ struct SpPlan {
     int slots;                   // joining: partial results of the prefix per row (< 0: as `cut` says)
     PrefixCut cut;
     size_t ml_at;                // where the (maximum, sum) of the partial results lie in the workspace
+    PrefixShare share;           // adapt: the prefix pass has written down its cut
 };
 
 // partial results: [slot][row][head][head_dim] weighted sums, then [slot][row][head][2] (maximum in log2, sum)
@@ -657,7 +658,6 @@ __global__ void __launch_bounds__(SP_JOIN) shared_prefix_join_kernel(const Share
     const int per_row = (a.n_head * (HD / 4) + SP_JOIN - 1) / SP_JOIN, t = blockIdx.x / per_row, e = blockIdx.x % per_row * SP_JOIN + threadIdx.x;
     const int G = a.n_head / a.n_kv, head = e / (HD / 4), d = e % (HD / 4) * 4, kvh = head / G;
     const bool in = head < a.n_head;
-    const int slots = !in ? 0 : p.slots >= 0 ? p.slots : p.cut.slots(kvh * p.cut.pairs + (t * G + head - kvh * G) / 256), all = slots + p.splits;
     const size_t at = sp_part(a, 0, t, head), step = (size_t)a.r.n_rows * a.n_head;
     const float* ml = a.work + p.ml_at + at * 2;
     const float* from = a.work + at * HD + d;
@@ -668,6 +668,12 @@ __global__ void __launch_bounds__(SP_JOIN) shared_prefix_join_kernel(const Share
     }
     griddep_wait();
     griddep_launch();
+    PrefixCut cut = p.cut;
+    if (p.share.adapt) {
+        const int2 took = *reinterpret_cast<const int2*>(a.work + p.share.cut_at);
+        cut.run = took.x; cut.per_unit = took.y;
+    }
+    const int slots = !in ? 0 : p.slots >= 0 ? p.slots : cut.slots(kvh * cut.pairs + (t * G + head - kvh * G) / 256), all = slots + p.splits;
     float m = -INFINITY, l = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int j0 = 0; j0 < all; j0 += B) {                        // (behind the prefix's: the own tokens')
@@ -702,7 +708,7 @@ __global__ void __launch_bounds__(SP_JOIN) shared_prefix_join_kernel(const Share
 
 // ---------------------------------------------------------------- host side
 namespace {
-constexpr int SP_SMS = 148;
+constexpr int SP_SMS = PREFIX_SMS;
 constexpr size_t sp_smem(int hd, int mrows) { return (size_t)sp_stages(hd) * 2 * SP_TT * hd * 2 + 2 * mrows * (hd + 8) * 2 + 1024; }
 
 template <typename E, int HD>
@@ -757,25 +763,63 @@ constexpr int SP_PREFIX_SPLITS = 32, SP_OWN_SPLITS = 8;
 }  // namespace
 
 // Runs of equal length over all units laid end to end, or over every unit by itself where that makes them no more than three blocks longer: a run that goes on
-// into another unit loads queries, starts and ends its pipeline and writes its results twice, which takes as long as three blocks (6 us).
-PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix) {
+// into another unit loads queries, starts and ends its pipeline and writes its results twice, which takes as long as three blocks (6 us). For `sms` CTAs at most.
+PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix, int sms) {
     PrefixCut c = {};
     c.pairs = (int)((n_rows * (n_head / n_kv) + 255) / 256);
     c.units = n_kv * c.pairs;
     c.blocks = (n_prefix + 127) / 128;
-    const long total = (long)c.units * c.blocks;
-    c.run = (int)((total + SP_SMS - 1) / SP_SMS);
-    const int parts = c.units <= SP_SMS ? SP_SMS / c.units : 1, each = (c.blocks + parts - 1) / parts;
-    c.per_unit = c.run && c.units <= SP_SMS && each <= c.run + 3;
+    const unsigned total = (unsigned)c.units * (unsigned)c.blocks, s = (unsigned)sms;      // (31 bits: see PrefixCut)
+    c.run = (int)((total + s - 1) / s);
+    const int parts = c.units <= sms ? (int)(s / (unsigned)c.units) : 1, each = (c.blocks + parts - 1) / parts;
+    c.per_unit = c.run && c.units <= sms && each <= c.run + 3;
     if (c.per_unit) c.run = each;
-    c.ctas = c.run == 0 ? 0 : c.per_unit ? c.units * ((c.blocks + each - 1) / each) : (int)((total + c.run - 1) / c.run);
+    c.ctas = c.run == 0 ? 0 : c.per_unit ? c.units * ((c.blocks + each - 1) / each) : (int)((total + (unsigned)c.run - 1) / (unsigned)c.run);
     return c;
+}
+
+// The cuts that bring the prefix pass and the pass over single own tokens to an end soonest. A run of blocks takes FIXED us and BLOCK a block, NEXT
+// more for every unit that it goes on into; a CTA of the other pass (three an SM) takes ITEM us for a sequence and KV head and BYTES a MB, all of them together no
+// less than the memory gives. They have the SMs that the prefix pass leaves, and all from its end on.
+// Measured (32 heads over 8 KV heads of 128; with all SMs for the prefix, as given here): 256 samples of 1 to 512 own tokens behind 8192 103 -> 87 us, on 64 SMs
+// (on 96: 96, on 48: 119); 64 of 16 to 300 behind 8000 42 -> 34, on 88; behind 2000 35 -> 26, on 48; 64 of 16 to 1000 behind 8000 66 -> 50, on 56; 32 of 20 to
+// 500 behind 1000 22.5 -> 19.5, on 32.
+static void sp_share(const SharedPrefixArgs& a, PrefixShare& share) {
+    constexpr float FIXED = 8.f, BLOCK = 2.2f, NEXT = 6.f, ITEM = 4.5f, BYTES = 35.f, MEMORY = 5.f;      // MEMORY: MB a us
+    struct Choice { PrefixCut cut; float beside, ends; } c[16];
+    int n = 0;
+    for (int sms = PREFIX_SMS; sms > PREFIX_SMS - 8 * 16; sms -= 8) {
+        const PrefixCut t = prefix_cut(a.r.n_rows, a.n_head, a.n_kv, a.n_prefix, sms);
+        if (n && c[n - 1].cut.ctas == t.ctas && c[n - 1].cut.run == t.run) continue;
+        c[n].cut = t;
+        c[n].beside = 3.f * (PREFIX_SMS - t.ctas);
+        c[n++].ends = FIXED + BLOCK * t.run + (t.per_unit ? 0.f : NEXT * (float)((t.run + t.blocks - 2) / t.blocks));
+    }
+    const float items = (float)a.r.n_seqs * a.n_kv;
+    const long most = (long)a.r.max_pages * a.r.block_tokens;
+    for (int l = 0; l < SHARE_LEVELS; l++) {
+        const float mb = fmaxf(32.f, 0.72f * (16 << l)) * a.head_dim * 4e-6f, alone = ITEM + BYTES * mb;
+        float least = INFINITY;
+        int best = 0;
+        if (l > 0 && most <= 16 << (l - 1)) {                    // (no sequence can hold as much)
+            share.run[l] = share.run[l - 1]; share.ctas[l] = share.ctas[l - 1]; share.per_unit[l] = share.per_unit[l - 1];
+            continue;
+        }
+        for (int i = 0; i < n; i++) {                            // (of equals the one with most SMs)
+            const float item = fmaxf(alone, c[i].beside * (mb / MEMORY)), begun = c[i].beside * ceilf(c[i].ends / item);
+            const float total = begun < items ? c[i].ends + fmaxf(ceilf((items - begun) * (1.f / (3.f * PREFIX_SMS))) * alone, (items - begun) * (mb / MEMORY))
+                                              : fmaxf(c[i].ends, ceilf(items / c[i].beside) * item);
+            if (total < least) { least = total; best = i; }
+        }
+        share.run[l] = c[best].cut.run; share.ctas[l] = (short)c[best].cut.ctas; share.per_unit[l] = (short)c[best].cut.per_unit;
+    }
+    share.adapt = 1;
 }
 
 // most partial results that a row's prefix can have: a unit of b blocks in runs of ceil(u b / 148) lies in at most ceil(148 / u) + 1 of them
 static long sp_prefix_slots(long n_rows, int n_head, int n_kv) {
     if (n_rows * (n_head / n_kv) <= SP_PREFIX_ROWS) return SP_PREFIX_SPLITS;
-    const PrefixCut c = prefix_cut(n_rows, n_head, n_kv, 1);
+    const PrefixCut c = prefix_cut(n_rows, n_head, n_kv, 1, SP_SMS);
     return (SP_SMS + c.units - 1) / c.units + 1;
 }
 // and its own tokens: the splits of the fewest CTAs that so many rows can be
@@ -783,7 +827,7 @@ static long sp_own_slots(long n_rows, int n_head, int n_kv) {
     return sp_splits((n_rows * (n_head / n_kv) + 63) / 64 * n_kv, LONG_MAX, SP_OWN_SPLITS);
 }
 size_t shared_prefix_work_floats(long n_rows, int n_head, int n_kv, int head_dim) {
-    return (size_t)(sp_prefix_slots(n_rows, n_head, n_kv) + sp_own_slots(n_rows, n_head, n_kv)) * n_rows * n_head * (head_dim + 2);
+    return (size_t)(sp_prefix_slots(n_rows, n_head, n_kv) + sp_own_slots(n_rows, n_head, n_kv)) * n_rows * n_head * (head_dim + 2) + 4;      // (and the cut that the prefix pass took)
 }
 
 // the prefix and the own tokens in one launch (grid.z: the sequences and the prefix)
@@ -801,7 +845,7 @@ cudaError_t shared_prefix_error(unsigned int* code) {
 cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s) {
     const int R = a.r.n_rows, G = a.n_head / a.n_kv, S = a.r.n_seqs;
     if (R == 0 || S == 0) return cudaSuccess;
-    if ((long)prefix_cut(R, a.n_head, a.n_kv, 1).units * ((a.n_prefix + 127) / 128) > INT_MAX / 2) return cudaErrorInvalidValue;
+    if ((long)prefix_cut(R, a.n_head, a.n_kv, 1, SP_SMS).units * ((a.n_prefix + 127) / 128) > INT_MAX / 2) return cudaErrorInvalidValue;
     cudaError_t e;
     const bool few = (long)R * G <= SP_PREFIX_ROWS, single = a.max_rows * G <= 16, h = a.type == ELEM_F16;
     const int mt = single ? 16 : 64, tiles = (a.max_rows * G + mt - 1) / mt;
@@ -831,9 +875,11 @@ cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s) {
             p.steal = 0;
             e = sp_rows_of(a, p, false, dim3(p.prefix_splits, a.n_kv, 1), s, g_chain_pdl);
         } else {
-            own.cut = prefix_cut(R, a.n_head, a.n_kv, a.n_prefix);
+            own.cut = prefix_cut(R, a.n_head, a.n_kv, a.n_prefix, SP_SMS);
             own.slots = -1;
-            e = shared_prefix_tc_launch(a, own.cut, own.ml_at, s);
+            if (single) sp_share(a, own.share);
+            own.share.cut_at = shared_prefix_work_floats(R, a.n_head, a.n_kv, a.head_dim) - 4;
+            e = shared_prefix_tc_launch(a, own.cut, own.ml_at, own.share, s);
         }
         if (e != cudaSuccess) return e;
         own.behind = 1;

@@ -27,13 +27,35 @@ __device__ __forceinline__ uint32_t st_pack(float a, float b) {
     if constexpr (F16) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
     else { const __nv_bfloat162 h = __floats2bfloat162_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 }
+// the sequences' own tokens on average, as a level of PrefixShare (of very many sequences a sample's)
+__device__ __forceinline__ int st_level(const SharedPrefixArgs& a) {
+    __shared__ float part[ST_THREADS / 32];
+    const int n_seqs = a.r.n_seqs, step = (n_seqs + 1023) / 1024, most = a.r.max_pages * a.r.block_tokens;
+    float own = 0.f;
+#pragma unroll 1
+    for (int z = threadIdx.x * step; z < n_seqs; z += ST_THREADS * step) {
+        const int held = a.tab ? a.tab[a.slots.slot[z]].ints[1] + 1 - a.n_prefix : a.r.lengths[z];
+        own += (float)min(max(held, 0), most);
+    }
+#pragma unroll 1
+    for (int o = 16; o; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = own;
+    __syncthreads();
+    own = 0.f;
+#pragma unroll 1
+    for (int w = 0; w < ST_THREADS / 32; w++) own += part[w];
+    const float mean = own * step / n_seqs;
+    int level = 0;
+    while (level < SHARE_LEVELS - 1 && mean > (float)(16 << level)) level++;
+    return level;
+}
 }  // namespace
 
 cudaError_t shared_prefix_tc_error(unsigned int* code) { return cudaMemcpyFromSymbol(code, st_error, sizeof(*code)); }
 
 template <int HD, bool F16>
 __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                         const SharedPrefixArgs a, const PrefixCut cut, const int box_rows, const size_t ml_at) {
+                                                                         const SharedPrefixArgs a, const PrefixCut all_sms, const int box_rows, const size_t ml_at, const __grid_constant__ PrefixShare share) {
     constexpr int PARTS = HD / 64;
     extern __shared__ uint8_t st_smem[];
     __shared__ uint64_t q_full[2], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2];
@@ -43,6 +65,15 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
     uint8_t* qs = reinterpret_cast<uint8_t*>(((uintptr_t)st_smem + 1023) & ~(uintptr_t)1023);      // [tile][part]
     uint8_t* ks = qs + 2 * PARTS * ST_PART;                      // [stage][part]
     uint8_t* vs = ks + 2 * PARTS * ST_PART;
+    griddep_wait();
+    griddep_launch();
+    PrefixCut cut = all_sms;
+    if (share.adapt) {
+        const int level = st_level(a);
+        cut.run = share.run[level]; cut.per_unit = share.per_unit[level]; cut.ctas = share.ctas[level];
+        if (blockIdx.x == 0 && threadIdx.x == 0) *reinterpret_cast<int2*>(a.work + share.cut_at) = make_int2(cut.run, cut.per_unit);
+        if ((int)blockIdx.x >= cut.ctas) return;                 // (all threads alike)
+    }
     if (warp == 9) {
         if (lane == 0) {
             for (int i = 0; i < 2; i++) {
@@ -57,8 +88,6 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
     tc_before_sync();
     __syncthreads();
     tc_after_sync();
-    griddep_wait();
-    griddep_launch();
     const uint32_t s_at = __shfl_sync(0xffffffffu, tmem_at, 0), o_at = s_at + 256;      // (known to be uniform)
     const int G = a.n_head / a.n_kv, M = a.r.n_rows * G, n_prefix = a.n_prefix;
     const int x0 = cut.begin(blockIdx.x), x1 = cut.end(blockIdx.x);
@@ -320,7 +349,7 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
 
 // ---------------------------------------------------------------- host side
 template <int HD, bool F16>
-static cudaError_t st_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, cudaStream_t s) {
+static cudaError_t st_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, const PrefixShare& share, cudaStream_t s) {
     constexpr int parts = HD / 64, smem = 6 * parts * ST_PART + 1024;
     if (!allow_smem<shared_prefix_tc_kernel<HD, F16>>(smem)) return cudaErrorInvalidValue;
     int box = ST_K;
@@ -328,13 +357,13 @@ static cudaError_t st_launch(const SharedPrefixArgs& a, const PrefixCut& cut, si
     const long rows = a.r.n_pages * a.n_kv * a.r.block_tokens;
     CUtensorMap mk, mv;                                          // (copies move 16-bit entries whatever their format)
     if (!bf16_rows_map(&mk, a.k_pool, HD, rows, HD, 1, 0, box) || !bf16_rows_map(&mv, a.v_pool, HD, rows, HD, 1, 0, box)) return cudaErrorInvalidValue;
-    return launch_chain(shared_prefix_tc_kernel<HD, F16>, dim3(cut.ctas), dim3(ST_THREADS), smem, s, mk, mv, a, cut, box, ml_at);
+    return launch_chain(shared_prefix_tc_kernel<HD, F16>, dim3(share.adapt ? PREFIX_SMS : cut.ctas), dim3(ST_THREADS), smem, s, mk, mv, a, cut, box, ml_at, share);
 }
 
-cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, cudaStream_t s) {
+cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, const PrefixShare& share, cudaStream_t s) {
     if (a.r.block_tokens % 16 || cut.ctas < 1) return cudaErrorInvalidValue;
-    if (a.head_dim == 64) return a.type == ELEM_F16 ? st_launch<64, true>(a, cut, ml_at, s) : st_launch<64, false>(a, cut, ml_at, s);
-    if (a.head_dim == 128) return a.type == ELEM_F16 ? st_launch<128, true>(a, cut, ml_at, s) : st_launch<128, false>(a, cut, ml_at, s);
+    if (a.head_dim == 64) return a.type == ELEM_F16 ? st_launch<64, true>(a, cut, ml_at, share, s) : st_launch<64, false>(a, cut, ml_at, share, s);
+    if (a.head_dim == 128) return a.type == ELEM_F16 ? st_launch<128, true>(a, cut, ml_at, share, s) : st_launch<128, false>(a, cut, ml_at, share, s);
     return cudaErrorInvalidValue;
 }
 

@@ -168,6 +168,49 @@ def test_shared_prefix(ops, heads, kv, dim, page, typ, prefix, rows, own):
     assert torch.equal(got, shared(ops, c, q, prefix, rows))            # the same bits again
 
 
+# single tokens behind a longer prefix: how many SMs the prefix gets goes by the mean of the own tokens, in levels that end at powers of two
+SPLITS = [
+    (32, 8, 128, 64, "f16", 2000, [1] * 40, [0] * 40),
+    (32, 8, 128, 64, "bf16", 2000, [1] * 40, [16] * 40),
+    (32, 8, 128, 64, "f16", 2000, [1] * 40, [16] * 39 + [17]),
+    (32, 8, 128, 64, "f16", 3333, [1] * 24, [512] * 24),                # all at the end of a level, which is all that the table holds but a page
+    (8, 1, 64, 16, "bf16", 700, [1] * 1500, [i % 5 for i in range(1500)]),         # the mean is that of every other sequence
+    (8, 1, 64, 16, "f16", 130, [1] * 1500, [1 + 99 * (i & 1) for i in range(1500)]),
+    (16, 4, 64, 32, "bf16", 5000, [1] * 90, [2100 if i == 7 else 3 for i in range(90)]),
+    (32, 8, 128, 64, "f16", 129, [1] * 300, [2 * i for i in range(300)]),
+]
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,typ,prefix,rows,own", SPLITS)
+def test_shared_prefix_beside_own_tokens(ops, heads, kv, dim, page, typ, prefix, rows, own):
+    test_shared_prefix(ops, heads, kv, dim, page, typ, prefix, rows, own)
+
+
+def test_shared_prefix_lengths_that_change_between_replays(ops):
+    """Captured once: how the SMs are split goes by the lengths at the time of the replay."""
+    c = Cache(5, 8, 128, 64, "f16", 2500, [400] * 48)
+    q = torch.randn(48, 32, 128, generator=c.g).half().cuda()
+    lengths, out = c.ints(c.own), torch.empty_like(q)
+    work = torch.full((ops.attention_shared_prefix_workspace(48, 32, 8, 128) // 4,), math.nan, device="cuda")
+    row_start = c.ints(range(49))
+    run = lambda stream=None: ops.attention_shared_prefix(q, c.k, c.v, c.prefix_pages, 2500, c.pages, row_start, lengths, out, work, max_rows=1, stream=stream)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        run(s)
+        s.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            run(s)
+        for own in ([1] * 48, [400] * 48, [0] * 48, [8 * i for i in range(48)]):
+            lengths.copy_(c.ints(own))
+            g.replay()
+            s.synchronize()
+            c.own = own
+            want, spread, reach = attention_exact(c, q, 2500, [1] * 48)
+            assert ((out.to(F64) - want).abs() <= attention_bar("f16", want, spread, reach, 128)).all()
+
+
 def test_shared_prefix_rows_without_keys_and_behind_the_last(ops):
     c = Cache(1, 2, 64, 16, "f16", 0, [0, 3, 0])
     q = torch.randn(8, 4, 64, generator=c.g).half().cuda()
