@@ -186,6 +186,26 @@ def test_shared_prefix_beside_own_tokens(ops, heads, kv, dim, page, typ, prefix,
     test_shared_prefix(ops, heads, kv, dim, page, typ, prefix, rows, own)
 
 
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("at,by", [([128], 20.0), ([129, 161, 193, 225], 20.0), ([159, 191, 223, 255], 17.0), ([300, 400, 500, 600, 700, 800], 16.0), ([0, 895], 40.0),
+                                   ([511, 512, 544], 30.0), ([250, 600], -20.0), ([330], 130.0), ([840, 850, 870, 899], 15.0)])
+def test_shared_prefix_scores_that_grow(ops, typ, dim, at, by):
+    """Scores (in log2) that rise along the prefix by `by` at some keys, by a half or a quarter of it or not at all in some rows: what a CTA has summed up by
+    then, in every part of a block of 128 keys, has to fall by as much. 640 blocks: a CTA has several."""
+    P, S = 900, 600
+    c = Cache(dim + len(at), 8, dim, 64, typ, P, [1] * S)
+    q = torch.randn(S, 32, dim, generator=c.g).to(TYPES[typ]).cuda()
+    q[..., 0] = torch.tensor([[0.0, 0.25, 0.5, 1.0][(r + h) % 4] for r in range(S) for h in range(32)]).view(S, 32).to(TYPES[typ]).cuda()
+    step = by / math.log2(math.e) * dim ** 0.5                                          # what one step adds to q k
+    for j in range(P):
+        c.k[c.prefix_pages[j // 64].long(), :, j % 64, 0] = step * sum(j >= k for k in at)
+    got = shared(ops, c, q, P, [1] * S)
+    want, spread, reach = attention_exact(c, q, P, [1] * S)
+    ratio = (got.to(F64) - want).abs() / attention_bar(typ, want, spread, reach, dim)
+    assert (ratio <= 1).all(), float(ratio.max())
+
+
 def test_shared_prefix_lengths_that_change_between_replays(ops):
     """Captured once: how the SMs are split goes by the lengths at the time of the replay."""
     c = Cache(5, 8, 128, 64, "f16", 2500, [400] * 48)
