@@ -1,13 +1,14 @@
 // Log probabilities of given tokens, the entropy of every row, and its most likely tokens, from one pass over the logits.
 // With m the row's largest logit, L = log2 e, d_i = (x_i - m) L, S = sum 2^d_i, T = sum d_i 2^d_i:
-//   logprob(t) = (d_t - log2 S) / L,   entropy = (log2 S - T / S) / L.
+//   logprob(t) = x_t - m - log2 S / L,   entropy = (log2 S - T / S) / L.
 // Every thread keeps (m, S, T) of its entries, S and T against its own running maximum; they are joined over the CTA and, where a row has a cluster of CTAs, over
 // the cluster. A masked entry (-infinity) adds nothing; a row of nothing else gets log probabilities of -infinity and entropy 0; a NaN makes the row's
 // numbers NaN.
 //
-// The most likely tokens come from the same pass: a thread's running maximum bounds its entries. Of the maxima of 32 or 64 groups of threads the n-th largest is
-// reached by n entries at least, so that the n most likely are among the entries that reach it, which lie with the few threads whose maximum does; their entries
-// are read once more (from L2) and ranked by (value, lower id). Rows that would give too many of those (hundreds of equal entries) are searched n times instead.
+// The most likely tokens come from the same pass: a thread's running maximum bounds its entries. Of the maxima of 32 to 128 groups of threads (two to four times n)
+// the n-th largest is reached by n entries at least, so that the n most likely are among the entries that reach it, which lie with the few threads whose maximum
+// does; their entries are read once more (from L2) and ranked by (value, lower id). Where those are too many (thousands of equal entries, a row masked but for
+// a few), the ones above the bound are ranked and the equal ones taken in the order of their ids; what that does not settle is searched n times.
 //
 // Bound by memory for many rows (each logit read once), by the latency of the phases behind the pass for few.
 #include "device_ops.h"
@@ -19,9 +20,7 @@ namespace b2 {
 
 namespace {
 constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_UNROLL = 2;              // 16-byte pieces a thread has under way (four, and five CTAs an SM: 1024 rows of 128256 110 instead of 92 us)
 constexpr int LP_CAND = 1024;             // entries that may be ranked
-constexpr int LP_SEL = 128;               // threads whose entries are read again
 constexpr float LP_LOG2E = 1.4426950408889634f, LP_LN2 = 0.6931471805599453f;
 constexpr float LP_FLOOR = -200.f;        // 2^-200 is 0 in 32 bits: keeps d 2^d of a masked entry from being infinity times 0
 
@@ -79,8 +78,9 @@ struct Pieces {
 
 struct LpShared {
     Sums sums[LP_WARPS], cta;
-    unsigned group[64], bound;
-    int n_sel, n_cand, n_own, sel[LP_SEL];
+    alignas(16) unsigned group[128];
+    unsigned bound;
+    int n_sel, n_cand, n_own, sel[LP_THREADS], warp_ties[LP_WARPS];
     unsigned long long cand[LP_CAND], own[LOGPROB_MAX_TOP], wbest[LP_WARPS];
 };
 
@@ -108,9 +108,9 @@ __device__ __forceinline__ unsigned long long lp_cluster_key(uint32_t address) {
 __device__ __forceinline__ uint32_t lp_cluster_rank() { uint32_t r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 }  // namespace
 
-// cluster of `parts` CTAs a row (1: none)
-template <typename T>
-__global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobArgs a, const RowMap map, int parts) {
+// cluster of `parts` CTAs a row (1: none); LP_UNROLL 16-byte pieces a thread has under way
+template <typename T, int LP_UNROLL, int CTAS>
+__global__ void __launch_bounds__(LP_THREADS, CTAS) logprobs_kernel(const LogprobArgs a, const RowMap map, int parts) {
     constexpr int VEC = 16 / sizeof(T);
     __shared__ LpShared sh;
     __shared__ unsigned long long all[8 * LOGPROB_MAX_TOP];
@@ -154,11 +154,11 @@ __global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobAr
         v = {m, s, t};
     }
     const unsigned mine = pc.n > tid ? lp_key(v.m) : 0u;
-    if (a.n_top > 0) {                                            // maxima of groups of four (eight) threads
+    const int size = a.n_top <= 16 ? 8 : a.n_top <= 32 ? 4 : 2, n_groups = LP_THREADS / size;
+    if (a.n_top > 0) {                                            // maxima of groups of `size` threads
         unsigned g = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
-        g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
-        if (a.n_top <= 32) g = max(g, __shfl_xor_sync(0xffffffffu, g, 4));
-        const int size = a.n_top <= 32 ? 8 : 4;
+        if (size >= 4) g = max(g, __shfl_xor_sync(0xffffffffu, g, 2));
+        if (size >= 8) g = max(g, __shfl_xor_sync(0xffffffffu, g, 4));
         if (tid % size == 0) sh.group[tid / size] = g;
     }
     const Sums w = lp_join_warp(v);
@@ -170,45 +170,75 @@ __global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobAr
         if (lane == 0) sh.cta = j;
     }
     if (a.n_top > 0 && top > 0) {
-        // ---- the top-th largest of the groups' maxima (of 32 or 64, equal ones in any order; 0 where fewer groups have entries)
-        if (warp == 0) {
-            const unsigned g0 = sh.group[lane], g1 = a.n_top <= 32 ? 0u : sh.group[lane + 32];
-            int above0 = 0, above1 = 0;
-#pragma unroll 8
-            for (int i = 0; i < 32; i++) {
-                const unsigned o0 = __shfl_sync(0xffffffffu, g0, i), o1 = __shfl_sync(0xffffffffu, g1, i);
-                above0 += (o0 > g0 || (o0 == g0 && i < lane)) + (o1 > g0);
-                above1 += (o0 > g1 || o0 == g1) + (o1 > g1 || (o1 == g1 && i < lane));
+        // ---- the top-th largest of the groups' maxima (equal ones in the groups' order; 0 where fewer groups have entries)
+        if (tid < n_groups) {
+            const unsigned g = sh.group[tid];
+            int above = 0;
+            for (int i = 0; i < n_groups; i += 4) {
+                const uint4 o = *reinterpret_cast<const uint4*>(&sh.group[i]);
+                above += (o.x > g || (o.x == g && i < tid)) + (o.y > g || (o.y == g && i + 1 < tid)) + (o.z > g || (o.z == g && i + 2 < tid)) + (o.w > g || (o.w == g && i + 3 < tid));
             }
-            if (above0 == top - 1) sh.bound = g0;
-            else if (above1 == top - 1) sh.bound = g1;
+            if (above == top - 1) sh.bound = g;
         }
         __syncthreads();
         const unsigned bound = sh.bound;
-        if (mine >= bound && pc.n > tid) {
-            const int i = atomicAdd(&sh.n_sel, 1);
-            if (i < LP_SEL) sh.sel[i] = tid;
-        }
-        __syncthreads();
-        const int n_sel = sh.n_sel, rounds = (pc.n + LP_THREADS - 1) / LP_THREADS;
-        if (n_sel <= LP_SEL) {
+        const int rounds = (pc.n + LP_THREADS - 1) / LP_THREADS;
+        // the entries whose keys are `from` or larger, as far as there is room
+        auto collect = [&](unsigned from) {
+            if (mine >= from && pc.n > tid) sh.sel[atomicAdd(&sh.n_sel, 1)] = tid;
+            __syncthreads();
+            const int n_sel = sh.n_sel;
             for (int i = tid; i < n_sel * rounds; i += LP_THREADS) {
                 const int p = sh.sel[i % n_sel] + i / n_sel * LP_THREADS;
                 const uint4 x = pc.load(p);
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
                     const int id = pc.first(p) + e;
-                    if (lp_key(pc.at(x, e)) >= bound && pc.id_ok(id)) {
+                    if (lp_key(pc.at(x, e)) >= from && pc.id_ok(id)) {
                         const int at = atomicAdd(&sh.n_cand, 1);
                         if (at < LP_CAND) sh.cand[at] = lp_rank_key(pc.at(x, e), id);
                     }
                 }
             }
             __syncthreads();
+        };
+        auto rank = [&](int want) { lp_rank(sh.cand, sh.n_cand, want, [&](int place, unsigned long long k) { sh.own[place] = k; }); };
+        collect(bound);
+        bool found = sh.n_cand <= LP_CAND && sh.n_cand >= top;    // (fewer: NaNs, which reach no bound)
+        if (found) rank(top);
+        else if (bound < 0xffffffffu) {
+            // too many equal entries: those above the bound, then the ones at it in the order of their ids
+            __syncthreads();
+            if (tid == 0) sh.n_sel = sh.n_cand = 0;
+            __syncthreads();
+            collect(bound + 1);
+            int at = sh.n_cand;
+            if (at <= LP_CAND) {
+                rank(top);
+                for (int p0 = 0; at < top && p0 < pc.n; p0 += LP_THREADS) {
+                    const uint4 x = pc.load(p0 + tid);
+                    int ties = 0;
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) ties += lp_key(pc.at(x, e)) == bound && pc.id_ok(pc.first(p0 + tid) + e);
+                    int before = ties;
+#pragma unroll
+                    for (int o = 1; o < 32; o <<= 1) { const int up = __shfl_up_sync(0xffffffffu, before, o); if (lane >= o) before += up; }
+                    if (lane == 31) sh.warp_ties[warp] = before;
+                    __syncthreads();
+                    before += at - ties;
+                    for (int i = 0; i < LP_WARPS; i++) { if (i < warp) before += sh.warp_ties[i]; at += sh.warp_ties[i]; }
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        const int id = pc.first(p0 + tid) + e;
+                        if (before < top && lp_key(pc.at(x, e)) == bound && pc.id_ok(id)) sh.own[before++] = lp_rank_key(pc.at(x, e), id);
+                    }
+                    __syncthreads();
+                }
+                found = at >= top;
+            }
         }
-        if (n_sel <= LP_SEL && sh.n_cand <= LP_CAND && sh.n_cand >= top) {      // (fewer: NaNs, which reach no bound)
-            lp_rank(sh.cand, sh.n_cand, top, [&](int rank, unsigned long long k) { sh.own[rank] = k; });
-        } else {
+        if (!found) {
+            __syncthreads();
             // many equal entries or NaNs: one search per place, below the key of the place before
             unsigned long long below = ~0ull;
             for (int place = 0; place < top; place++) {
@@ -267,7 +297,7 @@ __global__ void __launch_bounds__(LP_THREADS, 8) logprobs_kernel(const LogprobAr
         cluster_sync();
     }
     const float log2_s = log2f(total.s), ref = total.m == -INFINITY ? 0.f : total.m;
-    auto logprob = [&](float x) { return ((x - ref) * LP_LOG2E - log2_s) * LP_LN2; };
+    auto logprob = [&](float x) { return (x - ref) - log2_s * LP_LN2; };      // (not in powers of two: the type's lowest value stays finite)
     const bool none = total.s == 0.f;                              // every entry masked
     if (a.n_top > 0) {
         float* lp = a.top_logprob + (long)to * a.n_top;
@@ -298,7 +328,10 @@ static cudaError_t logprobs_typed(const LogprobArgs& a, const RowMap& map, cudaS
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = parts; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, a, map, parts);
+    // Four CTAs an SM hold all of them: twice as many pieces under way a thread. 32 rows of 128256 14.3 -> 13.1 us, 128 25.7 -> 22.6, 500 of 32003 in bf16 15.1 ->
+    // 14.4; more rows want the CTAs instead (1024 of 128256: 98 that way, 92 with eight CTAs an SM).
+    if (cfg.gridDim.x <= 4 * 148) return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, 4, 4>, a, map, parts);
+    return cudaLaunchKernelEx(&cfg, logprobs_kernel<T, 2, 8>, a, map, parts);
 }
 
 cudaError_t logprobs_launch(const LogprobArgs& a, cudaStream_t s, const RowMap* map) {

@@ -362,6 +362,54 @@ def test_logprobs_ties_masks_and_extremes(ops, R):
     assert (lp == 0).all() and (h == 0).all() and (ti == torch.tensor([100, V - 1, V - 2, V - 3], device="cuda")).all()
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("top", [1, 16, 17, 33, 64])
+@pytest.mark.parametrize("R", [1, 9, 300, 700])
+def test_logprobs_of_rows_with_thousands_of_equal_entries(ops, R, top, typ):
+    """Masked but for a few (more and fewer than are asked for), the rest at the type's lowest value, ties for the first places, ties at the end of the row: the
+    lowest ids come first. Values are whole, so that they tie in 16 bits too."""
+    V = 20011
+    g = torch.Generator(device="cuda")
+    g.manual_seed(R + top)
+    lowest = torch.finfo(TYPES[typ]).min
+    x = torch.empty(R, V, device="cuda")
+    noise = torch.randint(-30, 0, (R, V), device="cuda", generator=g).float()
+    kinds = ["masked", "lowest", "ties above", "ties at the end", "steps", "few and ties"]
+    for r in range(R):
+        kind = kinds[r % len(kinds)]
+        if kind in ("masked", "lowest"):
+            x[r] = -math.inf if kind == "masked" else lowest
+            few = torch.randperm(V, device="cuda", generator=g)[:[0, 3, 40, 1][r // len(kinds) % 4]]
+            x[r, few] = torch.arange(few.numel(), device="cuda").float() // 2
+        elif kind == "ties above":
+            x[r] = torch.where(noise[r] > -10, 5.0, noise[r])
+        elif kind == "ties at the end":
+            x[r] = -20.0
+            x[r, V - 3000:] = 2.0
+            x[r, V // 2] = 3.0
+        elif kind == "steps":
+            x[r] = -(torch.arange(V, device="cuda") // 4000).float()
+        else:
+            x[r] = -50.0
+            x[r, ::5] = 1.0
+            x[r, 11::4001] = 9.0
+    x = x.to(TYPES[typ])
+    tokens = torch.randint(0, V, (R,), device="cuda", generator=g, dtype=torch.int32)
+    lp, h, tl, ti = logprobs(ops, x, tokens, top)
+    _, _, _, ids = logprobs_exact(x, tokens, top)
+    empty = (x == -math.inf).all(1)                                     # (what such a row gives is tested above)
+    # (below the maximum first: next to the lowest value of 32 bits, 3.4e38, the logarithm of a sum is lost in 64 bits too, whose unit is 3.8e22 there)
+    d = x.to(F64) - x.to(F64).amax(1, keepdim=True)
+    full = d - d.exp().sum(1, keepdim=True).log()
+    entropy = -torch.where(full > -700.0, full.exp() * full, 0.0).sum(1)
+    want, top_lp = full.gather(1, tokens.long()[:, None])[:, 0], full.gather(1, ids)
+    assert torch.equal(ti.long(), ids)
+    ok = lambda a, b, bar: (a.to(F64) == b) | ((a.to(F64) - b).abs() <= bar)
+    bar, bar_h = logprob_bar(x, want.nan_to_num(neginf=0.0), entropy, V)
+    assert (ok(lp, want, bar) | empty).all() and (ok(h, entropy, bar_h) | empty).all()
+    assert (ok(tl, top_lp, logprob_bar(x, top_lp.nan_to_num(neginf=0.0), entropy[:, None], V)[0]) | empty[:, None]).all()
+
+
 def test_logprobs_no_numbers(ops):
     x = torch.zeros(3, 1000, device="cuda")
     x[0, 500] = math.nan
