@@ -6,6 +6,9 @@
 // two outputs. While one tile's softmax runs, the other's products do; the second product starts with the first half of the probabilities. Warps 0-3 and 4-7:
 // softmax of a tile, a thread a row, scores read from tensor memory twice (maximum, then exponentials); 8: copies; 9: matrix instructions.
 // The output is rescaled only where a row's maximum has grown by more than 2^8 (probabilities are then up to 2^8, sums stay 32-bit).
+// Bound by the chain of a tile (scores, maximum, exponentials, second product: 1.8 us a block, of which the tensor cores take 1.1 with heads of 128 and the
+// exponentials' unit 1.1), in which every instruction of the issuing warp counts. One pass over the scores with a vote every 32 whether the reference still
+// serves took a fifth longer, a third score tile for heads of 64 a tenth.
 #include "device_ops.h"
 #include "ptx.cuh"
 #include "tc05.cuh"
@@ -136,20 +139,22 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
         // ================= matrix instructions (all lanes run the loop, one issues)
         const uint32_t f16 = F16 ? ~((1u << 7) | (1u << 10)) : ~0u;      // (tc_idesc_bf16 without the bits that say bf16)
         const uint32_t id_s = tc_idesc_bf16(ST_ROWS, ST_K) & f16, id_o = tc_idesc_bf16(ST_ROWS, HD, true) & f16;
-        const uint32_t qa = smem_u32(qs), ka = smem_u32(ks), va = smem_u32(vs);
+        const uint64_t dq0 = tc_desc(smem_u32(qs)), dk0 = tc_desc(smem_u32(ks)), dv0 = tc_desc(smem_u32(vs), ST_PART);
         int it = 0, segs[2] = {0, 0}, done[2] = {0, 0};          // blocks of the CTA, segments and blocks of each tile so far
         for (int x = x0; x < x1;) {
             const Segment g = segment(x);
             x += g.n;
             const int tiles = g.two ? 2 : 1;
             auto scores = [&](int t, int at) {
-                const uint64_t dq = tc_desc(qa + t * PARTS * ST_PART), dk = tc_desc(ka + (at & 1) * PARTS * ST_PART);
+                const uint64_t dq = dq0 + t * (PARTS * ST_PART >> 4), dk = dk0 + (at & 1) * (PARTS * ST_PART >> 4);
 #pragma unroll
                 for (int c = 0; c < PARTS; c++) tc_mma4_one<2, 2>(s_at + t * ST_K, dq + c * (ST_PART >> 4), dk + c * (ST_PART >> 4), id_s, c ? 1u : 0u);
                 tc_commit_one(&s_full[t]);
             };
             mbar_wait_warp(&k_full[it & 1], (it >> 1) & 1, err, 0x90002u, (unsigned)it);
-            for (int t = 0; t < tiles; t++) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {                        // (unrolled: which tile it is costs no instructions)
+                if (t == tiles) break;
                 mbar_wait_warp(&q_full[t], segs[t]++ & 1, err, 0x90003u, (unsigned)it);
                 tc_after_sync();
                 scores(t, it);
@@ -167,8 +172,10 @@ __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const _
                     fence_proxy_async();
                     __syncwarp();
                 }
-                const uint64_t dv = tc_desc(va + (at & 1) * PARTS * ST_PART, ST_PART);
-                for (int t = 0; t < tiles; t++) {
+                const uint64_t dv = dv0 + (at & 1) * (PARTS * ST_PART >> 4);
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    if (t == tiles) break;
                     auto sums = [&](int k0, int k1) {            // 16-key steps k0 .. k1 - 1 of the block
                         if (k1 - k0 == 4) tc_mma4_ts_one<8, 128>(o_at + t * HD, s_at + t * ST_K + k0 * 8, dv + k0 * 128, id_o, (i | k0) ? 1u : 0u);
                         else for (int k = k0; k < k1; k++) tc_mma_ts_one(o_at + t * HD, s_at + t * ST_K + k * 8, dv + k * 128, id_o, (i | k) ? 1u : 0u);
