@@ -99,6 +99,16 @@ def check_token(req: Request, vocab: Vocab, tok: int) -> bool:
     return False
 
 
+def common_prefix(a: List[int], b: List[int]) -> int:
+    """How many tokens two sequences begin with alike."""
+    n, most = 0, min(len(a), len(b))
+    while n + 64 <= most and a[n:n + 64] == b[n:n + 64]:
+        n += 64
+    while n < most and a[n] == b[n]:
+        n += 1
+    return n
+
+
 class Scheduler:
     RUN_AHEAD = 8
     ADMIT_PER_STEP = 2     # while sequences are decoding, at most this many new prompts are processed between two decode steps
@@ -240,22 +250,14 @@ class Scheduler:
     def _admit(self, req: Request):
         free = [s for s in self.slots if s.req is None]
 
-        def lcp(a, b):
-            n = 0
-            for x, y in zip(a, b):
-                if x != y:
-                    break
-                n += 1
-            return n
-
-        same = lambda s: min(lcp(s.cached, req.prompt), len(req.prompt) - 1)
-        slot = max(free, key=same)
-        n_keep, other = same(slot), None
+        reuse = {s.idx: min(common_prefix(s.cached, req.prompt), len(req.prompt) - 1) for s in (self.slots if self.share_prefix else free)}
+        slot = max(free, key=lambda s: reuse[s.idx])
+        n_keep, other = reuse[slot.idx], None
         eng = self.engine
         if self.share_prefix:
             # a running sequence has a page or more of the prompt that no free slot has: begin with its pages, in the free slot with the least to lose
-            best = max(self.slots, key=same)
-            whole = same(best) // eng.block_tokens * eng.block_tokens
+            best = max(self.slots, key=lambda s: reuse[s.idx])
+            whole = reuse[best.idx] // eng.block_tokens * eng.block_tokens
             if whole >= n_keep + eng.block_tokens:
                 slot, n_keep, other = min(free, key=lambda s: len(s.cached)), whole, best
         slot.req = req

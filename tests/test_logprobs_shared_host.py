@@ -200,3 +200,15 @@ def test_a_request_that_fails_gives_shared_pages_back(tiny_path, monkeypatch):
     PagedFake.delay = 0.0
     assert results and out["usage"]["completion_tokens"] == 3 and PagedFake.wrong is None
     llm.close()
+
+
+def test_common_prefix():
+    from llama_cpp.scheduler import common_prefix
+    rng = np.random.default_rng(0)
+    for n in (0, 1, 63, 64, 65, 128, 200):
+        a = [int(t) for t in rng.integers(0, 9, size=n)]
+        assert common_prefix(a, list(a)) == common_prefix(a, a + [1]) == common_prefix(a + [2], a) == n
+        for i in range(0, n, 7):
+            b = list(a)
+            b[i] += 10
+            assert common_prefix(a, b) == common_prefix(b, a) == i
