@@ -10,7 +10,8 @@
 // does; their entries are read once more (from L2) and ranked by (value, lower id). Where those are too many (thousands of equal entries, a row masked but for
 // a few), the ones above the bound are ranked and the equal ones taken in the order of their ids; what that does not settle is searched n times.
 //
-// Bound by memory for many rows (each logit read once), by the latency of the phases behind the pass for few.
+// Bound by memory for many rows (each logit read once: 1024 rows of 128256 in 32 bits 93 us, 5.65 TB/s), by the latency of the phases behind the pass for few
+// (32 rows 13 us, of which the pass is 4; one row of 32000 7.6).
 #include "device_ops.h"
 #include "ptx.cuh"
 #include <cuda_bf16.h>

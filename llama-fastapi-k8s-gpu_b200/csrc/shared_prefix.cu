@@ -8,7 +8,7 @@
 // Three forms of a pass. A row of a tile is (token, head of the KV head's group).
 //   up to 16 rows (single tokens): shared_prefix_step_kernel; the four computing warps share each tile of 64 keys. A CTA whose keys are done takes over the work
 //     of one that has not started, so that copies of the next sequence are under way while this one ends.
-//   up to 64 rows: shared_prefix_rows_kernel; a warp has 16 rows and all keys.
+//   up to 32 rows of the batch, or several tokens of a sequence: shared_prefix_rows_kernel; tiles of 64 rows, a warp has 16 of them and all keys.
 //   more rows (the prefix of a batch): shared_prefix_tc.cu, on tensor memory.
 // Both kernels here: mma.sync m16n8k16, keys and values by tensor copies (a warp of its own) in 128-byte-swizzled rows. They are bound by the copies, not by
 // the products: 32 rows of 64 keys want 1 % of the tensor cores.
@@ -297,7 +297,8 @@ __device__ __forceinline__ void sp_end(const SpPlan& p) { if (p.behind) { gridde
 // Single tokens: a tile of up to 16 rows (the group's heads, a few tokens), the four computing warps share a tile of keys. Scores: a warp has 16 keys; maxima and
 // probabilities go through shared memory; weighted sums: a warp has a quarter of the dims and all 64 keys, so that nothing has to be merged at the end.
 // What a CTA waits for before its first keys are here takes as long as the keys of some 100 tokens (3 us): CTAs that run go on with the work of those that have not
-// started (p.steal), and their copies run ahead into it.
+// started (p.steal), and their copies run ahead into it. 256 sequences, 8 KV heads of 128, no prefix: of 256 tokens 50 us (5.4 TB/s), of 512 85 us (6.35), of 64
+// 24 us (2.8: nearly all of it what a CTA waits for, 3.8 us a sequence).
 // grid: (tile * splits + split, KV head, sequence), the prefix's CTAs among them (p.prefix_z) where its rows are as few
 template <typename E, int HD>
 __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedPrefixArgs a,
@@ -511,7 +512,8 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
     sp_end(p);
 }
 
-// Several tokens of a sequence, or the prefix pass of up to 64 rows: a tile of 64 rows, a warp has 16 of them and all keys.
+// Several tokens of a sequence, or the prefix pass of up to 32 rows: a tile of 64 rows, a warp has 16 of them and all keys. Own tokens of 40 sequences of 3 to 33
+// rows, 32 heads over 4 of 64: 13.5 us, most of it beside the prefix pass.
 // grid: (tile * splits + split, KV head, sequence, or prefix)
 template <typename E, int HD>
 __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedPrefixArgs a,
@@ -649,7 +651,8 @@ __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const
 }
 
 // The partial results of the prefix and of the own tokens, joined: a thread four dims of a row and head, all of whose reads
-// are under way at once (up to eight results; four CTAs' worth of one row in one CTA, three results at a time, took 12 us).
+// are under way at once (up to eight results; four CTAs' worth of one row in one CTA, three results at a time, took 12 us). 256 rows of 32 heads of 128 with
+// three results each: 8 us, 64 rows with ten: 7.
 constexpr int SP_JOIN = 128;
 template <typename E, int HD>
 __global__ void __launch_bounds__(SP_JOIN) shared_prefix_join_kernel(const SharedPrefixArgs a, const SpPlan p) {
@@ -758,7 +761,10 @@ int sp_splits(long tiles, long keys, int most) {
     while (2 * n <= most && tiles * n * 2 <= 2 * SP_SMS && keys / (2 * n) >= SP_TT) n *= 2;
     return n;
 }
-constexpr int SP_PREFIX_ROWS = 64;          // up to so many rows a KV head the prefix is read by the kernels above
+// Up to so many rows a KV head the prefix is read by the kernels above, more by the pass on tensor memory. 32 heads over 8 KV heads of 128, prefixes of 512, 2000
+// and 8000, own tokens 20 to 500, these kernels / tensor memory: 20 rows 10.4 / 14.3, 17.7 / 18.6, 24.9 / 22.9 us; 32 rows 11.0 / 15.1, 18.0 / 19.5, 26.6 / 25.8;
+// 64 rows 14.9 / 15.0, 22.0 / 18.6, 34.7 / 27.1.
+constexpr int SP_PREFIX_ROWS = 32;
 constexpr int SP_PREFIX_SPLITS = 32, SP_OWN_SPLITS = 8;
 }  // namespace
 
