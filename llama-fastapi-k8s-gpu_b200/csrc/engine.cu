@@ -913,6 +913,7 @@ static int ensure_batch_workspace(b2_engine* e) {
 // from about 16384 tokens in all: 8 sequences behind 1024 tokens 0.4, 4096: 20; 16 behind 512 -2, 1024: 4, 4096: 41; 32 behind 256 -5, 512: 2, 4096: 83;
 // 64 behind 128 -5, 256: 1, 512: 15, 4096: 180. Where prefix and own tokens are one launch (16 rows a KV head): 4 behind 128 0.6, 4096: 8.
 static int shared_prefix_tokens(const b2_engine* e, const BatchIdx& b) {
+    if (b.n < 2) return 0;
     const Slot& first = e->slots[b.slot[0]];
     size_t pages = first.blocks.size();
     for (int i = 0; i < b.n && pages; i++) {
