@@ -909,9 +909,9 @@ static int ensure_batch_workspace(b2_engine* e) {
 }
 
 // Tokens at the start that all sequences of a batched step have in the same pages (whole pages; the token that the step writes lies behind them). 0: reading
-// them once is not worth the launches. Measured per layer (32 heads over 8 KV heads of 128; saved, us): three launches instead of one cost about 9 us, won back
-// from about 16384 tokens in all: 8 sequences behind 1024 tokens 0.4, 4096: 20; 16 behind 512 -2, 1024: 4, 4096: 41; 32 behind 256 -5, 512: 2, 4096: 83;
-// 64 behind 128 -5, 256: 1, 512: 15, 4096: 180. Where prefix and own tokens are one launch (16 rows a KV head): 4 behind 128 0.6, 4096: 8.
+// them once is not worth the launches. Measured per layer (32 heads over 8 KV heads of 128; saved, us): three launches instead of one cost about 7 us, won back
+// from about 16384 tokens in all: 8 sequences behind 512 tokens -1.3, 1024: 1.4, 4096: 19; 16 behind 512 -1.7, 1024: 3.5, 4096: 36; 32 behind 256 -7, 512: -0.9,
+// 1024: 13, 4096: 87; 64 behind 128 -7, 256: -0.5, 512: 13, 4096: 183. Where prefix and own tokens are one launch (16 rows a KV head): 4 behind 128 0.9, 4096: 6.
 static int shared_prefix_tokens(const b2_engine* e, const BatchIdx& b) {
     if (b.n < 2) return 0;
     const Slot& first = e->slots[b.slot[0]];

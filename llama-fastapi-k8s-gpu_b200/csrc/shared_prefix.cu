@@ -784,8 +784,8 @@ PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix, int sms) {
     return c;
 }
 
-// The cuts that bring the prefix pass and the pass over single own tokens to an end soonest. A run of blocks takes FIXED us and BLOCK a block, NEXT
-// more for every unit that it goes on into; a CTA of the other pass (three an SM) takes ITEM us for a sequence and KV head and BYTES a MB, all of them together no
+// The cuts that bring the prefix pass and the pass over single own tokens to an end soonest. A run of blocks takes FIXED us and BLOCK a block (1.8
+// by itself, 2.2 beside the other pass), NEXT more for every unit that it goes on into; a CTA of the other pass (three an SM) takes ITEM us for a sequence and KV head and BYTES a MB, all of them together no
 // less than the memory gives. They have the SMs that the prefix pass leaves, and all from its end on.
 // Measured (32 heads over 8 KV heads of 128; with all SMs for the prefix, as given here): 256 samples of 1 to 512 own tokens behind 8192 103 -> 87 us, on 64 SMs
 // (on 96: 96, on 48: 119); 64 of 16 to 300 behind 8000 42 -> 34, on 88; behind 2000 35 -> 26, on 48; 64 of 16 to 1000 behind 8000 66 -> 50, on 56; 32 of 20 to
