@@ -908,40 +908,66 @@ static int ensure_batch_workspace(b2_engine* e) {
     return B2_OK;
 }
 
-// Tokens at the start that all sequences of a batched step have in the same pages (whole pages; the token that the step writes lies behind them). 0: reading
-// them once is not worth the launches. Measured per layer (32 heads over 8 KV heads of 128; saved, us): three launches instead of one cost about 7 us, won back
-// from about 16384 tokens in all: 8 sequences behind 512 tokens -1.3, 1024: 1.4, 4096: 19; 16 behind 512 -1.7, 1024: 3.5, 4096: 36; 32 behind 256 -7, 512: -0.9,
-// 1024: 13, 4096: 87; 64 behind 128 -7, 256: -0.5, 512: 13, 4096: 183. Where prefix and own tokens are one launch (16 rows a KV head): 4 behind 128 0.9, 4096: 6.
-static int shared_prefix_tokens(const b2_engine* e, const BatchIdx& b) {
-    if (b.n < 2) return 0;
-    const Slot& first = e->slots[b.slot[0]];
-    size_t pages = first.blocks.size();
-    for (int i = 0; i < b.n && pages; i++) {
-        const Slot& s = e->slots[b.slot[i]];
-        pages = std::min({pages, s.blocks.size(), (size_t)(s.n_past / e->cfg.kv_block_tokens)});
-        size_t same = 0;
-        while (same < pages && s.blocks[same] == first.blocks[same]) same++;
-        pages = same;
+// The sequences of a batched step whose tables begin with the same pages: the first n of the step's slots, and the tokens of those pages (whole pages; the token
+// that the step writes lies behind them). n 0: no group of which reading them once is worth the launches.
+// Measured per layer (32 heads over 8 KV heads of 128; saved, us): three launches instead of one cost about 7 us, won back from about 16384 tokens in all:
+// 8 sequences behind 512 tokens -1.3, 1024: 1.4, 4096: 19; 16 behind 512 -1.7, 1024: 3.5, 4096: 36; 32 behind 256 -7, 512: -0.9, 1024: 13, 4096: 87; 64 behind
+// 128 -7, 256: -0.5, 512: 13, 4096: 183. Where prefix and own tokens are one launch (16 rows a KV head): 4 behind 128 0.9, 4096: 6. The other sequences of the
+// step take a launch more: with one of those, 16 behind 1024 -3.4, 4096: 24; 32 behind 512 -13, 1024: 0.6, 4096: 70; 63 behind 512 5, 4096: 170.
+struct SharedGroup { int n = 0, tokens = 0; };
+static SharedGroup shared_group(const b2_engine* e, BatchIdx& b, BatchTokens& set, int* order) {
+    SharedGroup best;
+    uint64_t members = 0;                                        // of the best group
+    for (int i = 0; i < b.n; i++) order[i] = i;
+    if (e->attn_mma == 0) return best;
+    const int bt = e->cfg.kv_block_tokens, group = e->cfg.n_head / e->cfg.n_head_kv;
+    auto pages = [&](int i) { const Slot& s = e->slots[b.slot[i]]; return std::min(s.blocks.size(), (size_t)(s.n_past / bt)); };
+    uint64_t seen = 0;
+    for (int i = 0; i < b.n; i++) {
+        if (seen >> i & 1 || !pages(i)) continue;
+        const std::vector<int32_t>& first = e->slots[b.slot[i]].blocks;
+        uint64_t with = 0;
+        size_t common = pages(i);
+        int n = 0;
+        for (int j = i; j < b.n; j++) {
+            const std::vector<int32_t>& own = e->slots[b.slot[j]].blocks;
+            if (!pages(j) || own[0] != first[0]) continue;
+            with |= 1ull << j; n++;
+            common = std::min(common, pages(j));
+            size_t same = 0;
+            while (same < common && own[same] == first[same]) same++;
+            common = same;
+        }
+        seen |= with;
+        const long tokens = (long)common * bt, all = tokens * n;
+        const bool worth = n < 2 ? false : n == b.n && n * group <= 16 ? tokens >= 128 : all >= (n == b.n ? 16384 : 32768);
+        if (worth && all > (long)best.n * best.tokens) { best.n = n; best.tokens = (int)tokens; members = with; }
     }
-    const int tokens = (int)pages * e->cfg.kv_block_tokens;
-    const bool worth = b.n * (e->cfg.n_head / e->cfg.n_head_kv) <= 16 ? tokens >= 128 : (long)tokens * b.n >= 16384;
-    return e->attn_mma != 0 && worth ? tokens : 0;
+    if (best.n && best.n < b.n) {                                // they go first
+        const BatchIdx was = b;
+        const BatchTokens set_was = set;
+        int at = 0;
+        for (int pass = 1; pass >= 0; pass--)
+            for (int i = 0; i < was.n; i++)
+                if ((int)(members >> i & 1) == pass) { b.slot[at] = was.slot[i]; set.token[at] = set_was.token[i]; set.pos[at] = set_was.pos[i]; order[at++] = i; }
+    }
+    return best;
 }
+static_assert(BATCH_MAX <= 64, "members are bits");
 
 // One decode step for b.n sequences at once: the weights are read (and dequantised) once for all of them by the
 // tensor-core GEMM; attention and sampling run one CTA group per sequence from the per-slot device tables.
 // Enqueued kernel by kernel. Captured per list of slots, 8 steps of 32 sequences (4 layers of 4096) took 6580 us instead of 6750; but the list
 // changes whenever a chat starts or ends, and lists that live for three steps cost 5150 us instead of 4740 (16 layers: 16600 and 15600).
-static int batch_step(b2_engine* e, const BatchIdx& b, const BatchTokens& set, int32_t* tokens_out) {
+static int batch_step(b2_engine* e, const BatchIdx& b, const BatchTokens& set, const SharedGroup& shared, int32_t* tokens_out) {
     ChainPdl chain(e->chain_pdl && e->use_pdl);
     const b2_config& c = e->cfg;
     cudaStream_t st = e->stream;
     const int T = b.n, T_pad = (T + 15) / 16 * 16, E = c.n_embd, F = c.n_ff, hd = c.head_dim, qd = c.n_head * hd;
     int rc, np = 0;
     long ps = 0;
-    const int shared = shared_prefix_tokens(e, b);
-    if (shared > 0) {
-        const size_t need = shared_prefix_work_floats(T, c.n_head, c.n_head_kv, hd);
+    if (shared.n > 0) {
+        const size_t need = shared_prefix_work_floats(shared.n, c.n_head, c.n_head_kv, hd);
         if (need > e->sp_work_floats) {          // (frees only behind what runs: cudaFree waits)
             cudaFree(e->sp_work);
             e->sp_work = nullptr; e->sp_work_floats = 0;
@@ -966,18 +992,26 @@ static int batch_step(b2_engine* e, const BatchIdx& b, const BatchTokens& set, i
         a.n_head = c.n_head; a.n_kv = c.n_head_kv; a.head_dim = hd; a.block_tokens = c.kv_block_tokens;
         // enough CTAs to fill the GPU ~2x over, no more (8 sequences: 4 splits 4.36 ms/step, 8 splits 4.81): every extra split of a sequence re-pays the kernel's fixed latency
         int ns = e->n_splits;
-        while (ns > 1 && (long)ns * c.n_head_kv * T > 2L * e->n_sms) ns >>= 1;
+        while (ns > 1 && (long)ns * c.n_head_kv * (T - shared.n) > 2L * e->n_sms) ns >>= 1;      // (of the sequences that this kernel has)
         if (e->batch_attn_splits > 0 && e->batch_attn_splits <= e->n_splits) ns = e->batch_attn_splits;
         a.n_splits = ns; a.scale = 1.0f / sqrtf((float)hd); a.err = kernel_error_word(); a.max_pages = e->max_blocks;
-        if (shared > 0) {
+        if (shared.n > 0) {
             SharedPrefixArgs x = {};
-            x.r.n_seqs = x.r.n_rows = T; x.r.max_pages = e->max_blocks - shared / c.kv_block_tokens; x.r.block_tokens = c.kv_block_tokens; x.r.n_pages = c.kv_num_blocks;
+            x.r.n_seqs = x.r.n_rows = shared.n; x.r.max_pages = e->max_blocks - shared.tokens / c.kv_block_tokens; x.r.block_tokens = c.kv_block_tokens; x.r.n_pages = c.kv_num_blocks;
             x.q = e->bd_q; x.q_row = qd; x.q_head = hd; x.q_f32 = 1; x.k_pool = kc; x.v_pool = vc;
-            x.prefix_pages = e->slots[b.slot[0]].block_table; x.n_prefix = shared; x.work = e->sp_work; x.max_rows = 1;
+            x.prefix_pages = e->slots[b.slot[0]].block_table; x.n_prefix = shared.tokens; x.work = e->sp_work; x.max_rows = 1;
             x.n_head = c.n_head; x.n_kv = c.n_head_kv; x.head_dim = hd; x.type = ELEM_F16; x.scale_log2 = a.scale * 1.4426950408889634f;
             x.tab = e->slot_tab; x.slots = b; x.out_h = e->pf_att; x.out_T_pad = T_pad; x.err = a.err;
             CK(shared_prefix_launch(x, st));
             e->launches += shared_prefix_launches(x) - 1;
+            if (shared.n < T) {
+                BatchIdx rest = {};
+                rest.n = T - shared.n;
+                for (int i = 0; i < rest.n; i++) rest.slot[i] = b.slot[shared.n + i];
+                a.q += (size_t)shared.n * qd; a.out += (size_t)shared.n * qd; a.out_h = e->pf_att + shared.n * 8; a.out_T_pad = T_pad;
+                CK(attn_decode_mma_launch(a, e->slot_tab, &rest, st, false));
+                e->launches++;
+            }
         } else if (e->attn_mma != 0) {      // the tensor-core kernel writes f16 in the o-projection GEMM's operand order itself
             a.out_h = e->pf_att; a.out_T_pad = T_pad;
             CK(attn_decode_mma_launch(a, e->slot_tab, &b, st, false));
@@ -1028,20 +1062,25 @@ extern "C" int b2_decode(b2_engine* e, const int32_t* slots, int n, int32_t* out
         if (e->slots[slots[i]].n_past + 1 > e->cfg.n_ctx) return fail(B2_ERR_ARG, "context window full");
         for (int j = 0; j < i; j++) if (slots[j] == slots[i]) return fail(B2_ERR_ARG, "slot listed twice");
     }
+    std::vector<int> at;                   // where each slot's sampled token lies
     const bool batched = e->gemm_ok && block_elems(e->output.type) != 1 && n >= e->batch_min &&
                          (size_t)n * e->cfg.n_vocab <= (e->pf_part_floats ? e->pf_part_floats : (size_t)-1);
     if (batched) {
         int rc = ensure_batch_workspace(e); if (rc) return rc;
+        at.resize(n);
         for (int i0 = 0; i0 < n; i0 += BATCH_MAX) {
             BatchIdx b = {};
-            BatchTokens set;
+            BatchTokens set = {};
+            int order[BATCH_MAX];
             b.n = n - i0 < BATCH_MAX ? n - i0 : BATCH_MAX;
             for (int i = 0; i < b.n; i++) {
                 const Slot& s = e->slots[slots[i0 + i]];
                 b.slot[i] = slots[i0 + i]; set.token[i] = s.set_token; set.pos[i] = s.n_past;
             }
             if ((size_t)b.n * e->cfg.n_vocab > e->pf_part_floats) return fail(B2_ERR_UNSUPPORTED, "vocabulary too large for the batch workspace");
-            if ((rc = batch_step(e, b, set, e->pinned + i0))) return rc;
+            const SharedGroup shared = shared_group(e, b, set, order);
+            for (int i = 0; i < b.n; i++) at[i0 + order[i]] = i0 + i;
+            if ((rc = batch_step(e, b, set, shared, e->pinned + i0))) return rc;
             // logits of this step stay in the batch output until the next GEMM call reuses the buffer
             for (int i = 0; i < b.n; i++) e->slots[b.slot[i]].logits_view = e->pf_part + (size_t)i * e->cfg.n_vocab;
         }
@@ -1059,7 +1098,7 @@ extern "C" int b2_decode(b2_engine* e, const int32_t* slots, int n, int32_t* out
     }
     CK(cudaStreamSynchronize(e->stream));
     { int rc2 = b2_check_kernel_error(); if (rc2) return rc2; }
-    if (out) for (int i = 0; i < n; i++) out[i] = batched ? e->pinned[i] : e->slot_token[slots[i]];
+    if (out) for (int i = 0; i < n; i++) out[i] = batched ? e->pinned[at[i]] : e->slot_token[slots[i]];
     return B2_OK;
 }
 

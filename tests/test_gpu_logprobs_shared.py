@@ -196,6 +196,58 @@ def test_batched_decoding_over_shared_pages(native_lib, tmp_models, monkeypatch,
             assert np.abs(out[True][i][s - (n - rows)] - want[i]).max() <= 2 * LOGIT_TOL, (s, i)
 
 
+@pytest.mark.parametrize("arch,ftype,seed,bt,groups,wanted", [
+    ("tiny128", "Q8_0", 6, 16, [(40, 900), (9, 0)], (40, 896)),                 # one without anything in common, in between
+    ("tiny", "Q4_K_M", 1, 64, [(20, 300), (36, 980)], (36, 960)),               # two groups: the larger one
+    ("tiny128", "Q8_0", 6, 32, [(36, 980), (3, 900), (25, 40)], (36, 960)),     # the full step of 64
+    ("tiny", "Q4_K_M", 1, 16, [(8, 200), (8, 300)], None),                      # not worth it
+    ("tiny128", "Q8_0", 6, 16, [(30, 900), (1, 0)], None),                      # nor this, with another sequence beside
+])
+def test_batched_decoding_over_groups_of_shared_pages(native_lib, tmp_models, monkeypatch, arch, ftype, seed, bt, groups, wanted):
+    """Sequences of several groups in mixed order, every group with pages of its own in common: logits against the same steps over own pages, tokens in the
+    callers' order."""
+    monkeypatch.setenv("B2_BATCH_MIN", "3")
+    path = _model(tmp_models, arch, ftype, seed)
+    kinds = [g for g, (n, _) in enumerate(groups) for _ in range(n)]
+    np.random.default_rng(1).shuffle(kinds)
+    n = len(kinds)
+    heads = [prompt_of(common, 10 + g) for g, (_, common) in enumerate(groups)]
+    rest = [prompt_of(1 + (7 * i) % 29, 100 + i) for i in range(n)]
+    forced = [prompt_of(3, 500 + i) for i in range(n)]
+    order = [int(i) for i in np.random.default_rng(2).permutation(n)]
+    out, launches = {}, {}
+    for share in (False, True):
+        eng = _engine(path, max_seqs=n, n_ctx=1024, bt=bt)
+        eng.set_logprobs(2)
+        first = {}
+        for s in range(n):
+            g = kinds[s]
+            prompt = heads[g] + rest[s]
+            begin = eng.share_pages(s, first[g], groups[g][1]) if share and g in first else 0
+            first.setdefault(g, s)
+            eng.ensure_pages(s, len(prompt) + 8)
+            eng.seq_begin(s, begin, prompt[:begin], _greedy())
+            eng.prefill(s, prompt[begin:])
+        got = []
+        for i in range(3):
+            for s in range(n):
+                eng.set_token(s, forced[s][i])
+            before = eng.launch_count()
+            toks = eng.decode(order)
+            launches[share] = eng.launch_count() - before
+            rows = np.stack([eng.logits(s).copy() for s in range(n)])
+            for s, t in zip(order, toks):
+                assert t == int(rows[s].argmax())
+                check_logprobs(eng.logprobs(s), rows[s], t)
+            got.append(rows)
+        out[share] = np.stack(got)
+        eng.close()
+    group = {"tiny": 4, "tiny128": 2}[arch]
+    assert launches[True] - launches[False] == (0 if wanted is None else 2 * (1 + (1 if wanted[0] * group <= 16 else 2)))
+    assert wanted is None or wanted == max(((k, common // bt * bt) for k, common in groups), key=lambda g: g[0] * g[1])
+    assert np.abs(out[True] - out[False]).max() <= LOGIT_TOL
+
+
 def test_shared_pages_are_given_up_before_they_are_written(native_lib, tmp_models, monkeypatch):
     """A slot that goes on inside pages that another one holds gets its own there; the other's tokens stay as they were."""
     monkeypatch.setenv("B2_BATCH_MIN", "2")
