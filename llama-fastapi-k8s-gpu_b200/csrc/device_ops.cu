@@ -105,6 +105,7 @@ extern "C" int b2_attention_shared_prefix_workspace(int n_rows, int n_head, int 
     const char* what = "b2_attention_shared_prefix_workspace";
     if (int rc = check_heads(what, n_head, n_kv, head_dim)) return rc;
     if (!bytes || n_rows < 0) return bad(what, "null result or negative number of rows");
+    if ((int64_t)n_rows * n_head > INT32_MAX) return bad(what, "rows * n_head must fit 32 bits");      // (as the call: prefix_cut counts units in an int)
     *bytes = n_rows ? (int64_t)shared_prefix_work_floats(n_rows, n_head, n_kv, head_dim) * 4 : 0;
     return B2_OK;
 }

@@ -770,6 +770,7 @@ constexpr int SP_PREFIX_SPLITS = 32, SP_OWN_SPLITS = 8;
 
 // Runs of equal length over all units laid end to end, or over every unit by itself where that makes them no more than three blocks longer: a run that goes on
 // into another unit loads queries, starts and ends its pipeline and writes its results twice, which takes as long as three blocks (6 us). For `sms` CTAs at most.
+// (Units fit an int: every entry refuses n_rows * n_head of more than 31 bits.)
 PrefixCut prefix_cut(long n_rows, int n_head, int n_kv, int n_prefix, int sms) {
     PrefixCut c = {};
     c.pairs = (int)((n_rows * (n_head / n_kv) + 255) / 256);

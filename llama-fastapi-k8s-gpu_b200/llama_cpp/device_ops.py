@@ -157,6 +157,9 @@ def kv_append(k, v, k_pool, v_pool, pages, row_start, lengths, *, freqs=None, la
 
 def attention_shared_prefix_workspace(rows, n_head, n_kv, head_dim) -> int:
     """Bytes of workspace that attention_shared_prefix needs for so many rows, whatever the lengths."""
+    for name, n in (("rows", rows), ("n_head", n_head), ("n_kv", n_kv), ("head_dim", head_dim)):
+        if not 0 <= n < 1 << 31:                                 # (ctypes would drop the upper bits)
+            raise ValueError(f"{name} must be a number of 31 bits, not {n}")
     out = ctypes.c_int64()
     check(_cabi.load_library().b2_attention_shared_prefix_workspace(rows, n_head, n_kv, head_dim, ctypes.byref(out)), "b2_attention_shared_prefix_workspace")
     return out.value

@@ -1,10 +1,15 @@
 """What the operators over device tensors refuse, before anything reaches a device (no GPU here): the C entry points on sizes and pointers, the Python
 ones on tensors."""
 import ctypes
+import os
+import subprocess
+import sys
 
 import pytest
 
 torch = pytest.importorskip("torch")
+
+PACKAGE = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "llama-fastapi-k8s-gpu_b200")
 
 
 class OnGpu:
@@ -97,6 +102,23 @@ def test_shared_prefix_workspace_covers_every_prefix(native_lib):
     assert need(0, 8, 8, 64) == 0
     with pytest.raises(RuntimeError):
         need(4, 8, 3, 64)
+
+
+@pytest.mark.parametrize("sizes", [(2 ** 31 - 1, 512, 512, 128), (2 ** 30, 1024, 1024, 64), (2 ** 28, 4096, 4096, 64), (2 ** 27, 64, 1, 64), (2 ** 26, 32, 8, 128), (2 ** 32 + 5, 32, 8, 128),
+                                   (-1, 32, 8, 128), (5, 2 ** 32 + 32, 8, 128)])
+def test_shared_prefix_workspace_refusals(native_lib, sizes):
+    """Sizes that the call itself refuses have no workspace either. In a process of its own: a division by a wrapped product of the sizes ends it."""
+    code = ("import sys\nsys.path.insert(0, sys.argv[1])\nfrom llama_cpp.device_ops import attention_shared_prefix_workspace as need\n"
+            "try:\n    print(need(*eval(sys.argv[2])))\nexcept (RuntimeError, ValueError) as e:\n    print('refused:', e)")
+    r = subprocess.run([sys.executable, "-c", code, PACKAGE, repr(sizes)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.startswith("refused:"), (r.returncode, r.stdout, r.stderr[-500:])
+
+
+def test_shared_prefix_workspace_of_the_largest_sizes(native_lib):
+    """the largest that a call takes, rows * heads just inside 32 bits: there are two slots of partial results at least, prefix and own tokens, and nothing wraps"""
+    from llama_cpp.device_ops import attention_shared_prefix_workspace as need
+    for rows, heads, kv, dim in [(2 ** 26 - 1, 32, 8, 128), (2 ** 31 - 1, 1, 1, 64), ((2 ** 31 - 1) // 65535, 65535, 65535, 64), (1, 64 * 65535, 65535, 128)]:
+        assert need(rows, heads, kv, dim) >= 2 * rows * heads * (dim + 2) * 4
 
 
 LOGPROB_REFUSALS = [
