@@ -70,7 +70,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError("link failed")
     host = os.path.join(LIB, "libb200_hosttest.so")
     hsrc = os.path.join(CSRC, "host_selftest.cpp")
-    if force or _newer(host, [hsrc, os.path.join(CSRC, "quant_blocks.cuh"), os.path.join(CSRC, "gemm_ring.h"), os.path.join(CSRC, "per_device.h")]):
+    if force or _newer(host, [hsrc, *(os.path.join(CSRC, f) for f in ("quant_blocks.cuh", "gemm_ring.h", "per_device.h", "shared_group.h"))]):
         subprocess.run(["g++", "-O2", "-ffp-contract=off", "-fPIC", "-shared", hsrc, "-o", host], check=True)
     lists, include = os.path.join(LIB, "libb200_pylists" + sysconfig.get_config_var("EXT_SUFFIX")), sysconfig.get_paths()["include"]
     lsrc = [os.path.join(CSRC, f) for f in ("py_lists.cpp", "py_tensors.cpp")]

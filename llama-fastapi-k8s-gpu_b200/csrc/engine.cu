@@ -8,6 +8,7 @@
 #include "layered.h"
 #include "ptx.cuh"
 #include "quant_blocks.cuh"
+#include "shared_group.h"
 
 #include <math.h>
 #include <stdio.h>
@@ -908,52 +909,29 @@ static int ensure_batch_workspace(b2_engine* e) {
     return B2_OK;
 }
 
-// The sequences of a batched step whose tables begin with the same pages: the first n of the step's slots, and the tokens of those pages (whole pages; the token
-// that the step writes lies behind them). n 0: no group of which reading them once is worth the launches.
-// Measured per layer (32 heads over 8 KV heads of 128; saved, us): three launches instead of one cost about 7 us, won back from about 16384 tokens in all:
-// 8 sequences behind 512 tokens -1.3, 1024: 1.4, 4096: 19; 16 behind 512 -1.7, 1024: 3.5, 4096: 36; 32 behind 256 -7, 512: -0.9, 1024: 13, 4096: 87; 64 behind
-// 128 -7, 256: -0.5, 512: 13, 4096: 183. Where prefix and own tokens are one launch (16 rows a KV head): 4 behind 128 0.9, 4096: 6. The other sequences of the
-// step take a launch more: with one of those, 16 behind 1024 -3.4, 4096: 24; 32 behind 512 -13, 1024: 0.6, 4096: 70; 63 behind 512 5, 4096: 170.
-struct SharedGroup { int n = 0, tokens = 0; };
+// The sequences of a batched step that read their common leading pages once become the first of the step's slots (the token that the step writes lies behind
+// those pages); order: where each of the caller's slots went.
 static SharedGroup shared_group(const b2_engine* e, BatchIdx& b, BatchTokens& set, int* order) {
-    SharedGroup best;
-    uint64_t members = 0;                                        // of the best group
     for (int i = 0; i < b.n; i++) order[i] = i;
-    if (e->attn_mma == 0) return best;
-    const int bt = e->cfg.kv_block_tokens, group = e->cfg.n_head / e->cfg.n_head_kv;
-    auto pages = [&](int i) { const Slot& s = e->slots[b.slot[i]]; return std::min(s.blocks.size(), (size_t)(s.n_past / bt)); };
-    uint64_t seen = 0;
+    if (e->attn_mma == 0) return {};
+    const int32_t* pages[BATCH_MAX];
+    int n_pages[BATCH_MAX];
     for (int i = 0; i < b.n; i++) {
-        if (seen >> i & 1 || !pages(i)) continue;
-        const std::vector<int32_t>& first = e->slots[b.slot[i]].blocks;
-        uint64_t with = 0;
-        size_t common = pages(i);
-        int n = 0;
-        for (int j = i; j < b.n; j++) {
-            const std::vector<int32_t>& own = e->slots[b.slot[j]].blocks;
-            if (!pages(j) || own[0] != first[0]) continue;
-            with |= 1ull << j; n++;
-            common = std::min(common, pages(j));
-            size_t same = 0;
-            while (same < common && own[same] == first[same]) same++;
-            common = same;
-        }
-        seen |= with;
-        const long tokens = (long)common * bt, all = tokens * n;
-        const bool worth = n < 2 ? false : n == b.n && n * group <= 16 ? tokens >= 128 : all >= (n == b.n ? 16384 : 32768);
-        if (worth && all > (long)best.n * best.tokens) { best.n = n; best.tokens = (int)tokens; members = with; }
+        const Slot& s = e->slots[b.slot[i]];
+        pages[i] = s.blocks.data(); n_pages[i] = (int)std::min(s.blocks.size(), (size_t)(s.n_past / e->cfg.kv_block_tokens));
     }
-    if (best.n && best.n < b.n) {                                // they go first
+    const SharedGroup best = shared_group_of(pages, n_pages, b.n, e->cfg.kv_block_tokens, e->cfg.n_head / e->cfg.n_head_kv);
+    if (best.n && best.n < b.n) {
         const BatchIdx was = b;
         const BatchTokens set_was = set;
         int at = 0;
         for (int pass = 1; pass >= 0; pass--)
             for (int i = 0; i < was.n; i++)
-                if ((int)(members >> i & 1) == pass) { b.slot[at] = was.slot[i]; set.token[at] = set_was.token[i]; set.pos[at] = set_was.pos[i]; order[at++] = i; }
+                if ((int)(best.members >> i & 1) == pass) { b.slot[at] = was.slot[i]; set.token[at] = set_was.token[i]; set.pos[at] = set_was.pos[i]; order[at++] = i; }
     }
     return best;
 }
-static_assert(BATCH_MAX <= 64, "members are bits");
+static_assert(BATCH_MAX <= SHARED_GROUP_MAX, "members are bits");
 
 // One decode step for b.n sequences at once: the weights are read (and dequantised) once for all of them by the
 // tensor-core GEMM; attention and sampling run one CTA group per sequence from the per-slot device tables.

@@ -6,6 +6,7 @@
 #include "gemm_ring.h"
 #include "per_device.h"
 #include "quant_blocks.cuh"
+#include "shared_group.h"
 
 template <int T>
 static float host_row(const uint8_t* rowp, int K, const b2::ActView& v, bool act2) {
@@ -38,6 +39,15 @@ void b2_host_per_device(const int* calls, int n_calls, int* times, int* ready) {
         const int device = calls[i] < 0 ? -1 - calls[i] : calls[i];
         ready[i] = once.ready(device, [&] { times[device]++; return calls[i] >= 0; });
     }
+}
+
+// the sequences that read their common pages once (shared_group.h): tables [n][stride]; returns how many, their bits and the tokens that they share
+int b2_host_shared_group(const int32_t* tables, int stride, const int32_t* n_pages, int n, int block_tokens, int heads_a_kv, uint64_t* members, int32_t* tokens) {
+    const int32_t* pages[b2::SHARED_GROUP_MAX];
+    for (int i = 0; i < n; i++) pages[i] = tables + (long)i * stride;
+    const b2::SharedGroup g = b2::shared_group_of(pages, n_pages, n, block_tokens, heads_a_kv);
+    *members = g.members; *tokens = g.tokens;
+    return g.n;
 }
 
 // dequantise n_elems elements (whole blocks) with the exact element routine

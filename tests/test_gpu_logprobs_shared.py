@@ -248,6 +248,53 @@ def test_batched_decoding_over_groups_of_shared_pages(native_lib, tmp_models, mo
     assert np.abs(out[True] - out[False]).max() <= LOGIT_TOL
 
 
+@pytest.mark.parametrize("arch,ftype,seed,bt,first,groups", [
+    ("tiny", "Q4_K_M", 1, 16, 64, [(36, 960), (20, 64)]),                       # a group, and sequences that share its first pages alone
+    ("tiny128", "Q8_0", 6, 16, 16, [(38, 896), (1, 16)]),                       # one such sequence, one page
+    ("tiny", "Q4_K_M", 1, 64, 128, [(36, 960), (26, 704)]),                     # two groups behind a common head
+])
+def test_batched_decoding_over_groups_with_a_common_head(native_lib, tmp_models, monkeypatch, arch, ftype, seed, bt, first, groups):
+    """Every sequence begins with the same `first` tokens in the same pages, and those of a group share more: the larger group reads all that it shares once. Logits
+    against the same steps over own pages."""
+    monkeypatch.setenv("B2_BATCH_MIN", "3")
+    path = _model(tmp_models, arch, ftype, seed)
+    kinds = [g for g, (n, _) in enumerate(groups) for _ in range(n)]
+    np.random.default_rng(3).shuffle(kinds)
+    n = len(kinds)
+    head = prompt_of(first, 9)
+    heads = [head + prompt_of(common - first, 10 + g) for g, (_, common) in enumerate(groups)]
+    rest = [prompt_of(1 + (7 * i) % 29, 100 + i) for i in range(n)]
+    forced = [prompt_of(2, 500 + i) for i in range(n)]
+    out, launches = {}, {}
+    for share in (False, True):
+        eng = _engine(path, max_seqs=n, n_ctx=1024, bt=bt)
+        owner = {}
+        for s in range(n):
+            g, prompt = kinds[s], heads[kinds[s]] + rest[s]
+            begin = 0
+            if share and s:
+                begin = eng.share_pages(s, owner.get(g, 0), groups[g][1] if g in owner else first)
+            owner.setdefault(g, s)
+            eng.ensure_pages(s, len(prompt) + 8)
+            eng.seq_begin(s, begin, prompt[:begin], _greedy())
+            eng.prefill(s, prompt[begin:])
+        if share:
+            assert len({tuple(eng.pages.table(s)[:first // bt]) for s in range(n)}) == 1
+            assert len({tuple(eng.pages.table(s)[:groups[0][1] // bt]) for s in range(n) if kinds[s] == 0}) == 1
+        got = []
+        for i in range(2):
+            for s in range(n):
+                eng.set_token(s, forced[s][i])
+            before = eng.launch_count()
+            eng.decode(list(range(n)))
+            launches[share] = eng.launch_count() - before
+            got.append(np.stack([eng.logits(s).copy() for s in range(n)]))
+        out[share] = np.stack(got)
+        eng.close()
+    assert launches[True] - launches[False] == 2 * 3              # two layers: prefix, own tokens and joining beside the others' attention
+    assert np.abs(out[True] - out[False]).max() <= LOGIT_TOL
+
+
 def test_shared_pages_are_given_up_before_they_are_written(native_lib, tmp_models, monkeypatch):
     """A slot that goes on inside pages that another one holds gets its own there; the other's tokens stay as they were."""
     monkeypatch.setenv("B2_BATCH_MIN", "2")
