@@ -15,6 +15,7 @@ import queue
 import threading
 import time
 import uuid
+import warnings
 from typing import Any, Dict, Iterator, List, Optional, Sequence, Union
 
 import numpy as np
@@ -365,7 +366,8 @@ class Llama:
                                logprobs: Optional[bool] = None, top_logprobs: Optional[int] = None,
                                cancel_event: Optional[threading.Event] = None, **kwargs: Any):
         """OpenAI-shaped chat completion; `messages` is not modified (the caller already owns and
-        mutates it: api.py:39,44). `cancel_event` (not in upstream) abandons the generation when set."""
+        mutates it: api.py:39,44). `cancel_event` (not in upstream) abandons the generation when set. `logprobs`: the choice's "logprobs" as create_completion gives
+        them, with `top_logprobs` alternatives (64 at most are given, whatever is asked for); a stream has none, and warns."""
         if functions or tools or response_format is not None:
             raise NotImplementedError("functions / tools / response_format are not implemented")
         fmt = self._chat_formatter if self._chat_formatter is not None else cf.FORMATS[self.chat_format]
@@ -374,14 +376,17 @@ class Llama:
         stops = [] if stop is None else ([stop] if isinstance(stop, str) else list(stop))
         if res.stop is not None:
             stops = stops + ([res.stop] if isinstance(res.stop, str) else list(res.stop))
+        alternatives = min(max(top_logprobs or 0, 0), 64) if logprobs else None
+        if alternatives is not None and (stream or not hasattr(self._engine, "set_logprobs")):
+            warnings.warn("log probabilities are not given for streamed chats" if stream else "this engine has no log probabilities", stacklevel=2)
+            alternatives = None
         out = self.create_completion(prompt=prompt, temperature=temperature, top_p=top_p, top_k=top_k, min_p=min_p,
                                      typical_p=typical_p, stream=stream, stop=stops, seed=seed, max_tokens=max_tokens,
                                      presence_penalty=presence_penalty, frequency_penalty=frequency_penalty,
                                      repeat_penalty=repeat_penalty, tfs_z=tfs_z, mirostat_mode=mirostat_mode,
                                      mirostat_tau=mirostat_tau, mirostat_eta=mirostat_eta, model=model,
                                      logits_processor=logits_processor, grammar=grammar, logit_bias=logit_bias,
-                                     cancel_event=cancel_event,
-                                     logprobs=(top_logprobs or 0) if logprobs and not stream and hasattr(self._engine, "set_logprobs") else None)
+                                     cancel_event=cancel_event, logprobs=alternatives)
         if stream:
             return self._chat_chunks(out)
         return {

@@ -144,6 +144,25 @@ def test_logprobs_refusals(tiny_path, monkeypatch):
     llm.close()
 
 
+def test_chats_that_ask_for_what_is_not_given(tiny_path, monkeypatch):
+    """A chat's stream has no log probabilities and says so; numbers of alternatives outside 0..64 are the nearest one inside. Both ran before there were any."""
+    llm = make(tiny_path, monkeypatch)
+    ask = lambda **kw: llm.create_chat_completion([{"role": "user", "content": "hello"}], max_tokens=5, temperature=0.0, **kw)
+    plain = list(ask(stream=True))
+    with pytest.warns(UserWarning, match="log probabilities"):
+        chunks = ask(stream=True, logprobs=True, top_logprobs=2)
+    strip = lambda cs: [c["choices"][0] for c in cs]
+    assert strip(chunks) == strip(plain) and llm._engine.n_top is None
+    for asked, kept in ((65, 64), (10 ** 6, 64), (-1, 0)):
+        lp = ask(logprobs=True, top_logprobs=asked)["choices"][0]["logprobs"]
+        assert len(lp["tokens"]) == 5 and llm._engine.n_top == kept
+    assert ask(logprobs=False, top_logprobs=65)["choices"][0]["logprobs"] is None
+    monkeypatch.setattr(PagedFake, "set_logprobs", property(lambda self: (_ for _ in ()).throw(AttributeError())))      # an engine that has none
+    with pytest.warns(UserWarning, match="log probabilities"):
+        assert ask(logprobs=True)["choices"][0]["logprobs"] is None
+    llm.close()
+
+
 @pytest.mark.parametrize("share", [False, True])
 def test_many_callers_with_one_prompt_in_front(tiny_path, monkeypatch, share):
     """Texts are the ones of single calls, whoever shares pages with whom; the shared prompt is evaluated once per run of callers that overlap."""
