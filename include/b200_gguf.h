@@ -99,8 +99,8 @@ int b2_engine_device_bytes(b2_engine* e, int64_t* weight_bytes, int64_t* kv_byte
  *      The page allocator lives in the host (llama_cpp/kv_pages.py); the engine only holds
  *      each slot's page table. -------------------------------------------------------------- */
 /* Tables may begin with the same pages: in a batched step (b2_decode) the largest group of slots that share whole pages
- * reads those once for all of them, if that is faster (from 16384 tokens over all slots, 32768 beside others, fewer where
- * heads and slots are few). No slot may write to a page that another one reads: the token at position n_past
+ * reads those once for all of them, if that is faster (from about 16384 tokens over all slots, 32768 or more
+ * beside others, fewer where heads and slots are few). No slot may write to a page that another one reads: the token at position n_past
  * has to lie behind the shared pages. */
 int b2_seq_set_blocks(b2_engine* e, int slot, const int32_t* host_blocks, int n_blocks);
 /* Start (or restart) a slot: n_past tokens are already in its KV pages; `host_history` are the

@@ -920,7 +920,7 @@ static SharedGroup shared_group(const b2_engine* e, BatchIdx& b, BatchTokens& se
         const Slot& s = e->slots[b.slot[i]];
         pages[i] = s.blocks.data(); n_pages[i] = (int)std::min(s.blocks.size(), (size_t)(s.n_past / e->cfg.kv_block_tokens));
     }
-    const SharedGroup best = shared_group_of(pages, n_pages, b.n, e->cfg.kv_block_tokens, e->cfg.n_head / e->cfg.n_head_kv);
+    const SharedGroup best = shared_group_of(pages, n_pages, b.n, e->cfg.kv_block_tokens, e->cfg.n_head / e->cfg.n_head_kv, e->cfg.n_head_kv * e->cfg.head_dim);
     if (best.n && best.n < b.n) {
         const BatchIdx was = b;
         const BatchTokens set_was = set;

@@ -42,10 +42,10 @@ void b2_host_per_device(const int* calls, int n_calls, int* times, int* ready) {
 }
 
 // the sequences that read their common pages once (shared_group.h): tables [n][stride]; returns how many, their bits and the tokens that they share
-int b2_host_shared_group(const int32_t* tables, int stride, const int32_t* n_pages, int n, int block_tokens, int heads_a_kv, uint64_t* members, int32_t* tokens) {
+int b2_host_shared_group(const int32_t* tables, int stride, const int32_t* n_pages, int n, int block_tokens, int heads_a_kv, int kv_width, uint64_t* members, int32_t* tokens) {
     const int32_t* pages[b2::SHARED_GROUP_MAX];
     for (int i = 0; i < n; i++) pages[i] = tables + (long)i * stride;
-    const b2::SharedGroup g = b2::shared_group_of(pages, n_pages, n, block_tokens, heads_a_kv);
+    const b2::SharedGroup g = b2::shared_group_of(pages, n_pages, n, block_tokens, heads_a_kv, kv_width);
     *members = g.members; *tokens = g.tokens;
     return g.n;
 }

@@ -15,7 +15,7 @@ def find(tmp_path_factory):
     subprocess.run(["g++", "-O2", "-ffp-contract=off", "-fPIC", "-shared", os.path.join(PKG, "csrc", "host_selftest.cpp"), "-o", out], check=True)
     lib = ctypes.CDLL(out)
 
-    def call(tables, bt, heads):
+    def call(tables, bt, heads, width=1024):
         """the members and the pages that they share"""
         n, stride = len(tables), max(1, max(len(t) for t in tables))
         flat = np.full((n, stride), -1, dtype=np.int32)
@@ -24,22 +24,24 @@ def find(tmp_path_factory):
         lens = np.array([len(t) for t in tables], dtype=np.int32)
         members, tokens = ctypes.c_uint64(), ctypes.c_int32()
         p = lambda a: a.ctypes.data_as(ctypes.c_void_p)
-        got = lib.b2_host_shared_group(p(flat), stride, p(lens), n, bt, heads, ctypes.byref(members), ctypes.byref(tokens))
+        got = lib.b2_host_shared_group(p(flat), stride, p(lens), n, bt, heads, width, ctypes.byref(members), ctypes.byref(tokens))
         who = [i for i in range(n) if members.value >> i & 1]
         assert got == len(who) and tokens.value % bt == 0
         return who, tokens.value // bt
     return call
 
 
-def pays(n, n_all, tokens, heads):
+def pays(n, n_all, tokens, heads, width):
     if n < 2:
         return False
-    if n == n_all and n * heads <= 16:
+    if n < n_all:
+        return n * tokens >= max(32768, 6144 * heads)
+    if n * heads <= 16:
         return tokens >= 128
-    return n * tokens >= (16384 if n == n_all else 32768)
+    return n * tokens >= (20480 if n > 16 and heads >= 4 and width >= 1024 else 16384)
 
 
-def most(tables, bt, heads):
+def most(tables, bt, heads, width):
     """members times tokens of the best set: sequences with the same first d pages, for every d"""
     best = 0
     for d in range(1, max(len(t) for t in tables) + 1):
@@ -47,15 +49,15 @@ def most(tables, bt, heads):
         for t in tables:
             if len(t) >= d:
                 sets[tuple(t[:d])] = sets.get(tuple(t[:d]), 0) + 1
-        best = max([best] + [n * d * bt for n in sets.values() if pays(n, len(tables), d * bt, heads)])
+        best = max([best] + [n * d * bt for n in sets.values() if pays(n, len(tables), d * bt, heads, width)])
     return best
 
 
-def check(find, tables, bt, heads):
-    who, depth = find(tables, bt, heads)
-    assert len(who) * depth * bt == most(tables, bt, heads)
+def check(find, tables, bt, heads, width=1024):
+    who, depth = find(tables, bt, heads, width)
+    assert len(who) * depth * bt == most(tables, bt, heads, width)
     assert len({tuple(tables[i][:depth]) for i in who}) <= 1 and all(len(tables[i]) >= depth for i in who)
-    assert not who or pays(len(who), len(tables), depth * bt, heads)
+    assert not who or pays(len(who), len(tables), depth * bt, heads, width)
     return who, depth
 
 
@@ -86,16 +88,27 @@ def test_a_group_within_a_group(find):
     check(find, tables, 64, 4)
 
 
-@pytest.mark.parametrize("heads", [1, 4, 8])
-def test_edges_of_the_rule(find, heads):
+@pytest.mark.parametrize("heads,width", [(1, 4096), (4, 1024), (4, 128), (7, 512), (8, 256), (8, 1024)])
+def test_edges_of_the_rule(find, heads, width):
     common = list(range(5000))
     for n in (1, 2, 3, 4, 5, 16, 17, 63, 64):
         for others in (0, 1):
-            for tokens in (64, 128, 192, 256, 512, 16384 // n, 16384 // n + 64, 32768 // n, 32768 // n + 64):
+            for tokens in (64, 128, 192, 256, 512, *(t // n + more for t in (16384, 20480, 32768, 43008, 49152) for more in (0, 63, 64))):
                 depth = tokens // 64
                 if n + others <= 64:
-                    check(find, [common[:depth] + [6000 + i] for i in range(n)] + [[9000]] * others, 64, heads)
-    assert find([[], []], 64, heads) == ([], 0)
+                    check(find, [common[:depth] + [6000 + i] for i in range(n)] + [[9000]] * others, 64, heads, width)
+    assert find([[], []], 64, heads, width) == ([], 0)
+
+
+def test_where_every_sequence_for_itself_was_faster(find):
+    """the measured points next to the edges, us a layer won or lost by reading common pages once"""
+    for n, others, tokens, heads, width, won in [(32, 0, 512, 4, 1024, -2.5), (64, 0, 256, 4, 1024, -2.3), (32, 0, 512, 8, 1024, -2.7), (32, 0, 1024, 4, 1024, 9), (64, 0, 512, 4, 1024, 10),
+                                                 (16, 0, 1024, 4, 1024, 2.5), (8, 0, 2048, 8, 1024, 5.3), (32, 0, 512, 8, 256, 21), (64, 0, 256, 8, 256, 16), (32, 0, 512, 1, 4096, 68),
+                                                 (32, 1, 1024, 8, 256, -6), (16, 1, 2048, 8, 256, -6.9), (32, 1, 1024, 8, 1024, -8.2), (16, 1, 2048, 8, 1024, -5.3), (32, 1, 1024, 7, 512, -8.3),
+                                                 (32, 1, 2048, 8, 256, 3.5), (57, 7, 1024, 8, 1024, 12.5), (26, 7, 2048, 8, 256, 2.8), (32, 1, 2048, 4, 1024, 19.5), (32, 1, 1024, 1, 4096, 74)]:
+        common = list(range(tokens // 64))
+        who, _ = find([common + [6000 + i] for i in range(n)] + [[9000 + i] for i in range(others)], 64, heads, width)
+        assert (len(who) == n) == (won > 0), (n, others, tokens, heads, width)
 
 
 def test_random_trees(find):
@@ -110,4 +123,4 @@ def test_random_trees(find):
             tables.append(t + list(range(fresh, fresh + k)))
             fresh += k
         order = rng.permutation(n)
-        check(find, [tables[i] for i in order], bt, int(rng.choice([1, 2, 4, 8])))
+        check(find, [tables[i] for i in order], bt, int(rng.choice([1, 2, 4, 8])), int(rng.choice([128, 1024])))
