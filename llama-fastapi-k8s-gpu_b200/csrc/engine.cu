@@ -22,7 +22,11 @@
 #include <vector>
 
 static thread_local std::string g_err;
-int b2_fail(int code, const std::string& msg) { g_err = msg; return code; }
+int b2_fail(int code, const std::string& msg) {
+    g_err = msg;
+    if (code == B2_ERR_CUDA) cudaGetLastError();      // reported here: the next launch that asks for the last error is not to find it
+    return code;
+}
 static int fail(int code, const std::string& msg) { return b2_fail(code, msg); }
 
 // kernel watchdogs (ptx.cuh mbar_wait) report through a host-mapped word; call after a sync

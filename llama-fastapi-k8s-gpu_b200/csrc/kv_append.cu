@@ -166,8 +166,9 @@ static cudaError_t kv_append_rows(const KvAppendArgs& a, cudaStream_t s) {
     const int turned = HALVES ? a.rot_dims / 2 / VEC : 0, pieces = turned + (a.head_dim - turned * 2 * VEC) / VEC, wide = pieces < KA_THREADS / 2 ? pieces : KA_THREADS / 2;
     // smaller CTAs, more of them at different points of their chains, once there are many rows: 16384 of 48 heads of 128 78 -> 70 us, 872 of 40 heads of 64 7.6 -> 8.3
     const int most = a.r.n_rows > 8 * 148 ? KA_THREADS / 2 : KA_THREADS, threads = (most / wide * wide + 31) / 32 * 32;
-    kv_append_kernel<In, Out, VEC, HALVES><<<a.r.n_rows, threads, sizeof(float2) * (a.rot_dims / 2), s>>>(a, wide);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)a.r.n_rows); cfg.blockDim = dim3(threads); cfg.dynamicSmemBytes = sizeof(float2) * (a.rot_dims / 2); cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, kv_append_kernel<In, Out, VEC, HALVES>, a, wide);      // (this launch's own status)
 }
 
 template <typename In, typename Out>

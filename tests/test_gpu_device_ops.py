@@ -524,3 +524,24 @@ def test_no_wait_ran_out(native_lib):
     import ctypes
     code = ctypes.c_uint32(9)
     assert native_lib.b2_device_op_error(0, ctypes.byref(code)) == 0 and code.value == 0
+
+
+def test_a_failed_call_is_not_reported_by_the_next_one(native_lib, ops):
+    """a device that is not there: the calls behind it say how they went themselves"""
+    import ctypes
+    import numpy as np
+    c = Cache(1, 2, 64, 16, "f16", 0, [3])
+    k = torch.randn(3, 2, 64, generator=c.g).cuda()
+    start, held = c.ints([0, 3]), c.ints([3])
+    x, w, y = np.ones(64, np.float32), np.ones(64, np.float32), np.zeros(64, np.float32)
+    ptr = lambda a: a.ctypes.data_as(ctypes.c_void_p)
+    torch.cuda.synchronize()
+    code = ctypes.c_uint32()
+    fails = [lambda: native_lib.b2_device_op_error(99, ctypes.byref(code)), lambda: native_lib.b2_token_logprobs(99, 256, 0, 8, 1, 8, None, None, 256, 0, None, None, None)]
+    for fail in fails:
+        assert fail() < 0 and "invalid device" in native_lib.b2_last_error().decode()
+        ops.kv_append(k, k, c.k, c.v, c.pages, start, held)
+        assert fail() < 0
+        assert native_lib.b2_op_rmsnorm(0, ptr(x), ptr(w), 1e-5, 64, 1, ptr(y)) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(c.k[c.pages[0, 0], :, :3], k.half().transpose(0, 1)) and np.abs(y - 1).max() < 1e-4
