@@ -487,9 +487,12 @@ int b2_token_logprobs(int device, const void* logits, int type, int64_t row_stri
                       const int32_t* tokens, float* logprob, float* entropy, int n_top, float* top_logprob,
                       int32_t* top_id, void* stream);
 
-/* Kernels of these operators bound every wait; the code of the first wait that ran out on the device (0: none; results
- * since then are not to be used). Waits for the device. */
+/* Kernels of these operators bound every wait; the code of the first wait that ran out on the device since the last time
+ * that this was asked (0: none; results of the calls in between are not to be used). Waits for all work on the device, so
+ * not while a stream is being captured. */
 int b2_device_op_error(int device, uint32_t* code);
+/* For tests: enqueue what a wait that ran out leaves behind (the words of one of two files), without the wait. */
+int b2_op_give_up(int device, int tensor_memory, uint32_t code, void* stream);
 
 #ifdef __cplusplus
 }

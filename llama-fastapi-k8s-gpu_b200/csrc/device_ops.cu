@@ -143,3 +143,8 @@ extern "C" int b2_device_op_error(int device, uint32_t* code) {
     if (on.status != cudaSuccess) return done("b2_device_op_error", on.status);
     return done("b2_device_op_error", shared_prefix_error(code));
 }
+
+extern "C" int b2_op_give_up(int device, int tensor_memory, uint32_t code, void* stream) {
+    OnDevice on(device);
+    return done("b2_op_give_up", on.status != cudaSuccess ? on.status : shared_prefix_give_up(code, tensor_memory != 0, (cudaStream_t)stream));
+}

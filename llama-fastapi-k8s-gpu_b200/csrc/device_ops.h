@@ -114,8 +114,20 @@ constexpr int SHARE_LEVELS = 8;
 struct PrefixShare { int adapt; size_t cut_at; int run[SHARE_LEVELS]; short ctas[SHARE_LEVELS], per_unit[SHARE_LEVELS]; };      // adapt 0: all SMs
 cudaError_t shared_prefix_tc_launch(const SharedPrefixArgs& a, const PrefixCut& cut, size_t ml_at, const PrefixShare& share, cudaStream_t s);      // ml_at: see SpPlan
 
-// code of the first wait of these kernels that ran out on the current device (0: none); waits for the device
+// code of the first wait of these kernels that ran out on the current device since the last call (0: none); waits for the device
 cudaError_t shared_prefix_error(unsigned int* code);
-cudaError_t shared_prefix_tc_error(unsigned int* code);
+cudaError_t shared_prefix_tc_error(unsigned int* code);      // (of that file; does not wait)
+// enqueue: what a wait that ran out leaves behind, without the wait (for tests)
+cudaError_t shared_prefix_give_up(unsigned int code, bool tensor_memory, cudaStream_t s);
+cudaError_t shared_prefix_tc_give_up(unsigned int code, cudaStream_t s);
+#ifdef __CUDACC__
+// a file's error words (see mbar_give_up): the code, and none from here on, so that later calls can be told apart from earlier ones
+template <size_t N>
+cudaError_t take_error_word(const unsigned int (&symbol)[N], unsigned int* code) {
+    const cudaError_t e = cudaMemcpyFromSymbol(code, symbol, sizeof(*code));
+    const unsigned int none = 0;
+    return e == cudaSuccess && *code ? cudaMemcpyToSymbol(symbol, &none, sizeof(none)) : e;
+}
+#endif
 
 }  // namespace b2

@@ -845,8 +845,20 @@ static bool sp_one_launch(const SharedPrefixArgs& a) {
 int shared_prefix_launches(const SharedPrefixArgs& a) { return a.n_prefix == 0 ? 1 : sp_one_launch(a) ? 2 : 3; }
 
 cudaError_t shared_prefix_error(unsigned int* code) {
-    const cudaError_t e = cudaMemcpyFromSymbol(code, sp_error, sizeof(*code));
-    return e == cudaSuccess && *code == 0 ? shared_prefix_tc_error(code) : e;
+    // (all streams: a copy on the default one does not wait for those that were made not to wait for it)
+    cudaError_t e = cudaDeviceSynchronize();
+    unsigned int more = 0;
+    if (e == cudaSuccess) e = take_error_word(sp_error, code);
+    if (e == cudaSuccess) e = shared_prefix_tc_error(&more);
+    if (e == cudaSuccess && *code == 0) *code = more;
+    return e;
+}
+__global__ void sp_give_up_kernel(unsigned int code) { mbar_give_up(0, sp_error, code, 0); }
+cudaError_t shared_prefix_give_up(unsigned int code, bool tensor_memory, cudaStream_t s) {
+    if (tensor_memory) return shared_prefix_tc_give_up(code, s);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = cfg.blockDim = dim3(1); cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, sp_give_up_kernel, code);
 }
 
 cudaError_t shared_prefix_launch(const SharedPrefixArgs& a, cudaStream_t s) {

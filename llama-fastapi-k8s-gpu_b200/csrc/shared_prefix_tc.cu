@@ -54,7 +54,13 @@ __device__ __forceinline__ int st_level(const SharedPrefixArgs& a) {
 }
 }  // namespace
 
-cudaError_t shared_prefix_tc_error(unsigned int* code) { return cudaMemcpyFromSymbol(code, st_error, sizeof(*code)); }
+cudaError_t shared_prefix_tc_error(unsigned int* code) { return take_error_word(st_error, code); }
+__global__ void st_give_up_kernel(unsigned int code) { mbar_give_up(0, st_error, code, 0); }
+cudaError_t shared_prefix_tc_give_up(unsigned int code, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = cfg.blockDim = dim3(1); cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, st_give_up_kernel, code);
+}
 
 template <int HD, bool F16>
 __global__ void __launch_bounds__(ST_THREADS, 1) shared_prefix_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,

@@ -140,6 +140,7 @@ SIGNATURES = {
     "b2_attention_shared_prefix_workspace": (c_int, [c_int] * 4 + [POINTER(c_int64)]),
     "b2_token_logprobs": (c_int, [c_int, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "b2_device_op_error": (c_int, [c_int, POINTER(ctypes.c_uint32)]),
+    "b2_op_give_up": (c_int, [c_int, c_int, ctypes.c_uint32, c_void_p]),
     "b2_op_sample": (c_int, [c_int, c_void_p, c_int, POINTER(B2Sampling), c_void_p, c_int, c_double, POINTER(c_int32)]),
 }
 

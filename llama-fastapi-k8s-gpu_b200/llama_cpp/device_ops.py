@@ -7,7 +7,8 @@ attending to the prompt's pages once for all of them, and reading the log probab
 A tensor is a torch tensor on a CUDA device, or anything with its `data_ptr()`, `shape`, `stride()`, `dtype`, `get_device()` and `is_contiguous()` (this
 package does not import torch itself); results go into tensors of the caller's, nothing is allocated. `stream` is a stream object with `cuda_stream`, its
 handle, or None for the default stream; the call only enqueues work there, so tensors that other streams use must be ordered by the caller. Wrong
-shapes, types or devices raise ValueError before anything is enqueued.
+shapes, types or devices raise ValueError before anything is enqueued. Waits inside the attention kernels are bounded: `error(device)` says
+whether one ran out since it was last asked, after which results are not to be used.
 
 A call is made by native code where that has been built (csrc/py_tensors.cpp: a single token's call is a few microseconds of device time, and reading a dozen
 tensors in Python takes more). What it does not take comes back here, where the same checks say what is wrong: one condition a tensor, and what was
@@ -236,3 +237,11 @@ def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_logprob=
         pti, ptl = _dense("top_id", top_id, (n, n_top), (_I32,), device), _dense("top_logprob", top_logprob, (n, n_top), (_F32,), device)
     check(_cabi.load_library().b2_token_logprobs(device, p, kind, stride[0] if n > 1 else vocab, n, vocab, pt, pl, pe, n_top, ptl, pti,
                                                  stream), "b2_token_logprobs")
+
+
+def error(device) -> int:
+    """Code of the first wait of attention_shared_prefix's kernels that ran out on this CUDA device since the last time that this was asked (0: none;
+    b2_device_op_error): results of the calls in between are not to be used. Waits for all work on the device; not while a stream is being captured."""
+    code = ctypes.c_uint32()
+    check(_cabi.load_library().b2_device_op_error(device, ctypes.byref(code)), "b2_device_op_error")
+    return code.value

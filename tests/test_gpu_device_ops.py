@@ -545,3 +545,25 @@ def test_a_failed_call_is_not_reported_by_the_next_one(native_lib, ops):
         assert native_lib.b2_op_rmsnorm(0, ptr(x), ptr(w), 1e-5, 64, 1, ptr(y)) == 0
     torch.cuda.synchronize()
     assert torch.equal(c.k[c.pages[0, 0], :, :3], k.half().transpose(0, 1)) and np.abs(y - 1).max() < 1e-4
+
+
+@pytest.mark.parametrize("tensor_memory", [0, 1])
+def test_a_wait_that_ran_out_is_reported_once(native_lib, tensor_memory):
+    """also from a stream that the default one does not wait for, behind work that is still under way"""
+    from llama_cpp import device_ops as ops
+    assert ops.error(0) == 0
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(int(2e8))
+    assert native_lib.b2_op_give_up(0, tensor_memory, 0x90001 + tensor_memory, side.cuda_stream) == 0
+    assert native_lib.b2_op_give_up(0, tensor_memory, 0x77, side.cuda_stream) == 0          # (not the first)
+    assert ops.error(0) == 0x90001 + tensor_memory
+    assert ops.error(0) == 0
+    for words in (0, 1):                                                                    # both files' words are taken at once
+        assert native_lib.b2_op_give_up(0, words, 0x11 + words, None) == 0
+    assert ops.error(0) == 0x11 and ops.error(0) == 0
+    with pytest.raises(RuntimeError):
+        ops.error(99)
+    with pytest.raises(RuntimeError):
+        ops.error(-1)
+    assert ops.error(0) == 0
