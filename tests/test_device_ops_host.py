@@ -104,6 +104,47 @@ def test_shared_prefix_workspace_covers_every_prefix(native_lib):
         need(4, 8, 3, 64)
 
 
+def own_slots(rows, heads, kv):
+    """partial results of own tokens: splits of the fewest CTAs that so many rows can be"""
+    tiles, n = -(-rows * (heads // kv) // 64) * kv, 1
+    while 2 * n <= 8 and tiles * 2 * n <= 2 * 148:
+        n *= 2
+    return n
+
+
+def prefix_cut(units, blocks, sms):
+    """the runs of key blocks that CTAs take: (length, cut unit by unit)"""
+    run = -(-units * blocks // sms)
+    parts = sms // units if units <= sms else 1
+    each = -(-blocks // parts)
+    return (each, True) if units <= sms and each <= run + 3 else (run, False)
+
+
+@pytest.mark.parametrize("rows,heads,kv,dim", [(1, 8, 8, 64), (8, 32, 8, 128), (33, 8, 8, 128), (9, 32, 8, 128), (12, 32, 8, 64), (16, 32, 8, 128), (5, 32, 4, 64), (17, 32, 8, 128),
+                                               (64, 32, 8, 128), (1, 64, 1, 64), (65, 64, 1, 64), (256, 32, 8, 128), (720, 32, 4, 64), (1000, 32, 4, 64), (5000, 8, 8, 128), (40, 149, 149, 64)])
+def test_prefix_results_stay_ahead_of_the_own_tokens(native_lib, rows, heads, kv, dim):
+    """The prefix's partial results of every length, cut end to end or unit by unit for any number of SMs that it may get, lie in the slots ahead of the own tokens'."""
+    from llama_cpp.device_ops import attention_shared_prefix_workspace as need
+    one = rows * heads * (dim + 2) * 4
+    total, rest = divmod(need(rows, heads, kv, dim), one)
+    assert rest == 16
+    prefix, group = total - own_slots(rows, heads, kv), heads // kv
+    if rows * group <= 32:
+        assert prefix == 32                                       # (that kernel's splits, 32 at most)
+        return
+    units = kv * -(-rows * group // 256)
+    most = 0
+    for blocks in [*range(1, 400), 1000, 8000, 100000]:
+        for sms in range(148, 20, -8):
+            run, per_unit = prefix_cut(units, blocks, sms)
+            if per_unit:
+                most = max(most, -(-blocks // run))
+                assert units * -(-blocks // run) <= sms
+            else:
+                most = max(most, *(((u + 1) * blocks - 1) // run - u * blocks // run + 1 for u in range(units)))
+    assert most <= prefix
+
+
 @pytest.mark.parametrize("sizes", [(2 ** 31 - 1, 512, 512, 128), (2 ** 30, 1024, 1024, 64), (2 ** 28, 4096, 4096, 64), (2 ** 27, 64, 1, 64), (2 ** 26, 32, 8, 128), (2 ** 32 + 5, 32, 8, 128),
                                    (-1, 32, 8, 128), (5, 2 ** 32 + 32, 8, 128)])
 def test_shared_prefix_workspace_refusals(native_lib, sizes):
