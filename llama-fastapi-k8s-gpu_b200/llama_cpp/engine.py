@@ -462,6 +462,8 @@ class LayeredEngine(EngineBase):
         """One ragged step that scores: log probabilities of given tokens instead of logits. entries as for `step`; want: per entry, indices into its tokens;
         tokens: per entry, for each of those, the token whose log probability is asked for (the one that follows, say). Returns (logprob, entropy, top_logprob,
         top_id) with a row per wanted token, in entry order. The entries must fit one native step."""
+        if not len(entries) == len(want) == len(tokens):
+            raise ValueError(f"{len(entries)} entries, {len(want)} lists of wanted rows and {len(tokens)} of tokens do not go together")
         flat, rows, asked, lens = [], [], [], []
         for (_, toks), w, t in zip(entries, want, tokens):
             if len(w) != len(t) or not all(0 <= i < len(toks) for i in w):

@@ -231,3 +231,23 @@ def test_common_prefix():
             b = list(a)
             b[i] += 10
             assert common_prefix(a, b) == common_prefix(b, a) == i
+
+
+def test_score_refuses_lists_that_do_not_go_together():
+    """one list of wanted rows and one of tokens an entry: the native step reads a length for every entry"""
+    from llama_cpp.engine import LayeredEngine
+    eng, calls = LayeredEngine.__new__(LayeredEngine), []
+
+    class Lib:
+        @staticmethod
+        def b2_step_scores(handle, n_entries, slots, lens, *rest):
+            calls.append((n_entries, len(slots), len(lens)))
+            return 0
+    eng.lib, eng._h = Lib, None
+    entries = [(0, [1, 2, 3]), (1, [4, 5])]
+    for want, tokens in (([[0]], [[7]]), ([[0], [1]], [[7]]), ([[0]], [[7], [8]]), ([[0], [1], []], [[7], [8], []]), ([], []), ([[0], [2]], [[7], [8]]), ([[0], [1]], [[7], [8, 9]])):
+        with pytest.raises(ValueError):
+            eng.score(entries, want, tokens)
+    assert not calls
+    eng.score(entries, [[0], []], [[7], []])
+    assert calls == [(2, 2, 2)]
