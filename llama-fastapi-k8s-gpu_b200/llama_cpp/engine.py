@@ -144,6 +144,8 @@ class EngineBase:
             raise ValueError("layer-list models start every sequence at position 0: pages cannot be shared")
         if slot == other:
             raise ValueError("a slot cannot share its own pages")
+        if n_tokens < 0 or not 0 <= min(slot, other) <= max(slot, other) < self.max_seqs:      # (ahead of the release)
+            raise ValueError(f"slots {slot} and {other} of {self.max_seqs} cannot share {n_tokens} tokens")
         self.pages.release(slot)
         n = self.pages.share(slot, other, n_tokens)
         self._set_table(slot)

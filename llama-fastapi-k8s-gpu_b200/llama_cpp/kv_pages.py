@@ -72,6 +72,8 @@ class PageAllocator:
 
     def share(self, seq_id: int, other: int, n_tokens: int) -> int:
         """Give seq_id, which must hold nothing, the whole pages of `other`'s first n_tokens. Returns the tokens they cover."""
+        if n_tokens < 0:
+            raise ValueError("n_tokens must not be negative")
         with self._lock:
             if self._owned.get(seq_id):
                 raise ValueError(f"sequence {seq_id} holds pages already")
@@ -84,6 +86,8 @@ class PageAllocator:
     def own_from(self, seq_id: int, n_tokens: int) -> int:
         """Before seq_id writes from its token n_tokens on: the pages from there on that others hold too are dropped from its table. Returns how many of
         its tokens are still cached: n_tokens, or fewer where the page of that token was shared (it is to be written anew)."""
+        if n_tokens < 0:
+            raise ValueError("n_tokens must not be negative")
         with self._lock:
             pages = self._owned.get(seq_id, [])
             first = next((i for i in range(n_tokens // self.block_tokens, len(pages)) if pages[i] in self._more), None)

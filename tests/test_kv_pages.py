@@ -79,3 +79,31 @@ def test_shared_pages_are_counted_and_never_written(ops):
         assert held.isdisjoint(a._free) and len(set(a._free)) == len(a._free)
         for p in held:
             assert len({t.index(p) for t in tables if p in t}) == 1
+
+
+def test_negative_tokens_are_refused():
+    """a negative count would be counted from the other table's end"""
+    from llama_cpp.kv_pages import PageAllocator
+    a = PageAllocator(20, 16)
+    assert a.ensure(0, 100)
+    for call in (lambda: a.share(1, 0, -1), lambda: a.share(1, 0, -17), lambda: a.own_from(0, -1)):
+        with pytest.raises(ValueError):
+            call()
+    assert a.table(1) == [] and len(a.table(0)) == 7 and a.free_pages == 13
+    assert a.share(1, 0, 0) == 0 and a.share(1, 0, 33) == 32
+    assert a.own_from(0, 20) == 16 and a.free_pages == 18      # (its second page is the other's too)
+
+
+def test_sharing_that_is_refused_leaves_the_slot_its_pages():
+    from llama_cpp.engine import EngineBase
+    from llama_cpp.kv_pages import PageAllocator
+    eng = EngineBase.__new__(EngineBase)
+    eng.pages, eng.max_seqs, eng._h, eng.lib, told = PageAllocator(20, 16), 3, None, None, []
+    eng._set_table = told.append
+    eng.pages.ensure(0, 100)
+    eng.pages.ensure(1, 50)
+    for slot, other, n in ((1, 0, -1), (1, 3, 32), (3, 0, 32), (-1, 0, 32), (1, -1, 32), (1, 1, 32)):
+        with pytest.raises(ValueError):
+            eng.share_pages(slot, other, n)
+    assert len(eng.pages.table(1)) == 4 and eng.pages.free_pages == 9 and not told
+    assert eng.share_pages(1, 0, 40) == 32 and told == [1] and eng.pages.free_pages == 13
