@@ -426,7 +426,7 @@ typedef struct b2_ragged_pages {
     int64_t table_stride;
     int64_t n_pages;          /* pages of the pools */
     int32_t max_pages, n_seqs /* <= 65535 */, n_rows;
-    int32_t block_tokens;     /* tokens of a page, a multiple of 16 */
+    int32_t block_tokens;     /* tokens of a page, a multiple of 16; max_pages * block_tokens < 2^31 - 4096 */
 } b2_ragged_pages;
 
 /* Append the rows' keys and values to the cache, the keys rotated by their positions; rotate the rows' queries beside

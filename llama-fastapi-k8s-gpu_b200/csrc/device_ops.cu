@@ -37,7 +37,8 @@ int check_where(const char* what, const b2_ragged_pages& w, RaggedPages& out) {
     if (w.n_seqs > 65535) return bad(what, "at most 65535 sequences");
     if (w.block_tokens <= 0 || w.block_tokens % 16) return bad(what, "block_tokens must be a positive multiple of 16");
     if (w.max_pages <= 0 || w.n_pages <= 0) return bad(what, "max_pages and n_pages must be positive");
-    if ((int64_t)w.max_pages * w.block_tokens > INT32_MAX) return bad(what, "max_pages * block_tokens must fit 32 bits");
+    // (kernels go on from the last token to the end of its tile and of a warp's page ids)
+    if ((int64_t)w.max_pages * w.block_tokens > INT32_MAX - 4096) return bad(what, "max_pages * block_tokens must fit 32 bits, less 4096");
     if (w.n_pages > INT32_MAX) return bad(what, "n_pages must fit 32 bits");
     if (w.n_seqs > 1 && w.table_stride < w.max_pages) return bad(what, "table_stride is smaller than max_pages");
     if (w.n_rows && w.n_seqs && (!w.row_start || !w.lengths || !w.pages)) return bad(what, "null row_start, lengths or pages");

@@ -113,8 +113,9 @@ struct SpWork {
         split = x % splits;
         r0 = 0; n_tok = a.r.n_rows; own = a.n_prefix; table = a.prefix_pages;
         if (own_pass) {
-            r0 = max(0, r.b); n_tok = min(r.e, a.r.n_rows) - r0; table = table_of(a, z);
-            own = min(r.held, a.r.max_pages * a.r.block_tokens);
+            // (whatever the arrays hold: limits and row numbers that wrapped would be followed)
+            r0 = min(max(r.b, 0), a.r.n_rows); n_tok = min(max(r.e, 0), a.r.n_rows) - r0; table = table_of(a, z);
+            own = min(max(r.held, 0), a.r.max_pages * a.r.block_tokens);
         }
         f0 = tile * mt; n_f = min(mt, (own_pass ? min(n_tok, a.max_rows) : n_tok) * G - f0);
         lim_lo = limit(f0 / G); lim_hi = limit((f0 + max(n_f, 1) - 1) / G);

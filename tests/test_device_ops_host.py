@@ -162,6 +162,15 @@ def test_shared_prefix_workspace_of_the_largest_sizes(native_lib):
         assert need(rows, heads, kv, dim) >= 2 * rows * heads * (dim + 2) * 4
 
 
+def test_tables_of_nearly_32_bits_of_tokens_are_refused(native_lib):
+    """the kernels count on from the last token to the end of its tile"""
+    for pages, ok in ((2 ** 27 - 1, False), (2 ** 27 - 256, False), (2 ** 27 - 257, True)):
+        for args, call in ((append_args, native_lib.b2_kv_append), (shared_args, native_lib.b2_attention_shared_prefix)):
+            where, x = args(max_pages=pages, block_tokens=16, table_stride=pages, n_rows=0)
+            assert (call(0, ctypes.byref(where), ctypes.byref(x), None) == 0) == ok
+            assert ok or "32 bits" in native_lib.b2_last_error().decode()
+
+
 LOGPROB_REFUSALS = [
     (dict(type=2), "f32, f16 or bf16"), (dict(n_rows=-1), "n_rows"), (dict(n_vocab=0), "n_vocab"), (dict(row_stride=99), "row_stride"), (dict(n_top=65), "n_top"),
     (dict(n_top=-1), "n_top"), (dict(logits=None), "null"), (dict(tokens=None), "null"), (dict(top_id=None), "null"), (dict(logits=66), "aligned"), (dict(entropy=66), "aligned"),

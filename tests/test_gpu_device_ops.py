@@ -305,6 +305,35 @@ def test_shared_prefix_lengths_past_the_table(ops):
     assert torch.equal(shared(ops, c, q, 40, [1]), good)
 
 
+@pytest.mark.parametrize("prefix", [0, 200])
+@pytest.mark.parametrize("rows,max_rows", [([130, 5, 1], 130), ([1, 1, 1], 1), ([3, 2, 3], 3)])
+def test_shared_prefix_lengths_at_the_end_of_32_bits(ops, prefix, rows, max_rows):
+    """lengths below zero are no own tokens, however far below: limits of rows would wrap to the other end"""
+    c = Cache(14, 4, 64, 16, "bf16", prefix, [0, 0, 0])
+    q = torch.randn(sum(rows), 32, 64, generator=c.g).bfloat16().cuda()
+    none = shared(ops, c, q, prefix, rows, max_rows=max_rows)
+    for own in ([-2 ** 31, -2 ** 31 + 2, -1], [-2 ** 31 + 100, -2 ** 31 + 129, -2 ** 31]):
+        c.own = own
+        assert torch.equal(shared(ops, c, q, prefix, rows, max_rows=max_rows), none)
+
+
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_shared_prefix_row_starts_that_are_no_numbers_of_rows(ops, prefix):
+    """sequences whose rows end below zero or begin behind the last have none"""
+    c = Cache(15, 4, 64, 16, "f16", prefix, [9, 9, 9, 9])
+    q = torch.randn(6, 32, 64, generator=c.g).half().cuda()
+    out = torch.full_like(q, 5.0)
+    work = torch.empty(ops.attention_shared_prefix_workspace(6, 32, 4, 64), dtype=torch.uint8, device="cuda")
+    run = lambda at: ops.attention_shared_prefix(q, c.k, c.v, c.prefix_pages, prefix, c.pages, c.ints(at), c.ints(c.own), out, work, max_rows=3)
+    run([0, 3, 3, 3, 3])
+    good = out.clone()
+    assert (good[3:] == 5.0).all() and (good[:3] != 5.0).any()
+    for at in ([0, 3, -2 ** 31, -2 ** 31, -2 ** 31], [0, 3, -1, -7, 0]):
+        out.fill_(5.0)
+        run(at)
+        assert torch.equal(out[:3], good[:3])
+
+
 # ------------------------------------------------------------------------------------------------------- log probabilities
 def logprob_bar(x, lp, entropy, V):
     """S is a sum of up to V / 256 + 40 terms a chain in 32 bits, of exponentials off by 2^-21: relative, so absolute in its logarithm; the difference to the
