@@ -8,7 +8,8 @@
 // Bound by memory: every entry is read once and written once. A CTA takes one row; a thread keeps one 16-byte piece of a head (both halves of a pair of pieces
 // under "halves", so that q may be rotated in place) and has three heads at a time. Its loads are under way while the row's sequence, its page and the angles
 // are found, a chain of two to three dependent reads; what hides that chain is other CTAs, so registers are few. Eight rows a CTA, which find all of that once, kept
-// too few CTAs on an SM (16384 rows of 48 heads of 128: 107 us instead of 93 with five CTAs an SM). Now 70 us there, 5.75 TB/s; 32 rows 4.0 us.
+// too few CTAs on an SM (16384 rows of 48 heads of 128: 107 us instead of 93 with five CTAs an SM). A row a CTA takes 70 us there in a graph, 5.75 TB/s, and 76 a call;
+// 32 rows 4.0 and 10.1.
 #include "device_ops.h"
 #include "ptx.cuh"
 #include <cuda_bf16.h>

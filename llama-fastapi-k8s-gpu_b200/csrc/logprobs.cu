@@ -5,13 +5,13 @@
 // the cluster. A masked entry (-infinity) adds nothing; a row of nothing else gets log probabilities of -infinity and entropy 0; a NaN makes the row's
 // numbers NaN.
 //
-// The most likely tokens come from the same pass: a thread's running maximum bounds its entries. Of the maxima of 32 to 128 groups of threads (two to four times n)
+// The most likely tokens come from the same pass: a thread's running maximum bounds its entries. Of the maxima of 32 to 128 groups of threads (at least twice n)
 // the n-th largest is reached by n entries at least, so that the n most likely are among the entries that reach it, which lie with the few threads whose maximum
 // does; their entries are read once more (from L2) and ranked by (value, lower id). Where those are too many (thousands of equal entries, a row masked but for
 // a few), the ones above the bound are ranked and the equal ones taken in the order of their ids; what that does not settle is searched n times.
 //
-// Bound by memory for many rows (each logit read once: 1024 rows of 128256 in 32 bits 93 us, 5.65 TB/s), by the latency of the phases behind the pass for few
-// (32 rows 13 us, of which the pass is 4; one row of 32000 7.6).
+// Bound by memory for many rows (each logit read once: 1024 rows of 128256 in 32 bits 93 us in a graph, 5.65 TB/s; 102 a call), by the latency of the phases behind the pass
+// for few (32 rows 13 us, of which the pass is 4; one row of 32000 7.6; calls 14.3 and 9.1).
 #include "device_ops.h"
 #include "ptx.cuh"
 #include <cuda_bf16.h>

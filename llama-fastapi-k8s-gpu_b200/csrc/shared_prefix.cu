@@ -12,7 +12,9 @@
 //   more rows (the prefix of a batch): shared_prefix_tc.cu, on tensor memory.
 // Both kernels here: mma.sync m16n8k16, keys and values by tensor copies (a warp of its own) in 128-byte-swizzled rows. They are bound by the copies, not by
 // the products: 32 rows of 64 keys want 1 % of the tensor cores.
-// The pass over own tokens runs beside the prefix pass (which leaves SMs or memory idle). Up to 16 rows of a KV head in the whole batch: one launch for both.
+// The pass over single own tokens runs beside the prefix pass, on SMs that one leaves it (sp_share). With several rows a sequence behind a prefix on tensor memory it has
+// the SMs that are left over, and else begins as CTAs of that pass end: no SM has registers for a CTA of each (320 and 160 threads of 168). Up to 16 rows of a KV
+// head in the whole batch: one launch for both.
 //
 // Probabilities are rounded to the cache's type for the weighted sum (the other operand is the cache as it is); scores, maxima, sums, joins stay 32-bit.
 #include "device_ops.h"
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(SP_THREADS, 3) shared_prefix_step_kernel(const
 }
 
 // Several tokens of a sequence, or the prefix pass of up to 32 rows: a tile of 64 rows, a warp has 16 of them and all keys. Own tokens of 40 sequences of 3 to 33
-// rows, 32 heads over 4 of 64: 13.5 us, most of it beside the prefix pass.
+// rows, 32 heads over 4 of 64: 13.5 us by themselves, behind a prefix most of them when its pass has ended.
 // grid: (tile * splits + split, KV head, sequence, or prefix)
 template <typename E, int HD>
 __global__ void __launch_bounds__(SP_THREADS, 2) shared_prefix_rows_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const SharedPrefixArgs a,
@@ -764,7 +766,7 @@ int sp_splits(long tiles, long keys, int most) {
 }
 // Up to so many rows a KV head the prefix is read by the kernels above, more by the pass on tensor memory. 32 heads over 8 KV heads of 128, prefixes of 512, 2000
 // and 8000, own tokens 20 to 500, these kernels / tensor memory: 20 rows 10.4 / 14.3, 17.7 / 18.6, 24.9 / 22.9 us; 32 rows 11.0 / 15.1, 18.0 / 19.5, 26.6 / 25.8;
-// 64 rows 14.9 / 15.0, 22.0 / 18.6, 34.7 / 27.1.
+// 64 rows 14.9 / 15.0, 22.0 / 18.6, 34.7 / 27.1. (The rule goes by rows alone, for a workspace that does not depend on the prefix: up to 2 us are lost behind 8000.)
 constexpr int SP_PREFIX_ROWS = 32;
 constexpr int SP_PREFIX_SPLITS = 32, SP_OWN_SPLITS = 8;
 }  // namespace

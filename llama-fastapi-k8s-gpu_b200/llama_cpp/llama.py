@@ -245,7 +245,7 @@ class Llama:
         """`cancel_event` (not in upstream): set it from another thread to abandon the generation; the call then returns
         what was produced so far with finish_reason "cancelled" and the sequence slot is free again. `logprobs` = n: the choice's "logprobs" holds every token's
         log probability and its n (at most 64) most likely alternatives, from the logits ahead of the penalties, as upstream; unlike there, no
-        `logits_all` is needed."""
+        `logits_all` is needed, and with `echo` the text holds the prompt but the log probabilities are the completion's alone. Such a request decodes step by step."""
         if logprobs is not None:
             if stream or not hasattr(self._engine, "set_logprobs"):
                 raise NotImplementedError("logprobs are not implemented for streamed completions" if stream else "this engine has no log probabilities")
@@ -281,7 +281,7 @@ class Llama:
         }
 
     def _logprobs_of(self, req: Request, offset: int) -> Dict[str, list]:
-        """The "logprobs" of a choice, shaped as upstream: tokens (those whose text the choice holds), where each begins in it, log probabilities, and per token a
+        """The "logprobs" of a choice, shaped as upstream: the completion's tokens (those whose text the choice holds), where each begins in it, log probabilities, and per token a
         dict of the alternatives' texts, the token itself among them."""
         out: Dict[str, list] = {"tokens": [], "text_offset": [], "token_logprobs": [], "top_logprobs": []}
         piece = lambda t: self._vocab.detokenize([t])
