@@ -36,6 +36,7 @@ extern "C" {
 #define B2_TYPE_Q5_K 13
 #define B2_TYPE_Q6_K 14
 #define B2_TYPE_I32 26    /* integer tables of layer-list models */
+#define B2_TYPE_U8 100    /* bytes of a cache in 4 bits (no GGUF type) */
 #define B2_TYPE_BF16 30   /* dense tensors of layer-list models (safetensors BF16) */
 
 typedef struct b2_engine b2_engine;
@@ -475,6 +476,51 @@ typedef struct b2_shared_prefix_args {
 int b2_attention_shared_prefix(int device, const b2_ragged_pages* where, const b2_shared_prefix_args* args, void* stream);
 /* bytes that a call with so many rows needs, whatever the lengths are */
 int b2_attention_shared_prefix_workspace(int n_rows, int n_head, int n_kv, int head_dim, int64_t* bytes);
+
+/* ---- a paged cache in 4 bits: 9/16 of a byte an entry instead of 2.
+ * A group is 32 neighbouring entries of a head. Its scale is m / -8 in f16, m the entry of greatest magnitude (of m and -m
+ * the negative one), held to the largest f16; an entry's code is round(entry / scale) + 8 (half to even) held to 0 .. 15, 8
+ * where the scale is 0; it stands for scale * (code - 8). A group that holds an infinity or a NaN reads as NaN. Pools are
+ * bytes, [n_pages][n_kv][block_tokens / 16][9 * head_dim]: a page is copied, shared or moved as any other, its insides are
+ * written and read by these calls alone. head_dim 64 or 128, pools 16-byte aligned. */
+
+/* b2_kv_append into a cache in 4 bits: pools in that form, cache_type is q_out's type. The rotation's angles, sines and
+ * cosines are computed in 64 bits, the latter rounded once, its products and sums in 32 bits one by one, and the codes from
+ * those; so the same rows always get the same codes. */
+int b2_kv_append_4bit(int device, const b2_ragged_pages* where, const b2_kv_append_args* args, void* stream);
+
+/* The rows' keys and values back (row i of n: token lengths[s] - n + i, as for appends), rounded once to out_type. Rows
+ * whose place is not in their table, whose page id is outside the pool or that have no sequence are left as they are. k or v
+ * may be NULL. */
+typedef struct b2_kv_read_4bit_args {
+    const void *k_pool, *v_pool;
+    void *k, *v;              /* [n_rows][n_kv][head_dim] of out_type */
+    int64_t k_row, k_head, v_row, v_head;    /* strides */
+    int32_t n_kv, head_dim;
+    int32_t out_type;         /* B2_TYPE_F32, _F16 or _BF16 */
+} b2_kv_read_4bit_args;
+int b2_kv_read_4bit(int device, const b2_ragged_pages* where, const b2_kv_read_4bit_args* args, void* stream);
+
+/* Attention of a ragged batch over a cache in 4 bits: row i of a sequence sees its tokens up to itself.
+ * out = softmax(scale * q.k) v over them, 0 where there are none. Queries and output are f16 or bf16; scores, maxima and sums
+ * are 32-bit, probabilities and values are rounded to f16 for the weighted sum. max_rows: most rows any sequence has (rows
+ * past it are not computed); 1 for single tokens. Page ids are held inside the pool. n_head a multiple of n_kv, at most 64
+ * times it. Lengths may be smaller than a sequence's rows (the rows ahead see nothing). Partial results of keys go
+ * through the workspace, 16-byte aligned. */
+typedef struct b2_attention_4bit_args {
+    const void* q;            /* [n_rows][n_head][head_dim] */
+    const void *k_pool, *v_pool;
+    void* out;                /* like q */
+    void* workspace;          /* b2_attention_4bit_workspace bytes */
+    int64_t workspace_bytes;
+    int64_t q_row, q_head, out_row, out_head;
+    int32_t max_rows, n_head, n_kv, head_dim;
+    int32_t type;             /* B2_TYPE_F16 or _BF16 */
+    float scale;              /* > 0, usually 1 / sqrt(head_dim) */
+} b2_attention_4bit_args;
+int b2_attention_4bit(int device, const b2_ragged_pages* where, const b2_attention_4bit_args* args, void* stream);
+/* bytes that a call with so many rows needs, whatever the lengths are */
+int b2_attention_4bit_workspace(int n_rows, int n_head, int n_kv, int head_dim, int64_t* bytes);
 
 /* Log softmax of logits [n_rows][n_vocab] (rows row_stride elements apart; B2_TYPE_F32, _F16 or _BF16): the log
  * probability of tokens[r] -> logprob[r], the entropy (nats) -> entropy[r] (either may be NULL), and the n_top (0..64)

@@ -17,7 +17,7 @@ import sysconfig
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.environ.get("B2_LIB_DIR") or os.path.join(HERE, "lib")   # B2_LIB_DIR: experiment builds (with B2_NVCC_EXTRA)
-CUDA_SOURCES = ["engine.cu", "layered.cu", "dense.cu", "dense_tc.cu", "dense_split.cu", "mixers.cu", "state_mixers.cu", "latent_attn.cu", "latent_tc.cu", "sigmoid_attn.cu", "sink_attn.cu", "softmax_tc.cu", "hyper.cu", "moe.cu", "matvec.cu", "matvec_extra.cu", "attention.cu", "attention_mma.cu", "gemm.cu", "prefill.cu", "prefill_tc.cu", "misc.cu", "sampler.cu", "device_ops.cu", "kv_append.cu", "logprobs.cu", "shared_prefix.cu", "shared_prefix_tc.cu", "tp.cu"]
+CUDA_SOURCES = ["engine.cu", "layered.cu", "dense.cu", "dense_tc.cu", "dense_split.cu", "mixers.cu", "state_mixers.cu", "latent_attn.cu", "latent_tc.cu", "sigmoid_attn.cu", "sink_attn.cu", "softmax_tc.cu", "hyper.cu", "moe.cu", "matvec.cu", "matvec_extra.cu", "attention.cu", "attention_mma.cu", "gemm.cu", "prefill.cu", "prefill_tc.cu", "misc.cu", "sampler.cu", "device_ops.cu", "kv_append.cu", "kv_4bit.cu", "attention_4bit.cu", "logprobs.cu", "shared_prefix.cu", "shared_prefix_tc.cu", "tp.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--expt-relaxed-constexpr"]
 
@@ -70,7 +70,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
             raise RuntimeError("link failed")
     host = os.path.join(LIB, "libb200_hosttest.so")
     hsrc = os.path.join(CSRC, "host_selftest.cpp")
-    if force or _newer(host, [hsrc, *(os.path.join(CSRC, f) for f in ("quant_blocks.cuh", "gemm_ring.h", "per_device.h", "shared_group.h"))]):
+    if force or _newer(host, [hsrc, *(os.path.join(CSRC, f) for f in ("quant_blocks.cuh", "gemm_ring.h", "kv_4bit.cuh", "per_device.h", "shared_group.h"))]):
         subprocess.run(["g++", "-O2", "-ffp-contract=off", "-fPIC", "-shared", hsrc, "-o", host], check=True)
     lists, include = os.path.join(LIB, "libb200_pylists" + sysconfig.get_config_var("EXT_SUFFIX")), sysconfig.get_paths()["include"]
     lsrc = [os.path.join(CSRC, f) for f in ("py_lists.cpp", "py_tensors.cpp")]

@@ -1,0 +1,619 @@
+// Attention of a ragged batch over a paged cache in 4 bits (kv_4bit.cuh).
+//   keys of row i of a sequence with n rows and c tokens: tokens 0 .. c - n + i;   out = sum_j 2^(s_j - m) v_j / sum_j 2^(s_j - m), s_j = scale log2(e) q.k_j. No key: 0.
+// Bound by the bytes of the cache (9/16 of a byte an entry) and, close behind, by the instructions that turn codes into operands.
+//
+// A warp works by itself: it has its own ring of steps of 32 keys, its own copies, and keeps the weighted sums of all dims. The steps of all (sequence, KV head, tile of rows)
+// laid end to end are cut into equal runs, one a warp; a run that begins or ends inside such a segment leaves a partial result (maximum, sum, weighted sum, 32 bits) there.
+// The CTA's warps join theirs through shared memory at the end, a small kernel joins those of several CTAs. All joins go in the order of the keys.
+//
+// Products are transposed, keys (dims) times rows, so that eight rows fill an instruction: mma.sync m16n8k16.
+//   scores: the operand of the keys is the codes c themselves as the subnormal f16 numbers c 2^-24 (c 2^-20 for every other one, where the query's entry is 1/16 of itself): a mask
+//     and nothing else. Queries are held in f16 at a power of two that puts a row's largest entry near 2^10; the code's offset of 8 is the sum's initial value, -8 2^-24 sum q
+//     over the group, and the group's scale multiplies the group's sum in 32 bits. No key is rounded.
+//   weighted sums: c - 8 times the scale, rounded to f16, and probabilities in f16 (2^-11 each), whatever the type of queries and output. The score fragment becomes the
+//     probabilities' operand by movmatrix.
+// The reference of a row's exponentials moves only where a score exceeds it by 2^6.
+#include "device_ops.h"
+#include "kv_4bit.cuh"
+#include "ptx.cuh"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <algorithm>
+#include <math.h>
+
+namespace b2 {
+
+namespace {
+constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS;
+constexpr int A4_KEYS = 32;          // keys of a step: two blocks of 16
+constexpr int A4_STAGES = 3;         // steps under way
+constexpr int A4_SMS = 148;
+
+__device__ unsigned int a4_error[5];                             // see mbar_give_up
+
+__device__ __forceinline__ float a4_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
+__device__ __forceinline__ uint32_t a4_half2(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+__device__ __forceinline__ __half2 a4_as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t a4_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ void a4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t a4_transpose(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+// chunks of a block's row: 16 bytes for heads of 128, 8 for heads of 64
+template <int NG> __device__ __forceinline__ void a4_chunk(const uint8_t* p, uint32_t (&w)[NG]) {
+    if constexpr (NG == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    else { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+}
+
+// what is known of a sequence: its first row, its rows (those that are computed), its tokens, and the keys that its first row sees
+struct A4Seq {
+    int r0, n, own, lim0, tiles, steps;
+    __device__ A4Seq() {}
+    __device__ A4Seq(const Attention4Args& a, int z, int mt) {
+        r0 = min(max(a.r.row_start[z], 0), a.r.n_rows);
+        const int all = max(min(max(a.r.row_start[z + 1], 0), a.r.n_rows) - r0, 0);      // (whatever the arrays hold)
+        n = min(all, a.max_rows);
+        own = min(max(a.r.lengths[z], 0), a.r.max_pages * a.r.block_tokens);
+        lim0 = own - all + 1;
+        tiles = (int)(((long)n * (a.n_head / a.n_kv) + mt - 1) / mt);
+        steps = n ? max(1, (own + A4_KEYS - 1) / A4_KEYS) : 0;
+    }
+    __device__ long units(int n_kv) const { return (long)n_kv * tiles * steps; }
+    __device__ int limit(int i) const { return max(0, lim0 + i); }                      // keys that row i sees
+};
+// a place in the steps of all segments laid end to end
+struct A4At {
+    int z, kvh, tile, step;
+    A4Seq s;
+    __device__ void next(const Attention4Args& a, int mt) {
+        if (++step < s.steps) return;
+        step = 0;
+        if (++tile < s.tiles) return;
+        tile = 0;
+        if (++kvh < a.n_kv) return;
+        kvh = 0;
+        do { if (++z >= a.r.n_seqs) return; s = A4Seq(a, z, mt); } while (s.steps == 0);
+    }
+};
+
+// partial results in 32 bits: [rows of a tile][D] weighted sums, then [rows][2] (reference in log2, sum)
+template <int D> __host__ __device__ constexpr int a4_part(int mt) { return mt * (D + 2); }
+
+// four neighbouring dims of a row's output
+__device__ __forceinline__ void a4_store_out(const Attention4Args& a, int t, int head, int d, float x, float y, float z, float w) {
+    uint32_t lo, hi;
+    if (a.type == ELEM_F16) { lo = a4_half2(x, y); hi = a4_half2(z, w); }
+    else {
+        const __nv_bfloat162 l = __floats2bfloat162_rn(x, y), h = __floats2bfloat162_rn(z, w);
+        lo = *reinterpret_cast<const uint32_t*>(&l); hi = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    uint16_t* dst = (uint16_t*)a.out + (size_t)t * a.out_row + (size_t)head * a.out_head + d;
+    if (((uintptr_t)dst & 7) == 0) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
+    else { dst[0] = (uint16_t)lo; dst[1] = (uint16_t)(lo >> 16); dst[2] = (uint16_t)hi; dst[3] = (uint16_t)(hi >> 16); }
+}
+
+// where a CTA's results of a segment that goes on in another CTA lie: the first, of one that began in an earlier CTA, and the last
+struct A4Desc { int rows, r0, f0, kvh, last; };      // rows of the tile (0: no such result), first row of the sequence, first (row, head) of the tile, the CTA where the segment ends
+template <int PART> __device__ __forceinline__ A4Desc* a4_desc(const Attention4Args& a, int ctas) { return reinterpret_cast<A4Desc*>(a.work + (size_t)ctas * 2 * PART); }
+
+// results of the same row over different keys, added up
+struct A4Sum {
+    float m = -INFINITY, l = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    __device__ __forceinline__ void most(float ref) { m = fmaxf(m, ref); }
+    __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+    __device__ __forceinline__ void fall(float before) {
+        const float c = a4_exp2(before - base());
+        l *= c; v.x *= c; v.y *= c; v.z *= c; v.w *= c;
+    }
+    __device__ __forceinline__ void add(float2 ml, float4 x) {
+        const float c = a4_exp2(ml.x - base());
+        l = fmaf(c, ml.y, l);
+        v.x = fmaf(c, x.x, v.x); v.y = fmaf(c, x.y, v.y); v.z = fmaf(c, x.z, v.z); v.w = fmaf(c, x.w, v.w);
+    }
+    __device__ __forceinline__ void out(const Attention4Args& a, int t, int head, int d) const {
+        const float inv = l == 0.f ? 0.f : 1.f / l;              // (0: no keys. A NaN stays one.)
+        a4_store_out(a, t, head, d, v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    }
+};
+
+// CTAs of a call: as many as run at once, no more than there can be steps for
+constexpr int A4_PER_SM[2] = {3, 2}, A4_MOST_CTAS = A4_SMS * 3;      // (of tiles of 8 and of 16 rows)
+inline int a4_ctas(const Attention4Args& a, int mt) {
+    const long steps = ((long)a.r.max_pages * a.r.block_tokens + A4_KEYS - 1) / A4_KEYS;
+    const double units = (double)a.r.n_seqs * a.n_kv * (((double)a.max_rows * (a.n_head / a.n_kv) + mt - 1) / mt) * steps;
+    return (int)std::min<double>(A4_SMS * A4_PER_SM[mt > 8], std::ceil(units / A4_WARPS));
+}
+}  // namespace
+
+template <int D, int NT>
+__global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_step_kernel(const Attention4Args a) {
+    constexpr int NG = D / Q4_GROUP, BLOCK = q4_block(D), STAGE = 4 * BLOCK, S = A4_STAGES, MT = 8 * NT, PART = a4_part<D>(MT);
+    constexpr int REGION = S * STAGE > PART * 4 ? S * STAGE : PART * 4;
+    extern __shared__ __align__(128) uint8_t a4_raw[];
+    __shared__ uint64_t full[A4_WARPS][S];
+    struct Held { int rows, r0, f0, kvh, ends, last; };          // rows 0: no result; `last`: the CTA where the segment ends
+    __shared__ Held held[A4_WARPS][2];                           // of segments that began before the warp's run, and that go on behind it
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+    uint8_t* ring = a4_raw + warp * REGION;                      // behind the last step: the result of a segment that goes on
+    float* const head_part = reinterpret_cast<float*>(a4_raw + A4_WARPS * REGION);      // [warp] results of segments that began before
+    if (lane == 0) {
+        for (int i = 0; i < S; i++) mbar_init(&full[warp][i], 1);
+        held[warp][0].rows = held[warp][1].rows = 0;
+        fence_mbar_init();
+    }
+    griddep_wait();
+    griddep_launch();
+    __syncwarp();
+    const int n_kv = a.n_kv, G = a.n_head / n_kv, bt = a.r.block_tokens, blocks = bt / Q4_TOKENS;
+
+    // ---- the steps of all sequences, and this warp's run [u0, u1) of them
+    long total = 0;
+    for (int z = lane; z < a.r.n_seqs; z += 32) total += A4Seq(a, z, MT).units(n_kv);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    const long all_warps = (long)gridDim.x * A4_WARPS, warps = min(all_warps, total), me = (long)blockIdx.x * A4_WARPS + warp;
+    // the first `longer` runs have a step more than the others
+    const long run = warps ? total / warps : 0, longer = total - run * warps;
+    const long u0 = me < warps ? run * me + min(me, longer) : 0, u1 = me < warps ? u0 + run + (me < longer) : 0;
+    A4At at;
+    at.z = a.r.n_seqs; at.kvh = at.tile = at.step = 0;
+    if (u0 < u1) {
+        long before = 0;
+        for (int z0 = 0; z0 < a.r.n_seqs; z0 += 32) {
+            const long mine = z0 + lane < a.r.n_seqs ? A4Seq(a, z0 + lane, MT).units(n_kv) : 0;
+            long sum = mine;                                     // of sequences z0 .. z0 + lane
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) { const long v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
+            const unsigned past = __ballot_sync(0xffffffffu, before + sum > u0);
+            if (past) {
+                const int l = __ffs(past) - 1;
+                at.z = z0 + l;
+                at.s = A4Seq(a, at.z, MT);
+                long rest = u0 - before - __shfl_sync(0xffffffffu, sum - mine, l);
+                const long per = (long)at.s.tiles * at.s.steps;
+                at.kvh = (int)(rest / per); rest -= at.kvh * per;
+                at.tile = (int)(rest / at.s.steps); at.step = (int)(rest - (long)at.tile * at.s.steps);
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+    }
+
+    // ---- copies: lanes 0 .. 3 have keys and values of the step's two blocks, the page's id read a step ahead
+    A4At ahead = at;
+    long copied = u0;
+    const int c_kv = lane >> 1 & 1, c_blk = lane & 1;
+    auto page_of = [&]() {
+        const int t = ahead.step * A4_KEYS + c_blk * Q4_TOKENS;
+        return lane < 4 && copied < u1 && t < ahead.s.own ? a.r.pages[ahead.z * a.r.table_stride + t / bt] : 0;
+    };
+    int id = page_of(), put = 0;
+    auto copy = [&]() {
+        if (copied >= u1) return;
+        const int t0 = ahead.step * A4_KEYS, n = min(2, (ahead.s.own - t0 + Q4_TOKENS - 1) / Q4_TOKENS);
+        if (lane == 0) mbar_arrive_expect_tx(&full[warp][put], (uint32_t)(max(n, 0) * 2 * BLOCK));
+        __syncwarp();
+        if (lane < 4 && c_blk < n) {
+            const int t = t0 + c_blk * Q4_TOKENS;
+            const long page = min(max((long)id, 0l), a.r.n_pages - 1);
+            const uint8_t* from = (const uint8_t*)(c_kv ? a.v_pool : a.k_pool) + ((page * n_kv + ahead.kvh) * blocks + t % bt / Q4_TOKENS) * BLOCK;
+            tma_load_1d(ring + put * STAGE + (c_kv * 2 + c_blk) * BLOCK, from, BLOCK, &full[warp][put]);
+        }
+        __syncwarp();
+        put = put + 1 == S ? 0 : put + 1;
+        ahead.next(a, MT);
+        copied++;
+        id = page_of();
+    };
+    for (int i = 0; i < S; i++) copy();
+
+    int st = 0;
+    uint32_t parity = 0;
+    for (long u = u0; u < u1;) {
+        // ================= a segment: queries, as the fragments of eight rows each; rows past the tile's are zeros
+        const A4Seq& s = at.s;
+        const int kvh = at.kvh, f0 = at.tile * MT, n_f = (int)min((long)MT, (long)s.n * G - f0), r0 = s.r0;
+        const long left = s.steps - at.step;
+        const int n = (int)min(left, u1 - u), step0 = at.step;
+        const bool begins = step0 == 0, ends = n == left;
+        uint32_t qb[NT][NG][4];
+        float off[NT][NG][2], by[NT][2];                         // of rows 2 tq and 2 tq + 1: the sums' initial values, and what a score is multiplied with
+        int lim[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int f = f0 + nt * 8 + g;
+            const bool in = nt * 8 + g < n_f;
+            const int i = in ? f / G : 0;
+            const size_t q_at = (size_t)(r0 + i) * a.q_row + (size_t)(kvh * G + (in ? f - i * G : 0)) * a.q_head + 8 * tq;
+            const uint16_t* q = (const uint16_t*)a.q + q_at;
+            uint4 raw[NG];
+#pragma unroll
+            for (int gi = 0; gi < NG; gi++) {
+                raw[gi] = make_uint4(0, 0, 0, 0);
+                if (!in) continue;
+                const uint16_t* p = q + gi * Q4_GROUP;
+                if (((uintptr_t)p & 15) == 0) raw[gi] = *reinterpret_cast<const uint4*>(p);
+                else raw[gi] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+            }
+            auto value = [&](int gi, int e) {
+                const uint32_t w = e < 2 ? raw[gi].x : e < 4 ? raw[gi].y : e < 6 ? raw[gi].z : raw[gi].w;
+                const uint16_t v = (uint16_t)(e & 1 ? w >> 16 : w);
+                return a.type == ELEM_F16 ? __half2float(__ushort_as_half(v)) : __uint_as_float((uint32_t)v << 16);
+            };
+            float top = 0.f;
+#pragma unroll
+            for (int gi = 0; gi < NG; gi++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(value(gi, e)));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
+            const float up = __uint_as_float((uint32_t)(137 - ex) << 23);                // 2^(10 - ex)
+            const float mine = scalbnf(a.scale_log2, ex + 14);                           // (2^24 of the codes, 2^(ex - 10) of the queries)
+#pragma unroll
+            for (int j = 0; j < 2; j++) by[nt][j] = __shfl_sync(0xffffffffu, mine, (2 * tq + j) * 4);
+#pragma unroll
+            for (int gi = 0; gi < NG; gi++) {
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {                    // entries e and e + 4: the codes e and e + 4 of a word are masked out together
+                    const float down = e & 1 ? 0.0625f : 1.f;
+                    const uint32_t h = a4_half2(value(gi, e) * up * down, value(gi, e + 4) * up * down);
+                    qb[nt][gi][e] = h;
+                    const float2 back = __half22float2(a4_as_half2(h));
+                    sum = fmaf(back.x + back.y, e & 1 ? 16.f : 1.f, sum);
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+                for (int j = 0; j < 2; j++) off[nt][gi][j] = __shfl_sync(0xffffffffu, sum, (2 * tq + j) * 4) * -0x1p-21f;      // 8 2^-24
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int row = nt * 8 + 2 * tq + j;
+                lim[nt][j] = row < n_f ? min(s.limit((f0 + row) / G), s.own) : s.own;
+            }
+        }
+        const int own = s.own, lim_lo = min(s.limit(f0 / G), own);                       // keys that all rows of the tile see
+        float o[NT][NG][2][4], ref[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            ref[nt][0] = ref[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+            for (int gi = 0; gi < NG; gi++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) o[nt][gi][e >> 2][e & 3] = 0.f;
+        }
+
+        for (int i = 0; i < n; i++) {
+            const int t0 = (step0 + i) * A4_KEYS;
+            const uint8_t* stage = ring + st * STAGE;
+            mbar_wait_warp(&full[warp][st], parity, a4_error, 0xb0001u, (unsigned)i);
+            // ---- scores: keys g and g + 8 of both blocks, rows 2 tq and 2 tq + 1
+            float sc[2][NT][4];
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const uint8_t* kb = stage + b * BLOCK;
+                uint32_t w[2][NG];
+                float ks[2][NG];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int key = g + 8 * h;
+                    a4_chunk<NG>(kb + key * (D / 2) + q4_chunk(D, key, tq) * NG * 4, w[h]);
+                    const __half2* sp = reinterpret_cast<const __half2*>(kb + q4_key_scale(D, key, 0));
+#pragma unroll
+                    for (int gi = 0; gi < NG; gi += 2) { const float2 v = __half22float2(sp[gi >> 1]); ks[h][gi] = v.x; ks[h][gi + 1] = v.y; }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) sc[b][nt][0] = sc[b][nt][1] = sc[b][nt][2] = sc[b][nt][3] = 0.f;
+#pragma unroll
+                for (int gi = 0; gi < NG; gi++) {
+                    const uint32_t x = w[0][gi], y = w[1][gi], x8 = x >> 8, y8 = y >> 8;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        float c[4] = {off[nt][gi][0], off[nt][gi][1], off[nt][gi][0], off[nt][gi][1]};
+                        a4_mma(c, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[nt][gi][0], qb[nt][gi][1]);
+                        a4_mma(c, x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u, qb[nt][gi][2], qb[nt][gi][3]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) sc[b][nt][e] = fmaf(ks[e >> 1][gi], c[e], sc[b][nt][e]);
+                    }
+                }
+            }
+            const bool part = t0 + A4_KEYS > lim_lo;             // not every row sees all of these keys
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float v = sc[b][nt][e] * by[nt][e & 1];
+                        sc[b][nt][e] = part && t0 + b * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? -INFINITY : v;
+                    }
+            // ---- the reference goes up where a score is far above it
+            bool above = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float mx = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]), fmaxf(sc[1][nt][j], sc[1][nt][j + 2]));
+                    above |= mx > ref[nt][j] + 6.f;
+                }
+            if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        float mx = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]), fmaxf(sc[1][nt][j], sc[1][nt][j + 2]));
+#pragma unroll
+                        for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                        mx = fmaxf(mx, ref[nt][j]);
+                        const float fall = ref[nt][j] == -INFINITY ? 0.f : a4_exp2(ref[nt][j] - mx);
+                        ref[nt][j] = mx;
+                        l[nt][j] *= fall;
+#pragma unroll
+                        for (int gi = 0; gi < NG; gi++)
+#pragma unroll
+                            for (int m = 0; m < 2; m++) { o[nt][gi][m][j] *= fall; o[nt][gi][m][j + 2] *= fall; }
+                    }
+            }
+            // ---- probabilities, as operands with keys in pairs
+            uint32_t pb[2][NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                const float r0f = ref[nt][0] == -INFINITY ? 0.f : ref[nt][0], r1f = ref[nt][1] == -INFINITY ? 0.f : ref[nt][1];
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const float p0 = a4_exp2(sc[b][nt][0] - r0f), p1 = a4_exp2(sc[b][nt][1] - r1f), p2 = a4_exp2(sc[b][nt][2] - r0f), p3 = a4_exp2(sc[b][nt][3] - r1f);
+                    l[nt][0] += p0 + p2; l[nt][1] += p1 + p3;
+                    pb[b][nt][0] = a4_transpose(a4_half2(p0, p1)); pb[b][nt][1] = a4_transpose(a4_half2(p2, p3));
+                }
+            }
+            // ---- weighted sums: dims 32 gi + 4 g + 2 m and + 1, keys 2 tq, 2 tq + 1 and the two 8 further on
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+                const int k0 = t0 + b * 16;
+                if (k0 >= own) break;
+                const uint8_t* vb = stage + (2 + b) * BLOCK;
+                const int chunk = q4_chunk(D, 2 * tq, g >> 1) * NG * 4;
+                uint32_t w[4][NG], vs[NG][2];
+#pragma unroll
+                for (int k = 0; k < 4; k++) a4_chunk<NG>(vb + (2 * tq + (k & 1) + 8 * (k >> 1)) * (D / 2) + chunk, w[k]);
+#pragma unroll
+                for (int gi = 0; gi < NG; gi += 2) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(vb + q4_value_scale(D, 2 * tq, gi));
+                    vs[gi][0] = v.x; vs[gi][1] = v.y; vs[gi + 1][0] = v.z; vs[gi + 1][1] = v.w;
+                }
+                bool bad = false;
+                if (k0 + 16 > lim_lo) {
+                    // keys that nobody sees: whatever lies there must not meet the zero weights as a value. A value that is no number must not reach rows that do not see it.
+#pragma unroll
+                    for (int gi = 0; gi < NG; gi++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int key = k0 + 2 * tq + 8 * h;
+                            vs[gi][h] &= (key < own ? 0xffffu : 0u) | (key + 1 < own ? 0xffff0000u : 0u);
+                            bad |= (vs[gi][h] & 0x7c00u) == 0x7c00u || (vs[gi][h] & 0x7c000000u) == 0x7c000000u;
+                        }
+                    bad = __any_sync(0xffffffffu, bad && lim_lo < own);
+                }
+                const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;  // this lane's four dims of a word
+                auto products = [&](auto&& sums) {
+#pragma unroll
+                    for (int gi = 0; gi < NG; gi++) {
+                        const uint32_t x = __byte_perm(w[0][gi], w[1][gi], sel), y = __byte_perm(w[2][gi], w[3][gi], sel);
+                        const __half2 s0 = a4_as_half2(vs[gi][0]), s1 = a4_as_half2(vs[gi][1]);
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {
+                            // 1024 + c and 1024 + 16 c as f16 numbers, then c - 8, all exact
+                            auto low = [&](uint32_t v) { return __hsub2(a4_as_half2((v >> (8 * m) & 0x000f000fu) | 0x64006400u), a4_as_half2(0x64086408u)); };
+                            auto high = [&](uint32_t v) { return __hfma2(a4_as_half2((v >> (8 * m) & 0x00f000f0u) | 0x64006400u), a4_as_half2(0x2c002c00u), a4_as_half2(0xd480d480u)); };
+                            sums(gi, m, a4_bits(__hmul2(low(x), s0)), a4_bits(__hmul2(high(x), s0)), a4_bits(__hmul2(low(y), s1)), a4_bits(__hmul2(high(y), s1)));
+                        }
+                    }
+                };
+                if (!bad) {
+                    products([&](int gi, int m, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) a4_mma(o[nt][gi][m], a0, a1, a2, a3, pb[b][nt][0], pb[b][nt][1]);
+                    });
+                } else {
+                    // row by row of the sequence: only the keys that it sees, only its heads' sums
+#pragma unroll 1
+                    for (int t = f0 / G; t <= (f0 + n_f - 1) / G; t++) {
+                        const int most = min(s.limit(t), own);
+                        uint32_t keep[NG][2];
+#pragma unroll
+                        for (int gi = 0; gi < NG; gi++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                const int key = k0 + 2 * tq + 8 * h;
+                                keep[gi][h] = vs[gi][h];
+                                vs[gi][h] &= (key < most ? 0xffffu : 0u) | (key + 1 < most ? 0xffff0000u : 0u);
+                            }
+                        products([&](int gi, int m, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) {
+                                float c[4] = {o[nt][gi][m][0], o[nt][gi][m][1], o[nt][gi][m][2], o[nt][gi][m][3]};
+                                a4_mma(c, a0, a1, a2, a3, pb[b][nt][0], pb[b][nt][1]);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) if ((f0 + nt * 8 + 2 * tq + (e & 1)) / G == t) o[nt][gi][m][e] = c[e];
+                            }
+                        });
+#pragma unroll
+                        for (int gi = 0; gi < NG; gi++) { vs[gi][0] = keep[gi][0]; vs[gi][1] = keep[gi][1]; }
+                    }
+                }
+            }
+            __syncwarp();                                        // the step's memory is free
+            copy();
+            if (++st == S) { st = 0; parity ^= 1; }
+        }
+        u += n;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
+        // ---- output, or a result for the joins
+        const int slot = begins ? 1 : 0;
+        float* part_at = begins ? reinterpret_cast<float*>(ring) : head_part + warp * PART;      // (a segment that goes on is the run's last: no copy is under way)
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int row = nt * 8 + 2 * tq + j;
+                if (row >= n_f) continue;
+                if (begins && ends) {
+                    const int f = f0 + row, i = f / G;
+                    const float inv = l[nt][j] == 0.f ? 0.f : 1.f / l[nt][j];            // (0: no keys. A NaN stays one.)
+#pragma unroll
+                    for (int gi = 0; gi < NG; gi++)
+                        a4_store_out(a, r0 + i, kvh * G + f - i * G, gi * Q4_GROUP + 4 * g, o[nt][gi][0][j] * inv, o[nt][gi][0][j + 2] * inv, o[nt][gi][1][j] * inv,
+                                     o[nt][gi][1][j + 2] * inv);
+                } else {
+#pragma unroll
+                    for (int gi = 0; gi < NG; gi++)
+                        *reinterpret_cast<float4*>(part_at + row * D + gi * Q4_GROUP + 4 * g) = make_float4(o[nt][gi][0][j], o[nt][gi][0][j + 2], o[nt][gi][1][j], o[nt][gi][1][j + 2]);
+                    if (g == 0) *reinterpret_cast<float2*>(part_at + MT * D + row * 2) = make_float2(ref[nt][j], l[nt][j]);
+                }
+            }
+        if (!(begins && ends) && lane == 0) {
+            const long end = u - n + left - 1, most = longer * (run + 1);        // the segment's last step
+            held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, (int)((end < most ? end / (run + 1) : longer + (end - most) / run) / A4_WARPS)};
+        }
+        // the segment behind it (not the sequence's loads if there is none)
+        if (u < u1) {
+            at.step = s.steps - 1;
+            at.next(a, MT);
+        }
+    }
+    __syncthreads();
+
+    // ================= what the CTA's warps have left, joined: from one warp's result on to where the segment ends. What an earlier CTA has begun, or a later one ends, goes to
+    // the workspace.
+    A4Desc* desc = a4_desc<PART>(a, gridDim.x) + blockIdx.x * 2;
+    bool left_open[2] = {false, false};
+    for (int w = 0; w < A4_WARPS; w++)
+        for (int slot = w == 0 ? 0 : 1; slot < 2; slot++) {      // (slot 0 of a later warp: joined with what it goes on from)
+            const Held h = held[w][slot];
+            if (h.rows == 0) continue;
+            int end = w;                                         // warps w .. end have results of this segment
+            bool ends = h.ends;
+            while (!ends && end + 1 < A4_WARPS) { end++; ends = held[end][0].ends; }
+            auto part_of = [&](int v) { return v == w && slot == 1 ? reinterpret_cast<const float*>(a4_raw + v * REGION) : head_part + v * PART; };
+            const bool finish = slot == 1 && ends;
+            float* to = a.work + ((size_t)blockIdx.x * 2 + slot) * PART;
+            for (int e = threadIdx.x; e < h.rows * (D / 4); e += A4_THREADS) {
+                const int row = e / (D / 4), d = e % (D / 4) * 4;
+                A4Sum sum;
+                for (int v = w; v <= end; v++) sum.most(part_of(v)[MT * D + row * 2]);
+                for (int v = w; v <= end; v++)
+                    sum.add(*reinterpret_cast<const float2*>(part_of(v) + MT * D + row * 2), *reinterpret_cast<const float4*>(part_of(v) + row * D + d));
+                if (finish) {
+                    const int f = h.f0 + row, i = f / G;
+                    sum.out(a, h.r0 + i, h.kvh * G + f - i * G, d);
+                } else {
+                    *reinterpret_cast<float4*>(to + row * D + d) = sum.v;
+                    if (d == 0) *reinterpret_cast<float2*>(to + MT * D + row * 2) = make_float2(sum.m, sum.l);
+                }
+            }
+            if (!finish) {
+                left_open[slot] = true;
+                if (threadIdx.x == 0) desc[slot] = {h.rows, h.r0, h.f0, h.kvh, h.last};
+            }
+        }
+    if (threadIdx.x < 2 && !left_open[threadIdx.x]) desc[threadIdx.x].rows = 0;      // (whatever the workspace held)
+}
+
+// The results of a segment that lies in several CTAs, from the one where it begins on: a row a CTA, a warp has every fourth result, a lane four dims (two for heads of 64)
+template <int D, int MT>
+__global__ void __launch_bounds__(128) attention_4bit_join_kernel(const Attention4Args a, const int ctas) {
+    constexpr int PART = a4_part<D>(MT), LANES = D / 4, PER = 128 / LANES, B = 8;
+    __shared__ float4 sums[PER][LANES];
+    __shared__ float2 refs[PER];
+    const int c = blockIdx.x, row = blockIdx.y, p = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+    griddep_wait();
+    griddep_launch();
+    const A4Desc h = a4_desc<PART>(a, ctas)[c * 2 + 1];
+    if (row >= h.rows) return;
+    const int n = min(h.last, ctas - 1) - c + 1;
+    A4Sum sum;
+    for (int j0 = p; j0 < n; j0 += PER * B) {
+        float2 ml[B];
+        float4 v[B];
+#pragma unroll
+        for (int j = 0; j < B; j++) {
+            ml[j] = make_float2(-INFINITY, 0.f); v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            const int i = j0 + j * PER;
+            if (i >= n) continue;
+            const float* from = a.work + ((size_t)(c + i) * 2 + (i == 0)) * PART;
+            ml[j] = __ldcg(reinterpret_cast<const float2*>(from + MT * D + row * 2));
+            v[j] = __ldcg(reinterpret_cast<const float4*>(from + row * D + d));
+        }
+        const float before = sum.m;
+#pragma unroll
+        for (int j = 0; j < B; j++) sum.most(ml[j].x);
+        sum.fall(before);
+#pragma unroll
+        for (int j = 0; j < B; j++) sum.add(ml[j], v[j]);
+    }
+    sums[p][d / 4] = sum.v;
+    if (d == 0) refs[p] = make_float2(sum.m, sum.l);
+    __syncthreads();
+    if (p) return;
+    A4Sum all;
+#pragma unroll
+    for (int j = 0; j < PER; j++) all.most(refs[j].x);
+#pragma unroll
+    for (int j = 0; j < PER; j++) all.add(refs[j], sums[j][d / 4]);
+    const int G = a.n_head / a.n_kv, f = h.f0 + row, i = f / G;
+    all.out(a, h.r0 + i, h.kvh * G + f - i * G, d);
+}
+
+// ---------------------------------------------------------------- host side
+namespace {
+template <int D, int NT>
+constexpr int a4_smem() {
+    constexpr int ring = A4_STAGES * 4 * q4_block(D), part = a4_part<D>(8 * NT) * 4;
+    return A4_WARPS * ((ring > part ? ring : part) + part);
+}
+template <int D, int NT>
+cudaError_t a4_step(const Attention4Args& a, cudaStream_t s) {
+    constexpr int MT = 8 * NT, smem = a4_smem<D, NT>();
+    if (!allow_smem<attention_4bit_step_kernel<D, NT>>(smem)) return cudaErrorInvalidValue;
+    // as many CTAs as run at once, no more than there can be steps for
+    const int ctas = a4_ctas(a, MT);
+    cudaError_t e = launch_chain(attention_4bit_step_kernel<D, NT>, dim3(ctas), dim3(A4_THREADS), smem, s, a);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, MT); cfg.blockDim = dim3(128); cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_4bit_join_kernel<D, MT>, a, ctas);
+}
+}  // namespace
+
+size_t attention_4bit_work_bytes(long n_rows, int n_head, int n_kv, int head_dim) {
+    const long rows = std::min<long>(16, n_rows * (n_head / n_kv) <= 8 ? 8 : 16);
+    return (size_t)A4_MOST_CTAS * 2 * (rows * (head_dim + 2) * 4 + sizeof(A4Desc));
+}
+
+cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s) {
+    if (a.r.n_rows == 0 || a.r.n_seqs == 0) return cudaSuccess;
+    const bool few = (long)a.max_rows * (a.n_head / a.n_kv) <= 8;
+    if (a.head_dim == 64) return few ? a4_step<64, 1>(a, s) : a4_step<64, 2>(a, s);
+    return few ? a4_step<128, 1>(a, s) : a4_step<128, 2>(a, s);
+}
+
+cudaError_t attention_4bit_error(unsigned int* code) { return take_error_word(a4_error, code); }
+
+}  // namespace b2

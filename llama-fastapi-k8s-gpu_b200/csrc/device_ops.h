@@ -48,6 +48,34 @@ struct KvAppendArgs {
 };
 cudaError_t kv_append_launch(const KvAppendArgs& a, cudaStream_t s);
 
+// ---------------------------------------------------------------- kv_4bit.cu: the same into a cache in 4 bits (kv_4bit.cuh; cache_type: q_out's), and out of it
+cudaError_t kv_append_4bit_launch(const KvAppendArgs& a, cudaStream_t s);
+struct KvReadArgs {
+    RaggedPages r;
+    const void *k_pool, *v_pool; // [n_pages][n_kv][block_tokens / 16][9 * head_dim] bytes
+    void *k, *v;                 // [n_rows][n_kv][head_dim] of out_type, either may be null
+    long k_row, k_head, v_row, v_head;
+    int n_kv, head_dim, out_type;
+};
+cudaError_t kv_read_4bit_launch(const KvReadArgs& a, cudaStream_t s);
+
+// ---------------------------------------------------------------- attention_4bit.cu
+struct Attention4Args {
+    RaggedPages r;
+    const void* q;               // [n_rows][n_head][head_dim] of `type`
+    long q_row, q_head;
+    const void *k_pool, *v_pool; // as KvReadArgs
+    void* out;                   // like q
+    long out_row, out_head;
+    float* work;                 // attention_4bit_work_bytes
+    int max_rows;                // most rows of a sequence
+    int n_head, n_kv, head_dim, type;
+    float scale_log2;
+};
+size_t attention_4bit_work_bytes(long n_rows, int n_head, int n_kv, int head_dim);
+cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s);
+cudaError_t attention_4bit_error(unsigned int* code);            // code of the first wait that ran out (does not wait), see shared_prefix_error
+
 // ---------------------------------------------------------------- logprobs.cu
 constexpr int LOGPROB_MAX_TOP = 64;
 struct RowMap { int n; int token[BATCH_MAX], out[BATCH_MAX]; };      // row r's token is tokens[token[r]], its results go to row out[r] (n 0: to r, tokens[r])

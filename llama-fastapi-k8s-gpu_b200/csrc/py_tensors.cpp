@@ -72,14 +72,18 @@ bool read(PyObject* t, int n, int device, int type, bool dense, Tensor& o) {
 
 bool fits(int64_t v) { return v >= 0 && v <= INT32_MAX; }
 
-// pools, tables and rows of a call
-bool read_where(PyObject* const* a, int64_t n_rows, int device, Tensor& k_pool, Tensor& v_pool, b2_ragged_pages& w) {
+// pools, tables and rows of a call. `codes`: pools in 4 bits, whose shape becomes [pages][KV heads][tokens of a page][head_dim]
+bool read_where(PyObject* const* a, int64_t n_rows, int device, Tensor& k_pool, Tensor& v_pool, b2_ragged_pages& w, bool codes = false) {
     Tensor pages, start, held;
-    if (!read(a[0], 4, device, -1, true, k_pool) || !read(a[1], 4, device, k_pool.type, true, v_pool) || !read(a[2], 2, device, B2_TYPE_I32, false, pages) ||
+    if (!read(a[0], 4, device, codes ? B2_TYPE_U8 : -1, true, k_pool) || !read(a[1], 4, device, k_pool.type, true, v_pool) || !read(a[2], 2, device, B2_TYPE_I32, false, pages) ||
         !read(a[3], 1, device, B2_TYPE_I32, true, start) || !read(a[4], 1, device, B2_TYPE_I32, true, held)) return false;
     for (int i = 0; i < 4; i++) if (k_pool.shape[i] != v_pool.shape[i]) return false;
     const int64_t n = held.shape[0];
-    if ((k_pool.type != B2_TYPE_F16 && k_pool.type != B2_TYPE_BF16) || pages.shape[0] != n || start.shape[0] != n + 1 || !fits(n) || !fits(pages.shape[1]) || !fits(n_rows) ||
+    if (codes) {
+        if (k_pool.shape[3] != 9 * 64 && k_pool.shape[3] != 9 * 128) return false;
+        k_pool.shape[2] *= 16; k_pool.shape[3] /= 9;
+    }
+    if ((!codes && k_pool.type != B2_TYPE_F16 && k_pool.type != B2_TYPE_BF16) || pages.shape[0] != n || start.shape[0] != n + 1 || !fits(n) || !fits(pages.shape[1]) || !fits(n_rows) ||
         !fits(k_pool.shape[1]) || !fits(k_pool.shape[2]) || !fits(k_pool.shape[3])) return false;
     w.row_start = (const int32_t*)start.p; w.lengths = (const int32_t*)held.p; w.pages = (const int32_t*)pages.p;
     w.table_stride = n > 1 ? pages.stride[0] : pages.shape[1];
@@ -93,6 +97,17 @@ bool read_stream(PyObject* s, void** out) {
     return !PyErr_Occurred();
 }
 
+// a contiguous tensor of any type on the device
+bool read_workspace(PyObject* t, int device, void*& p, int64_t& bytes) {
+    long long d, n;
+    if (t == Py_None || !read_int(PyObject_CallMethodNoArgs(t, s_get_device), &d) || d != device || !read_int(PyObject_GetAttr(t, s_nbytes), &n)) return false;
+    PyObject* c = PyObject_CallMethodNoArgs(t, s_is_contiguous);
+    const bool dense = c == Py_True;
+    Py_XDECREF(c);
+    bytes = n;
+    return dense && read_address(PyObject_CallMethodNoArgs(t, s_data_ptr), &p);
+}
+
 PyObject* not_ours() {
     PyErr_Clear();
     Py_RETURN_NONE;
@@ -101,13 +116,13 @@ PyObject* not_ours() {
 bool is_rows(int type) { return type == B2_TYPE_F32 || type == B2_TYPE_F16 || type == B2_TYPE_BF16; }
 
 // (entry point, k, v, k_pool, v_pool, pages, row_start, lengths, freqs, q, q_out, layout, first_pos, amplitude, stream) -> code, or None
-PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+PyObject* append(PyObject* const* a, Py_ssize_t n, bool codes) {
     if (n != 15) return not_ours();
     Tensor k, v, k_pool, v_pool, freqs, q, q_out;
     b2_ragged_pages w;
     b2_kv_append_args x = {};
     void *fn = PyLong_AsVoidPtr(a[0]), *stream;
-    if (!fn || !read(a[1], 3, -1, -1, false, k) || !is_rows(k.type) || !read(a[2], 3, k.device, k.type, false, v) || !read_where(a + 3, k.shape[0], k.device, k_pool, v_pool, w)) return not_ours();
+    if (!fn || !read(a[1], 3, -1, -1, false, k) || !is_rows(k.type) || !read(a[2], 3, k.device, k.type, false, v) || !read_where(a + 3, k.shape[0], k.device, k_pool, v_pool, w, codes)) return not_ours();
     for (int i = 0; i < 3; i++) if (k.shape[i] != v.shape[i]) return not_ours();
     if (k.shape[1] != k_pool.shape[1] || k.shape[2] != k_pool.shape[3]) return not_ours();
     if (a[8] != Py_None) {
@@ -115,20 +130,75 @@ PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         x.freqs = (const float*)freqs.p; x.rot_dims = (int32_t)(2 * freqs.shape[0]);
     }
     if ((a[9] == Py_None) != (a[10] == Py_None)) return not_ours();
+    x.cache_type = codes ? B2_TYPE_F16 : k_pool.type;
     if (a[9] != Py_None) {
-        if (!read(a[9], 3, k.device, k.type, false, q) || !read(a[10], 3, k.device, k_pool.type, false, q_out)) return not_ours();
+        if (!read(a[9], 3, k.device, k.type, false, q) || !read(a[10], 3, k.device, codes ? -1 : k_pool.type, false, q_out)) return not_ours();
+        if (codes) {
+            if (q_out.type != B2_TYPE_F16 && q_out.type != B2_TYPE_BF16) return not_ours();
+            x.cache_type = q_out.type;
+        }
         for (int i = 0; i < 3; i++) if (q.shape[i] != q_out.shape[i]) return not_ours();
         if (q.shape[0] != k.shape[0] || q.shape[2] != k.shape[2] || !fits(q.shape[1])) return not_ours();
         x.q = q.p; x.q_row = q.stride[0]; x.q_head = q.stride[1]; x.q_out = q_out.p; x.q_out_row = q_out.stride[0]; x.q_out_head = q_out.stride[1];
         x.n_head = (int32_t)q.shape[1];
     }
     x.k = k.p; x.v = v.p; x.k_row = k.stride[0]; x.k_head = k.stride[1]; x.v_row = v.stride[0]; x.v_head = v.stride[1];
-    x.k_pool = k_pool.p; x.v_pool = v_pool.p; x.in_type = k.type; x.cache_type = k_pool.type; x.n_kv = (int32_t)k.shape[1]; x.head_dim = (int32_t)k.shape[2];
+    x.k_pool = k_pool.p; x.v_pool = v_pool.p; x.in_type = k.type; x.n_kv = (int32_t)k.shape[1]; x.head_dim = (int32_t)k.shape[2];
     x.layout = (int32_t)PyLong_AsLong(a[11]); x.first_pos = PyLong_AsLongLong(a[12]); x.amplitude = (float)PyFloat_AsDouble(a[13]);
     if (!read_stream(a[14], &stream) || PyErr_Occurred()) return not_ours();
     int rc;
     Py_BEGIN_ALLOW_THREADS
     rc = ((decltype(&b2_kv_append))fn)(k.device, &w, &x, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t n) { return append(a, n, false); }
+PyObject* kv_append_4bit(PyObject*, PyObject* const* a, Py_ssize_t n) { return append(a, n, true); }
+
+// (entry point, k_pool, v_pool, pages, row_start, lengths, k, v, stream) -> code, or None
+PyObject* kv_read_4bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 9) return not_ours();
+    Tensor k, v, k_pool, v_pool;
+    b2_ragged_pages w;
+    b2_kv_read_4bit_args x = {};
+    void *fn = PyLong_AsVoidPtr(a[0]), *stream;
+    const bool has_k = a[6] != Py_None, has_v = a[7] != Py_None;
+    if (!fn || (!has_k && !has_v) || (has_k && !read(a[6], 3, -1, -1, false, k)) || (has_v && !read(a[7], 3, has_k ? k.device : -1, has_k ? k.type : -1, false, v))) return not_ours();
+    const Tensor& t = has_k ? k : v;
+    if (!is_rows(t.type) || !read_where(a + 1, t.shape[0], t.device, k_pool, v_pool, w, true)) return not_ours();
+    for (int i = 0; has_k && has_v && i < 3; i++) if (k.shape[i] != v.shape[i]) return not_ours();
+    if (t.shape[1] != k_pool.shape[1] || t.shape[2] != k_pool.shape[3]) return not_ours();
+    x.k_pool = k_pool.p; x.v_pool = v_pool.p; x.n_kv = (int32_t)t.shape[1]; x.head_dim = (int32_t)t.shape[2]; x.out_type = t.type;
+    if (has_k) { x.k = k.p; x.k_row = k.stride[0]; x.k_head = k.stride[1]; }
+    if (has_v) { x.v = v.p; x.v_row = v.stride[0]; x.v_head = v.stride[1]; }
+    if (!read_stream(a[8], &stream) || PyErr_Occurred()) return not_ours();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = ((decltype(&b2_kv_read_4bit))fn)(t.device, &w, &x, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+// (entry point, q, k_pool, v_pool, pages, row_start, lengths, out, workspace, max_rows, scale, stream) -> code, or None
+PyObject* attention_4bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 12) return not_ours();
+    Tensor q, out, k_pool, v_pool;
+    b2_ragged_pages w;
+    b2_attention_4bit_args x = {};
+    void *fn = PyLong_AsVoidPtr(a[0]), *stream;
+    if (!fn || !read(a[1], 3, -1, -1, false, q) || !read(a[7], 3, q.device, q.type, false, out) || !read_where(a + 2, q.shape[0], q.device, k_pool, v_pool, w, true)) return not_ours();
+    for (int i = 0; i < 3; i++) if (q.shape[i] != out.shape[i]) return not_ours();
+    if ((q.type != B2_TYPE_F16 && q.type != B2_TYPE_BF16) || q.shape[2] != k_pool.shape[3] || k_pool.shape[1] == 0 || !fits(q.shape[1]) || q.shape[1] % k_pool.shape[1]) return not_ours();
+    const long long max_rows = a[9] == Py_None ? (q.shape[0] > 1 ? q.shape[0] : 1) : PyLong_AsLongLong(a[9]);
+    if (PyErr_Occurred() || max_rows > INT32_MAX || max_rows < INT32_MIN || !read_workspace(a[8], q.device, x.workspace, x.workspace_bytes)) return not_ours();
+    x.q = q.p; x.k_pool = k_pool.p; x.v_pool = v_pool.p; x.out = out.p; x.q_row = q.stride[0]; x.q_head = q.stride[1]; x.out_row = out.stride[0]; x.out_head = out.stride[1];
+    x.max_rows = (int32_t)max_rows; x.n_head = (int32_t)q.shape[1]; x.n_kv = (int32_t)k_pool.shape[1]; x.head_dim = (int32_t)q.shape[2]; x.type = q.type;
+    x.scale = (float)(a[10] == Py_None ? 1.0 / sqrt((double)q.shape[2]) : PyFloat_AsDouble(a[10]));
+    if (!read_stream(a[11], &stream) || PyErr_Occurred()) return not_ours();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = ((decltype(&b2_attention_4bit))fn)(q.device, &w, &x, stream);
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(rc);
 }
@@ -146,14 +216,9 @@ PyObject* attention_shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const long long n_prefix = PyLong_AsLongLong(a[8]), max_rows = a[11] == Py_None ? (q.shape[0] > 1 ? q.shape[0] : 1) : PyLong_AsLongLong(a[11]);
     if (PyErr_Occurred() || n_prefix < 0 || n_prefix > INT32_MAX || max_rows > INT32_MAX || max_rows < INT32_MIN) return not_ours();
     if (n_prefix) {
-        long long device, bytes;
         if (!read(a[7], 1, q.device, B2_TYPE_I32, true, prefix) || n_prefix > prefix.shape[0] * k_pool.shape[2]) return not_ours();
-        if (a[10] == Py_None || !read_int(PyObject_CallMethodNoArgs(a[10], s_get_device), &device) || device != q.device || !read_int(PyObject_GetAttr(a[10], s_nbytes), &bytes)) return not_ours();
-        PyObject* c = PyObject_CallMethodNoArgs(a[10], s_is_contiguous);
-        const bool dense = c == Py_True;
-        Py_XDECREF(c);
-        if (!dense || !read_address(PyObject_CallMethodNoArgs(a[10], s_data_ptr), &x.workspace)) return not_ours();
-        x.workspace_bytes = bytes; x.prefix_pages = (const int32_t*)prefix.p;
+        if (!read_workspace(a[10], q.device, x.workspace, x.workspace_bytes)) return not_ours();
+        x.prefix_pages = (const int32_t*)prefix.p;
     }
     x.q = q.p; x.k_pool = k_pool.p; x.v_pool = v_pool.p; x.out = out.p; x.q_row = q.stride[0]; x.q_head = q.stride[1]; x.out_row = out.stride[0]; x.out_head = out.stride[1];
     x.n_prefix = (int32_t)n_prefix; x.max_rows = (int32_t)max_rows; x.n_head = (int32_t)q.shape[1]; x.n_kv = (int32_t)k_pool.shape[1]; x.head_dim = (int32_t)q.shape[2]; x.type = q.type;
@@ -204,6 +269,9 @@ PyObject* add_type(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"kv_append", (PyCFunction)(void (*)(void))kv_append, METH_FASTCALL, nullptr},
+    {"kv_append_4bit", (PyCFunction)(void (*)(void))kv_append_4bit, METH_FASTCALL, nullptr},
+    {"kv_read_4bit", (PyCFunction)(void (*)(void))kv_read_4bit, METH_FASTCALL, nullptr},
+    {"attention_4bit", (PyCFunction)(void (*)(void))attention_4bit, METH_FASTCALL, nullptr},
     {"attention_shared_prefix", (PyCFunction)(void (*)(void))attention_shared_prefix, METH_FASTCALL, nullptr},
     {"token_logprobs", (PyCFunction)(void (*)(void))token_logprobs, METH_FASTCALL, nullptr},
     {"add_type", (PyCFunction)(void (*)(void))add_type, METH_FASTCALL, nullptr},

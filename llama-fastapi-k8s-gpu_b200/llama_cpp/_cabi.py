@@ -17,7 +17,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libb200gguf.so")
 
 B2_FLAG_NO_GRAPH, B2_FLAG_NO_PDL, B2_FLAG_ACT8, B2_FLAG_F32 = 1, 2, 4, 8
-B2_TYPE_F32, B2_TYPE_F16, B2_TYPE_I32, B2_TYPE_BF16 = 0, 1, 26, 30
+B2_TYPE_F32, B2_TYPE_F16, B2_TYPE_I32, B2_TYPE_BF16, B2_TYPE_U8 = 0, 1, 26, 30, 100
 B2_MIX_WINDOW_SCAN, B2_MIX_MATRIX_MEMORY, B2_MIX_LATENT_ATTN, B2_MIX_DELTA_RULE, B2_MIX_SSD, B2_MIX_CHUNK_LINEAR = 1, 2, 3, 4, 5, 6
 B2_MIX_SINK_DELTA, B2_MIX_SINK_ATTN = 7, 8
 B2_FF_RELU2, B2_FF_MOE, B2_FF_GLU, B2_FF_PIECEWISE = 0, 1, 2, 3
@@ -85,6 +85,17 @@ class B2SharedPrefix(ctypes.Structure):
         (n, c_int32) for n in ("n_prefix", "max_rows", "n_head", "n_kv", "head_dim", "type")] + [("scale", c_float)]
 
 
+class B2KvRead4Bit(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("k_pool", "v_pool", "k", "v")] + [(n, c_int64) for n in ("k_row", "k_head", "v_row", "v_head")] + [
+        (n, c_int32) for n in ("n_kv", "head_dim", "out_type")]
+
+
+class B2Attention4Bit(ctypes.Structure):
+    _fields_ = [(n, c_void_p) for n in ("q", "k_pool", "v_pool", "out", "workspace")] + [
+        (n, c_int64) for n in ("workspace_bytes", "q_row", "q_head", "out_row", "out_head")] + [
+        (n, c_int32) for n in ("max_rows", "n_head", "n_kv", "head_dim", "type")] + [("scale", c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/b200_gguf.h declares
 SIGNATURES = {
     "b2_last_error": (c_char_p, []),
@@ -138,6 +149,10 @@ SIGNATURES = {
     "b2_kv_append": (c_int, [c_int, c_void_p, c_void_p, c_void_p]),          # b2_ragged_pages, b2_kv_append_args: structures or their bytes
     "b2_attention_shared_prefix": (c_int, [c_int, c_void_p, c_void_p, c_void_p]),
     "b2_attention_shared_prefix_workspace": (c_int, [c_int] * 4 + [POINTER(c_int64)]),
+    "b2_kv_append_4bit": (c_int, [c_int, c_void_p, c_void_p, c_void_p]),
+    "b2_kv_read_4bit": (c_int, [c_int, c_void_p, c_void_p, c_void_p]),
+    "b2_attention_4bit": (c_int, [c_int, c_void_p, c_void_p, c_void_p]),
+    "b2_attention_4bit_workspace": (c_int, [c_int] * 4 + [POINTER(c_int64)]),
     "b2_token_logprobs": (c_int, [c_int, c_void_p, c_int, c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "b2_device_op_error": (c_int, [c_int, POINTER(ctypes.c_uint32)]),
     "b2_op_give_up": (c_int, [c_int, c_int, ctypes.c_uint32, c_void_p]),

@@ -1,8 +1,11 @@
-"""Operators over device tensors that the caller owns: appending to a paged cache, attention of a batch over a shared prefix, log probabilities.
+"""Operators over device tensors that the caller owns: appending to a paged cache, attention of a batch over a shared prefix, log probabilities; the cache in 4 bits.
 
 They are the C entry points b2_kv_append, b2_attention_shared_prefix and b2_token_logprobs (include/b200_gguf.h says what each computes), for hosts that keep
 caches and logits of their own: score or continue several answers to one prompt by appending every answer's keys and values to pages of its own,
 attending to the prompt's pages once for all of them, and reading the log probabilities off the logits.
+
+b2_kv_append_4bit, b2_kv_read_4bit and b2_attention_4bit keep the cache in 4 bits and a scale for every 32 entries, 9/16 of a byte an entry: its pools are uint8 tensors
+[pages, kv heads, page tokens / 16, 9 * dim] (dim 64 or 128). Append every prompt's and every step's rows, attend to them; take rows out in 16 or 32 bits.
 
 A tensor is a torch tensor on a CUDA device, or anything with its `data_ptr()`, `shape`, `stride()`, `dtype`, `get_device()` and `is_contiguous()` (this
 package does not import torch itself); results go into tensors of the caller's, nothing is allocated. `stream` is a stream object with `cuda_stream`, its
@@ -23,8 +26,9 @@ import struct
 from . import _cabi
 from ._cabi import check
 
-_TYPES = {"float32": _cabi.B2_TYPE_F32, "float16": _cabi.B2_TYPE_F16, "bfloat16": _cabi.B2_TYPE_BF16, "int32": _cabi.B2_TYPE_I32}
-_F32, _F16, _BF16, _I32 = (_TYPES[n] for n in ("float32", "float16", "bfloat16", "int32"))
+_TYPES = {"float32": _cabi.B2_TYPE_F32, "float16": _cabi.B2_TYPE_F16, "bfloat16": _cabi.B2_TYPE_BF16, "int32": _cabi.B2_TYPE_I32,
+          "uint8": _cabi.B2_TYPE_U8}
+_F32, _F16, _BF16, _I32, _U8 = (_TYPES[n] for n in ("float32", "float16", "bfloat16", "int32", "uint8"))
 _NAMES = {v: k for k, v in _TYPES.items()}
 _ROWS, _CACHE = (_F32, _F16, _BF16), (_F16, _BF16)
 _LAYOUTS = {"pairs": _cabi.B2_ROTATE_PAIRS, "halves": _cabi.B2_ROTATE_HALVES}
@@ -61,7 +65,8 @@ def _packer(structure):
     return p.pack
 
 
-_ragged_pages, _kv_append, _shared_prefix = (_packer(s) for s in (_cabi.B2RaggedPages, _cabi.B2KvAppend, _cabi.B2SharedPrefix))
+_ragged_pages, _kv_append, _shared_prefix, _kv_read_4bit, _attention_4bit = (
+    _packer(s) for s in (_cabi.B2RaggedPages, _cabi.B2KvAppend, _cabi.B2SharedPrefix, _cabi.B2KvRead4Bit, _cabi.B2Attention4Bit))
 
 
 def _wrong(what, t, shape, types, device, dense):
@@ -101,16 +106,53 @@ def _begin(what, t, dims, types):
     return device, shape, code
 
 
-def _where(n_rows, k_pool, v_pool, pages, row_start, lengths, device):
-    """Pointers of the pools, their shape and type, and the packed b2_ragged_pages"""
+def _where(n_rows, k_pool, v_pool, pages, row_start, lengths, device, codes=False):
+    """Pointers of the pools, their shape [pages, kv heads, page tokens, dim] and type, and the packed b2_ragged_pages. `codes`: pools in 4 bits"""
     if len(lengths.shape) != 1 or len(pages.shape) != 2:
         raise ValueError(f"lengths must have one dimension and pages two, not {tuple(lengths.shape)} and {tuple(pages.shape)}")
-    _, pool, cache = _begin("k_pool", k_pool, 4, _CACHE)
+    _, pool, cache = _begin("k_pool", k_pool, 4, (_U8,) if codes else _CACHE)
     n_seqs, width = pages.shape
     table, stride = _rows("pages", pages, (n_seqs, width), (_I32,), device)
     kp, vp = _dense("k_pool", k_pool, pool, (cache,), device), _dense("v_pool", v_pool, pool, (cache,), device)
     start, held = _dense("row_start", row_start, (n_seqs + 1,), (_I32,), device), _dense("lengths", lengths, (n_seqs,), (_I32,), device)
+    if codes:
+        if pool[3] not in (576, 1152):
+            raise ValueError(f"pools {tuple(pool)}: the last dimension must be 9 * 64 or 9 * 128 bytes, 16 tokens of a head")
+        pool = (pool[0], pool[1], 16 * pool[2], pool[3] // 9)
     return kp, vp, pool, cache, _ragged_pages(start, held, table, stride[0] if n_seqs > 1 else width, pool[0], width, n_seqs, n_rows, pool[2])
+
+
+def _append(codes, k, v, k_pool, v_pool, pages, row_start, lengths, freqs, layout, first_pos, amplitude, q, q_out, stream):
+    """Checks and call of both appends. `codes`: pools in 4 bits"""
+    device, shape, rows = _begin("k", k, 3, _ROWS)
+    n, n_kv, dim = shape
+    kp, vp, pool, cache, where = _where(n, k_pool, v_pool, pages, row_start, lengths, device, codes)
+    if codes:
+        cache = _F16 if q_out is None else _code[q_out.dtype]
+    if n_kv != pool[1] or dim != pool[3]:
+        raise ValueError(f"k {tuple(shape)} and pools {tuple(pool)} do not go together")
+    pk, sk = _rows("k", k, shape, (rows,), device)
+    pv, sv = _rows("v", v, shape, (rows,), device)
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout must be 'pairs' or 'halves', not {layout!r}")
+    if (q is None) != (q_out is None):
+        raise ValueError("q and q_out go together")
+    pq = po = heads = 0
+    sq = so = (0, 0)
+    if q is not None:
+        shape_q = q.shape
+        if len(shape_q) != 3 or shape_q[0] != n or shape_q[2] != dim:
+            raise ValueError(f"q {tuple(shape_q)} and k {tuple(shape)} do not go together")
+        pq, sq = _rows("q", q, shape_q, (rows,), device)
+        po, so = _rows("q_out", q_out, shape_q, _CACHE if codes else (cache,), device)
+        heads = shape_q[1]
+    pf, rot = 0, 0
+    if freqs is not None:
+        pf, rot = _dense("freqs", freqs, freqs.shape if len(freqs.shape) == 1 else (None,), (_F32,), device), 2 * freqs.shape[0]
+    args = _kv_append(pk, pv, pq, kp, vp, po, pf, sk[0], sk[1], sv[0], sv[1], sq[0], sq[1], so[0], so[1], first_pos, rows, cache, heads, n_kv, dim, rot,
+                      _LAYOUTS[layout], amplitude)
+    entry = "b2_kv_append_4bit" if codes else "b2_kv_append"
+    check(getattr(_cabi.load_library(), entry)(device, where, args, stream), entry)
 
 
 def kv_append(k, v, k_pool, v_pool, pages, row_start, lengths, *, freqs=None, layout="pairs", first_pos=0, amplitude=1.0, q=None, q_out=None, stream=None):
@@ -128,32 +170,7 @@ def kv_append(k, v, k_pool, v_pool, pages, row_start, lengths, *, freqs=None, la
             if code:
                 check(code, "b2_kv_append")
             return
-    device, shape, rows = _begin("k", k, 3, _ROWS)
-    n, n_kv, dim = shape
-    kp, vp, pool, cache, where = _where(n, k_pool, v_pool, pages, row_start, lengths, device)
-    if n_kv != pool[1] or dim != pool[3]:
-        raise ValueError(f"k {tuple(shape)} and pools {tuple(pool)} do not go together")
-    pk, sk = _rows("k", k, shape, (rows,), device)
-    pv, sv = _rows("v", v, shape, (rows,), device)
-    if layout not in _LAYOUTS:
-        raise ValueError(f"layout must be 'pairs' or 'halves', not {layout!r}")
-    if (q is None) != (q_out is None):
-        raise ValueError("q and q_out go together")
-    pq = po = heads = 0
-    sq = so = (0, 0)
-    if q is not None:
-        shape_q = q.shape
-        if len(shape_q) != 3 or shape_q[0] != n or shape_q[2] != dim:
-            raise ValueError(f"q {tuple(shape_q)} and k {tuple(shape)} do not go together")
-        pq, sq = _rows("q", q, shape_q, (rows,), device)
-        po, so = _rows("q_out", q_out, shape_q, (cache,), device)
-        heads = shape_q[1]
-    pf, rot = 0, 0
-    if freqs is not None:
-        pf, rot = _dense("freqs", freqs, freqs.shape if len(freqs.shape) == 1 else (None,), (_F32,), device), 2 * freqs.shape[0]
-    args = _kv_append(pk, pv, pq, kp, vp, po, pf, sk[0], sk[1], sv[0], sv[1], sq[0], sq[1], so[0], so[1], first_pos, rows, cache, heads, n_kv, dim, rot,
-                      _LAYOUTS[layout], amplitude)
-    check(_cabi.load_library().b2_kv_append(device, where, args, stream), "b2_kv_append")
+    _append(False, k, v, k_pool, v_pool, pages, row_start, lengths, freqs, layout, first_pos, amplitude, q, q_out, stream)
 
 
 def attention_shared_prefix_workspace(rows, n_head, n_kv, head_dim) -> int:
@@ -204,6 +221,81 @@ def attention_shared_prefix(q, k_pool, v_pool, prefix_pages, n_prefix, pages, ro
     check(_cabi.load_library().b2_attention_shared_prefix(device, where, args, stream), "b2_attention_shared_prefix")
 
 
+def kv_append_4bit(k, v, k_pool, v_pool, pages, row_start, lengths, *, freqs=None, layout="pairs", first_pos=0, amplitude=1.0, q=None, q_out=None, stream=None):
+    """kv_append into a cache in 4 bits (b2_kv_append_4bit): pools uint8 [pages, kv heads, page tokens / 16, 9 * dim], dim 64 or 128; q_out float16 or bfloat16."""
+    stream = getattr(stream, "cuda_stream", stream)
+    call, entry = _entries.get("kv_append_4bit") or _entries.setdefault("kv_append_4bit", _entry("kv_append_4bit"))
+    if call is not None and layout in _LAYOUTS:
+        code = call(entry, k, v, k_pool, v_pool, pages, row_start, lengths, freqs, q, q_out, _LAYOUTS[layout], first_pos, amplitude, stream)
+        if code is not None:
+            if code:
+                check(code, "b2_kv_append_4bit")
+            return
+    _append(True, k, v, k_pool, v_pool, pages, row_start, lengths, freqs, layout, first_pos, amplitude, q, q_out, stream)
+
+
+def kv_read_4bit(k_pool, v_pool, pages, row_start, lengths, k, v, *, stream=None):
+    """Rows of a cache in 4 bits back (b2_kv_read_4bit): k, v [rows, kv heads, dim], both float32, float16 or bfloat16, either may be None. Rows row_start[s] ..
+    row_start[s + 1] - 1 are the newest of sequence s's first lengths[s] tokens; rows without a place in the cache are left as they are."""
+    stream = getattr(stream, "cuda_stream", stream)
+    call, entry = _entries.get("kv_read_4bit") or _entries.setdefault("kv_read_4bit", _entry("kv_read_4bit"))
+    if call is not None:
+        code = call(entry, k_pool, v_pool, pages, row_start, lengths, k, v, stream)
+        if code is not None:
+            if code:
+                check(code, "b2_kv_read_4bit")
+            return
+    name, first = ("v", v) if k is None else ("k", k)
+    if first is None:
+        raise ValueError("one of k and v must be given")
+    device, shape, kind = _begin(name, first, 3, _ROWS)
+    kp, vp, pool, _, where = _where(shape[0], k_pool, v_pool, pages, row_start, lengths, device, True)
+    if shape[1] != pool[1] or shape[2] != pool[3]:
+        raise ValueError(f"{name} {tuple(shape)} and pools of {pool[1]} KV heads of {pool[3]} do not go together")
+    pk, sk = (0, (0, 0)) if k is None else _rows("k", k, shape, (kind,), device)
+    pv, sv = (0, (0, 0)) if v is None else _rows("v", v, shape, (kind,), device)
+    args = _kv_read_4bit(kp, vp, pk, pv, sk[0], sk[1], sv[0], sv[1], pool[1], pool[3], kind)
+    check(_cabi.load_library().b2_kv_read_4bit(device, where, args, stream), "b2_kv_read_4bit")
+
+
+def attention_4bit_workspace(rows, n_head, n_kv, head_dim) -> int:
+    """Bytes of workspace that attention_4bit needs for so many rows, whatever the lengths."""
+    for name, n in (("rows", rows), ("n_head", n_head), ("n_kv", n_kv), ("head_dim", head_dim)):
+        if not 0 <= n < 1 << 31:                                 # (ctypes would drop the upper bits)
+            raise ValueError(f"{name} must be a number of 31 bits, not {n}")
+    out = ctypes.c_int64()
+    check(_cabi.load_library().b2_attention_4bit_workspace(rows, n_head, n_kv, head_dim, ctypes.byref(out)), "b2_attention_4bit_workspace")
+    return out.value
+
+
+def attention_4bit(q, k_pool, v_pool, pages, row_start, lengths, out, workspace, *, max_rows=None, scale=None, stream=None):
+    """Attention of a ragged batch over a cache in 4 bits (b2_attention_4bit): a sequence's rows see its tokens up to themselves.
+
+    q, out [rows, heads, dim] both float16 or both bfloat16; pools as for kv_append_4bit; pages, row_start, lengths int32 as for kv_append. `workspace`: a contiguous tensor of
+    at least attention_4bit_workspace bytes, which no other call on another stream uses meanwhile. `max_rows`: most rows of a sequence (None: all rows may be one
+    sequence's; 1 for a batched step of single tokens is much faster than leaving it open)."""
+    stream = getattr(stream, "cuda_stream", stream)
+    call, entry = _entries.get("attention_4bit") or _entries.setdefault("attention_4bit", _entry("attention_4bit"))
+    if call is not None:
+        code = call(entry, q, k_pool, v_pool, pages, row_start, lengths, out, workspace, max_rows, scale, stream)
+        if code is not None:
+            if code:
+                check(code, "b2_attention_4bit")
+            return
+    device, shape, kind = _begin("q", q, 3, _CACHE)
+    n, heads, dim = shape
+    kp, vp, pool, _, where = _where(n, k_pool, v_pool, pages, row_start, lengths, device, True)
+    if dim != pool[3] or pool[1] == 0 or heads % pool[1]:
+        raise ValueError(f"q {tuple(shape)} and pools of {pool[1]} KV heads of {pool[3]} do not go together")
+    pq, sq = _rows("q", q, shape, (kind,), device)
+    po, so = _rows("out", out, shape, (kind,), device)
+    if workspace is None or workspace.get_device() != device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the same device")
+    args = _attention_4bit(pq, kp, vp, po, workspace.data_ptr(), workspace.nbytes, sq[0], sq[1], so[0], so[1], max(1, n) if max_rows is None else max_rows, heads, pool[1], dim,
+                           kind, 1.0 / math.sqrt(dim) if scale is None else scale)
+    check(_cabi.load_library().b2_attention_4bit(device, where, args, stream), "b2_attention_4bit")
+
+
 def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_logprob=None, top_id=None, *, stream=None):
     """Log probabilities of `tokens` (int32 [rows]), entropy, and the most likely tokens of logits [rows, vocab] (b2_token_logprobs).
 
@@ -240,7 +332,7 @@ def token_logprobs(logits, tokens=None, logprob=None, entropy=None, top_logprob=
 
 
 def error(device) -> int:
-    """Code of the first wait of attention_shared_prefix's kernels that ran out on this CUDA device since the last time that this was asked (0: none;
+    """Code of the first wait of the attention kernels that ran out on this CUDA device since the last time that this was asked (0: none;
     b2_device_op_error): results of the calls in between are not to be used. Waits for all work on the device; not while a stream is being captured."""
     code = ctypes.c_uint32()
     check(_cabi.load_library().b2_device_op_error(device, ctypes.byref(code)), "b2_device_op_error")
