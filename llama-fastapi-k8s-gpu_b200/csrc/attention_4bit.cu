@@ -10,8 +10,9 @@
 //   scores: the operand of the keys is the codes c themselves as the subnormal f16 numbers c 2^-24 (c 2^-20 for every other one, where the query's entry is 1/16 of itself): a mask
 //     and nothing else. Queries are held in f16 at a power of two that puts a row's largest entry near 2^10; the code's offset of 8 is the sum's initial value, -8 2^-24 sum q
 //     over the group, and the group's scale multiplies the group's sum in 32 bits. No key is rounded.
-//   weighted sums: c - 8 times the scale, rounded to f16, and probabilities in f16 (2^-11 each), whatever the type of queries and output. The score fragment becomes the
-//     probabilities' operand by movmatrix.
+//   weighted sums: the operand of the values is again their codes alone, c 2^-24 and c 2^-20. A probability times the scale of its key's value, group by group, is the other, rounded
+//     to f16 once (2^-11), whatever the type of queries and output; the offset of 8 is a product of that operand and a constant. Scales are taken at a power of two that keeps the
+//     operand in f16's range, found from the scales as they come. Score fragments become operands by movmatrix.
 // The reference of a row's exponentials moves only where a score exceeds it by 2^6.
 #include "device_ops.h"
 #include "kv_4bit.cuh"
@@ -19,13 +20,15 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <float.h>
 #include <math.h>
+#include <type_traits>
 
 namespace b2 {
 
 namespace {
 constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS;
-constexpr int A4_KEYS = 32;          // keys of a step: two blocks of 16
+constexpr int A4_BLOCKS = 2, A4_KEYS = A4_BLOCKS * Q4_TOKENS;      // blocks and keys of a step
 constexpr int A4_STAGES = 3;         // steps under way
 constexpr int A4_SMS = 148;
 
@@ -39,6 +42,11 @@ __device__ __forceinline__ void a4_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same, from other initial values
+__device__ __forceinline__ void a4_mma_from(float (&d)[4], const float (&c)[2], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]));
+}
 __device__ __forceinline__ uint32_t a4_transpose(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -48,6 +56,14 @@ __device__ __forceinline__ uint32_t a4_transpose(uint32_t v) {
 template <int NG> __device__ __forceinline__ void a4_chunk(const uint8_t* p, uint32_t (&w)[NG]) {
     if constexpr (NG == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
     else { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+}
+
+template <int NG> __device__ __forceinline__ void a4_scales(const uint8_t* p, float (&s)[NG]) {
+#pragma unroll
+    for (int gi = 0; gi < NG; gi += 2) {
+        const float2 v = __half22float2(reinterpret_cast<const __half2*>(p)[gi >> 1]);
+        s[gi] = v.x; s[gi + 1] = v.y;
+    }
 }
 
 // what is known of a sequence: its first row, its rows (those that are computed), its tokens, and the keys that its first row sees
@@ -133,7 +149,7 @@ inline int a4_ctas(const Attention4Args& a, int mt) {
 
 template <int D, int NT>
 __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_step_kernel(const Attention4Args a) {
-    constexpr int NG = D / Q4_GROUP, BLOCK = q4_block(D), STAGE = 4 * BLOCK, S = A4_STAGES, MT = 8 * NT, PART = a4_part<D>(MT);
+    constexpr int NG = D / Q4_GROUP, BLOCK = q4_block(D), KB = A4_BLOCKS, STAGE = 2 * KB * BLOCK, S = A4_STAGES, MT = 8 * NT, PART = a4_part<D>(MT);
     constexpr int REGION = S * STAGE > PART * 4 ? S * STAGE : PART * 4;
     extern __shared__ __align__(128) uint8_t a4_raw[];
     __shared__ uint64_t full[A4_WARPS][S];
@@ -150,7 +166,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
     griddep_wait();
     griddep_launch();
     __syncwarp();
-    const int n_kv = a.n_kv, G = a.n_head / n_kv, bt = a.r.block_tokens, blocks = bt / Q4_TOKENS;
+    const int n_kv = a.n_kv, G = a.n_head / n_kv, blocks = a.r.block_tokens / Q4_TOKENS, last_page = (int)a.r.n_pages - 1;
 
     // ---- the steps of all sequences, and this warp's run [u0, u1) of them
     long total = 0;
@@ -185,31 +201,33 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
         }
     }
 
-    // ---- copies: lanes 0 .. 3 have keys and values of the step's two blocks, the page's id read a step ahead
+    // ---- copies: a lane has keys or values of one of the step's blocks, the page's id read a step ahead
     A4At ahead = at;
-    long copied = u0;
-    const int c_kv = lane >> 1 & 1, c_blk = lane & 1;
-    auto page_of = [&]() {
-        const int t = ahead.step * A4_KEYS + c_blk * Q4_TOKENS;
-        return lane < 4 && copied < u1 && t < ahead.s.own ? a.r.pages[ahead.z * a.r.table_stride + t / bt] : 0;
+    int to_copy = (int)(u1 - u0), id = 0, in_page = 0, put = 0;
+    const int c_kv = lane >= KB, c_blk = lane - c_kv * KB;
+    const uint8_t* const pool = (const uint8_t*)(c_kv ? a.v_pool : a.k_pool);
+    auto read_id = [&]() {
+        const unsigned b = ahead.step * KB + c_blk;              // block of the sequence
+        unsigned page = __umulhi(b, a.per_page);                 // the quotient by the page's blocks, or one less
+        in_page = (int)(b - page * blocks);
+        if (in_page >= blocks) { page++; in_page -= blocks; }
+        id = lane < 2 * KB && to_copy && (int)b * Q4_TOKENS < ahead.s.own ? a.r.pages[ahead.z * a.r.table_stride + page] : 0;
     };
-    int id = page_of(), put = 0;
+    read_id();
     auto copy = [&]() {
-        if (copied >= u1) return;
-        const int t0 = ahead.step * A4_KEYS, n = min(2, (ahead.s.own - t0 + Q4_TOKENS - 1) / Q4_TOKENS);
+        if (!to_copy) return;
+        const int n = min(KB, (ahead.s.own - ahead.step * A4_KEYS + Q4_TOKENS - 1) / Q4_TOKENS);
         if (lane == 0) mbar_arrive_expect_tx(&full[warp][put], (uint32_t)(max(n, 0) * 2 * BLOCK));
         __syncwarp();
-        if (lane < 4 && c_blk < n) {
-            const int t = t0 + c_blk * Q4_TOKENS;
-            const long page = min(max((long)id, 0l), a.r.n_pages - 1);
-            const uint8_t* from = (const uint8_t*)(c_kv ? a.v_pool : a.k_pool) + ((page * n_kv + ahead.kvh) * blocks + t % bt / Q4_TOKENS) * BLOCK;
-            tma_load_1d(ring + put * STAGE + (c_kv * 2 + c_blk) * BLOCK, from, BLOCK, &full[warp][put]);
+        if (lane < 2 * KB && c_blk < n) {
+            const long page = min(max(id, 0), last_page);
+            tma_load_1d(ring + put * STAGE + lane * BLOCK, pool + ((page * n_kv + ahead.kvh) * blocks + in_page) * BLOCK, BLOCK, &full[warp][put]);
         }
         __syncwarp();
         put = put + 1 == S ? 0 : put + 1;
         ahead.next(a, MT);
-        copied++;
-        id = page_of();
+        to_copy--;
+        read_id();
     };
     for (int i = 0; i < S; i++) copy();
 
@@ -281,179 +299,159 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
             }
         }
         const int own = s.own, lim_lo = min(s.limit(f0 / G), own);                       // keys that all rows of the tile see
-        float o[NT][NG][2][4], ref[NT][2], l[NT][2];
+        // weighted sums, 2^24 (even dims) and 2^20 (odd) over `up_v` times too small; references of the exponentials; sums
+        float o[NT][NG][2][4], ref[NT][2], l[NT][2], up_v = 0x1p120f;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            ref[nt][0] = ref[nt][1] = -INFINITY; l[nt][0] = l[nt][1] = 0.f;
+            ref[nt][0] = ref[nt][1] = -FLT_MAX; l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
             for (int gi = 0; gi < NG; gi++)
 #pragma unroll
                 for (int e = 0; e < 8; e++) o[nt][gi][e >> 2][e & 3] = 0.f;
         }
 
-        for (int i = 0; i < n; i++) {
-            const int t0 = (step0 + i) * A4_KEYS;
+        // one step; `part`: not every row sees all of its keys
+        auto step = [&](int t0, auto part) {
+            constexpr bool PARTLY = decltype(part)::value;
             const uint8_t* stage = ring + st * STAGE;
-            mbar_wait_warp(&full[warp][st], parity, a4_error, 0xb0001u, (unsigned)i);
-            // ---- scores: keys g and g + 8 of both blocks, rows 2 tq and 2 tq + 1
-            float sc[2][NT][4];
+            // ---- scores: keys g and g + 8 of a block, rows 2 tq and 2 tq + 1
+            float sc[KB][NT][4];
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < KB; b++) {
                 const uint8_t* kb = stage + b * BLOCK;
                 uint32_t w[2][NG];
                 float ks[2][NG];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const int key = g + 8 * h;
-                    a4_chunk<NG>(kb + key * (D / 2) + q4_chunk(D, key, tq) * NG * 4, w[h]);
-                    const __half2* sp = reinterpret_cast<const __half2*>(kb + q4_key_scale(D, key, 0));
-#pragma unroll
-                    for (int gi = 0; gi < NG; gi += 2) { const float2 v = __half22float2(sp[gi >> 1]); ks[h][gi] = v.x; ks[h][gi + 1] = v.y; }
+                    a4_chunk<NG>(kb + key * (D / 2) + q4_key_chunk(D, key, tq) * NG * 4, w[h]);
+                    a4_scales<NG>(kb + q4_scale(D, key, 0), ks[h]);
                 }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) sc[b][nt][0] = sc[b][nt][1] = sc[b][nt][2] = sc[b][nt][3] = 0.f;
 #pragma unroll
                 for (int gi = 0; gi < NG; gi++) {
                     const uint32_t x = w[0][gi], y = w[1][gi], x8 = x >> 8, y8 = y >> 8;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float c[4] = {off[nt][gi][0], off[nt][gi][1], off[nt][gi][0], off[nt][gi][1]};
-                        a4_mma(c, x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[nt][gi][0], qb[nt][gi][1]);
+                        float c[4];
+                        a4_mma_from(c, off[nt][gi], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[nt][gi][0], qb[nt][gi][1]);
                         a4_mma(c, x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u, qb[nt][gi][2], qb[nt][gi][3]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) sc[b][nt][e] = fmaf(ks[e >> 1][gi], c[e], sc[b][nt][e]);
+                        for (int e = 0; e < 4; e++) sc[b][nt][e] = gi ? fmaf(ks[e >> 1][gi], c[e], sc[b][nt][e]) : ks[e >> 1][gi] * c[e];
                     }
                 }
             }
-            const bool part = t0 + A4_KEYS > lim_lo;             // not every row sees all of these keys
+            // ---- scales of the values, and the largest of them
+            float vs[KB][2][NG];
+            __half2 most = a4_as_half2(0);
 #pragma unroll
-            for (int b = 0; b < 2; b++)
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const __half2* from = reinterpret_cast<const __half2*>(stage + (KB + b) * BLOCK + q4_scale(D, g + 8 * h, 0));
+#pragma unroll
+                    for (int gi = 0; gi < NG; gi += 2) {
+                        __half2 v = from[gi >> 1];
+                        if (PARTLY && t0 + b * 16 + g + 8 * h >= own) v = a4_as_half2(0);      // (whatever lies there)
+                        most = __hmax2(most, __habs2(v));
+                        const float2 f = __half22float2(v);
+                        vs[b][h][gi] = f.x; vs[b][h][gi + 1] = f.y;
+                    }
+                }
+            const float2 most2 = __half22float2(most);
+            const float top_v = fmaxf(most2.x, most2.y);
+            // ---- differences to the references, which go up where a score is far above them (as the values' power of two goes down where a scale is)
+            float up = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < KB; b++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float v = sc[b][nt][e] * by[nt][e & 1];
-                        sc[b][nt][e] = part && t0 + b * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1] ? -INFINITY : v;
+                        if (PARTLY && t0 + b * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1]) sc[b][nt][e] = -INFINITY;
+                        up = fmaxf(up, fmaf(sc[b][nt][e], by[nt][e & 1], -ref[nt][e & 1]));
                     }
-            // ---- the reference goes up where a score is far above it
-            bool above = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float mx = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]), fmaxf(sc[1][nt][j], sc[1][nt][j + 2]));
-                    above |= mx > ref[nt][j] + 6.f;
+            if (__any_sync(0xffffffffu, up > 6.f || top_v * up_v > 512.f)) {
+                float fall_v = 1.f;
+                const float all_v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
+                if (all_v * up_v > 512.f) {
+                    const float now = __uint_as_float((uint32_t)(133 - max((int)(__float_as_uint(all_v) >> 23) - 127, -24)) << 23);      // all_v * now in [64, 128)
+                    fall_v = now / up_v;                         // (powers of two; 2^-80 or less the first time, of sums that are 0)
+                    up_v = now;
                 }
-            if (__any_sync(0xffffffffu, above)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        float mx = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]), fmaxf(sc[1][nt][j], sc[1][nt][j + 2]));
+                        float mx = -INFINITY;
+#pragma unroll
+                        for (int b = 0; b < KB; b++) mx = fmaxf(mx, fmaxf(sc[b][nt][j] * by[nt][j], sc[b][nt][j + 2] * by[nt][j]));
 #pragma unroll
                         for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
                         mx = fmaxf(mx, ref[nt][j]);
-                        const float fall = ref[nt][j] == -INFINITY ? 0.f : a4_exp2(ref[nt][j] - mx);
+                        const float fall = a4_exp2(ref[nt][j] - mx);
                         ref[nt][j] = mx;
                         l[nt][j] *= fall;
 #pragma unroll
                         for (int gi = 0; gi < NG; gi++)
 #pragma unroll
-                            for (int m = 0; m < 2; m++) { o[nt][gi][m][j] *= fall; o[nt][gi][m][j + 2] *= fall; }
+                            for (int m = 0; m < 2; m++) { o[nt][gi][m][j] *= fall * fall_v; o[nt][gi][m][j + 2] *= fall * fall_v; }
                     }
             }
-            // ---- probabilities, as operands with keys in pairs
-            uint32_t pb[2][NT][2];
+            // ---- probabilities; times the values' scales, as operands with keys in pairs; weighted sums: dims 32 gi + 4 g + 2 m and + 1
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                const float r0f = ref[nt][0] == -INFINITY ? 0.f : ref[nt][0], r1f = ref[nt][1] == -INFINITY ? 0.f : ref[nt][1];
+            for (int b = 0; b < KB; b++) {
+                if (PARTLY && t0 + b * 16 >= own) break;
+                float pr[NT][4];
 #pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const float p0 = a4_exp2(sc[b][nt][0] - r0f), p1 = a4_exp2(sc[b][nt][1] - r1f), p2 = a4_exp2(sc[b][nt][2] - r0f), p3 = a4_exp2(sc[b][nt][3] - r1f);
-                    l[nt][0] += p0 + p2; l[nt][1] += p1 + p3;
-                    pb[b][nt][0] = a4_transpose(a4_half2(p0, p1)); pb[b][nt][1] = a4_transpose(a4_half2(p2, p3));
-                }
-            }
-            // ---- weighted sums: dims 32 gi + 4 g + 2 m and + 1, keys 2 tq, 2 tq + 1 and the two 8 further on
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const int k0 = t0 + b * 16;
-                if (k0 >= own) break;
-                const uint8_t* vb = stage + (2 + b) * BLOCK;
-                const int chunk = q4_chunk(D, 2 * tq, g >> 1) * NG * 4;
-                uint32_t w[4][NG], vs[NG][2];
+                    for (int e = 0; e < 4; e++) {
+                        pr[nt][e] = a4_exp2(fmaf(sc[b][nt][e], by[nt][e & 1], -ref[nt][e & 1]));
+                        l[nt][e & 1] += pr[nt][e];
+                    }
+                const uint8_t* vb = stage + (KB + b) * BLOCK;
+                uint32_t w[2][NG];
 #pragma unroll
-                for (int k = 0; k < 4; k++) a4_chunk<NG>(vb + (2 * tq + (k & 1) + 8 * (k >> 1)) * (D / 2) + chunk, w[k]);
+                for (int h = 0; h < 2; h++) a4_chunk<NG>(vb + (tq + 4 * h) * D + q4_value_chunk(D, tq, g) * NG * 4, w[h]);
 #pragma unroll
-                for (int gi = 0; gi < NG; gi += 2) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(vb + q4_value_scale(D, 2 * tq, gi));
-                    vs[gi][0] = v.x; vs[gi][1] = v.y; vs[gi + 1][0] = v.z; vs[gi + 1][1] = v.w;
-                }
-                bool bad = false;
-                if (k0 + 16 > lim_lo) {
-                    // keys that nobody sees: whatever lies there must not meet the zero weights as a value. A value that is no number must not reach rows that do not see it.
+                for (int gi = 0; gi < NG; gi++) {
+                    const uint32_t x = w[0][gi], y = w[1][gi], x8 = x >> 8, y8 = y >> 8;
+                    const float s0 = vs[b][0][gi] * up_v, s1 = vs[b][1][gi] * up_v;
 #pragma unroll
-                    for (int gi = 0; gi < NG; gi++)
+                    for (int nt = 0; nt < NT; nt++) {
+                        float z[4] = {pr[nt][0] * s0, pr[nt][1] * s0, pr[nt][2] * s1, pr[nt][3] * s1};
+                        if constexpr (PARTLY) {                  // (a scale that is no number must not reach rows that do not see its key)
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int key = k0 + 2 * tq + 8 * h;
-                            vs[gi][h] &= (key < own ? 0xffffu : 0u) | (key + 1 < own ? 0xffff0000u : 0u);
-                            bad |= (vs[gi][h] & 0x7c00u) == 0x7c00u || (vs[gi][h] & 0x7c000000u) == 0x7c000000u;
+                            for (int e = 0; e < 4; e++) if (sc[b][nt][e] == -INFINITY) z[e] = 0.f;
                         }
-                    bad = __any_sync(0xffffffffu, bad && lim_lo < own);
-                }
-                const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;  // this lane's four dims of a word
-                auto products = [&](auto&& sums) {
+                        const uint32_t b0 = a4_transpose(a4_half2(z[0], z[1])), b1 = a4_transpose(a4_half2(z[2], z[3]));
+                        a4_mma(o[nt][gi][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0, b1);
+                        a4_mma(o[nt][gi][1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, b0, b1);
 #pragma unroll
-                    for (int gi = 0; gi < NG; gi++) {
-                        const uint32_t x = __byte_perm(w[0][gi], w[1][gi], sel), y = __byte_perm(w[2][gi], w[3][gi], sel);
-                        const __half2 s0 = a4_as_half2(vs[gi][0]), s1 = a4_as_half2(vs[gi][1]);
-#pragma unroll
-                        for (int m = 0; m < 2; m++) {
-                            // 1024 + c and 1024 + 16 c as f16 numbers, then c - 8, all exact
-                            auto low = [&](uint32_t v) { return __hsub2(a4_as_half2((v >> (8 * m) & 0x000f000fu) | 0x64006400u), a4_as_half2(0x64086408u)); };
-                            auto high = [&](uint32_t v) { return __hfma2(a4_as_half2((v >> (8 * m) & 0x00f000f0u) | 0x64006400u), a4_as_half2(0x2c002c00u), a4_as_half2(0xd480d480u)); };
-                            sums(gi, m, a4_bits(__hmul2(low(x), s0)), a4_bits(__hmul2(high(x), s0)), a4_bits(__hmul2(low(y), s1)), a4_bits(__hmul2(high(y), s1)));
-                        }
-                    }
-                };
-                if (!bad) {
-                    products([&](int gi, int m, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++) a4_mma(o[nt][gi][m], a0, a1, a2, a3, pb[b][nt][0], pb[b][nt][1]);
-                    });
-                } else {
-                    // row by row of the sequence: only the keys that it sees, only its heads' sums
-#pragma unroll 1
-                    for (int t = f0 / G; t <= (f0 + n_f - 1) / G; t++) {
-                        const int most = min(s.limit(t), own);
-                        uint32_t keep[NG][2];
-#pragma unroll
-                        for (int gi = 0; gi < NG; gi++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                const int key = k0 + 2 * tq + 8 * h;
-                                keep[gi][h] = vs[gi][h];
-                                vs[gi][h] &= (key < most ? 0xffffu : 0u) | (key + 1 < most ? 0xffff0000u : 0u);
-                            }
-                        products([&](int gi, int m, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                float c[4] = {o[nt][gi][m][0], o[nt][gi][m][1], o[nt][gi][m][2], o[nt][gi][m][3]};
-                                a4_mma(c, a0, a1, a2, a3, pb[b][nt][0], pb[b][nt][1]);
-#pragma unroll
-                                for (int e = 0; e < 4; e++) if ((f0 + nt * 8 + 2 * tq + (e & 1)) / G == t) o[nt][gi][m][e] = c[e];
-                            }
-                        });
-#pragma unroll
-                        for (int gi = 0; gi < NG; gi++) { vs[gi][0] = keep[gi][0]; vs[gi][1] = keep[gi][1]; }
+                        for (int m = 0; m < 2; m++) a4_mma(o[nt][gi][m], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);      // -8 2^-24 and -8 2^-20
                     }
                 }
             }
+        };
+        for (int i = 0; i < n; i++) {
+            const int t0 = (step0 + i) * A4_KEYS;
+            mbar_wait_warp(&full[warp][st], parity, a4_error, 0xb0001u, (unsigned)i);
+            if (t0 + A4_KEYS > lim_lo) step(t0, std::true_type{});
+            else step(t0, std::false_type{});
             __syncwarp();                                        // the step's memory is free
             copy();
             if (++st == S) { st = 0; parity ^= 1; }
         }
+        // the sums as they are
+        const float down_v = 0x1p24f / up_v;
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int gi = 0; gi < NG; gi++)
+#pragma unroll
+                for (int m = 0; m < 2; m++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[nt][gi][m][e] *= e & 2 ? down_v * 0.0625f : down_v;
         u += n;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -581,15 +579,17 @@ __global__ void __launch_bounds__(128) attention_4bit_join_kernel(const Attentio
 namespace {
 template <int D, int NT>
 constexpr int a4_smem() {
-    constexpr int ring = A4_STAGES * 4 * q4_block(D), part = a4_part<D>(8 * NT) * 4;
+    constexpr int ring = A4_STAGES * 2 * A4_BLOCKS * q4_block(D), part = a4_part<D>(8 * NT) * 4;
     return A4_WARPS * ((ring > part ? ring : part) + part);
 }
 template <int D, int NT>
-cudaError_t a4_step(const Attention4Args& a, cudaStream_t s) {
+cudaError_t a4_step(Attention4Args a, cudaStream_t s) {
     constexpr int MT = 8 * NT, smem = a4_smem<D, NT>();
     if (!allow_smem<attention_4bit_step_kernel<D, NT>>(smem)) return cudaErrorInvalidValue;
     // as many CTAs as run at once, no more than there can be steps for
     const int ctas = a4_ctas(a, MT);
+    const unsigned blocks = a.r.block_tokens / Q4_TOKENS;
+    a.per_page = blocks == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / blocks);
     cudaError_t e = launch_chain(attention_4bit_step_kernel<D, NT>, dim3(ctas), dim3(A4_THREADS), smem, s, a);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};

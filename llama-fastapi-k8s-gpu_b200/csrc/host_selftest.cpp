@@ -34,8 +34,9 @@ int b2_host_gemm_group(int block) { return b2::gm_group(block); }
 int b2_host_gemm_stage(int block, int stages) { return b2::gm_stage(block, stages); }
 
 // a block of a cache in 4 bits (kv_4bit.cuh)
-int b2_host_q4_word(int dim, int token, int w) { return b2::q4_word(dim, token, w); }
-int b2_host_q4_scale(int dim, int keys, int token, int group) { return keys ? b2::q4_key_scale(dim, token, group) : b2::q4_value_scale(dim, token, group); }
+int b2_host_q4_key(int dim, int token, int w) { return b2::q4_key(dim, token, w); }
+int b2_host_q4_value(int dim, int token, int n) { return b2::q4_value(dim, token, n); }
+int b2_host_q4_scale(int dim, int token, int group) { return b2::q4_scale(dim, token, group); }
 
 // what is done once per device (per_device.h): `calls` devices in turn, refused (-1 - device) or not; how often each of the n was set up
 void b2_host_per_device(const int* calls, int n_calls, int* times, int* ready) {

@@ -2,17 +2,25 @@
 // The rotation is that of kv_append.cu, but sines and cosines too are computed in 64 bits and rounded once, and its products and sums are rounded one by one (no fused
 // multiply-add): which code an entry gets is decided at borders, and so it follows from the definition alone, whatever rotates the keys.
 //
-// Bound by memory. A CTA takes one row; a thread has a piece of eight entries of a head, one 32-bit word of codes, and four neighbouring lanes have a group.
+// Bound by memory. A warp takes a row, or a part of its heads where the rows are few, and finds its place by itself; a lane has a piece of eight entries of a head, 32 bits of
+// codes, and four neighbouring lanes have a group. Several pieces are under way at once.
 #include "device_ops.h"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 
 namespace b2 {
 
 namespace {
-constexpr int K4_THREADS = 256;
+constexpr int K4_WARPS = 8, K4_THREADS = 32 * K4_WARPS;
+// log2 of the warps a row, for up to four warps a scheduler, no more than leaves each a turn of 32 pieces of the keys
+inline int k4_parts(long rows, int pieces) {
+    int log = 0;
+    while (rows << (log + 1) <= 148 * 16 && pieces >> (log + 1) >= 32) log++;
+    return log;
+}
 
 template <typename T> __device__ __forceinline__ float k4_float(T v);
 template <> __device__ __forceinline__ float k4_float(float v) { return v; }
@@ -21,17 +29,6 @@ template <> __device__ __forceinline__ float k4_float(__nv_bfloat16 v) { return 
 
 template <typename T> struct alignas(16) K4Piece { T v[8]; };
 
-// eight entries from `p`
-template <typename T>
-__device__ __forceinline__ void k4_load(const T* p, bool wide, float (&x)[8]) {
-    K4Piece<T> t;
-    if (wide) t = *reinterpret_cast<const K4Piece<T>*>(p);
-    else
-#pragma unroll
-        for (int e = 0; e < 8; e++) t.v[e] = p[e];
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = k4_float(t.v[e]);
-}
 __device__ __forceinline__ void k4_store(__half* p, bool wide, const float (&x)[8]) {
     K4Piece<__half> t;
 #pragma unroll
@@ -59,140 +56,294 @@ __device__ __forceinline__ void k4_store(float* p, bool wide, const float (&x)[8
         for (int e = 0; e < 8; e++) p[e] = x[e];
 }
 
-// the place of a row: whether it belongs to a sequence, its token number there, and the first byte of KV head 0's block of 16 tokens, or -1; by a whole warp
-struct K4Place { int live; int token; long block; };
+// The place of a row: whether it belongs to a sequence, its token number there, and the first byte of KV head 0's block of 16 tokens, or -1; by a whole warp. Up to 32 sequences: their
+// starts and lengths in one read.
+struct K4Place { int live, token; long block; };
 __device__ __forceinline__ K4Place k4_place(const RaggedPages& r, int n_kv, int dim, int row, int lane) {
-    const int s = seq_of_row(r.row_start, r.n_seqs, row, lane);
-    K4Place p = {s < r.n_seqs && row >= r.row_start[0], 0, -1};
-    if (!p.live) return p;
-    const long at = (long)r.lengths[s] - ((long)r.row_start[s + 1] - row);
-    const long page_no = at >= 0 ? at / r.block_tokens : r.max_pages;
-    p.token = (int)at;
-    if (page_no < r.max_pages) {
-        const int page = r.pages[s * r.table_stride + page_no], blocks = r.block_tokens / Q4_TOKENS;
-        if (page >= 0 && page < r.n_pages) p.block = ((long)page * n_kv * blocks + at % r.block_tokens / Q4_TOKENS) * q4_block(dim);
+    int s, end = 0, held = 0;
+    const int first = r.row_start[0];
+    if (r.n_seqs <= 32) {
+        const bool one = lane < r.n_seqs;
+        const int e = one ? r.row_start[lane + 1] : 0, l = one ? r.lengths[lane] : 0;
+        s = __popc(__ballot_sync(0xffffffffu, one && e <= row));
+        end = __shfl_sync(0xffffffffu, e, s & 31);
+        held = __shfl_sync(0xffffffffu, l, s & 31);
+    } else {
+        s = seq_of_row(r.row_start, r.n_seqs, row, lane);
+        if (s < r.n_seqs) { end = r.row_start[s + 1]; held = r.lengths[s]; }
     }
+    K4Place p = {s < r.n_seqs && row >= first, 0, -1};
+    if (!p.live) return p;
+    const long at = (long)held - ((long)end - row);
+    p.token = (int)at;
+    if (at < 0 || at >= (long)r.max_pages * r.block_tokens) return p;      // (below 2^31)
+    const unsigned block = (unsigned)at / Q4_TOKENS, blocks = (unsigned)r.block_tokens / Q4_TOKENS, page_no = block / blocks;
+    const int page = r.pages[s * r.table_stride + page_no];
+    if (page >= 0 && page < r.n_pages) p.block = ((long)page * n_kv * blocks + (block - page_no * blocks)) * q4_block(dim);
     return p;
 }
 }  // namespace
 
-// Scale and codes of a group that four neighbouring lanes have: eight entries each, the eight codes of this lane's as a word
+// the larger one, NaN if one is
+__device__ __forceinline__ float k4_max(float a, float b) { float m; asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
+
+// Scale and codes of a group that four neighbouring lanes have: eight entries each, the eight codes of this lane's as a word.
+// A code is the low bits of entry * (1 / scale) + 8 + 1.5 2^23, whose last place is a whole number (ties to even). The product is off the quotient by 2^-22 of it at most (8.01), so that this
+// is the quotient rounded unless the fraction is within 2^-18 of a half; those are divided, as are entries by scales that are so small or large that the quotient may lie outside.
 __device__ __forceinline__ uint32_t k4_quantise(const float (&x)[8], __half& scale) {
-    float hi = x[0], lo = x[0], none = 0.f;                      // none: NaN if an entry is no finite number
+    float hi = x[0], lo = x[0];
 #pragma unroll
-    for (int e = 0; e < 8; e++) { hi = fmaxf(hi, x[e]); lo = fminf(lo, x[e]); none = fmaf(x[e], 0.f, none); }
+    for (int e = 1; e < 8; e++) { hi = k4_max(hi, x[e]); lo = fminf(lo, x[e]); }
 #pragma unroll
-    for (int o = 1; o < 4; o *= 2) {
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o)); lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        none += __shfl_xor_sync(0xffffffffu, none, o);
-    }
+    for (int o = 1; o < 4; o *= 2) { hi = k4_max(hi, __shfl_xor_sync(0xffffffffu, hi, o)); lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); }
     scale = __float2half_rn(fminf(fmaxf((hi > -lo ? hi : lo) * -0.125f, -65504.f), 65504.f));
     const float s = __half2float(scale);
+    constexpr float BIAS = 12582912.f;
+    const float r = __fdiv_rn(1.f, s);
     uint32_t word = 0;
+    float near = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const float c = s == 0.f ? 8.f : fminf(fmaxf(rintf(__fdiv_rn(x[e], s)) + 8.f, 0.f), 15.f);
-        word |= (uint32_t)c << (4 * e);
+    for (int e = 7; e >= 0; e--) {
+        const float t = fmaf(x[e], r, BIAS + 8.f);
+        near = fmaxf(near, fabsf(fmaf(x[e], r, (BIAS + 8.f) - t)));
+        word = word * 16 + __float_as_uint(fminf(t, BIAS + 15.f));
+    }
+    word -= 0x3f400000u;                                         // (what the upper bits of eight such numbers add up to)
+    if (!(near < 0.5f - 0x1p-18f) || !(fabsf(s) >= 0x1p-14f && fabsf(s) < 65504.f)) {
+        word = 0;
+#pragma unroll 1
+        for (int e = 0; e < 8; e++) {
+            float v = x[0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) v = e == i ? x[i] : v;
+            const float c = s == 0.f ? 8.f : fminf(fmaxf(rintf(__fdiv_rn(v, s)) + 8.f, 0.f), 15.f);
+            word |= (uint32_t)c << (4 * e);
+        }
     }
     if (s == 0.f) scale = __ushort_as_half(0);
-    if (none != 0.f) { scale = __ushort_as_half(0x7fff); word = 0x88888888u; }      // (NaN)
+    if (!(hi < INFINITY && lo > -INFINITY)) { scale = __ushort_as_half(0x7fff); word = 0x88888888u; }      // (NaN)
     return word;
 }
 
-template <typename In, typename Out>
-__global__ void __launch_bounds__(K4_THREADS) kv_append_4bit_kernel(const KvAppendArgs a, const int wide_k, const int wide_v, const int wide_q, const int wide_o) {
-    extern __shared__ float2 k4_turn[];                          // [rot_dims / 2] cosines and sines
-    __shared__ K4Place place;
-    const int tid = threadIdx.x, lane = tid & 31, D = a.head_dim, per_head = D / 8, half = a.rot_dims >> 1;
-    const long row = blockIdx.x;
-    if (tid < 32) {
-        const K4Place p = k4_place(a.r, a.n_kv, D, (int)row, lane);
-        if (lane == 0) place = p;
-    }
-    __syncthreads();
-    if (!place.live) return;
-    const double pos = (double)(a.first_pos + place.token);
-    for (int i = tid; i < half; i += K4_THREADS) {
-        const double turns = pos * (double)a.freqs[i] * 0.15915494309189533577;      // 1 / (2 pi)
-        double sn, cs;
-        sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
-        k4_turn[i] = make_float2((float)((double)a.amplitude * cs), (float)((double)a.amplitude * sn));
-    }
-    __syncthreads();
-    const int blocks = a.r.block_tokens / Q4_TOKENS, token = place.token & (Q4_TOKENS - 1);
-    const long block = place.block;
-    const int pieces = (2 * a.n_kv + (a.q ? a.n_head : 0)) * per_head;
-    for (int i = tid; i < (pieces + 31) / 32 * 32; i += K4_THREADS) {      // (whole warps: groups are shuffled together)
-        const bool in = i < pieces;
-        const int h = in ? i / per_head : 0, w = i - h * per_head, d = 8 * w, kind = h < a.n_kv ? 0 : h < 2 * a.n_kv ? 1 : 2;
-        const In* from = kind == 0 ? (const In*)a.k + row * a.k_row + h * a.k_head : kind == 1 ? (const In*)a.v + row * a.v_row + (h - a.n_kv) * a.v_head
-                                                                                              : (const In*)a.q + row * a.q_row + (h - 2 * a.n_kv) * a.q_head;
-        const bool wide = kind == 0 ? wide_k : kind == 1 ? wide_v : wide_q;
-        float x[8], y[8];
+__device__ __forceinline__ void k4_prefetch(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+template <typename T> __device__ __forceinline__ void k4_fetch(const T* p, bool wide, K4Piece<T>& t) {
+    if (wide) t = *reinterpret_cast<const K4Piece<T>*>(p);
+    else
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = y[e] = 0.f;
-        const bool turned = kind != 1 && d < a.rot_dims;
-        if (in) {
-            k4_load(from + d, wide, x);
-            if (turned && a.halves) {                            // the entries that these are rotated with
-                if (half % 8 == 0) k4_load(from + (d < half ? d + half : d - half), wide, y);
-                else
-#pragma unroll
-                    for (int e = 0; e < 8; e++) y[e] = d + e < a.rot_dims ? k4_float(from[d + e < half ? d + e + half : d + e - half]) : 0.f;
-            }
-        }
-        __syncwarp();                                            // a head's entries are read before they are replaced (q in place): a warp has whole heads
-        if (turned) {
-            float z[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const int at = d + e;
-                if (at >= a.rot_dims) { z[e] = x[e]; continue; }
-                const bool first = a.halves ? at < half : (e & 1) == 0;
-                const float2 t = k4_turn[a.halves ? (first ? at : at - half) : at >> 1];
-                const float other = a.halves ? y[e] : x[e ^ 1];
-                z[e] = first ? __fsub_rn(__fmul_rn(x[e], t.x), __fmul_rn(other, t.y)) : __fadd_rn(__fmul_rn(other, t.y), __fmul_rn(x[e], t.x));
-            }
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = z[e];
-        }
-        if (kind == 2) {
-            if (in) k4_store((Out*)a.q_out + row * a.qo_row + (h - 2 * a.n_kv) * a.qo_head + d, wide_o, x);
-        }
-        __half scale;
-        const uint32_t word = k4_quantise(x, scale);
-        if (in && kind != 2 && block >= 0) {
-            uint8_t* to = (uint8_t*)(kind == 0 ? a.k_pool : a.v_pool) + block + (long)(kind == 0 ? h : h - a.n_kv) * blocks * q4_block(D);
-            *reinterpret_cast<uint32_t*>(to + q4_word(D, token, w)) = word;
-            if ((w & 3) == 0) *reinterpret_cast<__half*>(to + (kind == 0 ? q4_key_scale(D, token, w >> 2) : q4_value_scale(D, token, w >> 2))) = scale;
-        }
-    }
+        for (int e = 0; e < 8; e++) t.v[e] = p[e];
 }
 
-// a row a CTA
-template <typename Out>
-__global__ void __launch_bounds__(K4_THREADS) kv_read_4bit_kernel(const KvReadArgs a, const int wide_k, const int wide_v) {
-    __shared__ K4Place place;
-    const int tid = threadIdx.x, D = a.head_dim, per_head = D / 8;
-    const long row = blockIdx.x;
-    if (tid < 32) {
-        const K4Place p = k4_place(a.r, a.n_kv, D, (int)row, tid);
-        if (tid == 0) place = p;
-    }
-    __syncthreads();
-    if (place.block < 0) return;
-    const int blocks = a.r.block_tokens / Q4_TOKENS, token = place.token & (Q4_TOKENS - 1);
-    const int first = a.k ? 0 : a.n_kv, last = a.v ? 2 * a.n_kv : a.n_kv;
-    for (int i = first * per_head + tid; i < last * per_head; i += K4_THREADS) {
-        const int h2 = i / per_head, w = i - h2 * per_head, h = h2 < a.n_kv ? h2 : h2 - a.n_kv;
-        const bool key = h2 < a.n_kv;
-        const uint8_t* from = (const uint8_t*)(key ? a.k_pool : a.v_pool) + place.block + (long)h * blocks * q4_block(D);
-        const uint32_t word = *reinterpret_cast<const uint32_t*>(from + q4_word(D, token, w));
-        const float s = __half2float(*reinterpret_cast<const __half*>(from + (key ? q4_key_scale(D, token, w >> 2) : q4_value_scale(D, token, w >> 2))));
-        float x[8];
+// How keys are rotated: entries of a piece with each other, a piece with another one, or any (halves that are no whole pieces, a rotation that ends inside one)
+enum K4Turn { K4_PAIRS, K4_HALVES, K4_ANY };
+
+// `wide`: bits 0 .. 3, whether pieces of k, v, q and q_out are 16 bytes at 16-byte addresses. `parts`: log2 of the warps a row
+template <typename In, int D, int TURN>
+__global__ void __launch_bounds__(K4_THREADS, 3) kv_append_4bit_kernel(const KvAppendArgs a, const int wide, const int parts) {
+    constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, UNROLL = sizeof(In) == 4 || TURN != K4_PAIRS ? 2 : 4;      // pieces of a head, heads of a turn, turns under way
+    __shared__ alignas(16) float2 turns[K4_WARPS][D / 2];        // cosines and sines of the warp's row
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.rot_dims >> 1;
+    const long item = (long)blockIdx.x * K4_WARPS + warp, row = item >> parts;
+    if (row >= a.r.n_rows) return;
+    const int part = (int)(item - (row << parts)), w = lane % PIECES, d = 8 * w, h0 = lane / PIECES;
+    const bool rotates = d < a.rot_dims, left = d < half;
+    K4Place place;
+    bool ready = false;
+    float2* turn = turns[warp];
+    const long step = (long)(a.r.block_tokens / Q4_TOKENS) * q4_block(D);
+    // KIND 0: keys, 1: values, 2: queries. Each warp of the row has a part of the heads of each. False: the row has no sequence.
+    auto heads_of = [&](auto kind, const In* base, long head, int heads, int wide_in) {
+        constexpr int KIND = decltype(kind)::value;
+        const int all = (heads + AT_ONCE - 1) / AT_ONCE, last = all * (part + 1) >> parts;
+        int i = all * part >> parts;
+        const In* from = base + (i * AT_ONCE + h0) * head;
+        K4Piece<In> x[UNROLL], y[UNROLL];
+        int loaded = i;                                          // turns whose entries are under way or here
+        auto load = [&](K4Piece<In>& p, K4Piece<In>& q) {
+            if (loaded < last && loaded * AT_ONCE + h0 < heads) {
+                k4_fetch(from, wide_in, p);
+                if constexpr (KIND != 1 && TURN == K4_HALVES) { if (rotates) k4_fetch(left ? from + half : from - half, wide_in, q); }
+                if constexpr (KIND != 1 && TURN == K4_ANY) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = s * (float)((int)(word >> (4 * e) & 15) - 8);
-        k4_store((key ? (Out*)a.k + row * a.k_row + h * a.k_head : (Out*)a.v + row * a.v_row + h * a.v_head) + 8 * w, key ? wide_k : wide_v, x);
+                    for (int e = 0; e < 8; e++) {
+                        const int at = d + e, other = a.halves ? (at < half ? at + half : at - half) : at ^ 1;
+                        q.v[e] = at < a.rot_dims ? from[other - d] : p.v[e];
+                    }
+                }
+            }
+            from += AT_ONCE * head;
+            loaded++;
+        };
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) load(x[u], y[u]);
+        if (!ready) {                                            // (the first entries are under way)
+            ready = true;
+            place = k4_place(a.r, a.n_kv, D, (int)row, lane);
+            if (!place.live) return false;
+            const double pos = (double)(a.first_pos + place.token);
+            for (int j = lane; j < half; j += 32) {
+                const double t = pos * (double)a.freqs[j] * 0.15915494309189533577;      // 1 / (2 pi)
+                double sn, cs;
+                sincospi(2.0 * (t - rint(t)), &sn, &cs);
+                turn[j] = make_float2((float)((double)a.amplitude * cs), (float)((double)a.amplitude * sn));
+            }
+            __syncwarp();
+        }
+        const int token = place.token & (Q4_TOKENS - 1);
+        uint8_t* pool = (uint8_t*)(KIND == 0 ? a.k_pool : a.v_pool) + place.block + (i * AT_ONCE + h0) * step;
+        const long out_at = KIND == 2 ? row * a.qo_row + d : 0;
+#pragma unroll 1
+        while (i < last) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                if (i >= last) break;
+                const int h = i * AT_ONCE + h0;
+                const bool in = h < heads;
+                float z[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) z[e] = in ? k4_float(x[u].v[e]) : 0.f;
+                if constexpr (KIND != 1) {
+                    if (rotates) {
+                        if constexpr (TURN == K4_PAIRS) {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 4) {
+                                const float4 t = *reinterpret_cast<const float4*>(turn + (d + e) / 2);
+                                const float v0 = z[e], v1 = z[e + 1], v2 = z[e + 2], v3 = z[e + 3];
+                                z[e] = __fsub_rn(__fmul_rn(v0, t.x), __fmul_rn(v1, t.y)); z[e + 1] = __fadd_rn(__fmul_rn(v1, t.x), __fmul_rn(v0, t.y));
+                                z[e + 2] = __fsub_rn(__fmul_rn(v2, t.z), __fmul_rn(v3, t.w)); z[e + 3] = __fadd_rn(__fmul_rn(v3, t.z), __fmul_rn(v2, t.w));
+                            }
+                        } else if constexpr (TURN == K4_HALVES) {
+                            const float2* with = turn + (left ? d : d - half);
+                            const float sign = left ? -1.f : 1.f;
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) {
+                                const float4 t = *reinterpret_cast<const float4*>(with + e);
+                                z[e] = __fadd_rn(__fmul_rn(z[e], t.x), __fmul_rn(k4_float(y[u].v[e]), sign * t.y));
+                                z[e + 1] = __fadd_rn(__fmul_rn(z[e + 1], t.z), __fmul_rn(k4_float(y[u].v[e + 1]), sign * t.w));
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                const int at = d + e;
+                                if (at >= a.rot_dims) continue;
+                                const bool one = a.halves ? at < half : (e & 1) == 0;
+                                const float2 t = turn[a.halves ? (one ? at : at - half) : at >> 1];
+                                z[e] = __fadd_rn(__fmul_rn(z[e], t.x), __fmul_rn(k4_float(y[u].v[e]), one ? -t.y : t.y));
+                            }
+                        }
+                    }
+                }
+                if constexpr (KIND == 2) {
+                    __syncwarp();                                // (a head's entries are read before they are replaced: q in place)
+                    if (in) {
+                        if (a.cache_type == ELEM_F16) k4_store((__half*)a.q_out + out_at + h * a.qo_head, wide >> 3 & 1, z);
+                        else k4_store((__nv_bfloat16*)a.q_out + out_at + h * a.qo_head, wide >> 3 & 1, z);
+                    }
+                    load(x[u], y[u]);
+                } else {
+                    load(x[u], y[u]);
+                    __half scale;
+                    const uint32_t word = k4_quantise(z, scale);
+                    if (in && place.block >= 0) {
+                        if (KIND == 0) *reinterpret_cast<uint32_t*>(pool + q4_key(D, token, w)) = word;
+                        else {
+                            *reinterpret_cast<uint16_t*>(pool + q4_value(D, token, 2 * w)) = (uint16_t)word;
+                            *reinterpret_cast<uint16_t*>(pool + q4_value(D, token, 2 * w + 1)) = (uint16_t)(word >> 16);
+                        }
+                        if ((w & 3) == 0) *reinterpret_cast<__half*>(pool + q4_scale(D, token, w >> 2)) = scale;
+                    }
+                    pool += AT_ONCE * step;
+                }
+                i++;
+            }
+        }
+        return true;
+    };
+    // the values and queries of a row that is one warp's alone: on their way into L2 while the keys are dealt with
+    if (parts == 0) {
+        constexpr int LINES = D * (int)sizeof(In) / 128;
+        for (int i = lane; i < a.n_kv * LINES; i += 32) k4_prefetch((const In*)a.v + row * a.v_row + i / LINES * a.v_head + i % LINES * (128 / sizeof(In)));
+        if (a.q) for (int i = lane; i < a.n_head * LINES; i += 32) k4_prefetch((const In*)a.q + row * a.q_row + i / LINES * a.q_head + i % LINES * (128 / sizeof(In)));
+    }
+    if (!heads_of(std::integral_constant<int, 0>{}, (const In*)a.k + row * a.k_row + d, a.k_head, a.n_kv, wide & 1)) return;
+    heads_of(std::integral_constant<int, 1>{}, (const In*)a.v + row * a.v_row + d, a.v_head, a.n_kv, wide >> 1 & 1);
+    if (a.q) heads_of(std::integral_constant<int, 2>{}, (const In*)a.q + row * a.q_row + d, a.q_head, a.n_head, wide >> 2 & 1);
+}
+
+// The eight codes of a word less 8, and those times their scale, rounded once
+__device__ __forceinline__ void k4_codes(uint32_t word, __half2 (&v)[4]) {
+    // byte i twice, its codes as 1024 + c and 1024 + 16 c, and those as c - 8, exact
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t two = (__byte_perm(word, 0, i | 0x40 | i << 8 | 0x4000) & 0x00f0000fu) | 0x64006400u;
+        v[i] = __hfma2(*reinterpret_cast<const __half2*>(&two), __halves2half2(__ushort_as_half(0x3c00), __ushort_as_half(0x2c00)),
+                       __halves2half2(__ushort_as_half(0xe408), __ushort_as_half(0xd480)));
+    }
+}
+__device__ __forceinline__ void k4_put(__half* p, bool wide, const __half2 (&v)[4], __half scale) {
+    K4Piece<__half> t;
+    const __half2 s = __half2half2(scale);
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const __half2 x = __hmul2(v[i], s); t.v[2 * i] = __low2half(x); t.v[2 * i + 1] = __high2half(x); }
+    if (wide) *reinterpret_cast<K4Piece<__half>*>(p) = t;
+    else
+#pragma unroll
+        for (int e = 0; e < 8; e++) p[e] = t.v[e];
+}
+template <typename Out>
+__device__ __forceinline__ void k4_put(Out* p, bool wide, const __half2 (&v)[4], __half scale) {
+    float x[8];
+    const float s = __half2float(scale);
+#pragma unroll
+    for (int i = 0; i < 4; i++) { const float2 f = __half22float2(v[i]); x[2 * i] = s * f.x; x[2 * i + 1] = s * f.y; }
+    k4_store(p, wide, x);
+}
+
+// ROWS: rows of a warp, whose places are found at once
+template <typename Out, int D, int ROWS>
+__global__ void __launch_bounds__(K4_THREADS) kv_read_4bit_kernel(const KvReadArgs a, const int wide, const int parts) {
+    constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, UNROLL = 4;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long item = (long)blockIdx.x * K4_WARPS + warp, row0 = (item >> parts) * ROWS;
+    if (row0 >= a.r.n_rows) return;
+    K4Place places[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) places[i] = k4_place(a.r, a.n_kv, D, (int)min(row0 + i, (long)a.r.n_rows - 1), lane);
+    const int part = (int)(item - (item >> parts << parts));
+#pragma unroll
+    for (int r = 0; r < ROWS; r++) {
+    const long row = row0 + r;
+    const K4Place place = places[r];
+    if (row >= a.r.n_rows || place.block < 0) continue;
+    const int token = place.token & (Q4_TOKENS - 1), w = lane % PIECES, h0 = lane / PIECES;
+    const int all = (a.n_kv + AT_ONCE - 1) / AT_ONCE, first = all * part >> parts, last = all * (part + 1) >> parts;
+    const long step = (long)(a.r.block_tokens / Q4_TOKENS) * q4_block(D), begin = place.block + (first * AT_ONCE + h0) * step;
+    const uint8_t *kp = (const uint8_t*)a.k_pool + begin + q4_key(D, token, w), *vp = (const uint8_t*)a.v_pool + begin + q4_value(D, token, 2 * w);
+    const int next = q4_value(D, token, 2 * w + 1) - q4_value(D, token, 2 * w), ks = q4_scale(D, token, w >> 2) - q4_key(D, token, w), vs = q4_scale(D, token, w >> 2) - q4_value(D, token, 2 * w);
+    Out* k = (Out*)a.k + row * a.k_row + (first * AT_ONCE + h0) * a.k_head + 8 * w;
+    Out* v = (Out*)a.v + row * a.v_row + (first * AT_ONCE + h0) * a.v_head + 8 * w;
+    const int n = min(last - first, (a.n_kv - h0 + AT_ONCE - 1) / AT_ONCE - first);      // heads of this lane
+    for (int i = 0; i < n; i += UNROLL) {
+        uint32_t kw[UNROLL], vw[UNROLL];
+        __half sk[UNROLL], sv[UNROLL];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            if (i + u >= n) break;
+            if (a.k) { kw[u] = *reinterpret_cast<const uint32_t*>(kp); sk[u] = *reinterpret_cast<const __half*>(kp + ks); }
+            if (a.v) {
+                vw[u] = *reinterpret_cast<const uint16_t*>(vp) | (uint32_t)*reinterpret_cast<const uint16_t*>(vp + next) << 16;
+                sv[u] = *reinterpret_cast<const __half*>(vp + vs);
+            }
+            kp += AT_ONCE * step; vp += AT_ONCE * step;
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            if (i + u >= n) break;
+            __half2 c[4];
+            if (a.k) { k4_codes(kw[u], c); k4_put(k, wide & 1, c, sk[u]); }
+            if (a.v) { k4_codes(vw[u], c); k4_put(v, wide >> 1 & 1, c, sv[u]); }
+            k += AT_ONCE * a.k_head; v += AT_ONCE * a.v_head;
+        }
+    }
     }
 }
 
@@ -200,33 +351,42 @@ __global__ void __launch_bounds__(K4_THREADS) kv_read_4bit_kernel(const KvReadAr
 // 16 bytes at a time wherever eight entries of a row start
 static int k4_wide(const void* p, long row, long head, int size) { return ((uintptr_t)p & 15) == 0 && row * size % 16 == 0 && head * size % 16 == 0; }
 
-template <typename In, typename Out>
+static unsigned k4_ctas(long rows, int parts) { return (unsigned)(((rows << parts) + K4_WARPS - 1) / K4_WARPS); }
+
+template <typename In, int D>
 static cudaError_t k4_append(const KvAppendArgs& a, cudaStream_t s) {
+    const int size = sizeof(In), parts = k4_parts(a.r.n_rows, a.n_kv * D / 8);
+    const int wide = k4_wide(a.k, a.k_row, a.k_head, size) | k4_wide(a.v, a.v_row, a.v_head, size) << 1 | k4_wide(a.q, a.q_row, a.q_head, size) << 2 | k4_wide(a.q_out, a.qo_row, a.qo_head, 2) << 3;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.r.n_rows); cfg.blockDim = dim3(K4_THREADS); cfg.dynamicSmemBytes = sizeof(float2) * (a.rot_dims / 2); cfg.stream = s;
-    const int size = sizeof(In);
-    return cudaLaunchKernelEx(&cfg, kv_append_4bit_kernel<In, Out>, a, k4_wide(a.k, a.k_row, a.k_head, size), k4_wide(a.v, a.v_row, a.v_head, size), k4_wide(a.q, a.q_row, a.q_head, size),
-                              k4_wide(a.q_out, a.qo_row, a.qo_head, 2));
+    cfg.gridDim = dim3(k4_ctas(a.r.n_rows, parts)); cfg.blockDim = dim3(K4_THREADS); cfg.stream = s;
+    if (a.rot_dims % (a.halves ? 16 : 8)) return cudaLaunchKernelEx(&cfg, kv_append_4bit_kernel<In, D, K4_ANY>, a, wide, parts);
+    return a.halves ? cudaLaunchKernelEx(&cfg, kv_append_4bit_kernel<In, D, K4_HALVES>, a, wide, parts) : cudaLaunchKernelEx(&cfg, kv_append_4bit_kernel<In, D, K4_PAIRS>, a, wide, parts);
 }
+template <typename In>
+static cudaError_t k4_append_dim(const KvAppendArgs& a, cudaStream_t s) { return a.head_dim == 64 ? k4_append<In, 64>(a, s) : k4_append<In, 128>(a, s); }
 cudaError_t kv_append_4bit_launch(const KvAppendArgs& a, cudaStream_t s) {
     if (a.r.n_rows == 0) return cudaSuccess;
-    const bool h = a.cache_type == ELEM_F16;
-    switch (a.in_type) {
-        case ELEM_F32: return h ? k4_append<float, __half>(a, s) : k4_append<float, __nv_bfloat16>(a, s);
-        case ELEM_F16: return h ? k4_append<__half, __half>(a, s) : k4_append<__half, __nv_bfloat16>(a, s);
-        default: return h ? k4_append<__nv_bfloat16, __half>(a, s) : k4_append<__nv_bfloat16, __nv_bfloat16>(a, s);
-    }
+    return a.in_type == ELEM_F32 ? k4_append_dim<float>(a, s) : a.in_type == ELEM_F16 ? k4_append_dim<__half>(a, s) : k4_append_dim<__nv_bfloat16>(a, s);
 }
 
-template <typename Out>
+template <typename Out, int D>
 static cudaError_t k4_read(const KvReadArgs& a, cudaStream_t s) {
+    const int parts = k4_parts(a.r.n_rows, a.n_kv * D / 8), wide = k4_wide(a.k, a.k_row, a.k_head, sizeof(Out)) | k4_wide(a.v, a.v_row, a.v_head, sizeof(Out)) << 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)a.r.n_rows); cfg.blockDim = dim3(K4_THREADS); cfg.stream = s;
-    return cudaLaunchKernelEx(&cfg, kv_read_4bit_kernel<Out>, a, k4_wide(a.k, a.k_row, a.k_head, sizeof(Out)), k4_wide(a.v, a.v_row, a.v_head, sizeof(Out)));
+    cfg.blockDim = dim3(K4_THREADS); cfg.stream = s;
+    // four rows a warp once that leaves a warp for every place on the SMs
+    if (a.r.n_rows >= 4 * 148 * 40) {
+        cfg.gridDim = dim3(k4_ctas((a.r.n_rows + 3) / 4, 0));
+        return cudaLaunchKernelEx(&cfg, kv_read_4bit_kernel<Out, D, 4>, a, wide, 0);
+    }
+    cfg.gridDim = dim3(k4_ctas(a.r.n_rows, parts));
+    return cudaLaunchKernelEx(&cfg, kv_read_4bit_kernel<Out, D, 1>, a, wide, parts);
 }
+template <typename Out>
+static cudaError_t k4_read_dim(const KvReadArgs& a, cudaStream_t s) { return a.head_dim == 64 ? k4_read<Out, 64>(a, s) : k4_read<Out, 128>(a, s); }
 cudaError_t kv_read_4bit_launch(const KvReadArgs& a, cudaStream_t s) {
     if (a.r.n_rows == 0 || (!a.k && !a.v)) return cudaSuccess;
-    return a.out_type == ELEM_F32 ? k4_read<float>(a, s) : a.out_type == ELEM_F16 ? k4_read<__half>(a, s) : k4_read<__nv_bfloat16>(a, s);
+    return a.out_type == ELEM_F32 ? k4_read_dim<float>(a, s) : a.out_type == ELEM_F16 ? k4_read_dim<__half>(a, s) : k4_read_dim<__nv_bfloat16>(a, s);
 }
 
 }  // namespace b2

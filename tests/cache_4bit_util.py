@@ -37,11 +37,15 @@ def places(D, keys):
     """byte of a block's codes [16, dim / 2] and 16-bit place of its scales [16, dim / 32], token by token"""
     n = D // GROUP
     t, j = torch.arange(16)[:, None], torch.arange(D // 2)[None]
-    word = j // 4
-    chunk = (word % 4) ^ ((t // 2) % 4 if D == 128 else (t // 4) % 2 * 2)
-    codes = t * (D // 2) + 4 * (chunk * n + word // 4) + j % 4
-    g = torch.arange(n)[None]
-    return codes, t * n + g if keys else t % 8 // 2 * 4 * n + 4 * g + t % 2 + 2 * (t // 8)
+    if keys:                         # four bytes a word, a row a token
+        word = j // 4
+        chunk = (word % 4) ^ ((t // 2) % 4 if D == 128 else (t // 4) % 2 * 2)
+        codes = t * (D // 2) + 4 * (chunk * n + word // 4) + j % 4
+    else:                            # two bytes a half of a word, a row two tokens
+        half = j // 2
+        chunk = (half % 8) ^ ((t // 2) % 4 * 2 if D == 128 else (t // 4) % 2 * 4)
+        codes = t // 2 * D + 4 * (chunk * n + half // 8) + t % 2 * 2 + j % 2
+    return codes, t * n + torch.arange(n)[None]
 
 
 def packed(codes, scales, keys):
@@ -123,17 +127,19 @@ class Cache4:
 
 
 def attention_exact(c, q, rows, scale=None, max_rows=None, k=None, v=None):
-    """out; sum of weight * |value|; scale * sum over d of |q_d| 8 |scale of the key's group|, the largest of a row; sum of |values| that a row sees"""
+    """out; sum of weight * |value|; the same of 8 |scale of the value's group|; scale * sum over d of |q_d| 8 |scale of the key's group|, the largest of a row; sum over the keys that a row
+    sees of |value| and an eighth of the head's largest scale"""
     R, H, D = q.shape
     G = H // c.n_kv
     scale = D ** -0.5 if scale is None else scale
     k, v = c.values(c.k) if k is None else k, c.values(c.v) if v is None else v
-    steps = 8 * quantised(c.k)[1].to(F64).abs().repeat_interleave(GROUP, -1).to(c.device)
+    steps, steps_v = (8 * torch.nan_to_num(quantised(x)[1].to(F64).abs()).repeat_interleave(GROUP, -1).to(c.device) for x in (c.k, c.v))
+    least = torch.nan_to_num(quantised(c.v)[1].to(F64).abs()).amax(-1).to(c.device) / 8
     out = torch.zeros(R, H, D, dtype=F64, device=q.device)
-    spread, all_v, reach = out.clone(), out.clone(), torch.zeros(R, H, dtype=F64, device=q.device)
+    spread, offset, all_v, reach = out.clone(), out.clone(), out.clone(), torch.zeros(R, H, dtype=F64, device=q.device)
     r0 = 0
     for s, (n, o) in enumerate(zip(rows, c.own)):
-        ks, vs, st = (x[c.start[s]:c.start[s] + o].transpose(0, 1) for x in (k, v, steps))
+        ks, vs, st, sv = (x[c.start[s]:c.start[s] + o].transpose(0, 1) for x in (k, v, steps, steps_v))
         seen = o - n + 1 + torch.arange(n, device=q.device)
         if max_rows is not None:
             seen[max_rows:] = 0
@@ -144,16 +150,20 @@ def attention_exact(c, q, rows, scale=None, max_rows=None, k=None, v=None):
             w = torch.nan_to_num(torch.softmax(score, -1)) if (seen <= 0).any() else torch.softmax(score, -1)
             out[r0:r0 + n] = (w @ vs).reshape(n, H, D)
             spread[r0:r0 + n] = (w @ vs.abs()).reshape(n, H, D)
-            all_v[r0:r0 + n] = (mask.to(F64)[:, None, None] @ vs.abs()).expand(n, c.n_kv, G, D).reshape(n, H, D)
+            offset[r0:r0 + n] = (w @ sv).reshape(n, H, D)
+            each = vs.abs() + least[c.start[s]:c.start[s] + o].amax(0)[:, None, None]
+            all_v[r0:r0 + n] = (mask.to(F64)[:, None, None] @ each).expand(n, c.n_kv, G, D).reshape(n, H, D)
             reach[r0:r0 + n] = (x.abs() @ st.transpose(1, 2)).masked_fill(~mask[:, None, None], 0.0).amax(-1).reshape(n, H) * scale
         r0 += n
-    return out, spread, reach, all_v
+    return out, spread, offset, reach, all_v
 
 
-def attention_bar(typ, out, spread, reach, all_v, dim):
-    """One rounding of the output. Probabilities and values are rounded to f16 each. A score is a sum of dim products and of one offset a group, none larger together than
-    |q| 8 |scale|, in 32 bits that a matrix instruction may cut off instead of rounding: within 2 (dim + 16) 2^-24 of it; weights change by that much relative, in numerator
-    and denominator. 2^-18 for the exponential's 2^-22 and for joins. The smallest f16 numbers are 2^-24 apart: every weight, relative to one that is at least 1, and every value may be off by half
-    of that."""
+def attention_bar(typ, out, spread, offset, reach, all_v, dim):
+    """One rounding of the output. Probabilities and values, or their scales, are rounded to f16, twice at most. A score is a sum of dim products and of one offset a group, none
+    larger together than |q| 8 |scale|, in 32 bits that a matrix instruction may cut off instead of rounding: within 2 (dim + 16) 2^-24 of it; weights change by that much relative,
+    in numerator and denominator. 2^-18 for the exponential's 2^-22 and for joins. The smallest f16 numbers are 2^-24 apart: a weight, relative to one that is at least 1, may be off by half of
+    that, and so may one times its value's scale where the largest scale is held to 64 or more: 8 / 64 of it an entry.
+    Codes are multiplied without their offset of 8, which is taken off the sum: per 16 keys two instructions of 17 addends that may each be cut off at 2^-23 of the largest, at most 15 / 8 of
+    a weight times 8 |scale|: within 2^-17 of the weighted sum of 8 |scale|."""
     u16 = unit("f16")
-    return unit(typ) * out.abs() + (2 * u16 + 4 * (dim + 16) * 2 ** -24 * reach[..., None] + 2 ** -18) * spread + 2 ** -25 * all_v + 2 ** -24
+    return unit(typ) * out.abs() + (2 * u16 + 4 * (dim + 16) * 2 ** -24 * reach[..., None] + 2 ** -18) * spread + 2 ** -17 * offset + 2 ** -25 * all_v + 2 ** -24

@@ -18,42 +18,39 @@ def host(native_lib):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
-def test_block_layout(host, dim):
-    """every word and scale of a block has a place of its own, all of them fill it, and it is the tests' own"""
+@pytest.mark.parametrize("keys", [True, False])
+def test_block_layout(host, dim, keys):
+    """every piece and scale of a block has a place of its own, all of them fill it, and it is the tests' own"""
+    codes, scales = torch.zeros(16, dim, dtype=torch.uint8), torch.zeros(16, dim // 32, dtype=torch.float16)
     used = [0] * (9 * dim)
-    for keys in (1, 0):
-        codes, scales = torch.zeros(16, dim, dtype=torch.uint8), torch.zeros(16, dim // 32, dtype=torch.float16)
-        used = [0] * (9 * dim)
-        for t in range(16):
-            for w in range(dim // 8):
-                at = host.b2_host_q4_word(dim, t, w)
-                assert at % 4 == 0
-                for b in range(4):
-                    used[at + b] += 1
-                one = codes.clone()
-                one[t, 8 * w:8 * w + 8] = torch.arange(1, 9)
-                assert packed(one, scales, keys)[at:at + 4].tolist() == [0x21, 0x43, 0x65, 0x87]
-            for g in range(dim // 32):
-                at = host.b2_host_q4_scale(dim, keys, t, g)
-                used[at] += 1
-                used[at + 1] += 1
-                one = scales.clone()
-                one[t, g] = 1.0
-                assert packed(codes, one, keys)[at + 1].item() == 0x3c
-        assert used == [1] * (9 * dim)
-    # the four words that a lane takes at once are neighbours, 16 (8) bytes aligned
-    n = dim // 32
+    size = 4 if keys else 2          # bytes of a piece
+    place = host.b2_host_q4_key if keys else host.b2_host_q4_value
     for t in range(16):
-        for w in range(4):
-            first = host.b2_host_q4_word(dim, t, w)
-            assert first % (4 * n) == 0 and [host.b2_host_q4_word(dim, t, w + 4 * g) for g in range(n)] == [first + 4 * g for g in range(n)]
-    # the two pairs of keys of a lane of a value fragment: chunk and scales alike
-    for t in range(0, 8, 2):
-        for w in range(4):
-            assert len({host.b2_host_q4_word(dim, u, w) - u * dim // 2 for u in (t, t + 1, t + 8, t + 9)}) == 1
-        for g in range(n):
-            first = host.b2_host_q4_scale(dim, 0, t, g)
-            assert first % 8 == 0 and [host.b2_host_q4_scale(dim, 0, u, g) - first for u in (t, t + 1, t + 8, t + 9)] == [0, 2, 4, 6]
+        for w in range(dim // 2 // size):
+            at = place(dim, t, w)
+            assert at % size == 0
+            for b in range(size):
+                used[at + b] += 1
+            one = codes.clone()
+            one[t, 2 * size * w:2 * size * (w + 1)] = torch.arange(1, 2 * size + 1)
+            assert packed(one, scales, keys)[at:at + size].tolist() == [0x21, 0x43, 0x65, 0x87][:size]
+        for g in range(dim // 32):
+            at = host.b2_host_q4_scale(dim, t, g)
+            used[at] += 1
+            used[at + 1] += 1
+            one = scales.clone()
+            one[t, g] = 1.0
+            assert packed(codes, one, keys)[at + 1].item() == 0x3c
+    assert used == [1] * (9 * dim)
+    # the words that a lane takes at once, one of every group, are neighbours, 16 (8) bytes aligned; no two of a quarter (half) warp's chunks share a bank
+    n, chunk = dim // 32, dim // 8
+    for t in range(16):
+        for w in range(4 if keys else 8):
+            first = place(dim, t & ~1 if not keys else t, w)
+            assert first % chunk == 0 and [place(dim, t & ~1 if not keys else t, w + (4 if keys else 8) * g) for g in range(n)] == [first + 4 * g for g in range(n)]
+    for lanes in range(0, 32, 128 // chunk):
+        where = [place(dim, lane >> 2, lane & 3) if keys else place(dim, 2 * (lane & 3), lane >> 2) for lane in range(lanes, lanes + 128 // chunk)]
+        assert len({at // chunk % (128 // chunk) for at in where}) == len(where)
 
 
 def test_definition():
@@ -70,15 +67,15 @@ def test_definition():
 
 def test_a_cache_holds_its_rows(host):
     c = Cache4(1, 2, 64, 48, [5, 0, 50], device="cpu", fill=0)
-    for pool, rows, keys in ((c.bytes_k, c.k, True), (c.bytes_v, c.v, False)):
+    for pool, rows, place, n in ((c.bytes_k, c.k, host.b2_host_q4_key, 8), (c.bytes_v, c.v, host.b2_host_q4_value, 4)):
         codes, scales = quantised(rows)
         for s, t in ((0, 0), (0, 4), (2, 0), (2, 33), (2, 49)):
             block, at = pool[c.table[s, t // 48].item(), 1, t % 48 // 16], c.start[s] + t
-            for w in range(8):
-                b = host.b2_host_q4_word(64, t % 16, w)
-                assert block[b:b + 4].tolist() == [int(codes[at, 1, 8 * w + e] + 16 * codes[at, 1, 8 * w + e + 1]) for e in range(0, 8, 2)]
+            for w in range(64 // n):
+                b = place(64, t % 16, w)
+                assert block[b:b + n // 2].tolist() == [int(codes[at, 1, n * w + e] + 16 * codes[at, 1, n * w + e + 1]) for e in range(0, n, 2)]
             for g in range(2):
-                b = host.b2_host_q4_scale(64, int(keys), t % 16, g)
+                b = host.b2_host_q4_scale(64, t % 16, g)
                 assert block[b:b + 2].view(torch.float16).item() == scales[at, 1, g].item()
         last = pool[c.table[0, 0].item(), :, 0]                  # five tokens of 16
         assert (last != 0).sum() <= 2 * 5 * (32 + 4) and (pool[c.table[0, 0].item(), :, 1:] == 0).all()
