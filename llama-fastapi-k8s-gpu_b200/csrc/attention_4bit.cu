@@ -14,7 +14,7 @@
 //     to f16 once (2^-11), whatever the type of queries and output; the offset of 8 is a product of that operand and a constant. Scales are taken at a power of two that keeps the
 //     operand in f16's range, found from the scales as they come. Score fragments become operands by movmatrix.
 // The reference of a row's exponentials moves only where a score exceeds it by 2^6.
-#include "device_ops.h"
+#include "attention_4bit.cuh"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"
 #include <cuda_bf16.h>
@@ -35,9 +35,7 @@ constexpr int A4_SMS = 148;
 __device__ unsigned int a4_error[5];                             // see mbar_give_up
 
 __device__ __forceinline__ float a4_exp2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ uint32_t a4_half2(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
 __device__ __forceinline__ __half2 a4_as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-__device__ __forceinline__ uint32_t a4_bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 __device__ __forceinline__ void a4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -99,23 +97,6 @@ struct A4At {
 
 // partial results in 32 bits: [rows of a tile][D] weighted sums, then [rows][2] (reference in log2, sum)
 template <int D> __host__ __device__ constexpr int a4_part(int mt) { return mt * (D + 2); }
-
-// four neighbouring dims of a row's output
-__device__ __forceinline__ void a4_store_out(const Attention4Args& a, int t, int head, int d, float x, float y, float z, float w) {
-    uint32_t lo, hi;
-    if (a.type == ELEM_F16) { lo = a4_half2(x, y); hi = a4_half2(z, w); }
-    else {
-        const __nv_bfloat162 l = __floats2bfloat162_rn(x, y), h = __floats2bfloat162_rn(z, w);
-        lo = *reinterpret_cast<const uint32_t*>(&l); hi = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    uint16_t* dst = (uint16_t*)a.out + (size_t)t * a.out_row + (size_t)head * a.out_head + d;
-    if (((uintptr_t)dst & 7) == 0) *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
-    else { dst[0] = (uint16_t)lo; dst[1] = (uint16_t)(lo >> 16); dst[2] = (uint16_t)hi; dst[3] = (uint16_t)(hi >> 16); }
-}
-
-// where a CTA's results of a segment that goes on in another CTA lie: the first, of one that began in an earlier CTA, and the last
-struct A4Desc { int rows, r0, f0, kvh, last; };      // rows of the tile (0: no such result), first row of the sequence, first (row, head) of the tile, the CTA where the segment ends
-template <int PART> __device__ __forceinline__ A4Desc* a4_desc(const Attention4Args& a, int ctas) { return reinterpret_cast<A4Desc*>(a.work + (size_t)ctas * 2 * PART); }
 
 // results of the same row over different keys, added up
 struct A4Sum {
@@ -582,6 +563,16 @@ constexpr int a4_smem() {
     constexpr int ring = A4_STAGES * 2 * A4_BLOCKS * q4_block(D), part = a4_part<D>(8 * NT) * 4;
     return A4_WARPS * ((ring > part ? ring : part) + part);
 }
+template <int D, int MT>
+cudaError_t a4_join(const Attention4Args& a, int ctas, cudaStream_t s) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, MT); cfg.blockDim = dim3(128); cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, attention_4bit_join_kernel<D, MT>, a, ctas);
+}
 template <int D, int NT>
 cudaError_t a4_step(Attention4Args a, cudaStream_t s) {
     constexpr int MT = 8 * NT, smem = a4_smem<D, NT>();
@@ -592,28 +583,41 @@ cudaError_t a4_step(Attention4Args a, cudaStream_t s) {
     a.per_page = blocks == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / blocks);
     cudaError_t e = launch_chain(attention_4bit_step_kernel<D, NT>, dim3(ctas), dim3(A4_THREADS), smem, s, a);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, MT); cfg.blockDim = dim3(128); cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_4bit_join_kernel<D, MT>, a, ctas);
+    return attention_4bit_join(a, ctas, MT, s);
 }
 }  // namespace
 
+cudaError_t attention_4bit_join(const Attention4Args& a, int ctas, int rows, cudaStream_t s) {
+    if (a.head_dim == 64) return rows == 8 ? a4_join<64, 8>(a, ctas, s) : rows == 16 ? a4_join<64, 16>(a, ctas, s) : a4_join<64, 256>(a, ctas, s);
+    return rows == 8 ? a4_join<128, 8>(a, ctas, s) : rows == 16 ? a4_join<128, 16>(a, ctas, s) : a4_join<128, 256>(a, ctas, s);
+}
+
+namespace {
+// Up to so many rows a KV head of a sequence this file's tiles of 16 rows, more on tensor memory
+constexpr long A4_TC_ROWS = 64;
+bool a4_many(long rows, int n_head, int n_kv) { return rows * (n_head / n_kv) > A4_TC_ROWS; }
+}  // namespace
+
 size_t attention_4bit_work_bytes(long n_rows, int n_head, int n_kv, int head_dim) {
-    const long rows = std::min<long>(16, n_rows * (n_head / n_kv) <= 8 ? 8 : 16);
-    return (size_t)A4_MOST_CTAS * 2 * (rows * (head_dim + 2) * 4 + sizeof(A4Desc));
+    const long rows = n_rows * (n_head / n_kv) <= 8 ? 8 : 16;
+    const size_t step = (size_t)A4_MOST_CTAS * 2 * (rows * (head_dim + 2) * 4 + sizeof(A4Desc));
+    return a4_many(n_rows, n_head, n_kv) ? std::max(step, attention_4bit_tc_work_bytes(head_dim)) : step;      // (all rows may be one sequence's)
 }
 
 cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s) {
     if (a.r.n_rows == 0 || a.r.n_seqs == 0) return cudaSuccess;
+    if (a4_many(a.max_rows, a.n_head, a.n_kv)) return attention_4bit_tc_launch(a, s);
     const bool few = (long)a.max_rows * (a.n_head / a.n_kv) <= 8;
     if (a.head_dim == 64) return few ? a4_step<64, 1>(a, s) : a4_step<64, 2>(a, s);
     return few ? a4_step<128, 1>(a, s) : a4_step<128, 2>(a, s);
 }
 
-cudaError_t attention_4bit_error(unsigned int* code) { return take_error_word(a4_error, code); }
+cudaError_t attention_4bit_error(unsigned int* code) {
+    unsigned int more = 0;
+    cudaError_t e = take_error_word(a4_error, code);
+    if (e == cudaSuccess) e = attention_4bit_tc_error(&more);
+    if (e == cudaSuccess && *code == 0) *code = more;
+    return e;
+}
 
 }  // namespace b2

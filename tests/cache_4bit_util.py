@@ -158,12 +158,13 @@ def attention_exact(c, q, rows, scale=None, max_rows=None, k=None, v=None):
     return out, spread, offset, reach, all_v
 
 
-def attention_bar(typ, out, spread, offset, reach, all_v, dim):
-    """One rounding of the output. Probabilities and values, or their scales, are rounded to f16, twice at most. A score is a sum of dim products and of one offset a group, none
+def attention_bar(typ, out, spread, offset, reach, all_v, dim, many=False):
+    """One rounding of the output. Probabilities and values, or their scales, are rounded to f16, twice at most; with
+    many rows of a sequence a KV head (`many`) probabilities are rounded to the queries' type and values are not. A score is a sum of dim products and of one offset a group, none
     larger together than |q| 8 |scale|, in 32 bits that a matrix instruction may cut off instead of rounding: within 2 (dim + 16) 2^-24 of it; weights change by that much relative,
     in numerator and denominator. 2^-18 for the exponential's 2^-22 and for joins. The smallest f16 numbers are 2^-24 apart: a weight, relative to one that is at least 1, may be off by half of
     that, and so may one times its value's scale where the largest scale is held to 64 or more: 8 / 64 of it an entry.
     Codes are multiplied without their offset of 8, which is taken off the sum: per 16 keys two instructions of 17 addends that may each be cut off at 2^-23 of the largest, at most 15 / 8 of
     a weight times 8 |scale|: within 2^-17 of the weighted sum of 8 |scale|."""
     u16 = unit("f16")
-    return unit(typ) * out.abs() + (2 * u16 + 4 * (dim + 16) * 2 ** -24 * reach[..., None] + 2 ** -18) * spread + 2 ** -17 * offset + 2 ** -25 * all_v + 2 ** -24
+    return unit(typ) * out.abs() + ((unit(typ) + 2 ** -14 if many else 2 * u16) + 4 * (dim + 16) * 2 ** -24 * reach[..., None] + 2 ** -18) * spread + 2 ** -17 * offset + 2 ** -25 * all_v + 2 ** -24

@@ -238,6 +238,6 @@ def test_attention(ops, heads, kv, dim, page, typ, rows, own):
     got = attend(ops, c, q, rows)
     want, *sizes = attention_exact(c, q, rows)
     err = (got.to(F64) - want).abs()
-    assert (err <= attention_bar(typ, want, *sizes, dim)).all(), float(err.max())
+    assert (err <= attention_bar(typ, want, *sizes, dim, max(rows) * heads // kv > 64)).all(), float(err.max())
     assert torch.equal(got, attend(ops, c, q, rows))                    # the same bits again
     assert ops.error(0) == 0
