@@ -3,12 +3,13 @@
 // Rows are (token, head of the KV head's group), numbered within their sequence; a unit is 256 of them with a KV head, two tiles of 128 rows. The blocks of 128 keys of all units laid
 // end to end are cut into equal runs, one a CTA; a run that begins or ends inside a unit leaves partial results in 32 bits, which a small kernel joins. A tile's last row says how many
 // blocks its unit has, so that a prompt's later keys cost its first rows nothing.
-// Warps 0-3 and 4-7: softmax of a tile, a thread a row, as in shared_prefix_tc.cu. 8-11: codes into operands. 12: copies of the cache's bytes. 13: matrix instructions. Tensor memory: two
+// Warps 0-3 and 4-7: softmax of a tile, a thread a row, as in shared_prefix_tc.cu. 8-15: codes into operands. 16: copies of the cache's bytes. 17: matrix instructions. Tensor memory: two
 // score tiles (probabilities are written over them) and two outputs.
 //
 // A value s (c - 8) has up to 14 bits, an f16 or bf16 operand 11 or 8. Rounded, keys would be off by 2^-12 each, and a score by more than all else together (relative error of the output
 // 3.5e-4 from the keys alone, 1.8e-4 from the values, where the output's own rounding to f16 is 2.1e-4). So keys and values are two operands each, exact to 2^-14 or better: with the upper
-// bits of the scale, and with the rest of it. That doubles the products. Probabilities are rounded to the queries' type.
+// bits of the scale, and with the rest of it. That doubles the products, which then are what this is bound by: 2048 rows behind 6000 tokens, 32 heads over 8 of 128, 389 us, 605 TFLOP/s of
+// what is asked for and twice as much of what is done. Probabilities are rounded to the queries' type.
 #include "attention_4bit.cuh"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"
@@ -23,7 +24,7 @@ namespace b2 {
 
 namespace {
 constexpr int T4_ROWS = 128, T4_K = 128, T4_PART = 128 * 128;    // rows of a tile, keys of a block; bytes of a part (128 rows x 64 columns)
-constexpr int T4_THREADS = 512, T4_RAW = 3;                      // copies under way: keys or values of a block
+constexpr int T4_THREADS = 640, T4_RAW = 3;                      // copies under way: keys or values of a block
 constexpr int T4_SMS = 148;
 constexpr int t4_stages(int d) { return d == 64 ? 2 : 1; }       // blocks of operands
 
@@ -37,8 +38,23 @@ __device__ __forceinline__ uint32_t t4_pack(float a, float b) {
 }
 template <int N> __device__ __forceinline__ void t4_more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void t4_fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// (512 threads begin with 128: 2 x 168, 104 and 64 a warp of the four groups are no more)
-constexpr int T4_REG_SOFTMAX = 168, T4_REG_OPERANDS = 104, T4_REG_OTHERS = 64;
+// (groups of four warps: two of the first, two of the second, one of the third. They begin with 96 each.)
+constexpr int T4_REG_SOFTMAX = 144, T4_REG_OPERANDS = 64, T4_REG_OTHERS = 56;
+static_assert(2 * T4_REG_SOFTMAX + 2 * T4_REG_OPERANDS + T4_REG_OTHERS <= 5 * 96, "registers of a block");
+
+// Four steps of K, each with two operands B whose products are added up: the queries are read once for both (the second takes them from where the first has left them). Shared memory
+// is read at 96 bytes a cycle then instead of 128, all that it has, and the warps that make operands write there too.
+template <int SA, int SB>
+__device__ __forceinline__ void t4_mma8_one(uint32_t d, uint64_t a, uint64_t b, uint64_t c, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q, e;\n\t.reg .b64 a1, b1, c1, a2, b2, c2, a3, b3, c3;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 q, 0, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+                 "add.s64 a1, %1, %6;\n\tadd.s64 b1, %2, %7;\n\tadd.s64 c1, %3, %7;\n\tadd.s64 a2, a1, %6;\n\tadd.s64 b2, b1, %7;\n\tadd.s64 c2, c1, %7;\n\t"
+                 "add.s64 a3, a2, %6;\n\tadd.s64 b3, b2, %7;\n\tadd.s64 c3, c2, %7;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16.collector::a::fill [%0], %1, %2, %4, p;\n\t@e tcgen05.mma.cta_group::1.kind::f16.collector::a::lastuse [%0], %1, %3, %4, q;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16.collector::a::fill [%0], a1, b1, %4, q;\n\t@e tcgen05.mma.cta_group::1.kind::f16.collector::a::lastuse [%0], a1, c1, %4, q;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16.collector::a::fill [%0], a2, b2, %4, q;\n\t@e tcgen05.mma.cta_group::1.kind::f16.collector::a::lastuse [%0], a2, c2, %4, q;\n\t"
+                 "@e tcgen05.mma.cta_group::1.kind::f16.collector::a::fill [%0], a3, b3, %4, q;\n\t@e tcgen05.mma.cta_group::1.kind::f16.collector::a::lastuse [%0], a3, c3, %4, q;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "l"(c), "r"(idesc), "r"(accumulate), "n"(SA), "n"(SB) : "memory");
+}
 
 struct T4Seq {
     int r0, n, own, lim0, tiles;     // first row, rows that are computed, tokens, keys of the first row, units a KV head
@@ -82,46 +98,61 @@ struct T4Walk {
     }
 };
 
-// four bytes of a and b; an index with bit 3 set: eight times that byte's sign
-__device__ __forceinline__ uint32_t t4_bytes(uint32_t a, uint32_t b, uint32_t which) {
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(which));
-    return r;
-}
-// Eight codes of a word (the first lowest) times a scale in two parts: 16 bytes each of the operands with its upper bits and with the rest
+// A group's scale in two parts of the operands' type, each twice: the upper ones of its bits (f16: 7, bf16: 5), so that a code times them is exact, and the others
 template <bool F16>
-__device__ __forceinline__ void t4_operands(uint32_t word, uint32_t s_hi, uint32_t s_lo, uint4& hi, uint4& lo) {
-    const uint32_t even = word & 0x0f0f0f0fu, odd = word >> 4 & 0x0f0f0f0fu;
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        // code 2 i and code 2 i + 1 as 16-bit numbers (the bytes between them: signs of bytes below 16), then as 1024 + c or 128 + c, then less 8
-        const uint32_t two = t4_bytes(even, odd, i | (8 | i) << 4 | (4 | i) << 8 | (12 | i) << 12) | (F16 ? 0x64006400u : 0x43004300u);
+struct T4Scale {
+    uint32_t hi, lo;
+    __device__ __forceinline__ explicit T4Scale(uint32_t bits) {
         if constexpr (F16) {
-            const uint32_t off = 0x64086408u;
-            const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&two), *reinterpret_cast<const __half2*>(&off));
-            const __half2 x = __hmul2(c, *reinterpret_cast<const __half2*>(&s_hi)), y = __hmul2(c, *reinterpret_cast<const __half2*>(&s_lo));
-            h[i] = *reinterpret_cast<const uint32_t*>(&x); l[i] = *reinterpret_cast<const uint32_t*>(&y);
+            const uint32_t two = bits | bits << 16;
+            hi = two & 0xfff0fff0u;
+            const __half2 rest = __hsub2(*reinterpret_cast<const __half2*>(&two), *reinterpret_cast<const __half2*>(&hi));
+            lo = *reinterpret_cast<const uint32_t*>(&rest);
         } else {
-            const uint32_t off = 0x43084308u;
-            const __nv_bfloat162 c = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&two), *reinterpret_cast<const __nv_bfloat162*>(&off));
-            const __nv_bfloat162 x = __hmul2(c, *reinterpret_cast<const __nv_bfloat162*>(&s_hi)), y = __hmul2(c, *reinterpret_cast<const __nv_bfloat162*>(&s_lo));
-            h[i] = *reinterpret_cast<const uint32_t*>(&x); l[i] = *reinterpret_cast<const uint32_t*>(&y);
+            const float s = __half2float(__ushort_as_half((uint16_t)bits)), up = __uint_as_float(__float_as_uint(s) & 0xfff80000u);
+            hi = __byte_perm(__float_as_uint(up), 0, 0x3232);
+            lo = t4_pack<false>(s - up, s - up);
         }
     }
-    hi = make_uint4(h[0], h[1], h[2], h[3]); lo = make_uint4(l[0], l[1], l[2], l[3]);
+};
+__device__ __forceinline__ uint32_t t4_fma(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
-// a scale (f16) as two of the operands' type, each twice: 8 (5) significant bits, so that a code times it is exact, and the others
-template <bool F16>
-__device__ __forceinline__ void t4_scale(uint16_t bits, uint32_t& hi, uint32_t& lo) {
-    if constexpr (F16) {
-        const uint16_t up = bits & 0xfff8u;
-        const uint16_t rest = __half_as_ushort(__hsub(__ushort_as_half(bits), __ushort_as_half(up)));
-        hi = up | (uint32_t)up << 16; lo = rest | (uint32_t)rest << 16;
-    } else {
-        const float s = __half2float(__ushort_as_half(bits)), up = __uint_as_float(__float_as_uint(s) & 0xfff80000u);
-        hi = __byte_perm(__float_as_uint(up), 0, 0x3232);
-        lo = t4_pack<false>(s - up, s - up);
+template <bool F16> __device__ __forceinline__ uint32_t t4_mul(uint32_t a, uint32_t b) {
+    uint32_t r;
+    if constexpr (F16) { const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b)); r = *reinterpret_cast<const uint32_t*>(&v); }
+    else { const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b)); r = *reinterpret_cast<const uint32_t*>(&v); }
+    return r;
+}
+// The codes of N words (the first lowest) less 8 and times a scale in two parts: 16 bytes of either operand each, codes in the order 0, 4, 1, 5, 2, 6, 3, 7, which a mask leaves them in
+// (queries are put into the same order, outputs taken out of it). f16: 64 + c is a code shifted into the number 64; that times a part of the scale less 72 times it is exact, up to
+// the scales whose 72-fold is past f16's range. bf16: 128 + c, less 136, times the parts.
+template <bool F16, int N>
+__device__ __forceinline__ void t4_operands(const uint32_t (&words)[N], uint32_t scale, uint4 (&hi)[N], uint4 (&lo)[N]) {
+    const T4Scale<F16> s(scale);
+    if (F16 && !__any_sync(0xffffffffu, (scale & 0x7fffu) >= 0x6000u)) {
+        const uint32_t off_hi = t4_mul<F16>(s.hi, 0xd480d480u), off_lo = t4_mul<F16>(s.lo, 0xd480d480u);      // -72
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const uint32_t w = words[n], c0 = (w << 4 & 0x00f000f0u) | 0x54005400u, c1 = (w & 0x00f000f0u) | 0x54005400u, c2 = (w >> 4 & 0x00f000f0u) | 0x54005400u,
+                           c3 = (w >> 8 & 0x00f000f0u) | 0x54005400u;
+            hi[n] = make_uint4(t4_fma(c0, s.hi, off_hi), t4_fma(c1, s.hi, off_hi), t4_fma(c2, s.hi, off_hi), t4_fma(c3, s.hi, off_hi));
+            lo[n] = make_uint4(t4_fma(c0, s.lo, off_lo), t4_fma(c1, s.lo, off_lo), t4_fma(c2, s.lo, off_lo), t4_fma(c3, s.lo, off_lo));
+        }
+        return;
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        uint32_t c[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t x = (words[n] >> (4 * i) & 0x000f000fu) | (F16 ? 0x64006400u : 0x43004300u), off = F16 ? 0x64086408u : 0x43084308u;
+            if constexpr (F16) { const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&off)); c[i] = *reinterpret_cast<const uint32_t*>(&v); }
+            else { const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&off)); c[i] = *reinterpret_cast<const uint32_t*>(&v); }
+        }
+        hi[n] = make_uint4(t4_mul<F16>(c[0], s.hi), t4_mul<F16>(c[1], s.hi), t4_mul<F16>(c[2], s.hi), t4_mul<F16>(c[3], s.hi));
+        lo[n] = make_uint4(t4_mul<F16>(c[0], s.lo), t4_mul<F16>(c[1], s.lo), t4_mul<F16>(c[2], s.lo), t4_mul<F16>(c[3], s.lo));
     }
 }
 }  // namespace
@@ -131,7 +162,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
     constexpr int PARTS = D / 64, NG = D / Q4_GROUP, BLOCK = q4_block(D), RAW = T4_K / Q4_TOKENS * BLOCK, ST = t4_stages(D), OPERAND = 2 * PARTS * T4_PART;      // (both halves of K or V)
     constexpr int PART = 2 * T4_ROWS * (D + 2);                  // floats of a partial result
     extern __shared__ uint8_t t4_smem[];
-    __shared__ uint64_t raw_full[T4_RAW], raw_empty[T4_RAW], q_full[2], k_full[ST], k_empty[ST], v_full[ST][2], v_empty[ST][2], s_full[2], p_half[2], p_full[2], pv_done[2], seg_done[2];
+    __shared__ uint64_t raw_full[T4_RAW], raw_empty[T4_RAW], q_full[2], k_full[ST][PARTS], k_empty[ST][PARTS], v_full[ST][2], v_empty[ST][2], s_full[2], p_half[2], p_full[2], pv_done[2], seg_done[2];
     __shared__ uint32_t tmem_at;
     __shared__ int first_bad[2][NG];                             // first key of the segment whose value's group is no number
     __shared__ T4Walk start;
@@ -144,15 +175,15 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
     const int G = a.n_head / a.n_kv;
     griddep_wait();
     griddep_launch();
-    if (warp == 13) {
+    if (warp == 17) {
         if (lane == 0) {
-            for (int i = 0; i < T4_RAW; i++) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 4); }
+            for (int i = 0; i < T4_RAW; i++) { mbar_init(&raw_full[i], 1); mbar_init(&raw_empty[i], 8); }
             for (int i = 0; i < 2; i++) {
                 mbar_init(&q_full[i], 128); mbar_init(&s_full[i], 1); mbar_init(&p_half[i], 128); mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1); mbar_init(&seg_done[i], 8);
             }
             for (int i = 0; i < ST; i++) {
-                mbar_init(&k_full[i], 4); mbar_init(&k_empty[i], 1);
-                for (int h = 0; h < 2; h++) { mbar_init(&v_full[i][h], 2); mbar_init(&v_empty[i][h], 1); }
+                for (int c = 0; c < PARTS; c++) { mbar_init(&k_full[i][c], 8); mbar_init(&k_empty[i][c], 1); }
+                for (int h = 0; h < 2; h++) { mbar_init(&v_full[i][h], 8); mbar_init(&v_empty[i][h], 1); }
             }
             fence_mbar_init();
         }
@@ -218,9 +249,9 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
     const uint32_t s_at = __shfl_sync(0xffffffffu, tmem_at, 0), o_at = s_at + 256;
     T4Walk walk = start;
 
-    if (warp >= 12) {
+    if (warp >= 16) {
         t4_fewer_registers<T4_REG_OTHERS>();
-        if (warp == 12) {
+        if (warp == 16) {
             // ================= copies: lane j has the block's 16-token block j, keys, then values
             const int blocks = a.r.block_tokens / Q4_TOKENS;
             int it = 0;
@@ -245,7 +276,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                     }
                 }
             }
-        } else if (warp == 13) {
+        } else if (warp == 17) {
             // ================= matrix instructions (all lanes run the loop, one issues)
             const uint32_t f16 = F16 ? ~((1u << 7) | (1u << 10)) : ~0u;      // (tc_idesc_bf16 without the bits that say bf16)
             const uint32_t id_s = tc_idesc_bf16(T4_ROWS, T4_K) & f16, id_o = tc_idesc_bf16(T4_ROWS, D, true) & f16;
@@ -253,24 +284,25 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             int it = 0, segs[2] = {0, 0}, done[2] = {0, 0};      // blocks of the CTA, segments and blocks of each tile so far
             for (; walk.next(a, G); walk.done(a)) {
                 const int n = walk.n, tiles = (long)walk.s.n * G - walk.seg_f0 > T4_ROWS ? 2 : 1;
-                auto scores = [&](int t, int at) {
-                    const uint64_t dq = dq0 + t * (PARTS * T4_PART >> 4), dk = dk0 + at % ST * (OPERAND >> 4);
+                // (`first`: nobody has waited for these keys yet; `last`: nobody needs them any more)
+                auto scores = [&](int t, int at, bool first, bool last) {
+                    const int st = at % ST;
+                    const uint64_t dq = dq0 + t * (PARTS * T4_PART >> 4), dk = dk0 + st * (OPERAND >> 4);
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
-#pragma unroll
-                        for (int c = 0; c < PARTS; c++)
-                            tc_mma4_one<2, 2>(s_at + t * T4_K, dq + c * (T4_PART >> 4), dk + (h * PARTS + c) * (T4_PART >> 4), id_s, h | c ? 1u : 0u);
+                    for (int c = 0; c < PARTS; c++) {
+                        if (first) { mbar_wait_warp(&k_full[st][c], (at / ST) & 1, t4_error, 0xc0002u, (unsigned)at); tc_after_sync(); }
+                        t4_mma8_one<2, 2>(s_at + t * T4_K, dq + c * (T4_PART >> 4), dk + c * (T4_PART >> 4), dk + (PARTS + c) * (T4_PART >> 4), id_s, c ? 1u : 0u);
+                        if (last) tc_commit_one(&k_empty[st][c]);
+                    }
                     tc_commit_one(&s_full[t]);
                 };
-                mbar_wait_warp(&k_full[it % ST], (it / ST) & 1, t4_error, 0xc0002u, (unsigned)it);
 #pragma unroll
                 for (int t = 0; t < 2; t++) {                    // (unrolled: which tile it is costs no instructions)
                     if (t == tiles) break;
                     mbar_wait_warp(&q_full[t], segs[t]++ & 1, t4_error, 0xc0003u, (unsigned)it);
                     tc_after_sync();
-                    scores(t, it);
+                    scores(t, it, t == 0, t == tiles - 1);
                 }
-                tc_commit_one(&k_empty[it % ST]);
                 for (int i = 0; i < n; i++) {
                     const int at = it + i, st = at % ST;
                     const uint32_t turn = (at / ST) & 1;
@@ -298,10 +330,8 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                         if (i + 1 < n) {
                             // the next scores replace the probabilities that this product reads
                             mbar_wait_warp(&pv_done[t], (done[t] - 1) & 1, t4_error, 0xc0009u, (unsigned)at);
-                            if (t == 0) mbar_wait_warp(&k_full[(at + 1) % ST], ((at + 1) / ST) & 1, t4_error, 0xc0002u, (unsigned)at);
                             tc_after_sync();
-                            scores(t, at + 1);
-                            if (t == tiles - 1) tc_commit_one(&k_empty[(at + 1) % ST]);
+                            scores(t, at + 1, t == 0, t == tiles - 1);
                         }
                     }
                 }
@@ -309,115 +339,74 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             }
         }
     } else if (warp >= 8) {
-        // ================= codes into operands: a warp has 32 keys of a block, two blocks of 16 tokens
+        // ================= codes into operands: keys 64 dims at a time, values 64 keys at a time, by all eight warps. What a warp is to write is ready before its place is free.
+        // (The tensor cores take 70 % of the time, and reading operands beside the warps that write them makes their products a fifth longer. Neither warps of their own for keys and values nor
+        // the second tile's product ahead of the first one's next scores where it is ready first made it faster: 395 us instead of 389 for 2048 rows behind 6000.)
         t4_fewer_registers<T4_REG_OPERANDS>();
-        const int dw = warp - 8;
+        const int dw = warp & 7, eight = lane & 7;               // (eight neighbouring lanes: keys that follow one another; a lane has the 32 dims of a group)
+        auto put = [&](uint8_t* row, int key, int g, const uint4 (&hi)[4], const uint4 (&lo)[4]) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                uint8_t* at = row + (((w + 4 * (g & 1)) ^ (key & 7)) << 4);
+                *reinterpret_cast<uint4*>(at) = hi[w];
+                *reinterpret_cast<uint4*>(at + PARTS * T4_PART) = lo[w];
+            }
+        };
+        const int k_token = (lane >> 4) * 8 + eight, k_g = lane >> 3 & 1;                                       // of block dw
+        const int v_key = NG == 4 ? dw * 8 + eight : dw * 16 + k_token, v_g = NG == 4 ? lane >> 3 : k_g;       // of 64 keys (heads of 64: four warps' work)
+        const int v_token = v_key % Q4_TOKENS, v_pair = v_token >> 1;
         int it = 0, seg = 0;
         for (; walk.next(a, G); walk.done(a), seg++) {
             if (seg >= 2) mbar_wait_warp(&seg_done[seg & 1], ((seg >> 1) - 1) & 1, t4_error, 0xc000bu, (unsigned)seg);
             if (dw == 0 && lane < NG) first_bad[seg & 1][lane] = INT_MAX;
-            named_bar_sync(1, 128);
+            named_bar_sync(1, 256);
             for (int i = 0; i < walk.n; i++, it++) {
                 const int j0 = (walk.b0 + i) * T4_K, st = it % ST;
-                // ---- keys
+                uint32_t words[4];
+                uint4 hi[4], lo[4];
                 int r = 2 * it;
                 mbar_wait_warp(&raw_full[r % T4_RAW], (r / T4_RAW) & 1, t4_error, 0xc000cu, (unsigned)it);
-                if (it >= ST) mbar_wait_warp(&k_empty[st], (it / ST - 1) & 1, t4_error, 0xc000du, (unsigned)it);
-                {
-                    const uint8_t* from = raw + r % T4_RAW * RAW;
-                    uint8_t* to = ks + st * OPERAND;
-                    // eight tokens with the same words in neighbouring lanes
-                    const int w = lane >> 3;
+                const uint8_t* p = raw + r % T4_RAW * RAW + dw * BLOCK;
+#pragma unroll 1
+                for (int c = 0; c < PARTS; c++) {
 #pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const int token = (b & 1) * 8 + (lane & 7), block = dw * 2 + (b >> 1), key = block * Q4_TOKENS + token;
-                        const uint8_t* p = from + block * BLOCK;
-                        uint32_t words[NG];
-                        uint16_t scales[NG];
-                        if constexpr (NG == 4) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(p + token * (D / 2) + q4_key_chunk(D, token, w) * 16);
-                            const uint2 s = *reinterpret_cast<const uint2*>(p + q4_scale(D, token, 0));
-                            words[0] = v.x; words[1] = v.y; words[2] = v.z; words[3] = v.w;
-                            scales[0] = (uint16_t)s.x; scales[1] = (uint16_t)(s.x >> 16); scales[2] = (uint16_t)s.y; scales[3] = (uint16_t)(s.y >> 16);
-                        } else {
-                            const uint2 v = *reinterpret_cast<const uint2*>(p + token * (D / 2) + q4_key_chunk(D, token, w) * 8);
-                            const uint32_t s = *reinterpret_cast<const uint32_t*>(p + q4_scale(D, token, 0));
-                            words[0] = v.x; words[1] = v.y;
-                            scales[0] = (uint16_t)s; scales[1] = (uint16_t)(s >> 16);
-                        }
-#pragma unroll
-                        for (int g = 0; g < NG; g++) {
-                            uint32_t s_hi, s_lo;
-                            uint4 hi, lo;
-                            t4_scale<F16>(scales[g], s_hi, s_lo);
-                            t4_operands<F16>(words[g], s_hi, s_lo, hi, lo);
-                            const int c8 = w + 4 * g;
-                            uint8_t* at = to + (c8 >> 3) * T4_PART + key * 128 + (((c8 ^ key) & 7) << 4);
-                            *reinterpret_cast<uint4*>(at) = hi;
-                            *reinterpret_cast<uint4*>(at + PARTS * T4_PART) = lo;
-                        }
-                    }
+                    for (int w = 0; w < 4; w++) words[w] = *reinterpret_cast<const uint32_t*>(p + k_token * (D / 2) + (q4_key_chunk(D, k_token, w) * NG + 2 * c + k_g) * 4);
+                    t4_operands<F16>(words, *reinterpret_cast<const uint16_t*>(p + q4_scale(D, k_token, 2 * c + k_g)), hi, lo);
+                    if (it >= ST) mbar_wait_warp(&k_empty[st][c], (it / ST - 1) & 1, t4_error, 0xc000du, (unsigned)it);
+                    put(ks + st * OPERAND + c * T4_PART + (dw * Q4_TOKENS + k_token) * 128, k_token, k_g, hi, lo);
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&k_full[st][c]);
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) { mbar_arrive(&raw_empty[r % T4_RAW]); mbar_arrive(&k_full[st]); }
-                // ---- values: a lane has a pair of tokens
+                if (lane == 0) mbar_arrive(&raw_empty[r % T4_RAW]);
                 r++;
                 mbar_wait_warp(&raw_full[r % T4_RAW], (r / T4_RAW) & 1, t4_error, 0xc000cu, (unsigned)it);
-                if (it >= ST) mbar_wait_warp(&v_empty[st][dw >> 1], (it / ST - 1) & 1, t4_error, 0xc000eu, (unsigned)it);
-                {
-                    const uint8_t* from = raw + r % T4_RAW * RAW;
-                    uint8_t* to = vs + st * OPERAND;
-                    const int pair = lane & 7, w = lane >> 3;
+#pragma unroll 1
+                for (int half = 0; half < 2; half++) {
+                    if (NG == 4 || dw < 4) {
+                        const uint8_t* p = raw + r % T4_RAW * RAW + (half * 4 + v_key / Q4_TOKENS) * BLOCK;
+                        const int k = half * 64 + v_key;
+                        uint32_t scale = *reinterpret_cast<const uint16_t*>(p + q4_scale(D, v_token, v_g));
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        const int block = dw * 2 + b, key = block * Q4_TOKENS + 2 * pair;
-                        const uint8_t* p = from + block * BLOCK;
-                        uint32_t x[2][NG], sc[NG];               // entries 8 w .. + 3 and + 4 .. + 7 of both tokens; their scales
-                        if constexpr (NG == 4) {
-#pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                const uint4 v = *reinterpret_cast<const uint4*>(p + pair * D + q4_value_chunk(D, pair, 2 * w + e) * 16);
-                                x[e][0] = v.x; x[e][1] = v.y; x[e][2] = v.z; x[e][3] = v.w;
-                            }
-                            const uint4 s = *reinterpret_cast<const uint4*>(p + q4_scale(D, 2 * pair, 0));
-                            sc[0] = s.x; sc[1] = s.y; sc[2] = s.z; sc[3] = s.w;
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                const uint2 v = *reinterpret_cast<const uint2*>(p + pair * D + q4_value_chunk(D, pair, 2 * w + e) * 8);
-                                x[e][0] = v.x; x[e][1] = v.y;
-                            }
-                            const uint2 s = *reinterpret_cast<const uint2*>(p + q4_scale(D, 2 * pair, 0));
-                            sc[0] = s.x; sc[1] = s.y;
+                        for (int w = 0; w < 4; w++)
+                            words[w] = __byte_perm(*reinterpret_cast<const uint32_t*>(p + v_pair * D + (q4_value_chunk(D, v_pair, 2 * w) * NG + v_g) * 4),
+                                                   *reinterpret_cast<const uint32_t*>(p + v_pair * D + (q4_value_chunk(D, v_pair, 2 * w + 1) * NG + v_g) * 4), v_token & 1 ? 0x7632u : 0x5410u);
+                        // keys that nobody has: zeros. A value that is no number must not meet the zero weights of rows that do not see it: it is written down instead.
+                        if (j0 + k >= walk.s.own) scale = 0;
+                        if ((scale & 0x7c00u) == 0x7c00u) {
+                            atomicMin(&first_bad[seg & 1][v_g], j0 + k);
+                            scale = 0;
                         }
-#pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            const bool there = j0 + key + t < walk.s.own;
-#pragma unroll
-                            for (int g = 0; g < NG; g++) {
-                                uint16_t scale = (uint16_t)(sc[(t * NG + g) >> 1] >> 16 * (g & 1));
-                                // keys that nobody has: zeros. A value that is no number must not meet the zero weights of rows that do not see it: it is written down instead.
-                                if (!there) scale = 0;
-                                if ((scale & 0x7c00u) == 0x7c00u) {
-                                    if (w == 0) atomicMin(&first_bad[seg & 1][g], j0 + key + t);
-                                    scale = 0;
-                                }
-                                uint32_t s_hi, s_lo;
-                                uint4 hi, lo;
-                                t4_scale<F16>(scale, s_hi, s_lo);
-                                t4_operands<F16>(__byte_perm(x[0][g], x[1][g], t ? 0x7632 : 0x5410), s_hi, s_lo, hi, lo);
-                                const int c8 = w + 4 * g, k = key + t;
-                                uint8_t* at = to + (c8 >> 3) * T4_PART + k * 128 + (((c8 ^ k) & 7) << 4);
-                                *reinterpret_cast<uint4*>(at) = hi;
-                                *reinterpret_cast<uint4*>(at + PARTS * T4_PART) = lo;
-                            }
-                        }
+                        __syncwarp();
+                        t4_operands<F16>(words, scale, hi, lo);
+                        if (it >= ST) mbar_wait_warp(&v_empty[st][half], (it / ST - 1) & 1, t4_error, 0xc000eu, (unsigned)it);
+                        put(vs + st * OPERAND + (v_g >> 1) * T4_PART + k * 128, k, v_g, hi, lo);
                     }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&v_full[st][half]);
                 }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) { mbar_arrive(&raw_empty[r % T4_RAW]); mbar_arrive(&v_full[st][dw >> 1]); }
+                if (lane == 0) mbar_arrive(&raw_empty[r % T4_RAW]);
             }
         }
     } else {
@@ -460,7 +449,9 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
 #pragma unroll
                 for (int b = 0; b < BATCH; b++) {
                     const int c8 = lane % LANES, row = (warp & 3) * 32 + i0 + b * ROWS + lane / LANES;
-                    *reinterpret_cast<uint4*>(qs + (t * PARTS + (c8 >> 3)) * T4_PART + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) = v[b];
+                    // (in the order of the keys' codes: 0, 4, 1, 5, ...)
+                    *reinterpret_cast<uint4*>(qs + (t * PARTS + (c8 >> 3)) * T4_PART + row * 128 + (((c8 & 7) ^ (row & 7)) << 4)) =
+                        make_uint4(__byte_perm(v[b].x, v[b].z, 0x5410), __byte_perm(v[b].x, v[b].z, 0x7632), __byte_perm(v[b].y, v[b].w, 0x5410), __byte_perm(v[b].y, v[b].w, 0x7632));
                 }
             }
             fence_proxy_async();
@@ -475,22 +466,25 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                 const int valid = lim - (walk.b0 + i) * T4_K;
                 // 32 scores at a time, the next ones on their way: the maximum, then the exponentials
                 uint32_t x[2][32];
-                auto load = [&](int c) { tc_ld32(s_mine + c * 32, x[c & 1]); };
-                auto mask = [&](int c) {
-                    if (valid < T4_K) {
+                const bool partly = __any_sync(0xffffffffu, valid < T4_K);
+                auto mask = [&](uint32_t (&v)[32], int left) {
+                    if (partly) {
 #pragma unroll
-                        for (int j = 0; j < 32; j++) if (c * 32 + j >= valid) x[c & 1][j] = 0xff800000u;
+                        for (int j = 0; j < 32; j++) if (j >= left) v[j] = 0xff800000u;
                     }
                 };
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                load(0);
+                tc_ld32(s_mine, x[0]);
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    tc_wait_ld(x[c & 1]);
-                    load((c + 1) & 3);                           // (the last of these: the first scores again)
-                    mask(c);
+                    for (int u = 0; u < 2; u++) {
+                        tc_wait_ld(x[u]);
+                        tc_ld32(s_mine + ((c + u + 1) & 3) * 32, x[u ^ 1]);      // (the last of these: the first scores again)
+                        mask(x[u], valid - (c + u) * 32);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) mx4[j & 3] = fmaxf(mx4[j & 3], __uint_as_float(x[c & 1][j]));
+                        for (int j = 0; j < 32; j += 2) mx4[j >> 1 & 3] = fmaxf(fmaxf(mx4[j >> 1 & 3], __uint_as_float(x[u][j])), __uint_as_float(x[u][j + 1]));
+                    }
                 }
                 const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
                 const bool grow = mx > m_ref + 8.f || (m_ref == -INFINITY && mx > -INFINITY);
@@ -516,25 +510,26 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                         tc_st16(o_mine + c, o);
                     }
                 }
+#pragma unroll 1
+                for (int c = 0; c < 4; c += 2) {
 #pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    tc_wait_ld(x[c & 1]);
-                    if (c < 3) load(c + 1);
-                    mask(c);
-                    uint32_t p[16];
+                    for (int u = 0; u < 2; u++) {
+                        tc_wait_ld(x[u]);
+                        if (c + u < 3) tc_ld32(s_mine + (c + u + 1) * 32, x[u ^ 1]);
+                        mask(x[u], valid - (c + u) * 32);
+                        uint32_t p[16];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
-                        const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(x[c & 1][j]), __uint_as_float(x[c & 1][j + 1])), scale2, ref2));
-                        const float e0 = t4_exp2(d.x), e1 = t4_exp2(d.y);
-                        if (j & 2) l3 = f2_add(l3, f2_pack(e0, e1)); else l2 = f2_add(l2, f2_pack(e0, e1));
-                        p[j >> 1] = t4_pack<F16>(e0, e1);
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(x[u][j]), __uint_as_float(x[u][j + 1])), scale2, ref2));
+                            const float e0 = t4_exp2(d.x), e1 = t4_exp2(d.y);
+                            if (j & 2) l3 = f2_add(l3, f2_pack(e0, e1)); else l2 = f2_add(l2, f2_pack(e0, e1));
+                            p[j >> 1] = t4_pack<F16>(e0, e1);
+                        }
+                        tc_st16(s_mine + (c + u) * 16, p);       // over scores that have been read
                     }
-                    tc_st16(s_mine + c * 16, p);                 // over scores that have been read
-                    if (c == 1 || c == 3) {
-                        tc_wait_st();
-                        tc_before_sync();
-                        mbar_arrive(c == 1 ? &p_half[t] : &p_full[t]);
-                    }
+                    tc_wait_st();
+                    tc_before_sync();
+                    mbar_arrive(c == 0 ? &p_half[t] : &p_full[t]);
                 }
             }
             // ---- this segment's results of the row: output, or a part of it
@@ -558,7 +553,8 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                 const bool none = lim > first_bad[seg & 1][g];   // a value that the row sees is no number
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
-                    float4 v = make_float4(__uint_as_float(o[e]) * by, __uint_as_float(o[e + 1]) * by, __uint_as_float(o[e + 2]) * by, __uint_as_float(o[e + 3]) * by);
+                    const int f = (e & ~7) + (e >> 2 & 1);       // columns are in the order of the codes
+                    float4 v = make_float4(__uint_as_float(o[f]) * by, __uint_as_float(o[f + 2]) * by, __uint_as_float(o[f + 4]) * by, __uint_as_float(o[f + 6]) * by);
                     if (l == 0.f) v = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (none) v = make_float4(NAN, NAN, NAN, NAN);
                     *reinterpret_cast<float4*>(mine + lane * 128 + (((e >> 2) ^ (lane & 7)) << 4)) = v;
@@ -588,7 +584,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
         if (warp == 0 && lane < 2 && !open[lane]) desc[lane].rows = 0;      // (whatever the workspace held)
     }
     __syncthreads();
-    if (warp == 13) tc_dealloc(tmem_at, 512);
+    if (warp == 17) tc_dealloc(tmem_at, 512);
 }
 
 // ---------------------------------------------------------------- host side
