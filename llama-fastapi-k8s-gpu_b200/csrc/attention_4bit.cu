@@ -64,34 +64,44 @@ template <int NG> __device__ __forceinline__ void a4_scales(const uint8_t* p, fl
     }
 }
 
-// what is known of a sequence: its first row, its rows (those that are computed), its tokens, and the keys that its first row sees
+// what is known of a sequence: its first row, its rows (those that are computed), its tokens, the keys that its first row sees, tiles of rows, steps
 struct A4Seq {
     int r0, n, own, lim0, tiles, steps;
     __device__ A4Seq() {}
-    __device__ A4Seq(const Attention4Args& a, int z, int mt) {
-        r0 = min(max(a.r.row_start[z], 0), a.r.n_rows);
-        const int all = max(min(max(a.r.row_start[z + 1], 0), a.r.n_rows) - r0, 0);      // (whatever the arrays hold)
+    __device__ A4Seq(const Attention4Args& a, int z, int mt) : A4Seq(a, a.r.row_start[z], a.r.row_start[z + 1], a.r.lengths[z], mt) {}
+    __device__ A4Seq(const Attention4Args& a, int b, int e, int held, int mt) {
+        r0 = min(max(b, 0), a.r.n_rows);
+        const int all = max(min(max(e, 0), a.r.n_rows) - r0, 0);                         // (whatever the arrays hold)
         n = min(all, a.max_rows);
-        own = min(max(a.r.lengths[z], 0), a.r.max_pages * a.r.block_tokens);
+        own = min(max(held, 0), a.r.max_pages * a.r.block_tokens);
         lim0 = own - all + 1;
-        tiles = (int)(((long)n * (a.n_head / a.n_kv) + mt - 1) / mt);
+        tiles = (n * (a.n_head / a.n_kv) + mt - 1) / mt;
         steps = n ? max(1, (own + A4_KEYS - 1) / A4_KEYS) : 0;
     }
-    __device__ long units(int n_kv) const { return (long)n_kv * tiles * steps; }
+    // units of work: a segment's steps, and one more for its beginning and end
+    __device__ long units(int n_kv) const { return steps ? (long)n_kv * tiles * (steps + 1) : 0; }
     __device__ int limit(int i) const { return max(0, lim0 + i); }                      // keys that row i sees
+    __device__ A4Seq from_lane(int l) const {
+        A4Seq s;
+        s.r0 = __shfl_sync(0xffffffffu, r0, l); s.n = __shfl_sync(0xffffffffu, n, l); s.own = __shfl_sync(0xffffffffu, own, l); s.lim0 = __shfl_sync(0xffffffffu, lim0, l);
+        s.tiles = __shfl_sync(0xffffffffu, tiles, l); s.steps = __shfl_sync(0xffffffffu, steps, l);
+        return s;
+    }
 };
-// a place in the steps of all segments laid end to end
+// a place in the steps of all segments laid end to end, each behind a unit for its beginning
 struct A4At {
     int z, kvh, tile, step;
     A4Seq s;
-    __device__ void next(const Attention4Args& a, int mt) {
-        if (++step < s.steps) return;
+    // to the next step; the units that this goes on by
+    __device__ int next(const Attention4Args& a, int mt) {
+        if (++step < s.steps) return 1;
         step = 0;
-        if (++tile < s.tiles) return;
+        if (++tile < s.tiles) return 2;
         tile = 0;
-        if (++kvh < a.n_kv) return;
+        if (++kvh < a.n_kv) return 2;
         kvh = 0;
-        do { if (++z >= a.r.n_seqs) return; s = A4Seq(a, z, mt); } while (s.steps == 0);
+        do { if (++z >= a.r.n_seqs) return 2; s = A4Seq(a, z, mt); } while (s.steps == 0);
+        return 2;
     }
 };
 
@@ -119,12 +129,11 @@ struct A4Sum {
     }
 };
 
-// CTAs of a call: as many as run at once, no more than there can be steps for
-constexpr int A4_PER_SM[2] = {3, 2}, A4_MOST_CTAS = A4_SMS * 3;      // (of tiles of 8 and of 16 rows)
-inline int a4_ctas(const Attention4Args& a, int mt) {
+constexpr int A4_PER_SM[2] = {3, 2}, A4_MOST_CTAS = A4_SMS * 3;      // CTAs that run at once (of tiles of 8 and of 16 rows)
+// units of work that a call can have at most
+inline double a4_most_units(const Attention4Args& a, int mt) {
     const long steps = ((long)a.r.max_pages * a.r.block_tokens + A4_KEYS - 1) / A4_KEYS;
-    const double units = (double)a.r.n_seqs * a.n_kv * (((double)a.max_rows * (a.n_head / a.n_kv) + mt - 1) / mt) * steps;
-    return (int)std::min<double>(A4_SMS * A4_PER_SM[mt > 8], std::ceil(units / A4_WARPS));
+    return (double)a.r.n_seqs * a.n_kv * (((double)a.max_rows * (a.n_head / a.n_kv) + mt - 1) / mt) * (steps + 1);
 }
 }  // namespace
 
@@ -149,42 +158,91 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
     __syncwarp();
     const int n_kv = a.n_kv, G = a.n_head / n_kv, blocks = a.r.block_tokens / Q4_TOKENS, last_page = (int)a.r.n_pages - 1;
 
-    // ---- the steps of all sequences, and this warp's run [u0, u1) of them
+    // ---- the units of all sequences, and this warp's run [u0, u1) of them. Up to 256 sequences are read at once and kept.
+    constexpr int KEPT = 8;
+    const int n_seqs = a.r.n_seqs;
+    A4Seq kept;
+    int kept_units[KEPT];
     long total = 0;
-    for (int z = lane; z < a.r.n_seqs; z += 32) total += A4Seq(a, z, MT).units(n_kv);
+    const bool keep = n_seqs <= 32 * KEPT && a.few_units;
+    if (keep) {
+        int b[KEPT], e[KEPT], h[KEPT];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        for (int i = 0; i < KEPT; i++) {
+            const int z = 32 * i + lane;
+            b[i] = e[i] = h[i] = 0;
+            if (z < n_seqs) { b[i] = a.r.row_start[z]; e[i] = a.r.row_start[z + 1]; h[i] = a.r.lengths[z]; }
+        }
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < KEPT; i++) {
+            const A4Seq s(a, b[i], e[i], h[i], MT);
+            kept_units[i] = 32 * i < n_seqs ? (int)s.units(n_kv) : 0;
+            if (i == 0) kept = s;
+            sum += kept_units[i];
+        }
+        total = __reduce_add_sync(0xffffffffu, (unsigned)sum);
+    } else {
+        for (int z = lane; z < n_seqs; z += 32) total += A4Seq(a, z, MT).units(n_kv);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    // the first `longer` runs have a unit more than the others
     const long all_warps = (long)gridDim.x * A4_WARPS, warps = min(all_warps, total), me = (long)blockIdx.x * A4_WARPS + warp;
-    // the first `longer` runs have a step more than the others
     const long run = warps ? total / warps : 0, longer = total - run * warps;
     const long u0 = me < warps ? run * me + min(me, longer) : 0, u1 = me < warps ? u0 + run + (me < longer) : 0;
     A4At at;
-    at.z = a.r.n_seqs; at.kvh = at.tile = at.step = 0;
+    at.z = n_seqs; at.kvh = at.tile = at.step = 0;
+    long first = u0;                                             // the first unit that is a step
     if (u0 < u1) {
-        long before = 0;
-        for (int z0 = 0; z0 < a.r.n_seqs; z0 += 32) {
-            const long mine = z0 + lane < a.r.n_seqs ? A4Seq(a, z0 + lane, MT).units(n_kv) : 0;
-            long sum = mine;                                     // of sequences z0 .. z0 + lane
+        long rest = 0;
+        if (keep) {
+            int before = 0;
+            bool found = false;
 #pragma unroll
-            for (int o = 1; o < 32; o *= 2) { const long v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
-            const unsigned past = __ballot_sync(0xffffffffu, before + sum > u0);
-            if (past) {
-                const int l = __ffs(past) - 1;
-                at.z = z0 + l;
-                at.s = A4Seq(a, at.z, MT);
-                long rest = u0 - before - __shfl_sync(0xffffffffu, sum - mine, l);
-                const long per = (long)at.s.tiles * at.s.steps;
-                at.kvh = (int)(rest / per); rest -= at.kvh * per;
-                at.tile = (int)(rest / at.s.steps); at.step = (int)(rest - (long)at.tile * at.s.steps);
-                break;
+            for (int i = 0; i < KEPT; i++) {
+                if (found || 32 * i >= n_seqs) continue;
+                int sum = kept_units[i];                         // of sequences 32 i .. 32 i + lane
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
+                const unsigned past = __ballot_sync(0xffffffffu, before + sum > (int)u0);
+                if (past) {
+                    const int l = __ffs(past) - 1;
+                    at.z = 32 * i + l;
+                    at.s = i == 0 ? kept.from_lane(l) : A4Seq(a, at.z, MT);
+                    rest = u0 - before - __shfl_sync(0xffffffffu, sum - kept_units[i], l);
+                    found = true;
+                }
+                before += __shfl_sync(0xffffffffu, sum, 31);
             }
-            before += __shfl_sync(0xffffffffu, sum, 31);
+        } else {
+            long before = 0;
+            for (int z0 = 0; z0 < n_seqs; z0 += 32) {
+                const long mine = z0 + lane < n_seqs ? A4Seq(a, z0 + lane, MT).units(n_kv) : 0;
+                long sum = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o *= 2) { const long v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
+                const unsigned past = __ballot_sync(0xffffffffu, before + sum > u0);
+                if (past) {
+                    const int l = __ffs(past) - 1;
+                    at.z = z0 + l;
+                    at.s = A4Seq(a, at.z, MT);
+                    rest = u0 - before - __shfl_sync(0xffffffffu, sum - mine, l);
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, sum, 31);
+            }
         }
+        const long each = at.s.steps + 1, per = at.s.tiles * each;
+        at.kvh = (int)(rest / per); rest -= at.kvh * per;
+        at.tile = (int)(rest / each); rest -= at.tile * each;
+        if (rest == 0) first++; else rest--;
+        at.step = (int)rest;
     }
 
     // ---- copies: a lane has keys or values of one of the step's blocks, the page's id read a step ahead
     A4At ahead = at;
-    int to_copy = (int)(u1 - u0), id = 0, in_page = 0, put = 0;
+    int to_copy = (int)max(u1 - first, 0l), id = 0, in_page = 0, put = 0;      // units of the run from the next copy on
     const int c_kv = lane >= KB, c_blk = lane - c_kv * KB;
     const uint8_t* const pool = (const uint8_t*)(c_kv ? a.v_pool : a.k_pool);
     auto read_id = [&]() {
@@ -192,11 +250,11 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
         unsigned page = __umulhi(b, a.per_page);                 // the quotient by the page's blocks, or one less
         in_page = (int)(b - page * blocks);
         if (in_page >= blocks) { page++; in_page -= blocks; }
-        id = lane < 2 * KB && to_copy && (int)b * Q4_TOKENS < ahead.s.own ? a.r.pages[ahead.z * a.r.table_stride + page] : 0;
+        id = lane < 2 * KB && to_copy > 0 && (int)b * Q4_TOKENS < ahead.s.own ? a.r.pages[ahead.z * a.r.table_stride + page] : 0;
     };
     read_id();
     auto copy = [&]() {
-        if (!to_copy) return;
+        if (to_copy <= 0) return;
         const int n = min(KB, (ahead.s.own - ahead.step * A4_KEYS + Q4_TOKENS - 1) / Q4_TOKENS);
         if (lane == 0) mbar_arrive_expect_tx(&full[warp][put], (uint32_t)(max(n, 0) * 2 * BLOCK));
         __syncwarp();
@@ -206,15 +264,22 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
         }
         __syncwarp();
         put = put + 1 == S ? 0 : put + 1;
-        ahead.next(a, MT);
-        to_copy--;
+        to_copy -= ahead.next(a, MT);
         read_id();
+        if (ahead.step == 0 && to_copy > 0) {                    // the next segment's queries, on their way into the L1 cache
+            const int f0 = ahead.tile * MT, row = lane >> 1;
+            if (row < min((long)MT, (long)ahead.s.n * G - f0)) {
+                const int f = f0 + row, i = f / G;
+                const uint16_t* q = (const uint16_t*)a.q + (size_t)(ahead.s.r0 + i) * a.q_row + (size_t)(ahead.kvh * G + f - i * G) * a.q_head + (lane & 1) * (D / 2);
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
+            }
+        }
     };
     for (int i = 0; i < S; i++) copy();
 
     int st = 0;
     uint32_t parity = 0;
-    for (long u = u0; u < u1;) {
+    for (long u = first; u < u1;) {
         // ================= a segment: queries, as the fragments of eight rows each; rows past the tile's are zeros
         const A4Seq& s = at.s;
         const int kvh = at.kvh, f0 = at.tile * MT, n_f = (int)min((long)MT, (long)s.n * G - f0), r0 = s.r0;
@@ -341,17 +406,23 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
             const float2 most2 = __half22float2(most);
             const float top_v = fmaxf(most2.x, most2.y);
             // ---- differences to the references, which go up where a score is far above them (as the values' power of two goes down where a scale is)
-            float up = -INFINITY;
+            bool above = top_v * up_v > 512.f;
 #pragma unroll
-            for (int b = 0; b < KB; b++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int j = 0; j < 2; j++) {
+                    float mx = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if (PARTLY && t0 + b * 16 + g + 8 * (e >> 1) >= lim[nt][e & 1]) sc[b][nt][e] = -INFINITY;
-                        up = fmaxf(up, fmaf(sc[b][nt][e], by[nt][e & 1], -ref[nt][e & 1]));
+                    for (int b = 0; b < KB; b++) {
+                        if constexpr (PARTLY) {
+#pragma unroll
+                            for (int h = 0; h < 2; h++) if (t0 + b * 16 + g + 8 * h >= lim[nt][j]) sc[b][nt][j + 2 * h] = -INFINITY;
+                        }
+                        mx = fmaxf(fmaxf(mx, sc[b][nt][j]), sc[b][nt][j + 2]);
                     }
-            if (__any_sync(0xffffffffu, up > 6.f || top_v * up_v > 512.f)) {
+                    above |= mx * by[nt][j] > ref[nt][j] + 6.f;
+                }
+            if (__any_sync(0xffffffffu, above)) {
                 float fall_v = 1.f;
                 const float all_v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
                 if (all_v * up_v > 512.f) {
@@ -365,7 +436,8 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
                     for (int j = 0; j < 2; j++) {
                         float mx = -INFINITY;
 #pragma unroll
-                        for (int b = 0; b < KB; b++) mx = fmaxf(mx, fmaxf(sc[b][nt][j] * by[nt][j], sc[b][nt][j + 2] * by[nt][j]));
+                        for (int b = 0; b < KB; b++) mx = fmaxf(fmaxf(mx, sc[b][nt][j]), sc[b][nt][j + 2]);
+                        mx *= by[nt][j];
 #pragma unroll
                         for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
                         mx = fmaxf(mx, ref[nt][j]);
@@ -464,10 +536,11 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
                 }
             }
         if (!(begins && ends) && lane == 0) {
-            const long end = u - n + left - 1, most = longer * (run + 1);        // the segment's last step
+            const long end = u - n + left - 1, most = longer * (run + 1);        // the segment's last unit
             held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, (int)((end < most ? end / (run + 1) : longer + (end - most) / run) / A4_WARPS)};
         }
         // the segment behind it (not the sequence's loads if there is none)
+        u++;                                                     // (its beginning)
         if (u < u1) {
             at.step = s.steps - 1;
             at.next(a, MT);
@@ -578,7 +651,9 @@ cudaError_t a4_step(Attention4Args a, cudaStream_t s) {
     constexpr int MT = 8 * NT, smem = a4_smem<D, NT>();
     if (!allow_smem<attention_4bit_step_kernel<D, NT>>(smem)) return cudaErrorInvalidValue;
     // as many CTAs as run at once, no more than there can be steps for
-    const int ctas = a4_ctas(a, MT);
+    const double units = a4_most_units(a, MT);
+    const int ctas = (int)std::min<double>(A4_SMS * A4_PER_SM[NT - 1], std::ceil(units / A4_WARPS));
+    a.few_units = units < 1e9;
     const unsigned blocks = a.r.block_tokens / Q4_TOKENS;
     a.per_page = blocks == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / blocks);
     cudaError_t e = launch_chain(attention_4bit_step_kernel<D, NT>, dim3(ctas), dim3(A4_THREADS), smem, s, a);

@@ -72,6 +72,7 @@ struct Attention4Args {
     int n_head, n_kv, head_dim, type;
     float scale_log2;
     unsigned per_page;           // 2^32 over the blocks of a page (set by the launch)
+    int few_units;               // units of work that tables and rows allow fit 31 bits (set by the launch)
 };
 size_t attention_4bit_work_bytes(long n_rows, int n_head, int n_kv, int head_dim);
 cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s);
