@@ -30,6 +30,7 @@ namespace {
 constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS;
 constexpr int A4_BLOCKS = 2, A4_KEYS = A4_BLOCKS * Q4_TOKENS;      // blocks and keys of a step
 constexpr int A4_STAGES = 3;         // steps under way
+constexpr int A4_BEGIN = 2;          // units that a segment's beginning and end count as, beside its steps
 constexpr int A4_SMS = 148;
 
 __device__ unsigned int a4_error[5];                             // see mbar_give_up
@@ -41,10 +42,13 @@ __device__ __forceinline__ void a4_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // the same, from other initial values
-__device__ __forceinline__ void a4_mma_from(float (&d)[4], const float (&c)[2], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]));
+__device__ __forceinline__ void a4_mma_from(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
+// a value that stays in a register of its own (fragments are neighbouring registers: made anew before every product, they cost a move each)
+__device__ __forceinline__ float a4_keep(float v) { float r; asm volatile("mov.b32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
+__device__ __forceinline__ uint32_t a4_keep(uint32_t v) { uint32_t r; asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v)); return r; }
 __device__ __forceinline__ uint32_t a4_transpose(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -78,8 +82,7 @@ struct A4Seq {
         tiles = (n * (a.n_head / a.n_kv) + mt - 1) / mt;
         steps = n ? max(1, (own + A4_KEYS - 1) / A4_KEYS) : 0;
     }
-    // units of work: a segment's steps, and one more for its beginning and end
-    __device__ long units(int n_kv) const { return steps ? (long)n_kv * tiles * (steps + 1) : 0; }
+    __device__ long units(int n_kv) const { return steps ? (long)n_kv * tiles * (steps + A4_BEGIN) : 0; }
     __device__ int limit(int i) const { return max(0, lim0 + i); }                      // keys that row i sees
     __device__ A4Seq from_lane(int l) const {
         A4Seq s;
@@ -88,20 +91,40 @@ struct A4Seq {
         return s;
     }
 };
-// a place in the steps of all segments laid end to end, each behind a unit for its beginning
+// a place in the steps of all segments laid end to end, each behind its beginning's units
 struct A4At {
     int z, kvh, tile, step;
     A4Seq s;
-    // to the next step; the units that this goes on by
-    __device__ int next(const Attention4Args& a, int mt) {
-        if (++step < s.steps) return 1;
+    // to the next segment
+    __device__ void next(const Attention4Args& a, int mt) {
         step = 0;
-        if (++tile < s.tiles) return 2;
+        if (++tile < s.tiles) return;
         tile = 0;
-        if (++kvh < a.n_kv) return 2;
+        if (++kvh < a.n_kv) return;
         kvh = 0;
-        do { if (++z >= a.r.n_seqs) return 2; s = A4Seq(a, z, mt); } while (s.steps == 0);
-        return 2;
+        do { if (++z >= a.r.n_seqs) return; s = A4Seq(a, z, mt); } while (s.steps == 0);
+    }
+};
+
+// All units cut into runs, one a warp, of equal length within a group of CTAs (the first of a group have a unit more). Where three CTAs are on an SM and runs are long there are three groups:
+// of an SM's warps the oldest are served first, so the CTAs that started first have more (with equal runs the thirds of 256 chats' CTAs ended at 121, 133 and 146 us).
+struct A4Cut {
+    long begin, run, longer;                                     // of a group: first unit, units of a run, runs that have one more
+    int group, per;                                              // its number, warps of a group
+    static constexpr long LONG_RUN = 16;
+    __device__ static long first(long total, int groups, int group) {      // first unit of a group: shares 36 : 32 : 28
+        return groups == 3 ? total * (group == 0 ? 0 : group == 1 ? 36 : group == 2 ? 68 : 96) / 96 : group ? total : 0;
+    }
+    __device__ A4Cut(const Attention4Args& a, long total, long warps, int groups, int g) : group(g), per((int)(warps / groups)) {
+        begin = first(total, groups, g);
+        const long n = first(total, groups, g + 1) - begin;
+        run = !n ? 0 : a.few_units ? (long)((unsigned)n / (unsigned)per) : n / per;      // (a division in 64 bits takes a hundred instructions)
+        longer = n - run * per;
+    }
+    __device__ long at(int i) const { return begin + run * i + min((long)i, longer); }      // first unit of the group's run i
+    __device__ int owner(long u) const {                         // the run that has a unit of the group
+        const long x = u - begin, most = longer * (run + 1);
+        return (int)(x < most ? x / (run + 1) : longer + (x - most) / run);
     }
 };
 
@@ -129,16 +152,17 @@ struct A4Sum {
     }
 };
 
-constexpr int A4_PER_SM[2] = {3, 2}, A4_MOST_CTAS = A4_SMS * 3;      // CTAs that run at once (of tiles of 8 and of 16 rows)
+constexpr int a4_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int A4_MOST_CTAS = A4_SMS * 3;      // CTAs that run at once (of tiles of 8 and of 16 rows)
 // units of work that a call can have at most
 inline double a4_most_units(const Attention4Args& a, int mt) {
     const long steps = ((long)a.r.max_pages * a.r.block_tokens + A4_KEYS - 1) / A4_KEYS;
-    return (double)a.r.n_seqs * a.n_kv * (((double)a.max_rows * (a.n_head / a.n_kv) + mt - 1) / mt) * (steps + 1);
+    return (double)a.r.n_seqs * a.n_kv * (((double)a.max_rows * (a.n_head / a.n_kv) + mt - 1) / mt) * (steps + A4_BEGIN);
 }
 }  // namespace
 
 template <int D, int NT>
-__global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_step_kernel(const Attention4Args a) {
+__global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step_kernel(const Attention4Args a) {
     constexpr int NG = D / Q4_GROUP, BLOCK = q4_block(D), KB = A4_BLOCKS, STAGE = 2 * KB * BLOCK, S = A4_STAGES, MT = 8 * NT, PART = a4_part<D>(MT);
     constexpr int REGION = S * STAGE > PART * 4 ? S * STAGE : PART * 4;
     extern __shared__ __align__(128) uint8_t a4_raw[];
@@ -187,12 +211,20 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
-    // the first `longer` runs have a unit more than the others
     const long all_warps = (long)gridDim.x * A4_WARPS, warps = min(all_warps, total), me = (long)blockIdx.x * A4_WARPS + warp;
-    const long run = warps ? total / warps : 0, longer = total - run * warps;
-    const long u0 = me < warps ? run * me + min(me, longer) : 0, u1 = me < warps ? u0 + run + (me < longer) : 0;
-    A4At at;
-    at.z = n_seqs; at.kvh = at.tile = at.step = 0;
+    const int groups = total >= all_warps * A4Cut::LONG_RUN && a4_per_sm(NT) == 3 && (int)gridDim.x == A4_SMS * 3 ? 3 : 1;
+    const int group = groups > 1 ? blockIdx.x / A4_SMS : 0;
+    long u0 = 0, u1 = 0;
+    if (me < warps) {
+        const A4Cut cut(a, total, warps, groups, group);
+        const int i = (int)me - group * cut.per;
+        u0 = cut.at(i); u1 = cut.at(i + 1);
+    }
+    __shared__ A4At places[A4_WARPS][2];                         // where the warp is, and where its copies are (few registers: they change once a segment)
+    A4At& at = places[warp][0];
+    A4At& ahead = places[warp][1];
+    A4At start;
+    start.z = n_seqs; start.kvh = start.tile = start.step = 0;
     long first = u0;                                             // the first unit that is a step
     if (u0 < u1) {
         long rest = 0;
@@ -208,8 +240,8 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
                 const unsigned past = __ballot_sync(0xffffffffu, before + sum > (int)u0);
                 if (past) {
                     const int l = __ffs(past) - 1;
-                    at.z = 32 * i + l;
-                    at.s = i == 0 ? kept.from_lane(l) : A4Seq(a, at.z, MT);
+                    start.z = 32 * i + l;
+                    start.s = i == 0 ? kept.from_lane(l) : A4Seq(a, start.z, MT);
                     rest = u0 - before - __shfl_sync(0xffffffffu, sum - kept_units[i], l);
                     found = true;
                 }
@@ -225,69 +257,82 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
                 const unsigned past = __ballot_sync(0xffffffffu, before + sum > u0);
                 if (past) {
                     const int l = __ffs(past) - 1;
-                    at.z = z0 + l;
-                    at.s = A4Seq(a, at.z, MT);
+                    start.z = z0 + l;
+                    start.s = A4Seq(a, start.z, MT);
                     rest = u0 - before - __shfl_sync(0xffffffffu, sum - mine, l);
                     break;
                 }
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
         }
-        const long each = at.s.steps + 1, per = at.s.tiles * each;
-        at.kvh = (int)(rest / per); rest -= at.kvh * per;
-        at.tile = (int)(rest / each); rest -= at.tile * each;
-        if (rest == 0) first++; else rest--;
-        at.step = (int)rest;
+        const long each = start.s.steps + A4_BEGIN, per = start.s.tiles * each;
+        start.kvh = a.few_units ? (int)((unsigned)rest / (unsigned)per) : (int)(rest / per); rest -= start.kvh * per;
+        start.tile = a.few_units ? (int)((unsigned)rest / (unsigned)each) : (int)(rest / each); rest -= start.tile * each;
+        first += max(A4_BEGIN - rest, 0l);
+        start.step = (int)max(rest - A4_BEGIN, 0l);
     }
 
     // ---- copies: a lane has keys or values of one of the step's blocks, the page's id read a step ahead
-    A4At ahead = at;
+    if (lane == 0) { at = start; ahead = start; }
     int to_copy = (int)max(u1 - first, 0l), id = 0, in_page = 0, put = 0;      // units of the run from the next copy on
+    int c_step = start.step, c_steps = start.s.steps, c_own = start.s.own;     // of the copies' segment
     const int c_kv = lane >= KB, c_blk = lane - c_kv * KB;
+    const long per_head = (long)blocks * BLOCK, per_page = n_kv * per_head;
     const uint8_t* const pool = (const uint8_t*)(c_kv ? a.v_pool : a.k_pool);
+    const uint8_t* from_head = pool + start.kvh * per_head;
+    const int* table = a.r.pages + start.z * a.r.table_stride;
     auto read_id = [&]() {
-        const unsigned b = ahead.step * KB + c_blk;              // block of the sequence
+        const unsigned b = c_step * KB + c_blk;                  // block of the sequence
         unsigned page = __umulhi(b, a.per_page);                 // the quotient by the page's blocks, or one less
         in_page = (int)(b - page * blocks);
         if (in_page >= blocks) { page++; in_page -= blocks; }
-        id = lane < 2 * KB && to_copy > 0 && (int)b * Q4_TOKENS < ahead.s.own ? a.r.pages[ahead.z * a.r.table_stride + page] : 0;
+        id = lane < 2 * KB && to_copy > 0 && (int)b * Q4_TOKENS < c_own ? table[page] : 0;
     };
     read_id();
+    __syncwarp();
     auto copy = [&]() {
         if (to_copy <= 0) return;
-        const int n = min(KB, (ahead.s.own - ahead.step * A4_KEYS + Q4_TOKENS - 1) / Q4_TOKENS);
+        const int n = min(KB, (c_own - c_step * A4_KEYS + Q4_TOKENS - 1) / Q4_TOKENS);
         if (lane == 0) mbar_arrive_expect_tx(&full[warp][put], (uint32_t)(max(n, 0) * 2 * BLOCK));
         __syncwarp();
-        if (lane < 2 * KB && c_blk < n) {
-            const long page = min(max(id, 0), last_page);
-            tma_load_1d(ring + put * STAGE + lane * BLOCK, pool + ((page * n_kv + ahead.kvh) * blocks + in_page) * BLOCK, BLOCK, &full[warp][put]);
-        }
+        if (lane < 2 * KB && c_blk < n)
+            tma_load_1d(ring + put * STAGE + lane * BLOCK, from_head + min(max(id, 0), last_page) * per_page + in_page * BLOCK, BLOCK, &full[warp][put]);
         __syncwarp();
         put = put + 1 == S ? 0 : put + 1;
-        to_copy -= ahead.next(a, MT);
-        read_id();
-        if (ahead.step == 0 && to_copy > 0) {                    // the next segment's queries, on their way into the L1 cache
+        to_copy--;
+        if (++c_step == c_steps) {                               // the next segment
+            to_copy -= A4_BEGIN;
+            c_step = 0;
+            if (lane == 0) ahead.next(a, MT);
+            __syncwarp();
+            c_steps = ahead.s.steps; c_own = ahead.s.own;
+            from_head = pool + ahead.kvh * per_head;
+            table = a.r.pages + ahead.z * a.r.table_stride;
+            // its queries, on their way into the L1 cache
             const int f0 = ahead.tile * MT, row = lane >> 1;
-            if (row < min((long)MT, (long)ahead.s.n * G - f0)) {
+            if (to_copy > 0 && row < min((long)MT, (long)ahead.s.n * G - f0)) {
                 const int f = f0 + row, i = f / G;
                 const uint16_t* q = (const uint16_t*)a.q + (size_t)(ahead.s.r0 + i) * a.q_row + (size_t)(ahead.kvh * G + f - i * G) * a.q_head + (lane & 1) * (D / 2);
                 asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
             }
+            __syncwarp();
         }
+        read_id();
     };
     for (int i = 0; i < S; i++) copy();
 
+    const uint32_t less[4] = {a4_keep(0x80088008u), a4_keep(0x80808080u), a4_keep(0x80088008u), a4_keep(0x80808080u)};      // -8 2^-24 and -8 2^-20
     int st = 0;
     uint32_t parity = 0;
     for (long u = first; u < u1;) {
         // ================= a segment: queries, as the fragments of eight rows each; rows past the tile's are zeros
-        const A4Seq& s = at.s;
+        const A4Seq s = at.s;
         const int kvh = at.kvh, f0 = at.tile * MT, n_f = (int)min((long)MT, (long)s.n * G - f0), r0 = s.r0;
         const long left = s.steps - at.step;
         const int n = (int)min(left, u1 - u), step0 = at.step;
         const bool begins = step0 == 0, ends = n == left;
         uint32_t qb[NT][NG][4];
-        float off[NT][NG][2], by[NT][2];                         // of rows 2 tq and 2 tq + 1: the sums' initial values, and what a score is multiplied with
+        float off[NT][NG][4], by[NT][2];                         // of rows 2 tq and 2 tq + 1: the sums' initial values, and what a score is multiplied with
         int lim[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -336,7 +381,9 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-                for (int j = 0; j < 2; j++) off[nt][gi][j] = __shfl_sync(0xffffffffu, sum, (2 * tq + j) * 4) * -0x1p-21f;      // 8 2^-24
+                for (int j = 0; j < 2; j++) off[nt][gi][j] = a4_keep(__shfl_sync(0xffffffffu, sum, (2 * tq + j) * 4) * -0x1p-21f);      // 8 2^-24
+#pragma unroll
+                for (int j = 0; j < 2; j++) off[nt][gi][j + 2] = a4_keep(off[nt][gi][j]);
             }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -481,7 +528,7 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
                         a4_mma(o[nt][gi][0], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, b0, b1);
                         a4_mma(o[nt][gi][1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, b0, b1);
 #pragma unroll
-                        for (int m = 0; m < 2; m++) a4_mma(o[nt][gi][m], 0x80088008u, 0x80808080u, 0x80088008u, 0x80808080u, b0, b1);      // -8 2^-24 and -8 2^-20
+                        for (int m = 0; m < 2; m++) a4_mma(o[nt][gi][m], less[0], less[1], less[2], less[3], b0, b1);
                     }
                 }
             }
@@ -536,15 +583,17 @@ __global__ void __launch_bounds__(A4_THREADS, A4_PER_SM[NT - 1]) attention_4bit_
                 }
             }
         if (!(begins && ends) && lane == 0) {
-            const long end = u - n + left - 1, most = longer * (run + 1);        // the segment's last unit
-            held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, (int)((end < most ? end / (run + 1) : longer + (end - most) / run) / A4_WARPS)};
+            const long end = u - n + left - 1;                   // the segment's last unit
+            int in = group;
+            while (in + 1 < groups && end >= A4Cut::first(total, groups, in + 1)) in++;
+            const A4Cut cut(a, total, warps, groups, in);
+            held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, (in * cut.per + cut.owner(end)) / A4_WARPS};
         }
         // the segment behind it (not the sequence's loads if there is none)
-        u++;                                                     // (its beginning)
-        if (u < u1) {
-            at.step = s.steps - 1;
-            at.next(a, MT);
-        }
+        u += A4_BEGIN;
+        __syncwarp();
+        if (u < u1 && lane == 0) at.next(a, MT);
+        __syncwarp();
     }
     __syncthreads();
 
@@ -652,7 +701,7 @@ cudaError_t a4_step(Attention4Args a, cudaStream_t s) {
     if (!allow_smem<attention_4bit_step_kernel<D, NT>>(smem)) return cudaErrorInvalidValue;
     // as many CTAs as run at once, no more than there can be steps for
     const double units = a4_most_units(a, MT);
-    const int ctas = (int)std::min<double>(A4_SMS * A4_PER_SM[NT - 1], std::ceil(units / A4_WARPS));
+    const int ctas = (int)std::min<double>(A4_SMS * a4_per_sm(NT), std::ceil(units / A4_WARPS));
     a.few_units = units < 1e9;
     const unsigned blocks = a.r.block_tokens / Q4_TOKENS;
     a.per_page = blocks == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / blocks);
