@@ -29,7 +29,7 @@ namespace b2 {
 namespace {
 constexpr int A4_WARPS = 4, A4_THREADS = 32 * A4_WARPS;
 constexpr int A4_BLOCKS = 2, A4_KEYS = A4_BLOCKS * Q4_TOKENS;      // blocks and keys of a step
-constexpr int A4_STAGES = 3;         // steps under way
+constexpr int A4_STAGES = 2;         // steps under way
 constexpr int A4_BEGIN = 2;          // units that a segment's beginning and end count as, beside its steps
 constexpr int A4_SMS = 148;
 
@@ -322,6 +322,9 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
     for (int i = 0; i < S; i++) copy();
 
     const uint32_t less[4] = {a4_keep(0x80088008u), a4_keep(0x80808080u), a4_keep(0x80088008u), a4_keep(0x80808080u)};      // -8 2^-24 and -8 2^-20
+    // where a lane's chunks and scales lie in a step: key g of a block (the one 8 further on is turned alike), pair tq of the values
+    const uint32_t k_from = a4_keep((uint32_t)(g * (D / 2) + q4_key_chunk(D, g, tq) * NG * 4)), k_scale = a4_keep((uint32_t)q4_scale(D, g, 0));
+    const uint32_t v_from = a4_keep((uint32_t)(KB * BLOCK + tq * D + q4_value_chunk(D, tq, g) * NG * 4)), v_scale = k_scale + KB * BLOCK;
     int st = 0;
     uint32_t parity = 0;
     for (long u = first; u < u1;) {
@@ -411,14 +414,12 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             float sc[KB][NT][4];
 #pragma unroll
             for (int b = 0; b < KB; b++) {
-                const uint8_t* kb = stage + b * BLOCK;
                 uint32_t w[2][NG];
                 float ks[2][NG];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int key = g + 8 * h;
-                    a4_chunk<NG>(kb + key * (D / 2) + q4_key_chunk(D, key, tq) * NG * 4, w[h]);
-                    a4_scales<NG>(kb + q4_scale(D, key, 0), ks[h]);
+                    a4_chunk<NG>(stage + k_from + b * BLOCK + 8 * h * (D / 2), w[h]);
+                    a4_scales<NG>(stage + k_scale + b * BLOCK + h * 8 * NG * 2, ks[h]);
                 }
 #pragma unroll
                 for (int gi = 0; gi < NG; gi++) {
@@ -433,21 +434,18 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                     }
                 }
             }
-            // ---- scales of the values, and the largest of them
-            float vs[KB][2][NG];
-            __half2 most = a4_as_half2(0);
+            // ---- the largest of the values' scales
+            __half2 most = a4_as_half2(0);                       // (read again below: few registers)
 #pragma unroll
             for (int b = 0; b < KB; b++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const __half2* from = reinterpret_cast<const __half2*>(stage + (KB + b) * BLOCK + q4_scale(D, g + 8 * h, 0));
+                    const __half2* from = reinterpret_cast<const __half2*>(stage + v_scale + b * BLOCK + h * 8 * NG * 2);
 #pragma unroll
                     for (int gi = 0; gi < NG; gi += 2) {
                         __half2 v = from[gi >> 1];
                         if (PARTLY && t0 + b * 16 + g + 8 * h >= own) v = a4_as_half2(0);      // (whatever lies there)
                         most = __hmax2(most, __habs2(v));
-                        const float2 f = __half22float2(v);
-                        vs[b][h][gi] = f.x; vs[b][h][gi + 1] = f.y;
                     }
                 }
             const float2 most2 = __half22float2(most);
@@ -509,14 +507,17 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                         pr[nt][e] = a4_exp2(fmaf(sc[b][nt][e], by[nt][e & 1], -ref[nt][e & 1]));
                         l[nt][e & 1] += pr[nt][e];
                     }
-                const uint8_t* vb = stage + (KB + b) * BLOCK;
                 uint32_t w[2][NG];
+                float vs[2][NG];
 #pragma unroll
-                for (int h = 0; h < 2; h++) a4_chunk<NG>(vb + (tq + 4 * h) * D + q4_value_chunk(D, tq, g) * NG * 4, w[h]);
+                for (int h = 0; h < 2; h++) {
+                    a4_chunk<NG>(stage + v_from + b * BLOCK + 4 * h * D, w[h]);
+                    a4_scales<NG>(stage + v_scale + b * BLOCK + h * 8 * NG * 2, vs[h]);
+                }
 #pragma unroll
                 for (int gi = 0; gi < NG; gi++) {
                     const uint32_t x = w[0][gi], y = w[1][gi], x8 = x >> 8, y8 = y >> 8;
-                    const float s0 = vs[b][0][gi] * up_v, s1 = vs[b][1][gi] * up_v;
+                    const float s0 = vs[0][gi] * up_v, s1 = vs[1][gi] * up_v;
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         float z[4] = {pr[nt][0] * s0, pr[nt][1] * s0, pr[nt][2] * s1, pr[nt][3] * s1};
