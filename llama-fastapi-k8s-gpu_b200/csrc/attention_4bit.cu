@@ -82,14 +82,8 @@ struct A4Seq {
         tiles = (n * (a.n_head / a.n_kv) + mt - 1) / mt;
         steps = n ? max(1, (own + A4_KEYS - 1) / A4_KEYS) : 0;
     }
-    __device__ long units(int n_kv) const { return steps ? (long)n_kv * tiles * (steps + A4_BEGIN) : 0; }
+    __device__ long units(int n_kv) const { return steps ? (long)(n_kv * tiles) * (steps + A4_BEGIN) : 0; }
     __device__ int limit(int i) const { return max(0, lim0 + i); }                      // keys that row i sees
-    __device__ A4Seq from_lane(int l) const {
-        A4Seq s;
-        s.r0 = __shfl_sync(0xffffffffu, r0, l); s.n = __shfl_sync(0xffffffffu, n, l); s.own = __shfl_sync(0xffffffffu, own, l); s.lim0 = __shfl_sync(0xffffffffu, lim0, l);
-        s.tiles = __shfl_sync(0xffffffffu, tiles, l); s.steps = __shfl_sync(0xffffffffu, steps, l);
-        return s;
-    }
 };
 // a place in the steps of all segments laid end to end, each behind its beginning's units
 struct A4At {
@@ -122,8 +116,9 @@ struct A4Cut {
         longer = n - run * per;
     }
     __device__ long at(int i) const { return begin + run * i + min((long)i, longer); }      // first unit of the group's run i
-    __device__ int owner(long u) const {                         // the run that has a unit of the group
+    __device__ int owner(const Attention4Args& a, long u) const {      // the run that has a unit of the group
         const long x = u - begin, most = longer * (run + 1);
+        if (a.few_units) return (int)(x < most ? (unsigned)x / (unsigned)(run + 1) : (unsigned)longer + (unsigned)(x - most) / (unsigned)run);
         return (int)(x < most ? x / (run + 1) : longer + (x - most) / run);
     }
 };
@@ -182,29 +177,22 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
     __syncwarp();
     const int n_kv = a.n_kv, G = a.n_head / n_kv, blocks = a.r.block_tokens / Q4_TOKENS, last_page = (int)a.r.n_pages - 1;
 
-    // ---- the units of all sequences, and this warp's run [u0, u1) of them. Up to 256 sequences are read at once and kept.
-    constexpr int KEPT = 8;
+    // ---- the units of all sequences, and this warp's run [u0, u1) of them. Up to 256 sequences are read once a CTA and kept. (All CTAs read the same few lines, one after the other.)
+    constexpr int KEPT = 256;
+    __shared__ int kept_units[KEPT];
+    __shared__ A4Seq kept[KEPT / 4];
     const int n_seqs = a.r.n_seqs;
-    A4Seq kept;
-    int kept_units[KEPT];
     long total = 0;
-    const bool keep = n_seqs <= 32 * KEPT && a.few_units;
+    const bool keep = n_seqs <= KEPT && a.few_units;
     if (keep) {
-        int b[KEPT], e[KEPT], h[KEPT];
-#pragma unroll
-        for (int i = 0; i < KEPT; i++) {
-            const int z = 32 * i + lane;
-            b[i] = e[i] = h[i] = 0;
-            if (z < n_seqs) { b[i] = a.r.row_start[z]; e[i] = a.r.row_start[z + 1]; h[i] = a.r.lengths[z]; }
+        for (int z = threadIdx.x; z < n_seqs; z += A4_THREADS) {
+            const A4Seq s(a, z, MT);
+            kept_units[z] = (int)s.units(n_kv);
+            if (z < KEPT / 4) kept[z] = s;
         }
+        __syncthreads();
         int sum = 0;
-#pragma unroll
-        for (int i = 0; i < KEPT; i++) {
-            const A4Seq s(a, b[i], e[i], h[i], MT);
-            kept_units[i] = 32 * i < n_seqs ? (int)s.units(n_kv) : 0;
-            if (i == 0) kept = s;
-            sum += kept_units[i];
-        }
+        for (int z = lane; z < n_seqs; z += 32) sum += kept_units[z];
         total = __reduce_add_sync(0xffffffffu, (unsigned)sum);
     } else {
         for (int z = lane; z < n_seqs; z += 32) total += A4Seq(a, z, MT).units(n_kv);
@@ -230,20 +218,18 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
         long rest = 0;
         if (keep) {
             int before = 0;
-            bool found = false;
-#pragma unroll
-            for (int i = 0; i < KEPT; i++) {
-                if (found || 32 * i >= n_seqs) continue;
-                int sum = kept_units[i];                         // of sequences 32 i .. 32 i + lane
+            for (int z0 = 0; z0 < n_seqs; z0 += 32) {
+                const int mine = z0 + lane < n_seqs ? kept_units[z0 + lane] : 0;
+                int sum = mine;                                  // of sequences z0 .. z0 + lane
 #pragma unroll
                 for (int o = 1; o < 32; o *= 2) { const int v = __shfl_up_sync(0xffffffffu, sum, o); if (lane >= o) sum += v; }
                 const unsigned past = __ballot_sync(0xffffffffu, before + sum > (int)u0);
                 if (past) {
                     const int l = __ffs(past) - 1;
-                    start.z = 32 * i + l;
-                    start.s = i == 0 ? kept.from_lane(l) : A4Seq(a, start.z, MT);
-                    rest = u0 - before - __shfl_sync(0xffffffffu, sum - kept_units[i], l);
-                    found = true;
+                    start.z = z0 + l;
+                    start.s = start.z < KEPT / 4 ? kept[start.z] : A4Seq(a, start.z, MT);
+                    rest = u0 - before - __shfl_sync(0xffffffffu, sum - mine, l);
+                    break;
                 }
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
@@ -588,7 +574,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             int in = group;
             while (in + 1 < groups && end >= A4Cut::first(total, groups, in + 1)) in++;
             const A4Cut cut(a, total, warps, groups, in);
-            held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, (in * cut.per + cut.owner(end)) / A4_WARPS};
+            held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, (in * cut.per + cut.owner(a, end)) / A4_WARPS};
         }
         // the segment behind it (not the sequence's loads if there is none)
         u += A4_BEGIN;
