@@ -674,13 +674,7 @@ constexpr int a4_smem() {
 }
 template <int D, int MT>
 cudaError_t a4_join(const Attention4Args& a, int ctas, cudaStream_t s) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, MT); cfg.blockDim = dim3(128); cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, attention_4bit_join_kernel<D, MT>, a, ctas);
+    return launch_chain(attention_4bit_join_kernel<D, MT>, dim3(ctas, MT), dim3(128), 0, s, a, ctas);
 }
 template <int D, int NT>
 cudaError_t a4_step(Attention4Args a, cudaStream_t s) {
@@ -717,6 +711,7 @@ size_t attention_4bit_work_bytes(long n_rows, int n_head, int n_kv, int head_dim
 
 cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s) {
     if (a.r.n_rows == 0 || a.r.n_seqs == 0) return cudaSuccess;
+    const DependentLaunch dependent;
     if (a4_many(a.max_rows, a.n_head, a.n_kv)) return attention_4bit_tc_launch(a, s);
     const bool few = (long)a.max_rows * (a.n_head / a.n_kv) <= 8;
     if (a.head_dim == 64) return few ? a4_step<64, 1>(a, s) : a4_step<64, 2>(a, s);

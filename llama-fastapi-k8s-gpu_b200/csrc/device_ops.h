@@ -33,6 +33,14 @@ __device__ __forceinline__ int seq_of_row(const int* row_start, int n_seqs, int 
 }
 #endif
 
+// Launches inside this scope may start while the kernel before them ends (launch_chain): they wait for it before they touch memory. Calls one after another, us each, with it and
+// without: attention of 32 chats over a cache in 4 bits 19.5 and 21.2, of one chat 11.5 and 12.3.
+struct DependentLaunch {
+    bool prev;
+    DependentLaunch() : prev(g_chain_pdl) { g_chain_pdl = true; }
+    ~DependentLaunch() { g_chain_pdl = prev; }
+};
+
 // ---------------------------------------------------------------- kv_append.cu
 struct KvAppendArgs {
     RaggedPages r;

@@ -143,6 +143,8 @@ __global__ void __launch_bounds__(K4_THREADS, 3) kv_append_4bit_kernel(const KvA
     __shared__ alignas(16) float2 turns[K4_WARPS][D / 2];        // cosines and sines of the warp's row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.rot_dims >> 1;
     const long item = (long)blockIdx.x * K4_WARPS + warp, row = item >> parts;
+    griddep_wait();
+    griddep_launch();
     if (row >= a.r.n_rows) return;
     const int part = (int)(item - (row << parts)), w = lane % PIECES, d = 8 * w, h0 = lane / PIECES;
     const bool rotates = d < a.rot_dims, left = d < half;
@@ -304,6 +306,8 @@ __global__ void __launch_bounds__(K4_THREADS) kv_read_4bit_kernel(const KvReadAr
     constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, UNROLL = 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long item = (long)blockIdx.x * K4_WARPS + warp, row0 = (item >> parts) * ROWS;
+    griddep_wait();
+    griddep_launch();
     if (row0 >= a.r.n_rows) return;
     K4Place places[ROWS];
 #pragma unroll
@@ -357,35 +361,29 @@ template <typename In, int D>
 static cudaError_t k4_append(const KvAppendArgs& a, cudaStream_t s) {
     const int size = sizeof(In), parts = k4_parts(a.r.n_rows, a.n_kv * D / 8);
     const int wide = k4_wide(a.k, a.k_row, a.k_head, size) | k4_wide(a.v, a.v_row, a.v_head, size) << 1 | k4_wide(a.q, a.q_row, a.q_head, size) << 2 | k4_wide(a.q_out, a.qo_row, a.qo_head, 2) << 3;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(k4_ctas(a.r.n_rows, parts)); cfg.blockDim = dim3(K4_THREADS); cfg.stream = s;
-    if (a.rot_dims % (a.halves ? 16 : 8)) return cudaLaunchKernelEx(&cfg, kv_append_4bit_kernel<In, D, K4_ANY>, a, wide, parts);
-    return a.halves ? cudaLaunchKernelEx(&cfg, kv_append_4bit_kernel<In, D, K4_HALVES>, a, wide, parts) : cudaLaunchKernelEx(&cfg, kv_append_4bit_kernel<In, D, K4_PAIRS>, a, wide, parts);
+    auto* kernel = a.rot_dims % (a.halves ? 16 : 8) ? kv_append_4bit_kernel<In, D, K4_ANY> : a.halves ? kv_append_4bit_kernel<In, D, K4_HALVES> : kv_append_4bit_kernel<In, D, K4_PAIRS>;
+    return launch_chain(kernel, dim3(k4_ctas(a.r.n_rows, parts)), dim3(K4_THREADS), 0, s, a, wide, parts);
 }
 template <typename In>
 static cudaError_t k4_append_dim(const KvAppendArgs& a, cudaStream_t s) { return a.head_dim == 64 ? k4_append<In, 64>(a, s) : k4_append<In, 128>(a, s); }
 cudaError_t kv_append_4bit_launch(const KvAppendArgs& a, cudaStream_t s) {
     if (a.r.n_rows == 0) return cudaSuccess;
+    const DependentLaunch dependent;
     return a.in_type == ELEM_F32 ? k4_append_dim<float>(a, s) : a.in_type == ELEM_F16 ? k4_append_dim<__half>(a, s) : k4_append_dim<__nv_bfloat16>(a, s);
 }
 
 template <typename Out, int D>
 static cudaError_t k4_read(const KvReadArgs& a, cudaStream_t s) {
     const int parts = k4_parts(a.r.n_rows, a.n_kv * D / 8), wide = k4_wide(a.k, a.k_row, a.k_head, sizeof(Out)) | k4_wide(a.v, a.v_row, a.v_head, sizeof(Out)) << 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(K4_THREADS); cfg.stream = s;
-    // four rows a warp once that leaves a warp for every place on the SMs
-    if (a.r.n_rows >= 4 * 148 * 40) {
-        cfg.gridDim = dim3(k4_ctas((a.r.n_rows + 3) / 4, 0));
-        return cudaLaunchKernelEx(&cfg, kv_read_4bit_kernel<Out, D, 4>, a, wide, 0);
-    }
-    cfg.gridDim = dim3(k4_ctas(a.r.n_rows, parts));
-    return cudaLaunchKernelEx(&cfg, kv_read_4bit_kernel<Out, D, 1>, a, wide, parts);
+    // four rows a warp once that leaves a warp for every place on the SMs: 65536 rows 77 -> 70 us
+    if (a.r.n_rows >= 4 * 148 * 40) return launch_chain(kv_read_4bit_kernel<Out, D, 4>, dim3(k4_ctas((a.r.n_rows + 3) / 4, 0)), dim3(K4_THREADS), 0, s, a, wide, 0);
+    return launch_chain(kv_read_4bit_kernel<Out, D, 1>, dim3(k4_ctas(a.r.n_rows, parts)), dim3(K4_THREADS), 0, s, a, wide, parts);
 }
 template <typename Out>
 static cudaError_t k4_read_dim(const KvReadArgs& a, cudaStream_t s) { return a.head_dim == 64 ? k4_read<Out, 64>(a, s) : k4_read<Out, 128>(a, s); }
 cudaError_t kv_read_4bit_launch(const KvReadArgs& a, cudaStream_t s) {
     if (a.r.n_rows == 0 || (!a.k && !a.v)) return cudaSuccess;
+    const DependentLaunch dependent;
     return a.out_type == ELEM_F32 ? k4_read_dim<float>(a, s) : a.out_type == ELEM_F16 ? k4_read_dim<__half>(a, s) : k4_read_dim<__nv_bfloat16>(a, s);
 }
 
