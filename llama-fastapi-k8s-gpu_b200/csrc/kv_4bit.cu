@@ -2,8 +2,10 @@
 // The rotation is that of kv_append.cu, but sines and cosines too are computed in 64 bits and rounded once, and its products and sums are rounded one by one (no fused
 // multiply-add): which code an entry gets is decided at borders, and so it follows from the definition alone, whatever rotates the keys.
 //
-// Bound by memory. A warp takes a row, or a part of its heads where the rows are few, and finds its place by itself; a lane has a piece of eight entries of a head, 32 bits of
-// codes, and four neighbouring lanes have a group. Several pieces are under way at once.
+// A warp takes a row, or a part of its heads where the rows are few, and finds its place by itself; a lane has a piece of eight entries of a head, 32 bits of codes, and four
+// neighbouring lanes have a group. Reads are bound by memory and by the chain that each row begins with (sequence, page, codes), so as many warps as an SM holds have two turns of pieces each
+// under way: 65536 rows of 2 x 8 heads of 128 to f16 67 us, 0.78 of the measured bandwidth (four turns and half the warps 78), 37000 ragged rows of 2 x 5 heads to bf16 30. Appends are bound by
+// instructions as much as by memory, some 170 a piece of keys and 60 a piece of queries: 16384 rows of 32 + 2 x 8 heads of 128 100 us, 3.7 TB/s, 32 rows 5.3.
 #include "device_ops.h"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"
@@ -138,8 +140,8 @@ enum K4Turn { K4_PAIRS, K4_HALVES, K4_ANY };
 
 // `wide`: bits 0 .. 3, whether pieces of k, v, q and q_out are 16 bytes at 16-byte addresses. `parts`: log2 of the warps a row
 template <typename In, int D, int TURN>
-__global__ void __launch_bounds__(K4_THREADS, 3) kv_append_4bit_kernel(const KvAppendArgs a, const int wide, const int parts) {
-    constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, UNROLL = sizeof(In) == 4 || TURN != K4_PAIRS ? 2 : 4;      // pieces of a head, heads of a turn, turns under way
+__global__ void __launch_bounds__(K4_THREADS, 4) kv_append_4bit_kernel(const KvAppendArgs a, const int wide, const int parts) {
+    constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, UNROLL = sizeof(In) == 4 || TURN != K4_PAIRS ? 1 : 2;      // pieces of a head, heads of a turn, turns under way
     __shared__ alignas(16) float2 turns[K4_WARPS][D / 2];        // cosines and sines of the warp's row
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, half = a.rot_dims >> 1;
     const long item = (long)blockIdx.x * K4_WARPS + warp, row = item >> parts;
@@ -302,8 +304,8 @@ __device__ __forceinline__ void k4_put(Out* p, bool wide, const __half2 (&v)[4],
 
 // ROWS: rows of a warp, whose places are found at once
 template <typename Out, int D, int ROWS>
-__global__ void __launch_bounds__(K4_THREADS) kv_read_4bit_kernel(const KvReadArgs a, const int wide, const int parts) {
-    constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, UNROLL = 4;
+__global__ void __launch_bounds__(K4_THREADS, 8) kv_read_4bit_kernel(const KvReadArgs a, const int wide, const int parts) {
+    constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, UNROLL = 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long item = (long)blockIdx.x * K4_WARPS + warp, row0 = (item >> parts) * ROWS;
     griddep_wait();
@@ -375,8 +377,8 @@ cudaError_t kv_append_4bit_launch(const KvAppendArgs& a, cudaStream_t s) {
 template <typename Out, int D>
 static cudaError_t k4_read(const KvReadArgs& a, cudaStream_t s) {
     const int parts = k4_parts(a.r.n_rows, a.n_kv * D / 8), wide = k4_wide(a.k, a.k_row, a.k_head, sizeof(Out)) | k4_wide(a.v, a.v_row, a.v_head, sizeof(Out)) << 1;
-    // four rows a warp once that leaves a warp for every place on the SMs: 65536 rows 77 -> 70 us
-    if (a.r.n_rows >= 4 * 148 * 40) return launch_chain(kv_read_4bit_kernel<Out, D, 4>, dim3(k4_ctas((a.r.n_rows + 3) / 4, 0)), dim3(K4_THREADS), 0, s, a, wide, 0);
+    // two rows a warp once that leaves a warp for every place on the SMs, one below: 37000 rows of 5 heads 29.9 and 30.2 us, 16384 rows of 8 heads 32.7 and 17.0
+    if (a.r.n_rows >= 2 * 148 * 64) return launch_chain(kv_read_4bit_kernel<Out, D, 2>, dim3(k4_ctas((a.r.n_rows + 1) / 2, 0)), dim3(K4_THREADS), 0, s, a, wide, 0);
     return launch_chain(kv_read_4bit_kernel<Out, D, 1>, dim3(k4_ctas(a.r.n_rows, parts)), dim3(K4_THREADS), 0, s, a, wide, parts);
 }
 template <typename Out>
