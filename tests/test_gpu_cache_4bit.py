@@ -241,3 +241,324 @@ def test_attention(ops, heads, kv, dim, page, typ, rows, own):
     assert (err <= attention_bar(typ, want, *sizes, dim, max(rows) * heads // kv > 64)).all(), float(err.max())
     assert torch.equal(got, attend(ops, c, q, rows))                    # the same bits again
     assert ops.error(0) == 0
+
+
+# more than 64 rows of a KV head of a sequence go another way than fewer; more than 8 and up to 8 too
+WAYS = [(4, [1, 1, 1]), (8, [3, 1, 4]), (16, [2, 9, 5]), (16, [60, 33, 100])]
+
+
+def visible_nan(c, q, rows, k, v):
+    """attention over values some of which are no numbers, by the definition: a row's dims are NaN where a value that it sees is, all of them where a key is"""
+    R, H, D = q.shape
+    G = H // c.n_kv
+    clean_k, clean_v = torch.nan_to_num(k, nan=0.0), torch.nan_to_num(v, nan=0.0)
+    out, *sizes = attention_exact(c, q, rows, k=clean_k, v=clean_v)
+    r0 = 0
+    for s, (n, o) in enumerate(zip(rows, c.own)):
+        for i in range(n):
+            seen = slice(c.start[s], c.start[s] + max(0, o - n + i + 1))
+            bad_v = torch.isnan(v[seen]).any(0)                          # [kv heads, dim]
+            bad_k = torch.isnan(k[seen]).any(0).any(-1, keepdim=True)
+            out[r0 + i][(bad_v | bad_k).repeat_interleave(G, 0)] = math.nan
+        r0 += n
+    return out, sizes
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,rows", WAYS)
+def test_attention_numbers_that_are_none(ops, heads, rows, dim, typ):
+    """a NaN or an infinity in a value reaches the dims of its group, in rows that see its key, and no others; in a key it reaches those rows alone; what lies behind the last token
+    (NaN everywhere) reaches nobody"""
+    own = [n + 37 + 50 * s for s, n in enumerate(rows)]
+    rows_k, rows_v = (torch.randn(sum(own), 2, dim).half() for _ in range(2))
+    start = [sum(own[:s]) for s in range(len(own))]
+    rows_v[start[1] - 1, 0, 5] = math.nan                                # the last token of sequence 0: its last row alone
+    rows_v[start[0] + 3, 1, 40] = math.inf                               # a token that all rows see
+    rows_v[start[2] - 2, 1, 33] = -math.inf                              # the last but one of sequence 1
+    rows_k[start[2] + own[2] - 1, 1, 7] = math.nan                       # a key, sequence 2
+    c = Cache4(1, 2, dim, 16, own, k=rows_k, v=rows_v, fill=0xff)
+    q = torch.randn(sum(rows), heads, dim, generator=c.g).to(TYPES[typ]).cuda()
+    got = attend(ops, c, q, rows)
+    want, sizes = visible_nan(c, q, rows, c.values(c.k), c.values(c.v))
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.isnan(want).any() and not torch.isnan(want).all()
+    fine = ~torch.isnan(want)
+    bar = attention_bar(typ, torch.nan_to_num(want), *sizes, dim, max(rows) * heads // 2 > 64)
+    assert ((got.to(F64) - want).abs() <= bar)[fine].all()
+
+
+@pytest.mark.parametrize("heads,rows", WAYS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_sizes_of_values(ops, heads, rows, dim):
+    """values and keys far apart in size from head to head, group to group and token to token: near the smallest f16 numbers, past the largest"""
+    own = [n + 70 + 30 * s for s, n in enumerate(rows)]
+    c0 = Cache4(2, 4, dim, 16, own, "bf16")
+    k, v = c0.k.float(), c0.v.float()
+    v[:, 0] *= 2.0 ** -17                                                # scales that f16 holds with few bits
+    v[:, 1] *= 3e4                                                       # past f16's largest number
+    v[:, 2] *= (10.0 ** torch.arange(-3, 4).float())[torch.arange(len(v)) % 7][:, None]
+    v[:, 3, :32] = 0.0
+    k[:, 1] *= 1e-4
+    k[:, 2] *= 2e4
+    c = Cache4(2, 4, dim, 16, own, k=k.bfloat16(), v=v.bfloat16())
+    q = torch.randn(sum(rows), heads, dim, generator=c.g)
+    q[:, heads // 2:heads // 4 * 3] *= 1e-4                              # (of the large keys)
+    q = q.bfloat16().cuda()
+    got = attend(ops, c, q, rows)
+    want, *sizes = attention_exact(c, q, rows)
+    assert torch.isfinite(got).all()
+    assert ((got.to(F64) - want).abs() <= attention_bar("bf16", want, *sizes, dim, max(rows) * heads // 4 > 64)).all()
+
+
+@pytest.mark.parametrize("heads,rows", WAYS)
+@pytest.mark.parametrize("at,by", [([0], 30.0), ([40], 20.0), ([33, 66, 99, 130], 15.0), ([131, 132], 40.0), ([64], -20.0)])
+def test_attention_scores_that_grow(ops, heads, rows, at, by):
+    """scores that rise by `by` (in log2) at some keys, by a half of it or not at all in some rows: what has been summed up by then falls by as much"""
+    own = [180 + n for n in rows]
+    c0 = Cache4(3, 2, 64, 16, own)
+    k = c0.k.float() * 0.3
+    k[:, :, 0] = 0.0
+    for a in at:
+        for s in range(len(own)):
+            k[c0.start[s] + a:c0.start[s + 1], :, 0] += 8.0
+    c = Cache4(3, 2, 64, 16, own, k=k.half(), v=c0.v)
+    q = torch.randn(sum(rows), heads, 64, generator=c.g)
+    q[..., 0] = torch.tensor([[0.0, 0.5, 1.0, 1.0][(r + h) % 4] * by / 8 / math.log2(math.e) * 8 for r in range(sum(rows)) for h in range(heads)]).view(sum(rows), heads)
+    q = q.half().cuda()
+    got = attend(ops, c, q, rows)
+    want, *sizes = attention_exact(c, q, rows)
+    assert ((got.to(F64) - want).abs() <= attention_bar("f16", want, *sizes, 64, max(rows) * heads // 2 > 64)).all()
+
+
+@pytest.mark.parametrize("heads,rows", WAYS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_strides_alignment_and_scale(ops, heads, rows, dim):
+    """rows and heads apart from each other, queries and outputs that start anywhere, another scale; what lies between the outputs, and behind the last sequence, stays"""
+    own = [n + 20 for n in rows]
+    c = Cache4(4, 4, dim, 48, own)
+    R = sum(rows)
+    wide = torch.randn(R + 3, heads + 1, dim + 7, generator=c.g).bfloat16().cuda()
+    q = wide[:, :heads, 3:3 + dim]
+    out_wide = torch.full((R + 3, heads, dim + 5), 9.0, dtype=torch.bfloat16, device="cuda")
+    out = out_wide[:, :, 1:1 + dim]
+    attend(ops, c, q, rows, scale=0.03, out=out)
+    want, *sizes = attention_exact(c, q[:R], rows, scale=0.03)
+    assert ((out[:R].to(F64) - want).abs() <= attention_bar("bf16", want, *sizes, dim, max(rows) * heads // 4 > 64)).all()
+    assert (out[R:] == 9.0).all() and (out_wide[..., 0] == 9.0).all() and (out_wide[..., 1 + dim:] == 9.0).all()
+    again = torch.full((R, heads, dim), 5.0, dtype=torch.bfloat16, device="cuda")
+    attend(ops, c, q[:R].contiguous(), rows, scale=0.03, out=again)
+    assert torch.equal(again, out[:R])
+
+
+@pytest.mark.parametrize("heads,rows", WAYS)
+def test_attention_rows_past_max_rows_and_what_lengths_say(ops, heads, rows):
+    """rows past max_rows stay; lengths below zero are no tokens, past the table all that it holds; page ids outside the pool are held inside it; rows of nobody stay"""
+    own = [n + 20 for n in rows]
+    c = Cache4(5, 2, 64, 16, own)
+    R, most = sum(rows), max(rows) - 1
+    q = torch.randn(R, heads, 64, generator=c.g).half().cuda()
+    whole = attend(ops, c, q, rows)
+    if most:
+        # the same way with fewer rows (more than 64 of a KV head, or not): rows that are computed are the same to rounding, those past it stay
+        got = attend(ops, c, q, rows, max_rows=most, fill=7.0)
+        want, *sizes = attention_exact(c, q, rows, max_rows=most)
+        r0 = 0
+        for n in rows:
+            assert (got[r0 + min(n, most):r0 + n] == 7.0).all()
+            here = slice(r0, r0 + min(n, most))
+            bar = attention_bar("f16", want, *sizes, 64, most * heads // 2 > 64)
+            assert ((got[here].to(F64) - want[here]).abs() <= bar[here]).all()
+            r0 += n
+    for lengths in ([-1, -2 ** 31, -7], [0, 0, 0]):
+        assert (attend(ops, c, q, rows, own=lengths) == 0).all()
+    full = c.pages.shape[1] * 16
+    c.pages = torch.randint(0, len(c.bytes_k), c.pages.shape, dtype=torch.int32, device="cuda")
+    all_held = attend(ops, c, q, rows, own=[full] * 3)
+    assert torch.equal(attend(ops, c, q, rows, own=[2 ** 31 - 1, full + 1, 10 ** 9]), all_held) or torch.isnan(all_held).any()
+    c.pages[0, 0], c.pages[1, 0] = -5, 2 ** 31 - 1
+    held = c.pages.clone()
+    held[0, 0], held[1, 0] = 0, len(c.bytes_k) - 1
+    a = attend(ops, c, q, rows)
+    c.pages = held
+    assert torch.equal(torch.nan_to_num(a), torch.nan_to_num(attend(ops, c, q, rows)))
+    out = torch.full_like(q, 3.0)
+    work = torch.empty(ops.attention_4bit_workspace(R, heads, 2, 64), dtype=torch.uint8, device="cuda")
+    for at in ([0, 0, 0, 0], [0, -5, -2 ** 31, -1], [R, R, R + 5, 2 ** 31 - 1]):
+        ops.attention_4bit(q, c.k_pool, c.v_pool, c.pages, c.ints(at), c.ints(own), out, work, max_rows=max(rows))
+        assert (out == 3.0).all()
+    assert whole.shape == out.shape and ops.error(0) == 0
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [90, 70]])
+def test_attention_table_that_could_hold_more_than_32_bits_of_work(ops, rows):
+    """the same result whatever the table could hold"""
+    c = Cache4(6, 8, 64, 64, [300, 77])
+    q = torch.randn(sum(rows), 8, 64, generator=c.g).half().cuda()
+    small = attend(ops, c, q, rows)
+    wide = torch.full((2, 2 ** 25 - 100), -1, dtype=torch.int32, device="cuda")
+    wide[:, :c.pages.shape[1]] = c.pages
+    c.pages = wide
+    assert torch.equal(attend(ops, c, q, rows), small)
+
+
+def test_pools_past_32_bits(ops):
+    """pages whose bytes begin past 2^31: appended to, read, attended to as others are"""
+    n_kv, dim, n_pages = 8, 128, 70000
+    own = [200, 64]
+    c = Cache4(7, n_kv, dim, 64, own)
+    far = [torch.empty(n_pages, n_kv, 4, 9 * dim, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    assert far[0].numel() > 2 ** 31
+    table = c.pages.clone()
+    table[table < len(c.bytes_k)] += n_pages - len(c.bytes_k)
+    ops.kv_append_4bit(c.k.cuda(), c.v.cuda(), far[0], far[1], table, c.ints(starts(own)), c.ints(own))
+    back = torch.zeros(sum(own), n_kv, dim, device="cuda")
+    ops.kv_read_4bit(far[0], far[1], table, c.ints(starts(own)), c.ints(own), back, None)
+    assert torch.equal(back.to(F64), c.values(c.k))
+    for rows in ([1, 1], [3, 2], [100, 20]):
+        q = torch.randn(sum(rows), 16, dim, generator=c.g).half().cuda()
+        near = attend(ops, c, q, rows)
+        out = torch.zeros_like(q)
+        work = torch.empty(ops.attention_4bit_workspace(sum(rows), 16, n_kv, dim), dtype=torch.uint8, device="cuda")
+        ops.attention_4bit(q, far[0], far[1], table, c.ints(starts(rows)), c.ints(own), out, work, max_rows=max(rows))
+        assert torch.equal(out, near)
+
+
+# -------------------------------------------------------------------------------------------------------------- the three together
+class Session:
+    """Chats over a cache in 4 bits: prompts, then tokens one by one; what the definition says beside it."""
+
+    def __init__(self, ops, heads, n_kv, dim, page, n_seqs, most, typ, layout, seed=0):
+        self.ops, self.heads, self.n_kv, self.dim, self.layout, self.typ = ops, heads, n_kv, dim, layout, typ
+        self.g = torch.Generator(device="cpu")
+        self.g.manual_seed(seed)
+        per = -(-most // page)
+        self.k_pool, self.v_pool = (torch.randint(0, 256, (n_seqs * per + 1, n_kv, page // 16, 9 * dim), dtype=torch.uint8, generator=self.g).cuda() for _ in range(2))
+        self.pages = torch.randperm(n_seqs * per + 1, generator=self.g)[:n_seqs * per].to(torch.int32).view(n_seqs, per).cuda()
+        self.freqs = (10000.0 ** (-torch.arange(0, dim, 2, dtype=F64) / dim)).float().cuda()
+        self.held = [0] * n_seqs
+        self.k_rows, self.v_rows = [[] for _ in range(n_seqs)], [[] for _ in range(n_seqs)]
+
+    def ints(self, values):
+        return torch.tensor(list(values), dtype=torch.int32, device="cuda")
+
+    def inputs(self, rows):
+        x = torch.randn(sum(rows), (self.heads + 2 * self.n_kv) * self.dim, generator=self.g).to(TYPES[self.typ]).cuda()
+        H, G, D = self.heads, self.n_kv, self.dim
+        return x[:, :H * D].view(-1, H, D), x[:, H * D:(H + G) * D].view(-1, G, D), x[:, (H + G) * D:].view(-1, G, D)
+
+    def call(self, q, k, v, rows, start, held, q_out, out, work, stream=None):
+        self.ops.kv_append_4bit(k, v, self.k_pool, self.v_pool, self.pages, start, held, freqs=self.freqs, layout=self.layout, q=q, q_out=q_out, stream=stream)
+        self.ops.attention_4bit(q_out, self.k_pool, self.v_pool, self.pages, start, held, out, work, max_rows=max(rows), stream=stream)
+
+    def note(self, k, v, rows):
+        r0 = 0
+        for s, n in enumerate(rows):
+            pos = torch.arange(self.held[s], self.held[s] + n, device="cuda")
+            self.k_rows[s].append(coded(rotated_32(k[r0:r0 + n], pos, self.freqs, self.layout)))
+            self.v_rows[s].append(coded(v[r0:r0 + n].float()))
+            self.held[s] += n
+            r0 += n
+
+    def check(self, q, rows, out):
+        """against the definition over what the cache has been given: the output's rounding and 2^-9 of the size of what is summed up (bf16: 2^-6): three times what the roundings come to"""
+        r0 = 0
+        for s, n in enumerate(rows):
+            if n == 0:
+                continue
+            pos = torch.arange(self.held[s] - n, self.held[s], device="cuda")
+            x = rotated_32(q[r0:r0 + n], pos, self.freqs, self.layout).to(TYPES[self.typ]).to(F64)
+            k, v = torch.cat(self.k_rows[s]).transpose(0, 1), torch.cat(self.v_rows[s]).transpose(0, 1)
+            mask = torch.arange(k.shape[1], device="cuda") > pos[:, None]
+            for h in range(self.heads):
+                g = h // (self.heads // self.n_kv)
+                w = torch.softmax((x[:, h] @ k[g].T * self.dim ** -0.5).masked_fill(mask, -math.inf), -1)
+                bar = {"f16": 2 ** -9, "bf16": 2 ** -6}[self.typ] * (w @ v[g].abs())
+                assert ((out[r0:r0 + n, h].to(F64) - w @ v[g]).abs() <= bar).all()
+            r0 += n
+
+    def step(self, rows, stream=None):
+        q, k, v = self.inputs(rows)
+        q_out, out = (torch.full((sum(rows), self.heads, self.dim), math.nan, dtype=TYPES[self.typ], device="cuda") for _ in range(2))
+        work = torch.empty(self.ops.attention_4bit_workspace(sum(rows), self.heads, self.n_kv, self.dim), dtype=torch.uint8, device="cuda")
+        held = [h + n for h, n in zip(self.held, rows)]
+        self.call(q, k, v, rows, self.ints(starts(rows)), self.ints(held), q_out, out, work, stream)
+        self.note(k, v, rows)
+        self.check(q, rows, out)
+
+
+@pytest.mark.parametrize("typ,layout,dim,page", [("f16", "pairs", 128, 64), ("bf16", "halves", 64, 16), ("f16", "halves", 64, 48)])
+def test_chats_over_the_cache(ops, typ, layout, dim, page):
+    """prompts of several lengths in one call, a second part of one of them, drafted tokens, single tokens; the whole cache read back in the end"""
+    s = Session(ops, 8, 2, dim, page, 4, 400, typ, layout)
+    for rows in ([130, 3, 40, 1], [0, 200, 0, 0], [1, 1, 1, 1], [4, 0, 2, 4], [1, 1, 1, 1], [1, 0, 1, 1]):
+        s.step(rows)
+    R = sum(s.held)
+    k, v = (torch.zeros(R, 2, dim, device="cuda") for _ in range(2))
+    ops.kv_read_4bit(s.k_pool, s.v_pool, s.pages, s.ints(starts(s.held)), s.ints(s.held), k, v)
+    assert torch.equal(k.to(F64), torch.cat([torch.cat(x) for x in s.k_rows])) and torch.equal(v.to(F64), torch.cat([torch.cat(x) for x in s.v_rows]))
+    assert ops.error(0) == 0
+
+
+@pytest.mark.parametrize("rows", [[1, 1, 1], [40, 17, 60]])
+def test_captured_steps(ops, rows):
+    """an append and attention in one graph, replayed with other rows and lengths in the same memory; two graphs with the same workspace, one after the other"""
+    s = Session(ops, 8, 2, 128, 64, 3, 500, "f16", "pairs", seed=1)
+    s.step([70, 5, 33])
+    q, k, v = (x.contiguous() for x in s.inputs(rows))
+    start, held = s.ints(starts(rows)), s.ints(s.held)
+    work = torch.empty(ops.attention_4bit_workspace(sum(rows), 8, 2, 128), dtype=torch.uint8, device="cuda")
+    graphs, outs = [], []
+    stream = torch.cuda.Stream()
+    q_out = torch.zeros_like(q)
+    s.call(q, k, v, rows, start, s.ints([h + n for h, n in zip(s.held, rows)]), q_out, torch.zeros_like(q), work)      # (attributes are set outside of a capture; what this stores is stored again)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        out = torch.zeros_like(q)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            s.call(q, k, v, rows, start, held, q_out, out, work, stream=torch.cuda.current_stream())
+        graphs.append(g)
+        outs.append(out)
+    for i in range(4):
+        for old, new in zip((q, k, v), s.inputs(rows)):
+            old.copy_(new)
+        held.copy_(s.ints([h + n for h, n in zip(s.held, rows)]))
+        graphs[i % 2].replay()
+        torch.cuda.synchronize()
+        s.note(k, v, rows)
+        s.check(q, rows, outs[i % 2])
+
+
+def test_two_streams_at_once(ops):
+    """calls with workspaces of their own on two streams give what they give one after the other"""
+    c = Cache4(8, 4, 128, 32, [3000, 700, 64, 1500])
+    cases = [([1, 1, 1, 1], 16), ([300, 2, 64, 120], 16), ([1, 2, 3, 4], 32), ([1, 1, 1, 1], 4)]
+    qs = [torch.randn(sum(rows), heads, 128, generator=c.g).bfloat16().cuda() for rows, heads in cases]
+    want = [attend(ops, c, q, rows) for (rows, _), q in zip(cases, qs)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    works = [[torch.empty(ops.attention_4bit_workspace(len(q), q.shape[1], 4, 128), dtype=torch.uint8, device="cuda") for q in qs] for _ in streams]
+    outs = [[torch.zeros_like(q) for q in qs] for _ in range(12)]
+    ints = [c.ints(starts(rows)) for rows, _ in cases]
+    own = c.ints(c.own)
+    torch.cuda.synchronize()
+    for i in range(12):
+        for j, (rows, _) in enumerate(cases):
+            ops.attention_4bit(qs[j], c.k_pool, c.v_pool, c.pages, ints[j], own, outs[i][j], works[i % 2][j], max_rows=max(rows), stream=streams[i % 2])
+    torch.cuda.synchronize()
+    for got in outs:
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+def test_empty_calls(ops):
+    c = Cache4(9, 2, 64, 16, [5])
+    none = torch.zeros(0, 4, 64, dtype=torch.float16, device="cuda")
+    kv = torch.zeros(0, 2, 64, dtype=torch.float16, device="cuda")
+    work = torch.zeros(16, dtype=torch.uint8, device="cuda")
+    ops.attention_4bit(none, c.k_pool, c.v_pool, c.pages, c.ints([0, 0]), c.ints([5]), none, work)
+    ops.kv_append_4bit(kv, kv, c.k_pool, c.v_pool, c.pages, c.ints([0, 0]), c.ints([5]), q=none, q_out=none)
+    ops.kv_read_4bit(c.k_pool, c.v_pool, c.pages, c.ints([0, 0]), c.ints([5]), kv, kv)
+    assert ops.attention_4bit_workspace(0, 4, 2, 64) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(c.k_pool.cpu(), c.bytes_k)
