@@ -32,6 +32,10 @@ constexpr int A4_BLOCKS = 2, A4_KEYS = A4_BLOCKS * Q4_TOKENS;      // blocks and
 constexpr int A4_STAGES = 2;         // steps under way
 constexpr int A4_BEGIN = 2;          // units that a segment's beginning and end count as, beside its steps
 constexpr int A4_SMS = 148;
+// The join's CTAs. 148 tiles of 256 rows, us: a row a CTA 41 (CTAs start one in 1.1 ns), 16 rows 4. Tiles of 8 and 16 rows, a call of (8 sequences, 12 rows a KV head) and (1, 16, 20000 tokens): 1 row a
+// CTA of 128 threads 19.4 and 18, 4 rows 16.3 and 18.0, 16 of 512 16.4 and 18.8; (1, 4, 4000 tokens) and (32, 4, 500): 1 row of 128 threads 13.1 and 18.1, 2 of 256 12.7 and 17.3.
+constexpr int a4_join_threads(int mt) { return mt == 8 ? 256 : mt == 16 ? 128 : 512; }
+constexpr int a4_join_rows(int mt) { return mt == 8 ? 2 : mt == 16 ? 4 : 16; }
 
 __device__ unsigned int a4_error[5];                             // see mbar_give_up
 
@@ -620,26 +624,31 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
     if (threadIdx.x < 2 && !left_open[threadIdx.x]) desc[threadIdx.x].rows = 0;      // (whatever the workspace held)
 }
 
-// The results of a segment that lies in several CTAs, from the one where it begins on: a row a CTA, a warp has every fourth result, a lane four dims (two for heads of 64)
+// The results of a segment that lies in several CTAs, from the one where it begins on: a CTA has up to 16 rows, a row the lanes of a warp (half of one for heads of 64), four dims each; where
+// there are fewer rows, a row that many times, the CTAs shared among them. (A row a CTA is bound by the start of CTAs, 1.1 ns each: 41 us for 148 tiles of 256 rows.)
 template <int D, int MT>
-__global__ void __launch_bounds__(128) attention_4bit_join_kernel(const Attention4Args a, const int ctas) {
-    constexpr int PART = a4_part<D>(MT), LANES = D / 4, PER = 128 / LANES, B = 8;
-    __shared__ float4 sums[PER][LANES];
-    __shared__ float2 refs[PER];
-    const int c = blockIdx.x, row = blockIdx.y, p = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
+__global__ void __launch_bounds__(a4_join_threads(MT), 1024 / a4_join_threads(MT)) attention_4bit_join_kernel(const Attention4Args a, const int ctas) {
+    constexpr int PART = a4_part<D>(MT), LANES = D / 4, THREADS = a4_join_threads(MT), ROWS = a4_join_rows(MT), GROUPS = THREADS / LANES, B = MT > 16 ? 4 : 8;
+    static_assert(ROWS <= GROUPS && MT % ROWS == 0, "lanes for every row of a CTA");
+    __shared__ float4 sums[GROUPS][LANES];
+    __shared__ float2 refs[GROUPS];
+    const int c = blockIdx.x, row0 = blockIdx.y * ROWS, at = threadIdx.x / LANES, d = threadIdx.x % LANES * 4;
     griddep_wait();
     griddep_launch();
     const A4Desc h = a4_desc<PART>(a, ctas)[c * 2 + 1];
-    if (row >= h.rows) return;
-    const int n = min(h.last, ctas - 1) - c + 1;
+    const int rows = min(h.rows - row0, ROWS);
+    if (rows <= 0) return;
+    int per = GROUPS / ROWS;                                     // lanes of a row's dims: so many times, each for a share of the CTAs
+    while (per * 2 * rows <= GROUPS) per *= 2;
+    const int row = row0 + at / per, n = row < h.rows ? min(h.last, ctas - 1) - c + 1 : 0;
     A4Sum sum;
-    for (int j0 = p; j0 < n; j0 += PER * B) {
+    for (int j0 = at % per; j0 < n; j0 += per * B) {
         float2 ml[B];
         float4 v[B];
 #pragma unroll
         for (int j = 0; j < B; j++) {
             ml[j] = make_float2(-INFINITY, 0.f); v[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-            const int i = j0 + j * PER;
+            const int i = j0 + j * per;
             if (i >= n) continue;
             const float* from = a.work + ((size_t)(c + i) * 2 + (i == 0)) * PART;
             ml[j] = __ldcg(reinterpret_cast<const float2*>(from + MT * D + row * 2));
@@ -652,15 +661,17 @@ __global__ void __launch_bounds__(128) attention_4bit_join_kernel(const Attentio
 #pragma unroll
         for (int j = 0; j < B; j++) sum.add(ml[j], v[j]);
     }
-    sums[p][d / 4] = sum.v;
-    if (d == 0) refs[p] = make_float2(sum.m, sum.l);
-    __syncthreads();
-    if (p) return;
-    A4Sum all;
-#pragma unroll
-    for (int j = 0; j < PER; j++) all.most(refs[j].x);
-#pragma unroll
-    for (int j = 0; j < PER; j++) all.add(refs[j], sums[j][d / 4]);
+    A4Sum all = sum;
+    if (per > 1) {
+        sums[at][d / 4] = sum.v;
+        if (d == 0) refs[at] = make_float2(sum.m, sum.l);
+        __syncthreads();
+        if (at % per) return;
+        all = A4Sum();
+        for (int j = at; j < at + per; j++) all.most(refs[j].x);
+        for (int j = at; j < at + per; j++) all.add(refs[j], sums[j][d / 4]);
+    }
+    if (row >= h.rows) return;
     const int G = a.n_head / a.n_kv, f = h.f0 + row, i = f / G;
     all.out(a, h.r0 + i, h.kvh * G + f - i * G, d);
 }
@@ -674,7 +685,7 @@ constexpr int a4_smem() {
 }
 template <int D, int MT>
 cudaError_t a4_join(const Attention4Args& a, int ctas, cudaStream_t s) {
-    return launch_chain(attention_4bit_join_kernel<D, MT>, dim3(ctas, MT), dim3(128), 0, s, a, ctas);
+    return launch_chain(attention_4bit_join_kernel<D, MT>, dim3(ctas, MT / a4_join_rows(MT)), dim3(a4_join_threads(MT)), 0, s, a, ctas);
 }
 template <int D, int NT>
 cudaError_t a4_step(Attention4Args a, cudaStream_t s) {
@@ -698,7 +709,8 @@ cudaError_t attention_4bit_join(const Attention4Args& a, int ctas, int rows, cud
 }
 
 namespace {
-// Up to so many rows a KV head of a sequence this file's tiles of 16 rows, more on tensor memory
+// Up to so many rows a KV head of a sequence this file's tiles of 16 rows, more on tensor memory. us here and there (heads of 128, 8 KV heads): a sequence of 4000 tokens with 32 rows a KV head
+// 21 and 26, 64 rows 24 and 27, 68 rows 28 and 27, 128 rows 33 and 27; 32 sequences of 1000 tokens with 64 rows 92 and 91, 68 rows 113 and 91, 256 rows 334 and 115.
 constexpr long A4_TC_ROWS = 64;
 bool a4_many(long rows, int n_head, int n_kv) { return rows * (n_head / n_kv) > A4_TC_ROWS; }
 }  // namespace
@@ -713,6 +725,8 @@ cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s) {
     if (a.r.n_rows == 0 || a.r.n_seqs == 0) return cudaSuccess;
     const DependentLaunch dependent;
     if (a4_many(a.max_rows, a.n_head, a.n_kv)) return attention_4bit_tc_launch(a, s);
+    // tiles of 8 rows where all fit one, of 16 (with more registers and less running at once) where not: 4 rows a KV head in tiles of 8 and of 16, us: 32 sequences of 500 tokens 17.6 and 23.6,
+    // 256 of 2000 155 and 229, one of 30000 20.7 and 30.1
     const bool few = (long)a.max_rows * (a.n_head / a.n_kv) <= 8;
     if (a.head_dim == 64) return few ? a4_step<64, 1>(a, s) : a4_step<64, 2>(a, s);
     return few ? a4_step<128, 1>(a, s) : a4_step<128, 2>(a, s);
