@@ -504,7 +504,8 @@ int b2_kv_read_4bit(int device, const b2_ragged_pages* where, const b2_kv_read_4
 /* Attention of a ragged batch over a cache in 4 bits: row i of a sequence sees its tokens up to itself.
  * out = softmax(scale * q.k) v over them, 0 where there are none. Queries and output are f16 or bf16; scores, maxima and sums
  * are 32-bit. For the weighted sum a probability times its value's scale is rounded to f16, or, with more than 64 rows
- * times heads a KV head, a probability to the queries' type (entries past 65504 then need bf16 queries). max_rows: most rows any sequence has (rows
+ * times heads a KV head, a probability to the queries' type (entries past 65504 then need bf16 queries). A NaN in a value
+ * makes the same dims of its group NaN in the rows that see it, one in a key all dims. max_rows: most rows any sequence has (rows
  * past it are not computed); 1 for single tokens. Page ids are held inside the pool. n_head a multiple of n_kv, at most 64
  * times it. Lengths may be smaller than a sequence's rows (the rows ahead see nothing). Partial results of keys go
  * through the workspace, 16-byte aligned. */
@@ -517,7 +518,7 @@ typedef struct b2_attention_4bit_args {
     int64_t q_row, q_head, out_row, out_head;
     int32_t max_rows, n_head, n_kv, head_dim;
     int32_t type;             /* B2_TYPE_F16 or _BF16 */
-    float scale;              /* > 0, usually 1 / sqrt(head_dim) */
+    float scale;              /* 2^-40 to 2^40, usually 1 / sqrt(head_dim) */
 } b2_attention_4bit_args;
 int b2_attention_4bit(int device, const b2_ragged_pages* where, const b2_attention_4bit_args* args, void* stream);
 /* bytes that a call with so many rows needs, whatever the lengths are */

@@ -13,7 +13,8 @@
 //   weighted sums: the operand of the values is again their codes alone, c 2^-24 and c 2^-20. A probability times the scale of its key's value, group by group, is the other, rounded
 //     to f16 once (2^-11), whatever the type of queries and output; the offset of 8 is a product of that operand and a constant. Scales are taken at a power of two that keeps the
 //     operand in f16's range, found from the scales as they come. Score fragments become operands by movmatrix.
-// The reference of a row's exponentials moves only where a score exceeds it by 2^6.
+// The reference of a row's exponentials moves only where a score exceeds it by 2^6. It is a score before it is scaled, so that the largest one's difference is exact however large it is (one
+// fused multiply-add with a scaled reference would save an instruction a score, and be off by as much as the reference's last place).
 #include "attention_4bit.cuh"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"
@@ -455,7 +456,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                         }
                         mx = fmaxf(fmaxf(mx, sc[b][nt][j]), sc[b][nt][j + 2]);
                     }
-                    above |= mx * by[nt][j] > ref[nt][j] + 6.f;
+                    above |= (mx - ref[nt][j]) * by[nt][j] > 6.f;
                 }
             if (__any_sync(0xffffffffu, above)) {
                 float fall_v = 1.f;
@@ -472,11 +473,10 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                         float mx = -INFINITY;
 #pragma unroll
                         for (int b = 0; b < KB; b++) mx = fmaxf(fmaxf(mx, sc[b][nt][j]), sc[b][nt][j + 2]);
-                        mx *= by[nt][j];
 #pragma unroll
                         for (int d = 4; d < 32; d *= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
                         mx = fmaxf(mx, ref[nt][j]);
-                        const float fall = a4_exp2(ref[nt][j] - mx);
+                        const float fall = a4_exp2((ref[nt][j] - mx) * by[nt][j]);
                         ref[nt][j] = mx;
                         l[nt][j] *= fall;
 #pragma unroll
@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        pr[nt][e] = a4_exp2(fmaf(sc[b][nt][e], by[nt][e & 1], -ref[nt][e & 1]));
+                        pr[nt][e] = a4_exp2((sc[b][nt][e] - ref[nt][e & 1]) * by[nt][e & 1]);
                         l[nt][e & 1] += pr[nt][e];
                     }
                 uint32_t w[2][NG];
@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 #pragma unroll
                     for (int gi = 0; gi < NG; gi++)
                         *reinterpret_cast<float4*>(part_at + row * D + gi * Q4_GROUP + 4 * g) = make_float4(o[nt][gi][0][j], o[nt][gi][0][j + 2], o[nt][gi][1][j], o[nt][gi][1][j + 2]);
-                    if (g == 0) *reinterpret_cast<float2*>(part_at + MT * D + row * 2) = make_float2(ref[nt][j], l[nt][j]);
+                    if (g == 0) *reinterpret_cast<float2*>(part_at + MT * D + row * 2) = make_float2(l[nt][j] == 0.f ? -INFINITY : ref[nt][j] * by[nt][j], l[nt][j]);
                 }
             }
         if (!(begins && ends) && lane == 0) {

@@ -486,11 +486,11 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                         for (int j = 0; j < 32; j += 2) mx4[j >> 1 & 3] = fmaxf(fmaxf(mx4[j >> 1 & 3], __uint_as_float(x[u][j])), __uint_as_float(x[u][j + 1]));
                     }
                 }
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * a.scale_log2;
-                const bool grow = mx > m_ref + 8.f || (m_ref == -INFINITY && mx > -INFINITY);
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+                const bool grow = (mx - m_ref) * a.scale_log2 > 8.f;      // (-inf less itself: no)
                 float fall = 1.f;
                 if (grow) {
-                    fall = t4_exp2(m_ref - mx);                  // (0 the first time)
+                    fall = t4_exp2((m_ref - mx) * a.scale_log2);      // (0 the first time)
                     m_ref = mx;
                     const uint64_t fall2 = f2_pack(fall, fall);
                     l2 = f2_mul(l2, fall2); l3 = f2_mul(l3, fall2);
@@ -520,7 +520,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                         uint32_t p[16];
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
-                            const float2 d = f2_unpack(f2_fma(f2_pack(__uint_as_float(x[u][j]), __uint_as_float(x[u][j + 1])), scale2, ref2));
+                            const float2 d = f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(x[u][j]), __uint_as_float(x[u][j + 1])), ref2), scale2));
                             const float e0 = t4_exp2(d.x), e1 = t4_exp2(d.y);
                             if (j & 2) l3 = f2_add(l3, f2_pack(e0, e1)); else l2 = f2_add(l2, f2_pack(e0, e1));
                             p[j >> 1] = t4_pack<F16>(e0, e1);
@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             }
             if (!whole) {
                 open[slot] = true;
-                if (in) *reinterpret_cast<float2*>(part + 2 * T4_ROWS * D + (t * T4_ROWS + (warp & 3) * 32 + lane) * 2) = make_float2(m_ref, l);
+                if (in) *reinterpret_cast<float2*>(part + 2 * T4_ROWS * D + (t * T4_ROWS + (warp & 3) * 32 + lane) * 2) = make_float2(m_ref * a.scale_log2, l);
                 if (t == 0 && warp == 0 && lane == 0) {
                     const long last = given + walk.steps - walk.b0 - 1, run = run_shared[0], longer = run_shared[1], most = longer * (run + 1);
                     desc[slot] = {n_f, r0, walk.seg_f0, walk.seg_kvh, (int)(last < most ? last / (run + 1) : longer + (last - most) / run)};

@@ -193,7 +193,8 @@ extern "C" int b2_attention_4bit(int device, const b2_ragged_pages* where, const
     if (a.type != ELEM_F16 && a.type != ELEM_BF16) return b2_fail(B2_ERR_UNSUPPORTED, "b2_attention_4bit: queries must be f16 or bf16");
     if (x->max_rows <= 0) return bad(what, "max_rows must be positive");
     if ((int64_t)where->n_rows * x->n_head > INT32_MAX || (int64_t)x->max_rows * x->n_head > INT32_MAX) return bad(what, "rows * n_head must fit 32 bits");
-    if (!(x->scale > 0.f) || !isfinite(x->scale)) return bad(what, "scale must be positive and finite");
+    // (scale times the power of two that queries are held at, 2^-86 at least, stays a normal number)
+    if (!(x->scale >= 0x1p-40f && x->scale <= 0x1p40f)) return bad(what, "scale must be between 2^-40 and 2^40");
     if (where->n_rows == 0 || where->n_seqs == 0) return B2_OK;
     if (!x->q || !x->k_pool || !x->v_pool || !x->out || !x->workspace) return bad(what, "null device pointer");
     if (((uintptr_t)x->k_pool | (uintptr_t)x->v_pool | (uintptr_t)x->workspace) & 15) return bad(what, "the pools and the workspace must be 16-byte aligned");

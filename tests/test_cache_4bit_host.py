@@ -110,7 +110,7 @@ READ_REFUSALS = WHERE_REFUSALS + [(dict(out_type=2), "f32, f16 or bf16"), (dict(
                                   (dict(k_pool=None), "null"), (dict(v_pool=None), "null"), (dict(k_pool=72), "16-byte"), (dict(v=65), "aligned")]
 ATTENTION_REFUSALS = WHERE_REFUSALS + [
     (dict(head_dim=96), "head_dim"), (dict(n_head=5), "multiple"), (dict(n_kv=0), "multiple"), (dict(n_head=130), "64 heads"), (dict(type=0), "f16 or bf16"), (dict(max_rows=0), "max_rows"),
-    (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(n_rows=2 ** 30), "32 bits"), (dict(max_rows=2 ** 30), "32 bits"), (dict(q=None), "null"),
+    (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=2.0 ** -41), "scale"), (dict(scale=1.1 * 2 ** 40), "scale"), (dict(scale=-1.0), "scale"), (dict(n_rows=2 ** 30), "32 bits"), (dict(max_rows=2 ** 30), "32 bits"), (dict(q=None), "null"),
     (dict(workspace=None), "null"), (dict(v_pool=None), "null"), (dict(k_pool=72), "16-byte"), (dict(workspace=72), "16-byte"), (dict(q=65), "aligned"), (dict(out=65), "aligned"),
     (dict(workspace_bytes=100), "workspace holds 100 bytes")]
 

@@ -310,6 +310,74 @@ def test_attention_sizes_of_values(ops, heads, rows, dim):
     assert ((got.to(F64) - want).abs() <= attention_bar("bf16", want, *sizes, dim, max(rows) * heads // 4 > 64)).all()
 
 
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,rows", WAYS)
+def test_attention_ends_of_the_scale(ops, heads, rows, typ):
+    """the smallest and the largest scale: even weights, and all weight on the largest score; queries of zero: even weights whatever the scale"""
+    own = [n + 40 for n in rows]
+    c = Cache4(10, 2, 64, 16, own)
+    q = torch.randn(sum(rows), heads, 64, generator=c.g).to(TYPES[typ]).cuda()
+    q[::2, ::3] = 0.0
+    for scale in (2.0 ** -40, 2.0 ** 40):
+        got = attend(ops, c, q, rows, scale=scale)
+        want, *sizes = attention_exact(c, q, rows, scale=scale)
+        assert torch.isfinite(got).all()
+        near = (got.to(F64) - want).abs() <= attention_bar(typ, want, *sizes, 64, max(rows) * heads // 2 > 64)
+        assert near.all()
+        if scale > 1:
+            # scores of 2^40 and more, whose two largest are apart by more than their errors: the largest one's value
+            k, v = c.values(c.k), c.values(c.v)
+            r0 = 0
+            for s, n in enumerate(rows):
+                for i in range(n):
+                    at = slice(c.start[s], c.start[s] + own[s] - n + i + 1)
+                    for h in range(heads):
+                        top = (k[at, h // (heads // 2)] @ q[r0 + i, h].to(F64)).topk(2)
+                        if top.values[0] - top.values[1] > 2 ** -6 * top.values[0].abs():
+                            one = v[at, h // (heads // 2)][top.indices[0]]
+                            assert ((got[r0 + i, h].to(F64) - one).abs() <= 2 ** -7 * one.abs() + 2 ** -20).all()
+                r0 += n
+
+
+@pytest.mark.parametrize("heads,rows", WAYS)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_largest_f16_entries(ops, heads, rows, dim):
+    """keys and values up to f16's largest number, in f16"""
+    own = [n + 50 for n in rows]
+    c0 = Cache4(11, 2, dim, 16, own)
+    k, v = c0.k.float(), c0.v.float()
+    k[:, 1] = (k[:, 1] * 2e4).clamp(-65504, 65504)
+    v[::3, 0, :32] = (v[::3, 0, :32] * 3e4).clamp(-65504, 65504)
+    v[5::7, 1] = 65504.0
+    k[7::9, 0, 32:] *= 3e3
+    c = Cache4(11, 2, dim, 16, own, k=k.half(), v=v.half())
+    q = torch.randn(sum(rows), heads, dim, generator=c.g)
+    q[:, heads // 2:] *= 1e-4
+    q[:, :heads // 2, 32:] *= 1e-3
+    q = q.half().cuda()
+    got = attend(ops, c, q, rows)
+    want, sizes = visible_nan(c, q, rows, c.values(c.k), c.values(c.v))      # (one of the keys is past it)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and not torch.isinf(got).any()
+    near = (got.to(F64) - want).abs() <= attention_bar("f16", torch.nan_to_num(want), *sizes, dim, max(rows) * heads // 2 > 64)
+    assert (near | torch.isnan(want)).all()
+
+
+@pytest.mark.parametrize("heads,kv,dim,page,rows,own", [
+    (16, 8, 64, 64, [1] * 64, [1500 + 20 * i for i in range(64)]),                  # long runs: warps that have more of it than others
+    (8, 2, 128, 64, [1 + i % 3 for i in range(300)], [i * 7 % 150 for i in range(300)]),      # more sequences than a CTA keeps; rows that see nothing
+    (32, 8, 128, 32, [300, 0, 1, 40, 700], [3000, 0, 1, 1700, 700]),                # units over several CTAs, several units a CTA
+    (32, 2, 64, 16, [1 + i % 37 for i in range(70)], [1 + i % 37 + 11 * i % 90 for i in range(70)]),      # many short prompts
+    (64, 1, 64, 16, [1100], [1500]),                                                # units of four rows
+])
+def test_attention_many(ops, heads, kv, dim, page, rows, own):
+    c = Cache4(sum(own), kv, dim, page, own)
+    q = torch.randn(sum(rows), heads, dim, generator=c.g).half().cuda()
+    got = attend(ops, c, q, rows)
+    want, *sizes = attention_exact(c, q, rows)
+    assert ((got.to(F64) - want).abs() <= attention_bar("f16", want, *sizes, dim, max(rows) * heads // kv > 64)).all()
+    assert torch.equal(got, attend(ops, c, q, rows)) and ops.error(0) == 0
+
+
 @pytest.mark.parametrize("heads,rows", WAYS)
 @pytest.mark.parametrize("at,by", [([0], 30.0), ([40], 20.0), ([33, 66, 99, 130], 15.0), ([131, 132], 40.0), ([64], -20.0)])
 def test_attention_scores_that_grow(ops, heads, rows, at, by):
