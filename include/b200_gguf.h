@@ -539,7 +539,8 @@ int b2_token_logprobs(int device, const void* logits, int type, int64_t row_stri
  * that this was asked (0: none; results of the calls in between are not to be used). Waits for all work on the device, so
  * not while a stream is being captured. */
 int b2_device_op_error(int device, uint32_t* code);
-/* For tests: enqueue what a wait that ran out leaves behind (the words of one of two files), without the wait. */
+/* For tests: enqueue what a wait that ran out leaves behind, without the wait (tensor_memory 0 and 1: the words of shared
+ * prefixes, 2 and 3: of the cache in 4 bits; 1 and 3 those of the kernels on tensor memory). */
 int b2_op_give_up(int device, int tensor_memory, uint32_t code, void* stream);
 
 #ifdef __cplusplus

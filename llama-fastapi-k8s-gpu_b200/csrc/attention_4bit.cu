@@ -732,6 +732,10 @@ cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s) {
     return few ? a4_step<128, 1>(a, s) : a4_step<128, 2>(a, s);
 }
 
+namespace { __global__ void a4_give_up_kernel(unsigned int code) { mbar_give_up(0, a4_error, code, 0); } }
+cudaError_t attention_4bit_give_up(unsigned int code, bool tensor_memory, cudaStream_t s) {
+    return tensor_memory ? attention_4bit_tc_give_up(code, s) : launch_chain(a4_give_up_kernel, dim3(1), dim3(1), 0, s, code);
+}
 cudaError_t attention_4bit_error(unsigned int* code) {
     unsigned int more = 0;
     cudaError_t e = take_error_word(a4_error, code);

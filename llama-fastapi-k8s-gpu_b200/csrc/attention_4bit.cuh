@@ -36,5 +36,6 @@ cudaError_t attention_4bit_join(const Attention4Args& a, int ctas, int rows, cud
 size_t attention_4bit_tc_work_bytes(int head_dim);
 cudaError_t attention_4bit_tc_launch(const Attention4Args& a, cudaStream_t s);
 cudaError_t attention_4bit_tc_error(unsigned int* code);
+cudaError_t attention_4bit_tc_give_up(unsigned int code, cudaStream_t s);
 
 }  // namespace b2

@@ -601,6 +601,8 @@ cudaError_t attention_4bit_tc_launch(const Attention4Args& a, cudaStream_t s) {
     if (a.head_dim == 64) return a.type == ELEM_F16 ? t4_launch<64, true>(a, s) : t4_launch<64, false>(a, s);
     return a.type == ELEM_F16 ? t4_launch<128, true>(a, s) : t4_launch<128, false>(a, s);
 }
+namespace { __global__ void t4_give_up_kernel(unsigned int code) { mbar_give_up(0, t4_error, code, 0); } }
+cudaError_t attention_4bit_tc_give_up(unsigned int code, cudaStream_t s) { return launch_chain(t4_give_up_kernel, dim3(1), dim3(1), 0, s, code); }
 cudaError_t attention_4bit_tc_error(unsigned int* code) { return take_error_word(t4_error, code); }
 
 }  // namespace b2

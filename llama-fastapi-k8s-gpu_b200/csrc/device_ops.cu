@@ -221,5 +221,6 @@ extern "C" int b2_device_op_error(int device, uint32_t* code) {
 
 extern "C" int b2_op_give_up(int device, int tensor_memory, uint32_t code, void* stream) {
     OnDevice on(device);
-    return done("b2_op_give_up", on.status != cudaSuccess ? on.status : shared_prefix_give_up(code, tensor_memory != 0, (cudaStream_t)stream));
+    return done("b2_op_give_up", on.status != cudaSuccess ? on.status : tensor_memory >= 2 ? attention_4bit_give_up(code, tensor_memory != 2, (cudaStream_t)stream) :
+                                     shared_prefix_give_up(code, tensor_memory != 0, (cudaStream_t)stream));
 }

@@ -85,6 +85,7 @@ struct Attention4Args {
 size_t attention_4bit_work_bytes(long n_rows, int n_head, int n_kv, int head_dim);
 cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s);
 cudaError_t attention_4bit_error(unsigned int* code);            // code of the first wait that ran out (does not wait), see shared_prefix_error
+cudaError_t attention_4bit_give_up(unsigned int code, bool tensor_memory, cudaStream_t s);      // see shared_prefix_give_up
 
 // ---------------------------------------------------------------- logprobs.cu
 constexpr int LOGPROB_MAX_TOP = 64;

@@ -619,6 +619,17 @@ def test_two_streams_at_once(ops):
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("words", [2, 3])
+def test_a_wait_that_ran_out_is_reported_once(ops, native_lib, words):
+    side = torch.cuda.Stream()
+    assert ops.error(0) == 0
+    assert native_lib.b2_op_give_up(0, words, 0xb0001, side.cuda_stream) == 0 and native_lib.b2_op_give_up(0, words, 0x77, side.cuda_stream) == 0
+    assert ops.error(0) == 0xb0001 and ops.error(0) == 0
+    for other in (0, 1, 2, 3):                                          # all files' words are taken at once
+        assert native_lib.b2_op_give_up(0, other, 0x11 + other, None) == 0
+    assert ops.error(0) == 0x11 and ops.error(0) == 0
+
+
 def test_empty_calls(ops):
     c = Cache4(9, 2, 64, 16, [5])
     none = torch.zeros(0, 4, 64, dtype=torch.float16, device="cuda")
