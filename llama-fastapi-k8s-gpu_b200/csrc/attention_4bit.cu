@@ -65,10 +65,17 @@ template <int NG> __device__ __forceinline__ void a4_chunk(const uint8_t* p, uin
     else { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
 }
 
+// a token's scales, two a word
+template <int NG> __device__ __forceinline__ void a4_scale_words(const uint8_t* p, uint32_t (&w)[NG / 2]) {
+    if constexpr (NG == 4) { const uint2 v = *reinterpret_cast<const uint2*>(p); w[0] = v.x; w[1] = v.y; }
+    else w[0] = *reinterpret_cast<const uint32_t*>(p);
+}
 template <int NG> __device__ __forceinline__ void a4_scales(const uint8_t* p, float (&s)[NG]) {
+    uint32_t w[NG / 2];
+    a4_scale_words<NG>(p, w);
 #pragma unroll
     for (int gi = 0; gi < NG; gi += 2) {
-        const float2 v = __half22float2(reinterpret_cast<const __half2*>(p)[gi >> 1]);
+        const float2 v = __half22float2(a4_as_half2(w[gi >> 1]));
         s[gi] = v.x; s[gi + 1] = v.y;
     }
 }
@@ -431,10 +438,11 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             for (int b = 0; b < KB; b++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const __half2* from = reinterpret_cast<const __half2*>(stage + v_scale + b * BLOCK + h * 8 * NG * 2);
+                    uint32_t two[NG / 2];
+                    a4_scale_words<NG>(stage + v_scale + b * BLOCK + h * 8 * NG * 2, two);
 #pragma unroll
                     for (int gi = 0; gi < NG; gi += 2) {
-                        __half2 v = from[gi >> 1];
+                        __half2 v = a4_as_half2(two[gi >> 1]);
                         if (PARTLY && t0 + b * 16 + g + 8 * h >= own) v = a4_as_half2(0);      // (whatever lies there)
                         most = __hmax2(most, __habs2(v));
                     }
