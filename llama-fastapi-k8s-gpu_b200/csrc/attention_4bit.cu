@@ -15,6 +15,9 @@
 //     operand in f16's range, found from the scales as they come. Score fragments become operands by movmatrix.
 // The reference of a row's exponentials moves only where a score exceeds it by 2^6. It is a score before it is scaled, so that the largest one's difference is exact however large it is (one
 // fused multiply-add with a scaled reference would save an instruction a score, and be off by as much as the reference's last place).
+// Measured (32 heads over 8 of 128, f16): 256 chats of 16 to 4100 tokens 160 us, 3.8 TB/s of what has to be read, 0.58 of a copy's; 32 chats of 20 to 1500 19, one of 32000 20.7, of 700 10.6. A step is some 600
+// instructions, issued one in two cycles by the twelve warps that fit an SM. More CTAs than fit (184 to 206 us for the 256 chats), four an SM with 128 registers (170), and the next step's scores beside
+// this one's values (173 where it was 159) were slower, products in other orders the same.
 #include "attention_4bit.cuh"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"

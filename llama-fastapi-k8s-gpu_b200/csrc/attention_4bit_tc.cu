@@ -8,7 +8,7 @@
 //
 // A value s (c - 8) has up to 14 bits, an f16 or bf16 operand 11 or 8. Rounded, keys would be off by 2^-12 each, and a score by more than all else together (relative error of the output
 // 3.5e-4 from the keys alone, 1.8e-4 from the values, where the output's own rounding to f16 is 2.1e-4). So keys and values are two operands each, exact to 2^-14 or better: with the upper
-// bits of the scale, and with the rest of it. That doubles the products, which then are what this is bound by: 2048 rows behind 6000 tokens, 32 heads over 8 of 128, 389 us, 605 TFLOP/s of
+// bits of the scale, and with the rest of it. That doubles the products, which then are what this is bound by: 2048 rows behind 6000 tokens, 32 heads over 8 of 128, 366 us, 643 TFLOP/s of
 // what is asked for and twice as much of what is done. Probabilities are rounded to the queries' type.
 #include "attention_4bit.cuh"
 #include "kv_4bit.cuh"
@@ -341,7 +341,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
     } else if (warp >= 8) {
         // ================= codes into operands: keys 64 dims at a time, values 64 keys at a time, by all eight warps. What a warp is to write is ready before its place is free.
         // (The tensor cores take 70 % of the time, and reading operands beside the warps that write them makes their products a fifth longer. Neither warps of their own for keys and values nor
-        // the second tile's product ahead of the first one's next scores where it is ready first made it faster: 395 us instead of 389 for 2048 rows behind 6000.)
+        // the second tile's product ahead of the first one's next scores where it is ready first made it faster: a hundredth slower for 2048 rows behind 6000.)
         t4_fewer_registers<T4_REG_OPERANDS>();
         const int dw = warp & 7, eight = lane & 7;               // (eight neighbouring lanes: keys that follow one another; a lane has the 32 dims of a group)
         auto put = [&](uint8_t* row, int key, int g, const uint4 (&hi)[4], const uint4 (&lo)[4]) {
