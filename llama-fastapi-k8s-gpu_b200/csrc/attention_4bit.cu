@@ -62,6 +62,22 @@ __device__ __forceinline__ uint32_t a4_transpose(uint32_t v) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+// by one lane of the warp: keys and values to two places, told to the barrier (`EXPECT`: with all the bytes that it is to wait for); every operand the same in all lanes
+template <bool EXPECT>
+__device__ __forceinline__ void a4_copy(uint32_t bar, uint32_t all, uint32_t to_k, uint32_t to_v, const void* k, const void* v, uint32_t bytes) {
+    if constexpr (EXPECT)
+        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t"
+                     "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%2], [%4], %6, [%0];\n\t"
+                     "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%3], [%5], %6, [%0];\n\t}"
+                     ::"r"(bar), "r"(all), "r"(to_k), "r"(to_v), "l"(k), "l"(v), "r"(bytes) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%1], [%3], %5, [%0];\n\t"
+                     "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%2], [%4], %5, [%0];\n\t}"
+                     ::"r"(bar), "r"(to_k), "r"(to_v), "l"(k), "l"(v), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void a4_no_copy(uint32_t bar) {
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t@e mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar) : "memory");
+}
 // chunks of a block's row: 16 bytes for heads of 128, 8 for heads of 64
 template <int NG> __device__ __forceinline__ void a4_chunk(const uint8_t* p, uint32_t (&w)[NG]) {
     if constexpr (NG == 4) { const uint4 v = *reinterpret_cast<const uint4*>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
@@ -273,31 +289,39 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
         start.step = (int)max(rest - A4_BEGIN, 0l);
     }
 
-    // ---- copies: a lane has keys or values of one of the step's blocks, the page's id read a step ahead
+    static_assert(KB == 2, "a page ends at most once in a step");
+    // ---- copies: by one lane, a step's keys and its values (neighbours in their page; two copies each where a page ends between), the page's id read a step ahead. Everything they
+    // need is the same in all lanes.
     if (lane == 0) { at = start; ahead = start; }
-    int to_copy = (int)max(u1 - first, 0l), id = 0, in_page = 0, put = 0;      // units of the run from the next copy on
+    int to_copy = (int)max(u1 - first, 0l), id = 0, id_2 = 0, in_page = 0, put = 0;      // units of the run from the next copy on; pages of the step's blocks
     int c_step = start.step, c_steps = start.s.steps, c_own = start.s.own;     // of the copies' segment
-    const int c_kv = lane >= KB, c_blk = lane - c_kv * KB;
     const long per_head = (long)blocks * BLOCK, per_page = n_kv * per_head;
-    const uint8_t* const pool = (const uint8_t*)(c_kv ? a.v_pool : a.k_pool);
-    const uint8_t* from_head = pool + start.kvh * per_head;
+    long from_head = start.kvh * per_head;
     const int* table = a.r.pages + start.z * a.r.table_stride;
     auto read_id = [&]() {
-        const unsigned b = c_step * KB + c_blk;                  // block of the sequence
+        const unsigned b = c_step * KB;                          // block of the sequence
         unsigned page = __umulhi(b, a.per_page);                 // the quotient by the page's blocks, or one less
         in_page = (int)(b - page * blocks);
         if (in_page >= blocks) { page++; in_page -= blocks; }
-        id = lane < 2 * KB && to_copy > 0 && (int)b * Q4_TOKENS < c_own ? table[page] : 0;
+        if (to_copy <= 0 || (int)b * Q4_TOKENS >= c_own) return;
+        id = table[page];
+        if (in_page + 1 == blocks && (int)(b + 1) * Q4_TOKENS < c_own) id_2 = table[page + 1];
     };
     read_id();
     __syncwarp();
     auto copy = [&]() {
         if (to_copy <= 0) return;
-        const int n = min(KB, (c_own - c_step * A4_KEYS + Q4_TOKENS - 1) / Q4_TOKENS);
-        if (lane == 0) mbar_arrive_expect_tx(&full[warp][put], (uint32_t)(max(n, 0) * 2 * BLOCK));
-        __syncwarp();
-        if (lane < 2 * KB && c_blk < n)
-            tma_load_1d(ring + put * STAGE + lane * BLOCK, from_head + min(max(id, 0), last_page) * per_page + in_page * BLOCK, BLOCK, &full[warp][put]);
+        const int n = min(KB, (c_own - c_step * A4_KEYS + Q4_TOKENS - 1) / Q4_TOKENS), here = in_page + 1 == blocks ? min(n, 1) : n;      // blocks, those of the first page
+        const uint32_t bar = smem_u32(&full[warp][put]), to = smem_u32(ring + put * STAGE);
+        if (n <= 0) a4_no_copy(bar);
+        else {
+            const long from = from_head + min(max(id, 0), last_page) * per_page + in_page * BLOCK;
+            a4_copy<true>(bar, (uint32_t)(n * 2 * BLOCK), to, to + KB * BLOCK, (const uint8_t*)a.k_pool + from, (const uint8_t*)a.v_pool + from, (uint32_t)(here * BLOCK));
+            if (here < n) {
+                const long from_2 = from_head + min(max(id_2, 0), last_page) * per_page;
+                a4_copy<false>(bar, 0, to + BLOCK, to + (KB + 1) * BLOCK, (const uint8_t*)a.k_pool + from_2, (const uint8_t*)a.v_pool + from_2, BLOCK);
+            }
+        }
         __syncwarp();
         put = put + 1 == S ? 0 : put + 1;
         to_copy--;
@@ -307,7 +331,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             if (lane == 0) ahead.next(a, MT);
             __syncwarp();
             c_steps = ahead.s.steps; c_own = ahead.s.own;
-            from_head = pool + ahead.kvh * per_head;
+            from_head = ahead.kvh * per_head;
             table = a.r.pages + ahead.z * a.r.table_stride;
             // its queries, on their way into the L1 cache
             const int f0 = ahead.tile * MT, row = lane >> 1;
