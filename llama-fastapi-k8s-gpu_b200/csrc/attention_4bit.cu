@@ -54,9 +54,6 @@ __device__ __forceinline__ void a4_mma_from(float (&d)[4], const float (&c)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
-// a value that stays in a register of its own (fragments are neighbouring registers: made anew before every product, they cost a move each)
-__device__ __forceinline__ float a4_keep(float v) { float r; asm volatile("mov.b32 %0, %1;" : "=f"(r) : "f"(v)); return r; }
-__device__ __forceinline__ uint32_t a4_keep(uint32_t v) { uint32_t r; asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v)); return r; }
 __device__ __forceinline__ uint32_t a4_transpose(uint32_t v) {
     uint32_t r;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
@@ -243,7 +240,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
     A4At& at = places[warp][0];
     A4At& ahead = places[warp][1];
     A4At start;
-    start.z = n_seqs; start.kvh = start.tile = start.step = 0;
+    start.z = n_seqs; start.kvh = start.tile = start.step = start.s.own = start.s.steps = start.s.tiles = 0;
     long first = u0;                                             // the first unit that is a step
     if (u0 < u1) {
         long rest = 0;
@@ -346,10 +343,11 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
     };
     for (int i = 0; i < S; i++) copy();
 
-    const uint32_t less[4] = {a4_keep(0x80088008u), a4_keep(0x80808080u), a4_keep(0x80088008u), a4_keep(0x80808080u)};      // -8 2^-24 and -8 2^-20
+    // -8 2^-24 and -8 2^-20. Not as constants: fragments are neighbouring registers, and constants would be moved there anew for every product
+    const uint32_t zero = (uint32_t)a.few_units >> 1, less[4] = {0x80088008u + zero, 0x80808080u + zero, 0x80088008u + 2 * zero, 0x80808080u + 2 * zero};
     // where a lane's chunks and scales lie in a step: key g of a block (the one 8 further on is turned alike), pair tq of the values
-    const uint32_t k_from = a4_keep((uint32_t)(g * (D / 2) + q4_key_chunk(D, g, tq) * NG * 4)), k_scale = a4_keep((uint32_t)q4_scale(D, g, 0));
-    const uint32_t v_from = a4_keep((uint32_t)(KB * BLOCK + tq * D + q4_value_chunk(D, tq, g) * NG * 4)), v_scale = k_scale + KB * BLOCK;
+    const uint32_t k_from = (uint32_t)(g * (D / 2) + q4_key_chunk(D, g, tq) * NG * 4), k_scale = (uint32_t)q4_scale(D, g, 0);
+    const uint32_t v_from = (uint32_t)(KB * BLOCK + tq * D + q4_value_chunk(D, tq, g) * NG * 4), v_scale = k_scale + KB * BLOCK;
     int st = 0;
     uint32_t parity = 0;
     for (long u = first; u < u1;) {
@@ -409,9 +407,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-                for (int j = 0; j < 2; j++) off[nt][gi][j] = a4_keep(__shfl_sync(0xffffffffu, sum, (2 * tq + j) * 4) * -0x1p-21f);      // 8 2^-24
-#pragma unroll
-                for (int j = 0; j < 2; j++) off[nt][gi][j + 2] = a4_keep(off[nt][gi][j]);
+                for (int e = 0; e < 4; e++) off[nt][gi][e] = __shfl_sync(0xffffffffu, sum, (2 * tq + (e & 1)) * 4 + (e >> 1)) * -0x1p-21f;      // 8 2^-24 (from different lanes, which have the same)
             }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -420,8 +416,9 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             }
         }
         const int own = s.own, lim_lo = min(s.limit(f0 / G), own);                       // keys that all rows of the tile see
-        // weighted sums, 2^24 (even dims) and 2^20 (odd) over `up_v` times too small; references of the exponentials; sums
-        float o[NT][NG][2][4], ref[NT][2], l[NT][2], up_v = 0x1p120f;
+        // weighted sums, 2^24 (even dims) and 2^20 (odd) times too small, and sums; both times 2^up_v, which goes down where a value's scale exceeds most_v, 2^(9 - up_v); references of the
+        // exponentials
+        float o[NT][NG][2][4], ref[NT][2], l[NT][2], up_v = 30.f, most_v = 0x1p-21f;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             ref[nt][0] = ref[nt][1] = -FLT_MAX; l[nt][0] = l[nt][1] = 0.f;
@@ -477,7 +474,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             const float2 most2 = __half22float2(most);
             const float top_v = fmaxf(most2.x, most2.y);
             // ---- differences to the references, which go up where a score is far above them (as the values' power of two goes down where a scale is)
-            bool above = top_v * up_v > 512.f;
+            bool above = top_v > most_v;
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -496,10 +493,11 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             if (__any_sync(0xffffffffu, above)) {
                 float fall_v = 1.f;
                 const float all_v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)));
-                if (all_v * up_v > 512.f) {
-                    const float now = __uint_as_float((uint32_t)(133 - max((int)(__float_as_uint(all_v) >> 23) - 127, -24)) << 23);      // all_v * now in [64, 128)
-                    fall_v = now / up_v;                         // (powers of two; 2^-80 or less the first time, of sums that are 0)
-                    up_v = now;
+                if (all_v > most_v) {
+                    const int e = min((int)(__float_as_uint(all_v) >> 23) - 127, 16);    // all_v * 2^(6 - e) in [64, 128)
+                    fall_v = a4_exp2(6 - e - up_v);
+                    up_v = 6 - e;
+                    most_v = __uint_as_float((uint32_t)(130 + e) << 23);
                 }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -513,7 +511,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                         mx = fmaxf(mx, ref[nt][j]);
                         const float fall = a4_exp2((ref[nt][j] - mx) * by[nt][j]);
                         ref[nt][j] = mx;
-                        l[nt][j] *= fall;
+                        l[nt][j] *= fall * fall_v;
 #pragma unroll
                         for (int gi = 0; gi < NG; gi++)
 #pragma unroll
@@ -529,7 +527,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        pr[nt][e] = a4_exp2((sc[b][nt][e] - ref[nt][e & 1]) * by[nt][e & 1]);
+                        pr[nt][e] = a4_exp2(fmaf(sc[b][nt][e] - ref[nt][e & 1], by[nt][e & 1], up_v));
                         l[nt][e & 1] += pr[nt][e];
                     }
                 uint32_t w[2][NG];
@@ -542,7 +540,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 #pragma unroll
                 for (int gi = 0; gi < NG; gi++) {
                     const uint32_t x = w[0][gi], y = w[1][gi], x8 = x >> 8, y8 = y >> 8;
-                    const float s0 = vs[0][gi] * up_v, s1 = vs[1][gi] * up_v;
+                    const float s0 = vs[0][gi], s1 = vs[1][gi];
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
                         float z[4] = {pr[nt][0] * s0, pr[nt][1] * s0, pr[nt][2] * s1, pr[nt][3] * s1};
@@ -569,7 +567,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             if (++st == S) { st = 0; parity ^= 1; }
         }
         // the sums as they are
-        const float down_v = 0x1p24f / up_v;
+        const float by_l = a4_exp2(-up_v), down_v = by_l * 0x1p24f;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -585,6 +583,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             for (int j = 0; j < 2; j++)
 #pragma unroll
                 for (int d = 4; d < 32; d *= 2) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) { l[nt][0] *= by_l; l[nt][1] *= by_l; }
         // ---- output, or a result for the joins
         const int slot = begins ? 1 : 0;
         float* part_at = begins ? reinterpret_cast<float*>(ring) : head_part + warp * PART;      // (a segment that goes on is the run's last: no copy is under way)
