@@ -452,7 +452,11 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                         a4_mma_from(c, off[nt][gi], x & 0x000f000fu, y & 0x000f000fu, x & 0x00f000f0u, y & 0x00f000f0u, qb[nt][gi][0], qb[nt][gi][1]);
                         a4_mma(c, x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u, qb[nt][gi][2], qb[nt][gi][3]);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) sc[b][nt][e] = gi ? fmaf(ks[e >> 1][gi], c[e], sc[b][nt][e]) : ks[e >> 1][gi] * c[e];
+                        for (int h = 0; h < 2; h++) {
+                            const uint64_t k2 = f2_pack(ks[h][gi], ks[h][gi]), c2 = f2_pack(c[2 * h], c[2 * h + 1]);
+                            const float2 t = f2_unpack(gi ? f2_fma(k2, c2, f2_pack(sc[b][nt][2 * h], sc[b][nt][2 * h + 1])) : f2_mul(k2, c2));
+                            sc[b][nt][2 * h] = t.x; sc[b][nt][2 * h + 1] = t.y;
+                        }
                     }
                 }
             }
@@ -543,7 +547,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                     const float s0 = vs[0][gi], s1 = vs[1][gi];
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++) {
-                        float z[4] = {pr[nt][0] * s0, pr[nt][1] * s0, pr[nt][2] * s1, pr[nt][3] * s1};
+                        const float2 za = f2_unpack(f2_mul(f2_pack(pr[nt][0], pr[nt][1]), f2_pack(s0, s0))), zb = f2_unpack(f2_mul(f2_pack(pr[nt][2], pr[nt][3]), f2_pack(s1, s1)));
+                        float z[4] = {za.x, za.y, zb.x, zb.y};
                         if constexpr (PARTLY) {                  // (a scale that is no number must not reach rows that do not see its key)
 #pragma unroll
                             for (int e = 0; e < 4; e++) if (sc[b][nt][e] == -INFINITY) z[e] = 0.f;
