@@ -107,7 +107,7 @@ struct A4Seq {
         n = min(all, a.max_rows);
         own = min(max(held, 0), a.r.max_pages * a.r.block_tokens);
         lim0 = own - all + 1;
-        tiles = (n * (a.n_head / a.n_kv) + mt - 1) / mt;
+        tiles = (n * a.group + mt - 1) / mt;
         steps = n ? max(1, (own + A4_KEYS - 1) / A4_KEYS) : 0;
     }
     __device__ long units(int n_kv) const { return steps ? (long)(n_kv * tiles) * (steps + A4_BEGIN) : 0; }
@@ -134,10 +134,10 @@ struct A4Cut {
     long begin, run, longer;                                     // of a group: first unit, units of a run, runs that have one more
     int group, per;                                              // its number, warps of a group
     static constexpr long LONG_RUN = 16;
-    __device__ static long first(long total, int groups, int group) {      // first unit of a group: shares 36 : 32 : 28
-        return groups == 3 ? total * (group == 0 ? 0 : group == 1 ? 36 : group == 2 ? 68 : 96) / 96 : group ? total : 0;
+    __device__ static long first(long total, int groups, int group) {      // first unit of a group: shares 48 : 43 : 37
+        return groups == 3 ? total * (group == 0 ? 0 : group == 1 ? 48 : group == 2 ? 91 : 128) / 128 : group ? total : 0;
     }
-    __device__ A4Cut(const Attention4Args& a, long total, long warps, int groups, int g) : group(g), per((int)(warps / groups)) {
+    __device__ A4Cut(const Attention4Args& a, long total, int warps, int groups, int g) : group(g), per(groups == 3 ? A4_SMS * A4_WARPS : warps) {
         begin = first(total, groups, g);
         const long n = first(total, groups, g + 1) - begin;
         run = !n ? 0 : a.few_units ? (long)((unsigned)n / (unsigned)per) : n / per;      // (a division in 64 bits takes a hundred instructions)
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
     griddep_wait();
     griddep_launch();
     __syncwarp();
-    const int n_kv = a.n_kv, G = a.n_head / n_kv, blocks = a.r.block_tokens / Q4_TOKENS, last_page = (int)a.r.n_pages - 1;
+    const int n_kv = a.n_kv, G = a.group, blocks = a.r.block_tokens / Q4_TOKENS, last_page = (int)a.r.n_pages - 1;
 
     // ---- the units of all sequences, and this warp's run [u0, u1) of them. Up to 256 sequences are read once a CTA and kept. (All CTAs read the same few lines, one after the other.)
     constexpr int KEPT = 256;
@@ -227,13 +227,13 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 #pragma unroll
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
-    const long all_warps = (long)gridDim.x * A4_WARPS, warps = min(all_warps, total), me = (long)blockIdx.x * A4_WARPS + warp;
+    const int all_warps = gridDim.x * A4_WARPS, warps = (int)min((long)all_warps, total), me = blockIdx.x * A4_WARPS + warp;
     const int groups = total >= all_warps * A4Cut::LONG_RUN && a4_per_sm(NT) == 3 && (int)gridDim.x == A4_SMS * 3 ? 3 : 1;
     const int group = groups > 1 ? blockIdx.x / A4_SMS : 0;
     long u0 = 0, u1 = 0;
     if (me < warps) {
         const A4Cut cut(a, total, warps, groups, group);
-        const int i = (int)me - group * cut.per;
+        const int i = me - group * cut.per;
         u0 = cut.at(i); u1 = cut.at(i + 1);
     }
     __shared__ A4At places[A4_WARPS][2];                         // where the warp is, and where its copies are (few registers: they change once a segment)
@@ -295,6 +295,14 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
     const long per_head = (long)blocks * BLOCK, per_page = n_kv * per_head;
     long from_head = start.kvh * per_head;
     const int* table = a.r.pages + start.z * a.r.table_stride;
+    // a segment's queries, on their way into the L1 cache
+    auto fetch_queries = [&](const A4At& p) {
+        const int f0 = p.tile * MT, row = lane >> 1;
+        if (row >= min((long)MT, (long)p.s.n * G - f0)) return;
+        const int f = f0 + row, i = a4_row(a, f);
+        const uint16_t* q = (const uint16_t*)a.q + (size_t)(p.s.r0 + i) * a.q_row + (size_t)(p.kvh * G + f - i * G) * a.q_head + (lane & 1) * (D / 2);
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
+    };
     auto read_id = [&]() {
         const unsigned b = c_step * KB;                          // block of the sequence
         unsigned page = __umulhi(b, a.per_page);                 // the quotient by the page's blocks, or one less
@@ -305,6 +313,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
         if (in_page + 1 == blocks && (int)(b + 1) * Q4_TOKENS < c_own) id_2 = table[page + 1];
     };
     read_id();
+    if (to_copy > 0) fetch_queries(start);
     __syncwarp();
     auto copy = [&]() {
         if (to_copy <= 0) return;
@@ -330,13 +339,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             c_steps = ahead.s.steps; c_own = ahead.s.own;
             from_head = ahead.kvh * per_head;
             table = a.r.pages + ahead.z * a.r.table_stride;
-            // its queries, on their way into the L1 cache
-            const int f0 = ahead.tile * MT, row = lane >> 1;
-            if (to_copy > 0 && row < min((long)MT, (long)ahead.s.n * G - f0)) {
-                const int f = f0 + row, i = f / G;
-                const uint16_t* q = (const uint16_t*)a.q + (size_t)(ahead.s.r0 + i) * a.q_row + (size_t)(ahead.kvh * G + f - i * G) * a.q_head + (lane & 1) * (D / 2);
-                asm volatile("prefetch.global.L1 [%0];" ::"l"(q));
-            }
+            if (to_copy > 0) fetch_queries(ahead);
             __syncwarp();
         }
         read_id();
@@ -364,7 +367,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
         for (int nt = 0; nt < NT; nt++) {
             const int f = f0 + nt * 8 + g;
             const bool in = nt * 8 + g < n_f;
-            const int i = in ? f / G : 0;
+            const int i = in ? a4_row(a, f) : 0;
             const size_t q_at = (size_t)(r0 + i) * a.q_row + (size_t)(kvh * G + (in ? f - i * G : 0)) * a.q_head + 8 * tq;
             const uint16_t* q = (const uint16_t*)a.q + q_at;
             uint4 raw[NG];
@@ -376,21 +379,29 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                 if (((uintptr_t)p & 15) == 0) raw[gi] = *reinterpret_cast<const uint4*>(p);
                 else raw[gi] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
             }
-            auto value = [&](int gi, int e) {
-                const uint32_t w = e < 2 ? raw[gi].x : e < 4 ? raw[gi].y : e < 6 ? raw[gi].z : raw[gi].w;
-                const uint16_t v = (uint16_t)(e & 1 ? w >> 16 : w);
-                return a.type == ELEM_F16 ? __half2float(__ushort_as_half(v)) : __uint_as_float((uint32_t)v << 16);
+            float value[NG][8], top = 0.f;
+            auto as_floats = [&](auto f16) {
+#pragma unroll
+                for (int gi = 0; gi < NG; gi++)
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const uint32_t w = e < 2 ? raw[gi].x : e < 4 ? raw[gi].y : e < 6 ? raw[gi].z : raw[gi].w;
+                        if constexpr (decltype(f16)::value) { const float2 v = __half22float2(a4_as_half2(w)); value[gi][e] = v.x; value[gi][e + 1] = v.y; }
+                        else { value[gi][e] = __uint_as_float(w << 16); value[gi][e + 1] = __uint_as_float(w & 0xffff0000u); }
+                    }
             };
-            float top = 0.f;
+            if (a.type == ELEM_F16) as_floats(std::true_type{});
+            else as_floats(std::false_type{});
 #pragma unroll
             for (int gi = 0; gi < NG; gi++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(value(gi, e)));
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(value[gi][e]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
             const float up = __uint_as_float((uint32_t)(137 - ex) << 23);                // 2^(10 - ex)
-            const float mine = scalbnf(a.scale_log2, ex + 14);                           // (2^24 of the codes, 2^(ex - 10) of the queries)
+            const int ex1 = (ex + 14) >> 1, ex2 = ex + 14 - ex1;                         // (2^24 of the codes, 2^(ex - 10) of the queries, in two steps: each is a normal number)
+            const float mine = a.scale_log2 * __uint_as_float((uint32_t)(127 + ex1) << 23) * __uint_as_float((uint32_t)(127 + ex2) << 23);
 #pragma unroll
             for (int j = 0; j < 2; j++) by[nt][j] = __shfl_sync(0xffffffffu, mine, (2 * tq + j) * 4);
 #pragma unroll
@@ -399,7 +410,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 #pragma unroll
                 for (int e = 0; e < 4; e++) {                    // entries e and e + 4: the codes e and e + 4 of a word are masked out together
                     const float down = e & 1 ? 0.0625f : 1.f;
-                    const uint32_t h = a4_half2(value(gi, e) * up * down, value(gi, e + 4) * up * down);
+                    const uint32_t h = a4_half2(value[gi][e] * (up * down), value[gi][e + 4] * (up * down));
                     qb[nt][gi][e] = h;
                     const float2 back = __half22float2(a4_as_half2(h));
                     sum = fmaf(back.x + back.y, e & 1 ? 16.f : 1.f, sum);
@@ -412,10 +423,10 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const int row = nt * 8 + 2 * tq + j;
-                lim[nt][j] = row < n_f ? min(s.limit((f0 + row) / G), s.own) : s.own;
+                lim[nt][j] = row < n_f ? min(s.limit(a4_row(a, f0 + row)), s.own) : s.own;
             }
         }
-        const int own = s.own, lim_lo = min(s.limit(f0 / G), own);                       // keys that all rows of the tile see
+        const int own = s.own, lim_lo = min(s.limit(a4_row(a, f0)), own);                       // keys that all rows of the tile see
         // weighted sums, 2^24 (even dims) and 2^20 (odd) times too small, and sums; both times 2^up_v, which goes down where a value's scale exceeds most_v, 2^(9 - up_v); references of the
         // exponentials
         float o[NT][NG][2][4], ref[NT][2], l[NT][2], up_v = 30.f, most_v = 0x1p-21f;
@@ -600,7 +611,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                 const int row = nt * 8 + 2 * tq + j;
                 if (row >= n_f) continue;
                 if (begins && ends) {
-                    const int f = f0 + row, i = f / G;
+                    const int f = f0 + row, i = a4_row(a, f);
                     const float inv = l[nt][j] == 0.f ? 0.f : 1.f / l[nt][j];            // (0: no keys. A NaN stays one.)
 #pragma unroll
                     for (int gi = 0; gi < NG; gi++)
@@ -649,7 +660,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                 for (int v = w; v <= end; v++)
                     sum.add(*reinterpret_cast<const float2*>(part_of(v) + MT * D + row * 2), *reinterpret_cast<const float4*>(part_of(v) + row * D + d));
                 if (finish) {
-                    const int f = h.f0 + row, i = f / G;
+                    const int f = h.f0 + row, i = a4_row(a, f);
                     sum.out(a, h.r0 + i, h.kvh * G + f - i * G, d);
                 } else {
                     *reinterpret_cast<float4*>(to + row * D + d) = sum.v;
@@ -712,7 +723,7 @@ __global__ void __launch_bounds__(a4_join_threads(MT), 1024 / a4_join_threads(MT
         for (int j = at; j < at + per; j++) all.add(refs[j], sums[j][d / 4]);
     }
     if (row >= h.rows) return;
-    const int G = a.n_head / a.n_kv, f = h.f0 + row, i = f / G;
+    const int G = a.group, f = h.f0 + row, i = a4_row(a, f);
     all.out(a, h.r0 + i, h.kvh * G + f - i * G, d);
 }
 
@@ -761,8 +772,11 @@ size_t attention_4bit_work_bytes(long n_rows, int n_head, int n_kv, int head_dim
     return a4_many(n_rows, n_head, n_kv) ? std::max(step, attention_4bit_tc_work_bytes(head_dim)) : step;      // (all rows may be one sequence's)
 }
 
-cudaError_t attention_4bit_launch(const Attention4Args& a, cudaStream_t s) {
+cudaError_t attention_4bit_launch(const Attention4Args& args, cudaStream_t s) {
+    Attention4Args a = args;
     if (a.r.n_rows == 0 || a.r.n_seqs == 0) return cudaSuccess;
+    a.group = a.n_head / a.n_kv;
+    a.per_group = a.group == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / a.group);
     const DependentLaunch dependent;
     if (a4_many(a.max_rows, a.n_head, a.n_kv)) return attention_4bit_tc_launch(a, s);
     // tiles of 8 rows where all fit one, of 16 (with more registers and less running at once) where not: 4 rows a KV head in tiles of 8 and of 16, us: 32 sequences of 500 tokens 17.6 and 23.6,

@@ -8,6 +8,11 @@ namespace b2 {
 
 #ifdef __CUDACC__
 __device__ __forceinline__ uint32_t a4_half2(float a, float b) { const __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<const uint32_t*>(&h); }
+// the row of its sequence that (row, head) f belongs to: f over the group's heads (the quotient by multiplication may be one less)
+__device__ __forceinline__ int a4_row(const Attention4Args& a, unsigned f) {
+    const unsigned i = __umulhi(f, a.per_group);
+    return (int)(i + (f - i * (unsigned)a.group >= (unsigned)a.group));
+}
 // four neighbouring dims of a row's output
 __device__ __forceinline__ void a4_store_out(const Attention4Args& a, int t, int head, int d, float x, float y, float z, float w) {
     uint32_t lo, hi;

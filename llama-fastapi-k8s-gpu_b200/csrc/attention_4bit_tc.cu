@@ -65,15 +65,15 @@ struct T4Seq {
         n = min(all, a.max_rows);
         own = min(max(a.r.lengths[z], 0), a.r.max_pages * a.r.block_tokens);
         lim0 = own - all + 1;
-        tiles = (int)(((long)n * (a.n_head / a.n_kv) + 2 * T4_ROWS - 1) / (2 * T4_ROWS));
+        tiles = (int)(((long)n * a.group + 2 * T4_ROWS - 1) / (2 * T4_ROWS));
     }
     __device__ int limit(int i) const { return max(0, lim0 + i); }
     // blocks of keys that the unit's last row sees
-    __device__ int steps(int tile, int G) const {
-        const int last = min(n - 1, (int)(((long)tile * 2 * T4_ROWS + 2 * T4_ROWS - 1) / G));
+    __device__ int steps(int tile, const Attention4Args& a) const {
+        const int last = min(n - 1, a4_row(a, (unsigned)tile * (2 * T4_ROWS) + 2 * T4_ROWS - 1));      // (below 2^31 + 256)
         return max(1, (min(limit(last), own) + T4_K - 1) / T4_K);
     }
-    __device__ long all_steps(int G) const { long s = 0; for (int t = 0; t < tiles; t++) s += steps(t, G); return s; }
+    __device__ long all_steps(const Attention4Args& a) const { long s = 0; for (int t = 0; t < tiles; t++) s += steps(t, a); return s; }
 };
 
 // the runs of blocks of one unit: every role walks them the same way
@@ -82,9 +82,9 @@ struct T4Walk {
     T4Seq s;
     int b0, n, steps;                // this segment: first block, blocks, blocks of its unit
     int seg_kvh, seg_f0, seg_z;
-    __device__ bool next(const Attention4Args& a, int G) {
+    __device__ bool next(const Attention4Args& a) {
         if (left <= 0) return false;
-        steps = s.steps(tile, G);
+        steps = s.steps(tile, a);
         b0 = block; n = min(steps - block, left); seg_kvh = kvh; seg_f0 = tile * 2 * T4_ROWS; seg_z = z;
         return true;
     }
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
     uint8_t* ks = qs + 2 * PARTS * T4_PART;                      // [stage][upper, rest][part]
     uint8_t* vs = ks + ST * OPERAND;
     uint8_t* raw = vs + ST * OPERAND;                            // [T4_RAW]
-    const int G = a.n_head / a.n_kv;
+    const int G = a.group;
     griddep_wait();
     griddep_launch();
     if (warp == 17) {
@@ -203,12 +203,12 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                         T4Seq one;
                         one.n = __shfl_sync(0xffffffffu, s.n, l); one.own = __shfl_sync(0xffffffffu, s.own, l); one.lim0 = __shfl_sync(0xffffffffu, s.lim0, l); one.tiles = __shfl_sync(0xffffffffu, s.tiles, l);
                         long sum = 0;
-                        for (int t = lane; t < one.tiles; t += 32) sum += one.steps(t, G);
+                        for (int t = lane; t < one.tiles; t += 32) sum += one.steps(t, a);
 #pragma unroll
                         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                         if (lane == l) mine = sum;
                     }
-                } else mine = s.all_steps(G);
+                } else mine = s.all_steps(a);
                 mine *= a.n_kv;
                 long sum = mine;
 #pragma unroll
@@ -221,11 +221,11 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                         if (lane == l) {
                             int tile = 0;
                             for (; tile + 1 < s.tiles; tile++) {
-                                const long here = (long)s.steps(tile, G) * a.n_kv;
+                                const long here = (long)s.steps(tile, a) * a.n_kv;
                                 if (rest < here) break;
                                 rest -= here;
                             }
-                            const int each = s.steps(tile, G);
+                            const int each = s.steps(tile, a);
                             start.z = z0 + l; start.tile = tile; start.kvh = (int)(rest / each); start.block = (int)(rest % each); start.s = s;
                         }
                         break;
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             // ================= copies: lane j has the block's 16-token block j, keys, then values
             const int blocks = a.r.block_tokens / Q4_TOKENS;
             int it = 0;
-            for (; walk.next(a, G); walk.done(a)) {
+            for (; walk.next(a); walk.done(a)) {
                 const long table = walk.seg_z * a.r.table_stride;
                 const int own = walk.s.own;
                 for (int i = 0; i < walk.n; i++) {
@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             const uint32_t id_s = tc_idesc_bf16(T4_ROWS, T4_K) & f16, id_o = tc_idesc_bf16(T4_ROWS, D, true) & f16;
             const uint64_t dq0 = tc_desc(smem_u32(qs)), dk0 = tc_desc(smem_u32(ks)), dv0 = tc_desc(smem_u32(vs), T4_PART);
             int it = 0, segs[2] = {0, 0}, done[2] = {0, 0};      // blocks of the CTA, segments and blocks of each tile so far
-            for (; walk.next(a, G); walk.done(a)) {
+            for (; walk.next(a); walk.done(a)) {
                 const int n = walk.n, tiles = (long)walk.s.n * G - walk.seg_f0 > T4_ROWS ? 2 : 1;
                 // (`first`: nobody has waited for these keys yet; `last`: nobody needs them any more)
                 auto scores = [&](int t, int at, bool first, bool last) {
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
         const int v_key = NG == 4 ? dw * 8 + eight : dw * 16 + k_token, v_g = NG == 4 ? lane >> 3 : k_g;       // of 64 keys (heads of 64: four warps' work)
         const int v_token = v_key % Q4_TOKENS, v_pair = v_token >> 1;
         int it = 0, seg = 0;
-        for (; walk.next(a, G); walk.done(a), seg++) {
+        for (; walk.next(a); walk.done(a), seg++) {
             if (seg >= 2) mbar_wait_warp(&seg_done[seg & 1], ((seg >> 1) - 1) & 1, t4_error, 0xc000bu, (unsigned)seg);
             if (dw == 0 && lane < NG) first_bad[seg & 1][lane] = INT_MAX;
             named_bar_sync(1, 256);
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
         uint32_t done = 0;                                       // blocks of this tile so far
         int seg = 0;
         long given = run_shared[0] * blockIdx.x + min((long)blockIdx.x, run_shared[1]);      // the segment's first block among all
-        for (; walk.next(a, G); given += walk.n, walk.done(a), seg++) {
+        for (; walk.next(a); given += walk.n, walk.done(a), seg++) {
             const int M = (int)min((long)INT_MAX, (long)walk.s.n * G), n_f = min(2 * T4_ROWS, M - walk.seg_f0), r0 = walk.s.r0, own = walk.s.own;
             const bool begins = walk.b0 == 0, ends = walk.b0 + walk.n == walk.steps;
             if (t == 1 && n_f <= T4_ROWS) {
@@ -430,7 +430,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             // ---- the warp's 32 queries, into 128-byte-swizzled rows (rows past the end: zeros): neighbouring lanes have neighbouring pieces of a row
             const int f0 = walk.seg_f0 + t * T4_ROWS + (warp & 3) * 32, f = f0 + lane;
             const bool in = f < M;
-            const int i_mine = in ? f / G : 0, head = walk.seg_kvh * G + (in ? f - i_mine * G : 0), r = r0 + i_mine;
+            const int i_mine = in ? a4_row(a, f) : 0, head = walk.seg_kvh * G + (in ? f - i_mine * G : 0), r = r0 + i_mine;
             const int lim = in ? min(walk.s.limit(i_mine), own) : 0;
             const size_t q_mine = (size_t)r * a.q_row + (size_t)head * a.q_head;
             constexpr int LANES = D / 8, ROWS = 32 / LANES, BATCH = 8;      // lanes a row, rows at once

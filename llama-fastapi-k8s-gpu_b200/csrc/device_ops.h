@@ -79,6 +79,8 @@ struct Attention4Args {
     int max_rows;                // most rows of a sequence
     int n_head, n_kv, head_dim, type;
     float scale_log2;
+    int group;                   // heads of a KV head, and 2^32 over them (both set by the launch)
+    unsigned per_group;
     unsigned per_page;           // 2^32 over the blocks of a page (set by the launch)
     int few_units;               // units of work that tables and rows allow fit 31 bits (set by the launch)
 };
