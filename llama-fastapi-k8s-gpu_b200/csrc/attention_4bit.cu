@@ -36,6 +36,7 @@ constexpr int A4_BLOCKS = 2, A4_KEYS = A4_BLOCKS * Q4_TOKENS;      // blocks and
 constexpr int A4_STAGES = 2;         // steps under way
 constexpr int A4_BEGIN = 2;          // units that a segment's beginning and end count as, beside its steps
 constexpr int A4_SMS = 148;
+constexpr int A4_LONG_RUN = 16;      // units of a run from which on the warps of an SM get different shares (A4Cut)
 // The join's CTAs. 148 tiles of 256 rows, us: a row a CTA 41 (CTAs start one in 1.1 ns), 16 rows 4. Tiles of 8 and 16 rows, a call of (8 sequences, 12 rows a KV head) and (1, 16, 20000 tokens): 1 row a
 // CTA of 128 threads 19.4 and 18, 4 rows 16.3 and 18.0, 16 of 512 16.4 and 18.8; (1, 4, 4000 tokens) and (32, 4, 500): 1 row of 128 threads 13.1 and 18.1, 2 of 256 12.7 and 17.3.
 constexpr int a4_join_threads(int mt) { return mt == 8 ? 256 : mt == 16 ? 128 : 512; }
@@ -128,26 +129,36 @@ struct A4At {
     }
 };
 
+// x / y for quotients below 2^20: an approximate one is off by at most one
+__device__ __forceinline__ int a4_quotient(int x, int y) {
+    const int q = (int)__fdividef((float)x, (float)y), r = x - q * y;
+    return q + (r >= y) - (r < 0);
+}
+
 // All units cut into runs, one a warp, of equal length within a group of CTAs (the first of a group have a unit more). Where three CTAs are on an SM and runs are long there are three groups:
 // of an SM's warps the oldest are served first, so the CTAs that started first have more (with equal runs the thirds of 256 chats' CTAs ended at 121, 133 and 146 us).
+template <typename T>                                            // of numbers of units: int where all fit (64-bit products and quotients take a hundred instructions)
 struct A4Cut {
-    long begin, run, longer;                                     // of a group: first unit, units of a run, runs that have one more
+    T begin, run, longer;                                     // of a group: first unit, units of a run, runs that have one more
     int group, per;                                              // its number, warps of a group
-    static constexpr long LONG_RUN = 16;
-    __device__ static long first(long total, int groups, int group) {      // first unit of a group: shares 48 : 43 : 37
-        return groups == 3 ? total * (group == 0 ? 0 : group == 1 ? 48 : group == 2 ? 91 : 128) / 128 : group ? total : 0;
+    __device__ static T over(T x, T y) {
+        if constexpr (sizeof(T) == 4) return a4_quotient(x, y);
+        else return x / y;
     }
-    __device__ A4Cut(const Attention4Args& a, long total, int warps, int groups, int g) : group(g), per(groups == 3 ? A4_SMS * A4_WARPS : warps) {
+    __device__ static T first(T total, int groups, int group) {      // first unit of a group: shares 48 : 43 : 37
+        const int share = group == 0 ? 0 : group == 1 ? 48 : group == 2 ? 91 : 128;
+        return groups == 3 ? total / 128 * share + total % 128 * share / 128 : group ? total : 0;
+    }
+    __device__ A4Cut(T total, int warps, int groups, int g) : group(g), per(groups == 3 ? A4_SMS * A4_WARPS : warps) {
         begin = first(total, groups, g);
-        const long n = first(total, groups, g + 1) - begin;
-        run = !n ? 0 : a.few_units ? (long)((unsigned)n / (unsigned)per) : n / per;      // (a division in 64 bits takes a hundred instructions)
+        const T n = first(total, groups, g + 1) - begin;
+        run = over(n, per);
         longer = n - run * per;
     }
-    __device__ long at(int i) const { return begin + run * i + min((long)i, longer); }      // first unit of the group's run i
-    __device__ int owner(const Attention4Args& a, long u) const {      // the run that has a unit of the group
-        const long x = u - begin, most = longer * (run + 1);
-        if (a.few_units) return (int)(x < most ? (unsigned)x / (unsigned)(run + 1) : (unsigned)longer + (unsigned)(x - most) / (unsigned)run);
-        return (int)(x < most ? x / (run + 1) : longer + (x - most) / run);
+    __device__ T at(int i) const { return begin + run * i + min((T)i, longer); }      // first unit of the group's run i
+    __device__ int owner(T u) const {      // the run that has a unit of the group
+        const T x = u - begin, most = longer * (run + 1);
+        return (int)(x < most ? over(x, run + 1) : longer + over(x - most, run));
     }
 };
 
@@ -190,7 +201,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
     constexpr int REGION = S * STAGE > PART * 4 ? S * STAGE : PART * 4;
     extern __shared__ __align__(128) uint8_t a4_raw[];
     __shared__ uint64_t full[A4_WARPS][S];
-    struct Held { int rows, r0, f0, kvh, ends, last; };          // rows 0: no result; `last`: the CTA where the segment ends
+    struct Held { int rows, r0, f0, kvh, ends, last; };          // rows 0: no result; `last`: the CTA where a segment that begins here ends
     __shared__ Held held[A4_WARPS][2];                           // of segments that began before the warp's run, and that go on behind it
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
     uint8_t* ring = a4_raw + warp * REGION;                      // behind the last step: the result of a segment that goes on
@@ -228,13 +239,17 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
     const int all_warps = gridDim.x * A4_WARPS, warps = (int)min((long)all_warps, total), me = blockIdx.x * A4_WARPS + warp;
-    const int groups = total >= all_warps * A4Cut::LONG_RUN && a4_per_sm(NT) == 3 && (int)gridDim.x == A4_SMS * 3 ? 3 : 1;
+    const int groups = total >= all_warps * A4_LONG_RUN && a4_per_sm(NT) == 3 && (int)gridDim.x == A4_SMS * 3 ? 3 : 1;
     const int group = groups > 1 ? blockIdx.x / A4_SMS : 0;
     long u0 = 0, u1 = 0;
     if (me < warps) {
-        const A4Cut cut(a, total, warps, groups, group);
-        const int i = me - group * cut.per;
-        u0 = cut.at(i); u1 = cut.at(i + 1);
+        auto run = [&](auto zero) {
+            const A4Cut<decltype(zero)> cut((decltype(zero))total, warps, groups, group);
+            const int i = me - group * cut.per;
+            u0 = cut.at(i); u1 = cut.at(i + 1);
+        };
+        if (a.few_units) run(0);
+        else run(0l);
     }
     __shared__ A4At places[A4_WARPS][2];                         // where the warp is, and where its copies are (few registers: they change once a segment)
     A4At& at = places[warp][0];
@@ -279,11 +294,19 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
                 before += __shfl_sync(0xffffffffu, sum, 31);
             }
         }
-        const long each = start.s.steps + A4_BEGIN, per = start.s.tiles * each;
-        start.kvh = a.few_units ? (int)((unsigned)rest / (unsigned)per) : (int)(rest / per); rest -= start.kvh * per;
-        start.tile = a.few_units ? (int)((unsigned)rest / (unsigned)each) : (int)(rest / each); rest -= start.tile * each;
-        first += max(A4_BEGIN - rest, 0l);
-        start.step = (int)max(rest - A4_BEGIN, 0l);
+        const int each = start.s.steps + A4_BEGIN;
+        if (a.few_units) {
+            const int per = start.s.tiles * each;
+            start.kvh = a4_quotient((int)rest, per);
+            start.tile = a4_quotient((int)rest - start.kvh * per, each);
+        } else {
+            const long per = start.s.tiles * (long)each;
+            start.kvh = (int)(rest / per);
+            start.tile = (int)((rest - start.kvh * per) / each);
+        }
+        const int in = (int)(rest - ((long)start.kvh * start.s.tiles + start.tile) * each);
+        first += max(A4_BEGIN - in, 0);
+        start.step = max(in - A4_BEGIN, 0);
     }
 
     static_assert(KB == 2, "a page ends at most once in a step");
@@ -372,12 +395,16 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             const uint16_t* q = (const uint16_t*)a.q + q_at;
             uint4 raw[NG];
 #pragma unroll
-            for (int gi = 0; gi < NG; gi++) {
-                raw[gi] = make_uint4(0, 0, 0, 0);
-                if (!in) continue;
-                const uint16_t* p = q + gi * Q4_GROUP;
-                if (((uintptr_t)p & 15) == 0) raw[gi] = *reinterpret_cast<const uint4*>(p);
-                else raw[gi] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+            for (int gi = 0; gi < NG; gi++) raw[gi] = make_uint4(0, 0, 0, 0);
+            if (in && ((uintptr_t)q & 15) == 0) {
+#pragma unroll
+                for (int gi = 0; gi < NG; gi++) raw[gi] = *reinterpret_cast<const uint4*>(q + gi * Q4_GROUP);
+            } else if (in) {
+#pragma unroll
+                for (int gi = 0; gi < NG; gi++) {
+                    const uint16_t* p = q + gi * Q4_GROUP;
+                    raw[gi] = make_uint4(p[0] | (uint32_t)p[1] << 16, p[2] | (uint32_t)p[3] << 16, p[4] | (uint32_t)p[5] << 16, p[6] | (uint32_t)p[7] << 16);
+                }
             }
             float value[NG][8], top = 0.f;
             auto as_floats = [&](auto f16) {
@@ -626,10 +653,14 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             }
         if (!(begins && ends) && lane == 0) {
             const long end = u - n + left - 1;                   // the segment's last unit
-            int in = group;
-            while (in + 1 < groups && end >= A4Cut::first(total, groups, in + 1)) in++;
-            const A4Cut cut(a, total, warps, groups, in);
-            held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, (in * cut.per + cut.owner(a, end)) / A4_WARPS};
+            auto owner = [&](auto zero) {
+                using T = decltype(zero);
+                int in = group;
+                while (in + 1 < groups && (T)end >= A4Cut<T>::first((T)total, groups, in + 1)) in++;
+                const A4Cut<T> cut((T)total, warps, groups, in);
+                return (in * cut.per + cut.owner((T)end)) / A4_WARPS;
+            };
+            held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, !begins ? 0 : a.few_units ? owner(0) : owner(0l)};
         }
         // the segment behind it (not the sequence's loads if there is none)
         u += A4_BEGIN;
@@ -745,7 +776,7 @@ cudaError_t a4_step(Attention4Args a, cudaStream_t s) {
     // as many CTAs as run at once, no more than there can be steps for
     const double units = a4_most_units(a, MT);
     const int ctas = (int)std::min<double>(A4_SMS * a4_per_sm(NT), std::ceil(units / A4_WARPS));
-    a.few_units = units < 1e9;
+    a.few_units = units < 1e9 && a.n_kv < 1 << 20;               // (quotients: a4_quotient)
     const unsigned blocks = a.r.block_tokens / Q4_TOKENS;
     a.per_page = blocks == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / blocks);
     cudaError_t e = launch_chain(attention_4bit_step_kernel<D, NT>, dim3(ctas), dim3(A4_THREADS), smem, s, a);
