@@ -36,7 +36,6 @@ constexpr int A4_BLOCKS = 2, A4_KEYS = A4_BLOCKS * Q4_TOKENS;      // blocks and
 constexpr int A4_STAGES = 2;         // steps under way
 constexpr int A4_BEGIN = 2;          // units that a segment's beginning and end count as, beside its steps
 constexpr int A4_SMS = 148;
-constexpr int A4_LONG_RUN = 16;      // units of a run from which on the warps of an SM get different shares (A4Cut)
 // The join's CTAs. 148 tiles of 256 rows, us: a row a CTA 41 (CTAs start one in 1.1 ns), 16 rows 4. Tiles of 8 and 16 rows, a call of (8 sequences, 12 rows a KV head) and (1, 16, 20000 tokens): 1 row a
 // CTA of 128 threads 19.4 and 18, 4 rows 16.3 and 18.0, 16 of 512 16.4 and 18.8; (1, 4, 4000 tokens) and (32, 4, 500): 1 row of 128 threads 13.1 and 18.1, 2 of 256 12.7 and 17.3.
 constexpr int a4_join_threads(int mt) { return mt == 8 ? 256 : mt == 16 ? 128 : 512; }
@@ -135,30 +134,19 @@ __device__ __forceinline__ int a4_quotient(int x, int y) {
     return q + (r >= y) - (r < 0);
 }
 
-// All units cut into runs, one a warp, of equal length within a group of CTAs (the first of a group have a unit more). Where three CTAs are on an SM and runs are long there are three groups:
-// of an SM's warps the oldest are served first, so the CTAs that started first have more (with equal runs the thirds of 256 chats' CTAs ended at 121, 133 and 146 us).
-template <typename T>                                            // of numbers of units: int where all fit (64-bit products and quotients take a hundred instructions)
+// All units cut into equal runs, one a warp (the first have a unit more). T: of numbers of units, int where all fit (64-bit products and quotients take a hundred instructions).
+template <typename T>
 struct A4Cut {
-    T begin, run, longer;                                     // of a group: first unit, units of a run, runs that have one more
-    int group, per;                                              // its number, warps of a group
+    T run, longer;                                               // units of a run, runs that have one more
     __device__ static T over(T x, T y) {
         if constexpr (sizeof(T) == 4) return a4_quotient(x, y);
         else return x / y;
     }
-    __device__ static T first(T total, int groups, int group) {      // first unit of a group: shares 48 : 43 : 37
-        const int share = group == 0 ? 0 : group == 1 ? 48 : group == 2 ? 91 : 128;
-        return groups == 3 ? total / 128 * share + total % 128 * share / 128 : group ? total : 0;
-    }
-    __device__ A4Cut(T total, int warps, int groups, int g) : group(g), per(groups == 3 ? A4_SMS * A4_WARPS : warps) {
-        begin = first(total, groups, g);
-        const T n = first(total, groups, g + 1) - begin;
-        run = over(n, per);
-        longer = n - run * per;
-    }
-    __device__ T at(int i) const { return begin + run * i + min((T)i, longer); }      // first unit of the group's run i
-    __device__ int owner(T u) const {      // the run that has a unit of the group
-        const T x = u - begin, most = longer * (run + 1);
-        return (int)(x < most ? over(x, run + 1) : longer + over(x - most, run));
+    __device__ A4Cut(T total, int warps) : run(over(total, warps)), longer(total - run * warps) {}
+    __device__ T at(int i) const { return run * i + min((T)i, longer); }      // first unit of run i
+    __device__ int owner(T u) const {                            // the run that has a unit
+        const T most = longer * (run + 1);
+        return (int)(u < most ? over(u, run + 1) : longer + over(u - most, run));
     }
 };
 
@@ -239,14 +227,11 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
         for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     }
     const int all_warps = gridDim.x * A4_WARPS, warps = (int)min((long)all_warps, total), me = blockIdx.x * A4_WARPS + warp;
-    const int groups = total >= all_warps * A4_LONG_RUN && a4_per_sm(NT) == 3 && (int)gridDim.x == A4_SMS * 3 ? 3 : 1;
-    const int group = groups > 1 ? blockIdx.x / A4_SMS : 0;
     long u0 = 0, u1 = 0;
     if (me < warps) {
         auto run = [&](auto zero) {
-            const A4Cut<decltype(zero)> cut((decltype(zero))total, warps, groups, group);
-            const int i = me - group * cut.per;
-            u0 = cut.at(i); u1 = cut.at(i + 1);
+            const A4Cut<decltype(zero)> cut((decltype(zero))total, warps);
+            u0 = cut.at(me); u1 = cut.at(me + 1);
         };
         if (a.few_units) run(0);
         else run(0l);
@@ -655,10 +640,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             const long end = u - n + left - 1;                   // the segment's last unit
             auto owner = [&](auto zero) {
                 using T = decltype(zero);
-                int in = group;
-                while (in + 1 < groups && (T)end >= A4Cut<T>::first((T)total, groups, in + 1)) in++;
-                const A4Cut<T> cut((T)total, warps, groups, in);
-                return (in * cut.per + cut.owner((T)end)) / A4_WARPS;
+                return A4Cut<T>((T)total, warps).owner((T)end) / A4_WARPS;
             };
             held[warp][slot] = {n_f, r0, f0, kvh, ends ? 1 : 0, !begins ? 0 : a.few_units ? owner(0) : owner(0l)};
         }
