@@ -15,9 +15,10 @@
 //     operand in f16's range, found from the scales as they come. Score fragments become operands by movmatrix.
 // The reference of a row's exponentials moves only where a score exceeds it by 2^6. It is a score before it is scaled, so that the largest one's difference is exact however large it is (one
 // fused multiply-add with a scaled reference would save an instruction a score, and be off by as much as the reference's last place).
-// Measured (32 heads over 8 of 128, f16): 256 chats of 16 to 4100 tokens 160 us, 3.8 TB/s of what has to be read, 0.58 of a copy's; 32 chats of 20 to 1500 19, one of 32000 20.7, of 700 10.6. A step is some 600
-// instructions, issued one in two cycles by the twelve warps that fit an SM. More CTAs than fit (184 to 206 us for the 256 chats), four an SM with 128 registers (170), and the next step's scores beside
-// this one's values (173 where it was 159) were slower, products in other orders the same.
+// Measured (32 heads over 8 of 128, f16): 256 chats of 16 to 4100 tokens 141 us, 4.4 TB/s of what has to be read, 0.66 of a copy's; 32 chats of 20 to 1500 16.5, one of 32000 18.6, of 700 8.5. A step is
+// some 600 instructions, issued one in two cycles by the twelve warps that fit an SM: those of unpacking (160) and of the values' weights (100) are the most. More CTAs than fit were a fifth slower, four an
+// SM with 128 registers a tenth, the next step's scores beside this one's values a tenth; products in other orders were the same, and so were larger shares for the CTAs that an SM serves first. A call
+// begins with 2 us of finding a warp's place and 1 of its queries, beside the copies.
 #include "attention_4bit.cuh"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"
@@ -774,7 +775,7 @@ cudaError_t attention_4bit_join(const Attention4Args& a, int ctas, int rows, cud
 
 namespace {
 // Up to so many rows a KV head of a sequence this file's tiles of 16 rows, more on tensor memory. us here and there (heads of 128, 8 KV heads): a sequence of 4000 tokens with 32 rows a KV head
-// 21 and 26, 64 rows 24 and 27, 68 rows 28 and 27, 128 rows 33 and 27; 32 sequences of 1000 tokens with 64 rows 92 and 91, 68 rows 113 and 91, 256 rows 334 and 115.
+// 17 and 23, 64 rows 18 and 24, 128 rows 24 and 25; 32 sequences of 1000 tokens with 32 rows 40 and 82, 64 rows 69 and 83, 68 rows 82 and 83, 256 rows 244 and 105.
 constexpr long A4_TC_ROWS = 64;
 bool a4_many(long rows, int n_head, int n_kv) { return rows * (n_head / n_kv) > A4_TC_ROWS; }
 }  // namespace
@@ -792,8 +793,8 @@ cudaError_t attention_4bit_launch(const Attention4Args& args, cudaStream_t s) {
     a.per_group = a.group == 1 ? 0xffffffffu : (unsigned)((1ull << 32) / a.group);
     const DependentLaunch dependent;
     if (a4_many(a.max_rows, a.n_head, a.n_kv)) return attention_4bit_tc_launch(a, s);
-    // tiles of 8 rows where all fit one, of 16 (with more registers and less running at once) where not: 4 rows a KV head in tiles of 8 and of 16, us: 32 sequences of 500 tokens 17.6 and 23.6,
-    // 256 of 2000 155 and 229, one of 30000 20.7 and 30.1
+    // tiles of 8 rows where all fit one, of 16 (with more registers and less running at once) where not: 4 rows a KV head in tiles of 8 and of 16, us: 32 sequences of 500 tokens 15.2 and 17.6,
+    // 256 of 2000 138 and 206, one of 30000 18.4 and 24.2
     const bool few = (long)a.max_rows * (a.n_head / a.n_kv) <= 8;
     if (a.head_dim == 64) return few ? a4_step<64, 1>(a, s) : a4_step<64, 2>(a, s);
     return few ? a4_step<128, 1>(a, s) : a4_step<128, 2>(a, s);
