@@ -8,7 +8,7 @@ torch = pytest.importorskip("torch")
 
 from cache_4bit_util import Cache4, coded, packed, quantised
 from conftest import PKG
-from test_device_ops_host import OnGpu, append_args, tensors
+from test_device_ops_host import OnGpu, append_args, native_calls, tensors
 
 
 @pytest.fixture(scope="module")
@@ -196,3 +196,50 @@ def test_python_refusals_of_attention(native_lib):
         attention_4bit(**good)
     with pytest.raises(RuntimeError, match="max_rows"):
         attention_4bit(**good, max_rows=0)
+
+
+def test_native_calls_pass_what_the_python_ones_pass(native_lib, monkeypatch):
+    """every argument reaches the entry points alike, whether the call is made in native code or in Python"""
+    import struct
+    from llama_cpp import _cabi, device_ops as ops
+    calls = native_calls()
+    seen = []
+    where, *kinds = (struct.Struct("@" + "".join({ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f"}[t] for _, t in k._fields_))
+                     for k in (_cabi.B2RaggedPages, _cabi.B2KvAppend, _cabi.B2KvRead4Bit, _cabi.B2Attention4Bit))
+
+    def entry(kind):
+        def f(device, w, args, stream):
+            seen.append((device, where.unpack(ctypes.string_at(w, where.size)), kind.unpack(ctypes.string_at(args, kind.size)), stream))
+            return 0
+        return ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p)(f)
+
+    names = ("kv_append_4bit", "kv_read_4bit", "attention_4bit")
+    Lib = type("Lib", (), {"b2_" + n: staticmethod(entry(k)) for n, k in zip(names, kinds)})
+    f, i = tensors()
+    g = lambda *s, dtype=torch.float16: f(*s, dtype=dtype, device=3)
+    j = lambda *s: g(*s, dtype=torch.int32)
+    wide = OnGpu(torch.zeros(5, 9, 64).half(), 3)
+    part = lambda a, b: OnGpu(wide.t[:, a:b], 3)
+    cache = dict(k_pool=g(9, 2, 3, 576, dtype=torch.uint8), v_pool=g(9, 2, 3, 576, dtype=torch.uint8), pages=j(3, 4), row_start=j(4), lengths=j(3))
+    out, work = g(5, 4, 64), g(1000)
+    freqs, q_out, k32 = g(20, dtype=torch.float32), g(5, 5, 64), g(5, 2, 64, dtype=torch.float32)
+    jobs = [lambda: ops.kv_append_4bit(part(0, 2), part(2, 4), **cache, freqs=freqs, layout="halves", first_pos=77, amplitude=1.5, q=part(4, 9), q_out=q_out, stream=1234),
+            lambda: ops.kv_append_4bit(k32, k32, **{**cache, "pages": OnGpu(cache["pages"].t[:, :2], 3)}),
+            lambda: ops.kv_read_4bit(**cache, k=part(0, 2), v=part(2, 4), stream=7),
+            lambda: ops.kv_read_4bit(**cache, k=None, v=k32),
+            lambda: ops.attention_4bit(part(0, 4), *cache.values(), out, work, max_rows=2, stream=5),
+            lambda: ops.attention_4bit(part(4, 8), *cache.values(), out, work, scale=0.3)]
+    monkeypatch.setattr(_cabi, "load_library", lambda path=None: Lib)
+    for job in jobs:
+        both = []
+        for native in (None, True, False):                               # (None: dtypes are met)
+            monkeypatch.setattr(ops, "_entries", {n: (None, None) for n in names} if native is False else {})
+            made = []
+            if native:
+                for n in names:
+                    ops._entries[n] = ((lambda fn: lambda *a: made.append(fn(*a)) or made[-1])(getattr(calls, n)), ctypes.cast(getattr(Lib, "b2_" + n), ctypes.c_void_p).value)
+            seen.clear()
+            job()
+            assert len(seen) == 1 and (not native or made == [0])
+            both.append(seen[0])
+        assert both[1] == both[2] and both[1][0] == 3
