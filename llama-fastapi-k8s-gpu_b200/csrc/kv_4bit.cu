@@ -86,29 +86,34 @@ __device__ __forceinline__ K4Place k4_place(const RaggedPages& r, int n_kv, int 
 }
 }  // namespace
 
-// the larger one, NaN if one is
+// the larger one, NaN if one is; the largest and the smallest of three
 __device__ __forceinline__ float k4_max(float a, float b) { float m; asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b)); return m; }
+__device__ __forceinline__ float k4_max(float a, float b, float c) { float m; asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c)); return m; }
+__device__ __forceinline__ float k4_min(float a, float b, float c) { float m; asm("min.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c)); return m; }
 
 // Scale and codes of a group that four neighbouring lanes have: eight entries each, the eight codes of this lane's as a word.
-// A code is the low bits of entry * (1 / scale) + 8 + 1.5 2^23, whose last place is a whole number (ties to even). The product is off the quotient by 2^-22 of it at most (8.01), so that this
-// is the quotient rounded unless the fraction is within 2^-18 of a half; those are divided, as are entries by scales that are so small or large that the quotient may lie outside.
+// A code is the low bits of entry * (1 / scale) + 8 + 1.5 2^23, whose last place is a whole number (ties to even). The reciprocal is off by 2^-23 of it at most, and the product by as
+// much of the quotient (8.01), so that this is the quotient rounded unless the fraction is within 2^-18 of a half; those are divided, as are entries by scales that are so small or large that the quotient may lie outside.
 __device__ __forceinline__ uint32_t k4_quantise(const float (&x)[8], __half& scale) {
-    float hi = x[0], lo = x[0];
+    float hi = k4_max(x[0], x[1]), lo = fminf(x[0], x[1]);
 #pragma unroll
-    for (int e = 1; e < 8; e++) { hi = k4_max(hi, x[e]); lo = fminf(lo, x[e]); }
+    for (int e = 2; e < 8; e += 2) { hi = k4_max(hi, x[e], x[e + 1]); lo = k4_min(lo, x[e], x[e + 1]); }
 #pragma unroll
     for (int o = 1; o < 4; o *= 2) { hi = k4_max(hi, __shfl_xor_sync(0xffffffffu, hi, o)); lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o)); }
     scale = __float2half_rn(fminf(fmaxf((hi > -lo ? hi : lo) * -0.125f, -65504.f), 65504.f));
     const float s = __half2float(scale);
     constexpr float BIAS = 12582912.f;
-    const float r = __fdiv_rn(1.f, s);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
     uint32_t word = 0;
     float near = 0.f;
+    const uint64_t r2 = f2_pack(r, r), bias2 = f2_pack(BIAS + 8.f, BIAS + 8.f), minus2 = f2_pack(-1.f, -1.f);
 #pragma unroll
-    for (int e = 7; e >= 0; e--) {
-        const float t = fmaf(x[e], r, BIAS + 8.f);
-        near = fmaxf(near, fabsf(fmaf(x[e], r, (BIAS + 8.f) - t)));
-        word = word * 16 + __float_as_uint(fminf(t, BIAS + 15.f));
+    for (int e = 6; e >= 0; e -= 2) {
+        const uint64_t x2 = f2_pack(x[e], x[e + 1]), t2 = f2_fma(x2, r2, bias2);
+        const float2 t = f2_unpack(t2), rest = f2_unpack(f2_fma(x2, r2, f2_fma(t2, minus2, bias2)));
+        near = fmaxf(near, fmaxf(fabsf(rest.x), fabsf(rest.y)));
+        word = (word * 16 + __float_as_uint(fminf(t.y, BIAS + 15.f))) * 16 + __float_as_uint(fminf(t.x, BIAS + 15.f));
     }
     word -= 0x3f400000u;                                         // (what the upper bits of eight such numbers add up to)
     if (!(near < 0.5f - 0x1p-18f) || !(fabsf(s) >= 0x1p-14f && fabsf(s) < 65504.f)) {
@@ -157,13 +162,13 @@ __global__ void __launch_bounds__(K4_THREADS, 4) kv_append_4bit_kernel(const KvA
     // KIND 0: keys, 1: values, 2: queries. Each warp of the row has a part of the heads of each. False: the row has no sequence.
     auto heads_of = [&](auto kind, const In* base, long head, int heads, int wide_in) {
         constexpr int KIND = decltype(kind)::value;
-        const int all = (heads + AT_ONCE - 1) / AT_ONCE, last = all * (part + 1) >> parts;
+        const int all = (heads + AT_ONCE - 1) / AT_ONCE, last = all * (part + 1) >> parts, mine = min(last, (heads - h0 + AT_ONCE - 1) / AT_ONCE);      // (this lane's)
         int i = all * part >> parts;
         const In* from = base + (i * AT_ONCE + h0) * head;
-        K4Piece<In> x[UNROLL], y[UNROLL];
+        K4Piece<In> x[UNROLL] = {}, y[UNROLL] = {};              // (a lane without a head of its own goes on with zeros)
         int loaded = i;                                          // turns whose entries are under way or here
         auto load = [&](K4Piece<In>& p, K4Piece<In>& q) {
-            if (loaded < last && loaded * AT_ONCE + h0 < heads) {
+            if (loaded < mine) {
                 k4_fetch(from, wide_in, p);
                 if constexpr (KIND != 1 && TURN == K4_HALVES) { if (rotates) k4_fetch(left ? from + half : from - half, wide_in, q); }
                 if constexpr (KIND != 1 && TURN == K4_ANY) {
@@ -194,72 +199,73 @@ __global__ void __launch_bounds__(K4_THREADS, 4) kv_append_4bit_kernel(const KvA
         }
         const int token = place.token & (Q4_TOKENS - 1);
         uint8_t* pool = (uint8_t*)(KIND == 0 ? a.k_pool : a.v_pool) + place.block + (i * AT_ONCE + h0) * step;
-        const long out_at = KIND == 2 ? row * a.qo_row + d : 0;
+        uint16_t* to = KIND == 2 ? (uint16_t*)a.q_out + row * a.qo_row + d + (i * AT_ONCE + h0) * a.qo_head : nullptr;
+        auto turns_of = [&](auto f16) {
 #pragma unroll 1
-        while (i < last) {
+            while (i < last) {
 #pragma unroll
-            for (int u = 0; u < UNROLL; u++) {
-                if (i >= last) break;
-                const int h = i * AT_ONCE + h0;
-                const bool in = h < heads;
-                float z[8];
+                for (int u = 0; u < UNROLL; u++) {
+                    if (i >= last) break;
+                    const bool in = i < mine;
+                    float z[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) z[e] = in ? k4_float(x[u].v[e]) : 0.f;
-                if constexpr (KIND != 1) {
-                    if (rotates) {
-                        if constexpr (TURN == K4_PAIRS) {
+                    for (int e = 0; e < 8; e++) z[e] = k4_float(x[u].v[e]);
+                    if constexpr (KIND != 1) {
+                        if (rotates) {
+                            if constexpr (TURN == K4_PAIRS) {
 #pragma unroll
-                            for (int e = 0; e < 8; e += 4) {
-                                const float4 t = *reinterpret_cast<const float4*>(turn + (d + e) / 2);
-                                const float v0 = z[e], v1 = z[e + 1], v2 = z[e + 2], v3 = z[e + 3];
-                                z[e] = __fsub_rn(__fmul_rn(v0, t.x), __fmul_rn(v1, t.y)); z[e + 1] = __fadd_rn(__fmul_rn(v1, t.x), __fmul_rn(v0, t.y));
-                                z[e + 2] = __fsub_rn(__fmul_rn(v2, t.z), __fmul_rn(v3, t.w)); z[e + 3] = __fadd_rn(__fmul_rn(v3, t.z), __fmul_rn(v2, t.w));
-                            }
-                        } else if constexpr (TURN == K4_HALVES) {
-                            const float2* with = turn + (left ? d : d - half);
-                            const float sign = left ? -1.f : 1.f;
+                                for (int e = 0; e < 8; e += 4) {
+                                    const float4 t = *reinterpret_cast<const float4*>(turn + (d + e) / 2);
+                                    const float v0 = z[e], v1 = z[e + 1], v2 = z[e + 2], v3 = z[e + 3];
+                                    z[e] = __fsub_rn(__fmul_rn(v0, t.x), __fmul_rn(v1, t.y)); z[e + 1] = __fadd_rn(__fmul_rn(v1, t.x), __fmul_rn(v0, t.y));
+                                    z[e + 2] = __fsub_rn(__fmul_rn(v2, t.z), __fmul_rn(v3, t.w)); z[e + 3] = __fadd_rn(__fmul_rn(v3, t.z), __fmul_rn(v2, t.w));
+                                }
+                            } else if constexpr (TURN == K4_HALVES) {
+                                const float2* with = turn + (left ? d : d - half);
+                                const float sign = left ? -1.f : 1.f;
 #pragma unroll
-                            for (int e = 0; e < 8; e += 2) {
-                                const float4 t = *reinterpret_cast<const float4*>(with + e);
-                                z[e] = __fadd_rn(__fmul_rn(z[e], t.x), __fmul_rn(k4_float(y[u].v[e]), sign * t.y));
-                                z[e + 1] = __fadd_rn(__fmul_rn(z[e + 1], t.z), __fmul_rn(k4_float(y[u].v[e + 1]), sign * t.w));
-                            }
-                        } else {
+                                for (int e = 0; e < 8; e += 2) {
+                                    const float4 t = *reinterpret_cast<const float4*>(with + e);
+                                    z[e] = __fadd_rn(__fmul_rn(z[e], t.x), __fmul_rn(k4_float(y[u].v[e]), sign * t.y));
+                                    z[e + 1] = __fadd_rn(__fmul_rn(z[e + 1], t.z), __fmul_rn(k4_float(y[u].v[e + 1]), sign * t.w));
+                                }
+                            } else {
 #pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                const int at = d + e;
-                                if (at >= a.rot_dims) continue;
-                                const bool one = a.halves ? at < half : (e & 1) == 0;
-                                const float2 t = turn[a.halves ? (one ? at : at - half) : at >> 1];
-                                z[e] = __fadd_rn(__fmul_rn(z[e], t.x), __fmul_rn(k4_float(y[u].v[e]), one ? -t.y : t.y));
+                                for (int e = 0; e < 8; e++) {
+                                    const int at = d + e;
+                                    if (at >= a.rot_dims) continue;
+                                    const bool one = a.halves ? at < half : (e & 1) == 0;
+                                    const float2 t = turn[a.halves ? (one ? at : at - half) : at >> 1];
+                                    z[e] = __fadd_rn(__fmul_rn(z[e], t.x), __fmul_rn(k4_float(y[u].v[e]), one ? -t.y : t.y));
+                                }
                             }
                         }
                     }
-                }
-                if constexpr (KIND == 2) {
-                    __syncwarp();                                // (a head's entries are read before they are replaced: q in place)
-                    if (in) {
-                        if (a.cache_type == ELEM_F16) k4_store((__half*)a.q_out + out_at + h * a.qo_head, wide >> 3 & 1, z);
-                        else k4_store((__nv_bfloat16*)a.q_out + out_at + h * a.qo_head, wide >> 3 & 1, z);
-                    }
-                    load(x[u], y[u]);
-                } else {
-                    load(x[u], y[u]);
-                    __half scale;
-                    const uint32_t word = k4_quantise(z, scale);
-                    if (in && place.block >= 0) {
-                        if (KIND == 0) *reinterpret_cast<uint32_t*>(pool + q4_key(D, token, w)) = word;
-                        else {
-                            *reinterpret_cast<uint16_t*>(pool + q4_value(D, token, 2 * w)) = (uint16_t)word;
-                            *reinterpret_cast<uint16_t*>(pool + q4_value(D, token, 2 * w + 1)) = (uint16_t)(word >> 16);
+                    if constexpr (KIND == 2) {
+                        __syncwarp();                                // (a head's entries are read before they are replaced: q in place)
+                        if (in) k4_store((std::conditional_t<decltype(f16)::value, __half, __nv_bfloat16>*)to, wide >> 3 & 1, z);
+                        to += AT_ONCE * a.qo_head;
+                        load(x[u], y[u]);
+                    } else {
+                        load(x[u], y[u]);
+                        __half scale;
+                        const uint32_t word = k4_quantise(z, scale);
+                        if (in && place.block >= 0) {
+                            if (KIND == 0) *reinterpret_cast<uint32_t*>(pool + q4_key(D, token, w)) = word;
+                            else {
+                                *reinterpret_cast<uint16_t*>(pool + q4_value(D, token, 2 * w)) = (uint16_t)word;
+                                *reinterpret_cast<uint16_t*>(pool + q4_value(D, token, 2 * w + 1)) = (uint16_t)(word >> 16);
+                            }
+                            if ((w & 3) == 0) *reinterpret_cast<__half*>(pool + q4_scale(D, token, w >> 2)) = scale;
                         }
-                        if ((w & 3) == 0) *reinterpret_cast<__half*>(pool + q4_scale(D, token, w >> 2)) = scale;
+                        pool += AT_ONCE * step;
                     }
-                    pool += AT_ONCE * step;
+                    i++;
                 }
-                i++;
             }
-        }
+        };
+        if (KIND != 2 || a.cache_type == ELEM_F16) turns_of(std::true_type{});
+        else turns_of(std::false_type{});
         return true;
     };
     // the values and queries of a row that is one warp's alone: on their way into L2 while the keys are dealt with
