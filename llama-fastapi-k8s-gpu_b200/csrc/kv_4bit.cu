@@ -5,7 +5,8 @@
 // A warp takes a row, or a part of its heads where the rows are few, and finds its place by itself; a lane has a piece of eight entries of a head, 32 bits of codes, and four
 // neighbouring lanes have a group. Reads are bound by memory and by the chain that each row begins with (sequence, page, codes), so as many warps as an SM holds have two turns of pieces each
 // under way: 65536 rows of 2 x 8 heads of 128 to f16 67 us, 0.78 of the measured bandwidth (four turns and half the warps 78), 37000 ragged rows of 2 x 5 heads to bf16 30. Appends are bound by
-// instructions as much as by memory, some 170 a piece of keys and 60 a piece of queries: 16384 rows of 32 + 2 x 8 heads of 128 100 us, 3.7 TB/s, 32 rows 5.3.
+// instructions as much as by memory, 3500 a row of 32 + 2 x 8 heads of 128: 16384 such rows 93 us, 3.8 TB/s, 32 rows 5.2. (More
+// turns of queries under way, one CTA an SM more or fewer: 1 to 6 % slower.)
 #include "device_ops.h"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"
