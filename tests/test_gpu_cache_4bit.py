@@ -364,10 +364,11 @@ def test_attention_largest_f16_entries(ops, heads, rows, dim):
 
 @pytest.mark.parametrize("heads,kv,dim,page,rows,own", [
     (16, 8, 64, 64, [1] * 64, [1500 + 20 * i for i in range(64)]),                  # long runs: warps that have more of it than others
-    (8, 2, 128, 64, [1 + i % 3 for i in range(300)], [i * 7 % 150 for i in range(300)]),      # more sequences than a CTA keeps; rows that see nothing
+    (8, 2, 128, 64, [1 + i % 3 for i in range(300)], [i * 7 % 150 for i in range(300)]),      # many sequences; rows that see nothing
     (32, 8, 128, 32, [300, 0, 1, 40, 700], [3000, 0, 1, 1700, 700]),                # units over several CTAs, several units a CTA
     (32, 2, 64, 16, [1 + i % 37 for i in range(70)], [1 + i % 37 + 11 * i % 90 for i in range(70)]),      # many short prompts
     (64, 1, 64, 16, [1100], [1500]),                                                # units of four rows
+    (8, 2, 64, 16, [1] * 1030, [1 + i * 7 % 50 for i in range(1030)]),              # more sequences than a CTA keeps
 ])
 def test_attention_many(ops, heads, kv, dim, page, rows, own):
     c = Cache4(sum(own), kv, dim, page, own)
