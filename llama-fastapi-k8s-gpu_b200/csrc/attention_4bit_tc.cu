@@ -423,7 +423,8 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             const int M = (int)min((long)INT_MAX, (long)walk.s.n * G), n_f = min(2 * T4_ROWS, M - walk.seg_f0), r0 = walk.s.r0, own = walk.s.own;
             const bool begins = walk.b0 == 0, ends = walk.b0 + walk.n == walk.steps;
             if (t == 1 && n_f <= T4_ROWS) {
-                __syncwarp();
+                // No rows for these warps. They go no further than two segments ahead of the other tile: arrivals of a later segment would count as ones of this phase.
+                if (seg >= 2) mbar_wait_warp(&seg_done[seg & 1], ((seg >> 1) - 1) & 1, t4_error, 0xc000fu, (unsigned)seg);
                 if (lane == 0) mbar_arrive(&seg_done[seg & 1]);
                 continue;
             }
