@@ -355,6 +355,8 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
         const int k_token = (lane >> 4) * 8 + eight, k_g = lane >> 3 & 1;                                       // of block dw
         const int v_key = NG == 4 ? dw * 8 + eight : dw * 16 + k_token, v_g = NG == 4 ? lane >> 3 : k_g;       // of 64 keys (heads of 64: four warps' work)
         const int v_token = v_key % Q4_TOKENS, v_pair = v_token >> 1;
+        // scales of groups that are no numbers: NaN and infinities; in f16 operands those too whose eightfold is past the type's range, which would be infinities there
+        constexpr uint32_t NO_NUMBER = F16 ? 0x7000 : 0x7c00;
         int it = 0, seg = 0;
         for (; walk.next(a); walk.done(a), seg++) {
             if (seg >= 2) mbar_wait_warp(&seg_done[seg & 1], ((seg >> 1) - 1) & 1, t4_error, 0xc000bu, (unsigned)seg);
@@ -371,7 +373,9 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                 for (int c = 0; c < PARTS; c++) {
 #pragma unroll
                     for (int w = 0; w < 4; w++) words[w] = *reinterpret_cast<const uint32_t*>(p + k_token * (D / 2) + (q4_key_chunk(D, k_token, w) * NG + 2 * c + k_g) * 4);
-                    t4_operands<F16>(words, *reinterpret_cast<const uint16_t*>(p + q4_scale(D, k_token, 2 * c + k_g)), hi, lo);
+                    uint32_t scale = *reinterpret_cast<const uint16_t*>(p + q4_scale(D, k_token, 2 * c + k_g));
+                    if ((scale & 0x7fffu) >= NO_NUMBER) scale = 0x7fff;
+                    t4_operands<F16>(words, scale, hi, lo);
                     if (it >= ST) mbar_wait_warp(&k_empty[st][c], (it / ST - 1) & 1, t4_error, 0xc000du, (unsigned)it);
                     put(ks + st * OPERAND + c * T4_PART + (dw * Q4_TOKENS + k_token) * 128, k_token, k_g, hi, lo);
                     fence_proxy_async();
@@ -393,7 +397,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                                                    *reinterpret_cast<const uint32_t*>(p + v_pair * D + (q4_value_chunk(D, v_pair, 2 * w + 1) * NG + v_g) * 4), v_token & 1 ? 0x7632u : 0x5410u);
                         // keys that nobody has: zeros. A value that is no number must not meet the zero weights of rows that do not see it: it is written down instead.
                         if (j0 + k >= walk.s.own) scale = 0;
-                        if ((scale & 0x7c00u) == 0x7c00u) {
+                        if ((scale & 0x7fffu) >= NO_NUMBER) {
                             atomicMin(&first_bad[seg & 1][v_g], j0 + k);
                             scale = 0;
                         }

@@ -51,3 +51,44 @@ def test_many_units_of_one_tile(ops, heads, kv, dim, page, rows, behind, max_row
     assert (near | torch.isnan(want)).all()
     again = attend(ops, c, q, rows, max_rows=R if max_rows is None else max_rows)
     assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(again))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_entries_past_f16_reach_the_rows_that_see_them(ops, dim):
+    """f16 queries, more than 64 rows a KV head: a group with an entry past 65504 reads as NaN, for the rows that see its token and no others; entries of 65504 are numbers"""
+    rows, heads = [60, 33, 100, 150], 16
+    own = [n + 30 for n in rows]
+    start = [sum(own[:s]) for s in range(len(own))]
+    g = torch.Generator().manual_seed(dim)
+    k, v = (torch.randn(sum(own), 2, dim, generator=g).bfloat16().float() for _ in range(2))
+    v[start[1] - 1, 0, 5] = 1e5                                          # the last token of sequence 0
+    v[start[1] + 40, 1, 40], v[start[1] + 40, 1, 3] = -3e38, 65504.0
+    v[start[2] + 100, 0, 33:35] = 65536.0
+    v[start[2] + 3, 1, 60] = 65504.0
+    k[start[3] + 120, 1, 7] = 2e5
+    k[start[3] + 130, 0, 7] = 65504.0
+    c = Cache4(2, 2, dim, 16, own, k=k, v=v, fill=0xff)
+    q = (torch.randn(sum(rows), heads, dim, generator=c.g)).half()
+    q[..., 7] *= 1e-4
+    q = q.cuda()
+    keys, values = c.values(c.k), c.values(c.v)
+    for x in (keys, values):
+        groups = x.unflatten(-1, (-1, 32))
+        groups[(groups.abs() > 65519.0).any(-1)] = math.nan
+    got = attend(ops, c, q, rows)
+    want, sizes = visible_nan(c, q, rows, keys, values)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and not torch.isinf(got).any() and torch.isnan(want).any()
+    # (a row that sees a number is held to the bar of the numbers that it sees)
+    seen = torch.nan_to_num(torch.stack(sizes_of_what_rows_see(c, q, rows, keys, values)))
+    bar = attention_bar("f16", torch.nan_to_num(want), seen[0], seen[1], sizes[2], seen[2], dim, True)
+    assert ((got.to(F64) - want).abs() <= bar)[~torch.isnan(want)].all() and ops.error(0) == 0
+
+
+def sizes_of_what_rows_see(c, q, rows, k, v):
+    """attention_exact's spread, offset and all_v with the groups that are no numbers left out"""
+    k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+    clean = Cache4.__new__(Cache4)
+    clean.__dict__.update(c.__dict__)
+    clean.k, clean.v = k.cpu().float(), v.cpu().float()
+    _, spread, offset, _, all_v = attention_exact(clean, q, rows, k=k, v=v)
+    return spread, offset, all_v
