@@ -7,7 +7,7 @@
 // score tiles (probabilities are written over them) and two outputs.
 //
 // A value s (c - 8) has up to 14 bits, an f16 or bf16 operand 11 or 8. Rounded, keys would be off by 2^-12 each, and a score by more than all else together (relative error of the output
-// 3.5e-4 from the keys alone, 1.8e-4 from the values, where the output's own rounding to f16 is 2.1e-4). So keys and values are two operands each, exact to 2^-14 or better: with the upper
+// 3.5e-4 from the keys alone, 1.8e-4 from the values, where the output's own rounding to f16 is 2.1e-4). So keys and values are two operands each, both exact: with the upper
 // bits of the scale, and with the rest of it. That doubles the products, which then are what this is bound by: 2048 rows behind 6000 tokens, 32 heads over 8 of 128, 352 us, 670 TFLOP/s of
 // what is asked for and twice as much of what is done. Probabilities are rounded to the queries' type.
 #include "attention_4bit.cuh"
@@ -98,7 +98,8 @@ struct T4Walk {
     }
 };
 
-// A group's scale in two parts of the operands' type, each twice: the upper ones of its bits (f16: 7, bf16: 5), so that a code times them is exact, and the others
+// A group's scale in two parts of the operands' type, each twice, so that a code (3 bits, or a power of two) times either is exact. f16, 11 bits: the upper 7 of the scale's 11 bits, and the
+// other 4. bf16, 8 bits: rounded to 5, and what is left: 32 of the scale's last place at most, 5 bits.
 template <bool F16>
 struct T4Scale {
     uint32_t hi, lo;
@@ -109,7 +110,8 @@ struct T4Scale {
             const __half2 rest = __hsub2(*reinterpret_cast<const __half2*>(&two), *reinterpret_cast<const __half2*>(&hi));
             lo = *reinterpret_cast<const uint32_t*>(&rest);
         } else {
-            const float s = __half2float(__ushort_as_half((uint16_t)bits)), up = __uint_as_float(__float_as_uint(s) & 0xfff80000u);
+            // (a NaN may become a number in `up`; the rest is a NaN then)
+            const float s = __half2float(__ushort_as_half((uint16_t)bits)), up = __uint_as_float((__float_as_uint(s) + 0x40000u) & 0xfff80000u);
             hi = __byte_perm(__float_as_uint(up), 0, 0x3232);
             lo = t4_pack<false>(s - up, s - up);
         }

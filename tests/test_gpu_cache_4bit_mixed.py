@@ -92,3 +92,36 @@ def sizes_of_what_rows_see(c, q, rows, k, v):
     clean.k, clean.v = k.cpu().float(), v.cpu().float()
     _, spread, offset, _, all_v = attention_exact(clean, q, rows, k=k, v=v)
     return spread, offset, all_v
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,n", [(8, 1), (64, 2)])
+def test_one_token_comes_back(ops, heads, n, dim, typ):
+    """a row that sees one token has that token's value, scale * (code - 8) rounded once, whichever way it goes"""
+    kv = 8
+    c = Cache4(dim + heads, kv, dim, 16, [n] * 40)
+    q = torch.randn(40 * n, heads, dim, generator=c.g).to(TYPES[typ]).cuda()
+    got = attend(ops, c, q, [n] * 40, max_rows=n if n == 1 else 40 * n)
+    want = c.values(c.v)[::n].float().to(TYPES[typ])                     # (15 bits: exact in 32)
+    assert torch.equal(got[::n], want.repeat_interleave(heads // kv, 1))
+
+
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+def test_scores_of_many_rows_are_exact_products(ops, typ):
+    """keys whose scales have all their 11 bits, queries of one entry: scores are scale * (code - 8) * query to the bits of 32, weights what they say"""
+    rows, heads, dim = [40, 30], 8, 64
+    own = [n + 60 for n in rows]
+    T = sum(own)
+    s = 1 + (33 + 2 * (torch.arange(T) % 16)).float() / 1024             # 11 bits, the last one set
+    k = torch.zeros(T, 2, dim)
+    k[:, :, 3], k[:, :, 5] = -8 * s[:, None], 7 * s[:, None]             # codes 0 and 15
+    c = Cache4(12, 2, dim, 16, own, k=k)
+    q = torch.zeros(sum(rows), heads, dim)
+    q[..., 5] = 1.0 + torch.arange(heads) / 8
+    q = q.to(TYPES[typ]).cuda()
+    got = attend(ops, c, q, rows, scale=64.0)
+    want, spread, offset, reach, all_v = attention_exact(c, q, rows, scale=64.0)
+    # one product and one sum in 32 bits, both exact, the difference to the row's largest times the scale: 2^-22 of it
+    reach = 7 * 2 * 64.0 * 2 * torch.ones_like(reach) * 2 ** -22 / (4 * (dim + 16) * 2 ** -24)
+    assert ((got.to(F64) - want).abs() <= attention_bar(typ, want, spread, offset, reach, all_v, dim, True)).all()
