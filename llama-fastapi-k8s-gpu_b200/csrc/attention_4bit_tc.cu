@@ -465,7 +465,10 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             mbar_arrive(&q_full[t]);
             float m_ref = -INFINITY;
             uint64_t l2 = f2_pack(0.f, 0.f), l3 = l2;            // sums of even and odd entries, twice
-            const uint64_t scale2 = f2_pack(a.scale_log2, a.scale_log2);
+            // Weights are held 2^7 times as large in f16, 2^15 at most (the reference lags by 2^8): the smallest f16 number is then 2^-31 of the weight at the reference, and many small ones that
+            // count in the divisor count above it too. Sums and outputs have the same factor.
+            constexpr float UP = F16 ? 7.f : 0.f;
+            const uint64_t scale2 = f2_pack(a.scale_log2, a.scale_log2), up2 = f2_pack(UP, UP);
             for (int i = 0; i < walk.n; i++, done++) {
                 mbar_wait(&s_full[t], done & 1, t4_error, 0xc0006u, done);
                 tc_after_sync();
@@ -527,7 +530,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
                         uint32_t p[16];
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
-                            const float2 d = f2_unpack(f2_mul(f2_add(f2_pack(__uint_as_float(x[u][j]), __uint_as_float(x[u][j + 1])), ref2), scale2));
+                            const float2 d = f2_unpack(f2_fma(f2_add(f2_pack(__uint_as_float(x[u][j]), __uint_as_float(x[u][j + 1])), ref2), scale2, up2));
                             const float e0 = t4_exp2(d.x), e1 = t4_exp2(d.y);
                             if (j & 2) l3 = f2_add(l3, f2_pack(e0, e1)); else l2 = f2_add(l2, f2_pack(e0, e1));
                             p[j >> 1] = t4_pack<F16>(e0, e1);

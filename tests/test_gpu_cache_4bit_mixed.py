@@ -125,3 +125,28 @@ def test_scores_of_many_rows_are_exact_products(ops, typ):
     # one product and one sum in 32 bits, both exact, the difference to the row's largest times the scale: 2^-22 of it
     reach = 7 * 2 * 64.0 * 2 * torch.ones_like(reach) * 2 ** -22 / (4 * (dim + 16) * 2 ** -24)
     assert ((got.to(F64) - want).abs() <= attention_bar(typ, want, spread, offset, reach, all_v, dim, True)).all()
+
+
+@pytest.mark.parametrize("at", [0, 99980])
+def test_many_small_weights(ops, at):
+    """one key has the row's largest score by far, 100000 others share what is left: 2^-25.02 of its weight each, 0.3 % together. A weight may be off by 2^-31 of the largest one's and by a
+    rounding of itself, all of them together by 2^-14. As many sequences as a CTA needs to have most of one's keys, all with the same pages."""
+    n, kv, seqs = 100000, 8, 20
+    k, v = torch.zeros(n, kv, 64), torch.ones(n, kv, 64)
+    k[at, :, 0], v[at] = 17.34375, 0.0                                   # 25.02 ln 2
+    c = Cache4(13, kv, 64, 64, [n], k=k, v=v)
+    one, many = c.pages, c.pages.expand(seqs, -1).contiguous()
+    q = torch.zeros(9, 8 * kv, 64)
+    q[..., 0] = 1.0
+    for rows in (1, 9):
+        x = q[:rows].cuda()
+        c.pages = one
+        want, spread, *_ = attention_exact(c, x, [rows], scale=1.0)
+        assert (want / (n * math.exp(-17.34375)) - 1).abs().max() < 0.01
+        c.pages = many
+        for typ in ("f16", "bf16"):
+            got = attend(ops, c, x.to(TYPES[typ]).repeat(seqs, 1, 1), [rows] * seqs, scale=1.0, own=[n] * seqs)
+            # (sums and scores in 32 bits: 2^-14 as elsewhere)
+            unit = torch.finfo(TYPES[typ]).eps / 2
+            off = (got.view(seqs, *x.shape).to(F64) - want).abs()
+            assert (off <= unit * want + (unit + 2 ** -14) * spread + (2 ** -14 if typ == "f16" else 0)).all(), (rows, typ, float(got.min()), float(want.min()))
