@@ -4,7 +4,8 @@
 //
 // A warp works by itself: it has its own ring of steps of 32 keys, its own copies, and keeps the weighted sums of all dims. The steps of all (sequence, KV head, tile of rows)
 // laid end to end are cut into equal runs, one a warp; a run that begins or ends inside such a segment leaves a partial result (maximum, sum, weighted sum, 32 bits) there.
-// The CTA's warps join theirs through shared memory at the end, a small kernel joins those of several CTAs. All joins go in the order of the keys.
+// The CTA's warps join theirs through shared memory at the end, a small kernel joins those of several CTAs. All joins have an order that the call's sizes and lengths give, so that the same
+// call has the same bits.
 //
 // Products are transposed, keys (dims) times rows, so that eight rows fill an instruction: mma.sync m16n8k16.
 //   scores: the operand of the keys is the codes c themselves as the subnormal f16 numbers c 2^-24 (c 2^-20 for every other one, where the query's entry is 1/16 of itself): a mask
@@ -14,7 +15,8 @@
 //     to f16 once (2^-11), whatever the type of queries and output; the offset of 8 is a product of that operand and a constant. Scales are taken at a power of two that keeps the
 //     operand in f16's range, found from the scales as they come. Score fragments become operands by movmatrix.
 // The reference of a row's exponentials moves only where a score exceeds it by 2^6. It is a score before it is scaled, so that the largest one's difference is exact however large it is (one
-// fused multiply-add with a scaled reference would save an instruction a score, and be off by as much as the reference's last place).
+// fused multiply-add with a scaled reference would save an instruction a score, and be off by as much as the reference's last place). Partial results have a scaled one, and what it is off by
+// in their sums (a4_rest).
 // Measured (32 heads over 8 of 128, f16): 256 chats of 16 to 4100 tokens 141 us, 4.4 TB/s of what has to be read, 0.66 of a copy's; 32 chats of 20 to 1500 16.5, one of 32000 18.6, of 700 8.5. A step is
 // some 600 instructions, issued one in two cycles by the twelve warps that fit an SM: those of unpacking (160) and of the values' weights (100) are the most. More CTAs than fit were a fifth slower, four an
 // SM with 128 registers a tenth, the next step's scores beside this one's values a tenth; products in other orders were the same, and so were larger shares for the CTAs that an SM serves first. A call
@@ -151,7 +153,7 @@ struct A4Cut {
     }
 };
 
-// partial results in 32 bits: [rows of a tile][D] weighted sums, then [rows][2] (reference in log2, sum)
+// partial results in 32 bits: [rows of a tile][D] weighted sums, then [rows][2] (reference in log2, sum), see a4_rest
 template <int D> __host__ __device__ constexpr int a4_part(int mt) { return mt * (D + 2); }
 
 // results of the same row over different keys, added up
@@ -596,8 +598,15 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             copy();
             if (++st == S) { st = 0; parity ^= 1; }
         }
-        // the sums as they are
-        const float by_l = a4_exp2(-up_v), down_v = by_l * 0x1p24f;
+        // the sums as they are, for the reference times `by` as it is rounded where they are a partial result's
+        float scaled[NT][2], by_l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                scaled[nt][j] = ref[nt][j] * by[nt][j];
+                by_l[nt][j] = a4_exp2(begins && ends ? -up_v : a4_rest(ref[nt][j], by[nt][j], scaled[nt][j]) - up_v);
+            }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -605,7 +614,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 #pragma unroll
                 for (int m = 0; m < 2; m++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) o[nt][gi][m][e] *= e & 2 ? down_v * 0.0625f : down_v;
+                    for (int e = 0; e < 4; e++) o[nt][gi][m][e] *= by_l[nt][e & 1] * (e & 2 ? 0x1p20f : 0x1p24f);
         u += n;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
@@ -614,7 +623,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 #pragma unroll
                 for (int d = 4; d < 32; d *= 2) l[nt][j] += __shfl_xor_sync(0xffffffffu, l[nt][j], d);
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) { l[nt][0] *= by_l; l[nt][1] *= by_l; }
+        for (int nt = 0; nt < NT; nt++) { l[nt][0] *= by_l[nt][0]; l[nt][1] *= by_l[nt][1]; }
         // ---- output, or a result for the joins
         const int slot = begins ? 1 : 0;
         float* part_at = begins ? reinterpret_cast<float*>(ring) : head_part + warp * PART;      // (a segment that goes on is the run's last: no copy is under way)
@@ -635,7 +644,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 #pragma unroll
                     for (int gi = 0; gi < NG; gi++)
                         *reinterpret_cast<float4*>(part_at + row * D + gi * Q4_GROUP + 4 * g) = make_float4(o[nt][gi][0][j], o[nt][gi][0][j + 2], o[nt][gi][1][j], o[nt][gi][1][j + 2]);
-                    if (g == 0) *reinterpret_cast<float2*>(part_at + MT * D + row * 2) = make_float2(l[nt][j] == 0.f ? -INFINITY : ref[nt][j] * by[nt][j], l[nt][j]);
+                    if (g == 0) *reinterpret_cast<float2*>(part_at + MT * D + row * 2) = make_float2(l[nt][j] == 0.f ? -INFINITY : scaled[nt][j], l[nt][j]);
                 }
             }
         if (!(begins && ends) && lane == 0) {
@@ -691,7 +700,7 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
 }
 
 // The results of a segment that lies in several CTAs, from the one where it begins on: a CTA has up to 16 rows, a row the lanes of a warp (half of one for heads of 64), four dims each; where
-// there are fewer rows, a row that many times, the CTAs shared among them. (A row a CTA is bound by the start of CTAs, 1.1 ns each: 41 us for 148 tiles of 256 rows.)
+// there are fewer rows, a row that many times, every so many-th of the segment's CTAs for each. (A row a CTA is bound by the start of CTAs, 1.1 ns each: 41 us for 148 tiles of 256 rows.)
 template <int D, int MT>
 __global__ void __launch_bounds__(a4_join_threads(MT), 1024 / a4_join_threads(MT)) attention_4bit_join_kernel(const Attention4Args a, const int ctas) {
     constexpr int PART = a4_part<D>(MT), LANES = D / 4, THREADS = a4_join_threads(MT), ROWS = a4_join_rows(MT), GROUPS = THREADS / LANES, B = MT > 16 ? 4 : 8;

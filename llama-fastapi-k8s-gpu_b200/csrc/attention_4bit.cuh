@@ -13,6 +13,9 @@ __device__ __forceinline__ int a4_row(const Attention4Args& a, unsigned f) {
     const unsigned i = __umulhi(f, a.per_group);
     return (int)(i + (f - i * (unsigned)a.group >= (unsigned)a.group));
 }
+// A partial result has its reference in log2, rounded: reference * by. What that is off by, in log2, goes into its sums, so that weights between partial results are those of the exact references.
+// (Held to 2^60: scores of up to 2^84. A reference of none, less infinity or with sums that are NaN, gives some number.)
+__device__ __forceinline__ float a4_rest(float ref, float by, float scaled) { return fminf(fmaxf(fmaf(ref, by, -scaled), -60.f), 60.f); }
 // four neighbouring dims of a row's output
 __device__ __forceinline__ void a4_store_out(const Attention4Args& a, int t, int head, int d, float x, float y, float z, float w) {
     uint32_t lo, hi;

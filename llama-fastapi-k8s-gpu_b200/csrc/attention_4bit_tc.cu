@@ -549,7 +549,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             const float2 la = f2_unpack(l2), lb = f2_unpack(l3);
             const float l = (la.x + la.y) + (lb.x + lb.y);
             const bool whole = begins && ends;
-            const float by = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;      // (0: no keys. A NaN stays one.)
+            const float scaled = m_ref * a.scale_log2, rest = t4_exp2(a4_rest(m_ref, a.scale_log2, scaled)), by = !whole ? rest : l == 0.f ? 0.f : 1.f / l;      // (0: no keys. A NaN stays one.)
             const int slot = begins ? 1 : 0;
             float* part = a.work + ((size_t)blockIdx.x * 2 + slot) * PART;
             // 32 columns at a time through the part of shared memory that held the warp's queries (nothing reads them any more), so that a row's columns leave side by side
@@ -581,7 +581,7 @@ __global__ void __launch_bounds__(T4_THREADS, 1) attention_4bit_tc_kernel(const 
             }
             if (!whole) {
                 open[slot] = true;
-                if (in) *reinterpret_cast<float2*>(part + 2 * T4_ROWS * D + (t * T4_ROWS + (warp & 3) * 32 + lane) * 2) = make_float2(m_ref * a.scale_log2, l);
+                if (in) *reinterpret_cast<float2*>(part + 2 * T4_ROWS * D + (t * T4_ROWS + (warp & 3) * 32 + lane) * 2) = make_float2(scaled, l * rest);
                 if (t == 0 && warp == 0 && lane == 0) {
                     const long last = given + walk.steps - walk.b0 - 1, run = run_shared[0], longer = run_shared[1], most = longer * (run + 1);
                     desc[slot] = {n_f, r0, walk.seg_f0, walk.seg_kvh, (int)(last < most ? last / (run + 1) : longer + (last - most) / run)};

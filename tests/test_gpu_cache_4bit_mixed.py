@@ -150,3 +150,23 @@ def test_many_small_weights(ops, at):
             unit = torch.finfo(TYPES[typ]).eps / 2
             off = (got.view(seqs, *x.shape).to(F64) - want).abs()
             assert (off <= unit * want + (unit + 2 ** -14) * spread + (2 ** -14 if typ == "f16" else 0)).all(), (rows, typ, float(got.min()), float(want.min()))
+
+
+@pytest.mark.parametrize("heads,rows", [(4, [1]), (32, [1]), (16, [9])])
+@pytest.mark.parametrize("first,second", [(5, 2985), (2985, 5), (1000, 1040), (700, 2000), (40, 200)])
+@pytest.mark.parametrize("of", [0, 3, 5])
+def test_large_scores_in_different_partial_results(ops, heads, rows, first, second, of):
+    """two keys with scores of 2^22 and more, one apart, wherever partial results of the keys are cut: weights of 1 and e"""
+    n = sum(rows)
+    own, dim = [3000 + n], 64
+    k, v = torch.zeros(own[0], 2, dim), torch.zeros(own[0], 2, dim)
+    k[[first, second], :, 0] = 2048.0
+    k[second, :, 40] = 1.0
+    v[first], v[second] = 1.0, -1.0
+    c = Cache4(14, 2, dim, 64, own, k=k, v=v)
+    q = torch.zeros(n, heads, dim)
+    q[..., 0], q[..., 40] = 2048.0 * (1 + of / 8), 1.0
+    q = q.half().cuda()
+    got = attend(ops, c, q, rows, scale=1.0)
+    want = (1 - math.e) / (1 + math.e)
+    assert ((got.to(F64) - want).abs() <= 2 ** -9).all(), float(got[0, 0, 0])
