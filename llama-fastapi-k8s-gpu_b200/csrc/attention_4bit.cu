@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(A4_THREADS, a4_per_sm(NT)) attention_4bit_step
             const int ex = max((int)(__float_as_uint(top) >> 23) - 127, -100);
             const float up = __uint_as_float((uint32_t)(137 - ex) << 23);                // 2^(10 - ex)
             const int ex1 = (ex + 14) >> 1, ex2 = ex + 14 - ex1;                         // (2^24 of the codes, 2^(ex - 10) of the queries, in two steps: each is a normal number)
-            const float mine = a.scale_log2 * __uint_as_float((uint32_t)(127 + ex1) << 23) * __uint_as_float((uint32_t)(127 + ex2) << 23);
+            // (held to the largest number: no difference times it then is still none, and any other one far past every exponent)
+            const float mine = fminf(a.scale_log2 * __uint_as_float((uint32_t)(127 + ex1) << 23) * __uint_as_float((uint32_t)(127 + ex2) << 23), FLT_MAX);
 #pragma unroll
             for (int j = 0; j < 2; j++) by[nt][j] = __shfl_sync(0xffffffffu, mine, (2 * tq + j) * 4);
 #pragma unroll

@@ -170,3 +170,21 @@ def test_large_scores_in_different_partial_results(ops, heads, rows, first, seco
     got = attend(ops, c, q, rows, scale=1.0)
     want = (1 - math.e) / (1 + math.e)
     assert ((got.to(F64) - want).abs() <= 2 ** -9).all(), float(got[0, 0, 0])
+
+
+@pytest.mark.parametrize("heads,rows", [(4, [1, 1]), (16, [9, 12])])
+def test_large_queries_and_scale(ops, heads, rows):
+    """queries of 2^100 and a scale of 2^20, scores that 32 bits hold: all weight on the largest"""
+    own = [200 + n for n in rows]
+    T = sum(own)
+    k = torch.zeros(T, 2, 64)
+    k[:, :, 9] = 8.0
+    k[:, :, 3] = (torch.arange(T) % 15 - 7).float()[:, None]             # codes 1 .. 15
+    c = Cache4(15, 2, 64, 16, own, k=k)
+    q = torch.zeros(sum(rows), heads, 64)
+    q[..., 3] = 2.0 ** 100
+    q = q.bfloat16().cuda()
+    got = attend(ops, c, q, rows, scale=2.0 ** 20)
+    want, *_ = attention_exact(c, q, rows, scale=2.0 ** 20)
+    _, spread, *_ = attention_exact(c, q, rows, scale=2.0 ** 20)
+    assert ((got.to(F64) - want).abs() <= 2 ** -9 * want.abs() + (2 ** -9 + 2 ** -10) * spread + 2 ** -20).all()
