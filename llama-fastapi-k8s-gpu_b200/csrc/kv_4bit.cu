@@ -59,10 +59,10 @@ __device__ __forceinline__ void k4_store(float* p, bool wide, const float (&x)[8
         for (int e = 0; e < 8; e++) p[e] = x[e];
 }
 
-// The place of a row: whether it belongs to a sequence, its token number there, and the first byte of KV head 0's block of 16 tokens, or -1; by a whole warp. Up to 32 sequences: their
-// starts and lengths in one read.
+// The place of a row: whether it belongs to a sequence, its token number there (its last 32 bits; `number`: all of it, which lengths near -2^31 need), and the first byte of KV head 0's block
+// of 16 tokens, or -1; by a whole warp. Up to 32 sequences: their starts and lengths in one read.
 struct K4Place { int live, token; long block; };
-__device__ __forceinline__ K4Place k4_place(const RaggedPages& r, int n_kv, int dim, int row, int lane) {
+__device__ __forceinline__ K4Place k4_place(const RaggedPages& r, int n_kv, int dim, int row, int lane, long* number = nullptr) {
     int s, end = 0, held = 0;
     const int first = r.row_start[0];
     if (r.n_seqs <= 32) {
@@ -79,6 +79,7 @@ __device__ __forceinline__ K4Place k4_place(const RaggedPages& r, int n_kv, int 
     if (!p.live) return p;
     const long at = (long)held - ((long)end - row);
     p.token = (int)at;
+    if (number) *number = at;
     if (at < 0 || at >= (long)r.max_pages * r.block_tokens) return p;      // (below 2^31)
     const unsigned block = (unsigned)at / Q4_TOKENS, blocks = (unsigned)r.block_tokens / Q4_TOKENS, page_no = block / blocks;
     const int page = r.pages[s * r.table_stride + page_no];
@@ -187,9 +188,10 @@ __global__ void __launch_bounds__(K4_THREADS, 4) kv_append_4bit_kernel(const KvA
         for (int u = 0; u < UNROLL; u++) load(x[u], y[u]);
         if (!ready) {                                            // (the first entries are under way)
             ready = true;
-            place = k4_place(a.r, a.n_kv, D, (int)row, lane);
+            long number = 0;
+            place = k4_place(a.r, a.n_kv, D, (int)row, lane, &number);
             if (!place.live) return false;
-            const double pos = (double)(a.first_pos + place.token);
+            const double pos = (double)(a.first_pos + number);
             for (int j = lane; j < half; j += 32) {
                 const double t = pos * (double)a.freqs[j] * 0.15915494309189533577;      // 1 / (2 pi)
                 double sn, cs;

@@ -188,3 +188,24 @@ def test_large_queries_and_scale(ops, heads, rows):
     want, *_ = attention_exact(c, q, rows, scale=2.0 ** 20)
     _, spread, *_ = attention_exact(c, q, rows, scale=2.0 ** 20)
     assert ((got.to(F64) - want).abs() <= 2 ** -9 * want.abs() + (2 ** -9 + 2 ** -10) * spread + 2 ** -20).all()
+
+
+@pytest.mark.parametrize("seqs", [1, 40])
+def test_queries_of_rows_far_ahead_of_their_tokens(ops, seqs):
+    """rows without a place are rotated by their position all the same, whatever the length: one below -2^31 does not wrap"""
+    c = Cache4(18, 2, 64, 16, [16] * seqs)
+    n = 5
+    x = torch.randn(n * seqs, 2, 64, generator=c.g).cuda()
+    freqs = (2.0 ** (-28 - torch.arange(32) / 8)).float().cuda()
+    pos = (torch.arange(n) - n - 2 ** 31).repeat(seqs).cuda()
+    outs = []
+    for first in (0, 2 ** 33):
+        q_out = torch.zeros(n * seqs, 2, 64, dtype=torch.float16, device="cuda")
+        ops.kv_append_4bit(x, x, c.k_pool, c.v_pool, c.pages, c.ints(range(0, n * seqs + 1, n)), c.ints([-2 ** 31] * seqs), q=x, q_out=q_out, freqs=freqs, first_pos=first)
+        angle = (pos + first).to(F64)[:, None] * freqs.to(F64)
+        cos, sin = angle.cos()[:, None], angle.sin()[:, None]
+        a, b = x[..., 0::2].to(F64), x[..., 1::2].to(F64)
+        want = torch.stack([a * cos - b * sin, a * sin + b * cos], -1).flatten(-2)
+        assert ((q_out.to(F64) - want).abs() <= 2 ** -11 * want.abs() + 2 ** -20).all()
+        outs.append(q_out)
+    assert torch.equal(c.k_pool.cpu(), c.bytes_k) and not torch.equal(*outs)
