@@ -3,10 +3,14 @@
 // multiply-add): which code an entry gets is decided at borders, and so it follows from the definition alone, whatever rotates the keys.
 //
 // A warp takes a row, or a part of its heads where the rows are few, and finds its place by itself; a lane has a piece of eight entries of a head, 32 bits of codes, and four
-// neighbouring lanes have a group. Reads are bound by memory and by the chain that each row begins with (sequence, page, codes), so as many warps as an SM holds have two turns of pieces each
-// under way: 65536 rows of 2 x 8 heads of 128 to f16 67 us, 0.78 of the measured bandwidth (four turns and half the warps 78), 37000 ragged rows of 2 x 5 heads to bf16 30. Appends are bound by
-// instructions as much as by memory, 3500 a row of 32 + 2 x 8 heads of 128: 16384 such rows 93 us, 3.8 TB/s, 32 rows 5.2. (More
-// turns of queries under way, one CTA an SM more or fewer: 1 to 6 % slower.)
+// neighbouring lanes have a group.
+// Reads are bound by memory and by the chain that each row begins with (sequence, page, codes), so as many warps as an SM holds have two turns of pieces each under way, at 32 registers, which
+// spill 5 to 14 words a thread: 65536 rows of 2 x 8 heads of 128 to f16 66 us, 0.79 of the measured bandwidth (four turns and half the warps 78), to f32 135, 37000 ragged rows of 2 x 5 heads to bf16
+// 29.6. A warp takes 16 of the 32 bits that a word of values has, its neighbour's token the others. (Two rows a warp, both places found at once: 29.3 for those 37000 rows, 144 to f32, 23.1
+// instead of 22.5 for 20000 rows of 8 heads to f16.)
+// Appends wait: 16384 rows of 32 + 2 x 8 heads of 128 take 93 us, 3500 instructions a row at 0.60 of the issue slots, 3.8 TB/s or 0.58 of the measured bandwidth, and the largest stall is that of
+// entries on their way, with the 17 warps of an SM that run at 64 registers on average. 32 rows 5.2 us: their chain, and the turns of a row one after the other. (More turns of queries under way, one CTA
+// an SM more or fewer: 1 to 6 % slower.)
 #include "device_ops.h"
 #include "kv_4bit.cuh"
 #include "ptx.cuh"
@@ -311,24 +315,17 @@ __device__ __forceinline__ void k4_put(Out* p, bool wide, const __half2 (&v)[4],
     k4_store(p, wide, x);
 }
 
-// ROWS: rows of a warp, whose places are found at once
-template <typename Out, int D, int ROWS>
+template <typename Out, int D>
 __global__ void __launch_bounds__(K4_THREADS, 8) kv_read_4bit_kernel(const KvReadArgs a, const int wide, const int parts) {
     constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, UNROLL = 2;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long item = (long)blockIdx.x * K4_WARPS + warp, row0 = (item >> parts) * ROWS;
+    const long item = (long)blockIdx.x * K4_WARPS + warp, row = item >> parts;
     griddep_wait();
     griddep_launch();
-    if (row0 >= a.r.n_rows) return;
-    K4Place places[ROWS];
-#pragma unroll
-    for (int i = 0; i < ROWS; i++) places[i] = k4_place(a.r, a.n_kv, D, (int)min(row0 + i, (long)a.r.n_rows - 1), lane);
-    const int part = (int)(item - (item >> parts << parts));
-#pragma unroll
-    for (int r = 0; r < ROWS; r++) {
-    const long row = row0 + r;
-    const K4Place place = places[r];
-    if (row >= a.r.n_rows || place.block < 0) continue;
+    if (row >= a.r.n_rows) return;
+    const K4Place place = k4_place(a.r, a.n_kv, D, (int)row, lane);
+    if (place.block < 0) return;
+    const int part = (int)(item - (row << parts));
     const int token = place.token & (Q4_TOKENS - 1), w = lane % PIECES, h0 = lane / PIECES;
     const int all = (a.n_kv + AT_ONCE - 1) / AT_ONCE, first = all * part >> parts, last = all * (part + 1) >> parts;
     const long step = (long)(a.r.block_tokens / Q4_TOKENS) * q4_block(D), begin = place.block + (first * AT_ONCE + h0) * step;
@@ -359,7 +356,6 @@ __global__ void __launch_bounds__(K4_THREADS, 8) kv_read_4bit_kernel(const KvRea
             k += AT_ONCE * a.k_head; v += AT_ONCE * a.v_head;
         }
     }
-    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -386,9 +382,7 @@ cudaError_t kv_append_4bit_launch(const KvAppendArgs& a, cudaStream_t s) {
 template <typename Out, int D>
 static cudaError_t k4_read(const KvReadArgs& a, cudaStream_t s) {
     const int parts = k4_parts(a.r.n_rows, a.n_kv * D / 8), wide = k4_wide(a.k, a.k_row, a.k_head, sizeof(Out)) | k4_wide(a.v, a.v_row, a.v_head, sizeof(Out)) << 1;
-    // two rows a warp once that leaves a warp for every place on the SMs, one below: 37000 rows of 5 heads 29.9 and 30.2 us, 16384 rows of 8 heads 32.7 and 17.0
-    if (a.r.n_rows >= 2 * 148 * 64) return launch_chain(kv_read_4bit_kernel<Out, D, 2>, dim3(k4_ctas((a.r.n_rows + 1) / 2, 0)), dim3(K4_THREADS), 0, s, a, wide, 0);
-    return launch_chain(kv_read_4bit_kernel<Out, D, 1>, dim3(k4_ctas(a.r.n_rows, parts)), dim3(K4_THREADS), 0, s, a, wide, parts);
+    return launch_chain(kv_read_4bit_kernel<Out, D>, dim3(k4_ctas(a.r.n_rows, parts)), dim3(K4_THREADS), 0, s, a, wide, parts);
 }
 template <typename Out>
 static cudaError_t k4_read_dim(const KvReadArgs& a, cudaStream_t s) { return a.head_dim == 64 ? k4_read<Out, 64>(a, s) : k4_read<Out, 128>(a, s); }
