@@ -190,6 +190,38 @@ def test_large_queries_and_scale(ops, heads, rows):
     assert ((got.to(F64) - want).abs() <= 2 ** -9 * want.abs() + (2 ** -9 + 2 ** -10) * spread + 2 ** -20).all()
 
 
+@pytest.mark.parametrize("typ", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,rows", [(4, [1, 1, 1]), (16, [2, 9, 5]), (16, [60, 33, 100])])
+def test_lengths_past_the_tables(ops, heads, rows, typ):
+    """lengths past the table mean all that it holds, to the bit and by the definition"""
+    full = [208] * 3
+    c = Cache4(16, 2, 64, 16, full, "bf16")
+    c.pages = c.pages[:, :13].contiguous()
+    q = torch.randn(sum(rows), heads, 64, generator=c.g).to(TYPES[typ]).cuda()
+    held = attend(ops, c, q, rows)
+    assert torch.isfinite(held).all()
+    want, *sizes = attention_exact(c, q, rows)
+    assert ((held.to(F64) - want).abs() <= attention_bar(typ, want, *sizes, 64, max(rows) * heads // 2 > 64)).all()
+    for lengths in ([2 ** 31 - 1, 209, 10 ** 9], [224, 2 ** 31 - 1, 208]):
+        assert torch.equal(attend(ops, c, q, rows, own=lengths), held)
+
+
+@pytest.mark.parametrize("heads,rows", [(4, [1, 1, 1]), (16, [2, 9, 5]), (16, [60, 33, 100])])
+def test_page_ids_outside_the_pool(ops, heads, rows):
+    """they are held inside it: the first page and the last, to the bit and by the definition"""
+    own = [n + 20 for n in rows]
+    c = Cache4(17, 2, 64, 16, own, fill=0)
+    q = torch.randn(sum(rows), heads, 64, generator=c.g).half().cuda()
+    held = c.pages.clone()
+    held[0, 0], held[1, 0], held[2, 0] = 0, len(c.bytes_k) - 1, 0
+    c.pages = held
+    inside = attend(ops, c, q, rows)
+    assert torch.isfinite(inside).all() and inside.abs().sum() > 0
+    c.pages = held.clone()
+    c.pages[0, 0], c.pages[1, 0], c.pages[2, 0] = -5, 2 ** 31 - 1, -2 ** 31
+    assert torch.equal(attend(ops, c, q, rows), inside)
+
+
 @pytest.mark.parametrize("seqs", [1, 40])
 def test_queries_of_rows_far_ahead_of_their_tokens(ops, seqs):
     """rows without a place are rotated by their position all the same, whatever the length: one below -2^31 does not wrap"""
