@@ -503,13 +503,15 @@ int b2_kv_read_4bit(int device, const b2_ragged_pages* where, const b2_kv_read_4
 
 /* Attention of a ragged batch over a cache in 4 bits: row i of a sequence sees its tokens up to itself.
  * out = softmax(scale * q.k) v over them, 0 where there are none. Queries and output are f16 or bf16; scores, maxima and sums
- * are 32-bit. For the weighted sum a probability times its value's scale is rounded to f16, or, with more than 64 rows
- * times heads a KV head, a probability to the queries' type; with f16 queries a group with an entry past f16's range then
- * counts as NaN. A NaN in a value
- * makes the same dims of its group NaN in the rows that see it, one in a key all dims. max_rows: most rows any sequence has (rows
- * past it are not computed); 1 for single tokens. Page ids are held inside the pool. n_head a multiple of n_kv, at most 64
- * times it. Lengths may be smaller than a sequence's rows (the rows ahead see nothing). Partial results of keys go
- * through the workspace, 16-byte aligned. */
+ * are 32-bit. max_rows: most rows any sequence has (rows past it are not computed); 1 for single tokens. Page ids are held
+ * inside the pool. n_head a multiple of n_kv, at most 64 times it. Lengths may be smaller than a sequence's rows (the rows
+ * ahead see nothing); past its table they are all that it holds. Partial results of keys go through the workspace, 16-byte
+ * aligned. A NaN in a value makes the same dims of its group NaN in the rows that see it, one in a key all dims.
+ * The call as a whole goes one of two ways. Up to 64 for max_rows * n_head / n_kv: a probability times its value's scale is
+ * rounded to f16 (below 2^-20 of the KV head's largest scale with fewer bits), bf16 queries to f16 at a power of two for a row
+ * (entries below 2^-23 of its largest with fewer bits). More: probabilities are rounded to the queries' type, and with f16
+ * queries a group with an entry past f16's range counts as NaN. Single tokens cost several times as much the second way, so
+ * they are better off in another call than a prompt's rows. */
 typedef struct b2_attention_4bit_args {
     const void* q;            /* [n_rows][n_head][head_dim] */
     const void *k_pool, *v_pool;

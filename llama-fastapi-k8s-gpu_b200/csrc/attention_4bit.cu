@@ -785,7 +785,8 @@ cudaError_t attention_4bit_join(const Attention4Args& a, int ctas, int rows, cud
 }
 
 namespace {
-// Up to so many rows a KV head of a sequence this file's tiles of 16 rows, more on tensor memory. us here and there (heads of 128, 8 KV heads): a sequence of 4000 tokens with 32 rows a KV head
+// Where no sequence may have more rows a KV head than this, this file's tiles of 16 rows; else the whole call on tensor memory, short sequences too (200 chats of 16 to 2000 tokens beside 512 rows behind
+// 2000: 527 us, in two calls 141). us here and there (heads of 128, 8 KV heads): a sequence of 4000 tokens with 32 rows a KV head
 // 17 and 23, 64 rows 18 and 24, 128 rows 24 and 25; 32 sequences of 1000 tokens with 32 rows 40 and 82, 64 rows 69 and 83, 68 rows 82 and 83, 256 rows 244 and 105.
 constexpr long A4_TC_ROWS = 64;
 bool a4_many(long rows, int n_head, int n_kv) { return rows * (n_head / n_kv) > A4_TC_ROWS; }

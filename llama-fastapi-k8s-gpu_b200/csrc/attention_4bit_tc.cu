@@ -8,7 +8,7 @@
 //
 // A value s (c - 8) has up to 14 bits, an f16 or bf16 operand 11 or 8. Rounded, keys would be off by 2^-12 each, and a score by more than all else together (relative error of the output
 // 3.5e-4 from the keys alone, 1.8e-4 from the values, where the output's own rounding to f16 is 2.1e-4). So keys and values are two operands each, both exact: with the upper
-// bits of the scale, and with the rest of it. That doubles the products, which then are what this is bound by: 2048 rows behind 6000 tokens, 32 heads over 8 of 128, 352 us, 670 TFLOP/s of
+// bits of the scale, and with the rest of it. That doubles the products, which then are what this is bound by: 2048 rows behind 6000 tokens, 32 heads over 8 of 128, 353 to 361 us, 650 to 670 TFLOP/s of
 // what is asked for and twice as much of what is done. Probabilities are rounded to the queries' type.
 #include "attention_4bit.cuh"
 #include "kv_4bit.cuh"

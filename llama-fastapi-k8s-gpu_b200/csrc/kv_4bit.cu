@@ -9,7 +9,7 @@
 // 29.6. A warp takes 16 of the 32 bits that a word of values has, its neighbour's token the others. (Two rows a warp, both places found at once: 29.3 for those 37000 rows, 144 to f32, 23.1
 // instead of 22.5 for 20000 rows of 8 heads to f16.)
 // Appends wait: 16384 rows of 32 + 2 x 8 heads of 128 take 93 us, 3500 instructions a row at 0.60 of the issue slots, 3.8 TB/s or 0.58 of the measured bandwidth, and the largest stall is that of
-// entries on their way, with the 17 warps of an SM that run at 64 registers on average. 32 rows 5.2 us: their chain, and the turns of a row one after the other. (More turns of queries under way, one CTA
+// entries on their way, with 27 warps of an SM under way at 64 registers. 32 rows 5.2 us: their chain, and the turns of a row one after the other. (More turns of queries under way, one CTA
 // an SM more or fewer: 1 to 6 % slower.)
 #include "device_ops.h"
 #include "kv_4bit.cuh"

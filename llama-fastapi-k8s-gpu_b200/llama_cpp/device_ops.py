@@ -273,7 +273,7 @@ def attention_4bit(q, k_pool, v_pool, pages, row_start, lengths, out, workspace,
 
     q, out [rows, heads, dim] both float16 or both bfloat16; pools as for kv_append_4bit; pages, row_start, lengths int32 as for kv_append. `workspace`: a contiguous tensor of
     at least attention_4bit_workspace bytes, which no other call on another stream uses meanwhile. `max_rows`: most rows of a sequence (None: all rows may be one
-    sequence's; 1 for a batched step of single tokens is much faster than leaving it open)."""
+    sequence's; 1 for a batched step of single tokens is much faster than leaving it open, and two calls, one for single tokens and one for prompts, than one for both)."""
     stream = getattr(stream, "cuda_stream", stream)
     call, entry = _entries.get("attention_4bit") or _entries.setdefault("attention_4bit", _entry("attention_4bit"))
     if call is not None:
